@@ -183,7 +183,7 @@ def prepare(case, seed):
         s["qkv"], s["out"] = _normal(gen, T, (H + 2 * hk) * d), torch.zeros(T, H * d, device="cuda")
         if op == "train":
             s["g"] = _normal(gen, T, H * d, scale=1e-2)
-            s["lse"] = torch.zeros(H, T, device="cuda")
+            s["stats"] = torch.zeros(T, H, 2, device="cuda")
             s["dqkv"] = torch.zeros_like(s["qkv"])
         return s
     s["table"], pages = _table(case, lens, gen)
@@ -343,15 +343,15 @@ def _own_attention(s):
     lib, h, seqs, ld = p["lib"], _ctx.handle, p["seqs"].handle, (H + 2 * hk) * d
     q, out = s["qkv"].data_ptr(), s["out"].data_ptr()
     k, v = q + 4 * H * d, q + 4 * (H + hk) * d
-    lse = s["lse"].data_ptr() if case["op"] == "train" else None
-    _check(lib.numrs_hip_attention_packed_forward(h, seqs, q, ld, k, v, ld, out, H * d, lse, H, hk,
-                                                  d))
+    stats = s["stats"].data_ptr() if case["op"] == "train" else None
+    _check(lib.numrs_hip_attention_packed_forward(h, seqs, q, ld, k, v, ld, out, H * d, stats, H,
+                                                  hk, d))
     if case["op"] == "prompt":
         return {"out": s["out"]}
     dq = s["dqkv"].data_ptr()
     dk, dv = dq + 4 * H * d, dq + 4 * (H + hk) * d
     _check(lib.numrs_hip_attention_packed_backward(h, seqs, q, ld, k, v, ld, out, s["g"].data_ptr(),
-                                                   H * d, lse, dq, dk, dv, H, hk, d, 0))
+                                                   H * d, stats, dq, dk, dv, H, hk, d, 0))
     return {"out": s["out"], "dqkv": s["dqkv"]}
 
 
