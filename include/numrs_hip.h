@@ -344,6 +344,91 @@ int numrs_hip_attention_backward_out_strided(numrs_hip_ctx *ctx, const float *q,
                                              float *dq, float *dk, float *dv, int64_t B, int64_t S,
                                              int64_t H, int64_t D, int accumulate);
 
+/* A packed batch: sequences of different lengths whose tokens follow each
+ * other as the rows of one matrix (no reference counterpart; its ops take one
+ * shape).  `lengths` is a HOST array; a length may be 0.  The handle holds the
+ * device's copy and may be destroyed as soon as no further call names it; a
+ * graph that recorded such a call needs it until the graph is destroyed, and a
+ * tensor's backward keeps what it needs by itself. */
+typedef struct numrs_hip_seqs numrs_hip_seqs;
+int numrs_hip_seqs_create(numrs_hip_ctx *ctx, const int64_t *lengths, int64_t n,
+                          numrs_hip_seqs **out);
+int numrs_hip_seqs_destroy(numrs_hip_seqs *seqs);
+int64_t numrs_hip_seqs_total(const numrs_hip_seqs *seqs); /* the sum of the lengths; -1 for NULL */
+
+/* Causal attention over a packed batch with grouped heads (no reference op).
+ * Rows are tokens; query head h of a row is columns [h*dh, (h+1)*dh) of q, out,
+ * dout and dq, and attends to kv head h / (heads / kv_heads) of k and v over
+ * the tokens of its own sequence up to its own:
+ *   p = softmax(q . k / sqrt(dh)),  out = p v.
+ * q (and dq) rows are ld_q apart, k and v (dk, dv) rows ld_kv, out (dout) rows
+ * ld_out, so the operands can be column blocks of one projection.  dh is a
+ * multiple of 8 in 8..128.  stats [total, heads, 2] receives each row's
+ * softmax reference and sum for the backward; NULL where none follows.  Rows
+ * past the batch's total are not touched, and a row's result depends on no
+ * other token's values than those it attends to, finite or not.
+ * Backward, with r = dout . v and D = dout . out:
+ *   dv = sum p dout,  ds = p (r - D) / sqrt(dh),  dq = sum ds k,  dk = sum ds q,
+ * the last two over all query heads of the kv head; dq, dk or dv may be NULL.
+ * No S x S buffer, no atomics: the same call gives the same bits.  The outputs
+ * must not overlap any input. */
+int numrs_hip_attention_packed_forward(numrs_hip_ctx *ctx, const numrs_hip_seqs *seqs,
+                                       const float *q, int64_t ld_q, const float *k,
+                                       const float *v, int64_t ld_kv, float *out, int64_t ld_out,
+                                       float *stats, int64_t heads, int64_t kv_heads, int64_t dh);
+int numrs_hip_attention_packed_backward(numrs_hip_ctx *ctx, const numrs_hip_seqs *seqs,
+                                        const float *q, int64_t ld_q, const float *k,
+                                        const float *v, int64_t ld_kv, const float *out,
+                                        const float *dout, int64_t ld_out, const float *stats,
+                                        float *dq, float *dk, float *dv, int64_t heads,
+                                        int64_t kv_heads, int64_t dh, int accumulate);
+
+/* A paged key-value cache in the caller's device memory (no reference
+ * counterpart).  Page p, kv head g, slot t and value d of the keys are element
+ * ((p * kv_heads + g) * page_size + t) * head_dim + d of `k`, as floats or, in
+ * the 8-bit format, bytes; so are fp32 values of `v`.  The 8-bit values' codes
+ * of four neighbouring slots lie together: [page][head][slot / 4][d][slot % 4].
+ * A code stands for (code - 128) * scale with scale [page][head][slot] =
+ * max|x| / 127 of its row of head_dim values, code = clamp(round(x / scale),
+ * -127, 127) + 128, the quotients rounded to fp32 and ties to even (scale 0:
+ * code 128).  A row with a value that is not finite has the scale NaN and reads
+ * back as NaN.  k, v and the scales lie on 16 bytes; the scales are NULL for
+ * fp32.  page_size is a power of two in 16..65536, head_dim a multiple of 8 in
+ * 8..128. */
+enum { NUMRS_HIP_KV_F32 = 0, NUMRS_HIP_KV_INT8 = 1 };
+typedef struct numrs_hip_kv_cache {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  int64_t pages, page_size, kv_heads, head_dim;
+  int format;
+} numrs_hip_kv_cache;
+
+/* Writes rows of keys and values into the cache, or reads them back.  The
+ * packed rows of sequence i take positions ends[i] - length_i .. ends[i] - 1:
+ * `ends` [n] are the sequences' tokens in the cache with these, a prompt's
+ * lengths or, for a batch of one token each, the lengths after that token.
+ * table [n, max_pages] lists each sequence's pages in order; both are int32
+ * DEVICE arrays, read by the kernels only.  A position outside the table, or on
+ * a page that the cache does not have, is not written and reads as zeros.  Two
+ * rows of one call must not share a slot: what it then holds is not
+ * determined.  k and v rows are ld apart, heads side by side. */
+int numrs_hip_kv_cache_write(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cache,
+                             const numrs_hip_seqs *seqs, const float *k, const float *v,
+                             int64_t ld, const int32_t *table, int64_t max_pages,
+                             const int32_t *ends);
+int numrs_hip_kv_cache_read(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cache,
+                            const numrs_hip_seqs *seqs, float *k, float *v, int64_t ld,
+                            const int32_t *table, int64_t max_pages, const int32_t *ends);
+
+/* One query row for each of n sequences over its lengths[i] cached tokens
+ * (int32, device), heads grouped as above: out = softmax(q . k / sqrt(dh)) v.
+ * A length is taken within 0..max_pages * page_size; tokens on pages that the
+ * cache does not have are left out, and a row without any token is zeros. */
+int numrs_hip_attention_paged(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cache, const float *q,
+                              int64_t ld_q, int64_t heads, const int32_t *table,
+                              int64_t max_pages, const int32_t *lengths, int64_t n, float *out,
+                              int64_t ld_out);
+
 /* How the two-layer LSTM calls run their recurrences (no reference op).
  * AUTO (the default): one persistent launch for all steps of the forward
  * and one for the backward where they apply (H1 = H2 = 256, 16-byte aligned
@@ -762,6 +847,24 @@ int numrs_hip_tensor_attention(numrs_hip_tensor *q, numrs_hip_tensor *k, numrs_h
  * backward writes the packed grad [B*S, 3D]. */
 int numrs_hip_tensor_attention_qkv(numrs_hip_tensor *qkv, int64_t batch, int64_t seq,
                                    int64_t heads, numrs_hip_tensor **out);
+
+/* Causal attention node over a packed batch (numrs_hip_attention_packed_*):
+ * q [total, heads*dh], k and v [total, kv_heads*dh] -> [total, heads*dh]; _qkv
+ * takes one projection [total, (heads + 2 kv_heads)*dh] with the column blocks
+ * q, k and v, and its backward writes that projection's grad. */
+int numrs_hip_tensor_attention_packed(numrs_hip_tensor *q, numrs_hip_tensor *k,
+                                      numrs_hip_tensor *v, const numrs_hip_seqs *seqs,
+                                      int64_t heads, int64_t kv_heads, numrs_hip_tensor **out);
+int numrs_hip_tensor_attention_packed_qkv(numrs_hip_tensor *qkv, const numrs_hip_seqs *seqs,
+                                          int64_t heads, int64_t kv_heads,
+                                          numrs_hip_tensor **out);
+/* numrs_hip_attention_paged as a tensor op: the queries are the first
+ * heads * head_dim columns of x [n, columns] (a projection's other columns are
+ * left alone), the result is [n, heads * head_dim].  It has no backward and is
+ * refused where one would be recorded. */
+int numrs_hip_tensor_attention_paged(numrs_hip_tensor *x, const numrs_hip_kv_cache *cache,
+                                     int64_t heads, const int32_t *table, int64_t max_pages,
+                                     const int32_t *lengths, numrs_hip_tensor **out);
 
 /* SGD::new (optim/sgd.rs:47-69) / Adam::new (optim/adam.rs:64-99) over
  * parameter tensors; step / zero_grad / learning_rate / set_learning_rate

@@ -99,6 +99,16 @@ SIGNATURES = {
                                              [_i64] * 4 + [_i]),
     "numrs_hip_attention_backward_out_strided": (_i, [_vp] * 4 + [_i64, _vp, _vp, _vp, _i64] +
                                                  [_vp] * 3 + [_i64] * 4 + [_i]),
+    "numrs_hip_seqs_create": (_i, [_vp, _i64p, _i64, ctypes.POINTER(_vp)]),
+    "numrs_hip_seqs_destroy": (_i, [_vp]),
+    "numrs_hip_seqs_total": (_i64, [_vp]),
+    "numrs_hip_attention_packed_forward": (_i, [_vp, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp] +
+                                           [_i64] * 3),
+    "numrs_hip_attention_packed_backward": (_i, [_vp, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64] +
+                                            [_vp] * 4 + [_i64] * 3 + [_i]),
+    "numrs_hip_kv_cache_write": (_i, [_vp] * 5 + [_i64, _vp, _i64, _vp]),
+    "numrs_hip_kv_cache_read": (_i, [_vp] * 5 + [_i64, _vp, _i64, _vp]),
+    "numrs_hip_attention_paged": (_i, [_vp] * 3 + [_i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64]),
     # tensor engine
     "numrs_hip_set_grad_enabled": (None, [_i]),
     "numrs_hip_is_grad_enabled": (_i, []),
@@ -142,6 +152,9 @@ SIGNATURES = {
     "numrs_hip_tensor_time_slice": (_i, [_vp, _i64, ctypes.POINTER(_vp)]),
     "numrs_hip_tensor_attention": (_i, [_vp, _vp, _vp, _i64, _i64, _i64, ctypes.POINTER(_vp)]),
     "numrs_hip_tensor_attention_qkv": (_i, [_vp, _i64, _i64, _i64, ctypes.POINTER(_vp)]),
+    "numrs_hip_tensor_attention_packed": (_i, [_vp] * 4 + [_i64, _i64, ctypes.POINTER(_vp)]),
+    "numrs_hip_tensor_attention_packed_qkv": (_i, [_vp] * 2 + [_i64, _i64, ctypes.POINTER(_vp)]),
+    "numrs_hip_tensor_attention_paged": (_i, [_vp, _vp, _i64, _vp, _i64, _vp, ctypes.POINTER(_vp)]),
     "numrs_hip_optim_sgd": (_i, [_vp, ctypes.POINTER(_vp), _i, _f, _f, _f, ctypes.POINTER(_vp)]),
     "numrs_hip_optim_adam": (_i, [_vp, ctypes.POINTER(_vp), _i, _f, _f, _f, _f, _f,
                                  ctypes.POINTER(_vp)]),
@@ -183,7 +196,17 @@ ADD, SUB, MUL, DIV = range(4)
 RED_SUM, RED_MAX, RED_MIN, RED_MEAN, RED_ARGMAX, RED_VARIANCE = range(6)
 (OPT_ADAMW, OPT_RMSPROP, OPT_ADAGRAD, OPT_NADAM, OPT_RADAM, OPT_ADADELTA, OPT_ADABOUND, OPT_RPROP,
  OPT_LAMB) = range(9)
+KV_F32, KV_INT8 = 0, 1
 SCHED_STEP, SCHED_EXPONENTIAL, SCHED_COSINE, SCHED_PLATEAU, SCHED_WARMUP = range(5)
+
+
+
+class KVPages(ctypes.Structure):
+    """numrs_hip_kv_cache: where a paged key-value cache lies, its sizes and its format."""
+
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("pages", _i64),
+                ("page_size", _i64), ("kv_heads", _i64), ("head_dim", _i64), ("format", _i)]
+
 
 _lib = None
 

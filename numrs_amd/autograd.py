@@ -360,6 +360,32 @@ class Tensor:
         return self._out(L.load().numrs_hip_tensor_attention_qkv(self._h, batch, seq, heads,
                                                                  ctypes.byref(h)), h)
 
+    def attention_packed(self, k: "Tensor", v: "Tensor", seqs, heads: int, kv_heads: int
+                         ) -> "Tensor":
+        """Causal attention over a packed batch (`PackedSequences`) with self as
+        q [tokens, heads*dh] and k, v [tokens, kv_heads*dh]: query head h attends
+        to kv head h // (heads // kv_heads)."""
+        h = ctypes.c_void_p()
+        return self._out(L.load().numrs_hip_tensor_attention_packed(
+            self._h, k._h, v._h, seqs.handle, heads, kv_heads, ctypes.byref(h)), h)
+
+    def attention_packed_qkv(self, seqs, heads: int, kv_heads: int) -> "Tensor":
+        """The same over self = one projection [tokens, (heads + 2 kv_heads)*dh]
+        whose column blocks are q, k and v."""
+        h = ctypes.c_void_p()
+        return self._out(L.load().numrs_hip_tensor_attention_packed_qkv(
+            self._h, seqs.handle, heads, kv_heads, ctypes.byref(h)), h)
+
+    def attention_paged(self, cache, heads: int, table, lengths) -> "Tensor":
+        """One query row for each sequence over its tokens in a `KVCache`: the
+        queries are self's first heads * head_dim columns.  table [n, max_pages]
+        and lengths [n] are int32 device arrays.  No backward."""
+        most = cache.table_width(table, lengths, self.shape()[0])
+        h = ctypes.c_void_p()
+        return self._out(L.load().numrs_hip_tensor_attention_paged(
+            self._h, ctypes.byref(cache.pages), heads, table.ptr, most, lengths.ptr,
+            ctypes.byref(h)), h)
+
     def __repr__(self) -> str:
         return f"Tensor(shape={list(self.shape())}, requires_grad={self.requires_grad})"
 

@@ -29,6 +29,7 @@
 #include <vector>
 
 #include "common.h"
+#include "packed.h"
 
 namespace {
 
@@ -39,7 +40,7 @@ thread_local bool g_grad_enabled = true;  // mod.rs:194-206
 enum class Op {
   Leaf, Add, Sub, Mul, Div, MatMul, Transpose, Unary, Sum, Mean, MSE, CrossEntropy,
   CrossEntropyLabels, Reshape, Softmax, LayerNorm, Attention, Linear, LSTM, TimeSlice, SumAxis,
-  SoftmaxAxis, LSTM2
+  SoftmaxAxis, LSTM2, AttentionPacked
 };
 
 struct Storage {
@@ -84,6 +85,7 @@ struct Node {
   int64_t dims[3] = {0, 0, 0};  // attention batch, seq, heads; axis ops' [outer, n, inner]
   std::vector<T> inputs;
   std::vector<Buf> saved;  // LayerNorm mean/rstd, int32 labels
+  std::shared_ptr<const numrs_hip::Seqs> seqs;  // a packed batch's sequences
 };
 
 uint64_t next_node_id() {  // NodeId::new, mod.rs:46-51
@@ -545,6 +547,49 @@ int bw_attention(const T &out, const float *g, Node &n) {
   return NUMRS_HIP_OK;
 }
 
+// Causal attention over a packed batch: q, k, v as tensors of their own, or the column blocks of
+// one projection.
+int bw_attention_seqs(const T &out, const float *g, Node &n) {
+  const numrs_hip::PackedHeads h{n.dims[0], n.dims[1], n.dims[2]};
+  const int64_t wq = h.heads * h.dh, wk = h.kv_heads * h.dh;
+  const float *st = n.saved[0]->ptr, *o = out->data->ptr;
+  numrs_hip_ctx *ctx = out->ctx;
+  if (n.inputs.size() == 1) {
+    const T &x = n.inputs[0];
+    if (!x->requires_grad) return NUMRS_HIP_OK;
+    const float *p = x->data->ptr;
+    const int64_t ld = wq + 2 * wk;
+    float *d;
+    int acc;
+    if (int rc = grad_target(x, &d, &acc)) return rc;
+    return numrs_hip::packed_backward(ctx, *n.seqs, p, ld, p + wq, p + wq + wk, ld, o, g, wq, st, d,
+                                      d + wq, d + wq + wk, h, acc);
+  }
+  // Gradients whose cells take the same write or add go in one call; cells that are shared (one
+  // tensor as two operands) go one after another, so that each sees what the others left.
+  float *d[3] = {nullptr, nullptr, nullptr};
+  int acc[3] = {0, 0, 0};
+  bool one = true;
+  const GradCell *cell[3] = {nullptr, nullptr, nullptr};
+  for (int i = 0; i < 3; ++i) {
+    const T &x = n.inputs[i];
+    if (!x->requires_grad) continue;
+    cell[i] = x->grad.get();
+    if (int rc = grad_target(x, &d[i], &acc[i])) return rc;
+    for (int j = 0; j < i; ++j) one = one && (cell[j] == nullptr || (cell[j] != cell[i] && acc[j] == acc[i]));
+  }
+  auto run = [&](float *dq, float *dk, float *dv, int a) {
+    return numrs_hip::packed_backward(ctx, *n.seqs, n.inputs[0]->data->ptr, wq, n.inputs[1]->data->ptr,
+                                      n.inputs[2]->data->ptr, wk, o, g, wq, st, dq, dk, dv, h, a);
+  };
+  if (one) return run(d[0], d[1], d[2], acc[0] | acc[1] | acc[2]);
+  for (int i = 0; i < 3; ++i)
+    if (d[i] != nullptr)
+      if (int rc = run(i == 0 ? d[0] : nullptr, i == 1 ? d[1] : nullptr, i == 2 ? d[2] : nullptr, acc[i]))
+        return rc;
+  return NUMRS_HIP_OK;
+}
+
 int bw_linear(const T &out, const float *g, Node &n) {
   const T &x = n.inputs[0], &W = n.inputs[1];
   const bool relu = (n.kind & 1) != 0, has_res = (n.kind & 2) != 0, gelu = (n.kind & 4) != 0;
@@ -694,6 +739,7 @@ int run_backward_fn(const T &out) {
     case Op::Softmax: return bw_softmax(out, g, n);
     case Op::LayerNorm: return bw_layernorm(out, g, n);
     case Op::Attention: return bw_attention(out, g, n);
+    case Op::AttentionPacked: return bw_attention_seqs(out, g, n);
     case Op::Linear: return bw_linear(out, g, n);
     case Op::LSTM: return bw_lstm(out, g, n);
     case Op::LSTM2: return bw_lstm2(out, g, n);
@@ -1247,6 +1293,46 @@ int op_attention_qkv(const T &qkv, int64_t B, int64_t S, int64_t H, T *out) {
     r->node->dims[0] = B;
     r->node->dims[1] = S;
     r->node->dims[2] = H;
+  }
+  *out = std::move(r);
+  return NUMRS_HIP_OK;
+}
+
+// Causal attention over a packed batch; with k and v null, q is a projection of all three.
+int op_attention_seqs(const T &q, const T *k, const T *v, const numrs_hip_seqs *seqs, int64_t H,
+                      int64_t Hk, T *out) {
+  numrs_hip_ctx *ctx = q->ctx;
+  const auto &s = seqs->s;
+  if (s->ctx != ctx || (k != nullptr && ((*k)->ctx != ctx || (*v)->ctx != ctx)))
+    return fail(ctx, NUMRS_HIP_E_INVALID, "attention_packed: operands of different contexts");
+  if (q->shape.size() != 2 || q->shape[0] != s->total)
+    return fail(ctx, NUMRS_HIP_E_SHAPE, "attention_packed: operands must have a row for each token");
+  const int64_t parts = k != nullptr ? H : H + 2 * Hk;
+  if (H <= 0 || Hk <= 0 || H > 65535 || Hk > 65535 || q->shape[1] % parts != 0)
+    return fail(ctx, NUMRS_HIP_E_SHAPE, "attention_packed: the columns do not divide into the heads");
+  const int64_t dh = q->shape[1] / parts, wq = H * dh, wk = Hk * dh;
+  if (k != nullptr && ((*k)->shape != std::vector<int64_t>{s->total, wk} || (*v)->shape != (*k)->shape))
+    return fail(ctx, NUMRS_HIP_E_SHAPE, "attention_packed: k and v must be [tokens, kv_heads * dh]");
+  const bool rec = k != nullptr ? recording({&q, k, v}) : recording({&q});
+  T r;
+  if (int rc = make_tensor(ctx, {s->total, wq}, rec, &r)) return rc;
+  Buf st;
+  if (rec)
+    if (int rc = alloc_buf(ctx, s->total * H * 2, sizeof(float), &st)) return rc;
+  const float *p = q->data->ptr;
+  const int64_t ld = k != nullptr ? wq : wq + 2 * wk;
+  if (int rc = numrs_hip::packed_forward(ctx, *s, p, ld, k != nullptr ? (*k)->data->ptr : p + wq,
+                                         v != nullptr ? (*v)->data->ptr : p + wq + wk,
+                                         k != nullptr ? wk : ld, r->data->ptr, wq,
+                                         rec ? st->ptr : nullptr, {H, Hk, dh}))
+    return rc;
+  if (rec) {
+    if (k != nullptr)
+      attach(r, Op::AttentionPacked, {q, *k, *v}, 0, 0.f, {st});
+    else
+      attach(r, Op::AttentionPacked, {q}, 0, 0.f, {st});
+    r->node->dims[0] = H, r->node->dims[1] = Hk, r->node->dims[2] = dh;
+    r->node->seqs = s;
   }
   *out = std::move(r);
   return NUMRS_HIP_OK;
@@ -1819,6 +1905,45 @@ int numrs_hip_tensor_attention_qkv(numrs_hip_tensor *qkv, int64_t batch, int64_t
   if (qkv == nullptr || out == nullptr) return NUMRS_HIP_E_INVALID;
   T r;
   if (int rc = op_attention_qkv(qkv->t, batch, seq, heads, &r)) return rc;
+  return wrap(std::move(r), out);
+}
+
+int numrs_hip_tensor_attention_packed(numrs_hip_tensor *q, numrs_hip_tensor *k,
+                                      numrs_hip_tensor *v, const numrs_hip_seqs *seqs,
+                                      int64_t heads, int64_t kv_heads, numrs_hip_tensor **out) {
+  if (q == nullptr || k == nullptr || v == nullptr || seqs == nullptr || out == nullptr)
+    return NUMRS_HIP_E_INVALID;
+  T r;
+  if (int rc = op_attention_seqs(q->t, &k->t, &v->t, seqs, heads, kv_heads, &r)) return rc;
+  return wrap(std::move(r), out);
+}
+
+int numrs_hip_tensor_attention_packed_qkv(numrs_hip_tensor *qkv, const numrs_hip_seqs *seqs,
+                                          int64_t heads, int64_t kv_heads,
+                                          numrs_hip_tensor **out) {
+  if (qkv == nullptr || seqs == nullptr || out == nullptr) return NUMRS_HIP_E_INVALID;
+  T r;
+  if (int rc = op_attention_seqs(qkv->t, nullptr, nullptr, seqs, heads, kv_heads, &r)) return rc;
+  return wrap(std::move(r), out);
+}
+
+int numrs_hip_tensor_attention_paged(numrs_hip_tensor *x, const numrs_hip_kv_cache *cache,
+                                     int64_t heads, const int32_t *table, int64_t max_pages,
+                                     const int32_t *lengths, numrs_hip_tensor **out) {
+  if (x == nullptr || cache == nullptr || out == nullptr) return NUMRS_HIP_E_INVALID;
+  const T &t = x->t;
+  numrs_hip_ctx *ctx = t->ctx;
+  if (recording({&t}))
+    return fail(ctx, NUMRS_HIP_E_INVALID, "attention_paged has no backward: detach its input");
+  if (t->shape.size() != 2 || heads < 1 || heads > 65535 || cache->head_dim < 1 ||
+      cache->head_dim > 128 || t->shape[1] < heads * cache->head_dim)
+    return fail(ctx, NUMRS_HIP_E_SHAPE, "attention_paged: x must be [rows, at least heads * head_dim]");
+  T r;
+  if (int rc = make_tensor(ctx, {t->shape[0], heads * cache->head_dim}, false, &r)) return rc;
+  if (int rc = numrs_hip_attention_paged(ctx, cache, t->data->ptr, t->shape[1], heads, table,
+                                         max_pages, lengths, t->shape[0], r->data->ptr,
+                                         heads * cache->head_dim))
+    return rc;
   return wrap(std::move(r), out);
 }
 

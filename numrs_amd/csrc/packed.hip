@@ -1,0 +1,351 @@
+// Causal attention with grouped heads over packed sequences (no reference op), without an S x S
+// buffer: the forward keeps a running softmax reference m and sum l for each row,
+//   p_ij = exp(s_ij - m_i) / l_i,  s_ij = q_i . k_j / sqrt(dh),  j <= i of the same sequence,
+// and the backward forms p again from them.
+#include <algorithm>
+#include <cmath>
+#include <new>
+#include <vector>
+
+#include "packed.h"
+#include "paging.h"
+
+namespace {
+
+using namespace numrs_hip;
+
+constexpr float kLog2e = 1.44269504088896341f;
+
+struct FwdArgs {
+  const SeqTile *tiles;
+  const float *q, *k, *v;
+  float *out, *stats;
+  int64_t ld_q, ld_kv, ld_out;
+  int heads, kv_heads, dh;
+  float alpha;  // log2(e) / sqrt(dh)
+};
+
+__device__ __forceinline__ float lane_of(float v, int lane) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+
+// Dot product of a row in LDS and one in memory.
+__device__ __forceinline__ float dot_row(const float *x, const float *y, int dh) {
+  float s = 0.f;
+  for (int d = 0; d < dh; d += 8) {
+    float a = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a = fmaf(x[d + e], y[d + e], a);
+    s += a;
+  }
+  return s;
+}
+
+// One wave: query row r of head h, in plain fp32, 64 keys at a time (a key a lane for the scores,
+// a column a lane for the output).  x: the wave's dh floats of LDS.
+__device__ void row_forward(const FwdArgs &a, const SeqTile &t, int r, int h, float *x) {
+  const int lane = threadIdx.x & 63, g = h / (a.heads / a.kv_heads);
+  const int64_t row = t.row0 + r;
+  for (int d = lane; d < a.dh; d += 64) x[d] = a.q[row * a.ld_q + (int64_t)h * a.dh + d];
+  __builtin_amdgcn_wave_barrier();
+  const float *k = a.k + t.row0 * a.ld_kv + (int64_t)g * a.dh, *v = a.v + t.row0 * a.ld_kv + (int64_t)g * a.dh;
+  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
+  for (int j0 = 0; j0 <= r; j0 += 64) {
+    const int j = j0 + lane, n = min(64, r + 1 - j0);
+    const float s = lane < n ? dot_row(x, k + j * a.ld_kv, a.dh) * a.alpha : -INFINITY;
+    const float top = fmaxf(m, wave_max(s));
+    // A row whose scores are all -inf has no softmax: NaN, as the formula has it.
+    const float p = lane < n ? exp2f(s - top) : 0.f, c = j0 == 0 ? 0.f : exp2f(m - top);
+    m = top;
+    l = l * c + wave_sum(p);
+    float t0 = 0.f, t1 = 0.f;  // the block's sum apart, so that a long sum's rounding stays small
+    for (int e = 0; e < n; ++e) {
+      const float w = lane_of(p, e);
+      const float *y = v + (j0 + e) * a.ld_kv;
+      if (lane < a.dh) t0 = fmaf(w, y[lane], t0);
+      if (lane + 64 < a.dh) t1 = fmaf(w, y[lane + 64], t1);
+    }
+    o0 = fmaf(o0, c, t0), o1 = fmaf(o1, c, t1);
+  }
+  float *o = a.out + row * a.ld_out + (int64_t)h * a.dh;
+  if (lane < a.dh) o[lane] = o0 / l;
+  if (lane + 64 < a.dh) o[lane + 64] = o1 / l;
+  if (a.stats != nullptr && lane == 0) {
+    float *st = a.stats + (row * a.heads + h) * 2;
+    st[0] = m, st[1] = l;
+  }
+}
+
+constexpr int kRows = 4;  // waves of a workgroup
+
+__global__ void __launch_bounds__(64 * kRows) forward_rows(FwdArgs a) {
+  __shared__ float x[kRows][128];
+  const int w = threadIdx.x >> 6;
+  const SeqTile t = a.tiles[blockIdx.x / a.heads];
+  const int h = blockIdx.x % a.heads, end = min(t.len, t.t0 + kTile);
+  for (int r = t.t0 + w; r < end; r += kRows) row_forward(a, t, r, h, x[w]);
+}
+
+struct BwdArgs {
+  const SeqTile *tiles;
+  const float *q, *k, *v, *out, *dout, *stats;
+  float *D, *dq, *dk, *dv;  // D [total, heads]
+  int64_t ld_q, ld_kv, ld_out;
+  int heads, kv_heads, dh, accumulate;
+  float alpha, scale;  // log2(e) / sqrt(dh), 1 / sqrt(dh)
+};
+
+// D = dout . out of each row and head.
+__global__ void __launch_bounds__(256) row_dots(BwdArgs a, int64_t total) {
+  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (i >= total * a.heads) return;
+  const int64_t at = i / a.heads * a.ld_out + i % a.heads * a.dh;
+  float s = 0.f;
+  if (lane < a.dh) s = a.dout[at + lane] * a.out[at + lane];
+  if (lane + 64 < a.dh) s = fmaf(a.dout[at + lane + 64], a.out[at + lane + 64], s);
+  s = wave_sum(s);
+  if (lane == 0) a.D[i] = s;
+}
+
+__device__ __forceinline__ void put(float *p, float v, int accumulate) { *p = accumulate ? *p + v : v; }
+
+// One wave: dq of query row r and head h.  x: two rows of dh floats.
+__device__ void row_dq(const BwdArgs &a, const SeqTile &t, int r, int h, float *x) {
+  const int lane = threadIdx.x & 63, g = h / (a.heads / a.kv_heads);
+  const int64_t row = t.row0 + r;
+  for (int d = lane; d < a.dh; d += 64) {
+    x[d] = a.q[row * a.ld_q + (int64_t)h * a.dh + d];
+    x[128 + d] = a.dout[row * a.ld_out + (int64_t)h * a.dh + d];
+  }
+  __builtin_amdgcn_wave_barrier();
+  const float *k = a.k + t.row0 * a.ld_kv + (int64_t)g * a.dh, *v = a.v + t.row0 * a.ld_kv + (int64_t)g * a.dh;
+  const float *st = a.stats + (row * a.heads + h) * 2;
+  const float m = st[0], l = st[1], D = a.D[row * a.heads + h];
+  float o0 = 0.f, o1 = 0.f;
+  for (int j0 = 0; j0 <= r; j0 += 64) {
+    const int j = j0 + lane, n = min(64, r + 1 - j0);
+    float ds = 0.f;
+    if (lane < n) {
+      const float p = exp2f(dot_row(x, k + j * a.ld_kv, a.dh) * a.alpha - m) / l;
+      ds = p * (dot_row(x + 128, v + j * a.ld_kv, a.dh) - D);
+    }
+    float t0 = 0.f, t1 = 0.f;
+    for (int e = 0; e < n; ++e) {
+      const float w = lane_of(ds, e);
+      const float *y = k + (j0 + e) * a.ld_kv;
+      if (lane < a.dh) t0 = fmaf(w, y[lane], t0);
+      if (lane + 64 < a.dh) t1 = fmaf(w, y[lane + 64], t1);
+    }
+    o0 += t0, o1 += t1;
+  }
+  float *o = a.dq + row * a.ld_q + (int64_t)h * a.dh;
+  if (lane < a.dh) put(o + lane, o0 * a.scale, a.accumulate);
+  if (lane + 64 < a.dh) put(o + lane + 64, o1 * a.scale, a.accumulate);
+}
+
+// One wave: dk and dv of key row r and kv head g, over the query heads of g in order.
+__device__ void row_dkv(const BwdArgs &a, const SeqTile &t, int r, int g, float *x) {
+  const int lane = threadIdx.x & 63, group = a.heads / a.kv_heads;
+  const int64_t row = t.row0 + r, at = row * a.ld_kv + (int64_t)g * a.dh;
+  for (int d = lane; d < a.dh; d += 64) x[d] = a.k[at + d], x[128 + d] = a.v[at + d];
+  __builtin_amdgcn_wave_barrier();
+  float k0 = 0.f, k1 = 0.f, v0 = 0.f, v1 = 0.f;
+  for (int h = g * group; h < (g + 1) * group; ++h) {
+    const float *q = a.q + (int64_t)h * a.dh, *go = a.dout + (int64_t)h * a.dh;
+    for (int i0 = r; i0 < t.len; i0 += 64) {
+      const int n = min(64, t.len - i0);
+      float p = 0.f, ds = 0.f;
+      if (lane < n) {
+        const int64_t i = t.row0 + i0 + lane;
+        const float *st = a.stats + (i * a.heads + h) * 2;
+        p = exp2f(dot_row(x, q + i * a.ld_q, a.dh) * a.alpha - st[0]) / st[1];
+        ds = p * (dot_row(x + 128, go + i * a.ld_out, a.dh) - a.D[i * a.heads + h]);
+      }
+      float tk0 = 0.f, tk1 = 0.f, tv0 = 0.f, tv1 = 0.f;
+      for (int e = 0; e < n; ++e) {
+        const int64_t i = t.row0 + i0 + e;
+        const float w = lane_of(p, e), u = lane_of(ds, e);
+        if (lane < a.dh) {
+          tv0 = fmaf(w, go[i * a.ld_out + lane], tv0);
+          tk0 = fmaf(u, q[i * a.ld_q + lane], tk0);
+        }
+        if (lane + 64 < a.dh) {
+          tv1 = fmaf(w, go[i * a.ld_out + lane + 64], tv1);
+          tk1 = fmaf(u, q[i * a.ld_q + lane + 64], tk1);
+        }
+      }
+      k0 += tk0, k1 += tk1, v0 += tv0, v1 += tv1;
+    }
+  }
+  if (a.dk != nullptr) {
+    if (lane < a.dh) put(a.dk + at + lane, k0 * a.scale, a.accumulate);
+    if (lane + 64 < a.dh) put(a.dk + at + lane + 64, k1 * a.scale, a.accumulate);
+  }
+  if (a.dv != nullptr) {
+    if (lane < a.dh) put(a.dv + at + lane, v0, a.accumulate);
+    if (lane + 64 < a.dh) put(a.dv + at + lane + 64, v1, a.accumulate);
+  }
+}
+
+__global__ void __launch_bounds__(64 * kRows) dq_rows(BwdArgs a) {
+  __shared__ float x[kRows][256];
+  const int w = threadIdx.x >> 6;
+  const SeqTile t = a.tiles[blockIdx.x / a.heads];
+  const int h = blockIdx.x % a.heads, end = min(t.len, t.t0 + kTile);
+  for (int r = t.t0 + w; r < end; r += kRows) row_dq(a, t, r, h, x[w]);
+}
+
+__global__ void __launch_bounds__(64 * kRows) dkv_rows(BwdArgs a) {
+  __shared__ float x[kRows][256];
+  const int w = threadIdx.x >> 6;
+  const SeqTile t = a.tiles[blockIdx.x / a.kv_heads];
+  const int g = blockIdx.x % a.kv_heads, end = min(t.len, t.t0 + kTile);
+  for (int r = t.t0 + w; r < end; r += kRows) row_dkv(a, t, r, g, x[w]);
+}
+
+// The arguments that the forward and the backward share.
+int check_packed(numrs_hip_ctx *ctx, const Seqs &s, int64_t ld_q, int64_t ld_kv, int64_t ld_out,
+                 PackedHeads h, const char *what) {
+  if (ctx->destroyed) return fail(ctx, NUMRS_HIP_E_INVALID, "context already destroyed");
+  if (s.ctx != ctx)
+    return fail(ctx, NUMRS_HIP_E_INVALID, "%s: the sequences belong to another context", what);
+  if (const char *why = paging::refuse_heads(h.heads, h.kv_heads, h.dh))
+    return fail(ctx, NUMRS_HIP_E_SHAPE, "%s: %s", what, why);
+  if (paging::bad_stride(ld_q, h.heads * h.dh) || paging::bad_stride(ld_kv, h.kv_heads * h.dh) ||
+      paging::bad_stride(ld_out, h.heads * h.dh))
+    return fail(ctx, NUMRS_HIP_E_SHAPE, "%s: a row stride is below its row's width or above 2^31 - 1",
+                what);
+  if (s.tiles * h.heads >= int64_t{1} << 31)
+    return fail(ctx, NUMRS_HIP_E_SHAPE, "%s: too many tokens times heads", what);
+  return NUMRS_HIP_OK;
+}
+
+}  // namespace
+
+namespace numrs_hip {
+
+int packed_forward(numrs_hip_ctx *ctx, const Seqs &s, const float *q, int64_t ld_q, const float *k,
+                   const float *v, int64_t ld_kv, float *out, int64_t ld_out, float *stats,
+                   PackedHeads h) {
+  if (int rc = check_packed(ctx, s, ld_q, ld_kv, ld_out, h, "attention_packed")) return rc;
+  if (s.total == 0) return NUMRS_HIP_OK;
+  if (q == nullptr || k == nullptr || v == nullptr || out == nullptr)
+    return fail(ctx, NUMRS_HIP_E_INVALID, "attention_packed: null pointer");
+  DeviceScope dev(ctx);
+  const FwdArgs a{s.in_order, q, k, v, out, stats, ld_q, ld_kv, ld_out, (int)h.heads,
+                  (int)h.kv_heads, (int)h.dh, kLog2e / std::sqrt((float)h.dh)};
+  forward_rows<<<(unsigned)(s.tiles * h.heads), 64 * kRows, 0, ctx->stream>>>(a);
+  return check_launch(ctx, "forward_rows");
+}
+
+int packed_backward(numrs_hip_ctx *ctx, const Seqs &s, const float *q, int64_t ld_q, const float *k,
+                    const float *v, int64_t ld_kv, const float *out, const float *dout,
+                    int64_t ld_out, const float *stats, float *dq, float *dk, float *dv,
+                    PackedHeads h, int accumulate) {
+  if (int rc = check_packed(ctx, s, ld_q, ld_kv, ld_out, h, "attention_packed_backward")) return rc;
+  if (s.total == 0 || (dq == nullptr && dk == nullptr && dv == nullptr)) return NUMRS_HIP_OK;
+  if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || dout == nullptr ||
+      stats == nullptr)
+    return fail(ctx, NUMRS_HIP_E_INVALID, "attention_packed_backward: null pointer");
+  DeviceScope dev(ctx);
+  TempBlock D(ctx);
+  if (int rc = D.alloc((size_t)(s.total * h.heads) * sizeof(float))) return rc;
+  const float scale = 1.0f / std::sqrt((float)h.dh);
+  const BwdArgs a{s.in_order, q, k, v, out, dout, stats, D.f(), dq, dk, dv, ld_q, ld_kv, ld_out,
+                  (int)h.heads, (int)h.kv_heads, (int)h.dh, accumulate, kLog2e / std::sqrt((float)h.dh),
+                  scale};
+  row_dots<<<grid_for(s.total * h.heads, 4), 256, 0, ctx->stream>>>(a, s.total);
+  if (int rc = check_launch(ctx, "row_dots")) return rc;
+  if (dq != nullptr) {
+    dq_rows<<<(unsigned)(s.tiles * h.heads), 64 * kRows, 0, ctx->stream>>>(a);
+    if (int rc = check_launch(ctx, "dq_rows")) return rc;
+  }
+  if (dk != nullptr || dv != nullptr) {
+    dkv_rows<<<(unsigned)(s.tiles * h.kv_heads), 64 * kRows, 0, ctx->stream>>>(a);
+    if (int rc = check_launch(ctx, "dkv_rows")) return rc;
+  }
+  return NUMRS_HIP_OK;
+}
+
+}  // namespace numrs_hip
+
+extern "C" {
+
+int numrs_hip_seqs_create(numrs_hip_ctx *ctx, const int64_t *lengths, int64_t n,
+                          numrs_hip_seqs **out) {
+  NRS_CHECK_CTX(ctx);
+  if (out == nullptr) return fail(ctx, NUMRS_HIP_E_INVALID, "numrs_hip_seqs_create: null out pointer");
+  *out = nullptr;
+  if (ctx->destroyed) return fail(ctx, NUMRS_HIP_E_INVALID, "context already destroyed");
+  if (n < 0 || n >= int64_t{1} << 24 || (n > 0 && lengths == nullptr))
+    return fail(ctx, NUMRS_HIP_E_INVALID, "numrs_hip_seqs_create: 0 to 2^24 - 1 lengths are needed");
+  if (ctx->capturing)
+    return fail(ctx, NUMRS_HIP_E_INVALID,
+                "numrs_hip_seqs_create is not allowed while a graph is being recorded");
+  const int64_t total = paging::packed_total(lengths, n);
+  if (total < 0)
+    return fail(ctx, NUMRS_HIP_E_SHAPE,
+                "numrs_hip_seqs_create: lengths must be at least 0 and sum to at most 2^30");
+  DeviceScope dev(ctx);
+  try {
+    auto s = std::make_shared<Seqs>();
+    s->ctx = ctx, s->n = n, s->total = total;
+    std::vector<SeqTile> tiles;
+    int64_t row = 0;
+    for (int64_t i = 0; i < n; ++i) {
+      const int first = (int)tiles.size();
+      for (int64_t t = 0; t < lengths[i]; t += kTile)
+        tiles.push_back({(int)row, (int)lengths[i], (int)t, first, (int)i, {0, 0, 0}});
+      row += lengths[i];
+    }
+    s->tiles = (int64_t)tiles.size();
+    auto h = std::make_unique<numrs_hip_seqs>();
+    if (!tiles.empty()) {
+      void *p = nullptr;
+      const size_t bytes = tiles.size() * sizeof(SeqTile);
+      if (int rc = block_alloc(ctx, bytes, &p)) return rc;
+      s->in_order = static_cast<SeqTile *>(p), s->bytes = bytes;
+      if (int rc = numrs_hip_upload(ctx, p, tiles.data(), bytes)) return rc;
+    }
+    h->s = std::move(s);
+    *out = h.release();
+  } catch (const std::bad_alloc &) {
+    return fail(ctx, NUMRS_HIP_E_NOMEM, "numrs_hip_seqs_create: out of host memory");
+  }
+  return NUMRS_HIP_OK;
+}
+
+int numrs_hip_seqs_destroy(numrs_hip_seqs *seqs) {
+  delete seqs;
+  return NUMRS_HIP_OK;
+}
+
+int64_t numrs_hip_seqs_total(const numrs_hip_seqs *seqs) {
+  return seqs == nullptr ? -1 : seqs->s->total;
+}
+
+int numrs_hip_attention_packed_forward(numrs_hip_ctx *ctx, const numrs_hip_seqs *seqs,
+                                       const float *q, int64_t ld_q, const float *k,
+                                       const float *v, int64_t ld_kv, float *out, int64_t ld_out,
+                                       float *stats, int64_t heads, int64_t kv_heads, int64_t dh) {
+  NRS_CHECK_CTX(ctx);
+  if (seqs == nullptr) return fail(ctx, NUMRS_HIP_E_INVALID, "attention_packed: null sequences");
+  return packed_forward(ctx, *seqs->s, q, ld_q, k, v, ld_kv, out, ld_out, stats,
+                        {heads, kv_heads, dh});
+}
+
+int numrs_hip_attention_packed_backward(numrs_hip_ctx *ctx, const numrs_hip_seqs *seqs,
+                                        const float *q, int64_t ld_q, const float *k,
+                                        const float *v, int64_t ld_kv, const float *out,
+                                        const float *dout, int64_t ld_out, const float *stats,
+                                        float *dq, float *dk, float *dv, int64_t heads,
+                                        int64_t kv_heads, int64_t dh, int accumulate) {
+  NRS_CHECK_CTX(ctx);
+  if (seqs == nullptr)
+    return fail(ctx, NUMRS_HIP_E_INVALID, "attention_packed_backward: null sequences");
+  return packed_backward(ctx, *seqs->s, q, ld_q, k, v, ld_kv, out, dout, ld_out, stats, dq, dk, dv,
+                         {heads, kv_heads, dh}, accumulate);
+}
+
+}  // extern "C"

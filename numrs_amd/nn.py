@@ -219,6 +219,65 @@ class MultiHeadAttention(Module):
         return [p for m in self.projections + [self.o] for p in m.parameters()]
 
 
+class CausalSelfAttention(Module):
+    """A decoder's self-attention (no reference op): grouped heads over packed
+    sequences, each token attending to its sequence up to itself, and the same
+    over a paged cache for generation.  wq [heads*dh, d], wk and wv
+    [kv_heads*dh, d], wo [d, heads*dh]; zero biases.
+
+        y = attn.forward_packed(x, seqs)                       # training, with backward
+        with no_grad():
+            y = attn.prefill(x, seqs, cache, table, lengths)   # prompts, kept in the cache
+            y = attn.decode(x1, ones, cache, table, lengths)   # one token for each sequence
+
+    `lengths` (int32, device) counts a sequence's cached tokens, the new ones
+    included; `ones` is PackedSequences([1] * n)."""
+
+    def __init__(self, wq, wk, wv, wo, heads: int, kv_heads: int, ctx=None):
+        wq, wk, wv, wo = (np.asarray(a, np.float32) for a in (wq, wk, wv, wo))
+        if heads % kv_heads or wq.shape[0] % heads or wk.shape != wv.shape:
+            raise ValueError("CausalSelfAttention: the weights do not divide into the heads")
+        if wk.shape[0] * heads != wq.shape[0] * kv_heads:
+            raise ValueError("CausalSelfAttention: q and k heads must have one size")
+        self.heads, self.kv_heads, self.head_dim = heads, kv_heads, wq.shape[0] // heads
+        w = np.concatenate([wq, wk, wv])
+        self.qkv = Linear.with_weights(w.shape[1], w.shape[0], w, np.zeros(w.shape[0], np.float32),
+                                       ctx)
+        self.o = Linear.with_weights(wo.shape[1], wo.shape[0], wo, np.zeros(wo.shape[0], np.float32),
+                                     ctx)
+
+    def _project(self, a: Tensor, residual: Tensor | None) -> Tensor:
+        if residual is None:
+            return self.o(a)
+        if self.o.fused:
+            return a.linear(self.o.weight, self.o.bias, residual=residual)
+        return residual.add(self.o(a))
+
+    def forward_packed(self, x: Tensor, seqs, residual: Tensor | None = None) -> Tensor:
+        a = self.qkv(x).attention_packed_qkv(seqs, self.heads, self.kv_heads)
+        return self._project(a, residual)
+
+    def prefill(self, x: Tensor, seqs, cache, table, lengths, residual: Tensor | None = None
+                ) -> Tensor:
+        """forward_packed of whole prompts, whose keys and values also go into the
+        cache; `lengths` are the prompts' lengths."""
+        qkv = self.qkv(x)
+        cache.write_qkv(seqs, qkv, self.heads, table, lengths)
+        a = qkv.attention_packed_qkv(seqs, self.heads, self.kv_heads)
+        return self._project(a, residual)
+
+    def decode(self, x: Tensor, ones, cache, table, lengths, residual: Tensor | None = None
+               ) -> Tensor:
+        """One new token for each sequence, x [n, d]: its key and value go into the
+        cache, and it attends to all of its sequence's tokens."""
+        qkv = self.qkv(x)
+        cache.write_qkv(ones, qkv, self.heads, table, lengths)
+        return self._project(qkv.attention_paged(cache, self.heads, table, lengths), residual)
+
+    def parameters(self) -> list[Tensor]:
+        return self.qkv.parameters() + self.o.parameters()
+
+
 class TransformerEncoderBlock(Module):
     """Pre-LN encoder block on x [batch*seq, d_model]:
     r = x + Attn(LN1(x));  y = r + W2 GELU(W1 LN2(r)).
