@@ -21,8 +21,9 @@ constexpr int kTile = 64;
 // Lists of a batch's tiles on the device.
 struct Seqs {
   numrs_hip_ctx *ctx = nullptr;
-  int64_t n = 0, total = 0, tiles = 0;
+  int64_t n = 0, total = 0, tiles = 0, blocks = 0;
   SeqTile *in_order = nullptr;  // [tiles]; a tile's number is its place
+  SeqTile *by_work = nullptr;   // [blocks] of 128 tokens, those late in their sequence first
   size_t bytes = 0;
   ~Seqs() { block_free(ctx, in_order, bytes); }
 };

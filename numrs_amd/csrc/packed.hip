@@ -7,7 +7,7 @@
 #include <new>
 #include <vector>
 
-#include "packed.h"
+#include "packed_tiles.h"
 #include "paging.h"
 
 namespace {
@@ -78,12 +78,16 @@ __device__ void row_forward(const FwdArgs &a, const SeqTile &t, int r, int h, fl
 
 constexpr int kRows = 4;  // waves of a workgroup
 
-__global__ void __launch_bounds__(64 * kRows) forward_rows(FwdArgs a) {
-  __shared__ float x[kRows][128];
-  const int w = threadIdx.x >> 6;
+// A block of 128 query rows of one head.
+template <int DP>
+__global__ void __launch_bounds__(256, 2) forward_block(FwdArgs a, tiles::ForwardArgs f) {
+  constexpr int KT = DP <= 64 ? 64 : 32;
+  __shared__ __attribute__((aligned(16))) char lds[4 * KT * DP * 4];
   const SeqTile t = a.tiles[blockIdx.x / a.heads];
-  const int h = blockIdx.x % a.heads, end = min(t.len, t.t0 + kTile);
-  for (int r = t.t0 + w; r < end; r += kRows) row_forward(a, t, r, h, x[w]);
+  const int h = blockIdx.x % a.heads;
+  if (tiles::forward_tile<DP>(f, t, h, lds)) return;
+  const int w = threadIdx.x >> 6, end = min(t.len, t.t0 + 128);
+  for (int r = t.t0 + w; r < end; r += kRows) row_forward(a, t, r, h, reinterpret_cast<float *>(lds) + 128 * w);
 }
 
 struct BwdArgs {
@@ -216,10 +220,46 @@ int check_packed(numrs_hip_ctx *ctx, const Seqs &s, int64_t ld_q, int64_t ld_kv,
       paging::bad_stride(ld_out, h.heads * h.dh))
     return fail(ctx, NUMRS_HIP_E_SHAPE, "%s: a row stride is below its row's width or above 2^31 - 1",
                 what);
-  if (s.tiles * h.heads >= int64_t{1} << 31)
+  if (s.tiles * (h.heads + 2 * h.kv_heads) >= int64_t{1} << 31)
     return fail(ctx, NUMRS_HIP_E_SHAPE, "%s: too many tokens times heads", what);
   return NUMRS_HIP_OK;
 }
+
+// Magnitudes from which a tile's products might pass fp32's range: a score of two such operands
+// stays below 2^107, a sum of 2^20 such values times 2^15 below 2^127.
+constexpr float kMostScore = 0x1p50f, kMostValue = 0x1p90f;
+
+int padded(int dh) { return (dh + 31) / 32 * 32; }
+
+template <class F>
+int with_dp(int dh, F &&f) {
+  switch (padded(dh)) {
+    case 32: return f(std::integral_constant<int, 32>{});
+    case 64: return f(std::integral_constant<int, 64>{});
+    case 96: return f(std::integral_constant<int, 96>{});
+    default: return f(std::integral_constant<int, 128>{});
+  }
+}
+
+// Memory for one operand's fragments and exponents.
+struct Packed {
+  TempBlock block;
+  char *rows = nullptr, *cols = nullptr;
+  int *exps = nullptr;
+  explicit Packed(numrs_hip_ctx *ctx) : block(ctx) {}
+  int alloc(const Seqs &s, int heads, int dh, bool want_rows, bool want_cols) {
+    const size_t n = (size_t)s.tiles * heads, image = n * kTile * padded(dh) * 4;
+    if (int rc = block.alloc((want_rows + want_cols) * image + n * sizeof(int))) return rc;
+    char *p = static_cast<char *>(block.p);
+    if (want_rows) rows = p, p += image;
+    if (want_cols) cols = p, p += image;
+    exps = reinterpret_cast<int *>(p);
+    return NUMRS_HIP_OK;
+  }
+  tiles::Source source(const float *x, int64_t ld, int heads, float most) const {
+    return {x, ld, rows, cols, exps, most, heads};
+  }
+};
 
 }  // namespace
 
@@ -233,10 +273,26 @@ int packed_forward(numrs_hip_ctx *ctx, const Seqs &s, const float *q, int64_t ld
   if (q == nullptr || k == nullptr || v == nullptr || out == nullptr)
     return fail(ctx, NUMRS_HIP_E_INVALID, "attention_packed: null pointer");
   DeviceScope dev(ctx);
-  const FwdArgs a{s.in_order, q, k, v, out, stats, ld_q, ld_kv, ld_out, (int)h.heads,
-                  (int)h.kv_heads, (int)h.dh, kLog2e / std::sqrt((float)h.dh)};
-  forward_rows<<<(unsigned)(s.tiles * h.heads), 64 * kRows, 0, ctx->stream>>>(a);
-  return check_launch(ctx, "forward_rows");
+  Packed pq(ctx), pk(ctx), pv(ctx);
+  const int H = (int)h.heads, Hk = (int)h.kv_heads, dh = (int)h.dh;
+  if (int rc = pq.alloc(s, H, dh, true, false)) return rc;
+  if (int rc = pk.alloc(s, Hk, dh, true, false)) return rc;
+  if (int rc = pv.alloc(s, Hk, dh, false, true)) return rc;
+  const tiles::PackArgs p{s.in_order,
+                          {pq.source(q, ld_q, H, kMostScore), pk.source(k, ld_kv, Hk, kMostScore),
+                           pv.source(v, ld_kv, Hk, kMostValue), {}},
+                          H + 2 * Hk, dh};
+  const float alpha = kLog2e / std::sqrt((float)dh);
+  const FwdArgs a{s.by_work, q, k, v, out, stats, ld_q, ld_kv, ld_out, H, Hk, dh, alpha};
+  const tiles::ForwardArgs f{pq.rows, pk.rows, pv.cols, pq.exps, pk.exps, pv.exps, out, stats, ld_out,
+                             H, Hk, dh, alpha};
+  return with_dp(dh, [&](auto dp) {
+    constexpr int DP = decltype(dp)::value;
+    tiles::pack<DP><<<(unsigned)(s.tiles * p.slots), 256, 0, ctx->stream>>>(p);
+    if (int rc = check_launch(ctx, "pack")) return rc;
+    forward_block<DP><<<(unsigned)(s.blocks * H), 256, 0, ctx->stream>>>(a, f);
+    return check_launch(ctx, "forward_block");
+  });
 }
 
 int packed_backward(numrs_hip_ctx *ctx, const Seqs &s, const float *q, int64_t ld_q, const float *k,
@@ -300,12 +356,21 @@ int numrs_hip_seqs_create(numrs_hip_ctx *ctx, const int64_t *lengths, int64_t n,
       row += lengths[i];
     }
     s->tiles = (int64_t)tiles.size();
+    // Blocks of 128 rows, those with the most keys before them first: the last workgroups to start
+    // are the shortest.
+    std::vector<SeqTile> blocks;
+    for (const SeqTile &t : tiles)
+      if (t.t0 % 128 == 0) blocks.push_back(t);
+    std::stable_sort(blocks.begin(), blocks.end(), [](const SeqTile &a, const SeqTile &b) { return a.t0 > b.t0; });
+    s->blocks = (int64_t)blocks.size();
+    tiles.insert(tiles.end(), blocks.begin(), blocks.end());
     auto h = std::make_unique<numrs_hip_seqs>();
     if (!tiles.empty()) {
       void *p = nullptr;
       const size_t bytes = tiles.size() * sizeof(SeqTile);
       if (int rc = block_alloc(ctx, bytes, &p)) return rc;
       s->in_order = static_cast<SeqTile *>(p), s->bytes = bytes;
+      s->by_work = s->in_order + s->tiles;
       if (int rc = numrs_hip_upload(ctx, p, tiles.data(), bytes)) return rc;
     }
     h->s = std::move(s);
