@@ -23,7 +23,8 @@ struct Seqs {
   numrs_hip_ctx *ctx = nullptr;
   int64_t n = 0, total = 0, tiles = 0, blocks = 0;
   SeqTile *in_order = nullptr;  // [tiles]; a tile's number is its place
-  SeqTile *by_work = nullptr;   // [blocks] of 128 tokens, those late in their sequence first
+  SeqTile *by_work = nullptr;   // [blocks] of 128 tokens, those with the most tokens before them first
+  SeqTile *by_rest = nullptr;   // [blocks], those with the most tokens after them first
   size_t bytes = 0;
   ~Seqs() { block_free(ctx, in_order, bytes); }
 };

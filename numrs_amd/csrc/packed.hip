@@ -93,51 +93,38 @@ __global__ void __launch_bounds__(256, 2) forward_block(FwdArgs a, tiles::Forwar
 struct BwdArgs {
   const SeqTile *tiles;
   const float *q, *k, *v, *out, *dout, *stats;
-  float *D, *dq, *dk, *dv;  // D [total, heads]
   int64_t ld_q, ld_kv, ld_out;
-  int heads, kv_heads, dh, accumulate;
-  float alpha, scale;  // log2(e) / sqrt(dh), 1 / sqrt(dh)
 };
-
-// D = dout . out of each row and head.
-__global__ void __launch_bounds__(256) row_dots(BwdArgs a, int64_t total) {
-  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (i >= total * a.heads) return;
-  const int64_t at = i / a.heads * a.ld_out + i % a.heads * a.dh;
-  float s = 0.f;
-  if (lane < a.dh) s = a.dout[at + lane] * a.out[at + lane];
-  if (lane + 64 < a.dh) s = fmaf(a.dout[at + lane + 64], a.out[at + lane + 64], s);
-  s = wave_sum(s);
-  if (lane == 0) a.D[i] = s;
-}
 
 __device__ __forceinline__ void put(float *p, float v, int accumulate) { *p = accumulate ? *p + v : v; }
 
-// One wave: dq of query row r and head h.  x: two rows of dh floats.
-__device__ void row_dq(const BwdArgs &a, const SeqTile &t, int r, int h, float *x) {
+// One wave: dq of query row r and head h, in plain fp32.  x: two rows of LDS.
+__device__ void row_dq(const BwdArgs &b, const tiles::BackwardArgs &a, const SeqTile &t, int r, int h, float *x) {
   const int lane = threadIdx.x & 63, g = h / (a.heads / a.kv_heads);
-  const int64_t row = t.row0 + r;
+  const int64_t row = t.row0 + r, at = row * b.ld_out + (int64_t)h * a.dh;
+  float dot = 0.f;
   for (int d = lane; d < a.dh; d += 64) {
-    x[d] = a.q[row * a.ld_q + (int64_t)h * a.dh + d];
-    x[128 + d] = a.dout[row * a.ld_out + (int64_t)h * a.dh + d];
+    x[d] = b.q[row * b.ld_q + (int64_t)h * a.dh + d];
+    x[128 + d] = b.dout[at + d];
+    dot = fmaf(x[128 + d], b.out[at + d], dot);
   }
+  const float D = wave_sum(dot);
   __builtin_amdgcn_wave_barrier();
-  const float *k = a.k + t.row0 * a.ld_kv + (int64_t)g * a.dh, *v = a.v + t.row0 * a.ld_kv + (int64_t)g * a.dh;
-  const float *st = a.stats + (row * a.heads + h) * 2;
-  const float m = st[0], l = st[1], D = a.D[row * a.heads + h];
+  const float *k = b.k + t.row0 * b.ld_kv + (int64_t)g * a.dh, *v = b.v + t.row0 * b.ld_kv + (int64_t)g * a.dh;
+  const float *st = b.stats + (row * a.heads + h) * 2;
+  const float m = st[0], l = st[1];
   float o0 = 0.f, o1 = 0.f;
   for (int j0 = 0; j0 <= r; j0 += 64) {
     const int j = j0 + lane, n = min(64, r + 1 - j0);
     float ds = 0.f;
     if (lane < n) {
-      const float p = exp2f(dot_row(x, k + j * a.ld_kv, a.dh) * a.alpha - m) / l;
-      ds = p * (dot_row(x + 128, v + j * a.ld_kv, a.dh) - D);
+      const float p = exp2f(dot_row(x, k + j * b.ld_kv, a.dh) * a.alpha - m) / l;
+      ds = p * (dot_row(x + 128, v + j * b.ld_kv, a.dh) - D);
     }
     float t0 = 0.f, t1 = 0.f;
     for (int e = 0; e < n; ++e) {
       const float w = lane_of(ds, e);
-      const float *y = k + (j0 + e) * a.ld_kv;
+      const float *y = k + (j0 + e) * b.ld_kv;
       if (lane < a.dh) t0 = fmaf(w, y[lane], t0);
       if (lane + 64 < a.dh) t1 = fmaf(w, y[lane + 64], t1);
     }
@@ -148,64 +135,91 @@ __device__ void row_dq(const BwdArgs &a, const SeqTile &t, int r, int h, float *
   if (lane + 64 < a.dh) put(o + lane + 64, o1 * a.scale, a.accumulate);
 }
 
-// One wave: dk and dv of key row r and kv head g, over the query heads of g in order.
-__device__ void row_dkv(const BwdArgs &a, const SeqTile &t, int r, int g, float *x) {
-  const int lane = threadIdx.x & 63, group = a.heads / a.kv_heads;
-  const int64_t row = t.row0 + r, at = row * a.ld_kv + (int64_t)g * a.dh;
-  for (int d = lane; d < a.dh; d += 64) x[d] = a.k[at + d], x[128 + d] = a.v[at + d];
+// One wave: dk and dv of key row r, over a.each query heads from h0 in order.
+__device__ void row_dkv(const BwdArgs &b, const tiles::BackwardArgs &a, const SeqTile &t, int r, int h0, float *x) {
+  const int lane = threadIdx.x & 63, group = a.heads / a.kv_heads, g = h0 / group;
+  const int64_t row = t.row0 + r, at = row * b.ld_kv + (int64_t)g * a.dh;
+  for (int d = lane; d < a.dh; d += 64) x[d] = b.k[at + d], x[128 + d] = b.v[at + d];
   __builtin_amdgcn_wave_barrier();
   float k0 = 0.f, k1 = 0.f, v0 = 0.f, v1 = 0.f;
-  for (int h = g * group; h < (g + 1) * group; ++h) {
-    const float *q = a.q + (int64_t)h * a.dh, *go = a.dout + (int64_t)h * a.dh;
+  for (int h = h0; h < h0 + a.each; ++h) {
+    const float *q = b.q + (int64_t)h * a.dh, *go = b.dout + (int64_t)h * a.dh, *out = b.out + (int64_t)h * a.dh;
     for (int i0 = r; i0 < t.len; i0 += 64) {
       const int n = min(64, t.len - i0);
       float p = 0.f, ds = 0.f;
       if (lane < n) {
         const int64_t i = t.row0 + i0 + lane;
-        const float *st = a.stats + (i * a.heads + h) * 2;
-        p = exp2f(dot_row(x, q + i * a.ld_q, a.dh) * a.alpha - st[0]) / st[1];
-        ds = p * (dot_row(x + 128, go + i * a.ld_out, a.dh) - a.D[i * a.heads + h]);
+        const float *st = b.stats + (i * a.heads + h) * 2;
+        p = exp2f(dot_row(x, q + i * b.ld_q, a.dh) * a.alpha - st[0]) / st[1];
+        ds = p * (dot_row(x + 128, go + i * b.ld_out, a.dh) - dot_row(out + i * b.ld_out, go + i * b.ld_out, a.dh));
       }
       float tk0 = 0.f, tk1 = 0.f, tv0 = 0.f, tv1 = 0.f;
       for (int e = 0; e < n; ++e) {
         const int64_t i = t.row0 + i0 + e;
         const float w = lane_of(p, e), u = lane_of(ds, e);
         if (lane < a.dh) {
-          tv0 = fmaf(w, go[i * a.ld_out + lane], tv0);
-          tk0 = fmaf(u, q[i * a.ld_q + lane], tk0);
+          tv0 = fmaf(w, go[i * b.ld_out + lane], tv0);
+          tk0 = fmaf(u, q[i * b.ld_q + lane], tk0);
         }
         if (lane + 64 < a.dh) {
-          tv1 = fmaf(w, go[i * a.ld_out + lane + 64], tv1);
-          tk1 = fmaf(u, q[i * a.ld_q + lane + 64], tk1);
+          tv1 = fmaf(w, go[i * b.ld_out + lane + 64], tv1);
+          tk1 = fmaf(u, q[i * b.ld_q + lane + 64], tk1);
         }
       }
       k0 += tk0, k1 += tk1, v0 += tv0, v1 += tv1;
     }
   }
+  const int64_t part = ((int64_t)h0 * a.total + row) * a.dh;
+  const int64_t ck = a.each < group ? part : row * a.ld_k + (int64_t)g * a.dh;
+  const int64_t cv = a.each < group ? part : row * a.ld_v + (int64_t)g * a.dh;
   if (a.dk != nullptr) {
-    if (lane < a.dh) put(a.dk + at + lane, k0 * a.scale, a.accumulate);
-    if (lane + 64 < a.dh) put(a.dk + at + lane + 64, k1 * a.scale, a.accumulate);
+    if (lane < a.dh) put(a.dk + ck + lane, k0 * a.scale, a.accumulate);
+    if (lane + 64 < a.dh) put(a.dk + ck + lane + 64, k1 * a.scale, a.accumulate);
   }
   if (a.dv != nullptr) {
-    if (lane < a.dh) put(a.dv + at + lane, v0, a.accumulate);
-    if (lane + 64 < a.dh) put(a.dv + at + lane + 64, v1, a.accumulate);
+    if (lane < a.dh) put(a.dv + cv + lane, v0, a.accumulate);
+    if (lane + 64 < a.dh) put(a.dv + cv + lane + 64, v1, a.accumulate);
   }
 }
 
-__global__ void __launch_bounds__(64 * kRows) dq_rows(BwdArgs a) {
-  __shared__ float x[kRows][256];
-  const int w = threadIdx.x >> 6;
-  const SeqTile t = a.tiles[blockIdx.x / a.heads];
-  const int h = blockIdx.x % a.heads, end = min(t.len, t.t0 + kTile);
-  for (int r = t.t0 + w; r < end; r += kRows) row_dq(a, t, r, h, x[w]);
+// A block of 128 query rows of one head.
+template <int DP>
+__global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) dq_block(BwdArgs b, tiles::BackwardArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[2 * 3 * 32 * DP * 4];
+  const SeqTile t = b.tiles[blockIdx.x / a.heads];
+  const int h = blockIdx.x % a.heads;
+  if (tiles::dq_tile<DP>(a, t, h, lds)) return;
+  const int w = threadIdx.x >> 6, end = min(t.len, t.t0 + 128);
+  for (int r = t.t0 + w; r < end; r += kRows) row_dq(b, a, t, r, h, reinterpret_cast<float *>(lds) + 256 * w);
 }
 
-__global__ void __launch_bounds__(64 * kRows) dkv_rows(BwdArgs a) {
-  __shared__ float x[kRows][256];
-  const int w = threadIdx.x >> 6;
-  const SeqTile t = a.tiles[blockIdx.x / a.kv_heads];
-  const int g = blockIdx.x % a.kv_heads, end = min(t.len, t.t0 + kTile);
-  for (int r = t.t0 + w; r < end; r += kRows) row_dkv(a, t, r, g, x[w]);
+// A block of 128 key rows of one kv head, or one query head's part of it.
+template <int DP>
+__global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) dkv_block(BwdArgs b, tiles::BackwardArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[2 * (4 * 32 * DP * 4 + 256)];
+  const int slots = a.heads / a.each;
+  const SeqTile t = b.tiles[blockIdx.x / slots];
+  const int h0 = blockIdx.x % slots * a.each;
+  if (tiles::dkv_tile<DP>(a, t, h0, lds)) return;
+  const int w = threadIdx.x >> 6, end = min(t.len, t.t0 + 128);
+  for (int r = t.t0 + w; r < end; r += kRows) row_dkv(b, a, t, r, h0, reinterpret_cast<float *>(lds) + 256 * w);
+}
+
+// Adds the parts of a group's query heads in order, four values a thread: part [heads, total, dh].
+__global__ void __launch_bounds__(256)
+    join_heads(const float *part, float *out, int64_t ld, int64_t total, int heads, int kv_heads, int dh,
+               int accumulate) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int per = dh / 4, group = heads / kv_heads;
+  if (i >= total * kv_heads * per) return;
+  const int64_t row = i / (kv_heads * per);
+  const int g = (int)(i / per % kv_heads), d = (int)(i % per) * 4;
+  tiles::f4 s{};
+  for (int h = g * group; h < (g + 1) * group; ++h)
+    s += *reinterpret_cast<const tiles::f4 *>(part + ((int64_t)h * total + row) * dh + d);
+  tiles::f4u *o = reinterpret_cast<tiles::f4u *>(out + row * ld + (int64_t)g * dh + d);
+  if (accumulate) s += tiles::f4(*o);
+  *o = s;
 }
 
 // The arguments that the forward and the backward share.
@@ -220,7 +234,7 @@ int check_packed(numrs_hip_ctx *ctx, const Seqs &s, int64_t ld_q, int64_t ld_kv,
       paging::bad_stride(ld_out, h.heads * h.dh))
     return fail(ctx, NUMRS_HIP_E_SHAPE, "%s: a row stride is below its row's width or above 2^31 - 1",
                 what);
-  if (s.tiles * (h.heads + 2 * h.kv_heads) >= int64_t{1} << 31)
+  if (s.tiles * 2 * (h.heads + h.kv_heads) >= int64_t{1} << 31)
     return fail(ctx, NUMRS_HIP_E_SHAPE, "%s: too many tokens times heads", what);
   return NUMRS_HIP_OK;
 }
@@ -257,7 +271,7 @@ struct Packed {
     return NUMRS_HIP_OK;
   }
   tiles::Source source(const float *x, int64_t ld, int heads, float most) const {
-    return {x, ld, rows, cols, exps, most, heads};
+    return {x, ld, rows, cols, exps, most, heads, nullptr, nullptr, nullptr};
   }
 };
 
@@ -305,23 +319,58 @@ int packed_backward(numrs_hip_ctx *ctx, const Seqs &s, const float *q, int64_t l
       stats == nullptr)
     return fail(ctx, NUMRS_HIP_E_INVALID, "attention_packed_backward: null pointer");
   DeviceScope dev(ctx);
-  TempBlock D(ctx);
-  if (int rc = D.alloc((size_t)(s.total * h.heads) * sizeof(float))) return rc;
-  const float scale = 1.0f / std::sqrt((float)h.dh);
-  const BwdArgs a{s.in_order, q, k, v, out, dout, stats, D.f(), dq, dk, dv, ld_q, ld_kv, ld_out,
-                  (int)h.heads, (int)h.kv_heads, (int)h.dh, accumulate, kLog2e / std::sqrt((float)h.dh),
-                  scale};
-  row_dots<<<grid_for(s.total * h.heads, 4), 256, 0, ctx->stream>>>(a, s.total);
-  if (int rc = check_launch(ctx, "row_dots")) return rc;
-  if (dq != nullptr) {
-    dq_rows<<<(unsigned)(s.tiles * h.heads), 64 * kRows, 0, ctx->stream>>>(a);
-    if (int rc = check_launch(ctx, "dq_rows")) return rc;
-  }
-  if (dk != nullptr || dv != nullptr) {
-    dkv_rows<<<(unsigned)(s.tiles * h.kv_heads), 64 * kRows, 0, ctx->stream>>>(a);
-    if (int rc = check_launch(ctx, "dkv_rows")) return rc;
-  }
-  return NUMRS_HIP_OK;
+  const int H = (int)h.heads, Hk = (int)h.kv_heads, dh = (int)h.dh, group = H / Hk;
+  const bool keys = dk != nullptr || dv != nullptr;
+  // The query heads of a group go to workgroups of their own, whose parts are added afterwards,
+  // unless the key rows alone make enough of them.
+  const int each = group > 1 && s.blocks * Hk >= 4 * ctx->num_cus ? group : 1;
+  Packed pq(ctx), pk(ctx), pv(ctx), pg(ctx);
+  TempBlock rowstat(ctx), parts(ctx);
+  if (int rc = pq.alloc(s, H, dh, true, keys)) return rc;
+  if (int rc = pk.alloc(s, Hk, dh, true, dq != nullptr)) return rc;
+  if (int rc = pv.alloc(s, Hk, dh, true, false)) return rc;
+  if (int rc = pg.alloc(s, H, dh, true, keys)) return rc;
+  if (int rc = rowstat.alloc((size_t)s.tiles * H * kTile * 2 * sizeof(float))) return rc;
+  const size_t part = (size_t)s.total * H * dh * sizeof(float);
+  if (keys && each < group)
+    if (int rc = parts.alloc(((dk != nullptr) + (dv != nullptr)) * part)) return rc;
+  tiles::PackArgs p{s.in_order,
+                    {pq.source(q, ld_q, H, kMostScore), pk.source(k, ld_kv, Hk, kMostScore),
+                     pv.source(v, ld_kv, Hk, kMostValue), pg.source(dout, ld_out, H, kMostValue)},
+                    2 * H + 2 * Hk, dh};
+  p.src[3].out = out, p.src[3].stats = stats, p.src[3].rowstat = rowstat.f();
+  const float alpha = kLog2e / std::sqrt((float)dh), scale = 1.0f / std::sqrt((float)dh);
+  BwdArgs b{s.by_work, q, k, v, out, dout, stats, ld_q, ld_kv, ld_out};
+  tiles::BackwardArgs a{pq.rows, pq.cols, pk.rows, pk.cols, pv.rows, pg.rows, pg.cols, pq.exps, pk.exps,
+                        pv.exps, pg.exps, rowstat.f(), dq, dk, dv, ld_q, ld_kv, ld_kv, s.total,
+                        H, Hk, dh, accumulate, each, alpha, scale};
+  return with_dp(dh, [&](auto dp) {
+    constexpr int DP = decltype(dp)::value;
+    tiles::pack<DP><<<(unsigned)(s.tiles * p.slots), 256, 0, ctx->stream>>>(p);
+    if (int rc = check_launch(ctx, "pack")) return rc;
+    if (dq != nullptr) {
+      dq_block<DP><<<(unsigned)(s.blocks * H), 256, 0, ctx->stream>>>(b, a);
+      if (int rc = check_launch(ctx, "dq_block")) return rc;
+    }
+    if (!keys) return (int)NUMRS_HIP_OK;
+    b.tiles = s.by_rest;
+    if (each < group) {
+      a.dk = dk != nullptr ? parts.f() : nullptr;
+      a.dv = dv != nullptr ? parts.f() + (dk != nullptr ? part / sizeof(float) : 0) : nullptr;
+      a.accumulate = 0;
+    }
+    dkv_block<DP><<<(unsigned)(s.blocks * (H / each)), 256, 0, ctx->stream>>>(b, a);
+    if (int rc = check_launch(ctx, "dkv_block")) return rc;
+    if (each < group) {
+      const unsigned grid = grid_for(s.total * Hk * (dh / 4), 256);
+      if (dk != nullptr)
+        join_heads<<<grid, 256, 0, ctx->stream>>>(a.dk, dk, ld_kv, s.total, H, Hk, dh, accumulate);
+      if (dv != nullptr)
+        join_heads<<<grid, 256, 0, ctx->stream>>>(a.dv, dv, ld_kv, s.total, H, Hk, dh, accumulate);
+      return check_launch(ctx, "join_heads");
+    }
+    return (int)NUMRS_HIP_OK;
+  });
 }
 
 }  // namespace numrs_hip
@@ -364,13 +413,16 @@ int numrs_hip_seqs_create(numrs_hip_ctx *ctx, const int64_t *lengths, int64_t n,
     std::stable_sort(blocks.begin(), blocks.end(), [](const SeqTile &a, const SeqTile &b) { return a.t0 > b.t0; });
     s->blocks = (int64_t)blocks.size();
     tiles.insert(tiles.end(), blocks.begin(), blocks.end());
+    std::stable_sort(blocks.begin(), blocks.end(),
+                     [](const SeqTile &a, const SeqTile &b) { return a.len - a.t0 > b.len - b.t0; });
+    tiles.insert(tiles.end(), blocks.begin(), blocks.end());
     auto h = std::make_unique<numrs_hip_seqs>();
     if (!tiles.empty()) {
       void *p = nullptr;
       const size_t bytes = tiles.size() * sizeof(SeqTile);
       if (int rc = block_alloc(ctx, bytes, &p)) return rc;
       s->in_order = static_cast<SeqTile *>(p), s->bytes = bytes;
-      s->by_work = s->in_order + s->tiles;
+      s->by_work = s->in_order + s->tiles, s->by_rest = s->by_work + s->blocks;
       if (int rc = numrs_hip_upload(ctx, p, tiles.data(), bytes)) return rc;
     }
     h->s = std::move(s);
