@@ -1,9 +1,10 @@
 // A paged key-value cache in fp32 or 8-bit codes, written, read back and attended to (no reference
 // op).  paging.h says where a token lies; every position goes through paging::page_of.
+#include <algorithm>
 #include <cmath>
 
 #include "packed.h"
-#include "paging.h"
+#include "paged_split.h"
 
 namespace {
 
@@ -11,13 +12,7 @@ using namespace numrs_hip;
 
 constexpr float kLog2e = 1.44269504088896341f;
 
-struct Cache {
-  void *k, *v;
-  float *ks, *vs;
-  int64_t pages, max_pages;
-  const int32_t *table;
-  int shift, kv_heads, dh;
-};
+using paged::Cache;
 
 struct RowArgs {
   Cache c;
@@ -107,59 +102,6 @@ __global__ void __launch_bounds__(256) read_rows(RowArgs a) {
       a.vo[at + d] = read_one<INT8>(a.c, s, d, true);
     }
   }
-}
-
-struct PagedArgs {
-  Cache c;
-  const float *q;
-  const int32_t *lengths;
-  float *out;
-  int64_t ld_q, ld_out;
-  int heads;
-  float alpha;  // log2(e) / sqrt(dh)
-};
-
-// One wave a query row and head: 64 tokens at a time, a token a lane for the scores, a column a
-// lane for the output.
-template <bool INT8>
-__global__ void __launch_bounds__(64) paged_rows(PagedArgs a) {
-  __shared__ float x[128];
-  const int i = blockIdx.x / a.heads, h = blockIdx.x % a.heads, lane = threadIdx.x;
-  const int g = h / (a.heads / a.c.kv_heads), dh = a.c.dh;
-  for (int d = lane; d < dh; d += 64) x[d] = a.q[i * a.ld_q + (int64_t)h * dh + d];
-  __syncthreads();
-  const int64_t len = paging::held(a.lengths[i], a.c.max_pages, a.c.shift);
-  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-  bool any = false;
-  for (int64_t j0 = 0; j0 < len; j0 += 64) {
-    const int n = (int)min((int64_t)64, len - j0);
-    Slot s{0, 0, -1};
-    if (lane < n) s = slot_of(a.c, i, j0 + lane, g);
-    if (!__any(s.page >= 0)) continue;
-    float z = -INFINITY;
-    if (s.page >= 0) {
-      z = 0.f;
-      for (int d = 0; d < dh; ++d) z = fmaf(x[d], read_one<INT8>(a.c, s, d, false), z);
-      z *= a.alpha;
-    }
-    const float top = fmaxf(m, wave_max(z));
-    const float p = s.page >= 0 ? exp2f(z - top) : 0.f, c = any ? exp2f(m - top) : 0.f;
-    any = true;
-    m = top;
-    l = l * c + wave_sum(p);
-    float t0 = 0.f, t1 = 0.f;  // the block's sum apart, so that a long sum's rounding stays small
-    for (int e = 0; e < n; ++e) {
-      const Slot t = slot_of(a.c, i, j0 + e, g);
-      if (t.page < 0) continue;
-      const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, p), e));
-      if (lane < dh) t0 = fmaf(w, read_one<INT8>(a.c, t, lane, true), t0);
-      if (lane + 64 < dh) t1 = fmaf(w, read_one<INT8>(a.c, t, lane + 64, true), t1);
-    }
-    o0 = fmaf(o0, c, t0), o1 = fmaf(o1, c, t1);
-  }
-  float *o = a.out + i * a.ld_out + (int64_t)h * dh;
-  if (lane < dh) o[lane] = any ? o0 / l : 0.f;
-  if (lane + 64 < dh) o[lane + 64] = any ? o1 / l : 0.f;
 }
 
 Cache device_cache(const numrs_hip_kv_cache &c, const int32_t *table, int64_t max_pages) {
@@ -255,13 +197,33 @@ int numrs_hip_attention_paged(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cach
   if (q == nullptr || out == nullptr)
     return fail(ctx, NUMRS_HIP_E_INVALID, "attention_paged: null pointer");
   DeviceScope dev(ctx);
-  const PagedArgs a{device_cache(*cache, table, max_pages), q, lengths, out, ld_q, ld_out, (int)heads,
-                    kLog2e / std::sqrt((float)cache->head_dim)};
-  if (cache->format == NUMRS_HIP_KV_F32)
-    paged_rows<false><<<(unsigned)(n * heads), 64, 0, ctx->stream>>>(a);
-  else
-    paged_rows<true><<<(unsigned)(n * heads), 64, 0, ctx->stream>>>(a);
-  return check_launch(ctx, "paged_rows");
+  const int hk = (int)cache->kv_heads, dh = (int)cache->head_dim, group = (int)heads / hk;
+  const int blocks = (group + 15) / 16;
+  // Two workgroups a CU, which the registers allow, each with an even share of the tokens.
+  const int shares = std::max(1, (2 * ctx->num_cus + hk * blocks - 1) / (hk * blocks));
+  const int64_t wgs = (int64_t)shares * hk * blocks;
+  TempBlock parts(ctx);
+  const int dp = (dh + 31) / 32 * 32;
+  if (int rc = parts.alloc((size_t)(2 * wgs * (32 + 16 * dp)) * sizeof(float))) return rc;
+  unsigned *arrivals = nullptr;
+  if (int rc = arrival_counters(ctx, (size_t)(3 * wgs), &arrivals)) return rc;
+  const paged::SplitArgs a{device_cache(*cache, table, max_pages), q, lengths, out, parts.f(), arrivals, ld_q,
+                           ld_out, (int)n, (int)heads, blocks, shares,
+                           kLog2e / std::sqrt((float)dh)};
+  auto launch = [&](auto padded) {
+    constexpr int DP = decltype(padded)::value;
+    if (cache->format == NUMRS_HIP_KV_F32)
+      paged::split_rows<false, DP><<<(unsigned)wgs, 256, 0, ctx->stream>>>(a);
+    else
+      paged::split_rows<true, DP><<<(unsigned)wgs, 256, 0, ctx->stream>>>(a);
+  };
+  switch (dp) {
+    case 32: launch(std::integral_constant<int, 32>{}); break;
+    case 64: launch(std::integral_constant<int, 64>{}); break;
+    case 96: launch(std::integral_constant<int, 96>{}); break;
+    default: launch(std::integral_constant<int, 128>{});
+  }
+  return check_launch(ctx, "split_rows");
 }
 
 }  // extern "C"

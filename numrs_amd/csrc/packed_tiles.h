@@ -1,0 +1,641 @@
+// Causal attention over packed sequences on the fp16 matrix cores at fp32 accuracy.
+//
+// An fp32 operand x, times a power of two that puts its 64-token tile's largest magnitude into
+// [2^11, 2^12), is the sum h + m of two fp16 values, each rounded to nearest: h holds 11 bits, x -
+// h is exact and m holds its next 11, so h + m is x within 2^-23 |x| for |x| down to 2^-14 of the
+// largest and within 2^-36 of the largest below.  Of the four products of two such operands the
+// matrix cores form three, m h + h m + h h (the fourth is below 2^-22 of the product and of either
+// sign), each with fp32 accumulation: half of what three bf16 terms and six products take.
+// v_mfma_f32_32x32x16_f16 sums of at most 64 tokens (or one head) start from zero and are added to
+// fp32 totals: the matrix cores' own sum is cut off, not rounded.
+//
+// `pack` splits each operand once a call, in the order in which the products read it: a fragment is
+// 64 lanes x 16 bytes, so a tile goes to LDS by a plain copy and every LDS access is contiguous.
+//   row fragment (32 tokens, 16 columns): lane (g, c) has token c, columns 8 g .. + 7;
+//   column fragment (32 columns, 16 tokens): lane (g, c) has column c of the tokens 4 g .. + 3 and
+//   8 + 4 g .. + 3, which is the order in which a product leaves its results' rows: the
+//   probabilities of one product are the next one's operand in the lane that formed them.
+#pragma once
+
+#include "packed.h"
+
+namespace tiles {
+
+using numrs_hip::kTile;
+using numrs_hip::SeqTile;
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef float f16 __attribute__((ext_vector_type(16)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+
+// A tile's exponent where its values do not split: one that is not finite, or so large that a
+// product might pass fp32's range.  Workgroups that meet one take the row kernels' arithmetic.
+constexpr int kOdd = 1 << 20;
+
+// x = h + m of a pair.
+__device__ __forceinline__ void split(float a, float b, unsigned &h, unsigned &m) {
+  const h2 t = __builtin_convertvector(f2{a, b}, h2);
+  h = __builtin_bit_cast(unsigned, t);
+  // a - h with h taken from its half of the pair: one instruction instead of two
+  float r0, r1;
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(h), "v"(a));
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(h), "v"(b));
+  m = __builtin_bit_cast(unsigned, __builtin_convertvector(f2{r0, r1}, h2));
+}
+
+struct Terms {
+  h8 h, m;
+};
+
+__device__ __forceinline__ Terms split8(const float *x) {
+  u4 h, m;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    unsigned a, b;
+    split(x[2 * j], x[2 * j + 1], a, b);
+    h[j] = a, m[j] = b;
+  }
+  return {__builtin_bit_cast(h8, h), __builtin_bit_cast(h8, m)};
+}
+
+// acc += a b, the small products first.
+__device__ __forceinline__ void mma(f16 &acc, const Terms &a, const Terms &b) {
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.m, b.h, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, b.m, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, b.h, acc, 0, 0, 0);
+}
+
+// Row of a 32x32 result that register i of lane group g holds.
+__device__ __forceinline__ constexpr int out_row(int i, int g) { return 8 * (i >> 2) + 4 * g + (i & 3); }
+
+// A head size rounded up to DP: 64-token tiles of fragments, the two terms of each side by side.
+template <int DP>
+struct Shape {
+  static constexpr int NS = DP / 16, NB = DP / 32;  // steps of a product over the head, blocks of 32 columns
+  static constexpr int kBytes = kTile * DP * 4;     // a tile's fragments
+  // byte offsets of a fragment pair
+  static __device__ __forceinline__ constexpr int row_frag(int kb, int s) { return (kb * NS + s) * 2048; }
+  static __device__ __forceinline__ constexpr int col_frag(int kb, int s, int db) {
+    return ((kb * 2 + s) * NB + db) * 2048;
+  }
+};
+
+__device__ __forceinline__ Terms frag(const char *p, int lane) {
+  return {*reinterpret_cast<const h8 *>(p + lane * 16), *reinterpret_cast<const h8 *>(p + 1024 + lane * 16)};
+}
+
+// One operand to split: heads x tiles.
+struct Source {
+  const float *x;
+  int64_t ld;
+  char *rows, *cols;  // null: not needed in that order
+  int *exps;          // [tiles, heads]
+  float most;         // larger magnitudes make a tile odd
+  int heads;
+  // The output's gradient: its rows are divided by their softmax sum l, which turns the backward's
+  // p into 2^(s - m), and the rows' references and totals go to `rowstat` [tiles, heads, 64]: (m,
+  // out . dout / l) with the tile's factor; a row past the sequence has m = infinity (p = 0).
+  const float *out, *stats;
+  float *rowstat;
+};
+
+struct PackArgs {
+  const SeqTile *tiles;
+  Source src[4];
+  int slots, dh;  // heads of all sources
+};
+
+template <int DP>
+__global__ void __launch_bounds__(256) pack(PackArgs a) {
+  using S = Shape<DP>;
+  constexpr int NI = DP / 32, NC = DP / 8;  // a thread's chunks of 8 columns; chunks of a row
+  __shared__ unsigned image[kTile][DP + 1];
+  __shared__ float top[4];
+  __shared__ float part[kTile][NC + 1];  // out . dout of 8 columns
+  const int tile = blockIdx.x / a.slots, tid = threadIdx.x;
+  int head = blockIdx.x % a.slots, which = 0;
+  while (head >= a.src[which].heads) head -= a.src[which++].heads;
+  const Source s = a.src[which];
+  const SeqTile t = a.tiles[tile];
+  const int rows = min(kTile, t.len - t.t0);
+  const float *x = s.x + (int64_t)(t.row0 + t.t0) * s.ld + (int64_t)head * a.dh;
+  float v[NI][8], big = 0.f;
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int row = (i * 256 + tid) / NC, c = (i * 256 + tid) % NC;
+    f4 lo{}, hi{};
+    if (row < rows && c * 8 < a.dh) {
+      const float *p = x + row * s.ld + c * 8;
+      lo = *reinterpret_cast<const f4u *>(p), hi = *reinterpret_cast<const f4u *>(p + 4);
+    }
+    float inv = 1.f, dot = 0.f;
+    if (s.stats != nullptr && row < rows) {
+      const int64_t at = t.row0 + t.t0 + row;
+      inv = 1.f / s.stats[(at * s.heads + head) * 2 + 1];
+      if (c * 8 < a.dh) {
+        const float *p = s.out + at * s.ld + (int64_t)head * a.dh + c * 8;
+        const f4 x0 = *reinterpret_cast<const f4u *>(p), x1 = *reinterpret_cast<const f4u *>(p + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dot = fmaf(x0[j], lo[j], dot);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dot = fmaf(x1[j], hi[j], dot);
+      }
+      odd |= !__builtin_isfinite(dot);
+    }
+    if (s.stats != nullptr) part[row][c] = dot;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[i][j] = (j < 4 ? lo[j] : hi[j - 4]) * inv;
+      const float m = fabsf(v[i][j]);
+      odd |= !(m < s.most);
+      big = fmaxf(big, m);
+    }
+  }
+  big = wave_max(big);
+  if ((tid & 63) == 0) top[tid >> 6] = big;
+  const int any = __syncthreads_or(odd);
+  big = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+  if (any) {
+    if (tid == 0) s.exps[(int64_t)tile * s.heads + head] = kOdd;
+    return;
+  }
+  // below 2^-128 the factor itself would pass 2^140, and its inverse fp32's smallest
+  const int e = big > 0.f ? min(12 - __builtin_amdgcn_frexp_expf(big), 140) : 0;
+  if (tid == 0) s.exps[(int64_t)tile * s.heads + head] = e;
+  if (s.stats != nullptr && tid < kTile) {
+    float m = INFINITY, d = 0.f;
+    if (tid < rows) {
+      const float *st = s.stats + ((int64_t)(t.row0 + t.t0 + tid) * s.heads + head) * 2;
+      for (int c = 0; c < NC; ++c) d += part[tid][c];
+      m = st[0], d = __builtin_amdgcn_ldexpf(d / st[1], e);
+    }
+    *reinterpret_cast<f2 *>(s.rowstat + (((int64_t)tile * s.heads + head) * kTile + tid) * 2) = f2{m, d};
+  }
+  const int64_t at = ((int64_t)tile * s.heads + head) * S::kBytes;
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int row = (i * 256 + tid) / NC, c = (i * 256 + tid) % NC;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[i][j] = __builtin_amdgcn_ldexpf(v[i][j], e);
+    const Terms p = split8(v[i]);
+    if (s.rows != nullptr) {
+      char *o = s.rows + at + S::row_frag(row >> 5, c >> 1) + ((row & 31) + 32 * (c & 1)) * 16;
+      *reinterpret_cast<h8 *>(o) = p.h;
+      *reinterpret_cast<h8 *>(o + 1024) = p.m;
+    }
+    if (s.cols != nullptr) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const unsigned w = __builtin_bit_cast(unsigned, h2{p.h[j], p.m[j]});
+        image[row][c * 8 + j] = w;
+      }
+    }
+  }
+  if (s.cols == nullptr) return;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int f = (i * 256 + tid) >> 6, lane = tid & 63, g = lane >> 5;
+    const int db = f % S::NB, ks = f / S::NB;  // ks: 16 tokens
+    u4 h, m;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = 16 * ks + 4 * g + (j >= 2 ? 8 : 0) + 2 * (j & 1), d = 32 * db + (lane & 31);
+      const unsigned p = image[r][d], q = image[r + 1][d];
+      h[j] = (p & 0xffff) | q << 16;
+      m[j] = p >> 16 | (q & 0xffff0000);
+    }
+    char *o = s.cols + at + S::col_frag(ks >> 1, ks & 1, db) + lane * 16;
+    *reinterpret_cast<u4 *>(o) = h;
+    *reinterpret_cast<u4 *>(o + 1024) = m;
+  }
+}
+
+typedef __attribute__((address_space(3))) void lds_void;
+typedef const __attribute__((address_space(1))) void global_void;
+
+// Copies `bytes` (a multiple of 4096) of fragments to LDS without passing through registers: wave w
+// of four has every fourth kilobyte.
+template <int BYTES>
+__device__ __forceinline__ void fetch(const char *src, char *lds, int w, int lane) {
+  static_assert(BYTES % 4096 == 0);
+#pragma unroll
+  for (int i = 0; i < BYTES / 4096; ++i)
+    __builtin_amdgcn_global_load_lds((global_void *)(src + (i * 4 + w) * 1024 + lane * 16),
+                                     (lds_void *)(lds + (i * 4 + w) * 1024), 16, 0, 0);
+}
+
+// Waits for this wave's copies, then for the other waves': what any of them fetched is there.
+__device__ __forceinline__ void fetched() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
+template <class Op>
+__device__ __forceinline__ float over16(const f16 &x, Op op) {
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = op(x[2 * i], x[2 * i + 1]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = op(r[2 * i], r[2 * i + 1]);
+  return op(op(r[0], r[1]), op(r[2], r[3]));
+}
+
+struct ForwardArgs {
+  const char *q, *k, *v;      // fragments: rows of q and k, columns of v
+  const int *eq, *ek, *ev;
+  float *out, *stats;
+  int64_t ld_out;
+  int heads, kv_heads, dh;
+  float alpha;  // log2(e) / sqrt(dh)
+};
+
+// Four waves own 32 query rows each of a block of 128 and walk the keys before them.  S^T = K Q^T
+// leaves a query's scores in two lanes; p = 2^(s - m + 7) against a reference m that moves only
+// when a score passes it by 2^8 (so that p fits fp16), O^T += V^T P^T.
+//
+// Returns false, before any write, where a tile is odd.
+template <int DP>
+__device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile &t, int h, char *lds) {
+  using S = Shape<DP>;
+  constexpr int KT = DP <= 64 ? 64 : 32, KB = KT / 32, kStage = KT * DP * 4;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 31, hi = lane >> 5, g = h / (a.heads / a.kv_heads);
+  const int end = min(t.t0 + 128, t.len), q0 = t.t0 + 32 * w;
+  const int64_t kv0 = (int64_t)t.tile0 * a.kv_heads + g;  // the sequence's first tile of this head
+  const int first = t.t0 / kTile, last = (end - 1) / kTile;
+  bool odd = false;
+  for (int i = tid; i <= last; i += 256) {
+    odd |= a.ek[kv0 + (int64_t)i * a.kv_heads] == kOdd || a.ev[kv0 + (int64_t)i * a.kv_heads] == kOdd;
+    if (i >= first) odd |= a.eq[(int64_t)(t.tile0 + i) * a.heads + h] == kOdd;
+  }
+  if (__syncthreads_or(odd)) return false;
+
+  const bool live = q0 < t.len;
+  const int64_t qt = (int64_t)(t.tile0 + min(q0 / kTile, last)) * a.heads + h;
+  Terms q[S::NS];
+#pragma unroll
+  for (int s = 0; s < S::NS; ++s) q[s] = frag(a.q + qt * S::kBytes + S::row_frag(w & 1, s), lane);
+  const int eq = a.eq[qt];
+
+  f16 o[S::NB] = {};
+  float m = -INFINITY, top = -INFINITY, l = 0.f;
+  const int n = (end + KT - 1) / KT;              // key blocks of the workgroup
+  const int mine = live ? (q0 + 31) / KT + 1 : 0;  // and of the wave
+  auto tile_of = [&](int i) { return kv0 + (int64_t)(i * KT / kTile) * a.kv_heads; };
+  auto issue = [&](int i) {
+    const int64_t at = tile_of(i) * S::kBytes + (i * KT % kTile) * DP * 4;
+    char *to = lds + (i & 1) * 2 * kStage;
+    fetch<kStage>(a.k + at, to, w, lane);
+    fetch<kStage>(a.v + at, to + kStage, w, lane);
+  };
+  issue(0);
+  for (int i = 0; i < n; ++i) {
+    fetched();
+    if (i + 1 < n) issue(i + 1);
+    if (i >= mine) continue;
+    const char *kf = lds + (i & 1) * 2 * kStage, *vf = kf + kStage;
+    f16 s[KB] = {};
+#pragma unroll
+    for (int st = 0; st < S::NS; ++st)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) mma(s[kb], frag(kf + S::row_frag(kb, st), lane), q[st]);
+    // an underflow of f must not make -inf * f NaN
+    const float f = fmaxf(__builtin_amdgcn_ldexpf(a.alpha, -(eq + a.ek[tile_of(i)])), 1.17549435e-38f);
+    if ((i + 1) * KT > q0 + 1) {  // keys after a row of the wave
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (i * KT + 32 * kb + out_row(e, hi) > q0 + c) s[kb][e] = -INFINITY;
+    }
+    float most = over16(s[0], [](float x, float y) { return fmaxf(x, y); });
+    if constexpr (KB == 2) most = fmaxf(most, over16(s[1], [](float x, float y) { return fmaxf(x, y); }));
+    most *= f;
+    top = fmaxf(top, most);
+    if (__any(most > m + 8.f)) {
+      const float now = fmaxf(m, half_pair(most, [](float x, float y) { return fmaxf(x, y); }));
+      const float r = __builtin_amdgcn_exp2f(m - now);
+      m = now;
+      l *= r;
+#pragma unroll
+      for (int b = 0; b < S::NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[b][e] *= r;
+    }
+    Terms p[KB][2];
+    const float shift = 7.f - m;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[kb][e] = __builtin_amdgcn_exp2f(fmaf(s[kb][e], f, shift));
+      l += over16(s[kb], [](float x, float y) { return x + y; });
+      float x[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] = s[kb][e];
+      p[kb][0] = split8(x), p[kb][1] = split8(x + 8);
+    }
+    const float fv = __builtin_amdgcn_ldexpf(1.f, -a.ev[tile_of(i)]);
+#pragma unroll
+    for (int b = 0; b < S::NB; ++b) {
+      f16 x = {};
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int st = 0; st < 2; ++st) mma(x, frag(vf + S::col_frag(kb, st, b), lane), p[kb][st]);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[b][e] = fmaf(x[e], fv, o[b][e]);
+    }
+  }
+  const int row = q0 + c;
+  l = half_pair(l, [](float x, float y) { return x + y; });
+  top = half_pair(top, [](float x, float y) { return fmaxf(x, y); });
+  if (row >= t.len) return true;
+  const float inv = 1.f / l;
+  float *p = a.out + (int64_t)(t.row0 + row) * a.ld_out + (int64_t)h * a.dh;
+#pragma unroll
+  for (int b = 0; b < S::NB; ++b)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = 32 * b + 8 * e + 4 * hi;
+      if (d < a.dh) {
+        f4 x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = o[b][4 * e + j] * inv;
+        *reinterpret_cast<f4u *>(p + d) = x;
+      }
+    }
+  if (a.stats != nullptr && hi == 0) {
+    // relative to the largest score
+    float *st = a.stats + ((int64_t)(t.row0 + row) * a.heads + h) * 2;
+    st[0] = top, st[1] = l * __builtin_amdgcn_exp2f(m - 7.f - top);
+  }
+  return true;
+}
+
+struct BackwardArgs {
+  const char *q, *qt, *k, *kt, *v, *g, *gt;  // fragments: rows, and with t columns; g: the output's gradient
+  const int *eq, *ek, *ev, *eg;
+  const float *rowstat;
+  float *dq, *dk, *dv;
+  int64_t ld_q, ld_k, ld_v, total;
+  int heads, kv_heads, dh, accumulate;
+  int each;             // query heads of a workgroup of key rows: its group, or one
+  float alpha, scale;   // log2(e) / sqrt(dh), 1 / sqrt(dh)
+};
+
+__device__ __forceinline__ int wave_min(int v) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) v = min(v, __shfl_xor(v, d));
+  return v;
+}
+
+// Scales of dS.  With V's factors 2^ev and the gradient's 2^eg, dP comes as raw = dP 2^(ev + eg),
+// below 2^31; a row's total D may come from other tiles of V than the one at hand, so both are
+// brought to the smallest ev of the sequence, and by 2^-32 below 1:
+//   dS'' = 2^15 p (raw 2^(least - ev - 32) - D 2^(eg + least - 32)) = dS 2^(eg + least - 17),
+// at most 2^15 and split like any operand.
+__device__ __forceinline__ void dscores(const f16 &s, const f16 &raw, float f, float graw, const float *m,
+                                        const float *d, f16 &p, f16 &ds) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    p[e] = __builtin_amdgcn_exp2f(fmaf(s[e], f, 15.f - m[e]));
+    ds[e] = p[e] * fmaf(raw[e], graw, -d[e]);
+  }
+}
+
+// Writes a wave's 32 columns of a transposed result: row `row` of the matrix at p.
+template <int DP>
+__device__ __forceinline__ void put_rows(float *p, const f16 (&x)[DP / 32], int dh, int hi, int accumulate) {
+#pragma unroll
+  for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = 32 * b + 8 * e + 4 * hi;
+      if (d < dh) {
+        f4 y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = x[b][4 * e + j];
+        if (accumulate) y += f4(*reinterpret_cast<const f4u *>(p + d));
+        *reinterpret_cast<f4u *>(p + d) = y;
+      }
+    }
+}
+
+// dQ of 128 query rows of a head: like the forward, with S^T and dP^T of 32 keys at a time, dQ^T +=
+// K^T dS^T.  Returns false, before any write, where a tile is odd.
+template <int DP>
+__device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t, int h, char *lds) {
+  using S = Shape<DP>;
+  constexpr int kPart = 32 * DP * 4, kStage = 3 * kPart;
+  __shared__ int least4[4];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 31, hi = lane >> 5, g = h / (a.heads / a.kv_heads);
+  const int end = min(t.t0 + 128, t.len), q0 = t.t0 + 32 * w;
+  const int64_t kv0 = (int64_t)t.tile0 * a.kv_heads + g;
+  const int first = t.t0 / kTile, last = (end - 1) / kTile;
+  bool odd = false;
+  int least = kOdd;
+  for (int i = tid; i <= last; i += 256) {
+    const int ev = a.ev[kv0 + (int64_t)i * a.kv_heads];
+    least = min(least, ev);
+    odd |= a.ek[kv0 + (int64_t)i * a.kv_heads] == kOdd || ev == kOdd;
+    if (i >= first) {
+      const int64_t at = (int64_t)(t.tile0 + i) * a.heads + h;
+      odd |= a.eq[at] == kOdd || a.eg[at] == kOdd;
+    }
+  }
+  least = wave_min(least);
+  if (lane == 0) least4[w] = least;
+  if (__syncthreads_or(odd)) return false;
+  least = min(min(least4[0], least4[1]), min(least4[2], least4[3]));
+
+  const bool live = q0 < t.len;
+  const int64_t qt = (int64_t)(t.tile0 + min(q0 / kTile, last)) * a.heads + h;
+  Terms q[S::NS], go[S::NS];
+#pragma unroll
+  for (int s = 0; s < S::NS; ++s) {
+    q[s] = frag(a.q + qt * S::kBytes + S::row_frag(w & 1, s), lane);
+    go[s] = frag(a.g + qt * S::kBytes + S::row_frag(w & 1, s), lane);
+  }
+  const int eq = a.eq[qt], eg = a.eg[qt];
+  const f2 rs = *reinterpret_cast<const f2 *>(a.rowstat + (qt * kTile + 32 * (w & 1) + c) * 2);
+  float m[16], d[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) m[e] = rs[0], d[e] = __builtin_amdgcn_ldexpf(rs[1], least - 32);
+
+  f16 x[S::NB] = {};
+  const int n = (end + 31) / 32, mine = live ? q0 / 32 + 1 : 0;
+  auto tile_of = [&](int i) { return kv0 + (int64_t)(i >> 1) * a.kv_heads; };
+  auto issue = [&](int i) {
+    const int64_t at = tile_of(i) * S::kBytes + (i & 1) * kPart;
+    char *to = lds + (i & 1) * kStage;
+    fetch<kPart>(a.k + at, to, w, lane);
+    fetch<kPart>(a.v + at, to + kPart, w, lane);
+    fetch<kPart>(a.kt + at, to + 2 * kPart, w, lane);
+  };
+  issue(0);
+  for (int i = 0; i < n; ++i) {
+    fetched();
+    if (i + 1 < n) issue(i + 1);
+    if (i >= mine) continue;
+    const char *kf = lds + (i & 1) * kStage, *vf = kf + kPart, *ktf = vf + kPart;
+    f16 s = {}, r = {};
+#pragma unroll
+    for (int st = 0; st < S::NS; ++st) {
+      mma(s, frag(kf + S::row_frag(0, st), lane), q[st]);
+      mma(r, frag(vf + S::row_frag(0, st), lane), go[st]);
+    }
+    const int ek = a.ek[tile_of(i)], ev = a.ev[tile_of(i)];
+    f16 p, ds;
+    dscores(s, r, __builtin_amdgcn_ldexpf(a.alpha, -(eq + ek)), __builtin_amdgcn_ldexpf(1.f, least - ev - 32), m, d,
+            p, ds);
+    if (32 * i + 31 > q0) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (32 * i + out_row(e, hi) > q0 + c) ds[e] = 0.f;
+    }
+    float y[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) y[e] = ds[e];
+    const Terms b[2] = {split8(y), split8(y + 8)};
+    const float back = __builtin_amdgcn_ldexpf(a.scale, 17 - eg - least - ek);
+#pragma unroll
+    for (int nb = 0; nb < S::NB; ++nb) {
+      f16 z = {};
+      mma(z, frag(ktf + S::col_frag(0, 0, nb), lane), b[0]);
+      mma(z, frag(ktf + S::col_frag(0, 1, nb), lane), b[1]);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[nb][e] = fmaf(z[e], back, x[nb][e]);
+    }
+  }
+  const int row = q0 + c;
+  if (row < t.len)
+    put_rows<DP>(a.dq + (int64_t)(t.row0 + row) * a.ld_q + (int64_t)h * a.dh, x, a.dh, hi, a.accumulate);
+  return true;
+}
+
+// dK and dV of 128 key rows: four waves own 32 keys each and walk the queries from theirs on, for
+// each query head in turn: S = Q K^T and dP = dO V^T of 32 queries, dV^T += dO^T P, dK^T += Q^T dS.
+template <int DP>
+__device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t, int h0, char *lds) {
+  using S = Shape<DP>;
+  constexpr int kPart = 32 * DP * 4, kStage = 4 * kPart + 256;
+  __shared__ int least4[4];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 31, hi = lane >> 5, g = h0 / (a.heads / a.kv_heads);
+  const int end = min(t.t0 + 128, t.len), k0 = t.t0 + 32 * w;
+  const int64_t kv0 = (int64_t)t.tile0 * a.kv_heads + g;
+  const int first = t.t0 / kTile, last = (end - 1) / kTile, all = (t.len - 1) / kTile;
+  bool odd = false;
+  int least = kOdd;
+  for (int i = tid; i <= all; i += 256) {
+    const int ev = a.ev[kv0 + (int64_t)i * a.kv_heads];
+    least = min(least, ev);
+    odd |= ev == kOdd;
+    if (i >= first && i <= last) odd |= a.ek[kv0 + (int64_t)i * a.kv_heads] == kOdd;
+    if (i >= first)
+      for (int h = h0; h < h0 + a.each; ++h) {
+        const int64_t at = (int64_t)(t.tile0 + i) * a.heads + h;
+        odd |= a.eq[at] == kOdd || a.eg[at] == kOdd;
+      }
+  }
+  least = wave_min(least);
+  if (lane == 0) least4[w] = least;
+  if (__syncthreads_or(odd)) return false;
+  least = min(min(least4[0], least4[1]), min(least4[2], least4[3]));
+
+  const bool live = k0 < t.len;
+  const int64_t kt = kv0 + (int64_t)min(k0 / kTile, last) * a.kv_heads;
+  Terms k[S::NS], v[S::NS];
+#pragma unroll
+  for (int s = 0; s < S::NS; ++s) {
+    k[s] = frag(a.k + kt * S::kBytes + S::row_frag(w & 1, s), lane);
+    v[s] = frag(a.v + kt * S::kBytes + S::row_frag(w & 1, s), lane);
+  }
+  const int ek = a.ek[kt], ev = a.ev[kt];
+  const float graw = __builtin_amdgcn_ldexpf(1.f, least - ev - 32), gd = __builtin_amdgcn_ldexpf(1.f, least - 32);
+
+  f16 xk[S::NB] = {}, xv[S::NB] = {};
+  const int b0 = t.t0 / 32, per = (t.len + 31) / 32 - b0, n = per * a.each;
+  auto tile_of = [&](int i) {  // the query tile of stage i
+    return (int64_t)(t.tile0 + (b0 + i % per) / 2) * a.heads + h0 + i / per;
+  };
+  auto issue = [&](int i) {
+    const int half = (b0 + i % per) & 1;
+    const int64_t qt = tile_of(i), at = qt * S::kBytes + half * kPart;
+    char *to = lds + (i & 1) * kStage;
+    fetch<kPart>(a.q + at, to, w, lane);
+    fetch<kPart>(a.g + at, to + kPart, w, lane);
+    fetch<kPart>(a.qt + at, to + 2 * kPart, w, lane);
+    fetch<kPart>(a.gt + at, to + 3 * kPart, w, lane);
+    if (w == 0)
+      __builtin_amdgcn_global_load_lds((global_void *)(a.rowstat + (qt * kTile + 32 * half) * 2 + lane),
+                                       (lds_void *)(to + 4 * kPart), 4, 0, 0);
+  };
+  issue(0);
+  for (int i = 0; i < n; ++i) {
+    fetched();
+    if (i + 1 < n) issue(i + 1);
+    const int q0 = 32 * (b0 + i % per);
+    if (!live || q0 + 31 < k0) continue;
+    const char *qf = lds + (i & 1) * kStage, *gf = qf + kPart, *qtf = gf + kPart, *gtf = qtf + kPart;
+    const float *rs = reinterpret_cast<const float *>(gtf + kPart);
+    f16 s = {}, r = {};
+#pragma unroll
+    for (int st = 0; st < S::NS; ++st) {
+      mma(s, frag(qf + S::row_frag(0, st), lane), k[st]);
+      mma(r, frag(gf + S::row_frag(0, st), lane), v[st]);
+    }
+    float m[16], d[16];
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) {
+      const f4 y = *reinterpret_cast<const f4 *>(rs + 2 * out_row(e, hi));
+      m[e] = y[0], d[e] = y[1] * gd, m[e + 1] = y[2], d[e + 1] = y[3] * gd;
+    }
+    const int64_t qt = tile_of(i);
+    const int eq = a.eq[qt], eg = a.eg[qt];
+    f16 p, ds;
+    dscores(s, r, __builtin_amdgcn_ldexpf(a.alpha, -(eq + ek)), graw, m, d, p, ds);
+    if (q0 < k0 + 31) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (q0 + out_row(e, hi) < k0 + c) p[e] = 0.f, ds[e] = 0.f;
+    }
+    float y[16], z[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) y[e] = p[e], z[e] = ds[e];
+    const Terms pb[2] = {split8(y), split8(y + 8)}, sb[2] = {split8(z), split8(z + 8)};
+    const float bv = __builtin_amdgcn_ldexpf(1.f, -15 - eg), bk = __builtin_amdgcn_ldexpf(a.scale, 17 - eg - least - eq);
+#pragma unroll
+    for (int nb = 0; nb < S::NB; ++nb) {
+      f16 u = {}, x = {};
+      mma(u, frag(gtf + S::col_frag(0, 0, nb), lane), pb[0]);
+      mma(x, frag(qtf + S::col_frag(0, 0, nb), lane), sb[0]);
+      mma(u, frag(gtf + S::col_frag(0, 1, nb), lane), pb[1]);
+      mma(x, frag(qtf + S::col_frag(0, 1, nb), lane), sb[1]);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        xv[nb][e] = fmaf(u[e], bv, xv[nb][e]);
+        xk[nb][e] = fmaf(x[e], bk, xk[nb][e]);
+      }
+    }
+  }
+  const int row = k0 + c;
+  if (row >= t.len) return true;
+  // one head of several: its own part, [heads, total, dh]; else the result
+  const bool part = a.each < a.heads / a.kv_heads;
+  const int64_t at = part ? ((int64_t)h0 * a.total + t.row0 + row) * a.dh : 0;
+  const int64_t ck = part ? at : (int64_t)(t.row0 + row) * a.ld_k + (int64_t)g * a.dh;
+  const int64_t cv = part ? at : (int64_t)(t.row0 + row) * a.ld_v + (int64_t)g * a.dh;
+  if (a.dk != nullptr) put_rows<DP>(a.dk + ck, xk, a.dh, hi, a.accumulate);
+  if (a.dv != nullptr) put_rows<DP>(a.dv + cv, xv, a.dh, hi, a.accumulate);
+  return true;
+}
+
+}  // namespace tiles
