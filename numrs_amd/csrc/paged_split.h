@@ -64,10 +64,6 @@ constexpr float kNever = -1e30f;  // a softmax reference before any score
 template <int DP>
 constexpr int kPart = 32 + 16 * DP;
 
-__device__ __forceinline__ float load_dev(const float *p) {
-  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
 // The four bytes of w as fp16 code - 128: 1024 + byte is 0x6400 | byte, then less 1152.
 __device__ __forceinline__ void halves(unsigned w, unsigned &lo, unsigned &hi) {
   const h2 off = {(_Float16)1152.f, (_Float16)1152.f};
@@ -330,52 +326,83 @@ __device__ __forceinline__ int64_t units_of(const SplitArgs &a, int i) {
   return len > kUnit ? (len + kUnit - 1) / kUnit : 1;  // a sequence without tokens has a row to write too
 }
 
-// References and sums of up to kJoin parts, 16 heads, and the sum of their outputs.  part(j): where
-// the j-th is.  Thread (c, x) of 256 has head c and columns x, x + 16, ...
+// A thread of a join has head c = tid / 16 and, of each 64 columns, 4 x .. + 3 with x = tid % 16.
+template <int DP>
+struct Row {
+  static constexpr int NU = (DP + 63) / 64;
+  float m, l;  // l < 0: no token
+  f4 o[NU];
+  __device__ __forceinline__ static bool in(int u) { return DP % 64 == 0 || 64 * u + 4 * (threadIdx.x & 15) < DP; }
+};
+
+// Adds up to kJoin parts in order; part(j) is the j-th's place.  All loads go out before any is used:
+// they come from memory, whichever cache another workgroup's XCD has.
 template <int DP, class At>
-__device__ __forceinline__ void join(int count, At part, float &m, float &l, float (&o)[DP / 16]) {
+__device__ __forceinline__ Row<DP> join(__amdgpu_buffer_rsrc_t parts, int count, bool live, At part) {
+  using R = Row<DP>;
   const int c = threadIdx.x >> 4, x = threadIdx.x & 15;
-  m = kNever, l = -1.f;
-#pragma unroll
-  for (int j = 0; j < DP / 16; ++j) o[j] = 0.f;
   float ms[kJoin], ls[kJoin];
+  f4 v[kJoin][R::NU];
 #pragma unroll
   for (int i = 0; i < kJoin; ++i) {
-    ms[i] = i < count ? load_dev(part(i) + c) : kNever;
-    ls[i] = i < count ? load_dev(part(i) + 16 + c) : -1.f;
+    ms[i] = kNever, ls[i] = -1.f;
+    if (i < count && live) {
+      const int at = (int)part(i) * kPart<DP> * 4;
+      ms[i] = numrs_hip::ld_dev1(parts, at + 4 * c), ls[i] = numrs_hip::ld_dev1(parts, at + 64 + 4 * c);
+#pragma unroll
+      for (int u = 0; u < R::NU; ++u)
+        if (R::in(u)) v[i][u] = numrs_hip::ld_dev4(parts, at + 128 + (c * DP + 64 * u + 4 * x) * 4);
+    }
   }
+  R r;
+  r.m = kNever, r.l = -1.f;
 #pragma unroll
-  for (int i = 0; i < kJoin; ++i) m = fmaxf(m, ms[i]);
-  for (int i = 0; i < count; ++i) {
-    float lm = ms[0], ll = ls[0];
+  for (int u = 0; u < R::NU; ++u) r.o[u] = f4{};
 #pragma unroll
-    for (int k = 1; k < kJoin; ++k)
-      if (k == i) lm = ms[k], ll = ls[k];
-    if (ll < 0.f) continue;  // no token
-    const float w = __builtin_amdgcn_exp2f(lm - m);
-    l = fmaf(ll, w, fmaxf(l, 0.f));
-    const float *p = part(i) + 32 + c * DP + x;
+  for (int i = 0; i < kJoin; ++i) r.m = fmaxf(r.m, ms[i]);
 #pragma unroll
-    for (int j = 0; j < DP / 16; ++j) o[j] = fmaf(load_dev(p + 16 * j), w, o[j]);
+  for (int i = 0; i < kJoin; ++i) {
+    if (ls[i] < 0.f) continue;
+    const float w = __builtin_amdgcn_exp2f(ms[i] - r.m);
+    r.l = fmaf(ls[i], w, fmaxf(r.l, 0.f));
+#pragma unroll
+    for (int u = 0; u < R::NU; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r.o[u][j] = fmaf(v[i][u][j], w, r.o[u][j]);
   }
+  return r;
 }
 
-// What a thread of `join` has of head c, as the result or as a part for a later join.
+// The result, or a part for a later join.
 template <int DP>
-__device__ __forceinline__ void put_row(const SplitArgs &a, int i, int head, bool live, float l, const float (&o)[DP / 16]) {
+__device__ __forceinline__ void put_row(const SplitArgs &a, int i, int head, bool live, const Row<DP> &r) {
   const int x = threadIdx.x & 15;
   if (!live) return;
   float *p = a.out + i * a.ld_out + (int64_t)head * a.c.dh;
 #pragma unroll
-  for (int j = 0; j < DP / 16; ++j)
-    if (x + 16 * j < a.c.dh) p[x + 16 * j] = l < 0.f ? 0.f : o[j] / l;
+  for (int u = 0; u < Row<DP>::NU; ++u) {
+    const int d = 64 * u + 4 * x;
+    if (d >= a.c.dh) continue;
+    f4 y;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = r.l < 0.f ? 0.f : r.o[u][j] / r.l;
+    *reinterpret_cast<f4u *>(p + d) = y;
+  }
 }
 template <int DP>
-__device__ __forceinline__ void put_part(float *p, float m, float l, const float (&o)[DP / 16]) {
-  const int c = threadIdx.x >> 4, x = threadIdx.x & 15;
-  if (x == 0) numrs_hip::st_dev(p + c, m), numrs_hip::st_dev(p + 16 + c, l);
+__device__ __forceinline__ void put_part(__amdgpu_buffer_rsrc_t parts, int64_t place, bool live, const Row<DP> &r) {
+  const int c = threadIdx.x >> 4, x = threadIdx.x & 15, at = (int)place * kPart<DP> * 4;
+  if (!live) return;
+  if (x == 0) {
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, r.m), parts, at + 4 * c, 0, numrs_hip::kScDevice);
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, r.l), parts, at + 64 + 4 * c, 0,
+                                          numrs_hip::kScDevice);
+  }
 #pragma unroll
-  for (int j = 0; j < DP / 16; ++j) numrs_hip::st_dev(p + 32 + c * DP + x + 16 * j, o[j]);
+  for (int u = 0; u < Row<DP>::NU; ++u)
+    if (Row<DP>::in(u))
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, r.o[u]), parts,
+                                             at + 128 + (c * DP + 64 * u + 4 * x) * 4, 0, numrs_hip::kScDevice);
 }
 
 // Adds one to a counter once this workgroup's stores are out; whether it was the last of `count`,
@@ -396,12 +423,14 @@ template <bool INT8, int DP>
 __global__ void __launch_bounds__(256, 2) split_rows(SplitArgs a) {
   using S = State<INT8, DP>;
   constexpr int kStep = 16 * S::NB;
-  __shared__ float sm[4][16], sl[4][16], so[4][16][S::NU * 64 + 1];
+  __shared__ float sm[4][16], sl[4][16], so[4][16][S::NU * 64 + 4];
   __shared__ int64_t pre[257], total4[4];
   __shared__ int flag;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hc = blockIdx.x % (a.c.kv_heads * a.blocks), kv = hc / a.blocks, cb = hc % a.blocks;
   const int group = a.heads / a.c.kv_heads;
+  const __amdgpu_buffer_rsrc_t parts = numrs_hip::dev_rsrc(
+      a.parts, (int64_t)2 * a.c.kv_heads * a.blocks * a.shares * kPart<DP> * 4);
 
   auto block_sum = [&](int64_t v) {
 #pragma unroll
@@ -474,52 +503,60 @@ __global__ void __launch_bounds__(256, 2) split_rows(SplitArgs a) {
           for (int r = 0; r < 4; ++r) so[w][lane & 15][64 * u + 16 * (lane >> 4) + 4 * r + e] = st.o[u][e][r];
       __syncthreads();
       const int c = tid >> 4, x = tid & 15;
-      float m = fmaxf(fmaxf(sm[0][c], sm[1][c]), fmaxf(sm[2][c], sm[3][c])), lsum = -1.f, o[DP / 16] = {};
+      Row<DP> r;
+      r.m = fmaxf(fmaxf(sm[0][c], sm[1][c]), fmaxf(sm[2][c], sm[3][c])), r.l = -1.f;
+#pragma unroll
+      for (int u = 0; u < S::NU; ++u) r.o[u] = f4{};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if (sl[k][c] < 0.f) continue;
-        const float f = __builtin_amdgcn_exp2f(sm[k][c] - m);
-        lsum = fmaf(sl[k][c], f, fmaxf(lsum, 0.f));
+        const float f = __builtin_amdgcn_exp2f(sm[k][c] - r.m);
+        r.l = fmaf(sl[k][c], f, fmaxf(r.l, 0.f));
 #pragma unroll
-        for (int y = 0; y < DP / 16; ++y) o[y] = fmaf(so[k][c][x + 16 * y], f, o[y]);
+        for (int u = 0; u < S::NU; ++u) {
+          const f4 y = *reinterpret_cast<const f4 *>(&so[k][c][64 * u + 4 * x]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) r.o[u][e] = fmaf(y[e], f, r.o[u][e]);
+        }
       }
       const int out_head = kv * group + cb * 16 + c;
       const bool live = cb * 16 + c < group;
       if (ua == u0 && ub == u1) {
-        put_row<DP>(a, i, out_head, live, lsum, o);
+        put_row<DP>(a, i, out_head, live, r);
         continue;
       }
-      // Parts: a workgroup has at most one that begins its sequence (place 1) and one that does not.
+      // Places of parts: a workgroup has at most one that begins its sequence (place 1) and one that
+      // does not.
       const int pf = owner(u0, units, shares), pl = owner(u1 - 1, units, shares);
       auto wg = [&](int q) { return hc + (int64_t)q * stride; };
-      auto at = [&](int q) { return a.parts + (2 * wg(q) + (q == pf)) * kPart<DP>; };
-      put_part<DP>(at(p), m, lsum, o);
+      auto at = [&](int q) { return 2 * wg(q) + (q == pf); };
+      put_part<DP>(parts, at(p), live, r);
       const int lead = pf + (p - pf) / kJoin * kJoin, members = min(kJoin, pl - lead + 1);
-      const int64_t wgs = stride * a.shares;
-      if (!arrive(a.arrivals + 2 * wg(lead) + (lead == pf), members, &flag)) continue;
-      join<DP>(members, [&](int q) { return at(lead + q); }, m, lsum, o);
+      if (!arrive(a.arrivals + at(lead), members, &flag)) continue;
+      r = join<DP>(parts, members, live, [&](int q) { return at(lead + q); });
       const int groups = (pl - pf) / kJoin + 1;
       if (groups > 1) {
         // in place of the leader's part, which no one reads any more
         __syncthreads();
-        put_part<DP>(at(lead), m, lsum, o);
-        if (!arrive(a.arrivals + 2 * wgs + wg(pf), groups, &flag)) continue;
-        float gm = kNever, gl = -1.f, go[DP / 16] = {};
+        put_part<DP>(parts, at(lead), live, r);
+        if (!arrive(a.arrivals + 2 * stride * a.shares + wg(pf), groups, &flag)) continue;
+        r.m = kNever, r.l = -1.f;
+#pragma unroll
+        for (int u = 0; u < S::NU; ++u) r.o[u] = f4{};
         for (int q = 0; q < groups; q += kJoin) {
-          float jm, jl, jo[DP / 16];
-          join<DP>(min(kJoin, groups - q), [&](int y) { return at(pf + (q + y) * kJoin); }, jm, jl, jo);
-          if (jl < 0.f) continue;
-          const float now = fmaxf(gm, jm), fg = __builtin_amdgcn_exp2f(gm - now), fj = __builtin_amdgcn_exp2f(jm - now);
-          gl = fmaf(fmaxf(gl, 0.f), fg, jl * fj);
+          const Row<DP> y = join<DP>(parts, min(kJoin, groups - q), live,
+                                     [&](int z) { return at(pf + (q + z) * kJoin); });
+          if (y.l < 0.f) continue;
+          const float now = fmaxf(r.m, y.m), f0 = __builtin_amdgcn_exp2f(r.m - now), f1 = __builtin_amdgcn_exp2f(y.m - now);
+          r.l = fmaf(fmaxf(r.l, 0.f), f0, y.l * f1);
 #pragma unroll
-          for (int y = 0; y < DP / 16; ++y) go[y] = fmaf(go[y], fg, jo[y] * fj);
-          gm = now;
+          for (int u = 0; u < S::NU; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r.o[u][e] = fmaf(r.o[u][e], f0, y.o[u][e] * f1);
+          r.m = now;
         }
-        lsum = gl;
-#pragma unroll
-        for (int y = 0; y < DP / 16; ++y) o[y] = go[y];
       }
-      put_row<DP>(a, i, out_head, live, lsum, o);
+      put_row<DP>(a, i, out_head, live, r);
     }
     __syncthreads();
     base = next;
