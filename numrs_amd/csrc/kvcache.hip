@@ -199,8 +199,10 @@ int numrs_hip_attention_paged(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cach
   DeviceScope dev(ctx);
   const int hk = (int)cache->kv_heads, dh = (int)cache->head_dim, group = (int)heads / hk;
   const int blocks = (group + 15) / 16;
-  // Two workgroups a CU, which the registers allow, each with an even share of the tokens.
-  const int shares = std::max(1, (2 * ctx->num_cus + hk * blocks - 1) / (hk * blocks));
+  // A workgroup of eight waves a CU, which the registers allow, each with an even share of the tokens;
+  // a kv head has as many at most as two levels of joins add.
+  const int shares = std::min(std::max(1, (ctx->num_cus + hk * blocks - 1) / (hk * blocks)),
+                              paged::kJoin * paged::kJoin);
   const int64_t wgs = (int64_t)shares * hk * blocks;
   TempBlock parts(ctx);
   const int dp = (dh + 31) / 32 * 32;
@@ -213,9 +215,9 @@ int numrs_hip_attention_paged(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cach
   auto launch = [&](auto padded) {
     constexpr int DP = decltype(padded)::value;
     if (cache->format == NUMRS_HIP_KV_F32)
-      paged::split_rows<false, DP><<<(unsigned)wgs, 256, 0, ctx->stream>>>(a);
+      paged::split_rows<false, DP><<<(unsigned)wgs, 64 * paged::kWaves, 0, ctx->stream>>>(a);
     else
-      paged::split_rows<true, DP><<<(unsigned)wgs, 256, 0, ctx->stream>>>(a);
+      paged::split_rows<true, DP><<<(unsigned)wgs, 64 * paged::kWaves, 0, ctx->stream>>>(a);
   };
   switch (dp) {
     case 32: launch(std::integral_constant<int, 32>{}); break;

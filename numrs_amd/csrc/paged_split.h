@@ -57,7 +57,8 @@ struct SplitArgs {
 };
 
 constexpr int kUnit = 64;       // tokens
-constexpr int kJoin = 16;       // parts that one workgroup adds
+constexpr int kJoin = 16;       // parts that one workgroup adds: two levels for up to kJoin^2 shares
+constexpr int kWaves = 8;       // of a workgroup
 constexpr float kNever = -1e30f;  // a softmax reference before any score
 
 // Floats of a part: references and sums of 16 heads, then their outputs.
@@ -74,99 +75,169 @@ __device__ __forceinline__ void halves(unsigned w, unsigned &lo, unsigned &hi) {
 __device__ __forceinline__ float max4(f4 x) { return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])); }
 
 // A wave's running softmax of 16 heads over some tokens: lane (g, c) has head c; O of columns 64 u +
-// 16 g + 4 r + e in o[u][e][r].
+// 16 g + 4 r + e in o[u][e][r].  The heads' queries lie in LDS, a fragment of NT lanes' 16 bytes each
+// (fp32: four columns of each 16; 8 bits: eight columns of each 32, two terms).
 template <bool INT8, int DP>
 struct State {
   static constexpr int NU = (DP + 63) / 64, NT = INT8 ? DP / 32 : DP / 16;
-  static constexpr int NB = INT8 ? 4 : 2;  // blocks of 16 tokens a step
-  float m, l;
+  static constexpr int NB = INT8 ? 4 : 1;  // blocks of 16 tokens a step
+  static constexpr int kQueries = DP * 64;  // bytes of the queries' fragments
+  float m, l, fq;  // fq: log2(e) / sqrt(dh), less the queries' factor
   f4 o[NU][4];
   bool seen;
-  // the head's queries: fp32 a lane's four columns of each 16; else two terms and what their factor
-  // leaves of alpha
-  f4 q[INT8 ? 1 : NT];
-  Terms qt[INT8 ? NT : 1];
-  float fq;
+  // A step's tokens as loaded.
+  struct Load {
+    f4 k[NB][INT8 ? 1 : NT], v[NB][INT8 ? 1 : 4][INT8 ? 1 : NU], ks[INT8 ? NB : 1], vs[INT8 ? NB : 1];
+    u2 kc[NB][INT8 ? NT : 1];
+    u4 vc[NB][INT8 ? NU : 1];
+  };
 
-  __device__ __forceinline__ void begin(const SplitArgs &a, int i, int head, bool live) {
-    const int lane = threadIdx.x & 63, g = lane >> 4;
-    const float *p = a.q + i * a.ld_q + (int64_t)head * a.c.dh;
+  __device__ __forceinline__ void clear() {
     m = kNever, l = 0.f, seen = false;
 #pragma unroll
     for (int u = 0; u < NU; ++u)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[u][e] = f4{};
+  }
+
+  // The queries of head `head` (zeros where it is not live), from memory: fp32, wave w's fragment; 8
+  // bits, all of them, for their largest magnitude ...
+  static constexpr int kAsked = INT8 ? 2 * NT : (NT + kWaves - 1) / kWaves;
+  struct Queries {
+    f4 x[kAsked];
+  };
+  static __device__ __forceinline__ Queries ask(const SplitArgs &a, int i, int head, bool live, int w) {
+    const int g = (threadIdx.x & 63) >> 4;
+    const float *p = a.q + i * a.ld_q + (int64_t)head * a.c.dh;
+    Queries q;
+#pragma unroll
+    for (int t = 0; t < kAsked; ++t) {
+      const int d = INT8 ? 32 * (t >> 1) + 8 * g + 4 * (t & 1) : 16 * (w + t * kWaves) + 4 * g;
+      q.x[t] = live && d < a.c.dh ? f4(*reinterpret_cast<const f4u *>(p + d)) : f4{};
+    }
+    return q;
+  }
+  // ... into LDS: wave w has fragments w, w + kWaves, ...
+  __device__ __forceinline__ void keep(const SplitArgs &a, const Queries &q, char *lds, int w) {
+    const int lane = threadIdx.x & 63;
     if constexpr (!INT8) {
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int d = 16 * t + 4 * g;
-        q[t] = live && d < a.c.dh ? f4(*reinterpret_cast<const f4u *>(p + d)) : f4{};
-      }
       fq = a.alpha;
+#pragma unroll
+      for (int t = 0; t < kAsked; ++t)
+        if (w + t * kWaves < NT) *reinterpret_cast<f4 *>(lds + (w + t * kWaves) * 1024 + lane * 16) = q.x[t];
     } else {
-      float x[NT][8], big = 0.f;
+      float big = 0.f;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int d = 32 * t + 8 * g;
-        const bool in = live && d < a.c.dh;
-        const f4 lo = in ? f4(*reinterpret_cast<const f4u *>(p + d)) : f4{};
-        const f4 hi = in ? f4(*reinterpret_cast<const f4u *>(p + d + 4)) : f4{};
+      for (int t = 0; t < 2 * NT; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[t][j] = lo[j], x[t][4 + j] = hi[j];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(x[t][j]));
-      }
+        for (int j = 0; j < 4; ++j) big = fmaxf(big, fabsf(q.x[t][j]));
       big = rows4(big, [](float y, float z) { return fmaxf(y, z); });
       const int e = big > 0.f && big < INFINITY ? min(12 - __builtin_amdgcn_frexp_expf(big), 120) : 0;
+      fq = __builtin_amdgcn_ldexpf(a.alpha, -e);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
+        if (t % kWaves != w) continue;
+        float x[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[t][j] = __builtin_amdgcn_ldexpf(x[t][j], e);
-        qt[t] = tiles::split8(x[t]);
+        for (int j = 0; j < 8; ++j) x[j] = __builtin_amdgcn_ldexpf(q.x[2 * t + (j >> 2)][j & 3], e);
+        const Terms y = tiles::split8(x);
+        *reinterpret_cast<h8 *>(lds + t * 2048 + lane * 16) = y.h;
+        *reinterpret_cast<h8 *>(lds + t * 2048 + 1024 + lane * 16) = y.m;
       }
-      fq = __builtin_amdgcn_ldexpf(a.alpha, -e);
     }
   }
 
-  // Tokens pos .. + 16 NB - 1 of kv head `kv`, those before `end`; pages: of each block, -1 for one
-  // that the cache does not have.
-  __device__ __forceinline__ void step(const SplitArgs &a, int kv, int64_t pos, int64_t end, const int (&pages)[NB]) {
-    const Cache &c = a.c;
+  // Asks for the keys, or the values, of the tokens pos .. + 16 NB - 1 of kv head `kv` on `pages`, -1
+  // for one that the cache does not have (page 0 is read in its place, and masked).  Uniform addresses
+  // and 32-bit offsets of the lane.  A lane past the head's last column reads the last ones again: its
+  // products are with zeros (fp32 keys are zeroed, since theirs might be with infinity), its results
+  // are not written.
+  static __device__ __forceinline__ int64_t row_of(const Cache &c, int kv, int64_t pos, int page) {
+    return paging::page_base(max(page, 0), c.kv_heads, kv, c.shift, 1) + ((int)pos & ((1 << c.shift) - 1));
+  }
+  static __device__ __forceinline__ void load_keys(const Cache &c, int kv, int64_t pos, const int (&pages)[NB], Load &x) {
     const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
-    const int slot = (int)(pos & ((1 << c.shift) - 1));
-    f4 s[NB];
-    bool full = true;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const int64_t row = row_of(c, kv, pos + 16 * b, pages[b]);
+      if constexpr (!INT8) {
+        const char *p = reinterpret_cast<const char *>(static_cast<const float *>(c.k) + row * c.dh);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+          x.k[b][t] = *reinterpret_cast<const f4 *>(p + (unsigned)(4 * (col * c.dh + min(16 * t + 4 * g, c.dh - 4))));
+      } else {
+        const char *p = static_cast<const char *>(c.k) + row * c.dh;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+          x.kc[b][t] = *reinterpret_cast<const u2 *>(p + (unsigned)(col * c.dh + min(32 * t + 8 * g, c.dh - 8)));
+        x.ks[b] = *reinterpret_cast<const f4 *>(reinterpret_cast<const char *>(c.ks + row) + (unsigned)(16 * g));
+      }
+    }
+  }
+  static __device__ __forceinline__ void load_values(const Cache &c, int kv, int64_t pos, const int (&pages)[NB], Load &x) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const int64_t row = row_of(c, kv, pos + 16 * b, pages[b]);
+      if constexpr (!INT8) {
+        const char *p = reinterpret_cast<const char *>(static_cast<const float *>(c.v) + row * c.dh);
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            x.v[b][r][u] = *reinterpret_cast<const f4 *>(
+                p + r * c.dh * 4 + (unsigned)(4 * (4 * g * c.dh + min(64 * u + 4 * col, c.dh - 4))));
+      } else {
+        x.vs[b] = *reinterpret_cast<const f4 *>(reinterpret_cast<const char *>(c.vs + row) + (unsigned)(16 * g));
+        // the four slots 4 g .. + 3, columns 4 col .. + 3
+        const char *p = static_cast<const char *>(c.v) + row * c.dh;
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+          x.vc[b][u] = *reinterpret_cast<const u4 *>(p + (unsigned)(4 * (g * c.dh + min(64 * u + 4 * col, c.dh - 4))));
+      }
+    }
+  }
+
+  // The loaded keys' scores, in base 2.
+  __device__ __forceinline__ void scores(int dh, const Load &x, const char *queries, f4 (&s)[NB]) {
+    const int lane = threadIdx.x & 63, g = lane >> 4;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) s[b] = f4{};
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      if constexpr (!INT8) {
+        const f4 q = *reinterpret_cast<const f4 *>(queries + t * 1024 + lane * 16);
+        const bool in = 16 * t + 4 * g < dh;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            s[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(in ? x.k[b][t][e] : 0.f, q[e], s[b], 0, 0, 0);
+      } else {
+        const h8 qh = *reinterpret_cast<const h8 *>(queries + t * 2048 + lane * 16);
+        const h8 qm = *reinterpret_cast<const h8 *>(queries + t * 2048 + 1024 + lane * 16);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          u4 w;
+          unsigned lo, hi;
+          halves(x.kc[b][t][0], lo, hi), w[0] = lo, w[1] = hi;
+          halves(x.kc[b][t][1], lo, hi), w[2] = lo, w[3] = hi;
+          const h8 kh = __builtin_bit_cast(h8, w);
+          s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qm, s[b], 0, 0, 0);
+          s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh, s[b], 0, 0, 0);
+        }
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[b][r] *= INT8 ? x.ks[INT8 ? b : 0][r] * fq : fq;
+  }
+
+  // Adds the loaded values times the probabilities; `full`: all of them are tokens.
+  __device__ __forceinline__ void outputs(int64_t pos, int64_t end, const int (&pages)[NB], bool full, f4 (&s)[NB], Load &x) {
+    const int g = (threadIdx.x & 63) >> 4;
     if constexpr (!INT8) {
-      f4 k[NB][NT], v[NB][4][NU];
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const int at = (slot + 16 * b) & ((1 << c.shift) - 1);
-        const int64_t base = paging::page_base(max(pages[b], 0), c.kv_heads, kv, c.shift, c.dh) + (int64_t)at * c.dh;
-        const float *p = static_cast<const float *>(c.k) + base + (int64_t)col * c.dh + 4 * g;
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-          k[b][t] = 16 * t + 4 * g < c.dh ? *reinterpret_cast<const f4 *>(p + 16 * t) : f4{};
-      }
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const int at = (slot + 16 * b) & ((1 << c.shift) - 1);
-        const int64_t base = paging::page_base(max(pages[b], 0), c.kv_heads, kv, c.shift, c.dh) + (int64_t)at * c.dh;
-        const float *p = static_cast<const float *>(c.v) + base + (int64_t)(4 * g) * c.dh + 4 * col;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int u = 0; u < NU; ++u)
-            v[b][r][u] = 64 * u + 4 * col < c.dh ? *reinterpret_cast<const f4 *>(p + r * c.dh + 64 * u) : f4{};
-      }
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        s[b] = f4{};
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[b][t][e], q[t][e], s[b], 0, 0, 0);
-      }
-      probabilities(pos, end, pages, s, nullptr, full);
       if (!full) {  // what lies in slots of no token must not reach the sums
 #pragma unroll
         for (int b = 0; b < NB; ++b)
@@ -174,7 +245,7 @@ struct State {
           for (int r = 0; r < 4; ++r)
             if (pages[b] < 0 || pos + 16 * b + 4 * g + r >= end) {
 #pragma unroll
-              for (int u = 0; u < NU; ++u) v[b][r][u] = f4{};
+              for (int u = 0; u < NU; ++u) x.v[b][r][u] = f4{};
             }
       }
 #pragma unroll
@@ -185,69 +256,30 @@ struct State {
 #pragma unroll
           for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) t = __builtin_amdgcn_mfma_f32_16x16x4f32(v[b][r][u][e], s[b][r], t, 0, 0, 0);
+            for (int r = 0; r < 4; ++r) t = __builtin_amdgcn_mfma_f32_16x16x4f32(x.v[b][r][u][e], s[b][r], t, 0, 0, 0);
           o[u][e] += t;
         }
     } else {
-      u2 k[NB][NT];
-      u4 v[NB][NU];
-      f4 ks[NB], vs[NB];
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const int at = (slot + 16 * b) & ((1 << c.shift) - 1);
-        const int64_t head = paging::page_base(max(pages[b], 0), c.kv_heads, kv, c.shift, 1) + at;
-        const uint8_t *p = static_cast<const uint8_t *>(c.k) + (head + col) * c.dh + 8 * g;
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-          k[b][t] = 32 * t + 8 * g < c.dh ? *reinterpret_cast<const u2 *>(p + 32 * t) : u2{};
-        ks[b] = *reinterpret_cast<const f4 *>(c.ks + head + 4 * g);
-        vs[b] = *reinterpret_cast<const f4 *>(c.vs + head + 4 * g);
-      }
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const int at = (slot + 16 * b) & ((1 << c.shift) - 1);
-        const int64_t head = paging::page_base(max(pages[b], 0), c.kv_heads, kv, c.shift, 1) + at;
-        // slot group at / 4 + g, columns 4 col .. + 3
-        const uint8_t *p = static_cast<const uint8_t *>(c.v) + (head + 4 * g) * c.dh + 16 * col;
-#pragma unroll
-        for (int u = 0; u < NU; ++u)
-          v[b][u] = 64 * u + 4 * col < c.dh ? *reinterpret_cast<const u4 *>(p + 256 * u) : u4{};
-      }
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        s[b] = f4{};
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          u4 w;
-          unsigned x, y;
-          halves(k[b][t][0], x, y), w[0] = x, w[1] = y;
-          halves(k[b][t][1], x, y), w[2] = x, w[3] = y;
-          const h8 kh = __builtin_bit_cast(h8, w);
-          s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qt[t].m, s[b], 0, 0, 0);
-          s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qt[t].h, s[b], 0, 0, 0);
-        }
-      }
-      probabilities(pos, end, pages, s, ks, full);
       if (!full) {
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (pages[b] < 0 || pos + 16 * b + 4 * g + r >= end) vs[b][r] = 0.f;
+            if (pages[b] < 0 || pos + 16 * b + 4 * g + r >= end) x.vs[b][r] = 0.f;
       }
-      float big = max4(vs[0]);
+      float big = max4(x.vs[0]);
 #pragma unroll
-      for (int b = 1; b < NB; ++b) big = fmaxf(big, max4(vs[b]));
-      big = rows4(big, [](float x, float y) { return fmaxf(x, y); });
+      for (int b = 1; b < NB; ++b) big = fmaxf(big, max4(x.vs[b]));
+      big = rows4(big, [](float i, float j) { return fmaxf(i, j); });
       const int ev = big > 0.f ? max(__builtin_amdgcn_frexp_expf(big), -110) : 0;
       const float up = __builtin_amdgcn_ldexpf(1.f, 7 - ev), back = __builtin_amdgcn_ldexpf(1.f, ev - 7);
       Terms w[NB / 2];
 #pragma unroll
       for (int b = 0; b < NB; b += 2) {
-        float x[8];
+        float y[8];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = s[b][r] * (vs[b][r] * up), x[4 + r] = s[b + 1][r] * (vs[b + 1][r] * up);
-        w[b / 2] = tiles::split8(x);
+        for (int r = 0; r < 4; ++r) y[r] = s[b][r] * (x.vs[b][r] * up), y[4 + r] = s[b + 1][r] * (x.vs[b + 1][r] * up);
+        w[b / 2] = tiles::split8(y);
       }
 #pragma unroll
       for (int u = 0; u < NU; ++u)
@@ -256,11 +288,11 @@ struct State {
           f4 t{};
 #pragma unroll
           for (int b = 0; b < NB; b += 2) {
-            u4 y;
+            u4 z;
             unsigned lo, hi;
-            halves(v[b][u][e], lo, hi), y[0] = lo, y[1] = hi;
-            halves(v[b + 1][u][e], lo, hi), y[2] = lo, y[3] = hi;
-            const h8 vh = __builtin_bit_cast(h8, y);
+            halves(x.vc[b][u][e], lo, hi), z[0] = lo, z[1] = hi;
+            halves(x.vc[b + 1][u][e], lo, hi), z[2] = lo, z[3] = hi;
+            const h8 vh = __builtin_bit_cast(h8, z);
             t = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, w[b / 2].m, t, 0, 0, 0);
             t = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, w[b / 2].h, t, 0, 0, 0);
           }
@@ -272,7 +304,7 @@ struct State {
 
   // Scores to probabilities in place; the reference moves where one passes it by 2^8.
   __device__ __forceinline__ void probabilities(int64_t pos, int64_t end, const int (&pages)[NB], f4 (&s)[NB],
-                                                const f4 *ks, bool &full) {
+                                                bool &full) {
     const int g = (threadIdx.x & 63) >> 4;
     full = pos + 16 * NB <= end;
     bool any = false;
@@ -280,8 +312,6 @@ struct State {
     for (int b = 0; b < NB; ++b) {
       full &= pages[b] >= 0;
       any |= pages[b] >= 0;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) s[b][r] *= ks != nullptr ? ks[b][r] * fq : fq;
     }
     seen |= any;
     if (!full) {
@@ -295,7 +325,7 @@ struct State {
 #pragma unroll
     for (int b = 1; b < NB; ++b) most = fmaxf(most, max4(s[b]));
     if (__any(most > m + 8.f)) {
-      const float now = fmaxf(m, rows4(most, [](float x, float y) { return fmaxf(x, y); }));
+      const float now = fmaxf(m, rows4(most, [](float i, float j) { return fmaxf(i, j); }));
       const float r = __builtin_amdgcn_exp2f(m - now);
       m = now;
       l *= r;
@@ -315,6 +345,12 @@ struct State {
   }
 };
 
+// A value that is the same in every lane, as a scalar.
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 |
+                   (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
+
 // The workgroup of a kv head's block of query heads that has unit x of `units`, of `shares`.
 __device__ __forceinline__ int owner(int64_t x, int64_t units, int shares) {
   return (int)(((x + 1) * shares - 1) / units);
@@ -326,83 +362,63 @@ __device__ __forceinline__ int64_t units_of(const SplitArgs &a, int i) {
   return len > kUnit ? (len + kUnit - 1) / kUnit : 1;  // a sequence without tokens has a row to write too
 }
 
-// A thread of a join has head c = tid / 16 and, of each 64 columns, 4 x .. + 3 with x = tid % 16.
-template <int DP>
+// A thread of a join has head c = tid / 32 and columns 4 x .. + 3 with x = tid % 32.
 struct Row {
-  static constexpr int NU = (DP + 63) / 64;
   float m, l;  // l < 0: no token
-  f4 o[NU];
-  __device__ __forceinline__ static bool in(int u) { return DP % 64 == 0 || 64 * u + 4 * (threadIdx.x & 15) < DP; }
+  f4 o;
 };
 
 // Adds up to kJoin parts in order; part(j) is the j-th's place.  All loads go out before any is used:
 // they come from memory, whichever cache another workgroup's XCD has.
 template <int DP, class At>
-__device__ __forceinline__ Row<DP> join(__amdgpu_buffer_rsrc_t parts, int count, bool live, At part) {
-  using R = Row<DP>;
-  const int c = threadIdx.x >> 4, x = threadIdx.x & 15;
+__device__ __forceinline__ Row join(__amdgpu_buffer_rsrc_t parts, int count, bool live, At part) {
+  const int c = threadIdx.x >> 5, x = threadIdx.x & 31;
   float ms[kJoin], ls[kJoin];
-  f4 v[kJoin][R::NU];
+  f4 v[kJoin];
 #pragma unroll
   for (int i = 0; i < kJoin; ++i) {
-    ms[i] = kNever, ls[i] = -1.f;
-    if (i < count && live) {
-      const int at = (int)part(i) * kPart<DP> * 4;
-      ms[i] = numrs_hip::ld_dev1(parts, at + 4 * c), ls[i] = numrs_hip::ld_dev1(parts, at + 64 + 4 * c);
-#pragma unroll
-      for (int u = 0; u < R::NU; ++u)
-        if (R::in(u)) v[i][u] = numrs_hip::ld_dev4(parts, at + 128 + (c * DP + 64 * u + 4 * x) * 4);
-    }
+    const int at = (int)part(min(i, count - 1)) * kPart<DP> * 4;  // past the last: read again, not added
+    ms[i] = numrs_hip::ld_dev1(parts, at + 4 * c), ls[i] = numrs_hip::ld_dev1(parts, at + 64 + 4 * c);
+    v[i] = numrs_hip::ld_dev4(parts, at + 128 + (c * DP + 4 * min(x, DP / 4 - 1)) * 4);
   }
-  R r;
-  r.m = kNever, r.l = -1.f;
+  Row r{kNever, -1.f, {}};
 #pragma unroll
-  for (int u = 0; u < R::NU; ++u) r.o[u] = f4{};
-#pragma unroll
-  for (int i = 0; i < kJoin; ++i) r.m = fmaxf(r.m, ms[i]);
+  for (int i = 0; i < kJoin; ++i) {
+    if (i >= count || !live) ls[i] = -1.f;
+    r.m = fmaxf(r.m, ms[i]);
+  }
 #pragma unroll
   for (int i = 0; i < kJoin; ++i) {
     if (ls[i] < 0.f) continue;
     const float w = __builtin_amdgcn_exp2f(ms[i] - r.m);
     r.l = fmaf(ls[i], w, fmaxf(r.l, 0.f));
 #pragma unroll
-    for (int u = 0; u < R::NU; ++u)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) r.o[u][j] = fmaf(v[i][u][j], w, r.o[u][j]);
+    for (int j = 0; j < 4; ++j) r.o[j] = fmaf(v[i][j], w, r.o[j]);
   }
   return r;
 }
 
 // The result, or a part for a later join.
-template <int DP>
-__device__ __forceinline__ void put_row(const SplitArgs &a, int i, int head, bool live, const Row<DP> &r) {
-  const int x = threadIdx.x & 15;
-  if (!live) return;
-  float *p = a.out + i * a.ld_out + (int64_t)head * a.c.dh;
+__device__ __forceinline__ void put_row(const SplitArgs &a, int i, int head, bool live, const Row &r) {
+  const int d = 4 * (threadIdx.x & 31);
+  if (!live || d >= a.c.dh) return;
+  f4 y;
 #pragma unroll
-  for (int u = 0; u < Row<DP>::NU; ++u) {
-    const int d = 64 * u + 4 * x;
-    if (d >= a.c.dh) continue;
-    f4 y;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = r.l < 0.f ? 0.f : r.o[u][j] / r.l;
-    *reinterpret_cast<f4u *>(p + d) = y;
-  }
+  for (int j = 0; j < 4; ++j) y[j] = r.l < 0.f ? 0.f : r.o[j] / r.l;
+  *reinterpret_cast<f4u *>(a.out + i * a.ld_out + (int64_t)head * a.c.dh + d) = y;
 }
 template <int DP>
-__device__ __forceinline__ void put_part(__amdgpu_buffer_rsrc_t parts, int64_t place, bool live, const Row<DP> &r) {
-  const int c = threadIdx.x >> 4, x = threadIdx.x & 15, at = (int)place * kPart<DP> * 4;
+__device__ __forceinline__ void put_part(__amdgpu_buffer_rsrc_t parts, int64_t place, bool live, const Row &r) {
+  const int c = threadIdx.x >> 5, x = threadIdx.x & 31, at = (int)place * kPart<DP> * 4;
   if (!live) return;
   if (x == 0) {
     __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, r.m), parts, at + 4 * c, 0, numrs_hip::kScDevice);
     __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, r.l), parts, at + 64 + 4 * c, 0,
                                           numrs_hip::kScDevice);
   }
-#pragma unroll
-  for (int u = 0; u < Row<DP>::NU; ++u)
-    if (Row<DP>::in(u))
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, r.o[u]), parts,
-                                             at + 128 + (c * DP + 64 * u + 4 * x) * 4, 0, numrs_hip::kScDevice);
+  if (4 * x < DP)
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, r.o), parts, at + 128 + (c * DP + 4 * x) * 4, 0,
+                                           numrs_hip::kScDevice);
 }
 
 // Adds one to a counter once this workgroup's stores are out; whether it was the last of `count`,
@@ -416,147 +432,160 @@ __device__ __forceinline__ bool arrive(unsigned *counter, int count, int *flag) 
     if (*flag) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
-  return *flag != 0;
+  return __builtin_amdgcn_readfirstlane(*flag) != 0;
 }
 
 template <bool INT8, int DP>
-__global__ void __launch_bounds__(256, 2) split_rows(SplitArgs a) {
+__global__ void __launch_bounds__(64 * kWaves, 2) split_rows(SplitArgs a) {
   using S = State<INT8, DP>;
-  constexpr int kStep = 16 * S::NB;
-  __shared__ float sm[4][16], sl[4][16], so[4][16][S::NU * 64 + 4];
-  __shared__ int64_t pre[257], total4[4];
+  constexpr int kStep = 16 * S::NB, kThreads = 64 * kWaves, kCols = S::NU * 64 + 4;
+  // the queries while tokens are taken in, then the waves' outputs
+  constexpr int kOutputs = kWaves * 16 * kCols * 4;
+  __shared__ __attribute__((aligned(16))) char lds[kOutputs > S::kQueries ? kOutputs : S::kQueries];
+  __shared__ float sm[kWaves][16], sl[kWaves][16];
+  __shared__ int64_t pre[kThreads + 1], sums[kWaves];
   __shared__ int flag;
+  float(*so)[16][kCols] = reinterpret_cast<float(*)[16][kCols]>(lds);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hc = blockIdx.x % (a.c.kv_heads * a.blocks), kv = hc / a.blocks, cb = hc % a.blocks;
   const int group = a.heads / a.c.kv_heads;
   const __amdgpu_buffer_rsrc_t parts = numrs_hip::dev_rsrc(
       a.parts, (int64_t)2 * a.c.kv_heads * a.blocks * a.shares * kPart<DP> * 4);
 
-  auto block_sum = [&](int64_t v) {
+  // units before each of kThreads sequences from i0 on, in pre, with `base` before the first; their end
+  auto scan = [&](int i0, int64_t base) {
+    int64_t v = i0 + tid < a.n ? units_of(a, i0 + tid) : 0;
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t below = __shfl_up(v, d);
+      if (lane >= d) v += below;
+    }
     __syncthreads();
-    if (lane == 0) total4[w] = v;
+    if (lane == 63) sums[w] = v;
     __syncthreads();
-    return total4[0] + total4[1] + total4[2] + total4[3];
+    for (int k = 0; k < w; ++k) v += sums[k];
+    pre[tid + 1] = base + v;
+    if (tid == 0) pre[0] = base;
+    __syncthreads();
+    return uniform(pre[min(kThreads, a.n - i0)]);
   };
   int64_t units = 0;
-  for (int i = tid; i < a.n; i += 256) units += units_of(a, i);
-  units = block_sum(units);
+  for (int i0 = 0; i0 < a.n; i0 += kThreads) units = scan(i0, units);
   const int shares = (int)min((int64_t)a.shares, units), p = blockIdx.x / (a.c.kv_heads * a.blocks);
   if (p >= shares) return;
   const int64_t lo = first_unit(p, units, shares), hi = first_unit(p + 1, units, shares);
-  const int64_t me = (int64_t)blockIdx.x, stride = (int64_t)a.c.kv_heads * a.blocks;  // workgroup p' of this block: hc + p' stride
+  const int64_t stride = (int64_t)a.c.kv_heads * a.blocks;  // workgroup q of this block is hc + q stride
 
   int64_t base = 0;
-  for (int i0 = 0; i0 < a.n && base < hi; i0 += 256) {
-    // units before each of 256 sequences
-    const int64_t mine = i0 + tid < a.n ? units_of(a, i0 + tid) : 0;
-    int64_t scan = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int64_t below = __shfl_up(scan, d);
-      if (lane >= d) scan += below;
-    }
-    __syncthreads();
-    if (lane == 63) total4[w] = scan;
-    __syncthreads();
-    int64_t ahead = base;
-    for (int k = 0; k < w; ++k) ahead += total4[k];
-    pre[tid + 1] = ahead + scan;
-    if (tid == 0) pre[0] = base;
-    __syncthreads();
-    const int count = min(256, a.n - i0);
-    const int64_t next = pre[count];
+  for (int i0 = 0; i0 < a.n && base < hi; i0 += kThreads) {
+    const int count = min(kThreads, a.n - i0);
+    const int64_t next = a.n > kThreads ? scan(i0, base) : uniform(pre[count]);
     for (int j = 0; j < count && next > lo; ++j) {
-      const int64_t u0 = pre[j], u1 = pre[j + 1];
+      const int64_t u0 = uniform(pre[j]), u1 = uniform(pre[j + 1]);
       if (u1 <= lo) continue;
       if (u0 >= hi) break;
       const int i = i0 + j;
       const int64_t ua = max(u0, lo), ub = min(u1, hi);
-      const int64_t len = paging::held(a.lengths[i], a.c.max_pages, a.c.shift);
+      const int64_t len = paging::held(__builtin_amdgcn_readfirstlane(a.lengths[i]), a.c.max_pages, a.c.shift);
       const int64_t from = (ua - u0) * kUnit, end = min((ub - u0) * kUnit, len);
-      const int head = cb * 16 + (lane & 15);
-      S st;
-      st.begin(a, i, kv * group + min(head, group - 1), head < group);
       const int32_t *row = a.c.table + (int64_t)i * a.c.max_pages;
-      int pages[S::NB];
-      auto look = [&](int64_t pos) {
+      int32_t entries[S::NB];
+      auto look = [&](int64_t at) {
 #pragma unroll
         for (int b = 0; b < S::NB; ++b)
-          pages[b] = __builtin_amdgcn_readfirstlane(
-              pos + 16 * b < end ? paging::page_of(row, a.c.max_pages, a.c.shift, a.c.pages, pos + 16 * b) : -1);
+          entries[b] = at + 16 * b < end ? paging::entry_of(row, a.c.max_pages, a.c.shift, at + 16 * b) : -1;
       };
-      for (int64_t pos = from + w * kStep; pos < end; pos += 4 * kStep) {
-        look(pos);
-        st.step(a, kv, pos, end, pages);
+      int pages[S::NB], next[S::NB];
+      auto resolve = [&] {
+#pragma unroll
+        for (int b = 0; b < S::NB; ++b)
+          next[b] = paging::page_in(__builtin_amdgcn_readfirstlane(entries[b]), a.c.pages);
+      };
+      // The table's entries, the queries and the first tokens are asked for before any is waited for
+      // longer than the next needs.
+      S st;
+      typename S::Load x;
+      constexpr int64_t kNext = kWaves * kStep;
+      int64_t pos = from + w * kStep;
+      look(pos);
+      const int mine = cb * 16 + (lane & 15);
+      const auto q = S::ask(a, i, kv * group + min(mine, group - 1), mine < group, w);
+      resolve();
+      if (pos < end) S::load_keys(a.c, kv, pos, next, x), S::load_values(a.c, kv, pos, next, x);
+      look(pos + kNext);
+      st.clear();
+      __syncthreads();
+      st.keep(a, q, lds, w);
+      __syncthreads();
+      // The next step's keys take this one's place once its scores are formed, and so the values.
+      while (pos < end) {
+        f4 s[S::NB];
+        bool full;
+#pragma unroll
+        for (int b = 0; b < S::NB; ++b) pages[b] = next[b];
+        const bool more = pos + kNext < end;
+        resolve();
+        st.scores(a.c.dh, x, lds, s);
+        if (more) S::load_keys(a.c, kv, pos + kNext, next, x);
+        look(pos + 2 * kNext);
+        st.probabilities(pos, end, pages, s, full);
+        st.outputs(pos, end, pages, full, s, x);
+        if (more) S::load_values(a.c, kv, pos + kNext, next, x);
+        pos += kNext;
       }
-      // the four waves' states as one
+      // the waves' states as one
       const float l = rows4(st.l, [](float x, float y) { return x + y; });
       __syncthreads();
       if (lane < 16) sm[w][lane] = st.m, sl[w][lane] = st.seen ? l : -1.f;
 #pragma unroll
       for (int u = 0; u < S::NU; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+        for (int r = 0; r < 4; ++r) {
+          f4 y;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) so[w][lane & 15][64 * u + 16 * (lane >> 4) + 4 * r + e] = st.o[u][e][r];
+          for (int e = 0; e < 4; ++e) y[e] = st.o[u][e][r];
+          *reinterpret_cast<f4 *>(&so[w][lane & 15][64 * u + 16 * (lane >> 4) + 4 * r]) = y;
+        }
       __syncthreads();
-      const int c = tid >> 4, x = tid & 15;
-      Row<DP> r;
-      r.m = fmaxf(fmaxf(sm[0][c], sm[1][c]), fmaxf(sm[2][c], sm[3][c])), r.l = -1.f;
+      const int c = tid >> 5, col = tid & 31;
+      Row r{kNever, -1.f, {}};
 #pragma unroll
-      for (int u = 0; u < S::NU; ++u) r.o[u] = f4{};
+      for (int k = 0; k < kWaves; ++k) r.m = fmaxf(r.m, sm[k][c]);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < kWaves; ++k) {
         if (sl[k][c] < 0.f) continue;
         const float f = __builtin_amdgcn_exp2f(sm[k][c] - r.m);
         r.l = fmaf(sl[k][c], f, fmaxf(r.l, 0.f));
+        if (4 * col < DP) {
+          const f4 z = *reinterpret_cast<const f4 *>(&so[k][c][4 * col]);
 #pragma unroll
-        for (int u = 0; u < S::NU; ++u) {
-          const f4 y = *reinterpret_cast<const f4 *>(&so[k][c][64 * u + 4 * x]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) r.o[u][e] = fmaf(y[e], f, r.o[u][e]);
+          for (int e = 0; e < 4; ++e) r.o[e] = fmaf(z[e], f, r.o[e]);
         }
       }
       const int out_head = kv * group + cb * 16 + c;
       const bool live = cb * 16 + c < group;
       if (ua == u0 && ub == u1) {
-        put_row<DP>(a, i, out_head, live, r);
+        put_row(a, i, out_head, live, r);
         continue;
       }
       // Places of parts: a workgroup has at most one that begins its sequence (place 1) and one that
       // does not.
       const int pf = owner(u0, units, shares), pl = owner(u1 - 1, units, shares);
-      auto wg = [&](int q) { return hc + (int64_t)q * stride; };
-      auto at = [&](int q) { return 2 * wg(q) + (q == pf); };
+      auto wg = [&](int k) { return hc + (int64_t)k * stride; };
+      auto at = [&](int k) { return 2 * wg(k) + (k == pf); };
       put_part<DP>(parts, at(p), live, r);
       const int lead = pf + (p - pf) / kJoin * kJoin, members = min(kJoin, pl - lead + 1);
       if (!arrive(a.arrivals + at(lead), members, &flag)) continue;
-      r = join<DP>(parts, members, live, [&](int q) { return at(lead + q); });
+      r = join<DP>(parts, members, live, [&](int k) { return at(lead + k); });
       const int groups = (pl - pf) / kJoin + 1;
       if (groups > 1) {
         // in place of the leader's part, which no one reads any more
         __syncthreads();
         put_part<DP>(parts, at(lead), live, r);
         if (!arrive(a.arrivals + 2 * stride * a.shares + wg(pf), groups, &flag)) continue;
-        r.m = kNever, r.l = -1.f;
-#pragma unroll
-        for (int u = 0; u < S::NU; ++u) r.o[u] = f4{};
-        for (int q = 0; q < groups; q += kJoin) {
-          const Row<DP> y = join<DP>(parts, min(kJoin, groups - q), live,
-                                     [&](int z) { return at(pf + (q + z) * kJoin); });
-          if (y.l < 0.f) continue;
-          const float now = fmaxf(r.m, y.m), f0 = __builtin_amdgcn_exp2f(r.m - now), f1 = __builtin_amdgcn_exp2f(y.m - now);
-          r.l = fmaf(fmaxf(r.l, 0.f), f0, y.l * f1);
-#pragma unroll
-          for (int u = 0; u < S::NU; ++u)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) r.o[u][e] = fmaf(r.o[u][e], f0, y.o[u][e] * f1);
-          r.m = now;
-        }
+        r = join<DP>(parts, groups, live, [&](int k) { return at(pf + k * kJoin); });
       }
-      put_row<DP>(a, i, out_head, live, r);
+      put_row(a, i, out_head, live, r);
     }
     __syncthreads();
     base = next;

@@ -17,10 +17,13 @@ namespace paging {
 // The page that holds position `pos` of the sequence whose pages `row` lists, or -1: a position
 // before the first or past the listed pages, or a page that the cache does not have.  Every
 // access to a cache goes through here, so no table and no length can lead outside it.
+// (In two steps, so that a kernel can wait for an entry later than it asks for it.)
+NRS_HD int32_t entry_of(const int32_t *row, int64_t max_pages, int shift, int64_t pos) {
+  return pos < 0 || pos >> shift >= max_pages ? -1 : row[pos >> shift];
+}
+NRS_HD int page_in(int32_t entry, int64_t pages) { return entry >= 0 && entry < pages ? entry : -1; }
 NRS_HD int page_of(const int32_t *row, int64_t max_pages, int shift, int64_t pages, int64_t pos) {
-  if (pos < 0 || pos >> shift >= max_pages) return -1;
-  const int32_t p = row[pos >> shift];
-  return p >= 0 && p < pages ? p : -1;
+  return page_in(entry_of(row, max_pages, shift, pos), pages);
 }
 
 // Element offset of slot 0 of a page and head; rows of keys (and of fp32 values) follow at dh
