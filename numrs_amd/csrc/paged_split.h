@@ -80,7 +80,7 @@ __device__ __forceinline__ float max4(f4 x) { return fmaxf(fmaxf(x[0], x[1]), fm
 template <bool INT8, int DP>
 struct State {
   static constexpr int NU = (DP + 63) / 64, NT = INT8 ? DP / 32 : DP / 16;
-  static constexpr int NB = INT8 ? 4 : 1;  // blocks of 16 tokens a step
+  static constexpr int NB = INT8 ? 2 : 1;  // blocks of 16 tokens a step
   static constexpr int kQueries = DP * 64;  // bytes of the queries' fragments
   float m, l, fq;  // fq: log2(e) / sqrt(dh), less the queries' factor
   f4 o[NU][4];
@@ -100,31 +100,28 @@ struct State {
       for (int e = 0; e < 4; ++e) o[u][e] = f4{};
   }
 
-  // The queries of head `head` (zeros where it is not live), from memory: fp32, wave w's fragment; 8
-  // bits, all of them, for their largest magnitude ...
-  static constexpr int kAsked = INT8 ? 2 * NT : (NT + kWaves - 1) / kWaves;
+  // The queries of head `head` (zeros where it is not live), from memory ...
   struct Queries {
-    f4 x[kAsked];
+    f4 x[INT8 ? 2 * NT : NT];
   };
-  static __device__ __forceinline__ Queries ask(const SplitArgs &a, int i, int head, bool live, int w) {
+  static __device__ __forceinline__ Queries ask(const SplitArgs &a, int i, int head, bool live) {
     const int g = (threadIdx.x & 63) >> 4;
     const float *p = a.q + i * a.ld_q + (int64_t)head * a.c.dh;
     Queries q;
 #pragma unroll
-    for (int t = 0; t < kAsked; ++t) {
-      const int d = INT8 ? 32 * (t >> 1) + 8 * g + 4 * (t & 1) : 16 * (w + t * kWaves) + 4 * g;
+    for (int t = 0; t < (INT8 ? 2 * NT : NT); ++t) {
+      const int d = INT8 ? 32 * (t >> 1) + 8 * g + 4 * (t & 1) : 16 * t + 4 * g;
       q.x[t] = live && d < a.c.dh ? f4(*reinterpret_cast<const f4u *>(p + d)) : f4{};
     }
     return q;
   }
-  // ... into LDS: wave w has fragments w, w + kWaves, ...
-  __device__ __forceinline__ void keep(const SplitArgs &a, const Queries &q, char *lds, int w) {
+  // ... into the wave's part of LDS.
+  __device__ __forceinline__ void keep(const SplitArgs &a, const Queries &q, char *lds) {
     const int lane = threadIdx.x & 63;
     if constexpr (!INT8) {
       fq = a.alpha;
 #pragma unroll
-      for (int t = 0; t < kAsked; ++t)
-        if (w + t * kWaves < NT) *reinterpret_cast<f4 *>(lds + (w + t * kWaves) * 1024 + lane * 16) = q.x[t];
+      for (int t = 0; t < NT; ++t) *reinterpret_cast<f4 *>(lds + t * 1024 + lane * 16) = q.x[t];
     } else {
       float big = 0.f;
 #pragma unroll
@@ -136,7 +133,6 @@ struct State {
       fq = __builtin_amdgcn_ldexpf(a.alpha, -e);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        if (t % kWaves != w) continue;
         float x[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = __builtin_amdgcn_ldexpf(q.x[2 * t + (j >> 2)][j & 3], e);
@@ -357,11 +353,6 @@ __device__ __forceinline__ int owner(int64_t x, int64_t units, int shares) {
 }
 __device__ __forceinline__ int64_t first_unit(int p, int64_t units, int shares) { return units * p / shares; }
 
-__device__ __forceinline__ int64_t units_of(const SplitArgs &a, int i) {
-  const int64_t len = paging::held(a.lengths[i], a.c.max_pages, a.c.shift);
-  return len > kUnit ? (len + kUnit - 1) / kUnit : 1;  // a sequence without tokens has a row to write too
-}
-
 // A thread of a join has head c = tid / 32 and columns 4 x .. + 3 with x = tid % 32.
 struct Row {
   float m, l;  // l < 0: no token
@@ -439,28 +430,32 @@ template <bool INT8, int DP>
 __global__ void __launch_bounds__(64 * kWaves, 2) split_rows(SplitArgs a) {
   using S = State<INT8, DP>;
   constexpr int kStep = 16 * S::NB, kThreads = 64 * kWaves, kCols = S::NU * 64 + 4;
-  // the queries while tokens are taken in, then the waves' outputs
-  constexpr int kOutputs = kWaves * 16 * kCols * 4;
-  __shared__ __attribute__((aligned(16))) char lds[kOutputs > S::kQueries ? kOutputs : S::kQueries];
+  // of each wave: its queries while it takes tokens in, then its outputs
+  __shared__ __attribute__((aligned(16))) float so[kWaves][16][kCols];
+  static_assert(16 * kCols * 4 >= S::kQueries);
   __shared__ float sm[kWaves][16], sl[kWaves][16];
   __shared__ int64_t pre[kThreads + 1], sums[kWaves];
+  __shared__ int tokens[kThreads];
   __shared__ int flag;
-  float(*so)[16][kCols] = reinterpret_cast<float(*)[16][kCols]>(lds);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hc = blockIdx.x % (a.c.kv_heads * a.blocks), kv = hc / a.blocks, cb = hc % a.blocks;
   const int group = a.heads / a.c.kv_heads;
   const __amdgpu_buffer_rsrc_t parts = numrs_hip::dev_rsrc(
       a.parts, (int64_t)2 * a.c.kv_heads * a.blocks * a.shares * kPart<DP> * 4);
 
-  // units before each of kThreads sequences from i0 on, in pre, with `base` before the first; their end
+  // Of kThreads sequences from i0 on: their tokens, and the units before each in pre, with `base`
+  // before the first; returns their end.
   auto scan = [&](int i0, int64_t base) {
-    int64_t v = i0 + tid < a.n ? units_of(a, i0 + tid) : 0;
+    const int len = i0 + tid < a.n ? (int)paging::held(a.lengths[i0 + tid], a.c.max_pages, a.c.shift) : 0;
+    // a sequence without tokens has a row to write too
+    int64_t v = i0 + tid < a.n ? max(1, (int)(((unsigned)len + kUnit - 1) / kUnit)) : 0;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int64_t below = __shfl_up(v, d);
       if (lane >= d) v += below;
     }
     __syncthreads();
+    tokens[tid] = len;
     if (lane == 63) sums[w] = v;
     __syncthreads();
     for (int k = 0; k < w; ++k) v += sums[k];
@@ -476,119 +471,149 @@ __global__ void __launch_bounds__(64 * kWaves, 2) split_rows(SplitArgs a) {
   const int64_t lo = first_unit(p, units, shares), hi = first_unit(p + 1, units, shares);
   const int64_t stride = (int64_t)a.c.kv_heads * a.blocks;  // workgroup q of this block is hc + q stride
 
+  // This workgroup's part of the j-th sequence of those in LDS.
+  struct Stretch {
+    int64_t u0, u1, ua, ub;  // the sequence's units, and the workgroup's of them
+    int64_t from, end;       // its tokens
+    int waves;               // that share them
+  };
+  auto stretch = [&](int j) {
+    Stretch s;
+    s.u0 = uniform(pre[j]), s.u1 = uniform(pre[j + 1]);
+    s.ua = max(s.u0, lo), s.ub = min(s.u1, hi);
+    s.from = (s.ua - s.u0) * kUnit;
+    s.end = min((s.ub - s.u0) * kUnit, (int64_t)__builtin_amdgcn_readfirstlane(tokens[j]));
+    // Two steps a wave at least, so that several short sequences go at once; one where this is all
+    // that the workgroup has.
+    const int64_t steps = (s.end - s.from + kStep - 1) / kStep;
+    s.waves = (int)max((int64_t)1, min((int64_t)kWaves, s.ub - s.ua == hi - lo ? steps : (steps + 1) / 2));
+    return s;
+  };
+
   int64_t base = 0;
   for (int i0 = 0; i0 < a.n && base < hi; i0 += kThreads) {
     const int count = min(kThreads, a.n - i0);
-    const int64_t next = a.n > kThreads ? scan(i0, base) : uniform(pre[count]);
-    for (int j = 0; j < count && next > lo; ++j) {
-      const int64_t u0 = uniform(pre[j]), u1 = uniform(pre[j + 1]);
-      if (u1 <= lo) continue;
-      if (u0 >= hi) break;
-      const int i = i0 + j;
-      const int64_t ua = max(u0, lo), ub = min(u1, hi);
-      const int64_t len = paging::held(__builtin_amdgcn_readfirstlane(a.lengths[i]), a.c.max_pages, a.c.shift);
-      const int64_t from = (ua - u0) * kUnit, end = min((ub - u0) * kUnit, len);
-      const int32_t *row = a.c.table + (int64_t)i * a.c.max_pages;
-      int32_t entries[S::NB];
-      auto look = [&](int64_t at) {
-#pragma unroll
-        for (int b = 0; b < S::NB; ++b)
-          entries[b] = at + 16 * b < end ? paging::entry_of(row, a.c.max_pages, a.c.shift, at + 16 * b) : -1;
-      };
-      int pages[S::NB], next[S::NB];
-      auto resolve = [&] {
-#pragma unroll
-        for (int b = 0; b < S::NB; ++b)
-          next[b] = paging::page_in(__builtin_amdgcn_readfirstlane(entries[b]), a.c.pages);
-      };
-      // The table's entries, the queries and the first tokens are asked for before any is waited for
-      // longer than the next needs.
+    const int64_t next_base = a.n > kThreads ? scan(i0, base) : uniform(pre[count]);
+    int j = 0;
+    if (next_base <= lo) j = count;
+    while (j < count && uniform(pre[j + 1]) <= lo) ++j;
+    while (j < count && uniform(pre[j]) < hi) {
+      // As many sequences as the waves go round, and this wave's place.
+      int last = j, used = 0, mine = -1, first = 0;
+      Stretch my{};
+      while (last < count && uniform(pre[last]) < hi) {
+        const Stretch s = stretch(last);
+        if (used + s.waves > kWaves) break;
+        if (w >= used && w < used + s.waves) mine = last, first = used, my = s;
+        used += s.waves, ++last;
+      }
       S st;
-      typename S::Load x;
-      constexpr int64_t kNext = kWaves * kStep;
-      int64_t pos = from + w * kStep;
-      look(pos);
-      const int mine = cb * 16 + (lane & 15);
-      const auto q = S::ask(a, i, kv * group + min(mine, group - 1), mine < group, w);
-      resolve();
-      if (pos < end) S::load_keys(a.c, kv, pos, next, x), S::load_values(a.c, kv, pos, next, x);
-      look(pos + kNext);
       st.clear();
-      __syncthreads();
-      st.keep(a, q, lds, w);
-      __syncthreads();
-      // The next step's keys take this one's place once its scores are formed, and so the values.
-      while (pos < end) {
-        f4 s[S::NB];
-        bool full;
+      if (mine >= 0) {
+        const int i = i0 + mine;
+        const int32_t *row = a.c.table + (int64_t)i * a.c.max_pages;
+        char *queries = reinterpret_cast<char *>(so[w]);
+        int32_t entries[S::NB];
+        int pages[S::NB], next[S::NB];
+        auto look = [&](int64_t at) {
 #pragma unroll
-        for (int b = 0; b < S::NB; ++b) pages[b] = next[b];
-        const bool more = pos + kNext < end;
+          for (int b = 0; b < S::NB; ++b)
+            entries[b] = at + 16 * b < my.end ? paging::entry_of(row, a.c.max_pages, a.c.shift, at + 16 * b) : -1;
+        };
+        auto resolve = [&] {
+#pragma unroll
+          for (int b = 0; b < S::NB; ++b)
+            next[b] = paging::page_in(__builtin_amdgcn_readfirstlane(entries[b]), a.c.pages);
+        };
+        // The table's entries, the queries and the first tokens are asked for before any is waited for
+        // longer than the next needs.
+        typename S::Load x;
+        const int64_t ahead = my.waves * kStep;
+        int64_t pos = my.from + (w - first) * kStep;
+        look(pos);
+        const int head = cb * 16 + (lane & 15);
+        const auto q = S::ask(a, i, kv * group + min(head, group - 1), head < group);
         resolve();
-        st.scores(a.c.dh, x, lds, s);
-        if (more) S::load_keys(a.c, kv, pos + kNext, next, x);
-        look(pos + 2 * kNext);
-        st.probabilities(pos, end, pages, s, full);
-        st.outputs(pos, end, pages, full, s, x);
-        if (more) S::load_values(a.c, kv, pos + kNext, next, x);
-        pos += kNext;
-      }
-      // the waves' states as one
-      const float l = rows4(st.l, [](float x, float y) { return x + y; });
-      __syncthreads();
-      if (lane < 16) sm[w][lane] = st.m, sl[w][lane] = st.seen ? l : -1.f;
+        if (pos < my.end) S::load_keys(a.c, kv, pos, next, x), S::load_values(a.c, kv, pos, next, x);
+        look(pos + ahead);
+        st.keep(a, q, queries);
+        __builtin_amdgcn_wave_barrier();
+        // The next step's keys take this one's place once its scores are formed, and so the values.
+        while (pos < my.end) {
+          f4 s[S::NB];
+          bool full;
 #pragma unroll
-      for (int u = 0; u < S::NU; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          f4 y;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = st.o[u][e][r];
-          *reinterpret_cast<f4 *>(&so[w][lane & 15][64 * u + 16 * (lane >> 4) + 4 * r]) = y;
+          for (int b = 0; b < S::NB; ++b) pages[b] = next[b];
+          const bool more = pos + ahead < my.end;
+          resolve();
+          st.scores(a.c.dh, x, queries, s);
+          if (more) S::load_keys(a.c, kv, pos + ahead, next, x);
+          look(pos + 2 * ahead);
+          st.probabilities(pos, my.end, pages, s, full);
+          st.outputs(pos, my.end, pages, full, s, x);
+          if (more) S::load_values(a.c, kv, pos + ahead, next, x);
+          pos += ahead;
         }
-      __syncthreads();
-      const int c = tid >> 5, col = tid & 31;
-      Row r{kNever, -1.f, {}};
+        __builtin_amdgcn_wave_barrier();
+        const float l = rows4(st.l, [](float x, float y) { return x + y; });
+        if (lane < 16) sm[w][lane] = st.m, sl[w][lane] = st.seen ? l : -1.f;
 #pragma unroll
-      for (int k = 0; k < kWaves; ++k) r.m = fmaxf(r.m, sm[k][c]);
+        for (int u = 0; u < S::NU; ++u)
 #pragma unroll
-      for (int k = 0; k < kWaves; ++k) {
-        if (sl[k][c] < 0.f) continue;
-        const float f = __builtin_amdgcn_exp2f(sm[k][c] - r.m);
-        r.l = fmaf(sl[k][c], f, fmaxf(r.l, 0.f));
-        if (4 * col < DP) {
-          const f4 z = *reinterpret_cast<const f4 *>(&so[k][c][4 * col]);
+          for (int r = 0; r < 4; ++r) {
+            f4 y;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) r.o[e] = fmaf(z[e], f, r.o[e]);
-        }
+            for (int e = 0; e < 4; ++e) y[e] = st.o[u][e][r];
+            *reinterpret_cast<f4 *>(&so[w][lane & 15][64 * u + 16 * (lane >> 4) + 4 * r]) = y;
+          }
       }
-      const int out_head = kv * group + cb * 16 + c;
-      const bool live = cb * 16 + c < group;
-      if (ua == u0 && ub == u1) {
+      __syncthreads();
+      // each sequence's waves' states as one
+      used = 0;
+      for (; j < last; ++j) {
+        const Stretch s = stretch(j);
+        const int i = i0 + j, c = tid >> 5, col = tid & 31, w1 = used + s.waves;
+        Row r{kNever, -1.f, {}};
+        for (int k = used; k < w1; ++k) r.m = fmaxf(r.m, sm[k][c]);
+        for (int k = used; k < w1; ++k) {
+          if (sl[k][c] < 0.f) continue;
+          const float f = __builtin_amdgcn_exp2f(sm[k][c] - r.m);
+          r.l = fmaf(sl[k][c], f, fmaxf(r.l, 0.f));
+          if (4 * col < DP) {
+            const f4 z = *reinterpret_cast<const f4 *>(&so[k][c][4 * col]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r.o[e] = fmaf(z[e], f, r.o[e]);
+          }
+        }
+        used = w1;
+        const int out_head = kv * group + cb * 16 + c;
+        const bool live = cb * 16 + c < group;
+        if (s.ua == s.u0 && s.ub == s.u1) {
+          put_row(a, i, out_head, live, r);
+          continue;
+        }
+        // Places of parts: a workgroup has at most one that begins its sequence (place 1) and one that
+        // does not.
+        const int pf = owner(s.u0, units, shares), pl = owner(s.u1 - 1, units, shares);
+        auto wg = [&](int k) { return hc + (int64_t)k * stride; };
+        auto at = [&](int k) { return 2 * wg(k) + (k == pf); };
+        put_part<DP>(parts, at(p), live, r);
+        const int lead = pf + (p - pf) / kJoin * kJoin, members = min(kJoin, pl - lead + 1);
+        if (!arrive(a.arrivals + at(lead), members, &flag)) continue;
+        r = join<DP>(parts, members, live, [&](int k) { return at(lead + k); });
+        const int groups = (pl - pf) / kJoin + 1;
+        if (groups > 1) {
+          // in place of the leader's part, which no one reads any more
+          __syncthreads();
+          put_part<DP>(parts, at(lead), live, r);
+          if (!arrive(a.arrivals + 2 * stride * a.shares + wg(pf), groups, &flag)) continue;
+          r = join<DP>(parts, groups, live, [&](int k) { return at(pf + k * kJoin); });
+        }
         put_row(a, i, out_head, live, r);
-        continue;
       }
-      // Places of parts: a workgroup has at most one that begins its sequence (place 1) and one that
-      // does not.
-      const int pf = owner(u0, units, shares), pl = owner(u1 - 1, units, shares);
-      auto wg = [&](int k) { return hc + (int64_t)k * stride; };
-      auto at = [&](int k) { return 2 * wg(k) + (k == pf); };
-      put_part<DP>(parts, at(p), live, r);
-      const int lead = pf + (p - pf) / kJoin * kJoin, members = min(kJoin, pl - lead + 1);
-      if (!arrive(a.arrivals + at(lead), members, &flag)) continue;
-      r = join<DP>(parts, members, live, [&](int k) { return at(lead + k); });
-      const int groups = (pl - pf) / kJoin + 1;
-      if (groups > 1) {
-        // in place of the leader's part, which no one reads any more
-        __syncthreads();
-        put_part<DP>(parts, at(lead), live, r);
-        if (!arrive(a.arrivals + 2 * stride * a.shares + wg(pf), groups, &flag)) continue;
-        r = join<DP>(parts, groups, live, [&](int k) { return at(pf + k * kJoin); });
-      }
-      put_row(a, i, out_head, live, r);
+      __syncthreads();
     }
-    __syncthreads();
-    base = next;
+    base = next_base;
   }
 }
 
