@@ -23,86 +23,218 @@ struct RowArgs {
   int64_t ld;
 };
 
-// The slot of a packed row: element offset of its page and head, and its place there; page < 0
-// where it has none.
-struct Slot {
-  int64_t base;
-  int at, page;
+// The rows of a batch go by groups of four positions, 4 q .. + 3: four slots of one page, whose 8-bit
+// values lie together.  A thread has four columns of a group: four 16-byte loads of keys and of values
+// in flight, and 16 bytes of codes to store or load at once.
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+
+struct Group {
+  int64_t base;  // element offset of its first slot in its page and head
+  int page;      // -1: the cache has no place for it
+  int row[4];    // the packed rows within the sequence, -1 for a position that is none of the tile's
 };
-__device__ __forceinline__ Slot slot_of(const Cache &c, int seq, int64_t pos, int g) {
-  const int page = paging::page_of(c.table + seq * c.max_pages, c.max_pages, c.shift, c.pages, pos);
-  if (page < 0) return {0, 0, -1};
-  return {paging::page_base(page, c.kv_heads, g, c.shift, c.dh), (int)(pos & ((1 << c.shift) - 1)), page};
-}
 
-__device__ __forceinline__ float quantised_scale(float top) { return top / 127.0f; }
-
-// The code of x in a row of that scale: x / scale is rounded to fp32, then to a whole number.
-__device__ __forceinline__ uint8_t code_of(float x, float scale) {
-  if (!(scale > 0.f)) return 128;
-  return (uint8_t)((int)fminf(fmaxf(rintf(x / scale), -127.f), 127.f) + 128);
-}
-
-// One wave: a row of keys or values.
-template <bool INT8>
-__device__ void write_row(const Cache &c, const float *x, const Slot &s, bool values) {
-  const int lane = threadIdx.x & 63;
-  const float x0 = lane < c.dh ? x[lane] : 0.f, x1 = lane + 64 < c.dh ? x[lane + 64] : 0.f;
-  void *p = values ? c.v : c.k;
-  if constexpr (!INT8) {
-    float *o = static_cast<float *>(p) + s.base + (int64_t)s.at * c.dh;
-    if (lane < c.dh) o[lane] = x0;
-    if (lane + 64 < c.dh) o[lane + 64] = x1;
-  } else {
-    const bool finite = __builtin_isfinite(x0) && __builtin_isfinite(x1);
-    const float top = wave_max(fmaxf(fabsf(x0), fabsf(x1)));
-    const float scale = __all(finite) ? quantised_scale(top) : NAN;
-    uint8_t *o = static_cast<uint8_t *>(p) + s.base;
-    const int64_t row = (int64_t)s.at * c.dh;
-    if (lane < c.dh) o[values ? paging::value_code(s.at, lane, c.dh) : row + lane] = code_of(x0, scale);
-    if (lane + 64 < c.dh)
-      o[values ? paging::value_code(s.at, lane + 64, c.dh) : row + lane + 64] = code_of(x1, scale);
-    if (lane == 0) (values ? c.vs : c.ks)[s.base / c.dh + s.at] = scale;
+// Calls f(group, d) for this thread's groups of tile t and head g, for its columns d .. + 3; lanes of a
+// wave that share a group's rows are 2^lanes neighbours, d >= dh for those past the head.
+template <class F>
+__device__ __forceinline__ void for_groups(const Cache &c, const SeqTile &t, int g, const int32_t *ends, int lanes, F &&f) {
+  const int rows = min(t.len - t.t0, kTile), d = 4 * (threadIdx.x & ((1 << lanes) - 1));
+  const int64_t start = (int64_t)ends[t.seq] - t.len, p0 = start + t.t0;
+  const int64_t q0 = p0 >> 2, q1 = (p0 + rows - 1) >> 2;
+  for (int64_t q = q0 + (threadIdx.x >> lanes); q <= q1; q += 256 >> lanes) {
+    Group x;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int64_t row = 4 * q + r - start;
+      x.row[r] = row >= t.t0 && row < t.t0 + rows ? (int)row : -1;
+    }
+    x.page = paging::page_of(c.table + (int64_t)t.seq * c.max_pages, c.max_pages, c.shift, c.pages, 4 * q);
+    x.base = paging::page_base(max(x.page, 0), c.kv_heads, g, c.shift, 1) + (int)((4 * q) & ((1 << c.shift) - 1));
+    f(x, d);
   }
 }
 
-template <bool INT8>
-__global__ void __launch_bounds__(256) write_rows(RowArgs a) {
-  const SeqTile t = a.tiles[blockIdx.x / a.c.kv_heads];
-  const int g = blockIdx.x % a.c.kv_heads, end = min(t.len, t.t0 + kTile);
-  for (int r = t.t0 + (threadIdx.x >> 6); r < end; r += 4) {
-    const Slot s = slot_of(a.c, t.seq, (int64_t)a.ends[t.seq] - t.len + r, g);
-    if (s.page < 0) continue;
-    const int64_t at = (int64_t)(t.row0 + r) * a.ld + (int64_t)g * a.c.dh;
-    write_row<INT8>(a.c, a.k + at, s, false);
-    write_row<INT8>(a.c, a.v + at, s, true);
-  }
+template <int CTRL>
+__device__ __forceinline__ unsigned dpp_max(unsigned v) {
+  return max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false));
 }
 
-template <bool INT8>
-__device__ __forceinline__ float read_one(const Cache &c, const Slot &s, int d, bool values) {
-  if (s.page < 0) return 0.f;
-  const void *p = values ? c.v : c.k;
-  if constexpr (!INT8) return static_cast<const float *>(p)[s.base + (int64_t)s.at * c.dh + d];
-  const uint8_t *o = static_cast<const uint8_t *>(p) + s.base;
-  const float scale = (values ? c.vs : c.ks)[s.base / c.dh + s.at];
-  const int code = o[values ? paging::value_code(s.at, d, c.dh) : (int64_t)s.at * c.dh + d];
-  return (float)(code - 128) * scale;
-}
-
-template <bool INT8>
-__global__ void __launch_bounds__(256) read_rows(RowArgs a) {
-  const SeqTile t = a.tiles[blockIdx.x / a.c.kv_heads];
-  const int g = blockIdx.x % a.c.kv_heads, end = min(t.len, t.t0 + kTile), lane = threadIdx.x & 63;
-  for (int r = t.t0 + (threadIdx.x >> 6); r < end; r += 4) {
-    const Slot s = slot_of(a.c, t.seq, (int64_t)a.ends[t.seq] - t.len + r, g);
-    const int64_t at = (int64_t)(t.row0 + r) * a.ld + (int64_t)g * a.c.dh;
-    for (int d = lane; d < a.c.dh; d += 64) {
-      a.ko[at + d] = read_one<INT8>(a.c, s, d, false);
-      a.vo[at + d] = read_one<INT8>(a.c, s, d, true);
+// The largest of 2^lanes neighbours of each of N values, for `lanes` up to 5: lanes 1 and 2 apart by
+// quads, then the other four of eight and the other eight of sixteen by mirrors (what they hold is
+// their group's already), then the other row of a pair.
+template <int N>
+__device__ __forceinline__ void max_of(unsigned (&v)[N], int lanes) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (lanes > 0) v[i] = dpp_max<0xB1>(v[i]);
+    if (lanes > 1) v[i] = dpp_max<0x4E>(v[i]);
+    if (lanes > 2) v[i] = dpp_max<0x141>(v[i]);
+    if (lanes > 3) v[i] = dpp_max<0x140>(v[i]);
+    if (lanes > 4) {
+      const auto r = __builtin_amdgcn_permlane16_swap(v[i], v[i], false, false);
+      v[i] = max((unsigned)r[0], (unsigned)r[1]);
     }
   }
 }
+
+// Codes of four values of a row of that scale: x / scale is rounded to fp32, then to a whole number.
+// x times the reciprocal is within 2 of its last places (2^-16 at 127) of the quotient and rounds to
+// the same number unless it lies that near the middle between two: then, in a wave where any does, the
+// quotient is formed.  A row of zeros, or whose scale is NaN, has the codes 128.
+__device__ __forceinline__ unsigned codes_of(f4 x, float scale) {
+  // Added to 1.5 2^23, a number below 2^22 is rounded to a whole one, whose low bits end the sum's.
+  constexpr float kWhole = 12582912.f;
+  const float inv = __builtin_amdgcn_rcpf(scale);
+  unsigned b[4];
+  float off = 0.f;
+  bool odd = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float z = x[j] * inv, s = z + kWhole;
+    b[j] = __builtin_bit_cast(unsigned, s);
+    off = fmaxf(off, fabsf(z - (s - kWhole)));
+  }
+  // (an inverse that is infinite makes z infinite or NaN)
+  odd = scale > 0.f && !(off < 0.4999f && inv < INFINITY);
+  if (__any(odd)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float s = fminf(fmaxf(rintf(x[j] / scale), -127.f), 127.f) + kWhole;
+      b[j] = __builtin_bit_cast(unsigned, s);
+    }
+  }
+  const unsigned lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
+  return scale > 0.f ? (lo | hi) ^ 0x80808080u : 0x80808080u;
+}
+
+// The scale of a row from its largest magnitude's bits: NaN is above infinity, infinity above every
+// number, and such a row's scale is NaN.
+__device__ __forceinline__ float scale_of(unsigned top) {
+  return top < 0x7f800000u ? __builtin_bit_cast(float, top) / 127.0f : NAN;
+}
+__device__ __forceinline__ unsigned top_of(f4 x) {
+  unsigned top = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float y = x[j];  // (a bit cast of the vector's element itself takes the first element's bits)
+    top = max(top, __builtin_bit_cast(unsigned, y) & 0x7fffffffu);
+  }
+  return top;
+}
+
+// A 4 x 4 block of bytes, rows to columns.
+__device__ __forceinline__ u4 transposed(u4 x) {
+  const unsigned a = __builtin_amdgcn_perm(x[1], x[0], 0x05010400u), b = __builtin_amdgcn_perm(x[1], x[0], 0x07030602u);
+  const unsigned c = __builtin_amdgcn_perm(x[3], x[2], 0x05010400u), d = __builtin_amdgcn_perm(x[3], x[2], 0x07030602u);
+  return u4{__builtin_amdgcn_perm(c, a, 0x05040100u), __builtin_amdgcn_perm(c, a, 0x07060302u),
+            __builtin_amdgcn_perm(d, b, 0x05040100u), __builtin_amdgcn_perm(d, b, 0x07060302u)};
+}
+
+template <bool INT8>
+__global__ void __launch_bounds__(256) write_rows(RowArgs a, int lanes) {
+  const SeqTile t = a.tiles[blockIdx.x / a.c.kv_heads];
+  const int g = blockIdx.x % a.c.kv_heads, dh = a.c.dh;
+  for_groups(a.c, t, g, a.ends, lanes, [&](const Group &x, int d) {
+    f4 k[4], v[4];
+    const bool in = d < dh;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      k[r] = v[r] = f4{};
+      if (!in || x.row[r] < 0) continue;
+      const int64_t at = (int64_t)(t.row0 + x.row[r]) * a.ld + (int64_t)g * dh + d;
+      k[r] = *reinterpret_cast<const f4u *>(a.k + at), v[r] = *reinterpret_cast<const f4u *>(a.v + at);
+    }
+    if constexpr (!INT8) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (!in || x.row[r] < 0 || x.page < 0) continue;
+        const int64_t at = (x.base + r) * dh + d;
+        *reinterpret_cast<f4 *>(static_cast<float *>(a.c.k) + at) = k[r];
+        *reinterpret_cast<f4 *>(static_cast<float *>(a.c.v) + at) = v[r];
+      }
+    } else {
+      u4 kc, vc;
+      f4 ks, vs;
+      unsigned top[8];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) top[r] = top_of(k[r]), top[4 + r] = top_of(v[r]);
+      max_of(top, lanes);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        ks[r] = scale_of(top[r]), vs[r] = scale_of(top[4 + r]);
+        kc[r] = codes_of(k[r], ks[r]), vc[r] = codes_of(v[r], vs[r]);
+      }
+      if (x.page < 0) return;
+      const bool whole = (x.row[0] | x.row[1] | x.row[2] | x.row[3]) >= 0;
+      if (d == 0) {
+        if (whole) {
+          *reinterpret_cast<f4 *>(a.c.ks + x.base) = ks, *reinterpret_cast<f4 *>(a.c.vs + x.base) = vs;
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (x.row[r] >= 0) a.c.ks[x.base + r] = ks[r], a.c.vs[x.base + r] = vs[r];
+        }
+      }
+      if (!in) return;
+      uint8_t *pk = static_cast<uint8_t *>(a.c.k) + x.base * dh + d, *pv = static_cast<uint8_t *>(a.c.v) + x.base * dh + 4 * d;
+      if (whole) *reinterpret_cast<u4 *>(pv) = transposed(vc);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (x.row[r] < 0) continue;
+        *reinterpret_cast<unsigned *>(pk + r * dh) = kc[r];
+        if (!whole) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) pv[4 * j + r] = (uint8_t)(vc[r] >> (8 * j));
+        }
+      }
+    }
+  });
+}
+
+template <bool INT8>
+__global__ void __launch_bounds__(256) read_rows(RowArgs a, int lanes) {
+  const SeqTile t = a.tiles[blockIdx.x / a.c.kv_heads];
+  const int g = blockIdx.x % a.c.kv_heads, dh = a.c.dh;
+  for_groups(a.c, t, g, a.ends, lanes, [&](const Group &x, int d) {
+    if (d >= dh) return;
+    f4 k[4] = {}, v[4] = {};
+    if (x.page >= 0) {
+      if constexpr (!INT8) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int64_t at = (x.base + r) * dh + d;
+          k[r] = *reinterpret_cast<const f4 *>(static_cast<const float *>(a.c.k) + at);
+          v[r] = *reinterpret_cast<const f4 *>(static_cast<const float *>(a.c.v) + at);
+        }
+      } else {
+        const uint8_t *pk = static_cast<const uint8_t *>(a.c.k) + x.base * dh + d;
+        u4 kc;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) kc[r] = *reinterpret_cast<const unsigned *>(pk + r * dh);
+        const u4 vc = transposed(*reinterpret_cast<const u4 *>(static_cast<const uint8_t *>(a.c.v) + x.base * dh + 4 * d));
+        const f4 ks = *reinterpret_cast<const f4 *>(a.c.ks + x.base), vs = *reinterpret_cast<const f4 *>(a.c.vs + x.base);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            k[r][j] = (float)((int)(kc[r] >> (8 * j) & 255) - 128) * ks[r];
+            v[r][j] = (float)((int)(vc[r] >> (8 * j) & 255) - 128) * vs[r];
+          }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if (x.row[r] < 0) continue;
+      const int64_t at = (int64_t)(t.row0 + x.row[r]) * a.ld + (int64_t)g * dh + d;
+      *reinterpret_cast<f4u *>(a.ko + at) = k[r], *reinterpret_cast<f4u *>(a.vo + at) = v[r];
+    }
+  });
+}
+
+// Neighbours that share a row, four columns each: the power of two that covers a head.
+int row_lanes(int dh) { return paging::log2_of((dh + 3) / 4); }
 
 Cache device_cache(const numrs_hip_kv_cache &c, const int32_t *table, int64_t max_pages) {
   return {c.k, c.v, c.k_scale, c.v_scale, c.pages, max_pages, table, paging::log2_of(c.page_size),
@@ -155,9 +287,9 @@ int numrs_hip_kv_cache_write(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cache
   const RowArgs a{device_cache(*cache, table, max_pages), s.in_order, ends, k, v, nullptr, nullptr, ld};
   const unsigned grid = (unsigned)(s.tiles * cache->kv_heads);
   if (cache->format == NUMRS_HIP_KV_F32)
-    write_rows<false><<<grid, 256, 0, ctx->stream>>>(a);
+    write_rows<false><<<grid, 256, 0, ctx->stream>>>(a, row_lanes((int)cache->head_dim));
   else
-    write_rows<true><<<grid, 256, 0, ctx->stream>>>(a);
+    write_rows<true><<<grid, 256, 0, ctx->stream>>>(a, row_lanes((int)cache->head_dim));
   return check_launch(ctx, "write_rows");
 }
 
@@ -173,9 +305,9 @@ int numrs_hip_kv_cache_read(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cache,
   const RowArgs a{device_cache(*cache, table, max_pages), s.in_order, ends, nullptr, nullptr, k, v, ld};
   const unsigned grid = (unsigned)(s.tiles * cache->kv_heads);
   if (cache->format == NUMRS_HIP_KV_F32)
-    read_rows<false><<<grid, 256, 0, ctx->stream>>>(a);
+    read_rows<false><<<grid, 256, 0, ctx->stream>>>(a, row_lanes((int)cache->head_dim));
   else
-    read_rows<true><<<grid, 256, 0, ctx->stream>>>(a);
+    read_rows<true><<<grid, 256, 0, ctx->stream>>>(a, row_lanes((int)cache->head_dim));
   return check_launch(ctx, "read_rows");
 }
 
