@@ -185,7 +185,7 @@ __device__ void row_dkv(const BwdArgs &b, const tiles::BackwardArgs &a, const Se
 // A block of 128 query rows of one head.
 template <int DP>
 __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) dq_block(BwdArgs b, tiles::BackwardArgs a) {
-  __shared__ __attribute__((aligned(16))) char lds[2 * 3 * 32 * DP * 4];
+  __shared__ __attribute__((aligned(16))) char lds[2 * 2 * 32 * DP * 4];
   const SeqTile t = b.tiles[blockIdx.x / a.heads];
   const int h = blockIdx.x % a.heads;
   if (tiles::dq_tile<DP>(a, t, h, lds)) return;
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) dq_block(BwdArgs b, til
 // A block of 128 key rows of one kv head, or one query head's part of it.
 template <int DP>
 __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) dkv_block(BwdArgs b, tiles::BackwardArgs a) {
-  __shared__ __attribute__((aligned(16))) char lds[2 * (4 * 32 * DP * 4 + 256)];
+  __shared__ __attribute__((aligned(16))) char lds[2 * (2 * 32 * DP * 4 + 256)];
   const int slots = a.heads / a.each;
   const SeqTile t = b.tiles[blockIdx.x / slots];
   const int h0 = blockIdx.x % slots * a.each;
@@ -258,20 +258,18 @@ int with_dp(int dh, F &&f) {
 // Memory for one operand's fragments and exponents.
 struct Packed {
   TempBlock block;
-  char *rows = nullptr, *cols = nullptr;
+  char *rows = nullptr;
   int *exps = nullptr;
   explicit Packed(numrs_hip_ctx *ctx) : block(ctx) {}
-  int alloc(const Seqs &s, int heads, int dh, bool want_rows, bool want_cols) {
+  int alloc(const Seqs &s, int heads, int dh) {
     const size_t n = (size_t)s.tiles * heads, image = n * kTile * padded(dh) * 4;
-    if (int rc = block.alloc((want_rows + want_cols) * image + n * sizeof(int))) return rc;
-    char *p = static_cast<char *>(block.p);
-    if (want_rows) rows = p, p += image;
-    if (want_cols) cols = p, p += image;
-    exps = reinterpret_cast<int *>(p);
+    if (int rc = block.alloc(image + n * sizeof(int))) return rc;
+    rows = static_cast<char *>(block.p);
+    exps = reinterpret_cast<int *>(rows + image);
     return NUMRS_HIP_OK;
   }
   tiles::Source source(const float *x, int64_t ld, int heads, float most) const {
-    return {x, ld, rows, cols, exps, most, heads, nullptr, nullptr, nullptr};
+    return {x, ld, rows, exps, most, heads, nullptr, nullptr, nullptr};
   }
 };
 
@@ -287,19 +285,17 @@ int packed_forward(numrs_hip_ctx *ctx, const Seqs &s, const float *q, int64_t ld
   if (q == nullptr || k == nullptr || v == nullptr || out == nullptr)
     return fail(ctx, NUMRS_HIP_E_INVALID, "attention_packed: null pointer");
   DeviceScope dev(ctx);
-  Packed pq(ctx), pk(ctx), pv(ctx);
+  Packed pk(ctx), pv(ctx);
   const int H = (int)h.heads, Hk = (int)h.kv_heads, dh = (int)h.dh;
-  if (int rc = pq.alloc(s, H, dh, true, false)) return rc;
-  if (int rc = pk.alloc(s, Hk, dh, true, false)) return rc;
-  if (int rc = pv.alloc(s, Hk, dh, false, true)) return rc;
+  if (int rc = pk.alloc(s, Hk, dh)) return rc;
+  if (int rc = pv.alloc(s, Hk, dh)) return rc;
   const tiles::PackArgs p{s.in_order,
-                          {pq.source(q, ld_q, H, kMostScore), pk.source(k, ld_kv, Hk, kMostScore),
-                           pv.source(v, ld_kv, Hk, kMostValue), {}},
-                          H + 2 * Hk, dh};
+                          {pk.source(k, ld_kv, Hk, kMostScore), pv.source(v, ld_kv, Hk, kMostValue), {}, {}},
+                          2 * Hk, dh};
   const float alpha = kLog2e / std::sqrt((float)dh);
   const FwdArgs a{s.by_work, q, k, v, out, stats, ld_q, ld_kv, ld_out, H, Hk, dh, alpha};
-  const tiles::ForwardArgs f{pq.rows, pk.rows, pv.cols, pq.exps, pk.exps, pv.exps, out, stats, ld_out,
-                             H, Hk, dh, alpha};
+  const tiles::ForwardArgs f{q, pk.rows, pv.rows, pk.exps, pv.exps, out, stats, ld_q, ld_out,
+                             H, Hk, dh, alpha, kMostScore};
   return with_dp(dh, [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
     tiles::pack<DP><<<(unsigned)(s.tiles * p.slots), 256, 0, ctx->stream>>>(p);
@@ -326,24 +322,28 @@ int packed_backward(numrs_hip_ctx *ctx, const Seqs &s, const float *q, int64_t l
   const int each = group > 1 && s.blocks * Hk >= 4 * ctx->num_cus ? group : 1;
   Packed pq(ctx), pk(ctx), pv(ctx), pg(ctx);
   TempBlock rowstat(ctx), parts(ctx);
-  if (int rc = pq.alloc(s, H, dh, true, keys)) return rc;
-  if (int rc = pk.alloc(s, Hk, dh, true, dq != nullptr)) return rc;
-  if (int rc = pv.alloc(s, Hk, dh, true, false)) return rc;
-  if (int rc = pg.alloc(s, H, dh, true, keys)) return rc;
-  if (int rc = rowstat.alloc((size_t)s.tiles * H * kTile * 2 * sizeof(float))) return rc;
+  // The key rows walk over the queries and the output's gradient, the query rows over keys and values
+  // (whose factors both need).
+  if (int rc = pk.alloc(s, Hk, dh)) return rc;
+  if (int rc = pv.alloc(s, Hk, dh)) return rc;
+  if (keys) {
+    if (int rc = pq.alloc(s, H, dh)) return rc;
+    if (int rc = pg.alloc(s, H, dh)) return rc;
+    if (int rc = rowstat.alloc((size_t)s.tiles * H * kTile * 2 * sizeof(float))) return rc;
+  }
   const size_t part = (size_t)s.total * H * dh * sizeof(float);
   if (keys && each < group)
     if (int rc = parts.alloc(((dk != nullptr) + (dv != nullptr)) * part)) return rc;
   tiles::PackArgs p{s.in_order,
-                    {pq.source(q, ld_q, H, kMostScore), pk.source(k, ld_kv, Hk, kMostScore),
-                     pv.source(v, ld_kv, Hk, kMostValue), pg.source(dout, ld_out, H, kMostValue)},
-                    2 * H + 2 * Hk, dh};
+                    {pk.source(k, ld_kv, Hk, kMostScore), pv.source(v, ld_kv, Hk, kMostValue),
+                     pq.source(q, ld_q, H, kMostScore), pg.source(dout, ld_out, H, kMostValue)},
+                    2 * Hk + (keys ? 2 * H : 0), dh};
   p.src[3].out = out, p.src[3].stats = stats, p.src[3].rowstat = rowstat.f();
   const float alpha = kLog2e / std::sqrt((float)dh), scale = 1.0f / std::sqrt((float)dh);
   BwdArgs b{s.by_work, q, k, v, out, dout, stats, ld_q, ld_kv, ld_out};
-  tiles::BackwardArgs a{pq.rows, pq.cols, pk.rows, pk.cols, pv.rows, pg.rows, pg.cols, pq.exps, pk.exps,
-                        pv.exps, pg.exps, rowstat.f(), dq, dk, dv, ld_q, ld_kv, ld_kv, s.total,
-                        H, Hk, dh, accumulate, each, alpha, scale};
+  tiles::BackwardArgs a{q, k, v, out, dout, stats, ld_q, ld_kv, ld_out, pq.rows, pk.rows, pv.rows, pg.rows,
+                        pq.exps, pk.exps, pv.exps, pg.exps, rowstat.f(), dq, dk, dv, ld_q, ld_kv, ld_kv, s.total,
+                        H, Hk, dh, accumulate, each, alpha, scale, kMostScore, kMostValue};
   return with_dp(dh, [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
     tiles::pack<DP><<<(unsigned)(s.tiles * p.slots), 256, 0, ctx->stream>>>(p);

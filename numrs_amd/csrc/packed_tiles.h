@@ -9,12 +9,13 @@
 // v_mfma_f32_32x32x16_f16 sums of at most 64 tokens (or one head) start from zero and are added to
 // fp32 totals: the matrix cores' own sum is cut off, not rounded.
 //
-// `pack` splits each operand once a call, in the order in which the products read it: a fragment is
-// 64 lanes x 16 bytes, so a tile goes to LDS by a plain copy and every LDS access is contiguous.
-//   row fragment (32 tokens, 16 columns): lane (g, c) has token c, columns 8 g .. + 7;
-//   column fragment (32 columns, 16 tokens): lane (g, c) has column c of the tokens 4 g .. + 3 and
-//   8 + 4 g .. + 3, which is the order in which a product leaves its results' rows: the
-//   probabilities of one product are the next one's operand in the lane that formed them.
+// `pack` splits what the kernels walk over once a call, in the order in which the products read it: a
+// fragment is the 32 tokens x 16 columns of a term, lane (g, c)'s 16 bytes being token c's columns 8 g
+// .. + 7, so a tile goes to LDS by a plain copy.  The products over tokens need columns: the transposing
+// LDS read gives lane (g, c) column c of the tokens 4 g .. + 3 and 8 + 4 g .. + 3, which is the order in
+// which a product leaves its results' rows, so the probabilities of one product are the next one's
+// operand in the lane that formed them.  Token c's second 16 bytes lie at place c ^ 4 of their half, so
+// that the 16 lanes of a transposing read, four tokens' 32 bytes each, meet no bank twice.
 #pragma once
 
 #include "packed.h"
@@ -77,24 +78,80 @@ template <int DP>
 struct Shape {
   static constexpr int NS = DP / 16, NB = DP / 32;  // steps of a product over the head, blocks of 32 columns
   static constexpr int kBytes = kTile * DP * 4;     // a tile's fragments
-  // byte offsets of a fragment pair
-  static __device__ __forceinline__ constexpr int row_frag(int kb, int s) { return (kb * NS + s) * 2048; }
-  static __device__ __forceinline__ constexpr int col_frag(int kb, int s, int db) {
-    return ((kb * 2 + s) * NB + db) * 2048;
-  }
+  static constexpr int kHalf = kBytes / 2;          // 32 tokens'
 };
 
-__device__ __forceinline__ Terms frag(const char *p, int lane) {
-  return {*reinterpret_cast<const h8 *>(p + lane * 16), *reinterpret_cast<const h8 *>(p + 1024 + lane * 16)};
+// Byte offset of token c's columns 8 g .. + 7 in a fragment.
+__device__ __forceinline__ int place(int g, int c) { return (32 * g + (c ^ 4 * g)) * 16; }
+
+// Step s of 32 tokens' rows at p: lane (g, c) has token c, columns 16 s + 8 g .. + 7.  off: place(g, c).
+__device__ __forceinline__ Terms rows_of(const char *p, int s, int off) {
+  p += s * 2048 + off;
+  return {*reinterpret_cast<const h8 *>(p), *reinterpret_cast<const h8 *>(p + 1024)};
 }
+
+// Columns 32 b + c of 16 tokens (the st-th 16 of the 32 at p).  off: columns_place(lane).
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef short s8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) s4 lds_s4;
+__device__ __forceinline__ int columns_place(int lane) {
+  // lane 4 r + x of a group of 16 reads four columns 4 x .. + 3 of token 4 g + r
+  const int g = lane >> 5, r = (lane & 15) >> 2, x = lane & 3;
+  return place(x >> 1, 4 * g + r) + (x & 1) * 8 + (lane >> 4 & 1) * 2048;
+}
+__device__ __forceinline__ h8 columns_term(const char *p) {
+  const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)p);
+  const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(p + 128));
+  return __builtin_bit_cast(h8, s8(__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7)));
+}
+__device__ __forceinline__ Terms columns_of(const char *p, int b, int st, int off) {
+  p += b * 4096 + st * 256 + off;
+  return {columns_term(p), columns_term(p + 1024)};
+}
+
+// A lane's row of an operand from memory, columns 16 s + 8 g .. + 7 of each step; zeros past the head.
+template <int DP>
+struct RowValues {
+  float x[DP / 16][8];
+  __device__ __forceinline__ void load(const float *p, bool live, int dh, int g) {
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+      const int d = 16 * s + 8 * g;
+      f4 lo{}, hi{};
+      if (live && d < dh) lo = *reinterpret_cast<const f4u *>(p + d), hi = *reinterpret_cast<const f4u *>(p + d + 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[s][j] = lo[j], x[s][4 + j] = hi[j];
+    }
+  }
+  // Splits it times 2^e, with e for the row's largest magnitude; odd: see kOdd.
+  __device__ __forceinline__ int split_into(Terms (&t)[DP / 16], float most, bool &odd) {
+    float big = 0.f;
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        odd |= !(fabsf(x[s][j]) < most);
+        big = fmaxf(big, fabsf(x[s][j]));
+      }
+    big = half_pair(big, [](float a, float b) { return fmaxf(a, b); });
+    const int e = big > 0.f ? min(12 - __builtin_amdgcn_frexp_expf(big), 140) : 0;
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[s][j] = __builtin_amdgcn_ldexpf(x[s][j], e);
+      t[s] = split8(x[s]);
+    }
+    return e;
+  }
+};
 
 // One operand to split: heads x tiles.
 struct Source {
   const float *x;
   int64_t ld;
-  char *rows, *cols;  // null: not needed in that order
-  int *exps;          // [tiles, heads]
-  float most;         // larger magnitudes make a tile odd
+  char *rows;   // fragments [tiles, heads]
+  int *exps;    // [tiles, heads]
+  float most;   // larger magnitudes make a tile odd
   int heads;
   // The output's gradient: its rows are divided by their softmax sum l, which turns the backward's
   // p into 2^(s - m), and the rows' references and totals go to `rowstat` [tiles, heads, 64]: (m,
@@ -113,7 +170,6 @@ template <int DP>
 __global__ void __launch_bounds__(256) pack(PackArgs a) {
   using S = Shape<DP>;
   constexpr int NI = DP / 32, NC = DP / 8;  // a thread's chunks of 8 columns; chunks of a row
-  __shared__ unsigned image[kTile][DP + 1];
   __shared__ float top[4];
   __shared__ float part[kTile][NC + 1];  // out . dout of 8 columns
   const int tile = blockIdx.x / a.slots, tid = threadIdx.x;
@@ -183,36 +239,9 @@ __global__ void __launch_bounds__(256) pack(PackArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[i][j] = __builtin_amdgcn_ldexpf(v[i][j], e);
     const Terms p = split8(v[i]);
-    if (s.rows != nullptr) {
-      char *o = s.rows + at + S::row_frag(row >> 5, c >> 1) + ((row & 31) + 32 * (c & 1)) * 16;
-      *reinterpret_cast<h8 *>(o) = p.h;
-      *reinterpret_cast<h8 *>(o + 1024) = p.m;
-    }
-    if (s.cols != nullptr) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const unsigned w = __builtin_bit_cast(unsigned, h2{p.h[j], p.m[j]});
-        image[row][c * 8 + j] = w;
-      }
-    }
-  }
-  if (s.cols == nullptr) return;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < NI; ++i) {
-    const int f = (i * 256 + tid) >> 6, lane = tid & 63, g = lane >> 5;
-    const int db = f % S::NB, ks = f / S::NB;  // ks: 16 tokens
-    u4 h, m;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int r = 16 * ks + 4 * g + (j >= 2 ? 8 : 0) + 2 * (j & 1), d = 32 * db + (lane & 31);
-      const unsigned p = image[r][d], q = image[r + 1][d];
-      h[j] = (p & 0xffff) | q << 16;
-      m[j] = p >> 16 | (q & 0xffff0000);
-    }
-    char *o = s.cols + at + S::col_frag(ks >> 1, ks & 1, db) + lane * 16;
-    *reinterpret_cast<u4 *>(o) = h;
-    *reinterpret_cast<u4 *>(o + 1024) = m;
+    char *o = s.rows + at + (row >> 5) * S::kHalf + (c >> 1) * 2048 + place(c & 1, row & 31);
+    *reinterpret_cast<h8 *>(o) = p.h;
+    *reinterpret_cast<h8 *>(o + 1024) = p.m;
   }
 }
 
@@ -247,12 +276,13 @@ __device__ __forceinline__ float over16(const f16 &x, Op op) {
 }
 
 struct ForwardArgs {
-  const char *q, *k, *v;      // fragments: rows of q and k, columns of v
-  const int *eq, *ek, *ev;
+  const float *q;
+  const char *k, *v;  // fragments
+  const int *ek, *ev;
   float *out, *stats;
-  int64_t ld_out;
+  int64_t ld_q, ld_out;
   int heads, kv_heads, dh;
-  float alpha;  // log2(e) / sqrt(dh)
+  float alpha, most;  // log2(e) / sqrt(dh); a query's largest magnitude
 };
 
 // Four waves own 32 query rows each of a block of 128 and walk the keys before them.  S^T = K Q^T
@@ -268,20 +298,17 @@ __device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile
   const int c = lane & 31, hi = lane >> 5, g = h / (a.heads / a.kv_heads);
   const int end = min(t.t0 + 128, t.len), q0 = t.t0 + 32 * w;
   const int64_t kv0 = (int64_t)t.tile0 * a.kv_heads + g;  // the sequence's first tile of this head
-  const int first = t.t0 / kTile, last = (end - 1) / kTile;
-  bool odd = false;
-  for (int i = tid; i <= last; i += 256) {
-    odd |= a.ek[kv0 + (int64_t)i * a.kv_heads] == kOdd || a.ev[kv0 + (int64_t)i * a.kv_heads] == kOdd;
-    if (i >= first) odd |= a.eq[(int64_t)(t.tile0 + i) * a.heads + h] == kOdd;
-  }
-  if (__syncthreads_or(odd)) return false;
-
-  const bool live = q0 < t.len;
-  const int64_t qt = (int64_t)(t.tile0 + min(q0 / kTile, last)) * a.heads + h;
+  const int last = (end - 1) / kTile;
   Terms q[S::NS];
-#pragma unroll
-  for (int s = 0; s < S::NS; ++s) q[s] = frag(a.q + qt * S::kBytes + S::row_frag(w & 1, s), lane);
-  const int eq = a.eq[qt];
+  bool odd = false;
+  RowValues<DP> qx;
+  qx.load(a.q + (int64_t)(t.row0 + q0 + c) * a.ld_q + (int64_t)h * a.dh, q0 + c < t.len, a.dh, hi);
+  for (int i = tid; i <= last; i += 256)
+    odd |= a.ek[kv0 + (int64_t)i * a.kv_heads] == kOdd || a.ev[kv0 + (int64_t)i * a.kv_heads] == kOdd;
+  const int eq = qx.split_into(q, a.most, odd);
+  if (__syncthreads_or(odd)) return false;
+  const bool live = q0 < t.len;
+  const int ro = place(hi, c), co = columns_place(lane);
 
   f16 o[S::NB] = {};
   float m = -INFINITY, top = -INFINITY, l = 0.f;
@@ -304,7 +331,7 @@ __device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile
 #pragma unroll
     for (int st = 0; st < S::NS; ++st)
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) mma(s[kb], frag(kf + S::row_frag(kb, st), lane), q[st]);
+      for (int kb = 0; kb < KB; ++kb) mma(s[kb], rows_of(kf + kb * S::kHalf, st, ro), q[st]);
     // an underflow of f must not make -inf * f NaN
     const float f = fmaxf(__builtin_amdgcn_ldexpf(a.alpha, -(eq + a.ek[tile_of(i)])), 1.17549435e-38f);
     if ((i + 1) * KT > q0 + 1) {  // keys after a row of the wave
@@ -347,7 +374,7 @@ __device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int st = 0; st < 2; ++st) mma(x, frag(vf + S::col_frag(kb, st, b), lane), p[kb][st]);
+        for (int st = 0; st < 2; ++st) mma(x, columns_of(vf + kb * S::kHalf, b, st, co), p[kb][st]);
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[b][e] = fmaf(x[e], fv, o[b][e]);
     }
@@ -379,7 +406,9 @@ __device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile
 }
 
 struct BackwardArgs {
-  const char *q, *qt, *k, *kt, *v, *g, *gt;  // fragments: rows, and with t columns; g: the output's gradient
+  const float *xq, *xk, *xv, *out, *dout, *stats;
+  int64_t ld_xq, ld_xkv, ld_out;
+  const char *q, *k, *v, *g;  // fragments; g: the output's gradient
   const int *eq, *ek, *ev, *eg;
   const float *rowstat;
   float *dq, *dk, *dv;
@@ -387,6 +416,7 @@ struct BackwardArgs {
   int heads, kv_heads, dh, accumulate;
   int each;             // query heads of a workgroup of key rows: its group, or one
   float alpha, scale;   // log2(e) / sqrt(dh), 1 / sqrt(dh)
+  float most_score, most_value;  // see Source
 };
 
 __device__ __forceinline__ int wave_min(int v) {
@@ -400,14 +430,10 @@ __device__ __forceinline__ int wave_min(int v) {
 // brought to the smallest ev of the sequence, and by 2^-32 below 1:
 //   dS'' = 2^15 p (raw 2^(least - ev - 32) - D 2^(eg + least - 32)) = dS 2^(eg + least - 17),
 // at most 2^15 and split like any operand.
-__device__ __forceinline__ void dscores(const f16 &s, const f16 &raw, float f, float graw, const float *m,
-                                        const float *d, f16 &p, f16 &ds) {
-#pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    p[e] = __builtin_amdgcn_exp2f(fmaf(s[e], f, 15.f - m[e]));
-    ds[e] = p[e] * fmaf(raw[e], graw, -d[e]);
-  }
+__device__ __forceinline__ float score(float s, float f, float m) {
+  return __builtin_amdgcn_exp2f(fmaf(s, f, 15.f - m));
 }
+__device__ __forceinline__ float dscore(float p, float raw, float graw, float d) { return p * fmaf(raw, graw, -d); }
 
 // Writes a wave's 32 columns of a transposed result: row `row` of the matrix at p.
 template <int DP>
@@ -432,42 +458,52 @@ __device__ __forceinline__ void put_rows(float *p, const f16 (&x)[DP / 32], int 
 template <int DP>
 __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t, int h, char *lds) {
   using S = Shape<DP>;
-  constexpr int kPart = 32 * DP * 4, kStage = 3 * kPart;
+  constexpr int kPart = S::kHalf, kStage = 2 * kPart;
   __shared__ int least4[4];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, hi = lane >> 5, g = h / (a.heads / a.kv_heads);
   const int end = min(t.t0 + 128, t.len), q0 = t.t0 + 32 * w;
-  const int64_t kv0 = (int64_t)t.tile0 * a.kv_heads + g;
-  const int first = t.t0 / kTile, last = (end - 1) / kTile;
+  const int64_t kv0 = (int64_t)t.tile0 * a.kv_heads + g, row = t.row0 + q0 + c;
+  const int last = (end - 1) / kTile;
+  const bool live = q0 < t.len, mine_in = q0 + c < t.len;
   bool odd = false;
   int least = kOdd;
   for (int i = tid; i <= last; i += 256) {
     const int ev = a.ev[kv0 + (int64_t)i * a.kv_heads];
     least = min(least, ev);
     odd |= a.ek[kv0 + (int64_t)i * a.kv_heads] == kOdd || ev == kOdd;
-    if (i >= first) {
-      const int64_t at = (int64_t)(t.tile0 + i) * a.heads + h;
-      odd |= a.eq[at] == kOdd || a.eg[at] == kOdd;
+  }
+  Terms q[S::NS], go[S::NS];
+  float m = INFINITY, D = 0.f;  // a row past the sequence: p = 0
+  int eq, eg;
+  {
+    RowValues<DP> x, o;
+    x.load(a.xq + row * a.ld_xq + (int64_t)h * a.dh, mine_in, a.dh, hi);
+    eq = x.split_into(q, a.most_score, odd);
+    x.load(a.dout + row * a.ld_out + (int64_t)h * a.dh, mine_in, a.dh, hi);
+    o.load(a.out + row * a.ld_out + (int64_t)h * a.dh, mine_in, a.dh, hi);
+    float inv = 1.f;
+    if (mine_in) {
+      const float *st = a.stats + (row * a.heads + h) * 2;
+      m = st[0], inv = 1.f / st[1];
     }
+#pragma unroll
+    for (int s = 0; s < S::NS; ++s) {
+      float part = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) part = fmaf(x.x[s][j], o.x[s][j], part), x.x[s][j] *= inv;
+      D += part;
+    }
+    D = half_pair(D, [](float y, float z) { return y + z; }) * inv;
+    odd |= !__builtin_isfinite(D);
+    eg = x.split_into(go, a.most_value, odd);
   }
   least = wave_min(least);
   if (lane == 0) least4[w] = least;
   if (__syncthreads_or(odd)) return false;
   least = min(min(least4[0], least4[1]), min(least4[2], least4[3]));
-
-  const bool live = q0 < t.len;
-  const int64_t qt = (int64_t)(t.tile0 + min(q0 / kTile, last)) * a.heads + h;
-  Terms q[S::NS], go[S::NS];
-#pragma unroll
-  for (int s = 0; s < S::NS; ++s) {
-    q[s] = frag(a.q + qt * S::kBytes + S::row_frag(w & 1, s), lane);
-    go[s] = frag(a.g + qt * S::kBytes + S::row_frag(w & 1, s), lane);
-  }
-  const int eq = a.eq[qt], eg = a.eg[qt];
-  const f2 rs = *reinterpret_cast<const f2 *>(a.rowstat + (qt * kTile + 32 * (w & 1) + c) * 2);
-  float m[16], d[16];
-#pragma unroll
-  for (int e = 0; e < 16; ++e) m[e] = rs[0], d[e] = __builtin_amdgcn_ldexpf(rs[1], least - 32);
+  D = __builtin_amdgcn_ldexpf(D, eg + least - 32);
+  const int ro = place(hi, c), co = columns_place(lane);
 
   f16 x[S::NB] = {};
   const int n = (end + 31) / 32, mine = live ? q0 / 32 + 1 : 0;
@@ -477,24 +513,24 @@ __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t,
     char *to = lds + (i & 1) * kStage;
     fetch<kPart>(a.k + at, to, w, lane);
     fetch<kPart>(a.v + at, to + kPart, w, lane);
-    fetch<kPart>(a.kt + at, to + 2 * kPart, w, lane);
   };
   issue(0);
   for (int i = 0; i < n; ++i) {
     fetched();
     if (i + 1 < n) issue(i + 1);
     if (i >= mine) continue;
-    const char *kf = lds + (i & 1) * kStage, *vf = kf + kPart, *ktf = vf + kPart;
+    const char *kf = lds + (i & 1) * kStage, *vf = kf + kPart;
     f16 s = {}, r = {};
 #pragma unroll
     for (int st = 0; st < S::NS; ++st) {
-      mma(s, frag(kf + S::row_frag(0, st), lane), q[st]);
-      mma(r, frag(vf + S::row_frag(0, st), lane), go[st]);
+      mma(s, rows_of(kf, st, ro), q[st]);
+      mma(r, rows_of(vf, st, ro), go[st]);
     }
     const int ek = a.ek[tile_of(i)], ev = a.ev[tile_of(i)];
     f16 p, ds;
-    dscores(s, r, __builtin_amdgcn_ldexpf(a.alpha, -(eq + ek)), __builtin_amdgcn_ldexpf(1.f, least - ev - 32), m, d,
-            p, ds);
+    const float f = __builtin_amdgcn_ldexpf(a.alpha, -(eq + ek)), graw = __builtin_amdgcn_ldexpf(1.f, least - ev - 32);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) p[e] = score(s[e], f, m), ds[e] = dscore(p[e], r[e], graw, D);
     if (32 * i + 31 > q0) {
 #pragma unroll
       for (int e = 0; e < 16; ++e)
@@ -508,15 +544,13 @@ __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t,
 #pragma unroll
     for (int nb = 0; nb < S::NB; ++nb) {
       f16 z = {};
-      mma(z, frag(ktf + S::col_frag(0, 0, nb), lane), b[0]);
-      mma(z, frag(ktf + S::col_frag(0, 1, nb), lane), b[1]);
+      mma(z, columns_of(kf, nb, 0, co), b[0]);
+      mma(z, columns_of(kf, nb, 1, co), b[1]);
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[nb][e] = fmaf(z[e], back, x[nb][e]);
     }
   }
-  const int row = q0 + c;
-  if (row < t.len)
-    put_rows<DP>(a.dq + (int64_t)(t.row0 + row) * a.ld_q + (int64_t)h * a.dh, x, a.dh, hi, a.accumulate);
+  if (mine_in) put_rows<DP>(a.dq + row * a.ld_q + (int64_t)h * a.dh, x, a.dh, hi, a.accumulate);
   return true;
 }
 
@@ -525,41 +559,42 @@ __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t,
 template <int DP>
 __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t, int h0, char *lds) {
   using S = Shape<DP>;
-  constexpr int kPart = 32 * DP * 4, kStage = 4 * kPart + 256;
+  constexpr int kPart = S::kHalf, kStage = 2 * kPart + 256;
   __shared__ int least4[4];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, hi = lane >> 5, g = h0 / (a.heads / a.kv_heads);
-  const int end = min(t.t0 + 128, t.len), k0 = t.t0 + 32 * w;
-  const int64_t kv0 = (int64_t)t.tile0 * a.kv_heads + g;
-  const int first = t.t0 / kTile, last = (end - 1) / kTile, all = (t.len - 1) / kTile;
+  const int k0 = t.t0 + 32 * w;
+  const int64_t kv0 = (int64_t)t.tile0 * a.kv_heads + g, row = t.row0 + k0 + c;
+  const int first = t.t0 / kTile, all = (t.len - 1) / kTile;
+  const bool live = k0 < t.len, mine_in = k0 + c < t.len;
   bool odd = false;
   int least = kOdd;
   for (int i = tid; i <= all; i += 256) {
     const int ev = a.ev[kv0 + (int64_t)i * a.kv_heads];
     least = min(least, ev);
     odd |= ev == kOdd;
-    if (i >= first && i <= last) odd |= a.ek[kv0 + (int64_t)i * a.kv_heads] == kOdd;
     if (i >= first)
       for (int h = h0; h < h0 + a.each; ++h) {
         const int64_t at = (int64_t)(t.tile0 + i) * a.heads + h;
         odd |= a.eq[at] == kOdd || a.eg[at] == kOdd;
       }
   }
+  Terms k[S::NS], v[S::NS];
+  int ek, ev;
+  {
+    RowValues<DP> x;
+    x.load(a.xk + row * a.ld_xkv + (int64_t)g * a.dh, mine_in, a.dh, hi);
+    ek = x.split_into(k, a.most_score, odd);
+    x.load(a.xv + row * a.ld_xkv + (int64_t)g * a.dh, mine_in, a.dh, hi);
+    ev = x.split_into(v, a.most_value, odd);
+  }
   least = wave_min(least);
   if (lane == 0) least4[w] = least;
   if (__syncthreads_or(odd)) return false;
   least = min(min(least4[0], least4[1]), min(least4[2], least4[3]));
-
-  const bool live = k0 < t.len;
-  const int64_t kt = kv0 + (int64_t)min(k0 / kTile, last) * a.kv_heads;
-  Terms k[S::NS], v[S::NS];
-#pragma unroll
-  for (int s = 0; s < S::NS; ++s) {
-    k[s] = frag(a.k + kt * S::kBytes + S::row_frag(w & 1, s), lane);
-    v[s] = frag(a.v + kt * S::kBytes + S::row_frag(w & 1, s), lane);
-  }
-  const int ek = a.ek[kt], ev = a.ev[kt];
+  // (a row that is smaller than its tile's largest has the larger factor; one of zeros may have less)
   const float graw = __builtin_amdgcn_ldexpf(1.f, least - ev - 32), gd = __builtin_amdgcn_ldexpf(1.f, least - 32);
+  const int ro = place(hi, c), co = columns_place(lane);
 
   f16 xk[S::NB] = {}, xv[S::NB] = {};
   const int b0 = t.t0 / 32, per = (t.len + 31) / 32 - b0, n = per * a.each;
@@ -572,11 +607,9 @@ __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t
     char *to = lds + (i & 1) * kStage;
     fetch<kPart>(a.q + at, to, w, lane);
     fetch<kPart>(a.g + at, to + kPart, w, lane);
-    fetch<kPart>(a.qt + at, to + 2 * kPart, w, lane);
-    fetch<kPart>(a.gt + at, to + 3 * kPart, w, lane);
     if (w == 0)
       __builtin_amdgcn_global_load_lds((global_void *)(a.rowstat + (qt * kTile + 32 * half) * 2 + lane),
-                                       (lds_void *)(to + 4 * kPart), 4, 0, 0);
+                                       (lds_void *)(to + 2 * kPart), 4, 0, 0);
   };
   issue(0);
   for (int i = 0; i < n; ++i) {
@@ -584,13 +617,13 @@ __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t
     if (i + 1 < n) issue(i + 1);
     const int q0 = 32 * (b0 + i % per);
     if (!live || q0 + 31 < k0) continue;
-    const char *qf = lds + (i & 1) * kStage, *gf = qf + kPart, *qtf = gf + kPart, *gtf = qtf + kPart;
-    const float *rs = reinterpret_cast<const float *>(gtf + kPart);
+    const char *qf = lds + (i & 1) * kStage, *gf = qf + kPart;
+    const float *rs = reinterpret_cast<const float *>(gf + kPart);
     f16 s = {}, r = {};
 #pragma unroll
     for (int st = 0; st < S::NS; ++st) {
-      mma(s, frag(qf + S::row_frag(0, st), lane), k[st]);
-      mma(r, frag(gf + S::row_frag(0, st), lane), v[st]);
+      mma(s, rows_of(qf, st, ro), k[st]);
+      mma(r, rows_of(gf, st, ro), v[st]);
     }
     float m[16], d[16];
 #pragma unroll
@@ -601,7 +634,9 @@ __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t
     const int64_t qt = tile_of(i);
     const int eq = a.eq[qt], eg = a.eg[qt];
     f16 p, ds;
-    dscores(s, r, __builtin_amdgcn_ldexpf(a.alpha, -(eq + ek)), graw, m, d, p, ds);
+    const float f = __builtin_amdgcn_ldexpf(a.alpha, -(eq + ek));
+#pragma unroll
+    for (int e = 0; e < 16; ++e) p[e] = score(s[e], f, m[e]), ds[e] = dscore(p[e], r[e], graw, d[e]);
     if (q0 < k0 + 31) {
 #pragma unroll
       for (int e = 0; e < 16; ++e)
@@ -615,10 +650,10 @@ __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t
 #pragma unroll
     for (int nb = 0; nb < S::NB; ++nb) {
       f16 u = {}, x = {};
-      mma(u, frag(gtf + S::col_frag(0, 0, nb), lane), pb[0]);
-      mma(x, frag(qtf + S::col_frag(0, 0, nb), lane), sb[0]);
-      mma(u, frag(gtf + S::col_frag(0, 1, nb), lane), pb[1]);
-      mma(x, frag(qtf + S::col_frag(0, 1, nb), lane), sb[1]);
+      mma(u, columns_of(gf, nb, 0, co), pb[0]);
+      mma(x, columns_of(qf, nb, 0, co), sb[0]);
+      mma(u, columns_of(gf, nb, 1, co), pb[1]);
+      mma(x, columns_of(qf, nb, 1, co), sb[1]);
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         xv[nb][e] = fmaf(u[e], bv, xv[nb][e]);
@@ -626,13 +661,12 @@ __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t
       }
     }
   }
-  const int row = k0 + c;
-  if (row >= t.len) return true;
+  if (!mine_in) return true;
   // one head of several: its own part, [heads, total, dh]; else the result
   const bool part = a.each < a.heads / a.kv_heads;
-  const int64_t at = part ? ((int64_t)h0 * a.total + t.row0 + row) * a.dh : 0;
-  const int64_t ck = part ? at : (int64_t)(t.row0 + row) * a.ld_k + (int64_t)g * a.dh;
-  const int64_t cv = part ? at : (int64_t)(t.row0 + row) * a.ld_v + (int64_t)g * a.dh;
+  const int64_t at = part ? ((int64_t)h0 * a.total + row) * a.dh : 0;
+  const int64_t ck = part ? at : row * a.ld_k + (int64_t)g * a.dh;
+  const int64_t cv = part ? at : row * a.ld_v + (int64_t)g * a.dh;
   if (a.dk != nullptr) put_rows<DP>(a.dk + ck, xk, a.dh, hi, a.accumulate);
   if (a.dv != nullptr) put_rows<DP>(a.dv + cv, xv, a.dh, hi, a.accumulate);
   return true;
