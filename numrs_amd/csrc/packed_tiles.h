@@ -33,6 +33,12 @@ typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef float f16 __attribute__((ext_vector_type(16)));
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
 
+// A value that an earlier kernel left at an address that is the same in every lane: a scalar load, which
+// waits for no copy to LDS in flight.
+__device__ __forceinline__ int scalar(const int *p) {
+  return *(const __attribute__((address_space(4))) int *)p;
+}
+
 // A tile's exponent where its values do not split: one that is not finite, or so large that a
 // product might pass fp32's range.  Workgroups that meet one take the row kernels' arithmetic.
 constexpr int kOdd = 1 << 20;
@@ -327,13 +333,26 @@ __device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile
     if (i + 1 < n) issue(i + 1);
     if (i >= mine) continue;
     const char *kf = lds + (i & 1) * 2 * kStage, *vf = kf + kStage;
+    const int ek = scalar(a.ek + tile_of(i)), ev = scalar(a.ev + tile_of(i));
     f16 s[KB] = {};
+    Terms x[KB];
 #pragma unroll
-    for (int st = 0; st < S::NS; ++st)
+    for (int kb = 0; kb < KB; ++kb) x[kb] = rows_of(kf + kb * S::kHalf, 0, ro);
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) mma(s[kb], rows_of(kf + kb * S::kHalf, st, ro), q[st]);
+    for (int st = 0; st < S::NS; ++st) {
+      Terms y[KB];
+      if (st + 1 < S::NS) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) y[kb] = rows_of(kf + kb * S::kHalf, st + 1, ro);
+      }
+      __builtin_amdgcn_sched_barrier(0);  // the next step's operands are asked for before this one's products
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) mma(s[kb], x[kb], q[st]);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) x[kb] = y[kb];
+    }
     // an underflow of f must not make -inf * f NaN
-    const float f = fmaxf(__builtin_amdgcn_ldexpf(a.alpha, -(eq + a.ek[tile_of(i)])), 1.17549435e-38f);
+    const float f = fmaxf(__builtin_amdgcn_ldexpf(a.alpha, -(eq + ek)), 1.17549435e-38f);
     if ((i + 1) * KT > q0 + 1) {  // keys after a row of the wave
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
@@ -367,16 +386,23 @@ __device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile
       for (int e = 0; e < 16; ++e) x[e] = s[kb][e];
       p[kb][0] = split8(x), p[kb][1] = split8(x + 8);
     }
-    const float fv = __builtin_amdgcn_ldexpf(1.f, -a.ev[tile_of(i)]);
+    const float fv = __builtin_amdgcn_ldexpf(1.f, -ev);
+    constexpr int kSteps = 2 * KB;  // of 16 keys
+    Terms v = columns_of(vf, 0, 0, co);
 #pragma unroll
     for (int b = 0; b < S::NB; ++b) {
-      f16 x = {};
+      f16 z = {};
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
+      for (int st = 0; st < kSteps; ++st) {
+        const int nb = st + 1 < kSteps ? b : b + 1, ns = (st + 1) % kSteps;
+        Terms y;
+        if (nb < S::NB) y = columns_of(vf + (ns >> 1) * S::kHalf, nb, ns & 1, co);
+        __builtin_amdgcn_sched_barrier(0);
+        mma(z, v, p[st >> 1][st & 1]);
+        v = y;
+      }
 #pragma unroll
-        for (int st = 0; st < 2; ++st) mma(x, columns_of(vf + kb * S::kHalf, b, st, co), p[kb][st]);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) o[b][e] = fmaf(x[e], fv, o[b][e]);
+      for (int e = 0; e < 16; ++e) o[b][e] = fmaf(z[e], fv, o[b][e]);
     }
   }
   const int row = q0 + c;
@@ -434,6 +460,24 @@ __device__ __forceinline__ float score(float s, float f, float m) {
   return __builtin_amdgcn_exp2f(fmaf(s, f, 15.f - m));
 }
 __device__ __forceinline__ float dscore(float p, float raw, float graw, float d) { return p * fmaf(raw, graw, -d); }
+
+// s = A a^T and r = B b^T of 32 rows at pa and pb; the next step's operands are asked for before this
+// one's products.
+template <int DP>
+__device__ __forceinline__ void two_products(f16 &s, f16 &r, const char *pa, const char *pb, const Terms (&a)[DP / 16],
+                                             const Terms (&b)[DP / 16], int off) {
+  s = f16{}, r = f16{};
+  Terms x = rows_of(pa, 0, off), y = rows_of(pb, 0, off);
+#pragma unroll
+  for (int st = 0; st < DP / 16; ++st) {
+    Terms nx, ny;
+    if (st + 1 < DP / 16) nx = rows_of(pa, st + 1, off), ny = rows_of(pb, st + 1, off);
+    __builtin_amdgcn_sched_barrier(0);
+    mma(s, x, a[st]);
+    mma(r, y, b[st]);
+    x = nx, y = ny;
+  }
+}
 
 // Writes a wave's 32 columns of a transposed result: row `row` of the matrix at p.
 template <int DP>
@@ -520,13 +564,9 @@ __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t,
     if (i + 1 < n) issue(i + 1);
     if (i >= mine) continue;
     const char *kf = lds + (i & 1) * kStage, *vf = kf + kPart;
-    f16 s = {}, r = {};
-#pragma unroll
-    for (int st = 0; st < S::NS; ++st) {
-      mma(s, rows_of(kf, st, ro), q[st]);
-      mma(r, rows_of(vf, st, ro), go[st]);
-    }
-    const int ek = a.ek[tile_of(i)], ev = a.ev[tile_of(i)];
+    const int ek = scalar(a.ek + tile_of(i)), ev = scalar(a.ev + tile_of(i));
+    f16 s, r;
+    two_products<DP>(s, r, kf, vf, q, go, ro);
     f16 p, ds;
     const float f = __builtin_amdgcn_ldexpf(a.alpha, -(eq + ek)), graw = __builtin_amdgcn_ldexpf(1.f, least - ev - 32);
 #pragma unroll
@@ -541,13 +581,18 @@ __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t,
     for (int e = 0; e < 16; ++e) y[e] = ds[e];
     const Terms b[2] = {split8(y), split8(y + 8)};
     const float back = __builtin_amdgcn_ldexpf(a.scale, 17 - eg - least - ek);
+    Terms ka = columns_of(kf, 0, 0, co), kb = columns_of(kf, 0, 1, co);
 #pragma unroll
     for (int nb = 0; nb < S::NB; ++nb) {
+      Terms na, nc;
+      if (nb + 1 < S::NB) na = columns_of(kf, nb + 1, 0, co), nc = columns_of(kf, nb + 1, 1, co);
+      __builtin_amdgcn_sched_barrier(0);
       f16 z = {};
-      mma(z, columns_of(kf, nb, 0, co), b[0]);
-      mma(z, columns_of(kf, nb, 1, co), b[1]);
+      mma(z, ka, b[0]);
+      mma(z, kb, b[1]);
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[nb][e] = fmaf(z[e], back, x[nb][e]);
+      ka = na, kb = nc;
     }
   }
   if (mine_in) put_rows<DP>(a.dq + row * a.ld_q + (int64_t)h * a.dh, x, a.dh, hi, a.accumulate);
@@ -619,20 +664,16 @@ __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t
     if (!live || q0 + 31 < k0) continue;
     const char *qf = lds + (i & 1) * kStage, *gf = qf + kPart;
     const float *rs = reinterpret_cast<const float *>(gf + kPart);
-    f16 s = {}, r = {};
-#pragma unroll
-    for (int st = 0; st < S::NS; ++st) {
-      mma(s, rows_of(qf, st, ro), k[st]);
-      mma(r, rows_of(gf, st, ro), v[st]);
-    }
+    const int64_t qt = tile_of(i);
+    const int eq = scalar(a.eq + qt), eg = scalar(a.eg + qt);
+    f16 s, r;
+    two_products<DP>(s, r, qf, gf, k, v, ro);
     float m[16], d[16];
 #pragma unroll
     for (int e = 0; e < 16; e += 2) {
       const f4 y = *reinterpret_cast<const f4 *>(rs + 2 * out_row(e, hi));
       m[e] = y[0], d[e] = y[1] * gd, m[e + 1] = y[2], d[e + 1] = y[3] * gd;
     }
-    const int64_t qt = tile_of(i);
-    const int eq = a.eq[qt], eg = a.eg[qt];
     f16 p, ds;
     const float f = __builtin_amdgcn_ldexpf(a.alpha, -(eq + ek));
 #pragma unroll
@@ -647,13 +688,19 @@ __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t
     for (int e = 0; e < 16; ++e) y[e] = p[e], z[e] = ds[e];
     const Terms pb[2] = {split8(y), split8(y + 8)}, sb[2] = {split8(z), split8(z + 8)};
     const float bv = __builtin_amdgcn_ldexpf(1.f, -15 - eg), bk = __builtin_amdgcn_ldexpf(a.scale, 17 - eg - least - eq);
+    Terms ga = columns_of(gf, 0, 0, co), qa = columns_of(qf, 0, 0, co);
 #pragma unroll
     for (int nb = 0; nb < S::NB; ++nb) {
       f16 u = {}, x = {};
-      mma(u, columns_of(gf, nb, 0, co), pb[0]);
-      mma(x, columns_of(qf, nb, 0, co), sb[0]);
-      mma(u, columns_of(gf, nb, 1, co), pb[1]);
-      mma(x, columns_of(qf, nb, 1, co), sb[1]);
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        Terms gn, qn;
+        if (nb + st < S::NB) gn = columns_of(gf, nb + st, 1 - st, co), qn = columns_of(qf, nb + st, 1 - st, co);
+        __builtin_amdgcn_sched_barrier(0);
+        mma(u, ga, pb[st]);
+        mma(x, qa, sb[st]);
+        ga = gn, qa = qn;
+      }
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         xv[nb][e] = fmaf(u[e], bv, xv[nb][e]);
