@@ -251,18 +251,27 @@ __global__ void __launch_bounds__(256) pack(PackArgs a) {
   }
 }
 
-typedef __attribute__((address_space(3))) void lds_void;
-typedef const __attribute__((address_space(1))) void global_void;
+// Copies 64 lanes' 16 (or 4) bytes, each from the lane's address, to 64 consecutive places of LDS,
+// without passing through registers.  As an instruction of its own: the compiler's form is waited for
+// before any later LDS access, whichever place that reads.  There is no output register, and the
+// compiler's waits on its own loads only grow longer by these.
+__device__ __forceinline__ void copy16(const void *src, const void *lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src),
+               "s"((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)lds)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void copy4(const void *src, const void *lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src),
+               "s"((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)lds)
+               : "memory", "m0");
+}
 
-// Copies `bytes` (a multiple of 4096) of fragments to LDS without passing through registers: wave w
-// of four has every fourth kilobyte.
+// Copies `bytes` (a multiple of 4096) of fragments to LDS: wave w of four has every fourth kilobyte.
 template <int BYTES>
 __device__ __forceinline__ void fetch(const char *src, char *lds, int w, int lane) {
   static_assert(BYTES % 4096 == 0);
 #pragma unroll
-  for (int i = 0; i < BYTES / 4096; ++i)
-    __builtin_amdgcn_global_load_lds((global_void *)(src + (i * 4 + w) * 1024 + lane * 16),
-                                     (lds_void *)(lds + (i * 4 + w) * 1024), 16, 0, 0);
+  for (int i = 0; i < BYTES / 4096; ++i) copy16(src + (i * 4 + w) * 1024 + lane * 16, lds + (i * 4 + w) * 1024);
 }
 
 // Waits for this wave's copies, then for the other waves': what any of them fetched is there.
@@ -653,8 +662,7 @@ __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t
     fetch<kPart>(a.q + at, to, w, lane);
     fetch<kPart>(a.g + at, to + kPart, w, lane);
     if (w == 0)
-      __builtin_amdgcn_global_load_lds((global_void *)(a.rowstat + (qt * kTile + 32 * half) * 2 + lane),
-                                       (lds_void *)(to + 2 * kPart), 4, 0, 0);
+      copy4(a.rowstat + (qt * kTile + 32 * half) * 2 + lane, to + 2 * kPart);
   };
   issue(0);
   for (int i = 0; i < n; ++i) {
