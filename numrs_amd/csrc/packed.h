@@ -25,6 +25,7 @@ struct Seqs {
   SeqTile *in_order = nullptr;  // [tiles]; a tile's number is its place
   SeqTile *by_work = nullptr;   // [blocks] of 128 tokens, those with the most tokens before them first
   SeqTile *by_rest = nullptr;   // [blocks], those with the most tokens after them first
+  SeqTile *few_by_work = nullptr, *few_by_rest = nullptr;  // the same of the tiles
   size_t bytes = 0;
   ~Seqs() { block_free(ctx, in_order, bytes); }
 };

@@ -78,15 +78,14 @@ __device__ void row_forward(const FwdArgs &a, const SeqTile &t, int r, int h, fl
 
 constexpr int kRows = 4;  // waves of a workgroup
 
-// A block of 128 query rows of one head.
-template <int DP>
+// A block of query rows of one head.
+template <int DP, int Z>
 __global__ void __launch_bounds__(256, 2) forward_block(FwdArgs a, tiles::ForwardArgs f) {
-  constexpr int KT = DP <= 64 ? 64 : 32;
-  __shared__ __attribute__((aligned(16))) char lds[4 * KT * DP * 4];
+  __shared__ __attribute__((aligned(16))) char lds[tiles::Walk<DP, Z>::kForward];
   const SeqTile t = a.tiles[blockIdx.x / a.heads];
   const int h = blockIdx.x % a.heads;
-  if (tiles::forward_tile<DP>(f, t, h, lds)) return;
-  const int w = threadIdx.x >> 6, end = min(t.len, t.t0 + 128);
+  if (tiles::forward_tile<DP, Z>(f, t, h, lds)) return;
+  const int w = threadIdx.x >> 6, end = min(t.len, t.t0 + 128 / Z);
   for (int r = t.t0 + w; r < end; r += kRows) row_forward(a, t, r, h, reinterpret_cast<float *>(lds) + 128 * w);
 }
 
@@ -182,26 +181,26 @@ __device__ void row_dkv(const BwdArgs &b, const tiles::BackwardArgs &a, const Se
   }
 }
 
-// A block of 128 query rows of one head.
-template <int DP>
+// A block of query rows of one head.
+template <int DP, int Z>
 __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) dq_block(BwdArgs b, tiles::BackwardArgs a) {
-  __shared__ __attribute__((aligned(16))) char lds[2 * 2 * 32 * DP * 4];
+  __shared__ __attribute__((aligned(16))) char lds[tiles::Walk<DP, Z>::kBack];
   const SeqTile t = b.tiles[blockIdx.x / a.heads];
   const int h = blockIdx.x % a.heads;
-  if (tiles::dq_tile<DP>(a, t, h, lds)) return;
-  const int w = threadIdx.x >> 6, end = min(t.len, t.t0 + 128);
+  if (tiles::dq_tile<DP, Z>(a, t, h, lds)) return;
+  const int w = threadIdx.x >> 6, end = min(t.len, t.t0 + 128 / Z);
   for (int r = t.t0 + w; r < end; r += kRows) row_dq(b, a, t, r, h, reinterpret_cast<float *>(lds) + 256 * w);
 }
 
-// A block of 128 key rows of one kv head, or one query head's part of it.
-template <int DP>
+// A block of key rows of one kv head, or one query head's part of it.
+template <int DP, int Z>
 __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) dkv_block(BwdArgs b, tiles::BackwardArgs a) {
-  __shared__ __attribute__((aligned(16))) char lds[2 * (2 * 32 * DP * 4 + 256)];
+  __shared__ __attribute__((aligned(16))) char lds[tiles::Walk<DP, Z>::kBack];
   const int slots = a.heads / a.each;
   const SeqTile t = b.tiles[blockIdx.x / slots];
   const int h0 = blockIdx.x % slots * a.each;
-  if (tiles::dkv_tile<DP>(a, t, h0, lds)) return;
-  const int w = threadIdx.x >> 6, end = min(t.len, t.t0 + 128);
+  if (tiles::dkv_tile<DP, Z>(a, t, h0, lds)) return;
+  const int w = threadIdx.x >> 6, end = min(t.len, t.t0 + 128 / Z);
   for (int r = t.t0 + w; r < end; r += kRows) row_dkv(b, a, t, r, h0, reinterpret_cast<float *>(lds) + 256 * w);
 }
 
@@ -242,6 +241,13 @@ int check_packed(numrs_hip_ctx *ctx, const Seqs &s, int64_t ld_q, int64_t ld_kv,
 // Magnitudes from which a tile's products might pass fp32's range: a score of two such operands
 // stays below 2^107, a sum of 2^20 such values times 2^15 below 2^127.
 constexpr float kMostScore = 0x1p50f, kMostValue = 0x1p90f;
+
+// Whether the kernels take blocks of 64 rows whose keys two sets of waves share, in place of 128: where
+// there are fewer than two of the latter for each CU, and the longest walk decides.  Forward | query rows |
+// key rows on MI355X, 128 rows against 64, us: 256 blocks (16 x 256 tokens, 8 heads of 64) 14.2, 13.2 |
+// 19.0, 18.2 | 26.3, 22.9; 260 (2736 tokens, 10 heads of 80) 46, 35 | 63, 46 | 86, 57; 752 (5023 tokens, 16
+// heads of 64) 47, 47; 1024 (2 x 4096 tokens, 16 heads of 128) 403, 570 | 659, 739 | 978, 987.
+bool few_blocks(numrs_hip_ctx *ctx, const Seqs &s, int heads) { return s.blocks * heads < 2 * ctx->num_cus; }
 
 int padded(int dh) { return (dh + 31) / 32 * 32; }
 
@@ -294,13 +300,20 @@ int packed_forward(numrs_hip_ctx *ctx, const Seqs &s, const float *q, int64_t ld
                           2 * Hk, dh};
   const float alpha = kLog2e / std::sqrt((float)dh);
   const FwdArgs a{s.by_work, q, k, v, out, stats, ld_q, ld_kv, ld_out, H, Hk, dh, alpha};
+  const bool few = few_blocks(ctx, s, H);
   const tiles::ForwardArgs f{q, pk.rows, pv.rows, pk.exps, pv.exps, out, stats, ld_q, ld_out,
                              H, Hk, dh, alpha, kMostScore};
   return with_dp(dh, [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
     tiles::pack<DP><<<(unsigned)(s.tiles * p.slots), 256, 0, ctx->stream>>>(p);
     if (int rc = check_launch(ctx, "pack")) return rc;
-    forward_block<DP><<<(unsigned)(s.blocks * H), 256, 0, ctx->stream>>>(a, f);
+    FwdArgs b = a;
+    if (few) {
+      b.tiles = s.few_by_work;
+      forward_block<DP, 2><<<(unsigned)(s.tiles * H), 256, 0, ctx->stream>>>(b, f);
+    } else {
+      forward_block<DP, 1><<<(unsigned)(s.blocks * H), 256, 0, ctx->stream>>>(b, f);
+    }
     return check_launch(ctx, "forward_block");
   });
 }
@@ -340,7 +353,8 @@ int packed_backward(numrs_hip_ctx *ctx, const Seqs &s, const float *q, int64_t l
                     2 * Hk + (keys ? 2 * H : 0), dh};
   p.src[3].out = out, p.src[3].stats = stats, p.src[3].rowstat = rowstat.f();
   const float alpha = kLog2e / std::sqrt((float)dh), scale = 1.0f / std::sqrt((float)dh);
-  BwdArgs b{s.by_work, q, k, v, out, dout, stats, ld_q, ld_kv, ld_out};
+  const bool few = few_blocks(ctx, s, H);
+  BwdArgs b{few ? s.few_by_work : s.by_work, q, k, v, out, dout, stats, ld_q, ld_kv, ld_out};
   tiles::BackwardArgs a{q, k, v, out, dout, stats, ld_q, ld_kv, ld_out, pq.rows, pk.rows, pv.rows, pg.rows,
                         pq.exps, pk.exps, pv.exps, pg.exps, rowstat.f(), dq, dk, dv, ld_q, ld_kv, ld_kv, s.total,
                         H, Hk, dh, accumulate, each, alpha, scale, kMostScore, kMostValue};
@@ -349,17 +363,23 @@ int packed_backward(numrs_hip_ctx *ctx, const Seqs &s, const float *q, int64_t l
     tiles::pack<DP><<<(unsigned)(s.tiles * p.slots), 256, 0, ctx->stream>>>(p);
     if (int rc = check_launch(ctx, "pack")) return rc;
     if (dq != nullptr) {
-      dq_block<DP><<<(unsigned)(s.blocks * H), 256, 0, ctx->stream>>>(b, a);
+      if (few)
+        dq_block<DP, 2><<<(unsigned)(s.tiles * H), 256, 0, ctx->stream>>>(b, a);
+      else
+        dq_block<DP, 1><<<(unsigned)(s.blocks * H), 256, 0, ctx->stream>>>(b, a);
       if (int rc = check_launch(ctx, "dq_block")) return rc;
     }
     if (!keys) return (int)NUMRS_HIP_OK;
-    b.tiles = s.by_rest;
+    b.tiles = few ? s.few_by_rest : s.by_rest;
     if (each < group) {
       a.dk = dk != nullptr ? parts.f() : nullptr;
       a.dv = dv != nullptr ? parts.f() + (dk != nullptr ? part / sizeof(float) : 0) : nullptr;
       a.accumulate = 0;
     }
-    dkv_block<DP><<<(unsigned)(s.blocks * (H / each)), 256, 0, ctx->stream>>>(b, a);
+    if (few)
+      dkv_block<DP, 2><<<(unsigned)(s.tiles * (H / each)), 256, 0, ctx->stream>>>(b, a);
+    else
+      dkv_block<DP, 1><<<(unsigned)(s.blocks * (H / each)), 256, 0, ctx->stream>>>(b, a);
     if (int rc = check_launch(ctx, "dkv_block")) return rc;
     if (each < group) {
       const unsigned grid = grid_for(s.total * Hk * (dh / 4), 256);
@@ -410,20 +430,24 @@ int numrs_hip_seqs_create(numrs_hip_ctx *ctx, const int64_t *lengths, int64_t n,
     std::vector<SeqTile> blocks;
     for (const SeqTile &t : tiles)
       if (t.t0 % 128 == 0) blocks.push_back(t);
-    std::stable_sort(blocks.begin(), blocks.end(), [](const SeqTile &a, const SeqTile &b) { return a.t0 > b.t0; });
     s->blocks = (int64_t)blocks.size();
-    tiles.insert(tiles.end(), blocks.begin(), blocks.end());
-    std::stable_sort(blocks.begin(), blocks.end(),
-                     [](const SeqTile &a, const SeqTile &b) { return a.len - a.t0 > b.len - b.t0; });
-    tiles.insert(tiles.end(), blocks.begin(), blocks.end());
+    std::vector<SeqTile> lists = tiles;
+    auto add = [&](std::vector<SeqTile> &list, bool rest) {
+      std::stable_sort(list.begin(), list.end(), [=](const SeqTile &a, const SeqTile &b) {
+        return rest ? a.len - a.t0 > b.len - b.t0 : a.t0 > b.t0;
+      });
+      lists.insert(lists.end(), list.begin(), list.end());
+    };
+    add(blocks, false), add(blocks, true), add(tiles, false), add(tiles, true);
     auto h = std::make_unique<numrs_hip_seqs>();
-    if (!tiles.empty()) {
+    if (!lists.empty()) {
       void *p = nullptr;
-      const size_t bytes = tiles.size() * sizeof(SeqTile);
+      const size_t bytes = lists.size() * sizeof(SeqTile);
       if (int rc = block_alloc(ctx, bytes, &p)) return rc;
       s->in_order = static_cast<SeqTile *>(p), s->bytes = bytes;
       s->by_work = s->in_order + s->tiles, s->by_rest = s->by_work + s->blocks;
-      if (int rc = numrs_hip_upload(ctx, p, tiles.data(), bytes)) return rc;
+      s->few_by_work = s->by_rest + s->blocks, s->few_by_rest = s->few_by_work + s->tiles;
+      if (int rc = numrs_hip_upload(ctx, p, lists.data(), bytes)) return rc;
     }
     h->s = std::move(s);
     *out = h.release();

@@ -42,6 +42,8 @@ __device__ __forceinline__ int scalar(const int *p) {
 // A tile's exponent where its values do not split: one that is not finite, or so large that a
 // product might pass fp32's range.  Workgroups that meet one take the row kernels' arithmetic.
 constexpr int kOdd = 1 << 20;
+// A softmax reference before any score: below every score of a tile that is not odd.
+constexpr float kNone = -0x1p110f;
 
 // x = h + m of a pair.
 __device__ __forceinline__ void split(float a, float b, unsigned &h, unsigned &m) {
@@ -300,18 +302,64 @@ struct ForwardArgs {
   float alpha, most;  // log2(e) / sqrt(dh); a query's largest magnitude
 };
 
-// Four waves own 32 query rows each of a block of 128 and walk the keys before them.  S^T = K Q^T
-// leaves a query's scores in two lanes; p = 2^(s - m + 7) against a reference m that moves only
-// when a score passes it by 2^8 (so that p fits fp16), O^T += V^T P^T.
+// Four waves walk the keys before a block of query rows: Z = 1, one stretch of keys for 32 rows a wave
+// (128); Z = 2, two sets of waves with every other 32 keys each for 64 rows, joined at the end, where
+// there are few blocks and the longest walk decides.  Keys staged at a time: 64, or 32.
+template <int DP, int Z>
+struct Walk {
+  static constexpr int R = 4 / Z;                                // waves with rows of their own
+  static constexpr int KT = Z == 2 || DP <= 64 ? 64 : 32;        // the forward's stage
+  static constexpr int KB = KT / 32 / Z;                         // 32-key blocks of a wave
+  static constexpr int kForward = 4 * KT * DP * 4;               // LDS: two stages of keys and values
+  static constexpr int kBack = 2 * (2 * Z * 32 * DP * 4 + 256 * Z);  // and the backward's
+};
+
+// Adds the second set's results to the first's, through LDS: every lane N vectors of 16.  Returns whether
+// the wave is of the first set.
+template <int Z, int N>
+__device__ __forceinline__ void join_sets(f16 *const (&x)[N], char *lds, int r, int z, int lane) {
+  if constexpr (Z == 2) {
+    __syncthreads();
+    f4 *p = reinterpret_cast<f4 *>(lds) + (int64_t)r * N * 4 * 64 + lane;
+    if (z == 1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          f4 y;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) y[j] = (*x[i])[4 * e + j];
+          p[(4 * i + e) * 64] = y;
+        }
+    }
+    __syncthreads();
+    if (z == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const f4 y = p[(4 * i + e) * 64];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) (*x[i])[4 * e + j] += y[j];
+        }
+    }
+  }
+}
+
+// S^T = K Q^T leaves a query's scores in two lanes; p = 2^(s - m + 7) against a reference m that moves
+// only when a score passes it by 2^8 (so that p fits fp16), O^T += V^T P^T.
 //
 // Returns false, before any write, where a tile is odd.
-template <int DP>
+template <int DP, int Z>
 __device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile &t, int h, char *lds) {
   using S = Shape<DP>;
-  constexpr int KT = DP <= 64 ? 64 : 32, KB = KT / 32, kStage = KT * DP * 4;
+  using W = Walk<DP, Z>;
+  constexpr int KT = W::KT, KB = W::KB, kStage = KT * DP * 4;
+  __shared__ float joint[Z == 2 ? 3 : 1][64];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rw = w % W::R, z = w / W::R;
   const int c = lane & 31, hi = lane >> 5, g = h / (a.heads / a.kv_heads);
-  const int end = min(t.t0 + 128, t.len), q0 = t.t0 + 32 * w;
+  const int end = min(t.t0 + 32 * W::R, t.len), q0 = t.t0 + 32 * rw;
   const int64_t kv0 = (int64_t)t.tile0 * a.kv_heads + g;  // the sequence's first tile of this head
   const int last = (end - 1) / kTile;
   Terms q[S::NS];
@@ -326,7 +374,7 @@ __device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile
   const int ro = place(hi, c), co = columns_place(lane);
 
   f16 o[S::NB] = {};
-  float m = -INFINITY, top = -INFINITY, l = 0.f;
+  float m = kNone, top = kNone, l = 0.f;
   const int n = (end + KT - 1) / KT;              // key blocks of the workgroup
   const int mine = live ? (q0 + 31) / KT + 1 : 0;  // and of the wave
   auto tile_of = [&](int i) { return kv0 + (int64_t)(i * KT / kTile) * a.kv_heads; };
@@ -341,7 +389,9 @@ __device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile
     fetched();
     if (i + 1 < n) issue(i + 1);
     if (i >= mine) continue;
-    const char *kf = lds + (i & 1) * 2 * kStage, *vf = kf + kStage;
+    const char *kf = lds + (i & 1) * 2 * kStage + z * S::kHalf, *vf = kf + kStage;
+    const int key0 = i * KT + 32 * z;
+    if (key0 > q0 + 31) continue;  // all after the wave's rows
     const int ek = scalar(a.ek + tile_of(i)), ev = scalar(a.ev + tile_of(i));
     f16 s[KB] = {};
     Terms x[KB];
@@ -362,12 +412,12 @@ __device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile
     }
     // an underflow of f must not make -inf * f NaN
     const float f = fmaxf(__builtin_amdgcn_ldexpf(a.alpha, -(eq + ek)), 1.17549435e-38f);
-    if ((i + 1) * KT > q0 + 1) {  // keys after a row of the wave
+    if (key0 + 32 * KB > q0 + 1) {  // keys after a row of the wave
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (i * KT + 32 * kb + out_row(e, hi) > q0 + c) s[kb][e] = -INFINITY;
+          if (key0 + 32 * kb + out_row(e, hi) > q0 + c) s[kb][e] = -INFINITY;
     }
     float most = over16(s[0], [](float x, float y) { return fmaxf(x, y); });
     if constexpr (KB == 2) most = fmaxf(most, over16(s[1], [](float x, float y) { return fmaxf(x, y); }));
@@ -417,6 +467,27 @@ __device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile
   const int row = q0 + c;
   l = half_pair(l, [](float x, float y) { return x + y; });
   top = half_pair(top, [](float x, float y) { return fmaxf(x, y); });
+  if constexpr (Z == 2) {
+    // both sets relative to the larger reference
+    __syncthreads();
+    if (z == 1 && hi == 0) joint[0][32 * rw + c] = m, joint[1][32 * rw + c] = l, joint[2][32 * rw + c] = top;
+    if (z == 0 && hi == 0) reinterpret_cast<float *>(lds)[32 * rw + c] = m;
+    __syncthreads();
+    const float m0 = reinterpret_cast<float *>(lds)[32 * rw + c], m1 = joint[0][32 * rw + c];
+    const float now = fmaxf(m0, m1), f = __builtin_amdgcn_exp2f(m - now);
+#pragma unroll
+    for (int b = 0; b < S::NB; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[b][e] *= f;
+    l = fmaf(l, f, z == 0 ? joint[1][32 * rw + c] * __builtin_amdgcn_exp2f(m1 - now) : 0.f);
+    top = fmaxf(top, joint[2][32 * rw + c]);
+    m = now;
+    f16 *all[S::NB];
+#pragma unroll
+    for (int b = 0; b < S::NB; ++b) all[b] = &o[b];
+    join_sets<Z>(all, lds, rw, z, lane);
+    if (z == 1) return true;
+  }
   if (row >= t.len) return true;
   const float inv = 1.f / l;
   float *p = a.out + (int64_t)(t.row0 + row) * a.ld_out + (int64_t)h * a.dh;
@@ -506,16 +577,17 @@ __device__ __forceinline__ void put_rows(float *p, const f16 (&x)[DP / 32], int 
     }
 }
 
-// dQ of 128 query rows of a head: like the forward, with S^T and dP^T of 32 keys at a time, dQ^T +=
-// K^T dS^T.  Returns false, before any write, where a tile is odd.
-template <int DP>
+// dQ of a block of query rows of a head: like the forward, with S^T and dP^T of 32 keys at a time, dQ^T
+// += K^T dS^T.  Returns false, before any write, where a tile is odd.
+template <int DP, int Z>
 __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t, int h, char *lds) {
   using S = Shape<DP>;
-  constexpr int kPart = S::kHalf, kStage = 2 * kPart;
+  constexpr int R = 4 / Z, kPart = Z * S::kHalf, kStage = 2 * kPart;
   __shared__ int least4[4];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rw = w % R, z = w / R;
   const int c = lane & 31, hi = lane >> 5, g = h / (a.heads / a.kv_heads);
-  const int end = min(t.t0 + 128, t.len), q0 = t.t0 + 32 * w;
+  const int end = min(t.t0 + 32 * R, t.len), q0 = t.t0 + 32 * rw;
   const int64_t kv0 = (int64_t)t.tile0 * a.kv_heads + g, row = t.row0 + q0 + c;
   const int last = (end - 1) / kTile;
   const bool live = q0 < t.len, mine_in = q0 + c < t.len;
@@ -559,10 +631,10 @@ __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t,
   const int ro = place(hi, c), co = columns_place(lane);
 
   f16 x[S::NB] = {};
-  const int n = (end + 31) / 32, mine = live ? q0 / 32 + 1 : 0;
-  auto tile_of = [&](int i) { return kv0 + (int64_t)(i >> 1) * a.kv_heads; };
+  const int n = (end + 32 * Z - 1) / (32 * Z), mine = live ? q0 / 32 + 1 : 0;  // blocks of 32 Z keys, of 32
+  auto tile_of = [&](int i) { return kv0 + (int64_t)(i * Z >> 1) * a.kv_heads; };
   auto issue = [&](int i) {
-    const int64_t at = tile_of(i) * S::kBytes + (i & 1) * kPart;
+    const int64_t at = tile_of(i) * S::kBytes + (i * Z & 1) * kPart;
     char *to = lds + (i & 1) * kStage;
     fetch<kPart>(a.k + at, to, w, lane);
     fetch<kPart>(a.v + at, to + kPart, w, lane);
@@ -571,8 +643,9 @@ __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t,
   for (int i = 0; i < n; ++i) {
     fetched();
     if (i + 1 < n) issue(i + 1);
-    if (i >= mine) continue;
-    const char *kf = lds + (i & 1) * kStage, *vf = kf + kPart;
+    const int kb = i * Z + z;  // the wave's 32 keys
+    if (kb >= mine) continue;
+    const char *kf = lds + (i & 1) * kStage + z * S::kHalf, *vf = kf + kPart;
     const int ek = scalar(a.ek + tile_of(i)), ev = scalar(a.ev + tile_of(i));
     f16 s, r;
     two_products<DP>(s, r, kf, vf, q, go, ro);
@@ -580,44 +653,49 @@ __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t,
     const float f = __builtin_amdgcn_ldexpf(a.alpha, -(eq + ek)), graw = __builtin_amdgcn_ldexpf(1.f, least - ev - 32);
 #pragma unroll
     for (int e = 0; e < 16; ++e) p[e] = score(s[e], f, m), ds[e] = dscore(p[e], r[e], graw, D);
-    if (32 * i + 31 > q0) {
+    if (32 * kb + 31 > q0) {
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        if (32 * i + out_row(e, hi) > q0 + c) ds[e] = 0.f;
+        if (32 * kb + out_row(e, hi) > q0 + c) ds[e] = 0.f;
     }
     float y[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) y[e] = ds[e];
     const Terms b[2] = {split8(y), split8(y + 8)};
     const float back = __builtin_amdgcn_ldexpf(a.scale, 17 - eg - least - ek);
-    Terms ka = columns_of(kf, 0, 0, co), kb = columns_of(kf, 0, 1, co);
+    Terms k0 = columns_of(kf, 0, 0, co), k1 = columns_of(kf, 0, 1, co);
 #pragma unroll
     for (int nb = 0; nb < S::NB; ++nb) {
       Terms na, nc;
       if (nb + 1 < S::NB) na = columns_of(kf, nb + 1, 0, co), nc = columns_of(kf, nb + 1, 1, co);
       __builtin_amdgcn_sched_barrier(0);
-      f16 z = {};
-      mma(z, ka, b[0]);
-      mma(z, kb, b[1]);
+      f16 u = {};
+      mma(u, k0, b[0]);
+      mma(u, k1, b[1]);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[nb][e] = fmaf(z[e], back, x[nb][e]);
-      ka = na, kb = nc;
+      for (int e = 0; e < 16; ++e) x[nb][e] = fmaf(u[e], back, x[nb][e]);
+      k0 = na, k1 = nc;
     }
   }
-  if (mine_in) put_rows<DP>(a.dq + row * a.ld_q + (int64_t)h * a.dh, x, a.dh, hi, a.accumulate);
+  f16 *sets[S::NB];
+#pragma unroll
+  for (int b = 0; b < S::NB; ++b) sets[b] = &x[b];
+  join_sets<Z>(sets, lds, rw, z, lane);
+  if (mine_in && z == 0) put_rows<DP>(a.dq + row * a.ld_q + (int64_t)h * a.dh, x, a.dh, hi, a.accumulate);
   return true;
 }
 
-// dK and dV of 128 key rows: four waves own 32 keys each and walk the queries from theirs on, for
+// dK and dV of a block of key rows: the waves own 32 keys each and walk the queries from theirs on, for
 // each query head in turn: S = Q K^T and dP = dO V^T of 32 queries, dV^T += dO^T P, dK^T += Q^T dS.
-template <int DP>
+template <int DP, int Z>
 __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t, int h0, char *lds) {
   using S = Shape<DP>;
-  constexpr int kPart = S::kHalf, kStage = 2 * kPart + 256;
+  constexpr int R = 4 / Z, kPart = Z * S::kHalf, kStage = 2 * kPart + 256 * Z;
   __shared__ int least4[4];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rw = w % R, z = w / R;
   const int c = lane & 31, hi = lane >> 5, g = h0 / (a.heads / a.kv_heads);
-  const int k0 = t.t0 + 32 * w;
+  const int k0 = t.t0 + 32 * rw;
   const int64_t kv0 = (int64_t)t.tile0 * a.kv_heads + g, row = t.row0 + k0 + c;
   const int first = t.t0 / kTile, all = (t.len - 1) / kTile;
   const bool live = k0 < t.len, mine_in = k0 + c < t.len;
@@ -651,27 +729,27 @@ __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t
   const int ro = place(hi, c), co = columns_place(lane);
 
   f16 xk[S::NB] = {}, xv[S::NB] = {};
-  const int b0 = t.t0 / 32, per = (t.len + 31) / 32 - b0, n = per * a.each;
+  // stages of 32 Z queries
+  const int b0 = t.t0 / (32 * Z), per = (t.len + 32 * Z - 1) / (32 * Z) - b0, n = per * a.each;
   auto tile_of = [&](int i) {  // the query tile of stage i
-    return (int64_t)(t.tile0 + (b0 + i % per) / 2) * a.heads + h0 + i / per;
+    return (int64_t)(t.tile0 + (b0 + i % per) * Z / 2) * a.heads + h0 + i / per;
   };
   auto issue = [&](int i) {
-    const int half = (b0 + i % per) & 1;
+    const int half = (b0 + i % per) * Z & 1;
     const int64_t qt = tile_of(i), at = qt * S::kBytes + half * kPart;
     char *to = lds + (i & 1) * kStage;
     fetch<kPart>(a.q + at, to, w, lane);
     fetch<kPart>(a.g + at, to + kPart, w, lane);
-    if (w == 0)
-      copy4(a.rowstat + (qt * kTile + 32 * half) * 2 + lane, to + 2 * kPart);
+    if (w < Z) copy4(a.rowstat + (qt * kTile + 32 * (half + w)) * 2 + lane, to + 2 * kPart + 256 * w);
   };
   issue(0);
   for (int i = 0; i < n; ++i) {
     fetched();
     if (i + 1 < n) issue(i + 1);
-    const int q0 = 32 * (b0 + i % per);
-    if (!live || q0 + 31 < k0) continue;
-    const char *qf = lds + (i & 1) * kStage, *gf = qf + kPart;
-    const float *rs = reinterpret_cast<const float *>(gf + kPart);
+    const int q0 = 32 * ((b0 + i % per) * Z + z);
+    if (!live || q0 + 31 < k0 || q0 >= t.len) continue;
+    const char *stage = lds + (i & 1) * kStage, *qf = stage + z * S::kHalf, *gf = qf + kPart;
+    const float *rs = reinterpret_cast<const float *>(stage + 2 * kPart + 256 * z);
     const int64_t qt = tile_of(i);
     const int eq = scalar(a.eq + qt), eg = scalar(a.eg + qt);
     f16 s, r;
@@ -716,7 +794,11 @@ __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t
       }
     }
   }
-  if (!mine_in) return true;
+  f16 *sets[2 * S::NB];
+#pragma unroll
+  for (int b = 0; b < S::NB; ++b) sets[2 * b] = &xk[b], sets[2 * b + 1] = &xv[b];
+  join_sets<Z>(sets, lds, rw, z, lane);
+  if (!mine_in || z != 0) return true;
   // one head of several: its own part, [heads, total, dh]; else the result
   const bool part = a.each < a.heads / a.kv_heads;
   const int64_t at = part ? ((int64_t)h0 * a.total + row) * a.dh : 0;

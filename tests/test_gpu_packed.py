@@ -122,7 +122,11 @@ class _Call:
 SHAPES = [([1], 1, 1, 8), ([3, 0, 5, 0], 2, 1, 16), ([64], 8, 8, 64), ([65, 63, 1, 33], 4, 2, 40),
           ([127, 129], 6, 3, 80), ([300, 1, 257], 8, 2, 128), ([513], 5, 1, 96), ([200, 31], 4, 4, 72),
           ([777], 3, 1, 64), ([255, 256], 2, 2, 32), ([1, 2, 3, 4, 5, 6, 7] * 5, 16, 1, 24),
-          ([640], 16, 4, 64), ([400, 1, 1, 90], 2, 1, 104), ([1100, 60], 4, 2, 128)]
+          ([640], 16, 4, 64), ([400, 1, 1, 90], 2, 1, 104), ([1100, 60], 4, 2, 128),
+          # enough blocks of 128 rows for two a CU, of each padded size; and enough blocks of key rows
+          # that a workgroup takes all heads of a group
+          ([140] * 20, 16, 4, 64), ([260] * 8, 24, 8, 128), ([131] * 18, 16, 16, 96), ([100, 300] * 9, 16, 8, 32),
+          ([5, 33] * 150, 16, 4, 24)]
 
 
 @pytest.mark.parametrize("lengths,H,Hk,dh", SHAPES)
