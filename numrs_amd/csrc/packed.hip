@@ -172,51 +172,57 @@ __device__ void row_dkv(const BwdArgs &b, const tiles::BackwardArgs &a, const Se
   const int64_t ck = a.each < group ? part : row * a.ld_k + (int64_t)g * a.dh;
   const int64_t cv = a.each < group ? part : row * a.ld_v + (int64_t)g * a.dh;
   if (a.dk != nullptr) {
-    if (lane < a.dh) put(a.dk + ck + lane, k0 * a.scale, a.accumulate);
-    if (lane + 64 < a.dh) put(a.dk + ck + lane + 64, k1 * a.scale, a.accumulate);
+    if (lane < a.dh) put(a.dk + ck + lane, k0 * a.scale, a.acc_kv);
+    if (lane + 64 < a.dh) put(a.dk + ck + lane + 64, k1 * a.scale, a.acc_kv);
   }
   if (a.dv != nullptr) {
-    if (lane < a.dh) put(a.dv + cv + lane, v0, a.accumulate);
-    if (lane + 64 < a.dh) put(a.dv + cv + lane + 64, v1, a.accumulate);
+    if (lane < a.dh) put(a.dv + cv + lane, v0, a.acc_kv);
+    if (lane + 64 < a.dh) put(a.dv + cv + lane + 64, v1, a.acc_kv);
   }
 }
 
-// A block of query rows of one head.
+// The backward's blocks in one launch, so that each kind's last workgroups run beside the other's: first
+// `keys` workgroups with a block of key rows of one kv head, or one query head's part of it, then a block of
+// query rows of one head each.
 template <int DP, int Z>
-__global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) dq_block(BwdArgs b, tiles::BackwardArgs a) {
+__global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1)
+    backward_block(BwdArgs b, tiles::BackwardArgs a, const SeqTile *key_tiles, unsigned keys) {
   __shared__ __attribute__((aligned(16))) char lds[tiles::Walk<DP, Z>::kBack];
-  const SeqTile t = b.tiles[blockIdx.x / a.heads];
-  const int h = blockIdx.x % a.heads;
-  if (tiles::dq_tile<DP, Z>(a, t, h, lds)) return;
-  const int w = threadIdx.x >> 6, end = min(t.len, t.t0 + 128 / Z);
-  for (int r = t.t0 + w; r < end; r += kRows) row_dq(b, a, t, r, h, reinterpret_cast<float *>(lds) + 256 * w);
+  const int w = threadIdx.x >> 6;
+  float *row = reinterpret_cast<float *>(lds) + 256 * w;
+  if (blockIdx.x < keys) {
+    const int slots = a.heads / a.each;
+    const SeqTile t = key_tiles[blockIdx.x / slots];
+    const int h0 = blockIdx.x % slots * a.each;
+    if (tiles::dkv_tile<DP, Z>(a, t, h0, lds)) return;
+    for (int r = t.t0 + w; r < min(t.len, t.t0 + 128 / Z); r += kRows) row_dkv(b, a, t, r, h0, row);
+  } else {
+    const unsigned i = blockIdx.x - keys;
+    const SeqTile t = b.tiles[i / a.heads];
+    const int h = i % a.heads;
+    if (tiles::dq_tile<DP, Z>(a, t, h, lds)) return;
+    for (int r = t.t0 + w; r < min(t.len, t.t0 + 128 / Z); r += kRows) row_dq(b, a, t, r, h, row);
+  }
 }
 
-// A block of key rows of one kv head, or one query head's part of it.
-template <int DP, int Z>
-__global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) dkv_block(BwdArgs b, tiles::BackwardArgs a) {
-  __shared__ __attribute__((aligned(16))) char lds[tiles::Walk<DP, Z>::kBack];
-  const int slots = a.heads / a.each;
-  const SeqTile t = b.tiles[blockIdx.x / slots];
-  const int h0 = blockIdx.x % slots * a.each;
-  if (tiles::dkv_tile<DP, Z>(a, t, h0, lds)) return;
-  const int w = threadIdx.x >> 6, end = min(t.len, t.t0 + 128 / Z);
-  for (int r = t.t0 + w; r < end; r += kRows) row_dkv(b, a, t, r, h0, reinterpret_cast<float *>(lds) + 256 * w);
-}
-
-// Adds the parts of a group's query heads in order, four values a thread: part [heads, total, dh].
+// Adds the parts of a group's query heads in order, four values a thread: part [heads, total, dh]; dk's and
+// dv's by the grid's second index.
+struct Join {
+  const float *part[2];
+  float *out[2];
+};
 __global__ void __launch_bounds__(256)
-    join_heads(const float *part, float *out, int64_t ld, int64_t total, int heads, int kv_heads, int dh,
-               int accumulate) {
+    join_heads(Join j, int64_t ld, int64_t total, int heads, int kv_heads, int dh, int accumulate) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int per = dh / 4, group = heads / kv_heads;
   if (i >= total * kv_heads * per) return;
   const int64_t row = i / (kv_heads * per);
   const int g = (int)(i / per % kv_heads), d = (int)(i % per) * 4;
+  const float *part = j.part[blockIdx.y];
   tiles::f4 s{};
   for (int h = g * group; h < (g + 1) * group; ++h)
     s += *reinterpret_cast<const tiles::f4 *>(part + ((int64_t)h * total + row) * dh + d);
-  tiles::f4u *o = reinterpret_cast<tiles::f4u *>(out + row * ld + (int64_t)g * dh + d);
+  tiles::f4u *o = reinterpret_cast<tiles::f4u *>(j.out[blockIdx.y] + row * ld + (int64_t)g * dh + d);
   if (accumulate) s += tiles::f4(*o);
   *o = s;
 }
@@ -233,7 +239,7 @@ int check_packed(numrs_hip_ctx *ctx, const Seqs &s, int64_t ld_q, int64_t ld_kv,
       paging::bad_stride(ld_out, h.heads * h.dh))
     return fail(ctx, NUMRS_HIP_E_SHAPE, "%s: a row stride is below its row's width or above 2^31 - 1",
                 what);
-  if (s.tiles * 2 * (h.heads + h.kv_heads) >= int64_t{1} << 31)
+  if (s.tiles * 2 * (h.heads + h.kv_heads) >= int64_t{1} << 31)  // the largest grid
     return fail(ctx, NUMRS_HIP_E_SHAPE, "%s: too many tokens times heads", what);
   return NUMRS_HIP_OK;
 }
@@ -357,39 +363,30 @@ int packed_backward(numrs_hip_ctx *ctx, const Seqs &s, const float *q, int64_t l
   BwdArgs b{few ? s.few_by_work : s.by_work, q, k, v, out, dout, stats, ld_q, ld_kv, ld_out};
   tiles::BackwardArgs a{q, k, v, out, dout, stats, ld_q, ld_kv, ld_out, pq.rows, pk.rows, pv.rows, pg.rows,
                         pq.exps, pk.exps, pv.exps, pg.exps, rowstat.f(), dq, dk, dv, ld_q, ld_kv, ld_kv, s.total,
-                        H, Hk, dh, accumulate, each, alpha, scale, kMostScore, kMostValue};
+                        H, Hk, dh, accumulate, accumulate, each, alpha, scale, kMostScore, kMostValue};
   return with_dp(dh, [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
     tiles::pack<DP><<<(unsigned)(s.tiles * p.slots), 256, 0, ctx->stream>>>(p);
     if (int rc = check_launch(ctx, "pack")) return rc;
-    if (dq != nullptr) {
-      if (few)
-        dq_block<DP, 2><<<(unsigned)(s.tiles * H), 256, 0, ctx->stream>>>(b, a);
-      else
-        dq_block<DP, 1><<<(unsigned)(s.blocks * H), 256, 0, ctx->stream>>>(b, a);
-      if (int rc = check_launch(ctx, "dq_block")) return rc;
+    Join j{};
+    int joins = 0;
+    if (keys && each < group) {
+      float *at = parts.f();
+      for (float **p : {&a.dk, &a.dv})
+        if (*p != nullptr) j.out[joins] = *p, j.part[joins++] = *p = at, at += part / sizeof(float);
     }
-    if (!keys) return (int)NUMRS_HIP_OK;
-    b.tiles = few ? s.few_by_rest : s.by_rest;
-    if (each < group) {
-      a.dk = dk != nullptr ? parts.f() : nullptr;
-      a.dv = dv != nullptr ? parts.f() + (dk != nullptr ? part / sizeof(float) : 0) : nullptr;
-      a.accumulate = 0;
-    }
+    a.acc_kv = joins > 0 ? 0 : accumulate;
+    const int64_t n = few ? s.tiles : s.blocks;
+    const unsigned nk = keys ? (unsigned)(n * (H / each)) : 0, nq = dq != nullptr ? (unsigned)(n * H) : 0;
     if (few)
-      dkv_block<DP, 2><<<(unsigned)(s.tiles * (H / each)), 256, 0, ctx->stream>>>(b, a);
+      backward_block<DP, 2><<<nk + nq, 256, 0, ctx->stream>>>(b, a, s.few_by_rest, nk);
     else
-      dkv_block<DP, 1><<<(unsigned)(s.blocks * (H / each)), 256, 0, ctx->stream>>>(b, a);
-    if (int rc = check_launch(ctx, "dkv_block")) return rc;
-    if (each < group) {
-      const unsigned grid = grid_for(s.total * Hk * (dh / 4), 256);
-      if (dk != nullptr)
-        join_heads<<<grid, 256, 0, ctx->stream>>>(a.dk, dk, ld_kv, s.total, H, Hk, dh, accumulate);
-      if (dv != nullptr)
-        join_heads<<<grid, 256, 0, ctx->stream>>>(a.dv, dv, ld_kv, s.total, H, Hk, dh, accumulate);
-      return check_launch(ctx, "join_heads");
-    }
-    return (int)NUMRS_HIP_OK;
+      backward_block<DP, 1><<<nk + nq, 256, 0, ctx->stream>>>(b, a, s.by_rest, nk);
+    if (int rc = check_launch(ctx, "backward_block")) return rc;
+    if (joins == 0) return (int)NUMRS_HIP_OK;
+    join_heads<<<dim3(grid_for(s.total * Hk * (dh / 4), 256), joins), 256, 0, ctx->stream>>>(
+        j, ld_kv, s.total, H, Hk, dh, accumulate);
+    return check_launch(ctx, "join_heads");
   });
 }
 

@@ -519,7 +519,7 @@ struct BackwardArgs {
   const float *rowstat;
   float *dq, *dk, *dv;
   int64_t ld_q, ld_k, ld_v, total;
-  int heads, kv_heads, dh, accumulate;
+  int heads, kv_heads, dh, accumulate, acc_kv;  // acc_kv: for dk and dv
   int each;             // query heads of a workgroup of key rows: its group, or one
   float alpha, scale;   // log2(e) / sqrt(dh), 1 / sqrt(dh)
   float most_score, most_value;  // see Source
@@ -804,8 +804,8 @@ __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t
   const int64_t at = part ? ((int64_t)h0 * a.total + row) * a.dh : 0;
   const int64_t ck = part ? at : row * a.ld_k + (int64_t)g * a.dh;
   const int64_t cv = part ? at : row * a.ld_v + (int64_t)g * a.dh;
-  if (a.dk != nullptr) put_rows<DP>(a.dk + ck, xk, a.dh, hi, a.accumulate);
-  if (a.dv != nullptr) put_rows<DP>(a.dv + cv, xv, a.dh, hi, a.accumulate);
+  if (a.dk != nullptr) put_rows<DP>(a.dk + ck, xk, a.dh, hi, a.acc_kv);
+  if (a.dv != nullptr) put_rows<DP>(a.dv + cv, xv, a.dh, hi, a.acc_kv);
   return true;
 }
 
