@@ -347,9 +347,9 @@ int numrs_hip_attention_backward_out_strided(numrs_hip_ctx *ctx, const float *q,
 /* A packed batch: sequences of different lengths whose tokens follow each
  * other as the rows of one matrix (no reference counterpart; its ops take one
  * shape).  `lengths` is a HOST array; a length may be 0.  The handle holds the
- * device's copy and may be destroyed as soon as no further call names it; a
- * graph that recorded such a call needs it until the graph is destroyed, and a
- * tensor's backward keeps what it needs by itself. */
+ * device's copy and may be destroyed as soon as no further call names it: a
+ * tensor's backward, and a graph that recorded such a call, keep that copy by
+ * themselves. */
 typedef struct numrs_hip_seqs numrs_hip_seqs;
 int numrs_hip_seqs_create(numrs_hip_ctx *ctx, const int64_t *lengths, int64_t n,
                           numrs_hip_seqs **out);

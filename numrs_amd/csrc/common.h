@@ -8,6 +8,7 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <memory>
 #include <unordered_map>
 #include <vector>
 
@@ -42,6 +43,9 @@ struct numrs_hip_ctx {
   // -- and the graph takes them over when the recording ends.
   bool capturing = false;
   std::vector<std::pair<void *, size_t>> capture_held;
+  // Objects that recorded kernels read and whose owners may drop them: the
+  // graph takes these references over too.
+  std::vector<std::shared_ptr<const void>> capture_kept;
   // Instantiated graphs not yet destroyed.  Their kernels address the
   // workspace and scratch regions as they were when recorded, so while any
   // exist a region that grows keeps its old buffer in `retired`; the last

@@ -283,6 +283,7 @@ int numrs_hip_kv_cache_write(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cache
     return rc;
   const Seqs &s = *seqs->s;
   if (s.total == 0) return NUMRS_HIP_OK;
+  if (int rc = s.keep()) return rc;
   DeviceScope dev(ctx);
   const RowArgs a{device_cache(*cache, table, max_pages), s.in_order, ends, k, v, nullptr, nullptr, ld};
   const unsigned grid = (unsigned)(s.tiles * cache->kv_heads);
@@ -301,6 +302,7 @@ int numrs_hip_kv_cache_read(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cache,
     return rc;
   const Seqs &s = *seqs->s;
   if (s.total == 0) return NUMRS_HIP_OK;
+  if (int rc = s.keep()) return rc;
   DeviceScope dev(ctx);
   const RowArgs a{device_cache(*cache, table, max_pages), s.in_order, ends, nullptr, nullptr, k, v, ld};
   const unsigned grid = (unsigned)(s.tiles * cache->kv_heads);

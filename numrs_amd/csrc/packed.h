@@ -2,6 +2,7 @@
 #pragma once
 
 #include <memory>
+#include <new>
 
 #include "common.h"
 
@@ -19,7 +20,7 @@ struct SeqTile {
 constexpr int kTile = 64;
 
 // Lists of a batch's tiles on the device.
-struct Seqs {
+struct Seqs : std::enable_shared_from_this<Seqs> {
   numrs_hip_ctx *ctx = nullptr;
   int64_t n = 0, total = 0, tiles = 0, blocks = 0;
   SeqTile *in_order = nullptr;  // [tiles]; a tile's number is its place
@@ -28,6 +29,17 @@ struct Seqs {
   SeqTile *few_by_work = nullptr, *few_by_rest = nullptr;  // the same of the tiles
   size_t bytes = 0;
   ~Seqs() { block_free(ctx, in_order, bytes); }
+  // Called before a launch that reads the lists: a graph being recorded keeps them for its replays,
+  // whatever becomes of the handle.
+  int keep() const {
+    if (!ctx->capturing) return NUMRS_HIP_OK;
+    try {
+      ctx->capture_kept.push_back(shared_from_this());
+    } catch (const std::bad_alloc &) {
+      return fail(ctx, NUMRS_HIP_E_NOMEM, "out of host memory");
+    }
+    return NUMRS_HIP_OK;
+  }
 };
 
 struct PackedHeads {

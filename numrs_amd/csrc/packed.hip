@@ -296,6 +296,7 @@ int packed_forward(numrs_hip_ctx *ctx, const Seqs &s, const float *q, int64_t ld
   if (s.total == 0) return NUMRS_HIP_OK;
   if (q == nullptr || k == nullptr || v == nullptr || out == nullptr)
     return fail(ctx, NUMRS_HIP_E_INVALID, "attention_packed: null pointer");
+  if (int rc = s.keep()) return rc;
   DeviceScope dev(ctx);
   Packed pk(ctx), pv(ctx);
   const int H = (int)h.heads, Hk = (int)h.kv_heads, dh = (int)h.dh;
@@ -333,6 +334,7 @@ int packed_backward(numrs_hip_ctx *ctx, const Seqs &s, const float *q, int64_t l
   if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || dout == nullptr ||
       stats == nullptr)
     return fail(ctx, NUMRS_HIP_E_INVALID, "attention_packed_backward: null pointer");
+  if (int rc = s.keep()) return rc;
   DeviceScope dev(ctx);
   const int H = (int)h.heads, Hk = (int)h.kv_heads, dh = (int)h.dh, group = H / Hk;
   const bool keys = dk != nullptr || dv != nullptr;

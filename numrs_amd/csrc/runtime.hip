@@ -321,6 +321,7 @@ struct numrs_hip_graph {
   // blocks tensors released during the recording: the recorded kernels may
   // use them on every replay, so they return to the cache only on destroy
   std::vector<std::pair<void *, size_t>> held;
+  std::vector<std::shared_ptr<const void>> kept;  // see numrs_hip_ctx::capture_kept
 };
 
 static void return_held(numrs_hip_ctx *ctx, std::vector<std::pair<void *, size_t>> &held) {
@@ -362,6 +363,7 @@ int numrs_hip_graph_begin(numrs_hip_ctx *ctx) {
   NRS_HIP(ctx, hipStreamBeginCapture(ctx->stream, hipStreamCaptureModeRelaxed));
   ctx->capturing = true;
   ctx->capture_held.clear();
+  ctx->capture_kept.clear();
   return NUMRS_HIP_OK;
 }
 
@@ -377,6 +379,7 @@ int numrs_hip_graph_abort(numrs_hip_ctx *ctx) {
   std::vector<std::pair<void *, size_t>> held;
   held.swap(ctx->capture_held);
   return_held(ctx, held);
+  ctx->capture_kept.clear();
   if (run_pending_destroys(ctx)) delete ctx;
   return NUMRS_HIP_OK;
 }
@@ -389,6 +392,8 @@ int numrs_hip_graph_end(numrs_hip_ctx *ctx, numrs_hip_graph **out) {
   ctx->capturing = false;
   std::vector<std::pair<void *, size_t>> held;
   held.swap(ctx->capture_held);
+  std::vector<std::shared_ptr<const void>> kept;
+  kept.swap(ctx->capture_kept);
   hipGraph_t graph = nullptr;
   hipError_t e = hipStreamEndCapture(ctx->stream, &graph);
   if (e != hipSuccess || graph == nullptr) {
@@ -407,7 +412,7 @@ int numrs_hip_graph_end(numrs_hip_ctx *ctx, numrs_hip_graph **out) {
     (void)run_pending_destroys(ctx);
     return fail(ctx, NUMRS_HIP_E_HIP, "graph instantiation failed: %s", hipGetErrorString(e));
   }
-  *out = new numrs_hip_graph{ctx, graph, exec, std::move(held)};
+  *out = new numrs_hip_graph{ctx, graph, exec, std::move(held), std::move(kept)};
   ++ctx->live_blocks;  // the graph keeps the context alive, like a tensor's block
   ++ctx->live_graphs;
   (void)run_pending_destroys(ctx);  // the new graph keeps the context alive

@@ -274,6 +274,46 @@ def test_a_recorded_step_replays(hip_ctx):
     graph.close(), second.close()
 
 
+def test_a_graph_keeps_its_sequences(hip_ctx):
+    """A recorded step is replayed after the handle is gone and others have taken its memory."""
+    c, rng = hip_ctx, np.random.default_rng(13)
+    call = _Call(c, [190, 3, 65], 4, 2, 64, rng).upload()
+    q, k, v = call.ptrs
+    d = c.empty(call.x.shape)
+    cache = nr.KVCache(20, 16, 2, 64, "int8", ctx=c)
+    table = c.to_device(np.arange(60, dtype=np.int32).reshape(3, 20) % 20)
+    ends = c.to_device(np.array([190, 3, 65], np.int32))
+    ko, vo = c.empty((258, 128)), c.empty((258, 128))
+
+    def step():
+        lib, s, wq = L.load(), call.seqs.handle, call.wq
+        c._check(lib.numrs_hip_attention_packed_forward(c.handle, s, q, call.ld, k, v, call.ld, call.out.ptr,
+                                                        wq, call.stats.ptr, 4, 2, 64))
+        c._check(lib.numrs_hip_attention_packed_backward(
+            c.handle, s, q, call.ld, k, v, call.ld, call.out.ptr, call.gd.ptr, wq, call.stats.ptr, d.ptr,
+            d.ptr + 4 * wq, d.ptr + 4 * (wq + call.wk), 4, 2, 64, 0))
+        p = ctypes.byref(cache.pages)
+        c._check(lib.numrs_hip_kv_cache_read(c.handle, p, s, ko.ptr, vo.ptr, 128, table.ptr, 20, ends.ptr))
+
+    for a in (cache.k, cache.v):
+        a.upload(rng.integers(1, 256, a.shape, dtype=np.uint8))
+    cache.k_scale.fill(0.5), cache.v_scale.fill(0.25)
+    step()
+    want = [a.numpy() for a in (call.out, d, ko, vo)]
+    graph = nr.StepGraph(c, step)
+    call.seqs.close()
+    # as many lists of the same size, of sequences that would lead elsewhere
+    others = [nr.PackedSequences([3, 65, 190], ctx=c) for _ in range(4)]
+    for a in (call.out, d, ko, vo):
+        a.fill(0)
+    for _ in range(2):
+        graph.replay()
+        for a, w in zip((call.out, d, ko, vo), want):
+            assert_bits(a.numpy(), w)
+    graph.close()
+    assert all(len(o) == 3 for o in others)
+
+
 def test_two_contexts_and_a_stream_each():
     """Two contexts (a stream each) at once give what each gives alone."""
     rng = np.random.default_rng(4)
