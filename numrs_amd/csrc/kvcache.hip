@@ -265,7 +265,7 @@ int check_rows(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cache, const numrs_
   if (paging::bad_stride(ld, cache->kv_heads * cache->head_dim))
     return fail(ctx, NUMRS_HIP_E_SHAPE, "%s: the row stride is below a row's width or above 2^31 - 1",
                 what);
-  if (s.tiles * cache->kv_heads >= int64_t{1} << 31)
+  if (paging::bad_grid(s.tiles * cache->kv_heads))
     return fail(ctx, NUMRS_HIP_E_SHAPE, "%s: too many tokens times heads", what);
   return NUMRS_HIP_OK;
 }

@@ -239,7 +239,7 @@ int check_packed(numrs_hip_ctx *ctx, const Seqs &s, int64_t ld_q, int64_t ld_kv,
       paging::bad_stride(ld_out, h.heads * h.dh))
     return fail(ctx, NUMRS_HIP_E_SHAPE, "%s: a row stride is below its row's width or above 2^31 - 1",
                 what);
-  if (s.tiles * 2 * (h.heads + h.kv_heads) >= int64_t{1} << 31)  // the largest grid
+  if (paging::bad_grid(s.tiles * 2 * (h.heads + h.kv_heads)))  // the backward's largest
     return fail(ctx, NUMRS_HIP_E_SHAPE, "%s: too many tokens times heads", what);
   return NUMRS_HIP_OK;
 }

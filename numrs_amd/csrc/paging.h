@@ -96,6 +96,9 @@ inline const char *refuse_heads(int64_t heads, int64_t kv_heads, int64_t dh) {
 
 inline bool bad_stride(int64_t ld, int64_t width) { return ld < width || ld >= int64_t{1} << 31; }
 
+// More workgroups of 256 threads than a launch, of at most 2^32 - 1 threads, can have.
+inline bool bad_grid(int64_t groups) { return groups >= int64_t{1} << 24; }
+
 // Lengths of a packed batch: their sum, or -1 if one is negative or they pass 2^30 tokens.
 inline int64_t packed_total(const int64_t *lengths, int64_t n) {
   int64_t total = 0;

@@ -304,6 +304,50 @@ def test_large_magnitudes(hip_ctx):
             assert (d <= err + 1e-44).all(), (sq, sk, sv, format, (d / (err + 1e-300)).max())
 
 
+@pytest.mark.parametrize("format", ["f32", "int8"])
+def test_scores_near_the_lowest(hip_ctx, format):
+    """Equal scores of -3.5e32: the mean of the values, as for any other score."""
+    c, rng, n, dh = hip_ctx, np.random.default_rng(14), 300, 8
+    s = _Paged(c, [n], 16, 1, dh, format, rng)
+    k, v = np.zeros((n, dh), np.float32), rand(rng, (n, dh))
+    k[:, 3] = -1e16
+    q = np.zeros((1, dh), np.float32)
+    q[0, 3] = 1e17
+    s.cache.write(s.seqs, c.to_device(k), c.to_device(v), s.td, s.ends)
+    out, qd = c.empty((1, dh)), c.to_device(q)
+    c._check(L.load().numrs_hip_attention_paged(c.handle, ctypes.byref(s.cache.pages), qd.ptr, dh, 1, s.td.ptr,
+                                                s.table.shape[1], s.ends.ptr, 1, out.ptr, dh))
+    v = _stands_for(v.reshape(n, 1, dh), format)[:, 0].astype(np.float64)
+    assert (abs(out.numpy()[0] - v.mean(0)) <= 2 * U2 * (n + 8) * abs(v).mean(0)).all()
+
+
+@pytest.mark.parametrize("format", ["f32", "int8"])
+def test_more_sequences_than_a_workgroup_looks_at_once(hip_ctx, format):
+    """1300 sequences, most short, some empty, one long behind the first thousand: also the same twice."""
+    c, rng, page, H, Hk, dh = hip_ctx, np.random.default_rng(15), 16, 8, 2, 64
+    lengths = rng.integers(0, 40, 1300).tolist()
+    lengths[0], lengths[511], lengths[512], lengths[1100], lengths[1299] = 0, 130, 0, 2500, 65
+    s, n, T, w = _Paged(c, lengths, page, Hk, dh, format, rng), 1300, sum(lengths), Hk * dh
+    k, v, q = rand(rng, (T, w)), rand(rng, (T, w)), rand(rng, (n, H * dh))
+    s.cache.write(s.seqs, c.to_device(k), c.to_device(v), s.td, s.ends)
+    out, qd = c.empty((n, H * dh)), c.to_device(q)
+    call = lambda: c._check(L.load().numrs_hip_attention_paged(  # noqa: E731
+        c.handle, ctypes.byref(s.cache.pages), qd.ptr, H * dh, H, s.td.ptr, s.table.shape[1], s.ends.ptr, n,
+        out.ptr, H * dh))
+    call()
+    got = out.numpy()
+    k, v = (_stands_for(x.reshape(T, Hk, dh), format) for x in (k, v))
+    at = np.concatenate([[0], np.cumsum(lengths)])
+    for i in range(n):
+        ref, err = _attention(q[i].reshape(H, dh), k[at[i]:at[i + 1]], v[at[i]:at[i + 1]], Hk)
+        if lengths[i] == 0:
+            assert (got[i] == 0).all(), i
+        else:
+            _check(got[i].reshape(H, dh), ref, err, f"row {i}")
+    call()
+    assert_bits(out.numpy(), got)
+
+
 def test_refusals(hip_ctx):
     c, lib, rng = hip_ctx, L.load(), np.random.default_rng(6)
     s = _Paged(c, [5, 3], 16, 2, 16, "int8", rng)
@@ -319,6 +363,12 @@ def test_refusals(hip_ctx):
             bad[i] = value
             assert fn(*bad) == code, i
             assert lib.numrs_hip_last_error(h)
+    wide = nr.KVPages.from_buffer_copy(s.cache.pages)
+    wide.kv_heads, wide.head_dim, wide.pages = 65535, 8, 1
+    long = nr.PackedSequences([64 * 256 + 1], ctx=c)  # more work than a launch can have
+    assert lib.numrs_hip_kv_cache_write(h, ctypes.byref(wide), long.handle, x.ptr, x.ptr, 524280, s.td.ptr, 2,
+                                        s.ends.ptr) == L.E_SHAPE
+    assert b"too many" in lib.numrs_hip_last_error(h)
     fn = lib.numrs_hip_attention_paged
     good = [h, cp, x.ptr, 64, 4, s.td.ptr, 2, s.ends.ptr, 2, x.ptr + 512, 64]
     for i, value, code in ((1, None, L.E_INVALID), (2, None, L.E_INVALID), (3, 63, L.E_SHAPE), (4, 3, L.E_SHAPE),

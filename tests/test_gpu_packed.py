@@ -212,6 +212,38 @@ def test_values_that_no_row_attends_to(hip_ctx, dh):
     assert np.abs(call.parts(d)[0][:at] - clean.parts(e)[0][:at]).max() <= 1e-4
 
 
+@pytest.mark.parametrize("dh", [32, 64, 96, 128])
+def test_values_that_no_row_attends_to_among_many(hip_ctx, dh):
+    """The same where there are two blocks of 128 rows and more for each CU: a sequence of ordinary values
+    among others gives the same bits whatever those hold, earlier rows the same values."""
+    # 3 blocks each; of 90 also enough key rows that a workgroup takes all heads of a group
+    lengths, H, Hk = [300] * (90 if dh == 32 else 12), 16, 4
+    call, clean = (_Call(hip_ctx, lengths, H, Hk, dh, np.random.default_rng(dh)) for _ in range(2))
+    bad = 300 * 7 + 150
+    q, k, v = call.parts(call.x)
+    k[bad, 0], v[bad, dh + 1] = np.nan, np.inf
+    call.g[bad, 2 * (H // Hk) * dh] = np.inf  # kv head 2's first query head
+    q[bad, -1] = 1e20  # the last query head: finite, and past what the tiles take
+    call.upload(), clean.upload()
+    a, b = call.forward(), clean.forward()
+    d, e = (x.backward(hip_ctx.empty(x.x.shape)) for x in (call, clean))
+    inside = slice(300 * 7, 300 * 8)
+    for x, y in ((a, b), (d, e)):
+        others = np.ones(len(x), bool)
+        others[inside] = False
+        assert_bits(x[others], y[others])
+    assert np.abs(a[300 * 7:bad] - b[300 * 7:bad]).max() <= 1e-5
+    assert np.isnan(a[bad:300 * 8, :(H // Hk) * dh]).all()
+    dq, dk, dv = call.parts(d)
+    eq, ek, ev = clean.parts(e)
+    assert np.abs(dq[300 * 7:bad] - eq[300 * 7:bad]).max() <= 1e-4
+    for x, y in ((dk, ek), (dv, ev)):
+        x, y = x[inside], y[inside]
+        assert np.isnan(x[:151, :dh]).any() and not np.isfinite(x[:151, 2 * dh:3 * dh]).all()
+        # kv head 2's keys behind the row, which no such gradient reaches
+        assert np.abs(x[151:, 2 * dh:3 * dh] - y[151:, 2 * dh:3 * dh]).max() <= 1e-4
+
+
 @pytest.mark.parametrize("sq,sk,sv,sg", [(1e-18, 1e18, 1, 1), (1e15, 1e-15, 1e-30, 1e20), (1, 1, 1e30, 1e-30),
                                          (1, 1, 1e-37, 1), (1e-3, 1e-3, 1e-3, 1e-3), (0, 1, 1, 1), (1, 1, 0, 0)])
 def test_magnitudes(hip_ctx, sq, sk, sv, sg):
@@ -359,6 +391,10 @@ def test_refusals(hip_ctx):
         bad = list(good)
         bad[i] = None
         assert bwd(*bad) == L.E_INVALID, i
+    # more work than a launch can have: refused before anything is read
+    long = nr.PackedSequences([64 * 64 + 1], ctx=c)
+    assert fwd(h, long.handle, q, 524280, k, v, 524280, out, 524280, None, 65535, 65535, 8) == L.E_SHAPE
+    assert b"too many" in lib.numrs_hip_last_error(h)
     out_h = ctypes.c_void_p()
     for lengths, n, code in (([-1], 1, L.E_SHAPE), ([2**30, 1], 2, L.E_SHAPE), ([1], -1, L.E_INVALID),
                              ([1], 2**24, L.E_INVALID)):

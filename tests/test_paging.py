@@ -32,6 +32,7 @@ const char *refuse_table(const void *t, int64_t m, const void *l, int64_t n, int
   return paging::refuse_table(t, m, l, n, code);
 }
 const char *refuse_heads(int64_t h, int64_t hk, int64_t dh) { return paging::refuse_heads(h, hk, dh); }
+int bad_grid(int64_t n) { return paging::bad_grid(n); }
 int bad_stride(int64_t ld, int64_t w) { return paging::bad_stride(ld, w); }
 int64_t packed_total(const int64_t *l, int64_t n) { return paging::packed_total(l, n); }
 }
@@ -52,7 +53,7 @@ def lib(tmp_path_factory):
                             ("log2_of", i, [i64]), ("refuse_cache", ctypes.c_char_p, [p, p]),
                             ("refuse_table", ctypes.c_char_p, [p, i64, p, i64, p]),
                             ("refuse_heads", ctypes.c_char_p, [i64] * 3), ("bad_stride", i, [i64] * 2),
-                            ("packed_total", i64, [p, i64])):
+                            ("bad_grid", i, [i64]), ("packed_total", i64, [p, i64])):
         fn = getattr(lib, name)
         fn.restype, fn.argtypes = res, args
     return lib
@@ -136,6 +137,8 @@ def test_null_cache_tables_heads_and_strides(lib):
         assert (lib.refuse_heads(h, hk, dh) is None) == bool(ok), (h, hk, dh)
     assert not lib.bad_stride(64, 64) and lib.bad_stride(63, 64) and lib.bad_stride(-1, 64)
     assert lib.bad_stride(2**31, 64)
+    # 256 threads each: 2^32 - 1 at most
+    assert not lib.bad_grid(2**24 - 1) and lib.bad_grid(2**24)
 
 
 def test_packed_totals(lib):
