@@ -2,6 +2,12 @@
 // buffer: the forward keeps a running softmax reference m and sum l for each row,
 //   p_ij = exp(s_ij - m_i) / l_i,  s_ij = q_i . k_j / sqrt(dh),  j <= i of the same sequence,
 // and the backward forms p again from them.
+//
+// packed_tiles.h has the kernels that ordinary values take.  The row kernels here are the plain fp32 form,
+// a wave a row, for blocks that meet a value which those cannot take: not finite, or from 2^50 (queries and
+// keys) or 2^90 (values and the output's gradient) on.  They read every key a row at a time, 30 to 120
+// times slower (8192 tokens, 16 heads of 128: 93 ms against 0.8), and are there so that such a value does
+// to the rows that attend to it what fp32 arithmetic does, and nothing to the others.
 #include <algorithm>
 #include <cmath>
 #include <new>
@@ -181,9 +187,10 @@ __device__ void row_dkv(const BwdArgs &b, const tiles::BackwardArgs &a, const Se
   }
 }
 
-// The backward's blocks in one launch, so that each kind's last workgroups run beside the other's: first
-// `keys` workgroups with a block of key rows of one kv head, or one query head's part of it, then a block of
-// query rows of one head each.
+// The backward's blocks in one launch, so that each kind's last workgroups run beside the other's (35 us
+// against 18 + 23 for 16 x 256 tokens, 8 heads of 64; 93 against 46 + 57 for 2736 tokens, 10 heads of 80):
+// first `keys` workgroups with a block of key rows of one kv head, or one query head's part of it, then a
+// block of query rows of one head each.
 template <int DP, int Z>
 __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1)
     backward_block(BwdArgs b, tiles::BackwardArgs a, const SeqTile *key_tiles, unsigned keys) {
@@ -206,7 +213,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1)
 }
 
 // Adds the parts of a group's query heads in order, four values a thread: part [heads, total, dh]; dk's and
-// dv's by the grid's second index.
+// dv's by the grid's second index.  Bound by memory: 2 x 8192 tokens, 16 heads of 128 on 4 in 38 us, 4.4 TB/s.
 struct Join {
   const float *part[2];
   float *out[2];
@@ -338,9 +345,11 @@ int packed_backward(numrs_hip_ctx *ctx, const Seqs &s, const float *q, int64_t l
   DeviceScope dev(ctx);
   const int H = (int)h.heads, Hk = (int)h.kv_heads, dh = (int)h.dh, group = H / Hk;
   const bool keys = dk != nullptr || dv != nullptr;
-  // The query heads of a group go to workgroups of their own, whose parts are added afterwards,
-  // unless the key rows alone make enough of them.
-  const int each = group > 1 && s.blocks * Hk >= 4 * ctx->num_cus ? group : 1;
+  // The query heads of a group go to workgroups of their own, whose parts are added afterwards, unless the
+  // kv heads' blocks of key rows alone are two for each CU.  Forward and backward on MI355X, heads apart
+  // against together, us: 128 blocks (16 x 256 tokens, 8 heads on 2, of 64) 66, 70; 256 (2 x 4096, 16 on 4,
+  // of 128) 2008, 2099; 512 (16 x 1024, 16 on 4, of 64) 672, 616; 1024 (32 x 1024, of 128) 3043, 2696.
+  const int each = group > 1 && s.blocks * Hk >= 2 * ctx->num_cus ? group : 1;
   Packed pq(ctx), pk(ctx), pv(ctx), pg(ctx);
   TempBlock rowstat(ctx), parts(ctx);
   // The key rows walk over the queries and the output's gradient, the query rows over keys and values

@@ -20,6 +20,13 @@
 // one or several sequences.  A sequence cut by stretches leaves parts (m, l, O), and the workgroup
 // that finishes last of up to 16 adds theirs in order, the last of those groups the groups': no
 // workgroup waits, and the order of the sums does not depend on who is last.
+//
+// 5.2 GB of fp32 cache (96 sequences of 6000 and 8000 tokens, 8 heads of 128) are read in 868 us, 6.0 TB/s
+// (a large copy: 5.54); 134 MB (131072 tokens of one head) in 37, 3.6 TB/s; 70 MB of 8-bit cache of 40
+// sequences of 1 to 5000 tokens in 36; 333 tokens in 11.  In the short ones the way from the lengths to the
+// table, the tokens and the joins, each waiting for the one before, is what takes the time.  Loads of a
+// step into registers that a second step's leave free spilled (a wave's state, two steps' tokens): keys
+// and values are asked for into the place of those just used.
 #pragma once
 
 #include "packed_tiles.h"
@@ -484,7 +491,8 @@ __global__ void __launch_bounds__(64 * kWaves, 2) split_rows(SplitArgs a) {
     s.from = (s.ua - s.u0) * kUnit;
     s.end = min((s.ub - s.u0) * kUnit, (int64_t)__builtin_amdgcn_readfirstlane(tokens[j]));
     // Two steps a wave at least, so that several short sequences go at once; one where this is all
-    // that the workgroup has.
+    // that the workgroup has.  (Each sequence to all waves in turn: 64 us in place of 39 for the 40
+    // sequences above.)
     const int64_t steps = (s.end - s.from + kStep - 1) / kStep;
     s.waves = (int)max((int64_t)1, min((int64_t)kWaves, s.ub - s.ua == hi - lo ? steps : (steps + 1) / 2));
     return s;
