@@ -502,9 +502,8 @@ __global__ void __launch_bounds__(64 * kWaves, 2) split_rows(SplitArgs a) {
   for (int i0 = 0; i0 < a.n && base < hi; i0 += kThreads) {
     const int count = min(kThreads, a.n - i0);
     const int64_t next_base = a.n > kThreads ? scan(i0, base) : uniform(pre[count]);
-    int j = 0;
-    if (next_base <= lo) j = count;
-    while (j < count && uniform(pre[j + 1]) <= lo) ++j;
+    int j = 0;  // the first that ends after the workgroup's first unit
+    for (int k = 0; k < count; k += 64) j += __builtin_popcountll(__ballot(k + lane < count && pre[min(k + lane, count - 1) + 1] <= lo));
     while (j < count && uniform(pre[j]) < hi) {
       // As many sequences as the waves go round, and this wave's place.
       int last = j, used = 0, mine = -1, first = 0;
