@@ -380,6 +380,8 @@ class Tensor:
         """One query row for each sequence over its tokens in a `KVCache`: the
         queries are self's first heads * head_dim columns.  table [n, max_pages]
         and lengths [n] are int32 device arrays.  No backward."""
+        if cache.ctx is not self.ctx:
+            raise ValueError("the queries and the cache must belong to one context")
         most = cache.table_width(table, lengths, self.shape()[0])
         h = ctypes.c_void_p()
         return self._out(L.load().numrs_hip_tensor_attention_paged(

@@ -1305,6 +1305,7 @@ int op_attention_seqs(const T &q, const T *k, const T *v, const numrs_hip_seqs *
   const auto &s = seqs->s;
   if (s->ctx != ctx || (k != nullptr && ((*k)->ctx != ctx || (*v)->ctx != ctx)))
     return fail(ctx, NUMRS_HIP_E_INVALID, "attention_packed: operands of different contexts");
+  numrs_hip::DeviceScope dev(ctx);
   if (q->shape.size() != 2 || q->shape[0] != s->total)
     return fail(ctx, NUMRS_HIP_E_SHAPE, "attention_packed: operands must have a row for each token");
   const int64_t parts = k != nullptr ? H : H + 2 * Hk;
@@ -1935,6 +1936,7 @@ int numrs_hip_tensor_attention_paged(numrs_hip_tensor *x, const numrs_hip_kv_cac
   numrs_hip_ctx *ctx = t->ctx;
   if (recording({&t}))
     return fail(ctx, NUMRS_HIP_E_INVALID, "attention_paged has no backward: detach its input");
+  numrs_hip::DeviceScope dev(ctx);
   if (t->shape.size() != 2 || heads < 1 || heads > 65535 || cache->head_dim < 1 ||
       cache->head_dim > 128 || t->shape[1] < heads * cache->head_dim)
     return fail(ctx, NUMRS_HIP_E_SHAPE, "attention_paged: x must be [rows, at least heads * head_dim]");

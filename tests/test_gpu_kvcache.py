@@ -394,6 +394,33 @@ def test_refusals(hip_ctx):
         t.attention_paged(s.cache, 4, s.td, s.ends)
     with pytest.raises(nr.HipError):
         nr.Tensor.new(rand(rng, (2, 60)), ctx=c).attention_paged(s.cache, 4, s.td, s.ends)
+    with nr.Context(0) as other, pytest.raises(ValueError, match="one context"):
+        nr.Tensor.new(rand(rng, (2, 64)), ctx=other).attention_paged(s.cache, 4, s.td, s.ends)
+
+
+@pytest.mark.parametrize("format", ["f32", "int8"])
+def test_pages_past_32_bits(hip_ctx, format):
+    """A cache of 2.2e9 values: pages whose elements, and bytes, lie past 2^31 and 2^32."""
+    c, rng, page, Hk, dh, H = hip_ctx, np.random.default_rng(16), 1024, 2, 128, 6
+    pages = 2 ** 31 // (page * Hk * dh) + 10
+    cache = nr.KVCache(pages, page, Hk, dh, format, ctx=c)
+    # around 2^31 and 2^32 bytes of fp32 and around 2^31 values, and the last
+    table = np.array([[pages - 1, pages // 2, 3], [pages // 4, pages - 2, pages // 2 + 1], [0, pages - 9, 1]], np.int32)
+    lengths = [2500, 2049, 1100]
+    td, ends, seqs = c.to_device(table), c.to_device(np.array(lengths, np.int32)), nr.PackedSequences(lengths, ctx=c)
+    T = sum(lengths)
+    k, v, q = rand(rng, (T, Hk * dh)), rand(rng, (T, Hk * dh)), rand(rng, (3, H * dh))
+    cache.write(seqs, c.to_device(k), c.to_device(v), td, ends)
+    k, v = (_stands_for(x.reshape(T, Hk, dh), format) for x in (k, v))
+    got = [a.numpy().reshape(T, Hk, dh) for a in cache.read(seqs, td, ends)]
+    assert_bits(got[0], k)
+    assert_bits(got[1], v)
+    out, qd = c.empty((3, H * dh)), c.to_device(q)
+    c._check(L.load().numrs_hip_attention_paged(c.handle, ctypes.byref(cache.pages), qd.ptr, H * dh, H, td.ptr, 3,
+                                                ends.ptr, 3, out.ptr, H * dh))
+    got, at = out.numpy().reshape(3, H, dh), np.concatenate([[0], np.cumsum(lengths)])
+    for i in range(3):
+        _check(got[i], *_attention(q[i].reshape(H, dh), k[at[i]:at[i + 1]], v[at[i]:at[i + 1]], Hk), f"row {i}")
 
 
 # ---------------------------------------------------------------------------

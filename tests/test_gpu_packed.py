@@ -161,6 +161,30 @@ def test_forward_without_statistics_gives_the_same(hip_ctx):
     assert_bits(call.forward(stats=False), a)
 
 
+def test_rows_past_32_bits(hip_ctx):
+    """Rows 2^30 + 8 elements apart: the fourth lies past 2^31 elements and 2^33 bytes."""
+    c, rng, lib, H, Hk, dh, n, ld = hip_ctx, np.random.default_rng(17), L.load(), 2, 1, 32, 4, 2**30 + 8
+    near = _Call(c, [n], H, Hk, dh, rng).upload()
+    out, d = near.forward(), near.backward(c.empty(near.x.shape))
+    w, wq = near.ld, near.wq
+    far = [c.empty(((n - 1) * ld + w,)) for _ in range(2)]  # q, k, v, out, dout; dq, dk, dv
+    x, dx = far[0].ptr, far[1].ptr
+    for i in range(n):
+        far[0].view(i * ld, (w,)).upload(near.x[i])
+    o = c.empty(((n - 1) * ld + 2 * wq,))
+    for i in range(n):
+        o.view(i * ld + wq, (wq,)).upload(near.g[i])
+    stats = c.empty((n, H, 2))
+    c._check(lib.numrs_hip_attention_packed_forward(c.handle, near.seqs.handle, x, ld, x + 4 * wq, x + 4 * (wq + dh),
+                                                    ld, o.ptr, ld, stats.ptr, H, Hk, dh))
+    c._check(lib.numrs_hip_attention_packed_backward(
+        c.handle, near.seqs.handle, x, ld, x + 4 * wq, x + 4 * (wq + dh), ld, o.ptr, o.ptr + 4 * wq, ld, stats.ptr,
+        dx, dx + 4 * wq, dx + 4 * (wq + dh), H, Hk, dh, 0))
+    for i in range(n):
+        assert_bits(o.view(i * ld, (wq,)).numpy(), out[i])
+        assert_bits(far[1].view(i * ld, (w,)).numpy(), d[i])
+
+
 def test_the_same_call_gives_the_same_bits(hip_ctx):
     call = _Call(hip_ctx, [300, 17, 520], 8, 2, 64, np.random.default_rng(2)).upload()
     d = hip_ctx.empty(call.x.shape)
