@@ -571,3 +571,45 @@ def test_module_is_causal_and_trains(engine):
     assert np.abs(attn.qkv.weight.gradient()).max() > 0
     with pytest.raises(ValueError):
         nn.CausalSelfAttention(*w, heads=4, kv_heads=3)
+
+
+@pytest.mark.parametrize("lengths", [[70, 3, 129], [140] * 40])
+def test_a_recorded_training_step(engine, lengths):
+    """Steps of the module and SGD as a graph's replays equal eager ones to the bit, while an eager forward
+    of the same parameters is still to be swept, and after the sequences' handle is closed."""
+    from numrs_amd import optim
+    rng, d, H, Hk = np.random.default_rng(18), 32, 16, 4
+    w = [rand(rng, s, 0.2) for s in ((16 * H, d), (16 * Hk, d), (16 * Hk, d), (d, 16 * H))]
+    x, t = nr.Tensor.new(rand(rng, (sum(lengths), d))), nr.Tensor.new(rand(rng, (sum(lengths), d)))
+    seqs = nr.PackedSequences(lengths)
+
+    def make():
+        attn = nn.CausalSelfAttention(*w, heads=H, kv_heads=Hk)
+        sgd = optim.SGD.simple(attn.parameters(), 0.1)
+
+        def step():
+            loss = attn.forward_packed(x, seqs).mse_loss(t)
+            loss.backward()
+            sgd.step()
+            sgd.zero_grad()
+            return loss
+        return attn, step
+
+    (a, eager), (b, recorded) = make(), make()
+    assert eager().item() == recorded().item()
+    alive = b.forward_packed(x, seqs).sum()
+    graph = nr.StepGraph(engine, recorded)
+    want = [eager().item() for _ in range(4)]
+    seqs.close()
+    filler = [nr.PackedSequences(lengths[::-1]) for _ in range(3)]
+    for i, loss in enumerate(want):
+        graph.replay()
+        assert graph.outputs.item() == loss, i
+        if i == 1:  # the sweep adds to gradients that the next replay's step would take
+            alive.backward()
+            for p in b.parameters():
+                p.zero_grad()
+    for p, q in zip(a.parameters(), b.parameters()):
+        assert_bits(q.values(), p.values())
+    graph.close()
+    del filler
