@@ -5,9 +5,10 @@
 //
 // packed_tiles.h has the kernels that ordinary values take.  The row kernels here are the plain fp32 form,
 // a wave a row, for blocks that meet a value which those cannot take: not finite, or from 2^50 (queries and
-// keys) or 2^90 (values and the output's gradient) on.  They read every key a row at a time, 30 to 120
-// times slower (8192 tokens, 16 heads of 128: 93 ms against 0.8), and are there so that such a value does
-// to the rows that attend to it what fp32 arithmetic does, and nothing to the others.
+// keys) or 2^90 (values and the output's gradient) on.  They read every key a row at a time, some 150 times
+// slower (8192 tokens, 16 heads of 128, a value at their start infinite: 134 ms against 0.8; rows that are
+// NaN throughout end at the first such score), and are there so that such a value does to the rows that
+// attend to it what fp32 arithmetic does, and nothing to the others.
 #include <algorithm>
 #include <cmath>
 #include <new>
@@ -64,6 +65,7 @@ __device__ void row_forward(const FwdArgs &a, const SeqTile &t, int r, int h, fl
     const float p = lane < n ? exp2f(s - top) : 0.f, c = j0 == 0 ? 0.f : exp2f(m - top);
     m = top;
     l = l * c + wave_sum(p);
+    if (l != l) break;  // the row is NaN, whatever follows
     float t0 = 0.f, t1 = 0.f;  // the block's sum apart, so that a long sum's rounding stays small
     for (int e = 0; e < n; ++e) {
       const float w = lane_of(p, e);
@@ -134,6 +136,7 @@ __device__ void row_dq(const BwdArgs &b, const tiles::BackwardArgs &a, const Seq
       if (lane + 64 < a.dh) t1 = fmaf(w, y[lane + 64], t1);
     }
     o0 += t0, o1 += t1;
+    if (l != l) break;
   }
   float *o = a.dq + row * a.ld_q + (int64_t)h * a.dh;
   if (lane < a.dh) put(o + lane, o0 * a.scale, a.accumulate);
@@ -172,6 +175,10 @@ __device__ void row_dkv(const BwdArgs &b, const tiles::BackwardArgs &a, const Se
         }
       }
       k0 += tk0, k1 += tk1, v0 += tv0, v1 += tv1;
+      if (__any(p != p)) {  // (and ds with it) a row of NaN: so are all of these
+        h = h0 + a.each;
+        break;
+      }
     }
   }
   const int64_t part = ((int64_t)h0 * a.total + row) * a.dh;

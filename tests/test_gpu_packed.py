@@ -241,7 +241,7 @@ def test_values_that_no_row_attends_to_among_many(hip_ctx, dh):
     """The same where there are two blocks of 128 rows and more for each CU: a sequence of ordinary values
     among others gives the same bits whatever those hold, earlier rows the same values."""
     # 3 blocks each; of 90 also enough key rows that a workgroup takes all heads of a group
-    lengths, H, Hk = [300] * (90 if dh == 32 else 12), 16, 4
+    lengths, H, Hk = [300] * (90 if dh == 32 else 15), 12, 4
     call, clean = (_Call(hip_ctx, lengths, H, Hk, dh, np.random.default_rng(dh)) for _ in range(2))
     bad = 300 * 7 + 150
     q, k, v = call.parts(call.x)
