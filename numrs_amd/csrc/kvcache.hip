@@ -149,7 +149,8 @@ __global__ void __launch_bounds__(256) write_rows(RowArgs a, int lanes) {
       k[r] = v[r] = f4{};
       if (!in || x.row[r] < 0) continue;
       const int64_t at = (int64_t)(t.row0 + x.row[r]) * a.ld + (int64_t)g * dh + d;
-      k[r] = *reinterpret_cast<const f4u *>(a.k + at), v[r] = *reinterpret_cast<const f4u *>(a.v + at);
+      k[r] = __builtin_nontemporal_load(reinterpret_cast<const f4u *>(a.k + at));
+      v[r] = __builtin_nontemporal_load(reinterpret_cast<const f4u *>(a.v + at));
     }
     if constexpr (!INT8) {
 #pragma unroll
@@ -233,7 +234,8 @@ __global__ void __launch_bounds__(256) read_rows(RowArgs a, int lanes) {
     for (int r = 0; r < 4; ++r) {
       if (x.row[r] < 0) continue;
       const int64_t at = (int64_t)(t.row0 + x.row[r]) * a.ld + (int64_t)g * dh + d;
-      *reinterpret_cast<f4u *>(a.ko + at) = k[r], *reinterpret_cast<f4u *>(a.vo + at) = v[r];
+      __builtin_nontemporal_store(f4u(k[r]), reinterpret_cast<f4u *>(a.ko + at));
+      __builtin_nontemporal_store(f4u(v[r]), reinterpret_cast<f4u *>(a.vo + at));
     }
   });
 }
