@@ -40,9 +40,10 @@ struct Group {
 // wave that share a group's rows are 2^lanes neighbours, d >= dh for those past the head.
 //
 // A workgroup has one tile and one head.  Bound by memory: 28 thousand tokens of 8 heads of 128 in 8 bits,
-// 290 MB each way, are written in 79 us (3.7 TB/s) and read in 53 (5.5 TB/s); 452 tokens of 8 heads of 64
-// in fp32 take 4 us each, latency.  Slot by slot, without groups: 249 us in place of 132 for both, and 19.9
-// in place of 10.3; a workgroup with all heads of its tokens side by side: 141 in place of 132.
+// 290 MB each way, are written in 57 us (5.1 TB/s) and read in 44 (6.5 TB/s); 452 tokens of 8 heads of 64
+// in fp32 take 4 us each, latency.  The rows go past the caches, of which they would take all: 79 and 53 us
+// through them (the codes go through them: 11 us more past).  Before that, slot by slot, without groups,
+// 249 us in place of 132 for both; with all heads of its tokens in a workgroup 141.
 template <class F>
 __device__ __forceinline__ void for_groups(const Cache &c, const SeqTile &t, int g, const int32_t *ends, int lanes, F &&f) {
   const int rows = min(t.len - t.t0, kTile), d = 4 * (threadIdx.x & ((1 << lanes) - 1));

@@ -21,8 +21,8 @@
 // that finishes last of up to 16 adds theirs in order, the last of those groups the groups': no
 // workgroup waits, and the order of the sums does not depend on who is last.
 //
-// 5.2 GB of fp32 cache (96 sequences of 6000 and 8000 tokens, 8 heads of 128) are read in 845 to 868 us,
-// 6.0 TB/s and above (a large copy: 5.54); 134 MB (131072 tokens of one head) in 37, 3.6 TB/s; 70 MB of
+// 5.2 GB of fp32 cache (96 sequences of 6000 and 8000 tokens, 8 heads of 128) are read in 780 to 810 us,
+// 6.5 TB/s and above (a large copy: 5.54); 134 MB (131072 tokens of one head) in 37, 3.6 TB/s; 70 MB of
 // 8-bit cache of 40 sequences of 1 to 5000 tokens in 35; 333 tokens in 11.  In the short ones the way from the lengths to the
 // table, the tokens and the joins, each waiting for the one before, is what takes the time.  Loads of a
 // step into registers that a second step's leave free spilled (a wave's state, two steps' tokens): keys
@@ -51,6 +51,24 @@ struct Cache {
   const int32_t *table;
   int shift, kv_heads, dh;
 };
+
+// Loads past the caches, where what is read is more than they keep until the next step.
+template <class T, bool PAST>
+__device__ __forceinline__ T load(const char *p) {
+  if constexpr (PAST) return __builtin_nontemporal_load(reinterpret_cast<const T *>(p));
+  return *reinterpret_cast<const T *>(p);
+}
+// f(std::bool_constant<past>) with both kinds of loads kept apart, which the compiler would make one.
+template <class F>
+__device__ __forceinline__ void by_kind(bool past, F &&f) {
+  if (past) {
+    asm volatile("" ::: "memory");
+    f(std::true_type{});
+    asm volatile("" ::: "memory");
+  } else {
+    f(std::false_type{});
+  }
+}
 
 struct SplitArgs {
   Cache c;
@@ -158,47 +176,53 @@ struct State {
   static __device__ __forceinline__ int64_t row_of(const Cache &c, int kv, int64_t pos, int page) {
     return paging::page_base(max(page, 0), c.kv_heads, kv, c.shift, 1) + ((int)pos & ((1 << c.shift) - 1));
   }
-  static __device__ __forceinline__ void load_keys(const Cache &c, int kv, int64_t pos, const int (&pages)[NB], Load &x) {
+  static __device__ __forceinline__ void load_keys(const Cache &c, int kv, int64_t pos, const int (&pages)[NB], bool past, Load &x) {
     const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
+    by_kind(past, [&](auto kind) {
+      constexpr bool PAST = decltype(kind)::value;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const int64_t row = row_of(c, kv, pos + 16 * b, pages[b]);
-      if constexpr (!INT8) {
-        const char *p = reinterpret_cast<const char *>(static_cast<const float *>(c.k) + row * c.dh);
+      for (int b = 0; b < NB; ++b) {
+        const int64_t row = row_of(c, kv, pos + 16 * b, pages[b]);
+        if constexpr (!INT8) {
+          const char *p = reinterpret_cast<const char *>(static_cast<const float *>(c.k) + row * c.dh);
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-          x.k[b][t] = *reinterpret_cast<const f4 *>(p + (unsigned)(4 * (col * c.dh + min(16 * t + 4 * g, c.dh - 4))));
-      } else {
-        const char *p = static_cast<const char *>(c.k) + row * c.dh;
+          for (int t = 0; t < NT; ++t)
+            x.k[b][t] = load<f4, PAST>(p + (unsigned)(4 * (col * c.dh + min(16 * t + 4 * g, c.dh - 4))));
+        } else {
+          const char *p = static_cast<const char *>(c.k) + row * c.dh;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-          x.kc[b][t] = *reinterpret_cast<const u2 *>(p + (unsigned)(col * c.dh + min(32 * t + 8 * g, c.dh - 8)));
-        x.ks[b] = *reinterpret_cast<const f4 *>(reinterpret_cast<const char *>(c.ks + row) + (unsigned)(16 * g));
+          for (int t = 0; t < NT; ++t)
+            x.kc[b][t] = load<u2, PAST>(p + (unsigned)(col * c.dh + min(32 * t + 8 * g, c.dh - 8)));
+          x.ks[b] = *reinterpret_cast<const f4 *>(reinterpret_cast<const char *>(c.ks + row) + (unsigned)(16 * g));
+        }
       }
-    }
+    });
   }
-  static __device__ __forceinline__ void load_values(const Cache &c, int kv, int64_t pos, const int (&pages)[NB], Load &x) {
+  static __device__ __forceinline__ void load_values(const Cache &c, int kv, int64_t pos, const int (&pages)[NB], bool past, Load &x) {
     const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
+    by_kind(past, [&](auto kind) {
+      constexpr bool PAST = decltype(kind)::value;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const int64_t row = row_of(c, kv, pos + 16 * b, pages[b]);
-      if constexpr (!INT8) {
-        const char *p = reinterpret_cast<const char *>(static_cast<const float *>(c.v) + row * c.dh);
+      for (int b = 0; b < NB; ++b) {
+        const int64_t row = row_of(c, kv, pos + 16 * b, pages[b]);
+        if constexpr (!INT8) {
+          const char *p = reinterpret_cast<const char *>(static_cast<const float *>(c.v) + row * c.dh);
 #pragma unroll
-        for (int u = 0; u < NU; ++u)
+          for (int u = 0; u < NU; ++u)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            x.v[b][r][u] = *reinterpret_cast<const f4 *>(
-                p + r * c.dh * 4 + (unsigned)(4 * (4 * g * c.dh + min(64 * u + 4 * col, c.dh - 4))));
-      } else {
-        x.vs[b] = *reinterpret_cast<const f4 *>(reinterpret_cast<const char *>(c.vs + row) + (unsigned)(16 * g));
-        // the four slots 4 g .. + 3, columns 4 col .. + 3
-        const char *p = static_cast<const char *>(c.v) + row * c.dh;
+            for (int r = 0; r < 4; ++r)
+              x.v[b][r][u] = load<f4, PAST>(
+                  p + r * c.dh * 4 + (unsigned)(4 * (4 * g * c.dh + min(64 * u + 4 * col, c.dh - 4))));
+        } else {
+          x.vs[b] = *reinterpret_cast<const f4 *>(reinterpret_cast<const char *>(c.vs + row) + (unsigned)(16 * g));
+          // the four slots 4 g .. + 3, columns 4 col .. + 3
+          const char *p = static_cast<const char *>(c.v) + row * c.dh;
 #pragma unroll
-        for (int u = 0; u < NU; ++u)
-          x.vc[b][u] = *reinterpret_cast<const u4 *>(p + (unsigned)(4 * (g * c.dh + min(64 * u + 4 * col, c.dh - 4))));
+          for (int u = 0; u < NU; ++u)
+            x.vc[b][u] = load<u4, PAST>(p + (unsigned)(4 * (g * c.dh + min(64 * u + 4 * col, c.dh - 4))));
+        }
       }
-    }
+    });
   }
 
   // The loaded keys' scores, in base 2.
@@ -476,6 +500,9 @@ __global__ void __launch_bounds__(64 * kWaves, 2) split_rows(SplitArgs a) {
   const int shares = (int)min((int64_t)a.shares, units), p = blockIdx.x / (a.c.kv_heads * a.blocks);
   if (p >= shares) return;
   const int64_t lo = first_unit(p, units, shares), hi = first_unit(p + 1, units, shares);
+  // What all workgroups read against the 256 MB of the last cache.  Past it on MI355X: 5.2 GB in 784 us in
+  // place of 866; 70 MB, which that cache holds until the next step, in 42 in place of 38.
+  const bool past = units * kUnit * (INT8 ? 2 : 8) * a.c.kv_heads * a.c.dh > int64_t{256} << 20;
   const int64_t stride = (int64_t)a.c.kv_heads * a.blocks;  // workgroup q of this block is hc + q stride
 
   // This workgroup's part of the j-th sequence of those in LDS.
@@ -541,7 +568,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) split_rows(SplitArgs a) {
         const int head = cb * 16 + (lane & 15);
         const auto q = S::ask(a, i, kv * group + min(head, group - 1), head < group);
         resolve();
-        if (pos < my.end) S::load_keys(a.c, kv, pos, next, x), S::load_values(a.c, kv, pos, next, x);
+        if (pos < my.end) S::load_keys(a.c, kv, pos, next, past, x), S::load_values(a.c, kv, pos, next, past, x);
         look(pos + ahead);
         st.keep(a, q, queries);
         __builtin_amdgcn_wave_barrier();
@@ -554,11 +581,11 @@ __global__ void __launch_bounds__(64 * kWaves, 2) split_rows(SplitArgs a) {
           const bool more = pos + ahead < my.end;
           resolve();
           st.scores(a.c.dh, x, queries, s);
-          if (more) S::load_keys(a.c, kv, pos + ahead, next, x);
+          if (more) S::load_keys(a.c, kv, pos + ahead, next, past, x);
           look(pos + 2 * ahead);
           st.probabilities(pos, my.end, pages, s, full);
           st.outputs(pos, my.end, pages, full, s, x);
-          if (more) S::load_values(a.c, kv, pos + ahead, next, x);
+          if (more) S::load_values(a.c, kv, pos + ahead, next, past, x);
           pos += ahead;
         }
         __builtin_amdgcn_wave_barrier();

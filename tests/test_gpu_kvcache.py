@@ -399,6 +399,36 @@ def test_refusals(hip_ctx):
 
 
 @pytest.mark.parametrize("format", ["f32", "int8"])
+def test_more_tokens_than_the_caches_hold(hip_ctx, format):
+    """600 sequences of up to 4096 tokens on the same pages, 1.2 GB and more read by one call."""
+    c, rng, page, H, Hk, dh, n = hip_ctx, np.random.default_rng(19), 64, 4, 2, 128, 600
+    s = _Paged(c, [4096], page, Hk, dh, format, rng, wider=0)
+    k, v = rand(rng, (4096, Hk * dh)), rand(rng, (4096, Hk * dh))
+    s.cache.write(s.seqs, c.to_device(k), c.to_device(v), s.td, s.ends)
+    k, v = (_stands_for(x.reshape(4096, Hk, dh), format) for x in (k, v))
+    lengths = rng.integers(3900, 4097, n).astype(np.int32)
+    lengths[17], lengths[18] = 1, 0
+    q, out = rand(rng, (n, H * dh)), c.empty((n, H * dh))
+    td, ends, qd = c.to_device(np.repeat(s.table, n, 0)), c.to_device(lengths), c.to_device(q)
+    c._check(L.load().numrs_hip_attention_paged(c.handle, ctypes.byref(s.cache.pages), qd.ptr, H * dh, H, td.ptr,
+                                                s.table.shape[1], ends.ptr, n, out.ptr, H * dh))
+    got = out.numpy().reshape(n, H, dh)
+    assert (got[18] == 0).all()
+    for i in [0, 16, 17, 19, 300, 598, 599]:
+        m = lengths[i]
+        _check(got[i], *_attention(q[i].reshape(H, dh), k[:m], v[:m], Hk), f"row {i}")
+    # the others against float64 without the bound's arithmetic: the same 2-norm
+    K, V, Q = k.astype(np.float64), v.astype(np.float64), q.reshape(n, H, dh).astype(np.float64)
+    for h in range(H):
+        sc = Q[:, h] @ K[:, h // 2].T / math.sqrt(dh)
+        sc[np.arange(4096)[None] >= lengths[:, None]] = -np.inf
+        p = np.exp(sc - sc.max(1, keepdims=True, where=np.isfinite(sc), initial=-1e30))
+        ref = p @ V[:, h // 2] / np.maximum(p.sum(1, keepdims=True), 1e-300)
+        err = np.linalg.norm(got[:, h] - ref, axis=1) / np.maximum(np.linalg.norm(ref, axis=1), 1e-300)
+        assert np.delete(err, 18).max() <= 2e-6
+
+
+@pytest.mark.parametrize("format", ["f32", "int8"])
 def test_pages_past_32_bits(hip_ctx, format):
     """A cache of 2.2e9 values: pages whose elements, and bytes, lie past 2^31 and 2^32."""
     c, rng, page, Hk, dh, H = hip_ctx, np.random.default_rng(16), 1024, 2, 128, 6
