@@ -322,8 +322,8 @@ int packed_forward(numrs_hip_ctx *ctx, const Seqs &s, const float *q, int64_t ld
   const float alpha = kLog2e / std::sqrt((float)dh);
   const FwdArgs a{s.by_work, q, k, v, out, stats, ld_q, ld_kv, ld_out, H, Hk, dh, alpha};
   const bool few = few_blocks(ctx, s, H);
-  const tiles::ForwardArgs f{q, pk.rows, pv.rows, pk.exps, pv.exps, out, stats, ld_q, ld_out,
-                             H, Hk, dh, alpha, kMostScore};
+  tiles::ForwardArgs f{q, pk.rows, pv.rows, pk.exps, pv.exps, out, stats, ld_q, ld_out, H, Hk, dh, 0.f, 0, kMostScore};
+  f.mant = std::frexp(alpha, &f.exp);
   return with_dp(dh, [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
     tiles::pack<DP><<<(unsigned)(s.tiles * p.slots), 256, 0, ctx->stream>>>(p);

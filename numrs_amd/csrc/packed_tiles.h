@@ -56,10 +56,28 @@ __device__ __forceinline__ void split(float a, float b, unsigned &h, unsigned &m
   m = __builtin_bit_cast(unsigned, __builtin_convertvector(f2{r0, r1}, h2));
 }
 
+// The same of a c and b c, whose products are not rounded before.
+__device__ __forceinline__ void split(float a, float b, float c, unsigned &h, unsigned &m) {
+  asm("v_fma_mixlo_f16 %0, %1, %2, 0" : "=v"(h) : "v"(a), "v"(c));
+  asm("v_fma_mixhi_f16 %0, %1, %2, 0" : "+v"(h) : "v"(b), "v"(c));
+  asm("v_fma_mixlo_f16 %0, %1, %2, -%3 op_sel_hi:[0,0,1]" : "=v"(m) : "v"(a), "v"(c), "v"(h));
+  asm("v_fma_mixhi_f16 %0, %1, %2, -%3 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "+v"(m) : "v"(b), "v"(c), "v"(h));
+}
+
 struct Terms {
   h8 h, m;
 };
 
+__device__ __forceinline__ Terms split8(const float *x, float c) {
+  u4 h, m;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    unsigned a, b;
+    split(x[2 * j], x[2 * j + 1], c, a, b);
+    h[j] = a, m[j] = b;
+  }
+  return {__builtin_bit_cast(h8, h), __builtin_bit_cast(h8, m)};
+}
 __device__ __forceinline__ Terms split8(const float *x) {
   u4 h, m;
 #pragma unroll
@@ -76,6 +94,12 @@ __device__ __forceinline__ void mma(f16 &acc, const Terms &a, const Terms &b) {
   acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.m, b.h, acc, 0, 0, 0);
   acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, b.m, acc, 0, 0, 0);
   acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, b.h, acc, 0, 0, 0);
+}
+
+// The power of two that puts a largest magnitude into [2^11, 2^12). Not above 126, where its inverse is
+// still normal: fp16's smallest step is then below fp32's, and the terms hold all of a smaller value.
+__device__ __forceinline__ int exponent_for(float big) {
+  return big > 0.f ? min(12 - __builtin_amdgcn_frexp_expf(big), 126) : 0;
 }
 
 // Row of a 32x32 result that register i of lane group g holds.
@@ -131,8 +155,8 @@ struct RowValues {
       for (int j = 0; j < 4; ++j) x[s][j] = lo[j], x[s][4 + j] = hi[j];
     }
   }
-  // Splits it times 2^e, with e for the row's largest magnitude; odd: see kOdd.
-  __device__ __forceinline__ int split_into(Terms (&t)[DP / 16], float most, bool &odd) {
+  // Splits it times `by` 2^e, with e for the row's largest magnitude; odd: see kOdd.
+  __device__ __forceinline__ int split_into(Terms (&t)[DP / 16], float most, bool &odd, float by = 1.f) {
     float big = 0.f;
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s)
@@ -142,13 +166,10 @@ struct RowValues {
         big = fmaxf(big, fabsf(x[s][j]));
       }
     big = half_pair(big, [](float a, float b) { return fmaxf(a, b); });
-    const int e = big > 0.f ? min(12 - __builtin_amdgcn_frexp_expf(big), 140) : 0;
+    const int e = exponent_for(big);
+    by = __builtin_amdgcn_ldexpf(by, e);
 #pragma unroll
-    for (int s = 0; s < DP / 16; ++s) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[s][j] = __builtin_amdgcn_ldexpf(x[s][j], e);
-      t[s] = split8(x[s]);
-    }
+    for (int s = 0; s < DP / 16; ++s) t[s] = split8(x[s], by);
     return e;
   }
 };
@@ -231,8 +252,7 @@ __global__ void __launch_bounds__(256) pack(PackArgs a) {
     if (tid == 0) s.exps[(int64_t)tile * s.heads + head] = kOdd;
     return;
   }
-  // below 2^-128 the factor itself would pass 2^140, and its inverse fp32's smallest
-  const int e = big > 0.f ? min(12 - __builtin_amdgcn_frexp_expf(big), 140) : 0;
+  const int e = exponent_for(big);
   if (tid == 0) s.exps[(int64_t)tile * s.heads + head] = e;
   if (s.stats != nullptr && tid < kTile) {
     float m = INFINITY, d = 0.f;
@@ -244,12 +264,11 @@ __global__ void __launch_bounds__(256) pack(PackArgs a) {
     *reinterpret_cast<f2 *>(s.rowstat + (((int64_t)tile * s.heads + head) * kTile + tid) * 2) = f2{m, d};
   }
   const int64_t at = ((int64_t)tile * s.heads + head) * S::kBytes;
+  const float by = __builtin_amdgcn_ldexpf(1.f, e);
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
     const int row = (i * 256 + tid) / NC, c = (i * 256 + tid) % NC;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[i][j] = __builtin_amdgcn_ldexpf(v[i][j], e);
-    const Terms p = split8(v[i]);
+    const Terms p = split8(v[i], by);
     char *o = s.rows + at + (row >> 5) * S::kHalf + (c >> 1) * 2048 + place(c & 1, row & 31);
     *reinterpret_cast<h8 *>(o) = p.h;
     *reinterpret_cast<h8 *>(o + 1024) = p.m;
@@ -302,7 +321,9 @@ struct ForwardArgs {
   float *out, *stats;
   int64_t ld_q, ld_out;
   int heads, kv_heads, dh;
-  float alpha, most;  // log2(e) / sqrt(dh); a query's largest magnitude
+  float mant;  // log2(e) / sqrt(dh) is mant 2^exp, mant in [0.5, 1)
+  int exp;
+  float most;  // a query's largest magnitude
 };
 
 // Four waves walk the keys before a block of query rows: Z = 1, one stretch of keys for 32 rows a wave
@@ -349,8 +370,12 @@ __device__ __forceinline__ void join_sets(f16 *const (&x)[N], char *lds, int r, 
   }
 }
 
-// S^T = K Q^T leaves a query's scores in two lanes; p = 2^(s - m + 7) against a reference m that moves
-// only when a score passes it by 2^8 (so that p fits fp16), O^T += V^T P^T.
+// S^T = K Q^T leaves a query's scores in two lanes. The scale's mantissa is in the queries' terms, so that a
+// score in base 2 is its sum times a power of two, exactly, and 2^(score - x) takes one fma however large
+// the score: the largest's own exponent is never off by a product's rounding, which from 2^28 on would pass
+// what fp16 holds. O^T += V^T P^T with P = 2^(score - top + 14) for the stage's largest score `top`, whatever
+// the row's before: the split's smallest step, 2^-24, is then 2^-38 of the stage's largest probability. Sums
+// are relative to a reference m that moves only when a score passes it by 2^8.
 //
 // 8192 tokens, 16 heads of 128 on 4: 0.77 to 0.83 ms by card, 330 to 357 TFLOP/s of fp32 work and three
 // times that on the fp16 matrix cores, which are busy 64 % of the cycles at the 1.6 GHz that the card's
@@ -377,7 +402,7 @@ __device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile
   qx.load(a.q + (int64_t)(t.row0 + q0 + c) * a.ld_q + (int64_t)h * a.dh, q0 + c < t.len, a.dh, hi);
   for (int i = tid; i <= last; i += 256)
     odd |= a.ek[kv0 + (int64_t)i * a.kv_heads] == kOdd || a.ev[kv0 + (int64_t)i * a.kv_heads] == kOdd;
-  const int eq = qx.split_into(q, a.most, odd);
+  const int eq = qx.split_into(q, a.most, odd, a.mant);
   if (__syncthreads_or(odd)) return false;
   const bool live = q0 < t.len;
   const int ro = place(hi, c), co = columns_place(lane);
@@ -420,7 +445,7 @@ __device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile
       for (int kb = 0; kb < KB; ++kb) x[kb] = y[kb];
     }
     // an underflow of f must not make -inf * f NaN
-    const float f = fmaxf(__builtin_amdgcn_ldexpf(a.alpha, -(eq + ek)), 1.17549435e-38f);
+    const float f = fmaxf(__builtin_amdgcn_ldexpf(1.f, a.exp - eq - ek), 1.17549435e-38f);
     if (key0 + 32 * KB > q0 + 1) {  // keys after a row of the wave
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
@@ -430,10 +455,10 @@ __device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile
     }
     float most = over16(s[0], [](float x, float y) { return fmaxf(x, y); });
     if constexpr (KB == 2) most = fmaxf(most, over16(s[1], [](float x, float y) { return fmaxf(x, y); }));
-    most *= f;
+    most = half_pair(most, [](float x, float y) { return fmaxf(x, y); }) * f;
     top = fmaxf(top, most);
     if (__any(most > m + 8.f)) {
-      const float now = fmaxf(m, half_pair(most, [](float x, float y) { return fmaxf(x, y); }));
+      const float now = fmaxf(m, most);
       const float r = __builtin_amdgcn_exp2f(m - now);
       m = now;
       l *= r;
@@ -443,18 +468,19 @@ __device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile
         for (int e = 0; e < 16; ++e) o[b][e] *= r;
     }
     Terms p[KB][2];
-    const float shift = 7.f - m;
+    // from 2^24 on, where a float's steps pass 14, P is at most 1; every other score is then 2 below or more
+    const float ref = fabsf(most) < 0x1p24f ? most - 14.f : most, back = __builtin_amdgcn_exp2f(ref - m);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[kb][e] = __builtin_amdgcn_exp2f(fmaf(s[kb][e], f, shift));
-      l += over16(s[kb], [](float x, float y) { return x + y; });
+      for (int e = 0; e < 16; ++e) s[kb][e] = __builtin_amdgcn_exp2f(fmaf(s[kb][e], f, -ref));
+      l = fmaf(over16(s[kb], [](float x, float y) { return x + y; }), back, l);
       float x[16];
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[e] = s[kb][e];
       p[kb][0] = split8(x), p[kb][1] = split8(x + 8);
     }
-    const float fv = __builtin_amdgcn_ldexpf(1.f, -ev);
+    const float fv = __builtin_amdgcn_ldexpf(back, -ev);
     constexpr int kSteps = 2 * KB;  // of 16 keys
     Terms v = columns_of(vf, 0, 0, co);
 #pragma unroll
@@ -475,7 +501,6 @@ __device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile
   }
   const int row = q0 + c;
   l = half_pair(l, [](float x, float y) { return x + y; });
-  top = half_pair(top, [](float x, float y) { return fmaxf(x, y); });
   if constexpr (Z == 2) {
     // both sets relative to the larger reference
     __syncthreads();
@@ -515,7 +540,7 @@ __device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile
   if (a.stats != nullptr && hi == 0) {
     // relative to the largest score
     float *st = a.stats + ((int64_t)(t.row0 + row) * a.heads + h) * 2;
-    st[0] = top, st[1] = l * __builtin_amdgcn_exp2f(m - 7.f - top);
+    st[0] = top, st[1] = l * __builtin_amdgcn_exp2f(m - top);
   }
   return true;
 }

@@ -1,0 +1,96 @@
+"""Packed attention where magnitudes differ: large scores, tokens far above their neighbours, values of
+zero beside small ones, keys that hardly any row attends to, and what the row kernels take.
+
+Against float64 with the bounds of test_gpu_packed.py (u = 2^-24, an operation counted at 2u), with two
+differences: a score's error counts the products that are not zero, and a row's probabilities are off by
+what the scores of the keys that it attends to are off by: a key of probability below 2^-100 takes no part,
+and a row whose largest score stands out by more than 200 and both scores' errors is that key's alone,
+p = 1, whatever the scores' rounding."""
+import math
+
+import numpy as np
+import pytest
+
+from test_gpu_packed import U2, _Call, _check
+
+pytestmark = pytest.mark.gpu
+
+NAMES = ("out", "dq", "dk", "dv")
+
+
+def _ref(call, settled=False):
+    """{name: (value, bound)} of the call's out, dq, dk, dv. settled: for each row and head whether its
+    largest score stands out; the other rows must have no gradient."""
+    H, Hk, dh, T = call.H, call.Hk, call.dh, call.T
+    q, k, v = (p[:T].astype(np.float64) for p in call.parts(call.x))
+    g = call.g[:T, call.pad:].astype(np.float64)
+    a, G, at = 1 / math.sqrt(dh), H // Hk, 0
+    res = {n: (np.zeros(x.shape), np.zeros(x.shape)) for n, x in zip(NAMES, (q, q, k, v))}
+    alone = np.zeros((T, H), bool)
+    for n in call.lengths:
+        rows = slice(at, at + n)
+        at += n
+        if n == 0:
+            continue
+        mask = np.tril(np.ones((n, n), bool))
+        for h in range(H):
+            c, ck = slice(h * dh, h * dh + dh), slice(h // G * dh, h // G * dh + dh)
+            Q, K, V, O = q[rows, c], k[rows, ck], v[rows, ck], g[rows, c]
+            s = np.where(mask, Q @ K.T * a, -np.inf)
+            terms = min((Q != 0).sum(1).max(), (K != 0).sum(1).max())
+            e = U2 * (terms + 8) * a * np.where(mask, abs(Q) @ abs(K).T, 0)
+            p = np.exp(s - s.max(1, keepdims=True))
+            p /= p.sum(1, keepdims=True)
+            f = 2 * np.where(p > 2.0 ** -100, e, 0).max(1, keepdims=True) + U2 * (n + 8)
+            top = s.argmax(1)
+            lead = s.max(1) - e[np.arange(n), top]
+            rest = s + e
+            rest[np.arange(n), top] = -np.inf
+            one = lead - rest.max(1) > 200
+            alone[rows, h] = one
+            f[one] = 0
+            out = p @ V
+            out_err = (p * f) @ abs(V) + U2 * (n + 8) * (p @ abs(V))
+            r = O @ V.T
+            D = (O * out).sum(1, keepdims=True)
+            D_err = (abs(O) * out_err).sum(1, keepdims=True) + U2 * (dh + 8) * (abs(O) * abs(out)).sum(1, keepdims=True)
+            ds = p * (r - D)
+            ds_err = p * (f * abs(r - D) + U2 * (dh + 8) * (abs(O) @ abs(V).T) + D_err)
+            for name, s_, x, err in (("out", c, out, out_err),
+                                     ("dq", c, a * (ds @ K), a * (ds_err + U2 * (n + 8) * abs(ds)) @ abs(K)),
+                                     ("dk", ck, a * (ds.T @ Q), a * (ds_err + U2 * (n * G + 8) * abs(ds)).T @ abs(Q)),
+                                     ("dv", ck, p.T @ O, (p * (f + U2 * (n * G + 8))).T @ abs(O))):
+                res[name][0][rows, s_] += x
+                res[name][1][rows, s_] += err
+    return (res, alone) if settled else res
+
+
+def _run(call):
+    call.upload()
+    out = call.forward()[:call.T]
+    d = call.backward(call.c.empty(call.x.shape))
+    return dict(zip(NAMES, (out, *(p[:call.T] for p in call.parts(d)))))
+
+
+def _within(got, ref, what, rows=slice(None)):
+    """Every value within its bound."""
+    x, err = (r[rows] for r in ref)
+    d = abs(got[rows].astype(np.float64) - x)
+    bad = ~(d <= err + 1e-37)
+    assert not bad.any(), f"{what}: {bad.sum()} of {bad.size} outside their bounds, by up to " \
+                          f"{np.nanmax(d / (err + 1e-300)):.2g}"
+
+
+@pytest.mark.parametrize("dh", [64, 40, 128])
+@pytest.mark.parametrize("size", [20, 300, 3e3, 1e5, 1e10, 1e14])
+def test_large_scores_forward(hip_ctx, size, dh):
+    """q and k times `size`: scores of 400 to 1e28. A row whose largest score stands out has that key's
+    value, and a token that sees only itself its own."""
+    call = _Call(hip_ctx, [1] * 40 + [2, 64, 65, 150], 4, 2, dh, np.random.default_rng(int(math.log2(size)) + dh))
+    call.x[:, :call.wq + call.wk] *= np.float32(size)
+    ref, alone = _ref(call, settled=True)
+    assert alone[:40].all() and alone.mean() > (0.3 if size < 100 else 0.9)
+    call.upload()
+    out = call.forward().reshape(call.T, call.H, dh)
+    x, err = (r.reshape(out.shape)[alone] for r in ref["out"])
+    _within(out[alone], (x, err), "out")
