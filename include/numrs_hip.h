@@ -369,7 +369,7 @@ int64_t numrs_hip_seqs_total(const numrs_hip_seqs *seqs); /* the sum of the leng
  * other token's values than those it attends to, finite or not.  Operands are
  * held to 2^-23 of a value, and to 2^-36 of the largest magnitude among its
  * tile of 64 tokens of its head; 64 or 128 rows that see a value that is not
- * finite, a query or key from 2^50 or a value or gradient from 2^90 on take
+ * finite, a query or key from 2^50 or a value or gradient from 2^80 on take
  * plain fp32 arithmetic instead, some 150 times slower.
  * Backward, with r = dout . v and D = dout . out:
  *   dv = sum p dout,  ds = p (r - D) / sqrt(dh),  dq = sum ds k,  dk = sum ds q,

@@ -5,7 +5,7 @@
 //
 // packed_tiles.h has the kernels that ordinary values take.  The row kernels here are the plain fp32 form,
 // a wave a row, for blocks that meet a value which those cannot take: not finite, or from 2^50 (queries and
-// keys) or 2^90 (values and the output's gradient) on.  They read every key a row at a time, some 150 times
+// keys) or 2^80 (values and the output's gradient) on.  They read every key a row at a time, some 150 times
 // slower (8192 tokens, 16 heads of 128, a value at their start infinite: 134 ms against 0.8; rows that are
 // NaN throughout end at the first such score), and are there so that such a value does to the rows that
 // attend to it what fp32 arithmetic does, and nothing to the others.
@@ -259,8 +259,8 @@ int check_packed(numrs_hip_ctx *ctx, const Seqs &s, int64_t ld_q, int64_t ld_kv,
 }
 
 // Magnitudes from which a tile's products might pass fp32's range: a score of two such operands
-// stays below 2^107, a sum of 2^20 such values times 2^15 below 2^127.
-constexpr float kMostScore = 0x1p50f, kMostValue = 0x1p90f;
+// stays below 2^107, a sum of 2^20 such values times 2^22 below 2^123.
+constexpr float kMostScore = 0x1p50f, kMostValue = 0x1p80f;
 
 // Whether the kernels take blocks of 64 rows whose keys two sets of waves share, in place of 128: where
 // there are fewer than two of the latter for each CU, and the longest walk decides.  Forward | query rows |

@@ -375,7 +375,7 @@ __device__ __forceinline__ void join_sets(f16 *const (&x)[N], char *lds, int r, 
 // the score: the largest's own exponent is never off by a product's rounding, which from 2^28 on would pass
 // what fp16 holds. O^T += V^T P^T with P = 2^(score - top + 14) for the stage's largest score `top`, whatever
 // the row's before: the split's smallest step, 2^-24, is then 2^-38 of the stage's largest probability. Sums
-// are relative to a reference m that moves only when a score passes it by 2^8.
+// are 2^14 times those relative to a reference m, which moves only when a score passes it by 2^8.
 //
 // 8192 tokens, 16 heads of 128 on 4: 0.77 to 0.83 ms by card, 330 to 357 TFLOP/s of fp32 work and three
 // times that on the fp16 matrix cores, which are busy 64 % of the cycles at the 1.6 GHz that the card's
@@ -469,7 +469,9 @@ __device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile
     }
     Terms p[KB][2];
     // from 2^24 on, where a float's steps pass 14, P is at most 1; every other score is then 2 below or more
-    const float ref = fabsf(most) < 0x1p24f ? most - 14.f : most, back = __builtin_amdgcn_exp2f(ref - m);
+    const bool far = fabsf(most) >= 0x1p24f;
+    const float ref = far ? most : most - 14.f;
+    const float back = __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(most - m), far ? 14 : 0);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
@@ -540,7 +542,7 @@ __device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile
   if (a.stats != nullptr && hi == 0) {
     // relative to the largest score
     float *st = a.stats + ((int64_t)(t.row0 + row) * a.heads + h) * 2;
-    st[0] = top, st[1] = l * __builtin_amdgcn_exp2f(m - top);
+    st[0] = top, st[1] = l * 0x1p-14f * __builtin_amdgcn_exp2f(m - top);
   }
   return true;
 }

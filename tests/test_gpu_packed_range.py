@@ -5,7 +5,12 @@ Against float64 with the bounds of test_gpu_packed.py (u = 2^-24, an operation c
 differences: a score's error counts the products that are not zero, and a row's probabilities are off by
 what the scores of the keys that it attends to are off by: a key of probability below 2^-100 takes no part,
 and a row whose largest score stands out by more than 200 and both scores' errors is that key's alone,
-p = 1, whatever the scores' rounding."""
+p = 1, whatever the scores' rounding.
+
+The kernels hold an operand to 2^-23 of it, which the counts above cover, or to 2^-36 of the largest magnitude
+of its 64 tokens, as the header says: a tile is scaled so that this one lies in [2^11, 2^12), where half a
+step of the second fp16 term, at least 2^-25, is at most 2^-36 of it. What that leaves of a value alone (a
+probability of 1 and a value of 1e-5 beside ones of 4) is part of the bound."""
 import math
 
 import numpy as np
@@ -16,6 +21,11 @@ from test_gpu_packed import U2, _Call, _check
 pytestmark = pytest.mark.gpu
 
 NAMES = ("out", "dq", "dk", "dv")
+
+
+def _held(x):
+    """The largest magnitude of each row's 64 tokens."""
+    return np.repeat([abs(x[i:i + 64]).max() for i in range(0, len(x), 64)], 64)[:len(x), None]
 
 
 def _ref(call, settled=False):
@@ -50,7 +60,7 @@ def _ref(call, settled=False):
             alone[rows, h] = one
             f[one] = 0
             out = p @ V
-            out_err = (p * f) @ abs(V) + U2 * (n + 8) * (p @ abs(V))
+            out_err = (p * f) @ abs(V) + U2 * (n + 8) * (p @ abs(V)) + 2.0 ** -36 * (p @ _held(V))
             r = O @ V.T
             D = (O * out).sum(1, keepdims=True)
             D_err = (abs(O) * out_err).sum(1, keepdims=True) + U2 * (dh + 8) * (abs(O) * abs(out)).sum(1, keepdims=True)
@@ -59,7 +69,7 @@ def _ref(call, settled=False):
             for name, s_, x, err in (("out", c, out, out_err),
                                      ("dq", c, a * (ds @ K), a * (ds_err + U2 * (n + 8) * abs(ds)) @ abs(K)),
                                      ("dk", ck, a * (ds.T @ Q), a * (ds_err + U2 * (n * G + 8) * abs(ds)).T @ abs(Q)),
-                                     ("dv", ck, p.T @ O, (p * (f + U2 * (n * G + 8))).T @ abs(O))):
+                                     ("dv", ck, p.T @ O, (p * (f + U2 * (n * G + 8))).T @ abs(O) + 2.0 ** -36 * (p.T @ _held(O)))):
                 res[name][0][rows, s_] += x
                 res[name][1][rows, s_] += err
     return (res, alone) if settled else res
