@@ -103,6 +103,10 @@ struct BwdArgs {
   int64_t ld_q, ld_kv, ld_out;
 };
 
+// A score less the row's largest. Where the tiles had the row, whose sums run in another order, it may come
+// out above 0, which at large scores would be any power of two. NaN stays.
+__device__ __forceinline__ float at_most_0(float x) { return x > 0.f ? 0.f : x; }
+
 __device__ __forceinline__ void put(float *p, float v, int accumulate) { *p = accumulate ? *p + v : v; }
 
 // One wave: dq of query row r and head h, in plain fp32.  x: two rows of LDS.
@@ -125,7 +129,7 @@ __device__ void row_dq(const BwdArgs &b, const tiles::BackwardArgs &a, const Seq
     const int j = j0 + lane, n = min(64, r + 1 - j0);
     float ds = 0.f;
     if (lane < n) {
-      const float p = exp2f(dot_row(x, k + j * b.ld_kv, a.dh) * a.alpha - m) / l;
+      const float p = exp2f(at_most_0(dot_row(x, k + j * b.ld_kv, a.dh) * a.alpha - m)) / l;
       ds = p * (dot_row(x + 128, v + j * b.ld_kv, a.dh) - D);
     }
     float t0 = 0.f, t1 = 0.f;
@@ -158,7 +162,7 @@ __device__ void row_dkv(const BwdArgs &b, const tiles::BackwardArgs &a, const Se
       if (lane < n) {
         const int64_t i = t.row0 + i0 + lane;
         const float *st = b.stats + (i * a.heads + h) * 2;
-        p = exp2f(dot_row(x, q + i * b.ld_q, a.dh) * a.alpha - st[0]) / st[1];
+        p = exp2f(at_most_0(dot_row(x, q + i * b.ld_q, a.dh) * a.alpha - st[0])) / st[1];
         ds = p * (dot_row(x + 128, go + i * b.ld_out, a.dh) - dot_row(out + i * b.ld_out, go + i * b.ld_out, a.dh));
       }
       float tk0 = 0.f, tk1 = 0.f, tv0 = 0.f, tv1 = 0.f;
@@ -294,8 +298,8 @@ struct Packed {
     exps = reinterpret_cast<int *>(rows + image);
     return NUMRS_HIP_OK;
   }
-  tiles::Source source(const float *x, int64_t ld, int heads, float most) const {
-    return {x, ld, rows, exps, most, heads, nullptr, nullptr, nullptr};
+  tiles::Source source(const float *x, int64_t ld, int heads, float most, float by = 1.f) const {
+    return {x, ld, rows, exps, most, by, heads, nullptr, nullptr, nullptr};
   }
 };
 
@@ -371,17 +375,19 @@ int packed_backward(numrs_hip_ctx *ctx, const Seqs &s, const float *q, int64_t l
   const size_t part = (size_t)s.total * H * dh * sizeof(float);
   if (keys && each < group)
     if (int rc = parts.alloc(((dk != nullptr) + (dv != nullptr)) * part)) return rc;
+  const float alpha = kLog2e / std::sqrt((float)dh), scale = 1.0f / std::sqrt((float)dh);
+  int exp;
+  const float mant = std::frexp(alpha, &exp), scale_q = (float)((double)scale / mant);
   tiles::PackArgs p{s.in_order,
                     {pk.source(k, ld_kv, Hk, kMostScore), pv.source(v, ld_kv, Hk, kMostValue),
-                     pq.source(q, ld_q, H, kMostScore), pg.source(dout, ld_out, H, kMostValue)},
+                     pq.source(q, ld_q, H, kMostScore, mant), pg.source(dout, ld_out, H, kMostValue)},
                     2 * Hk + (keys ? 2 * H : 0), dh};
   p.src[3].out = out, p.src[3].stats = stats, p.src[3].rowstat = rowstat.f();
-  const float alpha = kLog2e / std::sqrt((float)dh), scale = 1.0f / std::sqrt((float)dh);
   const bool few = few_blocks(ctx, s, H);
   BwdArgs b{few ? s.few_by_work : s.by_work, q, k, v, out, dout, stats, ld_q, ld_kv, ld_out};
   tiles::BackwardArgs a{q, k, v, out, dout, stats, ld_q, ld_kv, ld_out, pq.rows, pk.rows, pv.rows, pg.rows,
                         pq.exps, pk.exps, pv.exps, pg.exps, rowstat.f(), dq, dk, dv, ld_q, ld_kv, ld_kv, s.total,
-                        H, Hk, dh, accumulate, accumulate, each, alpha, scale, kMostScore, kMostValue};
+                        H, Hk, dh, accumulate, accumulate, each, alpha, scale, mant, exp, scale_q, kMostScore, kMostValue};
   return with_dp(dh, [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
     tiles::pack<DP><<<(unsigned)(s.tiles * p.slots), 256, 0, ctx->stream>>>(p);

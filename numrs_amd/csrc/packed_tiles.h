@@ -89,10 +89,13 @@ __device__ __forceinline__ Terms split8(const float *x) {
   return {__builtin_bit_cast(h8, h), __builtin_bit_cast(h8, m)};
 }
 
-// acc += a b, the small products first.
+// acc += a b, the small products first: a's second term's, then b's. SWAPPED: b's first, so that a b^T and b a^T
+// have the same bits.
+template <bool SWAPPED = false>
 __device__ __forceinline__ void mma(f16 &acc, const Terms &a, const Terms &b) {
-  acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.m, b.h, acc, 0, 0, 0);
+  if constexpr (!SWAPPED) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.m, b.h, acc, 0, 0, 0);
   acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, b.m, acc, 0, 0, 0);
+  if constexpr (SWAPPED) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.m, b.h, acc, 0, 0, 0);
   acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, b.h, acc, 0, 0, 0);
 }
 
@@ -155,8 +158,8 @@ struct RowValues {
       for (int j = 0; j < 4; ++j) x[s][j] = lo[j], x[s][4 + j] = hi[j];
     }
   }
-  // Splits it times `by` 2^e, with e for the row's largest magnitude; odd: see kOdd.
-  __device__ __forceinline__ int split_into(Terms (&t)[DP / 16], float most, bool &odd, float by = 1.f) {
+  // Its largest magnitude; odd: see kOdd.
+  __device__ __forceinline__ float top(float most, bool &odd) const {
     float big = 0.f;
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s)
@@ -165,12 +168,12 @@ struct RowValues {
         odd |= !(fabsf(x[s][j]) < most);
         big = fmaxf(big, fabsf(x[s][j]));
       }
-    big = half_pair(big, [](float a, float b) { return fmaxf(a, b); });
-    const int e = exponent_for(big);
-    by = __builtin_amdgcn_ldexpf(by, e);
+    return half_pair(big, [](float a, float b) { return fmaxf(a, b); });
+  }
+  // Its terms times `by`.
+  __device__ __forceinline__ void split_into(Terms (&t)[DP / 16], float by) const {
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) t[s] = split8(x[s], by);
-    return e;
   }
 };
 
@@ -181,6 +184,7 @@ struct Source {
   char *rows;   // fragments [tiles, heads]
   int *exps;    // [tiles, heads]
   float most;   // larger magnitudes make a tile odd
+  float by;     // a factor in [0.5, 1] that the terms have besides the exponent's
   int heads;
   // The output's gradient: its rows are divided by their softmax sum l, which turns the backward's
   // p into 2^(s - m), and the rows' references and totals go to `rowstat` [tiles, heads, 64]: (m,
@@ -264,7 +268,7 @@ __global__ void __launch_bounds__(256) pack(PackArgs a) {
     *reinterpret_cast<f2 *>(s.rowstat + (((int64_t)tile * s.heads + head) * kTile + tid) * 2) = f2{m, d};
   }
   const int64_t at = ((int64_t)tile * s.heads + head) * S::kBytes;
-  const float by = __builtin_amdgcn_ldexpf(1.f, e);
+  const float by = __builtin_amdgcn_ldexpf(s.by, e);
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
     const int row = (i * 256 + tid) / NC, c = (i * 256 + tid) % NC;
@@ -377,6 +381,10 @@ __device__ __forceinline__ void join_sets(f16 *const (&x)[N], char *lds, int r, 
 // the row's before: the split's smallest step, 2^-24, is then 2^-38 of the stage's largest probability. Sums
 // are 2^14 times those relative to a reference m, which moves only when a score passes it by 2^8.
 //
+// The queries have the exponent that `pack` gives their 64 (two waves have a tile), as in the backward, where
+// they are packed: all three kernels then form a score from the same terms in the same order, to the same
+// bits, and a row whose largest score is all there is has p = 1.
+//
 // 8192 tokens, 16 heads of 128 on 4: 0.77 to 0.83 ms by card, 330 to 357 TFLOP/s of fp32 work and three
 // times that on the fp16 matrix cores, which are busy 64 % of the cycles at the 1.6 GHz that the card's
 // power leaves (a large fp16 library product: 1085 TFLOP/s).  13 prompts of 1 to 1290 tokens, 16 heads of
@@ -389,7 +397,7 @@ __device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile
   using S = Shape<DP>;
   using W = Walk<DP, Z>;
   constexpr int KT = W::KT, KB = W::KB, kStage = KT * DP * 4;
-  __shared__ float joint[Z == 2 ? 3 : 1][64];
+  __shared__ float joint[Z == 2 ? 3 : 1][64], tops[4];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rw = w % W::R, z = w / W::R;
   const int c = lane & 31, hi = lane >> 5, g = h / (a.heads / a.kv_heads);
@@ -402,8 +410,11 @@ __device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile
   qx.load(a.q + (int64_t)(t.row0 + q0 + c) * a.ld_q + (int64_t)h * a.dh, q0 + c < t.len, a.dh, hi);
   for (int i = tid; i <= last; i += 256)
     odd |= a.ek[kv0 + (int64_t)i * a.kv_heads] == kOdd || a.ev[kv0 + (int64_t)i * a.kv_heads] == kOdd;
-  const int eq = qx.split_into(q, a.most, odd, a.mant);
+  const float row_top = qx.top(a.most, odd);
+  tops[w] = wave_max(row_top);
   if (__syncthreads_or(odd)) return false;
+  const int eq = exponent_for(fmaxf(tops[w], tops[w ^ 1]));
+  qx.split_into(q, __builtin_amdgcn_ldexpf(a.mant, eq));
   const bool live = q0 < t.len;
   const int ro = place(hi, c), co = columns_place(lane);
 
@@ -469,9 +480,9 @@ __device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile
     }
     Terms p[KB][2];
     // from 2^24 on, where a float's steps pass 14, P is at most 1; every other score is then 2 below or more
-    const bool far = fabsf(most) >= 0x1p24f;
-    const float ref = far ? most : most - 14.f;
-    const float back = __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(most - m), far ? 14 : 0);
+    const float ref = fabsf(most) < 0x1p24f ? most - 14.f : most;
+    // from the reference as rounded
+    const float back = __builtin_amdgcn_exp2f(ref - m + 14.f);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
@@ -558,6 +569,9 @@ struct BackwardArgs {
   int heads, kv_heads, dh, accumulate, acc_kv;  // acc_kv: for dk and dv
   int each;             // query heads of a workgroup of key rows: its group, or one
   float alpha, scale;   // log2(e) / sqrt(dh), 1 / sqrt(dh)
+  float mant;           // alpha is mant 2^exp, mant in [0.5, 1)
+  int exp;
+  float scale_q;        // scale / mant: of sums over the packed queries
   float most_score, most_value;  // see Source
 };
 
@@ -570,16 +584,19 @@ __device__ __forceinline__ int wave_min(int v) {
 // Scales of dS.  With V's factors 2^ev and the gradient's 2^eg, dP comes as raw = dP 2^(ev + eg),
 // below 2^31; a row's total D may come from other tiles of V than the one at hand, so both are
 // brought to the smallest ev of the sequence, and by 2^-32 below 1:
-//   dS'' = 2^15 p (raw 2^(least - ev - 32) - D 2^(eg + least - 32)) = dS 2^(eg + least - 17),
+//   dS'' = p (raw 2^(least - ev - 17) - D 2^(eg + least - 17)) = dS 2^(eg + least - 17),
 // at most 2^15 and split like any operand.
+//
+// A probability times the row's sum, from a score and the row's largest. It is at most 1 as the forward has
+// it; where the row kernels had the row, whose sums run in another order, a score may be above.
 __device__ __forceinline__ float score(float s, float f, float m) {
-  return __builtin_amdgcn_exp2f(fmaf(s, f, 15.f - m));
+  return __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(fmaf(s, f, -m)), 0.f, 1.f);
 }
 __device__ __forceinline__ float dscore(float p, float raw, float graw, float d) { return p * fmaf(raw, graw, -d); }
 
 // s = A a^T and r = B b^T of 32 rows at pa and pb; the next step's operands are asked for before this
-// one's products.
-template <int DP>
+// one's products. SWAPPED: s with the order of a A^T.
+template <int DP, bool SWAPPED>
 __device__ __forceinline__ void two_products(f16 &s, f16 &r, const char *pa, const char *pb, const Terms (&a)[DP / 16],
                                              const Terms (&b)[DP / 16], int off) {
   s = f16{}, r = f16{};
@@ -589,7 +606,7 @@ __device__ __forceinline__ void two_products(f16 &s, f16 &r, const char *pa, con
     Terms nx, ny;
     if (st + 1 < DP / 16) nx = rows_of(pa, st + 1, off), ny = rows_of(pb, st + 1, off);
     __builtin_amdgcn_sched_barrier(0);
-    mma(s, x, a[st]);
+    mma<SWAPPED>(s, x, a[st]);
     mma(r, y, b[st]);
     x = nx, y = ny;
   }
@@ -627,6 +644,7 @@ __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t,
   using S = Shape<DP>;
   constexpr int R = 4 / Z, kPart = Z * S::kHalf, kStage = 2 * kPart;
   __shared__ int least4[4];
+  __shared__ float tops[4];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rw = w % R, z = w / R;
   const int c = lane & 31, hi = lane >> 5, g = h / (a.heads / a.kv_heads);
@@ -643,11 +661,13 @@ __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t,
   }
   Terms q[S::NS], go[S::NS];
   float m = INFINITY, D = 0.f;  // a row past the sequence: p = 0
-  int eq, eg;
+  int eg;
+  RowValues<DP> qx;
+  qx.load(a.xq + row * a.ld_xq + (int64_t)h * a.dh, mine_in, a.dh, hi);
+  const float q_top = qx.top(a.most_score, odd);
+  tops[w] = wave_max(q_top);
   {
     RowValues<DP> x, o;
-    x.load(a.xq + row * a.ld_xq + (int64_t)h * a.dh, mine_in, a.dh, hi);
-    eq = x.split_into(q, a.most_score, odd);
     x.load(a.dout + row * a.ld_out + (int64_t)h * a.dh, mine_in, a.dh, hi);
     o.load(a.out + row * a.ld_out + (int64_t)h * a.dh, mine_in, a.dh, hi);
     float inv = 1.f;
@@ -664,13 +684,16 @@ __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t,
     }
     D = half_pair(D, [](float y, float z) { return y + z; }) * inv;
     odd |= !__builtin_isfinite(D);
-    eg = x.split_into(go, a.most_value, odd);
+    eg = exponent_for(x.top(a.most_value, odd));
+    x.split_into(go, __builtin_amdgcn_ldexpf(1.f, eg));
   }
   least = wave_min(least);
   if (lane == 0) least4[w] = least;
   if (__syncthreads_or(odd)) return false;
   least = min(min(least4[0], least4[1]), min(least4[2], least4[3]));
-  D = __builtin_amdgcn_ldexpf(D, eg + least - 32);
+  const int eq = exponent_for(fmaxf(tops[w], tops[w ^ 1]));
+  qx.split_into(q, __builtin_amdgcn_ldexpf(a.mant, eq));
+  D = __builtin_amdgcn_ldexpf(D, eg + least - 17);
   const int ro = place(hi, c), co = columns_place(lane);
 
   f16 x[S::NB] = {};
@@ -691,9 +714,9 @@ __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t,
     const char *kf = lds + (i & 1) * kStage + z * S::kHalf, *vf = kf + kPart;
     const int ek = scalar(a.ek + tile_of(i)), ev = scalar(a.ev + tile_of(i));
     f16 s, r;
-    two_products<DP>(s, r, kf, vf, q, go, ro);
+    two_products<DP, false>(s, r, kf, vf, q, go, ro);
     f16 p, ds;
-    const float f = __builtin_amdgcn_ldexpf(a.alpha, -(eq + ek)), graw = __builtin_amdgcn_ldexpf(1.f, least - ev - 32);
+    const float f = __builtin_amdgcn_ldexpf(1.f, a.exp - eq - ek), graw = __builtin_amdgcn_ldexpf(1.f, least - ev - 17);
 #pragma unroll
     for (int e = 0; e < 16; ++e) p[e] = score(s[e], f, m), ds[e] = dscore(p[e], r[e], graw, D);
     if (32 * kb + 31 > q0) {
@@ -755,20 +778,24 @@ __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t
       }
   }
   Terms k[S::NS], v[S::NS];
-  int ek, ev;
+  // the keys' terms as they are packed
+  const int ek = live ? scalar(a.ek + kv0 + (int64_t)(k0 / kTile) * a.kv_heads) : 0;
+  odd |= ek == kOdd;
+  int ev;
   {
     RowValues<DP> x;
     x.load(a.xk + row * a.ld_xkv + (int64_t)g * a.dh, mine_in, a.dh, hi);
-    ek = x.split_into(k, a.most_score, odd);
+    x.split_into(k, __builtin_amdgcn_ldexpf(1.f, ek));
     x.load(a.xv + row * a.ld_xkv + (int64_t)g * a.dh, mine_in, a.dh, hi);
-    ev = x.split_into(v, a.most_value, odd);
+    ev = exponent_for(x.top(a.most_value, odd));
+    x.split_into(v, __builtin_amdgcn_ldexpf(1.f, ev));
   }
   least = wave_min(least);
   if (lane == 0) least4[w] = least;
   if (__syncthreads_or(odd)) return false;
   least = min(min(least4[0], least4[1]), min(least4[2], least4[3]));
   // (a row that is smaller than its tile's largest has the larger factor; one of zeros may have less)
-  const float graw = __builtin_amdgcn_ldexpf(1.f, least - ev - 32), gd = __builtin_amdgcn_ldexpf(1.f, least - 32);
+  const float graw = __builtin_amdgcn_ldexpf(1.f, least - ev - 17), gd = __builtin_amdgcn_ldexpf(1.f, least - 17);
   const int ro = place(hi, c), co = columns_place(lane);
 
   f16 xk[S::NB] = {}, xv[S::NB] = {};
@@ -796,7 +823,7 @@ __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t
     const int64_t qt = tile_of(i);
     const int eq = scalar(a.eq + qt), eg = scalar(a.eg + qt);
     f16 s, r;
-    two_products<DP>(s, r, qf, gf, k, v, ro);
+    two_products<DP, true>(s, r, qf, gf, k, v, ro);
     float m[16], d[16];
 #pragma unroll
     for (int e = 0; e < 16; e += 2) {
@@ -804,7 +831,7 @@ __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t
       m[e] = y[0], d[e] = y[1] * gd, m[e + 1] = y[2], d[e + 1] = y[3] * gd;
     }
     f16 p, ds;
-    const float f = __builtin_amdgcn_ldexpf(a.alpha, -(eq + ek));
+    const float f = __builtin_amdgcn_ldexpf(1.f, a.exp - eq - ek);
 #pragma unroll
     for (int e = 0; e < 16; ++e) p[e] = score(s[e], f, m[e]), ds[e] = dscore(p[e], r[e], graw, d[e]);
     if (q0 < k0 + 31) {
@@ -815,8 +842,8 @@ __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t
     float y[16], z[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) y[e] = p[e], z[e] = ds[e];
-    const Terms pb[2] = {split8(y), split8(y + 8)}, sb[2] = {split8(z), split8(z + 8)};
-    const float bv = __builtin_amdgcn_ldexpf(1.f, -15 - eg), bk = __builtin_amdgcn_ldexpf(a.scale, 17 - eg - least - eq);
+    const Terms pb[2] = {split8(y, 0x1p15f), split8(y + 8, 0x1p15f)}, sb[2] = {split8(z), split8(z + 8)};
+    const float bv = __builtin_amdgcn_ldexpf(1.f, -15 - eg), bk = __builtin_amdgcn_ldexpf(a.scale_q, 17 - eg - least - eq);
     Terms ga = columns_of(gf, 0, 0, co), qa = columns_of(qf, 0, 0, co);
 #pragma unroll
     for (int nb = 0; nb < S::NB; ++nb) {

@@ -104,3 +104,34 @@ def test_large_scores_forward(hip_ctx, size, dh):
     out = call.forward().reshape(call.T, call.H, dh)
     x, err = (r.reshape(out.shape)[alone] for r in ref["out"])
     _within(out[alone], (x, err), "out")
+
+
+@pytest.mark.parametrize("dh", [64, 40, 128])
+@pytest.mark.parametrize("size", [20, 300, 3e3, 1e5, 1e10, 1e14])
+def test_large_scores_backward(hip_ctx, size, dh):
+    """The same rows' gradients: the output's gradient goes to the one key's value, and nothing but the
+    rounding of r - D to queries and keys."""
+    call = _Call(hip_ctx, [1] * 40 + [2, 64, 65, 150], 4, 2, dh, np.random.default_rng(int(math.log2(size)) + dh))
+    call.x[:, :call.wq + call.wk] *= np.float32(size)
+    alone = _ref(call, settled=True)[1]
+    call.g *= np.repeat(alone, dh, axis=1)
+    ref, got = _ref(call), _run(call)
+    for name in ("dq", "dk", "dv"):
+        x, err = ref[name]
+        # a settled row's other probabilities are below e^-200, whatever float64 has of them
+        _within(got[name], (x, err), name)
+
+
+def test_large_scores_of_many_sequences_backward(hip_ctx):
+    """20 thousand tokens that see only themselves, at every size of score: dv is the output's gradient."""
+    rng, n, H, dh = np.random.default_rng(12), 20000, 2, 64
+    call = _Call(hip_ctx, [1] * n, H, H, dh, rng)
+    call.x[:, :2 * H * dh] *= (10.0 ** rng.uniform(-2, 14, (n, 1))).astype(np.float32)
+    got = _run(call)
+    x, v, g = call.x, call.parts(call.x)[2], call.g
+    assert np.abs(got["out"] - v).max() <= 9 * U2 * np.abs(v).max()
+    assert np.abs(got["dv"] - g).max() <= 9 * U2 * np.abs(g).max()
+    # r - D: both sums of dh products of v and the gradient
+    bound = 2 * U2 * (dh + 8) * (np.abs(g) * np.abs(v)).reshape(n, H, dh).sum(2) / math.sqrt(dh)
+    for name, other in (("dq", x[:, H * dh:2 * H * dh]), ("dk", x[:, :H * dh])):
+        assert (np.abs(got[name]).reshape(n, H, dh) <= bound[:, :, None] * np.abs(other).reshape(n, H, dh)).all(), name
