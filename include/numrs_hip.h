@@ -367,7 +367,7 @@ int64_t numrs_hip_seqs_total(const numrs_hip_seqs *seqs); /* the sum of the leng
  * softmax reference and sum for the backward; NULL where none follows.  Rows
  * past the batch's total are not touched, and a row's result depends on no
  * other token's values than those it attends to, finite or not.  Operands are
- * held to 2^-23 of a value, and to 2^-36 of the largest magnitude among its
+ * held to 2^-23 of a value, and to 2^-39 of the largest magnitude among its
  * tile of 64 tokens of its head; 64 or 128 rows that see a value that is not
  * finite, a query or key from 2^50 or a value or gradient from 2^80 on take
  * plain fp32 arithmetic instead, some 150 times slower.

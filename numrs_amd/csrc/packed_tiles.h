@@ -1,9 +1,9 @@
 // Causal attention over packed sequences on the fp16 matrix cores at fp32 accuracy.
 //
 // An fp32 operand x, times a power of two that puts its 64-token tile's largest magnitude into
-// [2^11, 2^12), is the sum h + m of two fp16 values, each rounded to nearest: h holds 11 bits, x -
-// h is exact and m holds its next 11, so h + m is x within 2^-23 |x| for |x| down to 2^-14 of the
-// largest and within 2^-36 of the largest below.  Of the four products of two such operands the
+// [2^14, 2^15), is the sum h + m of two fp16 values, each rounded to nearest: h holds 11 bits, x -
+// h is exact and m holds its next 11, so h + m is x within 2^-23 |x| for |x| down to 2^-17 of the
+// largest and within 2^-39 of the largest below.  Of the four products of two such operands the
 // matrix cores form three, m h + h m + h h (the fourth is below 2^-22 of the product and of either
 // sign), each with fp32 accumulation: half of what three bf16 terms and six products take.
 // v_mfma_f32_32x32x16_f16 sums of at most 64 tokens (or one head) start from zero and are added to
@@ -42,6 +42,8 @@ __device__ __forceinline__ int scalar(const int *p) {
 // A tile's exponent where its values do not split: one that is not finite, or so large that a
 // product might pass fp32's range.  Workgroups that meet one take the row kernels' arithmetic.
 constexpr int kOdd = 1 << 20;
+// And out . dout, at its gradient's exponent: what values below 2^80 give is below 2^103.
+constexpr float kMostTotal = 0x1p110f;
 // A softmax reference before any score: below every score of a tile that is not odd.
 constexpr float kNone = -0x1p110f;
 
@@ -99,10 +101,10 @@ __device__ __forceinline__ void mma(f16 &acc, const Terms &a, const Terms &b) {
   acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, b.h, acc, 0, 0, 0);
 }
 
-// The power of two that puts a largest magnitude into [2^11, 2^12). Not above 126, where its inverse is
+// The power of two that puts a largest magnitude into [2^14, 2^15). Not above 126, where its inverse is
 // still normal: fp16's smallest step is then below fp32's, and the terms hold all of a smaller value.
 __device__ __forceinline__ int exponent_for(float big) {
-  return big > 0.f ? min(12 - __builtin_amdgcn_frexp_expf(big), 126) : 0;
+  return big > 0.f ? min(15 - __builtin_amdgcn_frexp_expf(big), 126) : 0;
 }
 
 // Row of a 32x32 result that register i of lane group g holds.
@@ -257,15 +259,18 @@ __global__ void __launch_bounds__(256) pack(PackArgs a) {
     return;
   }
   const int e = exponent_for(big);
-  if (tid == 0) s.exps[(int64_t)tile * s.heads + head] = e;
-  if (s.stats != nullptr && tid < kTile) {
+  if (tid < kTile) {
     float m = INFINITY, d = 0.f;
-    if (tid < rows) {
-      const float *st = s.stats + ((int64_t)(t.row0 + t.t0 + tid) * s.heads + head) * 2;
-      for (int c = 0; c < NC; ++c) d += part[tid][c];
-      m = st[0], d = __builtin_amdgcn_ldexpf(d / st[1], e);
+    if (s.stats != nullptr) {
+      if (tid < rows) {
+        const float *st = s.stats + ((int64_t)(t.row0 + t.t0 + tid) * s.heads + head) * 2;
+        for (int c = 0; c < NC; ++c) d += part[tid][c];
+        m = st[0], d = __builtin_amdgcn_ldexpf(d / st[1], e);
+      }
+      *reinterpret_cast<f2 *>(s.rowstat + (((int64_t)tile * s.heads + head) * kTile + tid) * 2) = f2{m, d};
     }
-    *reinterpret_cast<f2 *>(s.rowstat + (((int64_t)tile * s.heads + head) * kTile + tid) * 2) = f2{m, d};
+    const bool far = __any(!(fabsf(d) < kMostTotal));
+    if (tid == 0) s.exps[(int64_t)tile * s.heads + head] = far ? kOdd : e;
   }
   const int64_t at = ((int64_t)tile * s.heads + head) * S::kBytes;
   const float by = __builtin_amdgcn_ldexpf(s.by, e);
@@ -575,18 +580,22 @@ struct BackwardArgs {
   float most_score, most_value;  // see Source
 };
 
-__device__ __forceinline__ int wave_min(int v) {
+// dS comes as dS'' = p (raw 2^-ev - D 2^eg) = dS 2^eg: with V's factor 2^ev and the gradient's 2^eg, raw = dP
+// 2^(ev + eg) is below 2^37 and ev in -65..126; D 2^eg, which may come from other tiles of V than the one at
+// hand, is below 2^110 (`kMostTotal`).
+
+// P and dS are split times a power of two that puts each column's largest of the 32 rows at hand into [2^14,
+// 2^15): the split's smallest step is then 2^-38 of that, however little of a row's probability the rows have
+// or however large another tile's values are. The scaled split costs what the plain one does, so this is eight
+// max3 and a swap for 16 elements.
+__device__ __forceinline__ int top_exponent(const f16 &x) {
+  float r = 0.f;
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v = min(v, __shfl_xor(v, d));
-  return v;
+  for (int i = 0; i < 16; i += 2) r = fmaxf(fmaxf(r, fabsf(x[i])), fabsf(x[i + 1]));
+  r = half_pair(r, [](float a, float b) { return fmaxf(a, b); });
+  return max(__builtin_amdgcn_frexp_expf(r), -100);
 }
 
-// Scales of dS.  With V's factors 2^ev and the gradient's 2^eg, dP comes as raw = dP 2^(ev + eg),
-// below 2^31; a row's total D may come from other tiles of V than the one at hand, so both are
-// brought to the smallest ev of the sequence, and by 2^-32 below 1:
-//   dS'' = p (raw 2^(least - ev - 17) - D 2^(eg + least - 17)) = dS 2^(eg + least - 17),
-// at most 2^15 and split like any operand.
-//
 // A probability times the row's sum, from a score and the row's largest. It is at most 1 as the forward has
 // it; where the row kernels had the row, whose sums run in another order, a score may be above.
 __device__ __forceinline__ float score(float s, float f, float m) {
@@ -643,7 +652,6 @@ template <int DP, int Z>
 __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t, int h, char *lds) {
   using S = Shape<DP>;
   constexpr int R = 4 / Z, kPart = Z * S::kHalf, kStage = 2 * kPart;
-  __shared__ int least4[4];
   __shared__ float tops[4];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rw = w % R, z = w / R;
@@ -653,12 +661,8 @@ __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t,
   const int last = (end - 1) / kTile;
   const bool live = q0 < t.len, mine_in = q0 + c < t.len;
   bool odd = false;
-  int least = kOdd;
-  for (int i = tid; i <= last; i += 256) {
-    const int ev = a.ev[kv0 + (int64_t)i * a.kv_heads];
-    least = min(least, ev);
-    odd |= a.ek[kv0 + (int64_t)i * a.kv_heads] == kOdd || ev == kOdd;
-  }
+  for (int i = tid; i <= last; i += 256)
+    odd |= a.ek[kv0 + (int64_t)i * a.kv_heads] == kOdd || a.ev[kv0 + (int64_t)i * a.kv_heads] == kOdd;
   Terms q[S::NS], go[S::NS];
   float m = INFINITY, D = 0.f;  // a row past the sequence: p = 0
   int eg;
@@ -683,17 +687,14 @@ __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t,
       D += part;
     }
     D = half_pair(D, [](float y, float z) { return y + z; }) * inv;
-    odd |= !__builtin_isfinite(D);
     eg = exponent_for(x.top(a.most_value, odd));
     x.split_into(go, __builtin_amdgcn_ldexpf(1.f, eg));
+    D = __builtin_amdgcn_ldexpf(D, eg);
+    odd |= !(fabsf(D) < kMostTotal);
   }
-  least = wave_min(least);
-  if (lane == 0) least4[w] = least;
   if (__syncthreads_or(odd)) return false;
-  least = min(min(least4[0], least4[1]), min(least4[2], least4[3]));
   const int eq = exponent_for(fmaxf(tops[w], tops[w ^ 1]));
   qx.split_into(q, __builtin_amdgcn_ldexpf(a.mant, eq));
-  D = __builtin_amdgcn_ldexpf(D, eg + least - 17);
   const int ro = place(hi, c), co = columns_place(lane);
 
   f16 x[S::NB] = {};
@@ -716,7 +717,7 @@ __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t,
     f16 s, r;
     two_products<DP, false>(s, r, kf, vf, q, go, ro);
     f16 p, ds;
-    const float f = __builtin_amdgcn_ldexpf(1.f, a.exp - eq - ek), graw = __builtin_amdgcn_ldexpf(1.f, least - ev - 17);
+    const float f = __builtin_amdgcn_ldexpf(1.f, a.exp - eq - ek), graw = __builtin_amdgcn_ldexpf(1.f, -ev);
 #pragma unroll
     for (int e = 0; e < 16; ++e) p[e] = score(s[e], f, m), ds[e] = dscore(p[e], r[e], graw, D);
     if (32 * kb + 31 > q0) {
@@ -727,8 +728,10 @@ __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t,
     float y[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) y[e] = ds[e];
-    const Terms b[2] = {split8(y), split8(y + 8)};
-    const float back = __builtin_amdgcn_ldexpf(a.scale, 17 - eg - least - ek);
+    const int top = top_exponent(ds);
+    const float up = __builtin_amdgcn_ldexpf(1.f, 15 - top);
+    const Terms b[2] = {split8(y, up), split8(y + 8, up)};
+    const float back = __builtin_amdgcn_ldexpf(a.scale, top - 15 - eg - ek);
     Terms k0 = columns_of(kf, 0, 0, co), k1 = columns_of(kf, 0, 1, co);
 #pragma unroll
     for (int nb = 0; nb < S::NB; ++nb) {
@@ -757,7 +760,6 @@ template <int DP, int Z>
 __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t, int h0, char *lds) {
   using S = Shape<DP>;
   constexpr int R = 4 / Z, kPart = Z * S::kHalf, kStage = 2 * kPart + 256 * Z;
-  __shared__ int least4[4];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rw = w % R, z = w / R;
   const int c = lane & 31, hi = lane >> 5, g = h0 / (a.heads / a.kv_heads);
@@ -766,17 +768,11 @@ __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t
   const int first = t.t0 / kTile, all = (t.len - 1) / kTile;
   const bool live = k0 < t.len, mine_in = k0 + c < t.len;
   bool odd = false;
-  int least = kOdd;
-  for (int i = tid; i <= all; i += 256) {
-    const int ev = a.ev[kv0 + (int64_t)i * a.kv_heads];
-    least = min(least, ev);
-    odd |= ev == kOdd;
-    if (i >= first)
-      for (int h = h0; h < h0 + a.each; ++h) {
-        const int64_t at = (int64_t)(t.tile0 + i) * a.heads + h;
-        odd |= a.eq[at] == kOdd || a.eg[at] == kOdd;
-      }
-  }
+  for (int i = first + tid; i <= all; i += 256)
+    for (int h = h0; h < h0 + a.each; ++h) {
+      const int64_t at = (int64_t)(t.tile0 + i) * a.heads + h;
+      odd |= a.eq[at] == kOdd || a.eg[at] == kOdd;
+    }
   Terms k[S::NS], v[S::NS];
   // the keys' terms as they are packed
   const int ek = live ? scalar(a.ek + kv0 + (int64_t)(k0 / kTile) * a.kv_heads) : 0;
@@ -790,12 +786,8 @@ __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t
     ev = exponent_for(x.top(a.most_value, odd));
     x.split_into(v, __builtin_amdgcn_ldexpf(1.f, ev));
   }
-  least = wave_min(least);
-  if (lane == 0) least4[w] = least;
   if (__syncthreads_or(odd)) return false;
-  least = min(min(least4[0], least4[1]), min(least4[2], least4[3]));
-  // (a row that is smaller than its tile's largest has the larger factor; one of zeros may have less)
-  const float graw = __builtin_amdgcn_ldexpf(1.f, least - ev - 17), gd = __builtin_amdgcn_ldexpf(1.f, least - 17);
+  const float graw = __builtin_amdgcn_ldexpf(1.f, -ev);
   const int ro = place(hi, c), co = columns_place(lane);
 
   f16 xk[S::NB] = {}, xv[S::NB] = {};
@@ -828,7 +820,7 @@ __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t
 #pragma unroll
     for (int e = 0; e < 16; e += 2) {
       const f4 y = *reinterpret_cast<const f4 *>(rs + 2 * out_row(e, hi));
-      m[e] = y[0], d[e] = y[1] * gd, m[e + 1] = y[2], d[e + 1] = y[3] * gd;
+      m[e] = y[0], d[e] = y[1], m[e + 1] = y[2], d[e + 1] = y[3];
     }
     f16 p, ds;
     const float f = __builtin_amdgcn_ldexpf(1.f, a.exp - eq - ek);
@@ -842,8 +834,11 @@ __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t
     float y[16], z[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) y[e] = p[e], z[e] = ds[e];
-    const Terms pb[2] = {split8(y, 0x1p15f), split8(y + 8, 0x1p15f)}, sb[2] = {split8(z), split8(z + 8)};
-    const float bv = __builtin_amdgcn_ldexpf(1.f, -15 - eg), bk = __builtin_amdgcn_ldexpf(a.scale_q, 17 - eg - least - eq);
+    const int ptop = top_exponent(p), stop = top_exponent(ds);
+    const float pup = __builtin_amdgcn_ldexpf(1.f, 15 - ptop), sup = __builtin_amdgcn_ldexpf(1.f, 15 - stop);
+    const Terms pb[2] = {split8(y, pup), split8(y + 8, pup)}, sb[2] = {split8(z, sup), split8(z + 8, sup)};
+    const float bv = __builtin_amdgcn_ldexpf(1.f, ptop - 15 - eg);
+    const float bk = __builtin_amdgcn_ldexpf(a.scale_q, stop - 15 - eg - eq);
     Terms ga = columns_of(gf, 0, 0, co), qa = columns_of(qf, 0, 0, co);
 #pragma unroll
     for (int nb = 0; nb < S::NB; ++nb) {

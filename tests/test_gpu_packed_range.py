@@ -7,9 +7,9 @@ what the scores of the keys that it attends to are off by: a key of probability 
 and a row whose largest score stands out by more than 200 and both scores' errors is that key's alone,
 p = 1, whatever the scores' rounding.
 
-The kernels hold an operand to 2^-23 of it, which the counts above cover, or to 2^-36 of the largest magnitude
-of its 64 tokens, as the header says: a tile is scaled so that this one lies in [2^11, 2^12), where half a
-step of the second fp16 term, at least 2^-25, is at most 2^-36 of it. What that leaves of a value alone (a
+The kernels hold an operand to 2^-23 of it, which the counts above cover, or to 2^-39 of the largest magnitude
+of its 64 tokens, as the header says: a tile is scaled so that this one lies in [2^14, 2^15), where half a
+step of the second fp16 term, at least 2^-25, is at most 2^-39 of it. What that leaves of a value alone (a
 probability of 1 and a value of 1e-5 beside ones of 4) is part of the bound."""
 import math
 
@@ -60,7 +60,7 @@ def _ref(call, settled=False):
             alone[rows, h] = one
             f[one] = 0
             out = p @ V
-            out_err = (p * f) @ abs(V) + U2 * (n + 8) * (p @ abs(V)) + 2.0 ** -36 * (p @ _held(V))
+            out_err = (p * f) @ abs(V) + U2 * (n + 8) * (p @ abs(V)) + 2.0 ** -39 * (p @ _held(V))
             r = O @ V.T
             D = (O * out).sum(1, keepdims=True)
             D_err = (abs(O) * out_err).sum(1, keepdims=True) + U2 * (dh + 8) * (abs(O) * abs(out)).sum(1, keepdims=True)
@@ -69,7 +69,7 @@ def _ref(call, settled=False):
             for name, s_, x, err in (("out", c, out, out_err),
                                      ("dq", c, a * (ds @ K), a * (ds_err + U2 * (n + 8) * abs(ds)) @ abs(K)),
                                      ("dk", ck, a * (ds.T @ Q), a * (ds_err + U2 * (n * G + 8) * abs(ds)).T @ abs(Q)),
-                                     ("dv", ck, p.T @ O, (p * (f + U2 * (n * G + 8))).T @ abs(O) + 2.0 ** -36 * (p.T @ _held(O)))):
+                                     ("dv", ck, p.T @ O, (p * (f + U2 * (n * G + 8))).T @ abs(O) + 2.0 ** -39 * (p.T @ _held(O)))):
                 res[name][0][rows, s_] += x
                 res[name][1][rows, s_] += err
     return (res, alone) if settled else res
@@ -135,3 +135,55 @@ def test_large_scores_of_many_sequences_backward(hip_ctx):
     bound = 2 * U2 * (dh + 8) * (np.abs(g) * np.abs(v)).reshape(n, H, dh).sum(2) / math.sqrt(dh)
     for name, other in (("dq", x[:, H * dh:2 * H * dh]), ("dk", x[:, :H * dh])):
         assert (np.abs(got[name]).reshape(n, H, dh) <= bound[:, :, None] * np.abs(other).reshape(n, H, dh)).all(), name
+
+
+@pytest.mark.parametrize("lengths", [[65], [200], [140] * 30])
+@pytest.mark.parametrize("size", [1e-3, 1e-6, 1e-12])
+def test_values_of_zero_beside_small_ones(hip_ctx, size, lengths):
+    """A sequence of small values whose last token's is zero, alone in its tile of 64."""
+    call = _Call(hip_ctx, lengths, 16, 4, 64, np.random.default_rng(21))
+    v = call.parts(call.x)[2]
+    v *= np.float32(size)
+    ends = np.cumsum(lengths)
+    v[ends - 1] = 0
+    got, ref = _run(call), _ref(call)
+    for name in NAMES:
+        _check(got[name], ref[name], name)
+
+
+@pytest.mark.parametrize("lengths", [[256], [900]])
+@pytest.mark.parametrize("size", [1e4, 1e6])
+def test_a_value_far_above_the_others(hip_ctx, size, lengths):
+    """A value that the rows behind it have no probability for: their gradients keep their accuracy."""
+    call = _Call(hip_ctx, lengths, 4, 2, 64, np.random.default_rng(9))
+    q, k, v = call.parts(call.x)
+    q[:] = abs(q)
+    k[100], v[100] = -200, size
+    call.g[100] = 0  # its own row attends to keys before it with a value among them that only it has
+    got, ref = _run(call), _ref(call)
+    for name in NAMES:
+        _check(got[name], ref[name], name)
+
+
+@pytest.mark.parametrize("gap", [15])
+@pytest.mark.parametrize("lengths", [[200], [140] * 30])
+def test_keys_with_hardly_any_probability(hip_ctx, gap, lengths):
+    """A key with 2^-gap of the others' probability in every row, its value 2^gap times theirs: half of the
+    output; and what it gets of the gradients, 2^-gap of theirs, to the same relative accuracy, less what a
+    score's own roundings (its scale's, its own, the difference's: half a step of gap each) leave of it."""
+    call = _Call(hip_ctx, lengths, 16, 4, 64, np.random.default_rng(gap))
+    q, k, v = call.parts(call.x)
+    q[:], k[:] = 0, 0
+    # one product a score: q k / 8, in base 2
+    q[:, ::64] = 8
+    k[:, ::64] = np.random.default_rng(3).uniform(-1, 1, (call.T, 4))
+    starts = np.cumsum(lengths) - lengths
+    k[starts + 70, ::64] = -np.float32(gap * math.log(2))
+    v[starts + 70] *= np.float32(2.0 ** gap)
+    got, ref = _run(call), _ref(call)
+    for name in NAMES:
+        _check(got[name], ref[name], name)
+        if name in ("dk", "dv"):
+            rows = starts + 70
+            _check(got[name][rows], tuple(r[rows] for r in ref[name]), f"{name} of those keys",
+                   2e-6 + 3 * gap * math.log(2) * U2 / 2)
