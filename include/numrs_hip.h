@@ -366,11 +366,14 @@ int64_t numrs_hip_seqs_total(const numrs_hip_seqs *seqs); /* the sum of the leng
  * multiple of 8 in 8..128.  stats [total, heads, 2] receives each row's
  * softmax reference and sum for the backward; NULL where none follows.  Rows
  * past the batch's total are not touched, and a row's result depends on no
- * other token's values than those it attends to, finite or not.  Operands are
- * held to 2^-23 of a value, and to 2^-39 of the largest magnitude among its
- * tile of 64 tokens of its head; 64 or 128 rows that see a value that is not
- * finite, a query or key from 2^50 or a value or gradient from 2^80 on take
- * plain fp32 arithmetic instead, some 150 times slower.
+ * other token's values than those it attends to, finite or not, beyond the last
+ * bits.  Operands are held to 2^-23 of a value, and to 2^-33 of the largest
+ * magnitude of its token and head; a row's probabilities, as the products with
+ * values and gradients take them, to 2^-23 of each and to 2^-38 of the largest
+ * of 32.  64 or 128 rows that see a value that is not finite, a query or key
+ * from 2^50 or a value or gradient from 2^80 on, or 64 neighbouring tokens
+ * whose largest magnitudes differ by more than 2^140, take plain fp32 arithmetic
+ * instead, some 150 times slower.
  * Backward, with r = dout . v and D = dout . out:
  *   dv = sum p dout,  ds = p (r - D) / sqrt(dh),  dq = sum ds k,  dk = sum ds q,
  * the last two over all query heads of the kv head; dq, dk or dv may be NULL.

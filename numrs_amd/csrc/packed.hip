@@ -289,17 +289,18 @@ int with_dp(int dh, F &&f) {
 struct Packed {
   TempBlock block;
   char *rows = nullptr;
-  int *exps = nullptr;
+  int *exps = nullptr, *each = nullptr;
   explicit Packed(numrs_hip_ctx *ctx) : block(ctx) {}
   int alloc(const Seqs &s, int heads, int dh) {
     const size_t n = (size_t)s.tiles * heads, image = n * kTile * padded(dh) * 4;
-    if (int rc = block.alloc(image + n * sizeof(int))) return rc;
+    if (int rc = block.alloc(image + n * (kTile + 1) * sizeof(int))) return rc;
     rows = static_cast<char *>(block.p);
-    exps = reinterpret_cast<int *>(rows + image);
+    each = reinterpret_cast<int *>(rows + image);
+    exps = each + n * kTile;
     return NUMRS_HIP_OK;
   }
   tiles::Source source(const float *x, int64_t ld, int heads, float most, float by = 1.f) const {
-    return {x, ld, rows, exps, most, by, heads, nullptr, nullptr, nullptr};
+    return {x, ld, rows, exps, each, most, by, heads, nullptr, nullptr, nullptr};
   }
 };
 
@@ -326,7 +327,8 @@ int packed_forward(numrs_hip_ctx *ctx, const Seqs &s, const float *q, int64_t ld
   const float alpha = kLog2e / std::sqrt((float)dh);
   const FwdArgs a{s.by_work, q, k, v, out, stats, ld_q, ld_kv, ld_out, H, Hk, dh, alpha};
   const bool few = few_blocks(ctx, s, H);
-  tiles::ForwardArgs f{q, pk.rows, pv.rows, pk.exps, pv.exps, out, stats, ld_q, ld_out, H, Hk, dh, 0.f, 0, kMostScore};
+  tiles::ForwardArgs f{q, pk.rows, pv.rows, pk.exps, pv.exps, pk.each, pv.each, out, stats,
+                       ld_q, ld_out, H, Hk, dh, 0.f, 0, kMostScore};
   f.mant = std::frexp(alpha, &f.exp);
   return with_dp(dh, [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
@@ -386,7 +388,7 @@ int packed_backward(numrs_hip_ctx *ctx, const Seqs &s, const float *q, int64_t l
   const bool few = few_blocks(ctx, s, H);
   BwdArgs b{few ? s.few_by_work : s.by_work, q, k, v, out, dout, stats, ld_q, ld_kv, ld_out};
   tiles::BackwardArgs a{q, k, v, out, dout, stats, ld_q, ld_kv, ld_out, pq.rows, pk.rows, pv.rows, pg.rows,
-                        pq.exps, pk.exps, pv.exps, pg.exps, rowstat.f(), dq, dk, dv, ld_q, ld_kv, ld_kv, s.total,
+                        pq.exps, pk.exps, pv.exps, pg.exps, pq.each, pk.each, pv.each, pg.each, rowstat.f(), dq, dk, dv, ld_q, ld_kv, ld_kv, s.total,
                         H, Hk, dh, accumulate, accumulate, each, alpha, scale, mant, exp, scale_q, kMostScore, kMostValue};
   return with_dp(dh, [&](auto dp) {
     constexpr int DP = decltype(dp)::value;

@@ -3,11 +3,16 @@
 // An fp32 operand x, times a power of two that puts its 64-token tile's largest magnitude into
 // [2^14, 2^15), is the sum h + m of two fp16 values, each rounded to nearest: h holds 11 bits, x -
 // h is exact and m holds its next 11, so h + m is x within 2^-23 |x| for |x| down to 2^-17 of the
-// largest and within 2^-39 of the largest below.  Of the four products of two such operands the
-// matrix cores form three, m h + h m + h h (the fourth is below 2^-22 of the product and of either
-// sign), each with fp32 accumulation: half of what three bf16 terms and six products take.
-// v_mfma_f32_32x32x16_f16 sums of at most 64 tokens (or one head) start from zero and are added to
-// fp32 totals: the matrix cores' own sum is cut off, not rounded.
+// largest and within 2^-39 of the largest below. Where a tile's tokens differ by more than 2^6, each
+// has an exponent of its own (kMixed), so that none costs another more than 2^-33 of its own largest:
+// neither one that its row does not see nor one that has no probability. Products take such a tile's
+// rows to one exponent, before and after the softmax, in a form of each walk that only workgroups
+// with such a tile take (its tests in the common one cost training on 2 x 4096 tokens 5 %).
+//
+// Of the four products of two such operands the matrix cores form three, m h + h m + h h (the fourth
+// is below 2^-22 of the product and of either sign), each with fp32 accumulation: half of what three
+// bf16 terms and six products take. v_mfma_f32_32x32x16_f16 sums of at most 64 tokens (or one head)
+// start from zero and are added to fp32 totals: the matrix cores' own sum is cut off, not rounded.
 //
 // `pack` splits what the kernels walk over once a call, in the order in which the products read it: a
 // fragment is the 32 tokens x 16 columns of a term, lane (g, c)'s 16 bytes being token c's columns 8 g
@@ -32,6 +37,7 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef float f16 __attribute__((ext_vector_type(16)));
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
+typedef int i4 __attribute__((ext_vector_type(4)));
 
 // A value that an earlier kernel left at an address that is the same in every lane: a scalar load, which
 // waits for no copy to LDS in flight.
@@ -42,6 +48,13 @@ __device__ __forceinline__ int scalar(const int *p) {
 // A tile's exponent where its values do not split: one that is not finite, or so large that a
 // product might pass fp32's range.  Workgroups that meet one take the row kernels' arithmetic.
 constexpr int kOdd = 1 << 20;
+// Added to the exponent of a tile whose tokens have exponents of their own: the largest token's. Tokens of zeros
+// have it too. Past a difference of 2^140 a tile is odd: what such exponents make of scores and of probabilities
+// would leave fp32's range.
+constexpr int kMixed = 1 << 16, kSpread = 6, kMostSpread = 140;
+__device__ __forceinline__ bool is_mixed(int word) { return word > kMixed / 2; }
+__device__ __forceinline__ int base_of(int word) { return is_mixed(word) ? word - kMixed : word; }
+
 // And out . dout, at its gradient's exponent: what values below 2^80 give is below 2^103.
 constexpr float kMostTotal = 0x1p110f;
 // A softmax reference before any score: below every score of a tile that is not odd.
@@ -107,8 +120,27 @@ __device__ __forceinline__ int exponent_for(float big) {
   return big > 0.f ? min(15 - __builtin_amdgcn_frexp_expf(big), 126) : 0;
 }
 
+// A tile's word from its tokens' largest and smallest magnitudes that are not 0 (infinity if all are), and a
+// token's exponent from its own.
+__device__ __forceinline__ int tile_word(float big, float small) {
+  const int e = exponent_for(big), spread = exponent_for(fminf(big, small)) - e;
+  return spread <= kSpread ? e : spread <= kMostSpread ? e + kMixed : kOdd;
+}
+__device__ __forceinline__ float not_zero(float top) { return top > 0.f ? top : INFINITY; }
+__device__ __forceinline__ float lower(float a, float b) { return fminf(a, b); }
+
 // Row of a 32x32 result that register i of lane group g holds.
 __device__ __forceinline__ constexpr int out_row(int i, int g) { return 8 * (i >> 2) + 4 * g + (i & 3); }
+
+// Rows of a result, those of 32 tokens whose own exponents are at `each`, brought to the exponent `base`.
+__device__ __forceinline__ void level(f16 &x, const int *each, int base, int hi) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const i4 e = *reinterpret_cast<const i4 *>(each + out_row(4 * i, hi));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[4 * i + j] = __builtin_amdgcn_ldexpf(x[4 * i + j], base - e[j]);
+  }
+}
 
 // A head size rounded up to DP: 64-token tiles of fragments, the two terms of each side by side.
 template <int DP>
@@ -184,7 +216,8 @@ struct Source {
   const float *x;
   int64_t ld;
   char *rows;   // fragments [tiles, heads]
-  int *exps;    // [tiles, heads]
+  int *exps;    // [tiles, heads]: an exponent, plus kMixed where each token has its own, or kOdd
+  int *each;    // [tiles, heads, 64]: those
   float most;   // larger magnitudes make a tile odd
   float by;     // a factor in [0.5, 1] that the terms have besides the exponent's
   int heads;
@@ -208,7 +241,7 @@ template <int DP>
 __global__ void __launch_bounds__(256) pack(PackArgs a) {
   using S = Shape<DP>;
   constexpr int NI = DP / 32, NC = DP / 8;  // a thread's chunks of 8 columns; chunks of a row
-  __shared__ float top[4];
+  __shared__ float tops[kTile][NC + 1];  // of 8 columns
   __shared__ float part[kTile][NC + 1];  // out . dout of 8 columns
   const int tile = blockIdx.x / a.slots, tid = threadIdx.x;
   int head = blockIdx.x % a.slots, which = 0;
@@ -217,7 +250,7 @@ __global__ void __launch_bounds__(256) pack(PackArgs a) {
   const SeqTile t = a.tiles[tile];
   const int rows = min(kTile, t.len - t.t0);
   const float *x = s.x + (int64_t)(t.row0 + t.t0) * s.ld + (int64_t)head * a.dh;
-  float v[NI][8], big = 0.f;
+  float v[NI][8];
   bool odd = false;
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
@@ -242,6 +275,7 @@ __global__ void __launch_bounds__(256) pack(PackArgs a) {
       odd |= !__builtin_isfinite(dot);
     }
     if (s.stats != nullptr) part[row][c] = dot;
+    float big = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       v[i][j] = (j < 4 ? lo[j] : hi[j - 4]) * inv;
@@ -249,17 +283,22 @@ __global__ void __launch_bounds__(256) pack(PackArgs a) {
       odd |= !(m < s.most);
       big = fmaxf(big, m);
     }
+    tops[row][c] = big;
   }
-  big = wave_max(big);
-  if ((tid & 63) == 0) top[tid >> 6] = big;
-  const int any = __syncthreads_or(odd);
-  big = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-  if (any) {
+  const int any = __syncthreads_or(odd), lane = tid & 63;
+  // every wave has all rows, one a lane
+  float top = 0.f;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) top = fmaxf(top, tops[lane][c]);
+  const int word = any ? kOdd : tile_word(wave_max(top), wave_butterfly(not_zero(top), lower));
+  if (word == kOdd) {
     if (tid == 0) s.exps[(int64_t)tile * s.heads + head] = kOdd;
     return;
   }
-  const int e = exponent_for(big);
+  const bool mixed = is_mixed(word);
+  const int e = base_of(word), mine = mixed && top > 0.f ? exponent_for(top) : e;
   if (tid < kTile) {
+    if (mixed) s.each[((int64_t)tile * s.heads + head) * kTile + tid] = mine;
     float m = INFINITY, d = 0.f;
     if (s.stats != nullptr) {
       if (tid < rows) {
@@ -270,13 +309,14 @@ __global__ void __launch_bounds__(256) pack(PackArgs a) {
       *reinterpret_cast<f2 *>(s.rowstat + (((int64_t)tile * s.heads + head) * kTile + tid) * 2) = f2{m, d};
     }
     const bool far = __any(!(fabsf(d) < kMostTotal));
-    if (tid == 0) s.exps[(int64_t)tile * s.heads + head] = far ? kOdd : e;
+    if (tid == 0) s.exps[(int64_t)tile * s.heads + head] = far ? kOdd : word;
   }
   const int64_t at = ((int64_t)tile * s.heads + head) * S::kBytes;
-  const float by = __builtin_amdgcn_ldexpf(s.by, e);
+  float by = __builtin_amdgcn_ldexpf(s.by, e);
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
     const int row = (i * 256 + tid) / NC, c = (i * 256 + tid) % NC;
+    if (mixed) by = __builtin_amdgcn_ldexpf(s.by, __shfl(mine, row));
     const Terms p = split8(v[i], by);
     char *o = s.rows + at + (row >> 5) * S::kHalf + (c >> 1) * 2048 + place(c & 1, row & 31);
     *reinterpret_cast<h8 *>(o) = p.h;
@@ -313,6 +353,21 @@ __device__ __forceinline__ void fetched() {
   __syncthreads();
 }
 
+// What the waves' lanes found, by one barrier: bit 0 a tile that is odd, bit 1 one that is mixed.
+__device__ __forceinline__ int found(int (&flags)[4], int w, bool odd, bool mixed) {
+  flags[w] = (__any(odd) ? 1 : 0) | (__any(mixed) ? 2 : 0);
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(flags[0] | flags[1] | flags[2] | flags[3]);
+}
+// f(std::bool_constant<mixed>).
+template <class F>
+__device__ __forceinline__ void by_tiles(bool mixed, F &&f) {
+  if (mixed)
+    f(std::true_type{});
+  else
+    f(std::false_type{});
+}
+
 template <class Op>
 __device__ __forceinline__ float over16(const f16 &x, Op op) {
   float r[8];
@@ -323,10 +378,41 @@ __device__ __forceinline__ float over16(const f16 &x, Op op) {
   return op(op(r[0], r[1]), op(r[2], r[3]));
 }
 
+// The backward's P and dS are split times a power of two that puts each column's largest of the 32 rows at
+// hand into [2^14, 2^15): the split's smallest step is then 2^-38 of that, however little of a row's
+// probability the rows have or however large another tile's values are. The scaled split costs what the plain one does, so this is eight
+// max3 and a swap for 16 elements.
+__device__ __forceinline__ float top_of(const f16 &x, float r) {
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) r = fmaxf(fmaxf(r, fabsf(x[i])), fabsf(x[i + 1]));
+  return r;
+}
+__device__ __forceinline__ int top_exponent(float lane_top) {
+  return max(__builtin_amdgcn_frexp_expf(half_pair(lane_top, [](float a, float b) { return fmaxf(a, b); })), -100);
+}
+
+// Weights of such tokens, brought to what the tokens count at the exponent `base`, and returns the power of two
+// besides: each column's largest comes to 2^100 at most, so that what tokens 2^140 below another weigh stays
+// above fp32's smallest.
+constexpr int kWeight = 100;
+__device__ __forceinline__ int weigh(f16 &x, const int *each, int base, int hi) {
+  const int up = kWeight - top_exponent(top_of(x, 0.f));
+  level(x, each, base + up, hi);
+  return up;
+}
+
+// The exponent of a row of wave w, of largest magnitude `top`, as `pack` has it: waves w and w ^ 1 have a tile.
+// (Where that is odd for its tokens' differences alone, the row's own or the largest's.)
+__device__ __forceinline__ int own_exponent(const float (&tops)[4], const float (&lows)[4], int w, float top) {
+  const float big = fmaxf(tops[w], tops[w ^ 1]);
+  const int word = tile_word(big, fminf(lows[w], lows[w ^ 1]));
+  return is_mixed(word) && top > 0.f ? exponent_for(top) : exponent_for(big);
+}
+
 struct ForwardArgs {
   const float *q;
   const char *k, *v;  // fragments
-  const int *ek, *ev;
+  const int *ek, *ev, *each_k, *each_v;
   float *out, *stats;
   int64_t ld_q, ld_out;
   int heads, kv_heads, dh;
@@ -402,7 +488,8 @@ __device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile
   using S = Shape<DP>;
   using W = Walk<DP, Z>;
   constexpr int KT = W::KT, KB = W::KB, kStage = KT * DP * 4;
-  __shared__ float joint[Z == 2 ? 3 : 1][64], tops[4];
+  __shared__ float joint[Z == 2 ? 3 : 1][64], tops[4], lows[4];
+  __shared__ int flags[4];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rw = w % W::R, z = w / W::R;
   const int c = lane & 31, hi = lane >> 5, g = h / (a.heads / a.kv_heads);
@@ -413,12 +500,16 @@ __device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile
   bool odd = false;
   RowValues<DP> qx;
   qx.load(a.q + (int64_t)(t.row0 + q0 + c) * a.ld_q + (int64_t)h * a.dh, q0 + c < t.len, a.dh, hi);
-  for (int i = tid; i <= last; i += 256)
-    odd |= a.ek[kv0 + (int64_t)i * a.kv_heads] == kOdd || a.ev[kv0 + (int64_t)i * a.kv_heads] == kOdd;
+  bool mixed = false;
+  for (int i = tid; i <= last; i += 256) {
+    const int wk = a.ek[kv0 + (int64_t)i * a.kv_heads], wv = a.ev[kv0 + (int64_t)i * a.kv_heads];
+    odd |= wk == kOdd || wv == kOdd, mixed |= is_mixed(wk) || is_mixed(wv);
+  }
   const float row_top = qx.top(a.most, odd);
-  tops[w] = wave_max(row_top);
-  if (__syncthreads_or(odd)) return false;
-  const int eq = exponent_for(fmaxf(tops[w], tops[w ^ 1]));
+  tops[w] = wave_max(row_top), lows[w] = wave_butterfly(not_zero(row_top), lower);
+  const int kinds = found(flags, w, odd, mixed);
+  if (kinds & 1) return false;
+  const int eq = own_exponent(tops, lows, w, row_top);
   qx.split_into(q, __builtin_amdgcn_ldexpf(a.mant, eq));
   const bool live = q0 < t.len;
   const int ro = place(hi, c), co = columns_place(lane);
@@ -435,88 +526,115 @@ __device__ __forceinline__ bool forward_tile(const ForwardArgs &a, const SeqTile
     fetch<kStage>(a.v + at, to + kStage, w, lane);
   };
   issue(0);
-  for (int i = 0; i < n; ++i) {
-    fetched();
-    if (i + 1 < n) issue(i + 1);
-    if (i >= mine) continue;
-    const char *kf = lds + (i & 1) * 2 * kStage + z * S::kHalf, *vf = kf + kStage;
-    const int key0 = i * KT + 32 * z;
-    if (key0 > q0 + 31) continue;  // all after the wave's rows
-    const int ek = scalar(a.ek + tile_of(i)), ev = scalar(a.ev + tile_of(i));
-    f16 s[KB] = {};
-    Terms x[KB];
+  by_tiles(kinds & 2, [&](auto kind) {
+    constexpr bool MIXED = decltype(kind)::value;
+    for (int i = 0; i < n; ++i) {
+      fetched();
+      if (i + 1 < n) issue(i + 1);
+      if (i >= mine) continue;
+      const char *kf = lds + (i & 1) * 2 * kStage + z * S::kHalf, *vf = kf + kStage;
+      const int key0 = i * KT + 32 * z;
+      if (key0 > q0 + 31) continue;  // all after the wave's rows
+      const int64_t tile = tile_of(i);
+      const int wk = scalar(a.ek + tile), wv = scalar(a.ev + tile);
+      const int ek = MIXED ? base_of(wk) : wk, ev = MIXED ? base_of(wv) : wv;
+      const int64_t in_tile = tile * kTile + i * KT % kTile + 32 * z;
+      f16 s[KB] = {};
+      Terms x[KB];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) x[kb] = rows_of(kf + kb * S::kHalf, 0, ro);
+      for (int kb = 0; kb < KB; ++kb) x[kb] = rows_of(kf + kb * S::kHalf, 0, ro);
 #pragma unroll
-    for (int st = 0; st < S::NS; ++st) {
-      Terms y[KB];
-      if (st + 1 < S::NS) {
+      for (int st = 0; st < S::NS; ++st) {
+        Terms y[KB];
+        if (st + 1 < S::NS) {
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) y[kb] = rows_of(kf + kb * S::kHalf, st + 1, ro);
+          for (int kb = 0; kb < KB; ++kb) y[kb] = rows_of(kf + kb * S::kHalf, st + 1, ro);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // the next step's operands are asked for before this one's products
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) mma(s[kb], x[kb], q[st]);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) x[kb] = y[kb];
       }
-      __builtin_amdgcn_sched_barrier(0);  // the next step's operands are asked for before this one's products
+      if (MIXED && is_mixed(wk)) {
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) mma(s[kb], x[kb], q[st]);
+        for (int kb = 0; kb < KB; ++kb) level(s[kb], a.each_k + in_tile + 32 * kb, ek, hi);
+      }
+      // an underflow of f must not make -inf * f NaN
+      const float f = fmaxf(__builtin_amdgcn_ldexpf(1.f, a.exp - eq - ek), 1.17549435e-38f);
+      if (key0 + 32 * KB > q0 + 1) {  // keys after a row of the wave
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) x[kb] = y[kb];
-    }
-    // an underflow of f must not make -inf * f NaN
-    const float f = fmaxf(__builtin_amdgcn_ldexpf(1.f, a.exp - eq - ek), 1.17549435e-38f);
-    if (key0 + 32 * KB > q0 + 1) {  // keys after a row of the wave
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
+          for (int e = 0; e < 16; ++e)
+            if (key0 + 32 * kb + out_row(e, hi) > q0 + c) s[kb][e] = -INFINITY;
+      }
+      float most = over16(s[0], [](float x, float y) { return fmaxf(x, y); });
+      if constexpr (KB == 2) most = fmaxf(most, over16(s[1], [](float x, float y) { return fmaxf(x, y); }));
+      most = half_pair(most, [](float x, float y) { return fmaxf(x, y); }) * f;
+      top = fmaxf(top, most);
+      if (__any(most > m + 8.f)) {
+        const float now = fmaxf(m, most);
+        const float r = __builtin_amdgcn_exp2f(m - now);
+        m = now;
+        l *= r;
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (key0 + 32 * kb + out_row(e, hi) > q0 + c) s[kb][e] = -INFINITY;
-    }
-    float most = over16(s[0], [](float x, float y) { return fmaxf(x, y); });
-    if constexpr (KB == 2) most = fmaxf(most, over16(s[1], [](float x, float y) { return fmaxf(x, y); }));
-    most = half_pair(most, [](float x, float y) { return fmaxf(x, y); }) * f;
-    top = fmaxf(top, most);
-    if (__any(most > m + 8.f)) {
-      const float now = fmaxf(m, most);
-      const float r = __builtin_amdgcn_exp2f(m - now);
-      m = now;
-      l *= r;
+        for (int b = 0; b < S::NB; ++b)
 #pragma unroll
-      for (int b = 0; b < S::NB; ++b)
+          for (int e = 0; e < 16; ++e) o[b][e] *= r;
+      }
+      Terms p[KB][2];
+      // from 2^24 on, where a float's steps pass 14, P is at most 1; every other score is then 2 below or more
+      const float ref = fabsf(most) < 0x1p24f ? most - 14.f : most;
+      // from the reference as rounded
+      const float back = __builtin_amdgcn_exp2f(ref - m + 14.f);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[b][e] *= r;
-    }
-    Terms p[KB][2];
-    // from 2^24 on, where a float's steps pass 14, P is at most 1; every other score is then 2 below or more
-    const float ref = fabsf(most) < 0x1p24f ? most - 14.f : most;
-    // from the reference as rounded
-    const float back = __builtin_amdgcn_exp2f(ref - m + 14.f);
+      for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
+        for (int e = 0; e < 16; ++e) s[kb][e] = __builtin_amdgcn_exp2f(fmaf(s[kb][e], f, -ref));
+        l = fmaf(over16(s[kb], [](float x, float y) { return x + y; }), back, l);
+      }
+      float fv = __builtin_amdgcn_ldexpf(back, -ev);
+      if (MIXED && is_mixed(wv)) {
+        float lane_top = 0.f;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[kb][e] = __builtin_amdgcn_exp2f(fmaf(s[kb][e], f, -ref));
-      l = fmaf(over16(s[kb], [](float x, float y) { return x + y; }), back, l);
-      float x[16];
+        for (int kb = 0; kb < KB; ++kb) {
+          level(s[kb], a.each_v + in_tile + 32 * kb, ev + kWeight - 15, hi);
+          lane_top = top_of(s[kb], lane_top);
+        }
+        const int big = top_exponent(lane_top);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = s[kb][e];
-      p[kb][0] = split8(x), p[kb][1] = split8(x + 8);
-    }
-    const float fv = __builtin_amdgcn_ldexpf(back, -ev);
-    constexpr int kSteps = 2 * KB;  // of 16 keys
-    Terms v = columns_of(vf, 0, 0, co);
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-    for (int b = 0; b < S::NB; ++b) {
-      f16 z = {};
-#pragma unroll
-      for (int st = 0; st < kSteps; ++st) {
-        const int nb = st + 1 < kSteps ? b : b + 1, ns = (st + 1) % kSteps;
-        Terms y;
-        if (nb < S::NB) y = columns_of(vf + (ns >> 1) * S::kHalf, nb, ns & 1, co);
-        __builtin_amdgcn_sched_barrier(0);
-        mma(z, v, p[st >> 1][st & 1]);
-        v = y;
+          for (int e = 0; e < 16; ++e) s[kb][e] = __builtin_amdgcn_ldexpf(s[kb][e], 15 - big);
+        fv = __builtin_amdgcn_ldexpf(back, big - kWeight - ev);
       }
 #pragma unroll
-      for (int e = 0; e < 16; ++e) o[b][e] = fmaf(z[e], fv, o[b][e]);
+      for (int kb = 0; kb < KB; ++kb) {
+        float x[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = s[kb][e];
+        p[kb][0] = split8(x), p[kb][1] = split8(x + 8);
+      }
+      constexpr int kSteps = 2 * KB;  // of 16 keys
+      Terms v = columns_of(vf, 0, 0, co);
+#pragma unroll
+      for (int b = 0; b < S::NB; ++b) {
+        f16 z = {};
+#pragma unroll
+        for (int st = 0; st < kSteps; ++st) {
+          const int nb = st + 1 < kSteps ? b : b + 1, ns = (st + 1) % kSteps;
+          Terms y;
+          if (nb < S::NB) y = columns_of(vf + (ns >> 1) * S::kHalf, nb, ns & 1, co);
+          __builtin_amdgcn_sched_barrier(0);
+          mma(z, v, p[st >> 1][st & 1]);
+          v = y;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[b][e] = fmaf(z[e], fv, o[b][e]);
+      }
     }
-  }
+  });
   const int row = q0 + c;
   l = half_pair(l, [](float x, float y) { return x + y; });
   if constexpr (Z == 2) {
@@ -567,7 +685,7 @@ struct BackwardArgs {
   const float *xq, *xk, *xv, *out, *dout, *stats;
   int64_t ld_xq, ld_xkv, ld_out;
   const char *q, *k, *v, *g;  // fragments; g: the output's gradient
-  const int *eq, *ek, *ev, *eg;
+  const int *eq, *ek, *ev, *eg, *each_q, *each_k, *each_v, *each_g;
   const float *rowstat;
   float *dq, *dk, *dv;
   int64_t ld_q, ld_k, ld_v, total;
@@ -583,18 +701,6 @@ struct BackwardArgs {
 // dS comes as dS'' = p (raw 2^-ev - D 2^eg) = dS 2^eg: with V's factor 2^ev and the gradient's 2^eg, raw = dP
 // 2^(ev + eg) is below 2^37 and ev in -65..126; D 2^eg, which may come from other tiles of V than the one at
 // hand, is below 2^110 (`kMostTotal`).
-
-// P and dS are split times a power of two that puts each column's largest of the 32 rows at hand into [2^14,
-// 2^15): the split's smallest step is then 2^-38 of that, however little of a row's probability the rows have
-// or however large another tile's values are. The scaled split costs what the plain one does, so this is eight
-// max3 and a swap for 16 elements.
-__device__ __forceinline__ int top_exponent(const f16 &x) {
-  float r = 0.f;
-#pragma unroll
-  for (int i = 0; i < 16; i += 2) r = fmaxf(fmaxf(r, fabsf(x[i])), fabsf(x[i + 1]));
-  r = half_pair(r, [](float a, float b) { return fmaxf(a, b); });
-  return max(__builtin_amdgcn_frexp_expf(r), -100);
-}
 
 // A probability times the row's sum, from a score and the row's largest. It is at most 1 as the forward has
 // it; where the row kernels had the row, whose sums run in another order, a score may be above.
@@ -652,7 +758,8 @@ template <int DP, int Z>
 __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t, int h, char *lds) {
   using S = Shape<DP>;
   constexpr int R = 4 / Z, kPart = Z * S::kHalf, kStage = 2 * kPart;
-  __shared__ float tops[4];
+  __shared__ float tops[4], lows[4];
+  __shared__ int flags[4];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rw = w % R, z = w / R;
   const int c = lane & 31, hi = lane >> 5, g = h / (a.heads / a.kv_heads);
@@ -661,15 +768,18 @@ __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t,
   const int last = (end - 1) / kTile;
   const bool live = q0 < t.len, mine_in = q0 + c < t.len;
   bool odd = false;
-  for (int i = tid; i <= last; i += 256)
-    odd |= a.ek[kv0 + (int64_t)i * a.kv_heads] == kOdd || a.ev[kv0 + (int64_t)i * a.kv_heads] == kOdd;
+  bool mixed = false;
+  for (int i = tid; i <= last; i += 256) {
+    const int wk = a.ek[kv0 + (int64_t)i * a.kv_heads], wv = a.ev[kv0 + (int64_t)i * a.kv_heads];
+    odd |= wk == kOdd || wv == kOdd, mixed |= is_mixed(wk) || is_mixed(wv);
+  }
   Terms q[S::NS], go[S::NS];
   float m = INFINITY, D = 0.f;  // a row past the sequence: p = 0
   int eg;
   RowValues<DP> qx;
   qx.load(a.xq + row * a.ld_xq + (int64_t)h * a.dh, mine_in, a.dh, hi);
   const float q_top = qx.top(a.most_score, odd);
-  tops[w] = wave_max(q_top);
+  tops[w] = wave_max(q_top), lows[w] = wave_butterfly(not_zero(q_top), lower);
   {
     RowValues<DP> x, o;
     x.load(a.dout + row * a.ld_out + (int64_t)h * a.dh, mine_in, a.dh, hi);
@@ -692,8 +802,9 @@ __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t,
     D = __builtin_amdgcn_ldexpf(D, eg);
     odd |= !(fabsf(D) < kMostTotal);
   }
-  if (__syncthreads_or(odd)) return false;
-  const int eq = exponent_for(fmaxf(tops[w], tops[w ^ 1]));
+  const int kinds = found(flags, w, odd, mixed);
+  if (kinds & 1) return false;
+  const int eq = own_exponent(tops, lows, w, q_top);
   qx.split_into(q, __builtin_amdgcn_ldexpf(a.mant, eq));
   const int ro = place(hi, c), co = columns_place(lane);
 
@@ -707,45 +818,54 @@ __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t,
     fetch<kPart>(a.v + at, to + kPart, w, lane);
   };
   issue(0);
-  for (int i = 0; i < n; ++i) {
-    fetched();
-    if (i + 1 < n) issue(i + 1);
-    const int kb = i * Z + z;  // the wave's 32 keys
-    if (kb >= mine) continue;
-    const char *kf = lds + (i & 1) * kStage + z * S::kHalf, *vf = kf + kPart;
-    const int ek = scalar(a.ek + tile_of(i)), ev = scalar(a.ev + tile_of(i));
-    f16 s, r;
-    two_products<DP, false>(s, r, kf, vf, q, go, ro);
-    f16 p, ds;
-    const float f = __builtin_amdgcn_ldexpf(1.f, a.exp - eq - ek), graw = __builtin_amdgcn_ldexpf(1.f, -ev);
+  by_tiles(kinds & 2, [&](auto kind) {
+    constexpr bool MIXED = decltype(kind)::value;
+    for (int i = 0; i < n; ++i) {
+      fetched();
+      if (i + 1 < n) issue(i + 1);
+      const int kb = i * Z + z;  // the wave's 32 keys
+      if (kb >= mine) continue;
+      const char *kf = lds + (i & 1) * kStage + z * S::kHalf, *vf = kf + kPart;
+      const int64_t tile = tile_of(i), in_tile = tile * kTile + 32 * (kb & 1);
+      const int wk = scalar(a.ek + tile), wv = scalar(a.ev + tile);
+      const int ek = MIXED ? base_of(wk) : wk, ev = MIXED ? base_of(wv) : wv;
+      f16 s, r;
+      two_products<DP, false>(s, r, kf, vf, q, go, ro);
+      if (MIXED && is_mixed(wk)) level(s, a.each_k + in_tile, ek, hi);
+      if (MIXED && is_mixed(wv)) level(r, a.each_v + in_tile, ev, hi);
+      f16 p, ds;
+      const float f = __builtin_amdgcn_ldexpf(1.f, a.exp - eq - ek), graw = __builtin_amdgcn_ldexpf(1.f, -ev);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) p[e] = score(s[e], f, m), ds[e] = dscore(p[e], r[e], graw, D);
-    if (32 * kb + 31 > q0) {
+      for (int e = 0; e < 16; ++e) p[e] = score(s[e], f, m), ds[e] = dscore(p[e], r[e], graw, D);
+      if (32 * kb + 31 > q0) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (32 * kb + out_row(e, hi) > q0 + c) ds[e] = 0.f;
+        for (int e = 0; e < 16; ++e)
+          if (32 * kb + out_row(e, hi) > q0 + c) ds[e] = 0.f;
+      }
+      int shift = 0;
+      if (MIXED && is_mixed(wk)) shift = weigh(ds, a.each_k + in_tile, ek, hi);
+      float y[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) y[e] = ds[e];
+      const int top = top_exponent(top_of(ds, 0.f));
+      const float up = __builtin_amdgcn_ldexpf(1.f, 15 - top);
+      const Terms b[2] = {split8(y, up), split8(y + 8, up)};
+      const float back = __builtin_amdgcn_ldexpf(a.scale, top - 15 - shift - eg - ek);
+      Terms k0 = columns_of(kf, 0, 0, co), k1 = columns_of(kf, 0, 1, co);
+#pragma unroll
+      for (int nb = 0; nb < S::NB; ++nb) {
+        Terms na, nc;
+        if (nb + 1 < S::NB) na = columns_of(kf, nb + 1, 0, co), nc = columns_of(kf, nb + 1, 1, co);
+        __builtin_amdgcn_sched_barrier(0);
+        f16 u = {};
+        mma(u, k0, b[0]);
+        mma(u, k1, b[1]);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[nb][e] = fmaf(u[e], back, x[nb][e]);
+        k0 = na, k1 = nc;
+      }
     }
-    float y[16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) y[e] = ds[e];
-    const int top = top_exponent(ds);
-    const float up = __builtin_amdgcn_ldexpf(1.f, 15 - top);
-    const Terms b[2] = {split8(y, up), split8(y + 8, up)};
-    const float back = __builtin_amdgcn_ldexpf(a.scale, top - 15 - eg - ek);
-    Terms k0 = columns_of(kf, 0, 0, co), k1 = columns_of(kf, 0, 1, co);
-#pragma unroll
-    for (int nb = 0; nb < S::NB; ++nb) {
-      Terms na, nc;
-      if (nb + 1 < S::NB) na = columns_of(kf, nb + 1, 0, co), nc = columns_of(kf, nb + 1, 1, co);
-      __builtin_amdgcn_sched_barrier(0);
-      f16 u = {};
-      mma(u, k0, b[0]);
-      mma(u, k1, b[1]);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) x[nb][e] = fmaf(u[e], back, x[nb][e]);
-      k0 = na, k1 = nc;
-    }
-  }
+  });
   f16 *sets[S::NB];
 #pragma unroll
   for (int b = 0; b < S::NB; ++b) sets[b] = &x[b];
@@ -760,6 +880,7 @@ template <int DP, int Z>
 __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t, int h0, char *lds) {
   using S = Shape<DP>;
   constexpr int R = 4 / Z, kPart = Z * S::kHalf, kStage = 2 * kPart + 256 * Z;
+  __shared__ int flags[4];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rw = w % R, z = w / R;
   const int c = lane & 31, hi = lane >> 5, g = h0 / (a.heads / a.kv_heads);
@@ -767,16 +888,18 @@ __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t
   const int64_t kv0 = (int64_t)t.tile0 * a.kv_heads + g, row = t.row0 + k0 + c;
   const int first = t.t0 / kTile, all = (t.len - 1) / kTile;
   const bool live = k0 < t.len, mine_in = k0 + c < t.len;
-  bool odd = false;
+  bool odd = false, mixed = false;
   for (int i = first + tid; i <= all; i += 256)
     for (int h = h0; h < h0 + a.each; ++h) {
       const int64_t at = (int64_t)(t.tile0 + i) * a.heads + h;
-      odd |= a.eq[at] == kOdd || a.eg[at] == kOdd;
+      const int wq = a.eq[at], wg = a.eg[at];
+      odd |= wq == kOdd || wg == kOdd, mixed |= is_mixed(wq) || is_mixed(wg);
     }
   Terms k[S::NS], v[S::NS];
   // the keys' terms as they are packed
-  const int ek = live ? scalar(a.ek + kv0 + (int64_t)(k0 / kTile) * a.kv_heads) : 0;
-  odd |= ek == kOdd;
+  const int64_t own = kv0 + (int64_t)((live ? k0 : t.t0) / kTile) * a.kv_heads;
+  const int wk = scalar(a.ek + own), ek = is_mixed(wk) ? a.each_k[own * kTile + (k0 & 32) + c] : wk;
+  odd |= wk == kOdd;
   int ev;
   {
     RowValues<DP> x;
@@ -786,7 +909,8 @@ __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t
     ev = exponent_for(x.top(a.most_value, odd));
     x.split_into(v, __builtin_amdgcn_ldexpf(1.f, ev));
   }
-  if (__syncthreads_or(odd)) return false;
+  const int kinds = found(flags, w, odd, mixed);
+  if (kinds & 1) return false;
   const float graw = __builtin_amdgcn_ldexpf(1.f, -ev);
   const int ro = place(hi, c), co = columns_place(lane);
 
@@ -805,60 +929,70 @@ __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t
     if (w < Z) copy4(a.rowstat + (qt * kTile + 32 * (half + w)) * 2 + lane, to + 2 * kPart + 256 * w);
   };
   issue(0);
-  for (int i = 0; i < n; ++i) {
-    fetched();
-    if (i + 1 < n) issue(i + 1);
-    const int q0 = 32 * ((b0 + i % per) * Z + z);
-    if (!live || q0 + 31 < k0 || q0 >= t.len) continue;
-    const char *stage = lds + (i & 1) * kStage, *qf = stage + z * S::kHalf, *gf = qf + kPart;
-    const float *rs = reinterpret_cast<const float *>(stage + 2 * kPart + 256 * z);
-    const int64_t qt = tile_of(i);
-    const int eq = scalar(a.eq + qt), eg = scalar(a.eg + qt);
-    f16 s, r;
-    two_products<DP, true>(s, r, qf, gf, k, v, ro);
-    float m[16], d[16];
+  by_tiles(kinds & 2, [&](auto kind) {
+    constexpr bool MIXED = decltype(kind)::value;
+    for (int i = 0; i < n; ++i) {
+      fetched();
+      if (i + 1 < n) issue(i + 1);
+      const int q0 = 32 * ((b0 + i % per) * Z + z);
+      if (!live || q0 + 31 < k0 || q0 >= t.len) continue;
+      const char *stage = lds + (i & 1) * kStage, *qf = stage + z * S::kHalf, *gf = qf + kPart;
+      const float *rs = reinterpret_cast<const float *>(stage + 2 * kPart + 256 * z);
+      const int64_t qt = tile_of(i);
+      const int64_t in_tile = qt * kTile + (q0 & 32);
+      const int wq = scalar(a.eq + qt), wg = scalar(a.eg + qt);
+      const int eq = MIXED ? base_of(wq) : wq, eg = MIXED ? base_of(wg) : wg;
+      f16 s, r;
+      two_products<DP, true>(s, r, qf, gf, k, v, ro);
+      if (MIXED && is_mixed(wq)) level(s, a.each_q + in_tile, eq, hi);
+      if (MIXED && is_mixed(wg)) level(r, a.each_g + in_tile, eg, hi);
+      float m[16], d[16];
 #pragma unroll
-    for (int e = 0; e < 16; e += 2) {
-      const f4 y = *reinterpret_cast<const f4 *>(rs + 2 * out_row(e, hi));
-      m[e] = y[0], d[e] = y[1], m[e + 1] = y[2], d[e + 1] = y[3];
-    }
-    f16 p, ds;
-    const float f = __builtin_amdgcn_ldexpf(1.f, a.exp - eq - ek);
-#pragma unroll
-    for (int e = 0; e < 16; ++e) p[e] = score(s[e], f, m[e]), ds[e] = dscore(p[e], r[e], graw, d[e]);
-    if (q0 < k0 + 31) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (q0 + out_row(e, hi) < k0 + c) p[e] = 0.f, ds[e] = 0.f;
-    }
-    float y[16], z[16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) y[e] = p[e], z[e] = ds[e];
-    const int ptop = top_exponent(p), stop = top_exponent(ds);
-    const float pup = __builtin_amdgcn_ldexpf(1.f, 15 - ptop), sup = __builtin_amdgcn_ldexpf(1.f, 15 - stop);
-    const Terms pb[2] = {split8(y, pup), split8(y + 8, pup)}, sb[2] = {split8(z, sup), split8(z + 8, sup)};
-    const float bv = __builtin_amdgcn_ldexpf(1.f, ptop - 15 - eg);
-    const float bk = __builtin_amdgcn_ldexpf(a.scale_q, stop - 15 - eg - eq);
-    Terms ga = columns_of(gf, 0, 0, co), qa = columns_of(qf, 0, 0, co);
-#pragma unroll
-    for (int nb = 0; nb < S::NB; ++nb) {
-      f16 u = {}, x = {};
-#pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        Terms gn, qn;
-        if (nb + st < S::NB) gn = columns_of(gf, nb + st, 1 - st, co), qn = columns_of(qf, nb + st, 1 - st, co);
-        __builtin_amdgcn_sched_barrier(0);
-        mma(u, ga, pb[st]);
-        mma(x, qa, sb[st]);
-        ga = gn, qa = qn;
+      for (int e = 0; e < 16; e += 2) {
+        const f4 y = *reinterpret_cast<const f4 *>(rs + 2 * out_row(e, hi));
+        m[e] = y[0], d[e] = y[1], m[e + 1] = y[2], d[e + 1] = y[3];
       }
+      f16 p, ds;
+      const float f = __builtin_amdgcn_ldexpf(1.f, a.exp - eq - ek);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        xv[nb][e] = fmaf(u[e], bv, xv[nb][e]);
-        xk[nb][e] = fmaf(x[e], bk, xk[nb][e]);
+      for (int e = 0; e < 16; ++e) p[e] = score(s[e], f, m[e]), ds[e] = dscore(p[e], r[e], graw, d[e]);
+      if (q0 < k0 + 31) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (q0 + out_row(e, hi) < k0 + c) p[e] = 0.f, ds[e] = 0.f;
+      }
+      int pshift = 0, sshift = 0;
+      if (MIXED && is_mixed(wg)) pshift = weigh(p, a.each_g + in_tile, eg, hi);
+      if (MIXED && is_mixed(wq)) sshift = weigh(ds, a.each_q + in_tile, eq, hi);
+      float y[16], z[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) y[e] = p[e], z[e] = ds[e];
+      const int ptop = top_exponent(top_of(p, 0.f)), stop = top_exponent(top_of(ds, 0.f));
+      const float pup = __builtin_amdgcn_ldexpf(1.f, 15 - ptop), sup = __builtin_amdgcn_ldexpf(1.f, 15 - stop);
+      const Terms pb[2] = {split8(y, pup), split8(y + 8, pup)}, sb[2] = {split8(z, sup), split8(z + 8, sup)};
+      const float bv = __builtin_amdgcn_ldexpf(1.f, ptop - 15 - pshift - eg);
+      const float bk = __builtin_amdgcn_ldexpf(a.scale_q, stop - 15 - sshift - eg - eq);
+      Terms ga = columns_of(gf, 0, 0, co), qa = columns_of(qf, 0, 0, co);
+#pragma unroll
+      for (int nb = 0; nb < S::NB; ++nb) {
+        f16 u = {}, x = {};
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          Terms gn, qn;
+          if (nb + st < S::NB) gn = columns_of(gf, nb + st, 1 - st, co), qn = columns_of(qf, nb + st, 1 - st, co);
+          __builtin_amdgcn_sched_barrier(0);
+          mma(u, ga, pb[st]);
+          mma(x, qa, sb[st]);
+          ga = gn, qa = qn;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          xv[nb][e] = fmaf(u[e], bv, xv[nb][e]);
+          xk[nb][e] = fmaf(x[e], bk, xk[nb][e]);
+        }
       }
     }
-  }
+  });
   f16 *sets[2 * S::NB];
 #pragma unroll
   for (int b = 0; b < S::NB; ++b) sets[2 * b] = &xk[b], sets[2 * b + 1] = &xv[b];

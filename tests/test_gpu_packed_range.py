@@ -7,10 +7,11 @@ what the scores of the keys that it attends to are off by: a key of probability 
 and a row whose largest score stands out by more than 200 and both scores' errors is that key's alone,
 p = 1, whatever the scores' rounding.
 
-The kernels hold an operand to 2^-23 of it, which the counts above cover, or to 2^-39 of the largest magnitude
-of its 64 tokens, as the header says: a tile is scaled so that this one lies in [2^14, 2^15), where half a
-step of the second fp16 term, at least 2^-25, is at most 2^-39 of it. What that leaves of a value alone (a
-probability of 1 and a value of 1e-5 beside ones of 4) is part of the bound."""
+The kernels hold an operand to 2^-23 of it, which the counts above cover, or to 2^-33 of the largest magnitude
+of its token and head, as the header says: 64 tokens are scaled so that their largest lies in [2^14, 2^15),
+where half a step of the second fp16 term, at least 2^-25, is at most 2^-39 of it; and tokens that differ by more
+than 2^6 are scaled each by itself. What that leaves of a value alone (a probability of 1 and a value of 1e-6
+beside ones of 4) is part of the bound."""
 import math
 
 import numpy as np
@@ -24,8 +25,8 @@ NAMES = ("out", "dq", "dk", "dv")
 
 
 def _held(x):
-    """The largest magnitude of each row's 64 tokens."""
-    return np.repeat([abs(x[i:i + 64]).max() for i in range(0, len(x), 64)], 64)[:len(x), None]
+    """The largest magnitude of each row."""
+    return abs(x).max(1, keepdims=True)
 
 
 def _ref(call, settled=False):
@@ -60,7 +61,7 @@ def _ref(call, settled=False):
             alone[rows, h] = one
             f[one] = 0
             out = p @ V
-            out_err = (p * f) @ abs(V) + U2 * (n + 8) * (p @ abs(V)) + 2.0 ** -39 * (p @ _held(V))
+            out_err = (p * f) @ abs(V) + U2 * (n + 8) * (p @ abs(V)) + 2.0 ** -33 * (p @ _held(V))
             r = O @ V.T
             D = (O * out).sum(1, keepdims=True)
             D_err = (abs(O) * out_err).sum(1, keepdims=True) + U2 * (dh + 8) * (abs(O) * abs(out)).sum(1, keepdims=True)
@@ -69,7 +70,7 @@ def _ref(call, settled=False):
             for name, s_, x, err in (("out", c, out, out_err),
                                      ("dq", c, a * (ds @ K), a * (ds_err + U2 * (n + 8) * abs(ds)) @ abs(K)),
                                      ("dk", ck, a * (ds.T @ Q), a * (ds_err + U2 * (n * G + 8) * abs(ds)).T @ abs(Q)),
-                                     ("dv", ck, p.T @ O, (p * (f + U2 * (n * G + 8))).T @ abs(O) + 2.0 ** -39 * (p.T @ _held(O)))):
+                                     ("dv", ck, p.T @ O, (p * (f + U2 * (n * G + 8))).T @ abs(O) + 2.0 ** -33 * (p.T @ _held(O)))):
                 res[name][0][rows, s_] += x
                 res[name][1][rows, s_] += err
     return (res, alone) if settled else res
@@ -152,7 +153,7 @@ def test_values_of_zero_beside_small_ones(hip_ctx, size, lengths):
 
 
 @pytest.mark.parametrize("lengths", [[256], [900]])
-@pytest.mark.parametrize("size", [1e4, 1e6])
+@pytest.mark.parametrize("size", [1e4, 1e6, 1e9, 1e15])
 def test_a_value_far_above_the_others(hip_ctx, size, lengths):
     """A value that the rows behind it have no probability for: their gradients keep their accuracy."""
     call = _Call(hip_ctx, lengths, 4, 2, 64, np.random.default_rng(9))
@@ -165,12 +166,14 @@ def test_a_value_far_above_the_others(hip_ctx, size, lengths):
         _check(got[name], ref[name], name)
 
 
-@pytest.mark.parametrize("gap", [15])
+@pytest.mark.parametrize("gap", [15, 30, 60])
 @pytest.mark.parametrize("lengths", [[200], [140] * 30])
 def test_keys_with_hardly_any_probability(hip_ctx, gap, lengths):
     """A key with 2^-gap of the others' probability in every row, its value 2^gap times theirs: half of the
-    output; and what it gets of the gradients, 2^-gap of theirs, to the same relative accuracy, less what a
-    score's own roundings (its scale's, its own, the difference's: half a step of gap each) leave of it."""
+    output, and of the sums in dq; and what it gets of the gradients, 2^-gap of theirs, to the same relative
+    accuracy, less what a score's own roundings (its scale's, its own, the difference's: half a step of gap
+    each) leave of its probability."""
+    norm = 2e-6 + 3 * gap * math.log(2) * U2 / 2
     call = _Call(hip_ctx, lengths, 16, 4, 64, np.random.default_rng(gap))
     q, k, v = call.parts(call.x)
     q[:], k[:] = 0, 0
@@ -182,8 +185,63 @@ def test_keys_with_hardly_any_probability(hip_ctx, gap, lengths):
     v[starts + 70] *= np.float32(2.0 ** gap)
     got, ref = _run(call), _ref(call)
     for name in NAMES:
-        _check(got[name], ref[name], name)
+        _check(got[name], ref[name], name, norm)
         if name in ("dk", "dv"):
             rows = starts + 70
-            _check(got[name][rows], tuple(r[rows] for r in ref[name]), f"{name} of those keys",
-                   2e-6 + 3 * gap * math.log(2) * U2 / 2)
+            _check(got[name][rows], tuple(r[rows] for r in ref[name]), f"{name} of those keys", norm)
+
+
+def _all_but(call, ref, got, rows, what):
+    """Every row of the outputs but the named ones."""
+    keep = np.ones(call.T, bool)
+    keep[rows] = False
+    for name in NAMES:
+        _check(got[name][keep], tuple(r[keep] for r in ref[name]), f"{what}: {name}")
+
+
+@pytest.mark.parametrize("lengths", [[64], [500], [150] * 30])
+@pytest.mark.parametrize("size", [1e3, 1e5, 1e8, 1e12, 1e14])
+def test_later_tokens_far_above(hip_ctx, size, lengths):
+    """A last query, key and value far above the others', which no earlier row attends to: the earlier rows
+    and what they pass on are as accurate as without it."""
+    call = _Call(hip_ctx, lengths, 16, 4, 64, np.random.default_rng(22))
+    last = np.cumsum(lengths) - 1
+    for x in call.parts(call.x):
+        x[last] *= np.float32(size)
+    call.g[last] = 0  # what its own row passes on has another scale
+    _all_but(call, _ref(call), _run(call), last, "last")
+
+
+@pytest.mark.parametrize("lengths", [[64], [500], [150] * 30])
+@pytest.mark.parametrize("size", [1e3, 1e5, 1e8, 1e12])
+def test_early_tokens_far_above(hip_ctx, size, lengths):
+    """A first output's gradient far above the others', which reaches the first key and value only; and a
+    second token whose key no later row attends to (their scores for it are far below) and whose value is
+    as far above the others'."""
+    call = _Call(hip_ctx, lengths, 16, 4, 64, np.random.default_rng(23))
+    q, k, v = call.parts(call.x)
+    first = np.cumsum(lengths) - lengths
+    call.g[first] *= np.float32(size)
+    q[:] = abs(q)
+    k[first + 1] = -abs(k[first + 1]) * np.float32(size) - 100
+    v[first + 1] *= np.float32(size)
+    call.g[first + 1] = 0
+    _all_but(call, _ref(call), _run(call), np.concatenate([first, first + 1]), "first")
+
+
+@pytest.mark.parametrize("part", ["q", "k", "v", "g"])
+@pytest.mark.parametrize("power", [-75, -30, -13, 13, 30, 59, 75])
+def test_tokens_of_every_size(hip_ctx, power, part):
+    """One operand's tokens spread over 2^|power|, the scores kept ordinary by the others. (Queries and keys of
+    2^75 are the row kernels'.)"""
+    call = _Call(hip_ctx, [64, 300, 33], 4, 2, 40, np.random.default_rng(power + 200))
+    rng = np.random.default_rng(5)
+    x = dict(zip("qkv", call.parts(call.x)), g=call.g)
+    spread = (2.0 ** (power * rng.random((call.T, 1)))).astype(np.float32)
+    x[part][:] *= spread
+    if part in "qk":
+        # so that the largest meets ordinary scores
+        x["k" if part == "q" else "q"][:] *= np.float32(2.0 ** min(0, -power))
+    got, ref = _run(call), _ref(call)
+    for name in NAMES:
+        _within(got[name], ref[name], name)
