@@ -727,9 +727,11 @@ __device__ __forceinline__ void two_products(f16 &s, f16 &r, const char *pa, con
   }
 }
 
-// Writes a wave's 32 columns of a transposed result: row `row` of the matrix at p.
+// Writes a wave's 32 columns of a transposed result, times `by`, to the row at p. (The sums are added with powers
+// of two alone, which are exact down to fp32's smallest: a scale with a mantissa among them lost bits of
+// results below 2^-97.)
 template <int DP>
-__device__ __forceinline__ void put_rows(float *p, const f16 (&x)[DP / 32], int dh, int hi, int accumulate) {
+__device__ __forceinline__ void put_rows(float *p, const f16 (&x)[DP / 32], float by, int dh, int hi, int accumulate) {
 #pragma unroll
   for (int b = 0; b < DP / 32; ++b)
 #pragma unroll
@@ -738,7 +740,7 @@ __device__ __forceinline__ void put_rows(float *p, const f16 (&x)[DP / 32], int 
       if (d < dh) {
         f4 y;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = x[b][4 * e + j];
+        for (int j = 0; j < 4; ++j) y[j] = x[b][4 * e + j] * by;
         if (accumulate) y += f4(*reinterpret_cast<const f4u *>(p + d));
         *reinterpret_cast<f4u *>(p + d) = y;
       }
@@ -850,7 +852,7 @@ __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t,
       const int top = top_exponent(top_of(ds, 0.f));
       const float up = __builtin_amdgcn_ldexpf(1.f, 15 - top);
       const Terms b[2] = {split8(y, up), split8(y + 8, up)};
-      const float back = __builtin_amdgcn_ldexpf(a.scale, top - 15 - shift - eg - ek);
+      const float back = __builtin_amdgcn_ldexpf(1.f, top - 15 - shift - eg - ek);
       Terms k0 = columns_of(kf, 0, 0, co), k1 = columns_of(kf, 0, 1, co);
 #pragma unroll
       for (int nb = 0; nb < S::NB; ++nb) {
@@ -870,7 +872,7 @@ __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t,
 #pragma unroll
   for (int b = 0; b < S::NB; ++b) sets[b] = &x[b];
   join_sets<Z>(sets, lds, rw, z, lane);
-  if (mine_in && z == 0) put_rows<DP>(a.dq + row * a.ld_q + (int64_t)h * a.dh, x, a.dh, hi, a.accumulate);
+  if (mine_in && z == 0) put_rows<DP>(a.dq + row * a.ld_q + (int64_t)h * a.dh, x, a.scale, a.dh, hi, a.accumulate);
   return true;
 }
 
@@ -971,7 +973,7 @@ __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t
       const float pup = __builtin_amdgcn_ldexpf(1.f, 15 - ptop), sup = __builtin_amdgcn_ldexpf(1.f, 15 - stop);
       const Terms pb[2] = {split8(y, pup), split8(y + 8, pup)}, sb[2] = {split8(z, sup), split8(z + 8, sup)};
       const float bv = __builtin_amdgcn_ldexpf(1.f, ptop - 15 - pshift - eg);
-      const float bk = __builtin_amdgcn_ldexpf(a.scale_q, stop - 15 - sshift - eg - eq);
+      const float bk = __builtin_amdgcn_ldexpf(1.f, stop - 15 - sshift - eg - eq);
       Terms ga = columns_of(gf, 0, 0, co), qa = columns_of(qf, 0, 0, co);
 #pragma unroll
       for (int nb = 0; nb < S::NB; ++nb) {
@@ -1003,8 +1005,8 @@ __device__ __forceinline__ bool dkv_tile(const BackwardArgs &a, const SeqTile &t
   const int64_t at = part ? ((int64_t)h0 * a.total + row) * a.dh : 0;
   const int64_t ck = part ? at : row * a.ld_k + (int64_t)g * a.dh;
   const int64_t cv = part ? at : row * a.ld_v + (int64_t)g * a.dh;
-  if (a.dk != nullptr) put_rows<DP>(a.dk + ck, xk, a.dh, hi, a.acc_kv);
-  if (a.dv != nullptr) put_rows<DP>(a.dv + cv, xv, a.dh, hi, a.acc_kv);
+  if (a.dk != nullptr) put_rows<DP>(a.dk + ck, xk, a.scale_q, a.dh, hi, a.acc_kv);
+  if (a.dv != nullptr) put_rows<DP>(a.dv + cv, xv, 1.f, a.dh, hi, a.acc_kv);
   return true;
 }
 

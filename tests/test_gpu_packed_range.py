@@ -230,7 +230,7 @@ def test_early_tokens_far_above(hip_ctx, size, lengths):
 
 
 @pytest.mark.parametrize("part", ["q", "k", "v", "g"])
-@pytest.mark.parametrize("power", [-75, -30, -13, 13, 30, 59, 75])
+@pytest.mark.parametrize("power", [-100, -75, -30, -13, 13, 30, 59, 75])
 def test_tokens_of_every_size(hip_ctx, power, part):
     """One operand's tokens spread over 2^|power|, the scores kept ordinary by the others. (Queries and keys of
     2^75 are the row kernels'.)"""
@@ -245,3 +245,13 @@ def test_tokens_of_every_size(hip_ctx, power, part):
     got, ref = _run(call), _ref(call)
     for name in NAMES:
         _within(got[name], ref[name], name)
+
+
+@pytest.mark.parametrize("lengths", [[90, 200], [140] * 30])
+def test_small_gradients(hip_ctx, lengths):
+    """Gradients of 2^-105, well inside fp32's normal range as their results are."""
+    call = _Call(hip_ctx, lengths, 16, 4, 64, np.random.default_rng(24))
+    call.g *= np.float32(2.0 ** -105)
+    got, ref = _run(call), _ref(call)
+    for name in NAMES:
+        _check(got[name], ref[name], name)
