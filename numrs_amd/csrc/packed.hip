@@ -61,11 +61,12 @@ __device__ void row_forward(const FwdArgs &a, const SeqTile &t, int r, int h, fl
     const int j = j0 + lane, n = min(64, r + 1 - j0);
     const float s = lane < n ? dot_row(x, k + j * a.ld_kv, a.dh) * a.alpha : -INFINITY;
     const float top = fmaxf(m, wave_max(s));
-    // A row whose scores are all -inf has no softmax: NaN, as the formula has it.
-    const float p = lane < n ? exp2f(s - top) : 0.f, c = j0 == 0 ? 0.f : exp2f(m - top);
+    // Scores of -inf so far count nothing beside a finite one that may follow. A row that has no other has no
+    // softmax: l stays 0 and the result NaN, as the formula has it.
+    const float p = lane >= n || s == -INFINITY ? 0.f : exp2f(s - top), c = m == -INFINITY ? 0.f : exp2f(m - top);
     m = top;
     l = l * c + wave_sum(p);
-    if (l != l) break;  // the row is NaN, whatever follows
+    if (l != l) break;  // a score is NaN or infinite: so is the row, whatever follows
     float t0 = 0.f, t1 = 0.f;  // the block's sum apart, so that a long sum's rounding stays small
     for (int e = 0; e < n; ++e) {
       const float w = lane_of(p, e);

@@ -255,3 +255,34 @@ def test_small_gradients(hip_ctx, lengths):
     got, ref = _run(call), _ref(call)
     for name in NAMES:
         _check(got[name], ref[name], name)
+
+
+@pytest.mark.parametrize("dh", [24, 128])
+def test_a_row_whose_first_scores_are_minus_infinity(hip_ctx, dh):
+    """The first 64 keys score -inf (an infinite column, or products past fp32): the rows behind attend to
+    the others alone, the rows before have no softmax."""
+    for kind in ("infinite", "past fp32"):
+        call = _Call(hip_ctx, [200], 2, 1, dh, np.random.default_rng(31))
+        q, k, v = call.parts(call.x)
+        q[:, 0], q[:, dh] = abs(q[:, 0]) + 1, abs(q[:, dh]) + 1
+        k[:, 0] = 0
+        k[:70, 0] = -np.inf
+        if kind == "past fp32":
+            q[:, 0] = q[:, dh] = 2e19
+            k[:70, 0] = -3e19
+        call.g[:70] = 0
+        got = _run(call)
+        # the same with the first 70 tokens' keys far below instead
+        call.x = call.x.copy()
+        q, k, v = call.parts(call.x)
+        q[:, 0] = q[:, dh] = 1
+        k[:70, 0] = -1e4
+        ref = _ref(call)
+        assert np.isnan(got["out"][:70]).all(), kind
+        _check(got["out"][70:], tuple(r[70:] for r in ref["out"]), f"{kind}: out")
+        if kind == "infinite":
+            continue  # its dq has 0 times infinity in it
+        for name in ("dq", "dk", "dv"):
+            # dk's first column has the queries' 2e19 in it
+            cols = slice(1, None) if name == "dk" else slice(None)
+            _check(got[name][70:, cols], tuple(r[70:, cols] for r in ref[name]), f"{kind}: {name}")
