@@ -286,3 +286,28 @@ def test_a_row_whose_first_scores_are_minus_infinity(hip_ctx, dh):
             # dk's first column has the queries' 2e19 in it
             cols = slice(1, None) if name == "dk" else slice(None)
             _check(got[name][70:, cols], tuple(r[70:, cols] for r in ref[name]), f"{kind}: {name}")
+
+
+@pytest.mark.parametrize("lengths,H,Hk", [([200, 65], 4, 2), ([140] * 30, 16, 4), ([129] * 150, 12, 4), ([33], 3, 1)])
+def test_the_row_kernels(hip_ctx, lengths, H, Hk):
+    """Finite values past what the tiles take, with ordinary results, so that whole sequences go to the row
+    kernels: in blocks of 64 and of 128 rows, a group's heads apart and together, written and added."""
+    call = _Call(hip_ctx, lengths, H, Hk, 32, np.random.default_rng(len(lengths)), pad=1)
+    q, k, v = call.parts(call.x)
+    q *= np.float32(2.0 ** 55)
+    k *= np.float32(2.0 ** -55)
+    ref = _ref(call)
+    call.upload()
+    T = call.T
+    _check(call.forward()[:T], ref["out"], "out")
+    prev = np.random.default_rng(1).standard_normal(call.x.shape).astype(np.float32)
+    # as large as what is added to it
+    for p, s in zip(call.parts(prev), (2.0 ** -55, 2.0 ** 55, 1)):
+        p *= np.float32(s)
+    for acc in (0, 1):
+        got = call.backward(hip_ctx.to_device(prev), acc=acc)
+        for name, part, old in zip(NAMES[1:], call.parts(got), call.parts(prev)):
+            x, err = ref[name]
+            if acc:
+                x, err = x + old[:T], err + U2 * abs(x + old[:T])
+            _check(part[:T], (x, err), f"{name}, {acc}")
