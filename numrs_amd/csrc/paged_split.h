@@ -11,8 +11,8 @@
 //   8 bits  a K block's lane has token c, columns 32 t + 8 g .. + 7, a V block's the codes of tokens
 //           4 g .. + 3 of columns 4 c .. + 3, which lie together: fp16 holds a code exactly, so the
 //           queries, and the probabilities times the values' scales, split in two fp16 terms (with
-//           a power of two that keeps them in range), are the products' only rounding:
-//           v_mfma_f32_16x16x32_f16.
+//           a power of two for each head that puts the largest into [2^14, 2^15)), are the
+//           products' only rounding: v_mfma_f32_16x16x32_f16.
 // S^T's result rows, tokens 4 g .. + 3 of a block, are the second product's operand in place.
 //
 // The tokens of all sequences, in units of 64, are dealt evenly to the workgroups of a kv head,
@@ -299,15 +299,23 @@ struct State {
       for (int b = 1; b < NB; ++b) big = fmaxf(big, max4(x.vs[b]));
       big = rows4(big, [](float i, float j) { return fmaxf(i, j); });
       const int ev = big > 0.f ? max(__builtin_amdgcn_frexp_expf(big), -110) : 0;
-      const float up = __builtin_amdgcn_ldexpf(1.f, 7 - ev), back = __builtin_amdgcn_ldexpf(1.f, ev - 7);
+      const float up = __builtin_amdgcn_ldexpf(1.f, -ev);
+      // The largest of a head's products comes to [2^14, 2^15) in turn: a token of a large scale and little
+      // probability must not cost the others their bits, nor have none itself.
+      float y[NB / 2][8], top = 0.f;
+#pragma unroll
+      for (int b = 0; b < NB; b += 2)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          y[b / 2][r] = s[b][r] * (x.vs[b][r] * up), y[b / 2][4 + r] = s[b + 1][r] * (x.vs[b + 1][r] * up);
+          top = fmaxf(fmaxf(top, y[b / 2][r]), y[b / 2][4 + r]);
+        }
+      top = rows4(top, [](float i, float j) { return fmaxf(i, j); });
+      const int et = max(__builtin_amdgcn_frexp_expf(top), -100);
+      const float lift = __builtin_amdgcn_ldexpf(1.f, 15 - et), back = __builtin_amdgcn_ldexpf(1.f, ev + et - 15);
       Terms w[NB / 2];
 #pragma unroll
-      for (int b = 0; b < NB; b += 2) {
-        float y[8];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) y[r] = s[b][r] * (x.vs[b][r] * up), y[4 + r] = s[b + 1][r] * (x.vs[b + 1][r] * up);
-        w[b / 2] = tiles::split8(y);
-      }
+      for (int b = 0; b < NB; b += 2) w[b / 2] = tiles::split8(y[b / 2], lift);
 #pragma unroll
       for (int u = 0; u < NU; ++u)
 #pragma unroll

@@ -1,0 +1,58 @@
+"""Attention over a paged cache where cached values differ in size, against float64 with the bounds of
+test_gpu_packed.py: a score is one product here, so its error is that of its roundings, ten operations'
+worth of it, for the keys that a row attends to (a probability above 2^-100)."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+
+import numrs_amd as nr
+from conftest import rand
+from numrs_amd import _lib as L
+from test_gpu_kvcache import U2, _Paged, _stands_for
+
+pytestmark = pytest.mark.gpu
+
+
+def _run(c, s, q, k, v, H):
+    """Rows written into the cache of `s` and attended to by one query a sequence: [n, H, dh]."""
+    n, dh = len(s.lengths), s.dh
+    s.cache.write(s.seqs, c.to_device(k), c.to_device(v), s.td, s.ends)
+    out, qd = c.empty((n, H * dh)), c.to_device(q)
+    c._check(L.load().numrs_hip_attention_paged(c.handle, ctypes.byref(s.cache.pages), qd.ptr, H * dh, H,
+                                                s.td.ptr, s.table.shape[1], s.ends.ptr, n, out.ptr, H * dh))
+    return out.numpy().reshape(n, H, dh)
+
+
+@pytest.mark.parametrize("format", ["f32", "int8"])
+@pytest.mark.parametrize("n", [40, 1500])
+@pytest.mark.parametrize("gap", [0, 13, 20, 30, 60, 500])
+def test_a_value_far_above_the_others(hip_ctx, gap, n, format):
+    """A token with 2^-gap of the others' probability and a value 2^min(gap, 60) times theirs; of 500, none of it."""
+    c, H, Hk, dh, rng = hip_ctx, 8, 2, 64, np.random.default_rng(gap + n)
+    s = _Paged(c, [n, 70], 16, Hk, dh, format, rng)
+    T = n + 70
+    k, v, q = np.zeros((T, Hk * dh), np.float32), rand(rng, (T, Hk * dh)), np.zeros((2, H * dh), np.float32)
+    q[:, ::dh] = 8
+    # a row of one value has the code 127 for it: the cache holds it to a rounding
+    k[:, ::dh] = rng.uniform(-1, 1, (T, Hk)).astype(np.float32)
+    for at in (7, n + 33):
+        k[at, ::dh] = -np.float32(gap * math.log(2))
+        v[at] *= np.float32(2.0 ** min(gap, 60))
+    got = _run(c, s, q, k, v, H)
+    K, V = (_stands_for(x.reshape(T, Hk, dh), format).astype(np.float64) for x in (k, v))
+    at = 0
+    for i, m in enumerate(s.lengths):
+        for h in range(H):
+            x, y = K[at:at + m, h // (H // Hk), 0], V[at:at + m, h // (H // Hk)]
+            p = np.exp(x - x.max())
+            p /= p.sum()
+            f = 2 * U2 * 10 * abs(x[p > 2.0 ** -100]).max() + U2 * (m + 8)
+            ref, err = p @ y, f * (p @ abs(y))
+            d = abs(got[i, h] - ref)
+            assert (d <= err).all(), f"row {i}, head {h}: off by {(d / err).max():.2g} of the bound"
+            # besides the worst case: sums of fp32 terms, and a score's three roundings at the gap's size
+            norm = 2e-6 + 3 * min(gap, 60) * math.log(2) * U2 / 2
+            assert np.linalg.norm(d) <= norm * np.linalg.norm(ref), f"row {i}, head {h}: {np.linalg.norm(d):.2g}"
+        at += m
