@@ -84,7 +84,7 @@ struct SplitArgs {
 constexpr int kUnit = 64;       // tokens
 constexpr int kJoin = 16;       // parts that one workgroup adds: two levels for up to kJoin^2 shares
 constexpr int kWaves = 8;       // of a workgroup
-constexpr float kNever = -3.4e38f;  // a softmax reference before any score: below every finite one
+constexpr float kNever = -__FLT_MAX__;  // a softmax reference before any score: no finite one is below
 
 // Floats of a part: references and sums of 16 heads, then their outputs.
 template <int DP>

@@ -56,3 +56,16 @@ def test_a_value_far_above_the_others(hip_ctx, gap, n, format):
             norm = 2e-6 + 3 * min(gap, 60) * math.log(2) * U2 / 2
             assert np.linalg.norm(d) <= norm * np.linalg.norm(ref), f"row {i}, head {h}: {np.linalg.norm(d):.2g}"
         at += m
+
+
+def test_the_lowest_scores(hip_ctx):
+    """One token whose score, in base 2, lies between fp32's lowest and -3.4e38: its value is the result."""
+    c, H, Hk, dh = hip_ctx, 2, 1, 64
+    s = _Paged(c, [1], 16, Hk, dh, "int8", np.random.default_rng(0))
+    k, q = np.zeros((1, dh), np.float32), np.zeros((1, H * dh), np.float32)
+    v = rand(np.random.default_rng(1), (1, dh))
+    k[0, 0] = -2.0 ** 66
+    q[0, ::dh] = 3.4015e38 / (math.log2(math.e) / 8) / 2.0 ** 66
+    got = _run(c, s, q, k, v, H)
+    want = _stands_for(v.reshape(1, Hk, dh), "int8").reshape(dh)
+    assert (abs(got[0] - want) <= 9 * U2 * abs(want)).all()
