@@ -508,9 +508,10 @@ __global__ void __launch_bounds__(64 * kWaves, 2) split_rows(SplitArgs a) {
   const int shares = (int)min((int64_t)a.shares, units), p = blockIdx.x / (a.c.kv_heads * a.blocks);
   if (p >= shares) return;
   const int64_t lo = first_unit(p, units, shares), hi = first_unit(p + 1, units, shares);
-  // What all workgroups read against the 256 MB of the last cache.  Past it on MI355X: 5.2 GB in 784 us in
-  // place of 866; 70 MB, which that cache holds until the next step, in 42 in place of 38.
-  const bool past = units * kUnit * (INT8 ? 2 : 8) * a.c.kv_heads * a.c.dh > int64_t{256} << 20;
+  // What all workgroups read, at most the whole cache however many sequences share its pages, against the
+  // 256 MB of the last cache.  Past it on MI355X: 5.2 GB in 784 us in place of 866; 70 MB, which that cache
+  // holds until the next step, in 42 in place of 38.
+  const bool past = min(units * kUnit, a.c.pages << a.c.shift) * (INT8 ? 2 : 8) * a.c.kv_heads * a.c.dh > int64_t{256} << 20;
   const int64_t stride = (int64_t)a.c.kv_heads * a.blocks;  // workgroup q of this block is hc + q stride
 
   // This workgroup's part of the j-th sequence of those in LDS.

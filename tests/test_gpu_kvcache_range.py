@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 import numrs_amd as nr
-from conftest import rand
+from conftest import assert_bits, rand
 from numrs_amd import _lib as L
 from test_gpu_kvcache import U2, _Paged, _stands_for
 
@@ -69,3 +69,27 @@ def test_the_lowest_scores(hip_ctx):
     got = _run(c, s, q, k, v, H)
     want = _stands_for(v.reshape(1, Hk, dh), "int8").reshape(dh)
     assert (abs(got[0] - want) <= 9 * U2 * abs(want)).all()
+
+
+@pytest.mark.parametrize("format", ["f32", "int8"])
+def test_shared_pages_of_a_large_and_of_a_small_cache(hip_ctx, format):
+    """600 sequences on the same 64 pages, 1.2 GB and more read by one call: the pages of a cache of 260 MB and
+    more, which is read past the caches, and of one that is said to end behind them, which is not."""
+    c, rng, page, H, Hk, dh, n = hip_ctx, np.random.default_rng(29), 64, 4, 2, 128, 600
+    token = Hk * dh * (8 if format == "f32" else 2)
+    cache = nr.KVCache(270_000_000 // (token * page), page, Hk, dh, format, ctx=c)
+    seqs, table = nr.PackedSequences([4096], ctx=c), c.to_device(np.arange(64, dtype=np.int32)[None])
+    k, v = (c.to_device(rand(rng, (4096, Hk * dh))) for _ in range(2))
+    cache.write(seqs, k, v, table, c.to_device(np.array([4096], np.int32)))
+    lengths = rng.integers(3900, 4097, n).astype(np.int32)
+    q, ends = c.to_device(rand(rng, (n, H * dh))), c.to_device(lengths)
+    td = c.to_device(np.repeat(np.arange(64, dtype=np.int32)[None], n, 0))
+    got = []
+    for pages in (cache.pages.pages, 64):
+        cache.pages.pages = pages
+        out = c.empty((n, H * dh))
+        c._check(L.load().numrs_hip_attention_paged(c.handle, ctypes.byref(cache.pages), q.ptr, H * dh, H, td.ptr,
+                                                    64, ends.ptr, n, out.ptr, H * dh))
+        got.append(out.numpy())
+    assert np.isfinite(got[0]).all() and (got[0] != 0).any(1).all()
+    assert_bits(got[1], got[0])
