@@ -41,9 +41,8 @@ struct Group {
 //
 // A workgroup has one tile and one head.  Bound by memory: 28 thousand tokens of 8 heads of 128 in 8 bits,
 // 290 MB each way, are written in 57 us (5.1 TB/s) and read in 44 (6.5 TB/s); 452 tokens of 8 heads of 64
-// in fp32 take 4 us each, latency.  The rows go past the caches, of which they would take all: 79 and 53 us
-// through them (the codes go through them: 11 us more past).  Before that, slot by slot, without groups,
-// 249 us in place of 132 for both; with all heads of its tokens in a workgroup 141.
+// in fp32 take 4 us each, latency.  Slot by slot, without groups, both took 249 us in place of 132; with all
+// heads of its tokens in a workgroup 141.
 template <class F>
 __device__ __forceinline__ void for_groups(const Cache &c, const SeqTile &t, int g, const int32_t *ends, int lanes, F &&f) {
   const int rows = min(t.len - t.t0, kTile), d = 4 * (threadIdx.x & ((1 << lanes) - 1));
@@ -138,7 +137,8 @@ __device__ __forceinline__ u4 transposed(u4 x) {
             __builtin_amdgcn_perm(d, b, 0x05040100u), __builtin_amdgcn_perm(d, b, 0x07060302u)};
 }
 
-template <bool INT8>
+// PAST: the rows go past the caches (see rows_past).
+template <bool INT8, bool PAST>
 __global__ void __launch_bounds__(256) write_rows(RowArgs a, int lanes) {
   const SeqTile t = a.tiles[blockIdx.x / a.c.kv_heads];
   const int g = blockIdx.x % a.c.kv_heads, dh = a.c.dh;
@@ -150,8 +150,8 @@ __global__ void __launch_bounds__(256) write_rows(RowArgs a, int lanes) {
       k[r] = v[r] = f4{};
       if (!in || x.row[r] < 0) continue;
       const int64_t at = (int64_t)(t.row0 + x.row[r]) * a.ld + (int64_t)g * dh + d;
-      k[r] = __builtin_nontemporal_load(reinterpret_cast<const f4u *>(a.k + at));
-      v[r] = __builtin_nontemporal_load(reinterpret_cast<const f4u *>(a.v + at));
+      k[r] = paged::load<f4u, PAST>(reinterpret_cast<const char *>(a.k + at));
+      v[r] = paged::load<f4u, PAST>(reinterpret_cast<const char *>(a.v + at));
     }
     if constexpr (!INT8) {
 #pragma unroll
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(256) write_rows(RowArgs a, int lanes) {
   });
 }
 
-template <bool INT8>
+template <bool INT8, bool PAST>
 __global__ void __launch_bounds__(256) read_rows(RowArgs a, int lanes) {
   const SeqTile t = a.tiles[blockIdx.x / a.c.kv_heads];
   const int g = blockIdx.x % a.c.kv_heads, dh = a.c.dh;
@@ -235,14 +235,37 @@ __global__ void __launch_bounds__(256) read_rows(RowArgs a, int lanes) {
     for (int r = 0; r < 4; ++r) {
       if (x.row[r] < 0) continue;
       const int64_t at = (int64_t)(t.row0 + x.row[r]) * a.ld + (int64_t)g * dh + d;
-      __builtin_nontemporal_store(f4u(k[r]), reinterpret_cast<f4u *>(a.ko + at));
-      __builtin_nontemporal_store(f4u(v[r]), reinterpret_cast<f4u *>(a.vo + at));
+      f4u *ko = reinterpret_cast<f4u *>(a.ko + at), *vo = reinterpret_cast<f4u *>(a.vo + at);
+      if constexpr (PAST)
+        __builtin_nontemporal_store(f4u(k[r]), ko), __builtin_nontemporal_store(f4u(v[r]), vo);
+      else
+        *ko = k[r], *vo = v[r];
     }
   });
 }
 
 // Neighbours that share a row, four columns each: the power of two that covers a head.
 int row_lanes(int dh) { return paging::log2_of((dh + 3) / 4); }
+
+// Whether a batch's rows go past the caches: where keys and values are more than half of the last cache's 256 MB,
+// so that they would take the place of what the next kernel reads.  On MI355X, through them against past, us:
+// 8 heads of 128, writes of rows just made | and attention over them | reads back | and attention over those, in
+// fp32: 16 MB 7.1, 7.4 | 59.6, 60.8 | 6.5, 5.2 | 48.7, 49.6; 64 MB 20, 22 | 182, 190 | 22, 22 | 137, 147; 128 MB
+// 35, 42 | 363, 366 | 41, 40 | 266, 272; 256 MB 110, 75 | 777, 765 | 97, 79 | 539, 534; in 8 bits: 64 MB 15, 18 |
+// 165, 174 | 14, 15 | 131, 136; 256 MB 69, 63 | 735, 716 | 73, 54 | 523, 513.  (Codes go through them throughout:
+// past, 11 us more at 230 MB of rows.)
+bool rows_past(const Seqs &s, const numrs_hip_kv_cache &c) {
+  return s.total * 2 * c.kv_heads * c.head_dim * (int64_t)sizeof(float) > int64_t{128} << 20;
+}
+
+// Calls f(std::bool_constant<8 bits>, std::bool_constant<past>).
+template <class F>
+void with_kind(bool int8, bool past, F &&f) {
+  if (int8)
+    past ? f(std::true_type{}, std::true_type{}) : f(std::true_type{}, std::false_type{});
+  else
+    past ? f(std::false_type{}, std::true_type{}) : f(std::false_type{}, std::false_type{});
+}
 
 Cache device_cache(const numrs_hip_kv_cache &c, const int32_t *table, int64_t max_pages) {
   return {c.k, c.v, c.k_scale, c.v_scale, c.pages, max_pages, table, paging::log2_of(c.page_size),
@@ -295,10 +318,10 @@ int numrs_hip_kv_cache_write(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cache
   DeviceScope dev(ctx);
   const RowArgs a{device_cache(*cache, table, max_pages), s.in_order, ends, k, v, nullptr, nullptr, ld};
   const unsigned grid = (unsigned)(s.tiles * cache->kv_heads);
-  if (cache->format == NUMRS_HIP_KV_F32)
-    write_rows<false><<<grid, 256, 0, ctx->stream>>>(a, row_lanes((int)cache->head_dim));
-  else
-    write_rows<true><<<grid, 256, 0, ctx->stream>>>(a, row_lanes((int)cache->head_dim));
+  with_kind(cache->format == NUMRS_HIP_KV_INT8, rows_past(s, *cache), [&](auto int8, auto past) {
+    write_rows<decltype(int8)::value, decltype(past)::value>
+        <<<grid, 256, 0, ctx->stream>>>(a, row_lanes((int)cache->head_dim));
+  });
   return check_launch(ctx, "write_rows");
 }
 
@@ -314,10 +337,10 @@ int numrs_hip_kv_cache_read(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cache,
   DeviceScope dev(ctx);
   const RowArgs a{device_cache(*cache, table, max_pages), s.in_order, ends, nullptr, nullptr, k, v, ld};
   const unsigned grid = (unsigned)(s.tiles * cache->kv_heads);
-  if (cache->format == NUMRS_HIP_KV_F32)
-    read_rows<false><<<grid, 256, 0, ctx->stream>>>(a, row_lanes((int)cache->head_dim));
-  else
-    read_rows<true><<<grid, 256, 0, ctx->stream>>>(a, row_lanes((int)cache->head_dim));
+  with_kind(cache->format == NUMRS_HIP_KV_INT8, rows_past(s, *cache), [&](auto int8, auto past) {
+    read_rows<decltype(int8)::value, decltype(past)::value>
+        <<<grid, 256, 0, ctx->stream>>>(a, row_lanes((int)cache->head_dim));
+  });
   return check_launch(ctx, "read_rows");
 }
 

@@ -93,3 +93,20 @@ def test_shared_pages_of_a_large_and_of_a_small_cache(hip_ctx, format):
         got.append(out.numpy())
     assert np.isfinite(got[0]).all() and (got[0] != 0).any(1).all()
     assert_bits(got[1], got[0])
+
+
+@pytest.mark.parametrize("format", ["f32", "int8"])
+def test_more_rows_than_the_caches_hold(hip_ctx, format):
+    """134 MB of keys and values, which are written and read back past the caches, and one row fewer, which are
+    not: to the bit."""
+    c, rng, page, Hk, dh, n = hip_ctx, np.random.default_rng(30), 256, 8, 128, 2 ** 14 + 1
+    k, v = rand(rng, (n, Hk * dh)), rand(rng, (n, Hk * dh))
+    kd, vd = c.to_device(k), c.to_device(v)
+    pages = -(-n // page)
+    table = c.to_device(np.arange(pages, dtype=np.int32)[None])
+    for m in (n, n - 1):
+        cache, seqs = nr.KVCache(pages, page, Hk, dh, format, ctx=c), nr.PackedSequences([m], ctx=c)
+        ends = c.to_device(np.array([m], np.int32))
+        cache.write(seqs, kd, vd, table, ends)
+        for got, x in zip(cache.read(seqs, table, ends), (k, v)):
+            assert_bits(got.numpy(), _stands_for(x[:m].reshape(m, Hk, dh), format).reshape(m, Hk * dh))
