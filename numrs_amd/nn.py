@@ -8,7 +8,9 @@ from __future__ import annotations
 
 import numpy as np
 
+from . import _lib as L
 from .autograd import Tensor, default_context
+from .device import HipError
 
 
 class Module:
@@ -269,8 +271,11 @@ class CausalSelfAttention(Module):
     def decode(self, x: Tensor, ones, cache, table, lengths, residual: Tensor | None = None
                ) -> Tensor:
         """One new token for each sequence, x [n, d]: its key and value go into the
-        cache, and it attends to all of its sequence's tokens."""
+        cache, and it attends to all of its sequence's tokens.  It has no backward:
+        where one would be recorded it is refused, and the cache is as it was."""
         qkv = self.qkv(x)
+        if qkv.requires_grad:
+            raise HipError(L.E_INVALID, "decode has no backward: call it under no_grad()")
         cache.write_qkv(ones, qkv, self.heads, table, lengths)
         return self._project(qkv.attention_paged(cache, self.heads, table, lengths), residual)
 

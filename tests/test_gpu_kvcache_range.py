@@ -10,6 +10,7 @@ import pytest
 import numrs_amd as nr
 from conftest import assert_bits, rand
 from numrs_amd import _lib as L
+from numrs_amd import nn
 from test_gpu_kvcache import U2, _Paged, _stands_for
 
 pytestmark = pytest.mark.gpu
@@ -110,3 +111,25 @@ def test_more_rows_than_the_caches_hold(hip_ctx, format):
         cache.write(seqs, kd, vd, table, ends)
         for got, x in zip(cache.read(seqs, table, ends), (k, v)):
             assert_bits(got.numpy(), _stands_for(x[:m].reshape(m, Hk, dh), format).reshape(m, Hk * dh))
+
+
+def test_decode_that_would_be_recorded_leaves_the_cache(hip_ctx):
+    """A step outside no_grad() is refused before anything is written."""
+    before = nr.default_context()
+    nr.set_default_context(hip_ctx)
+    try:
+        c, rng, d, H, Hk, dh = hip_ctx, np.random.default_rng(31), 32, 4, 2, 16
+        attn = nn.CausalSelfAttention(*(rand(rng, s, 0.2) for s in ((H * dh, d), (Hk * dh, d), (Hk * dh, d), (d, H * dh))),
+                                      heads=H, kv_heads=Hk)
+        s = _Paged(c, [5, 20], 16, Hk, dh, "f32", rng)
+        for a in (s.cache.k, s.cache.v):
+            a.fill(3.0)
+        ones, x = nr.PackedSequences([1, 1]), nr.Tensor.new(rand(rng, (2, d)))
+        with pytest.raises(nr.HipError, match="no backward"):
+            attn.decode(x, ones, s.cache, s.td, s.ends)
+        assert all((a == 3).all() for a in s.raw())
+        with nr.no_grad():
+            attn.decode(x, ones, s.cache, s.td, s.ends)
+        assert not (s.raw()[0] == 3).all()
+    finally:
+        nr.set_default_context(before)
