@@ -365,9 +365,10 @@ int numrs_hip_attention_paged(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cach
   const int hk = (int)cache->kv_heads, dh = (int)cache->head_dim, group = (int)heads / hk;
   const int blocks = (group + 15) / 16;
   // A workgroup of eight waves a CU, which the registers allow, each with an even share of the tokens;
-  // a kv head has as many at most as two levels of joins add.  Against two of four waves, us: 333 tokens of
-  // 8 heads of 64 in fp32 11.6, 11; 34 thousand tokens of 40 sequences in 8 bits 39, 52; 131072 tokens of
-  // one head of 128 41, 50; 640 thousand tokens of 96 sequences, 5.2 GB, 868, 882.  Shares of 2 to 16 units
+  // a kv head has as many at most as two levels of joins add.  Against two of four waves, with all loads
+  // through the caches, us: 333 tokens of 8 heads of 64 in fp32 11.6, 11; 34 thousand tokens of 40 sequences
+  // in 8 bits 39, 52; 131072 tokens of one head of 128 41, 50; 640 thousand tokens of 96 sequences, 5.2 GB, 868,
+  // 882 (784 past the caches as now).  Shares of 2 to 16 units
   // at least, which leave fewer parts to join, were slower throughout.
   const int shares = std::min(std::max(1, (ctx->num_cus + hk * blocks - 1) / (hk * blocks)),
                               paged::kJoin * paged::kJoin);

@@ -4,11 +4,11 @@
 // and the backward forms p again from them.
 //
 // packed_tiles.h has the kernels that ordinary values take.  The row kernels here are the plain fp32 form,
-// a wave a row, for blocks that meet a value which those cannot take: not finite, or from 2^50 (queries and
-// keys) or 2^80 (values and the output's gradient) on.  They read every key a row at a time, some 150 times
-// slower (8192 tokens, 16 heads of 128, a value at their start infinite: 134 ms against 0.8; rows that are
-// NaN throughout end at the first such score), and are there so that such a value does to the rows that
-// attend to it what fp32 arithmetic does, and nothing to the others.
+// a wave a row, for blocks that meet a value which those cannot take: not finite, from 2^50 (queries and keys)
+// or 2^80 (values and the output's gradient) on, or of 64 tokens that differ by more than 2^140.  They read every
+// key a row at a time, some 150 times slower (8192 tokens, 16 heads of 128, a value at their start infinite:
+// 134 ms against 0.8; rows that are NaN throughout end at the first such score), and are there so that such a
+// value does to the rows that attend to it what fp32 arithmetic does, and nothing to the others.
 #include <algorithm>
 #include <cmath>
 #include <new>
@@ -199,8 +199,9 @@ __device__ void row_dkv(const BwdArgs &b, const tiles::BackwardArgs &a, const Se
   }
 }
 
-// The backward's blocks in one launch, so that each kind's last workgroups run beside the other's (35 us
-// against 18 + 23 for 16 x 256 tokens, 8 heads of 64; 93 against 46 + 57 for 2736 tokens, 10 heads of 80):
+// The backward's blocks in one launch, so that each kind's last workgroups run beside the other's (37 us for 16
+// x 256 tokens, 8 heads of 64, 97 for 2736 tokens, 10 heads of 80; with earlier splits 35 against 18 + 23 apart,
+// and 93 against 46 + 57):
 // first `keys` workgroups with a block of key rows of one kv head, or one query head's part of it, then a
 // block of query rows of one head each.
 template <int DP, int Z>
@@ -268,10 +269,11 @@ int check_packed(numrs_hip_ctx *ctx, const Seqs &s, int64_t ld_q, int64_t ld_kv,
 constexpr float kMostScore = 0x1p50f, kMostValue = 0x1p80f;
 
 // Whether the kernels take blocks of 64 rows whose keys two sets of waves share, in place of 128: where
-// there are fewer than two of the latter for each CU, and the longest walk decides.  Forward | query rows |
-// key rows on MI355X, 128 rows against 64, us: 256 blocks (16 x 256 tokens, 8 heads of 64) 14.2, 13.2 |
-// 19.0, 18.2 | 26.3, 22.9; 260 (2736 tokens, 10 heads of 80) 46, 35 | 63, 46 | 86, 57; 752 (5023 tokens, 16
-// heads of 64) 47, 47; 1024 (2 x 4096 tokens, 16 heads of 128) 403, 570 | 659, 739 | 978, 987.
+// there are fewer than two of the latter for each CU, and the longest walk decides.  Forward | forward and
+// backward on MI355X, 64 rows against 128, us: 256 blocks (16 x 256 tokens, 8 heads of 64) 20, 21 | 68.6,
+// 65.2; 260 (2736 tokens, 10 heads of 80) 40, 52 | 146, 160; 752 (5023 tokens, 16 heads of 64) 51, 53 | 224,
+// 215; 1024 (2 x 4096 tokens, 16 heads of 128) 571, 421 | 2430, 2136.  The backward alone, 256 blocks of 8 heads
+// of 64: 49, 44 for 16 x 256 tokens, but 77, 91 for 4 x 1024 and 124, 156 for 2 x 2048.
 bool few_blocks(numrs_hip_ctx *ctx, const Seqs &s, int heads) { return s.blocks * heads < 2 * ctx->num_cus; }
 
 int padded(int dh) { return (dh + 31) / 32 * 32; }
@@ -361,8 +363,8 @@ int packed_backward(numrs_hip_ctx *ctx, const Seqs &s, const float *q, int64_t l
   const bool keys = dk != nullptr || dv != nullptr;
   // The query heads of a group go to workgroups of their own, whose parts are added afterwards, unless the
   // kv heads' blocks of key rows alone are two for each CU.  Forward and backward on MI355X, heads apart
-  // against together, us: 128 blocks (16 x 256 tokens, 8 heads on 2, of 64) 66, 70; 256 (2 x 4096, 16 on 4,
-  // of 128) 2008, 2099; 512 (16 x 1024, 16 on 4, of 64) 672, 616; 1024 (32 x 1024, of 128) 3043, 2696.
+  // against together, us: 64 blocks (16 x 256 tokens, 8 heads on 2, of 64) 67, 70; 256 (2 x 4096, 16 on 4,
+  // of 128) 2126, 2230; 512 (16 x 1024, 16 on 4, of 64) 717, 659; 1024 (32 x 1024, of 128) 3137, 2830.
   const int each = group > 1 && s.blocks * Hk >= 2 * ctx->num_cus ? group : 1;
   Packed pq(ctx), pk(ctx), pv(ctx), pg(ctx);
   TempBlock rowstat(ctx), parts(ctx);

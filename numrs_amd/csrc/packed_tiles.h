@@ -476,11 +476,11 @@ __device__ __forceinline__ void join_sets(f16 *const (&x)[N], char *lds, int r, 
 // they are packed: all three kernels then form a score from the same terms in the same order, to the same
 // bits, and a row whose largest score is all there is has p = 1.
 //
-// 8192 tokens, 16 heads of 128 on 4: 0.77 to 0.83 ms by card, 330 to 357 TFLOP/s of fp32 work and three
+// 8192 tokens, 16 heads of 128 on 4: 0.77 to 0.84 ms by card, 327 to 357 TFLOP/s of fp32 work and three
 // times that on the fp16 matrix cores, which are busy 64 % of the cycles at the 1.6 GHz that the card's
 // power leaves (a large fp16 library product: 1085 TFLOP/s).  13 prompts of 1 to 1290 tokens, 16 heads of
 // 64, take 48 us, of which the longest walk, 21 stages of 64 keys, is most.  Stages of 64 keys twice in LDS
-// against 32 four times, 64 and 32 three times, there: 47, 54, 62, 58 us.
+// against 32 four times, 64 and 32 three times, there, with earlier splits: 47, 54, 62, 58 us.
 //
 // Returns false, before any write, where a tile is odd.
 template <int DP, int Z>
@@ -752,8 +752,8 @@ __device__ __forceinline__ void put_rows(float *p, const f16 (&x)[DP / 32], floa
 //
 // The backward forms S and dP twice, here and for the key rows: seven products for the formula's five,
 // against writing dS, or adding dQ by atomics whose order would change the result.  2 x 4096 tokens, 16
-// heads of 128 on 4: 1.5 ms for both, 320 TFLOP/s of the seven products' fp32 work (229 of the five's), at
-// one wave a SIMD, matrix cores busy 42 % of the cycles and the VALU 35 %, at 2.17 GHz.  As many products a
+// heads of 128 on 4: 1.52 to 1.6 ms for both, 301 to 317 TFLOP/s of the seven products' fp32 work (215 to
+// 226 of the five's), at one wave a SIMD, matrix cores busy 41 % of the cycles and the VALU 33 %, at 2.17 GHz.  As many products a
 // second as in the forward: the card's power is what bounds them, so that products a stage ahead of their
 // elements (1520 us), more stages in flight (1850) or sums taken in turn (1520) gave nothing.
 template <int DP, int Z>

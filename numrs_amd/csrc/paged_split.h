@@ -23,10 +23,10 @@
 //
 // 5.2 GB of fp32 cache (96 sequences of 6000 and 8000 tokens, 8 heads of 128) are read in 780 to 810 us,
 // 6.5 TB/s and above (a large copy: 5.54); 134 MB (131072 tokens of one head) in 37, 3.6 TB/s; 70 MB of
-// 8-bit cache of 40 sequences of 1 to 5000 tokens in 35; 333 tokens in 11.  In the short ones the way from the lengths to the
-// table, the tokens and the joins, each waiting for the one before, is what takes the time.  Loads of a
-// step into registers that a second step's leave free spilled (a wave's state, two steps' tokens): keys
-// and values are asked for into the place of those just used.
+// 8-bit cache of 40 sequences of 1 to 5000 tokens in 36; 333 tokens in 11.  In the short ones the way from the
+// lengths to the table, the tokens and the joins, each waiting for the one before, is what takes the
+// time.  Loads of a step into registers that a second step's leave free spilled (a wave's state, two
+// steps' tokens): keys and values are asked for into the place of those just used.
 #pragma once
 
 #include "packed_tiles.h"
