@@ -104,8 +104,9 @@ struct BwdArgs {
   int64_t ld_q, ld_kv, ld_out;
 };
 
-// A score less the row's largest. Where the tiles had the row, whose sums run in another order, it may come
-// out above 0, which at large scores would be any power of two. NaN stays.
+// A score less the row's largest. Where the tiles had the row in the forward, whose sums run in another order, it
+// is off by some 2^-23 of the score, and may come out above 0, which at large scores would be any power of
+// two. NaN stays.
 __device__ __forceinline__ float at_most_0(float x) { return x > 0.f ? 0.f : x; }
 
 __device__ __forceinline__ void put(float *p, float v, int accumulate) { *p = accumulate ? *p + v : v; }

@@ -311,3 +311,55 @@ def test_the_row_kernels(hip_ctx, lengths, H, Hk):
             if acc:
                 x, err = x + old[:T], err + U2 * abs(x + old[:T])
             _check(part[:T], (x, err), f"{name}, {acc}")
+
+
+# blocks of 64 and of 128 rows; a group's heads apart and together
+BLOCKS = [([300, 33], 4, 2), ([150] * 30, 16, 4), ([260] * 50, 16, 4)]
+
+
+@pytest.mark.parametrize("lengths,H,Hk", BLOCKS)
+@pytest.mark.parametrize("dh", [8, 32, 72, 128])
+def test_large_scores_of_every_head_size(hip_ctx, dh, lengths, H, Hk):
+    """Scores of about 1e9 in every form of the kernels, forward and backward."""
+    call = _Call(hip_ctx, lengths, H, Hk, dh, np.random.default_rng(dh), pad=1)
+    call.x[:, :call.pad + call.wq + call.wk] *= np.float32(3e4)
+    alone = _ref(call, settled=True)[1]
+    assert alone.mean() > 0.9
+    call.g[:, call.pad:] *= np.repeat(alone, dh, axis=1)
+    ref, got = _ref(call), _run(call)
+    keep = np.repeat(alone, dh, axis=1)
+    x, err = (r[keep] for r in ref["out"])
+    _within(got["out"][keep], (x, err), "out")
+    for name in NAMES[1:]:
+        _within(got[name], ref[name], name)
+
+
+@pytest.mark.parametrize("lengths,H,Hk", BLOCKS)
+@pytest.mark.parametrize("dh", [8, 32, 72, 128])
+def test_mixed_tiles_of_every_head_size(hip_ctx, dh, lengths, H, Hk):
+    """Last tokens of 1e6 times the others', first gradients as large, and tokens in between of 1e-4, in every
+    form of the kernels."""
+    call = _Call(hip_ctx, lengths, H, Hk, dh, np.random.default_rng(dh + 1), pad=1)
+    ends = np.cumsum(lengths)
+    last, first = ends - 1, ends - np.array(lengths)
+    for x in call.parts(call.x):
+        x[last] *= np.float32(1e6)
+        x[first + 20] *= np.float32(1e-4)
+    call.g[last] = 0
+    call.g[first] *= np.float32(1e6)
+    _all_but(call, _ref(call), _run(call), np.concatenate([first, last]), "mixed")
+
+
+@pytest.mark.parametrize("part,low,high", [("q", -110, 40), ("k", -110, 40), ("v", -75, 75), ("g", -75, 75), ("v", -110, 0)])
+def test_tokens_of_more_than_the_tiles_range(hip_ctx, part, low, high):
+    """One operand's tokens spread over 2^150, which the row kernels take, and over 2^110, which the tiles do."""
+    call = _Call(hip_ctx, [64, 150, 33], 4, 2, 40, np.random.default_rng(77))
+    x = dict(zip("qkv", call.parts(call.x)), g=call.g)
+    size = np.random.default_rng(6).uniform(low, high, (call.T, 1))
+    size[::7], size[1::7] = low, high  # both in every tile
+    x[part][:] *= (2.0 ** size).astype(np.float32)
+    if part in "qk":
+        x["k" if part == "q" else "q"][:] *= np.float32(2.0 ** -high)
+    got, ref = _run(call), _ref(call)
+    for name in NAMES:
+        _within(got[name], ref[name], name)
