@@ -392,8 +392,9 @@ int packed_backward(numrs_hip_ctx *ctx, const Seqs &s, const float *q, int64_t l
   const bool few = few_blocks(ctx, s, H);
   BwdArgs b{few ? s.few_by_work : s.by_work, q, k, v, out, dout, stats, ld_q, ld_kv, ld_out};
   tiles::BackwardArgs a{q, k, v, out, dout, stats, ld_q, ld_kv, ld_out, pq.rows, pk.rows, pv.rows, pg.rows,
-                        pq.exps, pk.exps, pv.exps, pg.exps, pq.each, pk.each, pv.each, pg.each, rowstat.f(), dq, dk, dv, ld_q, ld_kv, ld_kv, s.total,
-                        H, Hk, dh, accumulate, accumulate, each, alpha, scale, mant, exp, scale_q, kMostScore, kMostValue};
+                        pq.exps, pk.exps, pv.exps, pg.exps, pq.each, pk.each, pv.each, pg.each, rowstat.f(), dq, dk,
+                        dv, ld_q, ld_kv, ld_kv, s.total, H, Hk, dh, accumulate, accumulate, each, alpha, scale,
+                        mant, exp, scale_q, kMostScore, kMostValue};
   return with_dp(dh, [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
     tiles::pack<DP><<<(unsigned)(s.tiles * p.slots), 256, 0, ctx->stream>>>(p);

@@ -380,8 +380,8 @@ __device__ __forceinline__ float over16(const f16 &x, Op op) {
 
 // The backward's P and dS are split times a power of two that puts each column's largest of the 32 rows at
 // hand into [2^14, 2^15): the split's smallest step is then 2^-38 of that, however little of a row's
-// probability the rows have or however large another tile's values are. The scaled split costs what the plain one does, so this is eight
-// max3 and a swap for 16 elements.
+// probability the rows have or however large another tile's values are. The scaled split costs what the
+// plain one does, so this is eight max3 and a swap for 16 elements.
 __device__ __forceinline__ float top_of(const f16 &x, float r) {
 #pragma unroll
   for (int i = 0; i < 16; i += 2) r = fmaxf(fmaxf(r, fabsf(x[i])), fabsf(x[i + 1]));
@@ -402,7 +402,7 @@ __device__ __forceinline__ int weigh(f16 &x, const int *each, int base, int hi) 
 }
 
 // The exponent of a row of wave w, of largest magnitude `top`, as `pack` has it: waves w and w ^ 1 have a tile.
-// (Where that is odd for its tokens' differences alone, the row's own or the largest's.)
+// (Where that is odd for its tokens' differences alone, the row's own.)
 __device__ __forceinline__ int own_exponent(const float (&tops)[4], const float (&lows)[4], int w, float top) {
   const float big = fmaxf(tops[w], tops[w ^ 1]);
   const int word = tile_word(big, fminf(lows[w], lows[w ^ 1]));
@@ -753,9 +753,10 @@ __device__ __forceinline__ void put_rows(float *p, const f16 (&x)[DP / 32], floa
 // The backward forms S and dP twice, here and for the key rows: seven products for the formula's five,
 // against writing dS, or adding dQ by atomics whose order would change the result.  2 x 4096 tokens, 16
 // heads of 128 on 4: 1.52 to 1.6 ms for both, 301 to 317 TFLOP/s of the seven products' fp32 work (215 to
-// 226 of the five's), at one wave a SIMD, matrix cores busy 41 % of the cycles and the VALU 33 %, at 2.17 GHz.  As many products a
-// second as in the forward: the card's power is what bounds them, so that products a stage ahead of their
-// elements (1520 us), more stages in flight (1850) or sums taken in turn (1520) gave nothing.
+// 226 of the five's), at one wave a SIMD, matrix cores busy 41 % of the cycles and the VALU 33 %, at 2.17
+// GHz.  As many products a second as in the forward: the card's power is what bounds them, so that products a
+// stage ahead of their elements, more stages in flight or sums taken in turn (1520, 1850, 1520 us where the
+// kernel of then took 1505) gave nothing.
 template <int DP, int Z>
 __device__ __forceinline__ bool dq_tile(const BackwardArgs &a, const SeqTile &t, int h, char *lds) {
   using S = Shape<DP>;
