@@ -394,6 +394,46 @@ int numrs_hip_attention_packed_backward(numrs_hip_ctx *ctx, const numrs_hip_seqs
                                         float *dq, float *dk, float *dv, int64_t heads,
                                         int64_t kv_heads, int64_t dh, int accumulate);
 
+/* Query and key heads made ready for attention (no reference counterpart).
+ * Each head of q and k is normed, where there is a weight [dh] for it, and then
+ * rotated by its token's position:
+ *   n = x / sqrt(mean(x^2) + eps) * w,  (a, b) -> (a cos t - b sin t, a sin t + b cos t)
+ * with t = position * freqs[i] for the pair i of the head's first `dims`
+ * columns: columns i and dims / 2 + i (HALVES), or 2 i and 2 i + 1 (PAIRS).  The
+ * other columns keep their values.  dims is a multiple of 8 up to the head size;
+ * freqs are dims / 2 HOST values in radians a position, at most 10^6, read
+ * before the call returns.  NULL or dims 0: no rotation.  Everything is formed
+ * in 64 bits and rounded once. */
+enum { NUMRS_HIP_ROTARY_HALVES = 0, NUMRS_HIP_ROTARY_PAIRS = 1 };
+typedef struct numrs_hip_rotary {
+  const double *freqs;
+  int64_t dims;
+  int layout;
+} numrs_hip_rotary;
+
+/* x and y are projections [total, (heads + 2 kv_heads) * dh] of a packed batch,
+ * the column blocks q, k and v, rows ld_x and ld_y apart; v is copied.  y may be
+ * x, with one stride: v is then left alone.  A token's position is its place in
+ * its sequence or, with `ends` (int32 [n], device), ends[i] - length_i + place.
+ * q_weight and k_weight are NULL where those heads are not normed.
+ * Backward: from dy the gradient of x and of the weights; x is only read for
+ * heads that are normed.  dx may be dy (one stride, nothing added), dx and the
+ * weights' gradients may be NULL, and one array may be both weights' gradient.
+ * `accumulate` has a bit for each that is added to instead of written; where the
+ * weights share one array, the second's is to be set.  No atomics: the same call
+ * gives the same bits. */
+enum { NUMRS_HIP_ACC_X = 1, NUMRS_HIP_ACC_Q_WEIGHT = 2, NUMRS_HIP_ACC_K_WEIGHT = 4 };
+int numrs_hip_qk_rotary_forward(numrs_hip_ctx *ctx, const numrs_hip_seqs *seqs, const int32_t *ends,
+                                const float *x, int64_t ld_x, const float *q_weight,
+                                const float *k_weight, float eps, const numrs_hip_rotary *rotary,
+                                float *y, int64_t ld_y, int64_t heads, int64_t kv_heads, int64_t dh);
+int numrs_hip_qk_rotary_backward(numrs_hip_ctx *ctx, const numrs_hip_seqs *seqs, const int32_t *ends,
+                                 const float *x, int64_t ld_x, const float *q_weight,
+                                 const float *k_weight, float eps, const numrs_hip_rotary *rotary,
+                                 const float *dy, int64_t ld_dy, float *dx, int64_t ld_dx,
+                                 float *dq_weight, float *dk_weight, int64_t heads, int64_t kv_heads,
+                                 int64_t dh, int accumulate);
+
 /* A paged key-value cache in the caller's device memory (no reference
  * counterpart).  Page p, kv head g, slot t and value d of the keys are element
  * ((p * kv_heads + g) * page_size + t) * head_dim + d of `k`, as floats or, in
@@ -431,6 +471,19 @@ int numrs_hip_kv_cache_read(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cache,
                             const numrs_hip_seqs *seqs, float *k, float *v, int64_t ld,
                             const int32_t *table, int64_t max_pages, const int32_t *ends);
 
+/* New tokens of sequences that the cache may hold already, from one projection
+ * qkv [total, (heads + 2 kv_heads) * head_dim]: k is normed and rotated as above
+ * and written with v where numrs_hip_kv_cache_write puts them, q normed, rotated
+ * and written to q [total, heads * head_dim] (rows ld_q apart) for the attention
+ * that follows.  Positions are ends[i] - length_i + place.  The same bits as
+ * numrs_hip_qk_rotary_forward and numrs_hip_kv_cache_write in turn.  q may be
+ * NULL (keys and values only) but must not overlap qkv. */
+int numrs_hip_kv_cache_append(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cache,
+                              const numrs_hip_seqs *seqs, const float *qkv, int64_t ld,
+                              const float *q_weight, const float *k_weight, float eps,
+                              const numrs_hip_rotary *rotary, float *q, int64_t ld_q, int64_t heads,
+                              const int32_t *table, int64_t max_pages, const int32_t *ends);
+
 /* One query row for each of n sequences over its lengths[i] cached tokens
  * (int32, device), heads grouped as above: out = softmax(q . k / sqrt(dh)) v.
  * A length is taken within 0..max_pages * page_size; tokens on pages that the
@@ -439,6 +492,19 @@ int numrs_hip_attention_paged(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cach
                               int64_t ld_q, int64_t heads, const int32_t *table,
                               int64_t max_pages, const int32_t *lengths, int64_t n, float *out,
                               int64_t ld_out);
+
+/* Attention of a packed batch's new tokens over the cache, where they are
+ * already (numrs_hip_kv_cache_append): token r of sequence i, at position p =
+ * ends[i] - length_i + r, attends to the cached tokens 0 .. p of its sequence.
+ * q and out are [total, heads * head_dim], rows ld_q and ld_out apart, heads
+ * grouped as above.  Tokens past what the table's pages can hold, and on pages
+ * that the cache does not have, are left out; a row without any token is zeros.
+ * With lengths of one it is numrs_hip_attention_paged, which is made for them.
+ * No backward, no atomics on values: the same call gives the same bits. */
+int numrs_hip_attention_paged_chunk(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cache,
+                                    const numrs_hip_seqs *seqs, const float *q, int64_t ld_q,
+                                    int64_t heads, const int32_t *table, int64_t max_pages,
+                                    const int32_t *ends, float *out, int64_t ld_out);
 
 /* How the two-layer LSTM calls run their recurrences (no reference op).
  * AUTO (the default): one persistent launch for all steps of the forward
@@ -869,6 +935,29 @@ int numrs_hip_tensor_attention_packed(numrs_hip_tensor *q, numrs_hip_tensor *k,
 int numrs_hip_tensor_attention_packed_qkv(numrs_hip_tensor *qkv, const numrs_hip_seqs *seqs,
                                           int64_t heads, int64_t kv_heads,
                                           numrs_hip_tensor **out);
+/* Query and key heads normed and rotated, as a node (numrs_hip_qk_rotary_*) over
+ * one projection x [total, (heads + 2 kv_heads) * dh] -> the same shape.  The
+ * weights are tensors [dh] or NULL (not normed); rotary NULL: not rotated. */
+int numrs_hip_tensor_qk_rotary(numrs_hip_tensor *x, const numrs_hip_seqs *seqs, int64_t heads,
+                               int64_t kv_heads, numrs_hip_tensor *q_weight,
+                               numrs_hip_tensor *k_weight, float eps,
+                               const numrs_hip_rotary *rotary, numrs_hip_tensor **out);
+/* numrs_hip_kv_cache_append of a projection x [total, (heads + 2 kv_heads) *
+ * head_dim]: the result is q [total, heads * head_dim].  It has no backward and
+ * is refused, the cache as it was, where one would be recorded. */
+int numrs_hip_tensor_kv_cache_append(numrs_hip_tensor *x, const numrs_hip_kv_cache *cache,
+                                     const numrs_hip_seqs *seqs, numrs_hip_tensor *q_weight,
+                                     numrs_hip_tensor *k_weight, float eps,
+                                     const numrs_hip_rotary *rotary, int64_t heads,
+                                     const int32_t *table, int64_t max_pages, const int32_t *ends,
+                                     numrs_hip_tensor **out);
+/* numrs_hip_attention_paged_chunk of the first heads * head_dim columns of x
+ * [total, columns], the result [total, heads * head_dim].  No backward, as
+ * below. */
+int numrs_hip_tensor_attention_paged_chunk(numrs_hip_tensor *x, const numrs_hip_kv_cache *cache,
+                                           const numrs_hip_seqs *seqs, int64_t heads,
+                                           const int32_t *table, int64_t max_pages,
+                                           const int32_t *ends, numrs_hip_tensor **out);
 /* numrs_hip_attention_paged as a tensor op: the queries are the first
  * heads * head_dim columns of x [n, columns] (a projection's other columns are
  * left alone), the result is [n, heads * head_dim].  It has no backward and is

@@ -106,6 +106,11 @@ SIGNATURES = {
                                            [_i64] * 3),
     "numrs_hip_attention_packed_backward": (_i, [_vp, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64] +
                                             [_vp] * 4 + [_i64] * 3 + [_i]),
+    "numrs_hip_qk_rotary_forward": (_i, [_vp] * 4 + [_i64, _vp, _vp, _f, _vp, _vp] + [_i64] * 4),
+    "numrs_hip_qk_rotary_backward": (_i, [_vp] * 4 + [_i64, _vp, _vp, _f, _vp, _vp, _i64, _vp, _i64, _vp, _vp] +
+                                     [_i64] * 3 + [_i]),
+    "numrs_hip_kv_cache_append": (_i, [_vp] * 4 + [_i64, _vp, _vp, _f, _vp, _vp, _i64, _i64, _vp, _i64, _vp]),
+    "numrs_hip_attention_paged_chunk": (_i, [_vp] * 4 + [_i64, _i64, _vp, _i64, _vp, _vp, _i64]),
     "numrs_hip_kv_cache_write": (_i, [_vp] * 5 + [_i64, _vp, _i64, _vp]),
     "numrs_hip_kv_cache_read": (_i, [_vp] * 5 + [_i64, _vp, _i64, _vp]),
     "numrs_hip_attention_paged": (_i, [_vp] * 3 + [_i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64]),
@@ -154,6 +159,10 @@ SIGNATURES = {
     "numrs_hip_tensor_attention_qkv": (_i, [_vp, _i64, _i64, _i64, ctypes.POINTER(_vp)]),
     "numrs_hip_tensor_attention_packed": (_i, [_vp] * 4 + [_i64, _i64, ctypes.POINTER(_vp)]),
     "numrs_hip_tensor_attention_packed_qkv": (_i, [_vp] * 2 + [_i64, _i64, ctypes.POINTER(_vp)]),
+    "numrs_hip_tensor_qk_rotary": (_i, [_vp] * 2 + [_i64, _i64, _vp, _vp, _f, _vp, ctypes.POINTER(_vp)]),
+    "numrs_hip_tensor_kv_cache_append": (_i, [_vp] * 3 + [_vp, _vp, _f, _vp, _i64, _vp, _i64, _vp,
+                                                          ctypes.POINTER(_vp)]),
+    "numrs_hip_tensor_attention_paged_chunk": (_i, [_vp] * 3 + [_i64, _vp, _i64, _vp, ctypes.POINTER(_vp)]),
     "numrs_hip_tensor_attention_paged": (_i, [_vp, _vp, _i64, _vp, _i64, _vp, ctypes.POINTER(_vp)]),
     "numrs_hip_optim_sgd": (_i, [_vp, ctypes.POINTER(_vp), _i, _f, _f, _f, ctypes.POINTER(_vp)]),
     "numrs_hip_optim_adam": (_i, [_vp, ctypes.POINTER(_vp), _i, _f, _f, _f, _f, _f,
@@ -197,6 +206,8 @@ RED_SUM, RED_MAX, RED_MIN, RED_MEAN, RED_ARGMAX, RED_VARIANCE = range(6)
 (OPT_ADAMW, OPT_RMSPROP, OPT_ADAGRAD, OPT_NADAM, OPT_RADAM, OPT_ADADELTA, OPT_ADABOUND, OPT_RPROP,
  OPT_LAMB) = range(9)
 KV_F32, KV_INT8 = 0, 1
+ROTARY_HALVES, ROTARY_PAIRS = 0, 1
+ACC_X, ACC_Q_WEIGHT, ACC_K_WEIGHT = 1, 2, 4
 SCHED_STEP, SCHED_EXPONENTIAL, SCHED_COSINE, SCHED_PLATEAU, SCHED_WARMUP = range(5)
 
 
@@ -206,6 +217,12 @@ class KVPages(ctypes.Structure):
 
     _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("pages", _i64),
                 ("page_size", _i64), ("kv_heads", _i64), ("head_dim", _i64), ("format", _i)]
+
+
+class RotarySpec(ctypes.Structure):
+    """numrs_hip_rotary: a rotation's frequencies (on the host), columns and layout."""
+
+    _fields_ = [("freqs", ctypes.POINTER(ctypes.c_double)), ("dims", _i64), ("layout", _i)]
 
 
 _lib = None

@@ -376,6 +376,52 @@ class Tensor:
         return self._out(L.load().numrs_hip_tensor_attention_packed_qkv(
             self._h, seqs.handle, heads, kv_heads, ctypes.byref(h)), h)
 
+    def _head_map(self, rotary, q_weight, k_weight):
+        """The C arguments of a head's norm and rotation."""
+        for w in (q_weight, k_weight):
+            if w is not None and w.ctx is not self.ctx:
+                raise ValueError("the projection and the norms' weights must belong to one context")
+        h = lambda w: w._h if w is not None else None  # noqa: E731
+        return h(q_weight), h(k_weight), ctypes.byref(rotary.spec) if rotary is not None else None
+
+    def qk_rotary(self, seqs, heads: int, kv_heads: int, rotary=None, q_weight: "Tensor | None" = None,
+                  k_weight: "Tensor | None" = None, eps: float = 1e-6) -> "Tensor":
+        """self = a packed batch's projection [tokens, (heads + 2 kv_heads)*dh] with
+        each query and key head x as x / sqrt(mean(x^2) + eps) * weight, where
+        there is a weight [dh], and rotated by its token's place in its sequence
+        (`Rotary`); the values as they are."""
+        wq, wk, rot = self._head_map(rotary, q_weight, k_weight)
+        h = ctypes.c_void_p()
+        return self._out(L.load().numrs_hip_tensor_qk_rotary(
+            self._h, seqs.handle, heads, kv_heads, wq, wk, eps, rot, ctypes.byref(h)), h)
+
+    def kv_cache_append(self, cache, seqs, heads: int, table, ends, rotary=None,
+                        q_weight: "Tensor | None" = None, k_weight: "Tensor | None" = None,
+                        eps: float = 1e-6) -> "Tensor":
+        """The same of new tokens on the way into a `KVCache`, at positions ends[i] -
+        length .. ends[i] - 1: keys and values are written, the queries returned as
+        [tokens, heads*dh].  No backward."""
+        if cache.ctx is not self.ctx or seqs.ctx is not self.ctx:
+            raise ValueError("the projection, the sequences and the cache must belong to one context")
+        wq, wk, rot = self._head_map(rotary, q_weight, k_weight)
+        most = cache.table_width(table, ends, len(seqs))
+        h = ctypes.c_void_p()
+        return self._out(L.load().numrs_hip_tensor_kv_cache_append(
+            self._h, ctypes.byref(cache.pages), seqs.handle, wq, wk, eps, rot, heads, table.ptr, most,
+            ends.ptr, ctypes.byref(h)), h)
+
+    def attention_paged_chunk(self, cache, seqs, heads: int, table, ends) -> "Tensor":
+        """Attention of a packed batch's new tokens, which are in the `KVCache`
+        already, each over its sequence's tokens up to itself; the queries are self's
+        first heads * head_dim columns.  No backward."""
+        if cache.ctx is not self.ctx or seqs.ctx is not self.ctx:
+            raise ValueError("the queries, the sequences and the cache must belong to one context")
+        most = cache.table_width(table, ends, len(seqs))
+        h = ctypes.c_void_p()
+        return self._out(L.load().numrs_hip_tensor_attention_paged_chunk(
+            self._h, ctypes.byref(cache.pages), seqs.handle, heads, table.ptr, most, ends.ptr,
+            ctypes.byref(h)), h)
+
     def attention_paged(self, cache, heads: int, table, lengths) -> "Tensor":
         """One query row for each sequence over its tokens in a `KVCache`: the
         queries are self's first heads * head_dim columns.  table [n, max_pages]

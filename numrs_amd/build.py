@@ -25,7 +25,8 @@ OBJ = os.path.join(PKG, "lib", "obj")
 LIB = os.path.join(PKG, "lib", "libnumrs_hip.so")
 
 SOURCES = ["runtime.hip", "gemm.hip", "eltwise.hip", "reduce.hip", "rowwise.hip", "fwd.hip",
-           "attention.hip", "packed.hip", "kvcache.hip", "lstm.hip", "optim.hip", "dispatch.hip", "autograd.hip"]
+           "attention.hip", "packed.hip", "rotary.hip", "kvcache.hip", "chunk.hip",
+           "lstm.hip", "optim.hip", "dispatch.hip", "autograd.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 CFLAGS = [

@@ -40,7 +40,7 @@ thread_local bool g_grad_enabled = true;  // mod.rs:194-206
 enum class Op {
   Leaf, Add, Sub, Mul, Div, MatMul, Transpose, Unary, Sum, Mean, MSE, CrossEntropy,
   CrossEntropyLabels, Reshape, Softmax, LayerNorm, Attention, Linear, LSTM, TimeSlice, SumAxis,
-  SoftmaxAxis, LSTM2, AttentionPacked
+  SoftmaxAxis, LSTM2, AttentionPacked, QKRotary
 };
 
 struct Storage {
@@ -58,6 +58,12 @@ struct GradCell {
   // loss's forward kernel together with the root gradient it pre-formed;
   // cleared by every other write to the cell.
   bool seed_preset = false;
+};
+
+// A rotation's description with frequencies of its own, for the tape.
+struct Rotary {
+  std::vector<double> freqs;
+  numrs_hip_rotary spec{};
 };
 
 struct Node;
@@ -86,6 +92,7 @@ struct Node {
   std::vector<T> inputs;
   std::vector<Buf> saved;  // LayerNorm mean/rstd, int32 labels
   std::shared_ptr<const numrs_hip::Seqs> seqs;  // a packed batch's sequences
+  std::shared_ptr<const Rotary> rotary;         // null: no rotation
 };
 
 uint64_t next_node_id() {  // NodeId::new, mod.rs:46-51
@@ -590,6 +597,29 @@ int bw_attention_seqs(const T &out, const float *g, Node &n) {
   return NUMRS_HIP_OK;
 }
 
+// Heads normed and rotated; inputs: the projection, then the weights that there are (kind: 1 the
+// queries', 2 the keys').
+int bw_qk_rotary(const T &out, const float *g, Node &n) {
+  const T &x = n.inputs[0];
+  const int64_t H = n.dims[0], Hk = n.dims[1], dh = n.dims[2], ld = (H + 2 * Hk) * dh;
+  size_t next = 1;
+  const T *wq = n.kind & 1 ? &n.inputs[next++] : nullptr, *wk = n.kind & 2 ? &n.inputs[next++] : nullptr;
+  float *dx = nullptr, *dq = nullptr, *dk = nullptr;
+  int ax = 0, aq = 0, ak = 0;
+  if (x->requires_grad)
+    if (int rc = grad_target(x, &dx, &ax)) return rc;
+  if (wq != nullptr && (*wq)->requires_grad)
+    if (int rc = grad_target(*wq, &dq, &aq)) return rc;
+  if (wk != nullptr && (*wk)->requires_grad)  // of one tensor for both: added to the queries' part
+    if (int rc = grad_target(*wk, &dk, &ak)) return rc;
+  const numrs_hip_seqs seqs{n.seqs};
+  return numrs_hip_qk_rotary_backward(
+      out->ctx, &seqs, nullptr, x->data->ptr, ld, wq != nullptr ? (*wq)->data->ptr : nullptr,
+      wk != nullptr ? (*wk)->data->ptr : nullptr, n.param, n.rotary ? &n.rotary->spec : nullptr, g, ld, dx, ld, dq,
+      dk, H, Hk, dh,
+      (ax ? NUMRS_HIP_ACC_X : 0) | (aq ? NUMRS_HIP_ACC_Q_WEIGHT : 0) | (ak ? NUMRS_HIP_ACC_K_WEIGHT : 0));
+}
+
 int bw_linear(const T &out, const float *g, Node &n) {
   const T &x = n.inputs[0], &W = n.inputs[1];
   const bool relu = (n.kind & 1) != 0, has_res = (n.kind & 2) != 0, gelu = (n.kind & 4) != 0;
@@ -740,6 +770,7 @@ int run_backward_fn(const T &out) {
     case Op::LayerNorm: return bw_layernorm(out, g, n);
     case Op::Attention: return bw_attention(out, g, n);
     case Op::AttentionPacked: return bw_attention_seqs(out, g, n);
+    case Op::QKRotary: return bw_qk_rotary(out, g, n);
     case Op::Linear: return bw_linear(out, g, n);
     case Op::LSTM: return bw_lstm(out, g, n);
     case Op::LSTM2: return bw_lstm2(out, g, n);
@@ -1334,6 +1365,56 @@ int op_attention_seqs(const T &q, const T *k, const T *v, const numrs_hip_seqs *
       attach(r, Op::AttentionPacked, {q}, 0, 0.f, {st});
     r->node->dims[0] = H, r->node->dims[1] = Hk, r->node->dims[2] = dh;
     r->node->seqs = s;
+  }
+  *out = std::move(r);
+  return NUMRS_HIP_OK;
+}
+
+// A head's weight: null, or a tensor [dh] of this context.
+int check_weight(numrs_hip_ctx *ctx, const T *w, int64_t dh, const char *what) {
+  if (w == nullptr) return NUMRS_HIP_OK;
+  if ((*w)->ctx != ctx) return fail(ctx, NUMRS_HIP_E_INVALID, "%s: operands of different contexts", what);
+  if ((*w)->shape != std::vector<int64_t>{dh})
+    return fail(ctx, NUMRS_HIP_E_SHAPE, "%s: a norm's weight must be [head size]", what);
+  return NUMRS_HIP_OK;
+}
+
+// The query and key heads of a packed projection, normed and rotated.
+int op_qk_rotary(const T &x, const numrs_hip_seqs *seqs, int64_t H, int64_t Hk, const T *wq, const T *wk,
+                 float eps, const numrs_hip_rotary *rot, T *out) {
+  numrs_hip_ctx *ctx = x->ctx;
+  const auto &s = seqs->s;
+  if (s->ctx != ctx) return fail(ctx, NUMRS_HIP_E_INVALID, "qk_rotary: operands of different contexts");
+  numrs_hip::DeviceScope dev(ctx);
+  if (x->shape.size() != 2 || x->shape[0] != s->total)
+    return fail(ctx, NUMRS_HIP_E_SHAPE, "qk_rotary: the projection must have a row for each token");
+  if (H <= 0 || Hk <= 0 || H > 65535 || Hk > 65535 || x->shape[1] % (H + 2 * Hk) != 0)
+    return fail(ctx, NUMRS_HIP_E_SHAPE, "qk_rotary: the columns do not divide into the heads");
+  const int64_t dh = x->shape[1] / (H + 2 * Hk), ld = x->shape[1];
+  for (const T *w : {wq, wk})
+    if (int rc = check_weight(ctx, w, dh, "qk_rotary")) return rc;
+  const bool rec = g_grad_enabled && (x->requires_grad || (wq != nullptr && (*wq)->requires_grad) ||
+                                      (wk != nullptr && (*wk)->requires_grad));
+  T r;
+  if (int rc = make_tensor(ctx, x->shape, rec, &r)) return rc;
+  if (int rc = numrs_hip_qk_rotary_forward(ctx, seqs, nullptr, x->data->ptr, ld,
+                                           wq != nullptr ? (*wq)->data->ptr : nullptr,
+                                           wk != nullptr ? (*wk)->data->ptr : nullptr, eps, rot, r->data->ptr, ld, H,
+                                           Hk, dh))
+    return rc;
+  if (rec) {
+    std::vector<T> in{x};
+    for (const T *w : {wq, wk})
+      if (w != nullptr) in.push_back(*w);
+    attach(r, Op::QKRotary, std::move(in), (wq != nullptr ? 1 : 0) | (wk != nullptr ? 2 : 0), eps);
+    r->node->dims[0] = H, r->node->dims[1] = Hk, r->node->dims[2] = dh;
+    r->node->seqs = s;
+    if (rot != nullptr && rot->dims > 0) {
+      auto own = std::make_shared<Rotary>();
+      own->freqs.assign(rot->freqs, rot->freqs + rot->dims / 2);
+      own->spec = {own->freqs.data(), rot->dims, rot->layout};
+      r->node->rotary = std::move(own);
+    }
   }
   *out = std::move(r);
   return NUMRS_HIP_OK;
@@ -1947,6 +2028,83 @@ int numrs_hip_tensor_attention_paged(numrs_hip_tensor *x, const numrs_hip_kv_cac
                                          heads * cache->head_dim))
     return rc;
   return wrap(std::move(r), out);
+}
+
+int numrs_hip_tensor_qk_rotary(numrs_hip_tensor *x, const numrs_hip_seqs *seqs, int64_t heads,
+                               int64_t kv_heads, numrs_hip_tensor *q_weight,
+                               numrs_hip_tensor *k_weight, float eps,
+                               const numrs_hip_rotary *rotary, numrs_hip_tensor **out) {
+  if (x == nullptr || seqs == nullptr || out == nullptr) return NUMRS_HIP_E_INVALID;
+  try {
+    T r;
+    if (int rc = op_qk_rotary(x->t, seqs, heads, kv_heads, q_weight != nullptr ? &q_weight->t : nullptr,
+                              k_weight != nullptr ? &k_weight->t : nullptr, eps, rotary, &r))
+      return rc;
+    return wrap(std::move(r), out);
+  } catch (const std::bad_alloc &) {
+    return fail(x->t->ctx, NUMRS_HIP_E_NOMEM, "qk_rotary: out of host memory");
+  }
+}
+
+int numrs_hip_tensor_kv_cache_append(numrs_hip_tensor *x, const numrs_hip_kv_cache *cache,
+                                     const numrs_hip_seqs *seqs, numrs_hip_tensor *q_weight,
+                                     numrs_hip_tensor *k_weight, float eps,
+                                     const numrs_hip_rotary *rotary, int64_t heads,
+                                     const int32_t *table, int64_t max_pages, const int32_t *ends,
+                                     numrs_hip_tensor **out) {
+  if (x == nullptr || cache == nullptr || seqs == nullptr || out == nullptr) return NUMRS_HIP_E_INVALID;
+  const T &t = x->t;
+  numrs_hip_ctx *ctx = t->ctx;
+  // (a weight that wants a gradient counts: its result would have none)
+  if (g_grad_enabled && (t->requires_grad || (q_weight != nullptr && q_weight->t->requires_grad) ||
+                         (k_weight != nullptr && k_weight->t->requires_grad)))
+    return fail(ctx, NUMRS_HIP_E_INVALID, "kv_cache_append has no backward: call it under no_grad()");
+  numrs_hip::DeviceScope dev(ctx);
+  const int64_t hk = cache->kv_heads, dh = cache->head_dim;
+  if (t->shape.size() != 2 || t->shape[0] != seqs->s->total || heads < 1 || heads > 65535 || hk < 1 || hk > 65535 ||
+      dh < 1 || dh > 128 || t->shape[1] != (heads + 2 * hk) * dh)
+    return fail(ctx, NUMRS_HIP_E_SHAPE,
+                "kv_cache_append: x must be [tokens, (heads + 2 kv_heads) * head_dim] of the cache");
+  for (numrs_hip_tensor *w : {q_weight, k_weight})
+    if (int rc = check_weight(ctx, w != nullptr ? &w->t : nullptr, dh, "kv_cache_append")) return rc;
+  try {
+    T r;
+    if (int rc = make_tensor(ctx, {t->shape[0], heads * dh}, false, &r)) return rc;
+    if (int rc = numrs_hip_kv_cache_append(ctx, cache, seqs, t->data->ptr, t->shape[1],
+                                           q_weight != nullptr ? q_weight->t->data->ptr : nullptr,
+                                           k_weight != nullptr ? k_weight->t->data->ptr : nullptr, eps, rotary,
+                                           r->data->ptr, heads * dh, heads, table, max_pages, ends))
+      return rc;
+    return wrap(std::move(r), out);
+  } catch (const std::bad_alloc &) {
+    return fail(ctx, NUMRS_HIP_E_NOMEM, "kv_cache_append: out of host memory");
+  }
+}
+
+int numrs_hip_tensor_attention_paged_chunk(numrs_hip_tensor *x, const numrs_hip_kv_cache *cache,
+                                           const numrs_hip_seqs *seqs, int64_t heads,
+                                           const int32_t *table, int64_t max_pages,
+                                           const int32_t *ends, numrs_hip_tensor **out) {
+  if (x == nullptr || cache == nullptr || seqs == nullptr || out == nullptr) return NUMRS_HIP_E_INVALID;
+  const T &t = x->t;
+  numrs_hip_ctx *ctx = t->ctx;
+  if (recording({&t}))
+    return fail(ctx, NUMRS_HIP_E_INVALID, "attention_paged_chunk has no backward: detach its input");
+  numrs_hip::DeviceScope dev(ctx);
+  if (t->shape.size() != 2 || t->shape[0] != seqs->s->total || heads < 1 || heads > 65535 || cache->head_dim < 1 ||
+      cache->head_dim > 128 || t->shape[1] < heads * cache->head_dim)
+    return fail(ctx, NUMRS_HIP_E_SHAPE,
+                "attention_paged_chunk: x must be [tokens, at least heads * head_dim]");
+  try {
+    T r;
+    if (int rc = make_tensor(ctx, {t->shape[0], heads * cache->head_dim}, false, &r)) return rc;
+    if (int rc = numrs_hip_attention_paged_chunk(ctx, cache, seqs, t->data->ptr, t->shape[1], heads, table,
+                                                 max_pages, ends, r->data->ptr, heads * cache->head_dim))
+      return rc;
+    return wrap(std::move(r), out);
+  } catch (const std::bad_alloc &) {
+    return fail(ctx, NUMRS_HIP_E_NOMEM, "attention_paged_chunk: out of host memory");
+  }
 }
 
 int numrs_hip_optim_sgd(numrs_hip_ctx *ctx, numrs_hip_tensor **params, int n, float lr,

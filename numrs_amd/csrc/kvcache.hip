@@ -5,6 +5,7 @@
 
 #include "packed.h"
 #include "paged_split.h"
+#include "rotary.h"
 
 namespace {
 
@@ -31,6 +32,7 @@ typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
 
 struct Group {
+  int64_t pos;   // its first position
   int64_t base;  // element offset of its first slot in its page and head
   int page;      // -1: the cache has no place for it
   int row[4];    // the packed rows within the sequence, -1 for a position that is none of the tile's
@@ -50,6 +52,7 @@ __device__ __forceinline__ void for_groups(const Cache &c, const SeqTile &t, int
   const int64_t q0 = p0 >> 2, q1 = (p0 + rows - 1) >> 2;
   for (int64_t q = q0 + (threadIdx.x >> lanes); q <= q1; q += 256 >> lanes) {
     Group x;
+    x.pos = 4 * q;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int64_t row = 4 * q + r - start;
@@ -137,6 +140,30 @@ __device__ __forceinline__ u4 transposed(u4 x) {
             __builtin_amdgcn_perm(d, b, 0x05040100u), __builtin_amdgcn_perm(d, b, 0x07060302u)};
 }
 
+// A group's scales, and its codes of four columns: keys' at pk, a row dh apart, values' 16 bytes at pv.  Slots
+// that are not the batch's are left alone; `whole`: all four are.
+__device__ __forceinline__ void put_scales(const Cache &c, const Group &x, bool whole, f4 ks, f4 vs) {
+  if (whole) {
+    *reinterpret_cast<f4 *>(c.ks + x.base) = ks, *reinterpret_cast<f4 *>(c.vs + x.base) = vs;
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (x.row[r] >= 0) c.ks[x.base + r] = ks[r], c.vs[x.base + r] = vs[r];
+  }
+}
+__device__ __forceinline__ void put_codes(const Group &x, bool whole, uint8_t *pk, uint8_t *pv, int dh, u4 kc, u4 vc) {
+  if (whole) *reinterpret_cast<u4 *>(pv) = transposed(vc);
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    if (x.row[r] < 0) continue;
+    *reinterpret_cast<unsigned *>(pk + r * dh) = kc[r];
+    if (!whole) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) pv[4 * j + r] = (uint8_t)(vc[r] >> (8 * j));
+    }
+  }
+}
+
 // PAST: the rows go past the caches (see rows_past).
 template <bool INT8, bool PAST>
 __global__ void __launch_bounds__(256) write_rows(RowArgs a, int lanes) {
@@ -175,27 +202,10 @@ __global__ void __launch_bounds__(256) write_rows(RowArgs a, int lanes) {
       }
       if (x.page < 0) return;
       const bool whole = (x.row[0] | x.row[1] | x.row[2] | x.row[3]) >= 0;
-      if (d == 0) {
-        if (whole) {
-          *reinterpret_cast<f4 *>(a.c.ks + x.base) = ks, *reinterpret_cast<f4 *>(a.c.vs + x.base) = vs;
-        } else {
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (x.row[r] >= 0) a.c.ks[x.base + r] = ks[r], a.c.vs[x.base + r] = vs[r];
-        }
-      }
+      if (d == 0) put_scales(a.c, x, whole, ks, vs);
       if (!in) return;
       uint8_t *pk = static_cast<uint8_t *>(a.c.k) + x.base * dh + d, *pv = static_cast<uint8_t *>(a.c.v) + x.base * dh + 4 * d;
-      if (whole) *reinterpret_cast<u4 *>(pv) = transposed(vc);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if (x.row[r] < 0) continue;
-        *reinterpret_cast<unsigned *>(pk + r * dh) = kc[r];
-        if (!whole) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) pv[4 * j + r] = (uint8_t)(vc[r] >> (8 * j));
-        }
-      }
+      put_codes(x, whole, pk, pv, dh, kc, vc);
     }
   });
 }
@@ -246,6 +256,90 @@ __global__ void __launch_bounds__(256) read_rows(RowArgs a, int lanes) {
 
 // Neighbours that share a row, four columns each: the power of two that covers a head.
 int row_lanes(int dh) { return paging::log2_of((dh + 3) / 4); }
+
+struct AppendArgs {
+  RowArgs c;            // where the keys and values go; k and v are not used
+  rotary::RowArgs row;  // the projection, and the queries' rows
+  unsigned keys;        // workgroups of keys and values, before those of queries
+  int parts;            // of a tile, for the queries
+};
+
+// Keys, normed and rotated, and values on their way into the cache: a workgroup a tile and kv head, a thread four
+// positions and eight columns.  After them a workgroup a tile's part and some of the query heads.
+template <bool INT8, bool PAST>
+__global__ void __launch_bounds__(256) append_rows(AppendArgs b) {
+  if (blockIdx.x >= b.keys) {
+    const unsigned n = b.row.slots > 0 ? (b.row.slots + b.row.per - 1) / b.row.per : 1, i = blockIdx.x - b.keys;
+    const int h0 = i % n * b.row.per;
+    rotary::rotate_part(b.row, b.row.tiles[i / n / b.parts], i / n % b.parts, h0, min(h0 + b.row.per, b.row.slots));
+    return;
+  }
+  const RowArgs &a = b.c;
+  const rotary::RowArgs &ra = b.row;
+  const SeqTile t = a.tiles[blockIdx.x / a.c.kv_heads];
+  const int g = blockIdx.x % a.c.kv_heads, dh = a.c.dh;
+  const bool nb = ra.turn.pairs;
+  for_groups(a.c, t, g, a.ends, ra.lanes, [&](const Group &x, int four_i) {
+    const int i = four_i / 4;
+    const rotary::Item it = rotary::item_of(i, dh, ra.turn);
+    f4 k0[4], k1[4], v0[4], v1[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      k0[r] = k1[r] = v0[r] = v1[r] = f4{};
+      if (!it.in || x.row[r] < 0) continue;
+      const char *k = reinterpret_cast<const char *>(ra.x + (int64_t)(t.row0 + x.row[r]) * ra.ld_x + (int64_t)(ra.heads + g) * dh);
+      const char *v = k + (int64_t)a.c.kv_heads * dh * 4;
+      k0[r] = paged::load<f4u, PAST>(k + 4 * it.d0), k1[r] = paged::load<f4u, PAST>(k + 4 * it.d1);
+      v0[r] = paged::load<f4u, PAST>(v + 32 * i), v1[r] = paged::load<f4u, PAST>(v + 32 * i + 16);
+    }
+    rotary::Weight w;
+    w.load(ra.wk, it, nb);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      double y[8];
+      rotary::pairs_of(k0[r], k1[r], nb, y);
+      if (ra.wk != nullptr) {
+        const double s = rotary::inverse_rms(y, ra.lanes, ra.inv_dh, ra.eps);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = y[j] * s * w.w[j];
+      }
+      if (x.row[r] >= 0) rotary::turn<false>(y, rotary::units_of(ra.turn, i, it, x.pos + r), it.turned);
+      rotary::columns_of(y, nb, k0[r], k1[r]);
+    }
+    if constexpr (!INT8) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (!it.in || x.row[r] < 0 || x.page < 0) continue;
+        float *k = static_cast<float *>(a.c.k) + (x.base + r) * dh, *v = static_cast<float *>(a.c.v) + (x.base + r) * dh;
+        *reinterpret_cast<f4 *>(k + it.d0) = k0[r], *reinterpret_cast<f4 *>(k + it.d1) = k1[r];
+        *reinterpret_cast<f4 *>(v + 8 * i) = v0[r], *reinterpret_cast<f4 *>(v + 8 * i + 4) = v1[r];
+      }
+    } else {
+      u4 kc0, kc1, vc0, vc1;
+      f4 ks, vs;
+      unsigned top[8];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        // (a lane past the head has zeros, or NaN where the norm of zeros is)
+        top[r] = it.in ? max(top_of(k0[r]), top_of(k1[r])) : 0, top[4 + r] = max(top_of(v0[r]), top_of(v1[r]));
+      }
+      max_of(top, ra.lanes);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        ks[r] = scale_of(top[r]), vs[r] = scale_of(top[4 + r]);
+        kc0[r] = codes_of(k0[r], ks[r]), kc1[r] = codes_of(k1[r], ks[r]);
+        vc0[r] = codes_of(v0[r], vs[r]), vc1[r] = codes_of(v1[r], vs[r]);
+      }
+      if (x.page < 0) return;
+      const bool whole = (x.row[0] | x.row[1] | x.row[2] | x.row[3]) >= 0;
+      if (i == 0) put_scales(a.c, x, whole, ks, vs);
+      if (!it.in) return;
+      uint8_t *pk = static_cast<uint8_t *>(a.c.k) + x.base * dh, *pv = static_cast<uint8_t *>(a.c.v) + x.base * dh + 32 * i;
+      put_codes(x, whole, pk + it.d0, pv, dh, kc0, vc0);
+      put_codes(x, whole, pk + it.d1, pv + 16, dh, kc1, vc1);
+    }
+  });
+}
 
 // Whether a batch's rows go past the caches: where keys and values are more than half of the last cache's 256 MB,
 // so that they would take the place of what the next kernel reads.  On MI355X, through them against past, us:
@@ -342,6 +436,43 @@ int numrs_hip_kv_cache_read(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cache,
         <<<grid, 256, 0, ctx->stream>>>(a, row_lanes((int)cache->head_dim));
   });
   return check_launch(ctx, "read_rows");
+}
+
+int numrs_hip_kv_cache_append(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cache,
+                              const numrs_hip_seqs *seqs, const float *qkv, int64_t ld,
+                              const float *q_weight, const float *k_weight, float eps,
+                              const numrs_hip_rotary *rotary, float *q, int64_t ld_q, int64_t heads,
+                              const int32_t *table, int64_t max_pages, const int32_t *ends) {
+  NRS_CHECK_CTX(ctx);
+  const char *what = "kv_cache_append";
+  if (int rc = check_rows(ctx, cache, seqs, qkv, qkv, ld, table, max_pages, ends, what)) return rc;
+  const int64_t hk = cache->kv_heads, dh = cache->head_dim;
+  if (const char *why = paging::refuse_heads(heads, hk, dh)) return fail(ctx, NUMRS_HIP_E_SHAPE, "%s: %s", what, why);
+  if (paging::bad_stride(ld, (heads + 2 * hk) * dh) || (q != nullptr && paging::bad_stride(ld_q, heads * dh)))
+    return fail(ctx, NUMRS_HIP_E_SHAPE, "%s: a row stride is below its row's width or above 2^31 - 1", what);
+  int code = 0;
+  if (const char *why = rotary::refuse_rotary(rotary, dh, &code)) return fail(ctx, code, "%s: %s", what, why);
+  if (const char *why = rotary::refuse_eps(eps)) return fail(ctx, NUMRS_HIP_E_INVALID, "%s: %s", what, why);
+  const Seqs &s = *seqs->s;
+  const int lanes = rotary::lanes_of(dh), parts = rotary::parts_of(lanes);
+  if (paging::bad_grid(s.tiles * (hk + 2 * parts)))
+    return fail(ctx, NUMRS_HIP_E_SHAPE, "%s: too many tokens times heads", what);
+  if (s.total == 0) return NUMRS_HIP_OK;
+  if (int rc = s.keep()) return rc;
+  DeviceScope dev(ctx);
+  AppendArgs b{{device_cache(*cache, table, max_pages), s.in_order, ends, nullptr, nullptr, nullptr, nullptr, ld},
+               {s.in_order, ends, qkv, q_weight, k_weight, q, ld, ld_q, (int)heads, (int)hk, q != nullptr ? (int)heads : 0,
+                1, (int)dh, lanes, eps, 1.0 / (double)dh, rotary::turn_of(rotary)},
+               (unsigned)(s.tiles * hk), parts};
+  unsigned grid = b.keys;
+  if (q != nullptr) {
+    b.row.per = rotary::heads_each(ctx, s.tiles * parts, b.row.slots);
+    grid += (unsigned)(s.tiles * parts) * ((b.row.slots + b.row.per - 1) / b.row.per);
+  }
+  with_kind(cache->format == NUMRS_HIP_KV_INT8, rows_past(s, *cache), [&](auto int8, auto past) {
+    append_rows<decltype(int8)::value, decltype(past)::value><<<grid, 256, 0, ctx->stream>>>(b);
+  });
+  return check_launch(ctx, "append_rows");
 }
 
 int numrs_hip_attention_paged(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cache, const float *q,

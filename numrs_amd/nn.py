@@ -230,12 +230,16 @@ class CausalSelfAttention(Module):
         y = attn.forward_packed(x, seqs)                       # training, with backward
         with no_grad():
             y = attn.prefill(x, seqs, cache, table, lengths)   # prompts, kept in the cache
+            y = attn.extend(x, seqs, cache, table, lengths)    # a prompt's next piece
             y = attn.decode(x1, ones, cache, table, lengths)   # one token for each sequence
 
     `lengths` (int32, device) counts a sequence's cached tokens, the new ones
-    included; `ones` is PackedSequences([1] * n)."""
+    included; `ones` is PackedSequences([1] * n).  With `rotary` (`Rotary`) query
+    and key heads are rotated by position, and with q_norm and k_norm (weights
+    [dh], trained with the others) normed before that."""
 
-    def __init__(self, wq, wk, wv, wo, heads: int, kv_heads: int, ctx=None):
+    def __init__(self, wq, wk, wv, wo, heads: int, kv_heads: int, ctx=None, rotary=None,
+                 q_norm=None, k_norm=None, norm_eps: float = 1e-6):
         wq, wk, wv, wo = (np.asarray(a, np.float32) for a in (wq, wk, wv, wo))
         if heads % kv_heads or wq.shape[0] % heads or wk.shape != wv.shape:
             raise ValueError("CausalSelfAttention: the weights do not divide into the heads")
@@ -247,6 +251,33 @@ class CausalSelfAttention(Module):
                                        ctx)
         self.o = Linear.with_weights(wo.shape[1], wo.shape[0], wo, np.zeros(wo.shape[0], np.float32),
                                      ctx)
+        if rotary is not None and rotary.head_dim != self.head_dim:
+            raise ValueError("CausalSelfAttention: the rotation is for heads of another size")
+        for w in (q_norm, k_norm):
+            if w is not None and np.asarray(w).size != self.head_dim:
+                raise ValueError("CausalSelfAttention: a norm's weight must be [head size]")
+        self.rotary, self.norm_eps = rotary, norm_eps
+        self.q_norm, self.k_norm = (
+            None if w is None else Tensor.new(np.asarray(w, np.float32).ravel(), True, ctx=self.qkv.weight.ctx)
+            for w in (q_norm, k_norm))
+
+    @property
+    def _maps_heads(self) -> bool:
+        return any(x is not None for x in (self.rotary, self.q_norm, self.k_norm))
+
+    def _heads(self, qkv: Tensor, seqs) -> Tensor:
+        if not self._maps_heads:
+            return qkv
+        return qkv.qk_rotary(seqs, self.heads, self.kv_heads, self.rotary, self.q_norm, self.k_norm,
+                             self.norm_eps)
+
+    def _into_cache(self, qkv: Tensor, seqs, cache, table, lengths) -> Tensor:
+        """New tokens' keys and values into the cache; their queries."""
+        if self._maps_heads:
+            return qkv.kv_cache_append(cache, seqs, self.heads, table, lengths, self.rotary, self.q_norm,
+                                       self.k_norm, self.norm_eps)
+        cache.write_qkv(seqs, qkv, self.heads, table, lengths)
+        return qkv
 
     def _project(self, a: Tensor, residual: Tensor | None) -> Tensor:
         if residual is None:
@@ -256,14 +287,14 @@ class CausalSelfAttention(Module):
         return residual.add(self.o(a))
 
     def forward_packed(self, x: Tensor, seqs, residual: Tensor | None = None) -> Tensor:
-        a = self.qkv(x).attention_packed_qkv(seqs, self.heads, self.kv_heads)
+        a = self._heads(self.qkv(x), seqs).attention_packed_qkv(seqs, self.heads, self.kv_heads)
         return self._project(a, residual)
 
     def prefill(self, x: Tensor, seqs, cache, table, lengths, residual: Tensor | None = None
                 ) -> Tensor:
         """forward_packed of whole prompts, whose keys and values also go into the
         cache; `lengths` are the prompts' lengths."""
-        qkv = self.qkv(x)
+        qkv = self._heads(self.qkv(x), seqs)
         cache.write_qkv(seqs, qkv, self.heads, table, lengths)
         a = qkv.attention_packed_qkv(seqs, self.heads, self.kv_heads)
         return self._project(a, residual)
@@ -276,11 +307,24 @@ class CausalSelfAttention(Module):
         qkv = self.qkv(x)
         if qkv.requires_grad:
             raise HipError(L.E_INVALID, "decode has no backward: call it under no_grad()")
-        cache.write_qkv(ones, qkv, self.heads, table, lengths)
-        return self._project(qkv.attention_paged(cache, self.heads, table, lengths), residual)
+        q = self._into_cache(qkv, ones, cache, table, lengths)
+        return self._project(q.attention_paged(cache, self.heads, table, lengths), residual)
+
+    def extend(self, x: Tensor, seqs, cache, table, lengths, residual: Tensor | None = None
+               ) -> Tensor:
+        """Any number of new tokens for each sequence, of prompts that go into the
+        cache in pieces or beside single tokens: their keys and values go into the
+        cache, and each attends to its sequence up to itself.  No backward, as
+        `decode`."""
+        qkv = self.qkv(x)
+        if qkv.requires_grad:
+            raise HipError(L.E_INVALID, "extend has no backward: call it under no_grad()")
+        q = self._into_cache(qkv, seqs, cache, table, lengths)
+        return self._project(q.attention_paged_chunk(cache, seqs, self.heads, table, lengths), residual)
 
     def parameters(self) -> list[Tensor]:
-        return self.qkv.parameters() + self.o.parameters()
+        norms = [w for w in (self.q_norm, self.k_norm) if w is not None]
+        return self.qkv.parameters() + norms + self.o.parameters()
 
 
 class TransformerEncoderBlock(Module):

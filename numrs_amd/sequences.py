@@ -8,6 +8,11 @@ attention-free ops take one shape).
     cache.write_qkv(seqs, qkv, heads, table, lengths)           # a prompt's keys and values
     cache.write_qkv(ones, qkv1, heads, table, lengths)          # one more token each
     out = qkv1.attention_paged(cache, heads, table, lengths)    # its attention
+    out = qkv.attention_paged_chunk(cache, seqs, heads, table, lengths)  # of a prompt's next piece
+
+    rotary = Rotary(head_dim, base=10000.0)          # positions
+    qkv = qkv.qk_rotary(seqs, heads, kv_heads, rotary)          # with backward
+    q = qkv.kv_cache_append(cache, seqs, heads, table, lengths, rotary)  # on the way into the cache
 
 `table` [n, max_pages] and `lengths` [n] are int32 device arrays that the
 program keeps and advances: which pages of the cache each sequence owns, and
@@ -25,6 +30,32 @@ from .autograd import Tensor, default_context
 from .device import Context, DeviceArray
 
 FORMATS = {"f32": L.KV_F32, "int8": L.KV_INT8}
+LAYOUTS = {"halves": L.ROTARY_HALVES, "pairs": L.ROTARY_PAIRS}
+
+
+class Rotary:
+    """A rotation of query and key heads by position (numrs_hip_rotary): the first
+    `dims` columns of a head (all of them by default), angle i of dims / 2 being
+    position * base^(-2 i / dims) or position * freqs[i].  layout "halves" turns
+    columns i and dims / 2 + i together, "pairs" 2 i and 2 i + 1."""
+
+    def __init__(self, head_dim: int, dims: int | None = None, base: float = 10000.0,
+                 layout: str = "halves", freqs=None):
+        if layout not in LAYOUTS:
+            raise ValueError(f"layout must be one of {sorted(LAYOUTS)}")
+        dims = int(head_dim if dims is None else dims)
+        if dims < 8 or dims % 8 or dims > head_dim:
+            raise ValueError(f"dims must be a multiple of 8 in 8..{head_dim}, not {dims}")
+        if freqs is None:
+            if not base > 0:
+                raise ValueError("the base must be positive")
+            freqs = float(base) ** (-2.0 * np.arange(dims // 2) / dims)
+        self.freqs = np.array(freqs, np.float64).ravel()
+        if self.freqs.size != dims // 2:
+            raise ValueError(f"{dims // 2} frequencies are needed, not {self.freqs.size}")
+        self.head_dim, self.dims, self.layout = int(head_dim), dims, layout
+        at = self.freqs.ctypes.data_as(ctypes.POINTER(ctypes.c_double))
+        self.spec = L.RotarySpec(at, dims, LAYOUTS[layout])
 
 
 class PackedSequences:
@@ -139,6 +170,13 @@ class KVCache:
         self._call(L.load().numrs_hip_kv_cache_write, seqs, p + 4 * wq, p + 4 * (wq + self.width),
                    shape[1], table, ends)
 
+    def append(self, seqs: PackedSequences, qkv: Tensor, heads: int, table: DeviceArray,
+               ends: DeviceArray, rotary: Rotary | None = None, q_weight: Tensor | None = None,
+               k_weight: Tensor | None = None, eps: float = 1e-6) -> Tensor:
+        """`Tensor.kv_cache_append` of a projection: its keys, normed and rotated, and
+        its values into the cache; its queries, normed and rotated, as the result."""
+        return qkv.kv_cache_append(self, seqs, heads, table, ends, rotary, q_weight, k_weight, eps)
+
     def read(self, seqs: PackedSequences, table: DeviceArray, ends: DeviceArray
              ) -> tuple[DeviceArray, DeviceArray]:
         """The packed rows at those positions, as float32 arrays k, v."""
@@ -148,4 +186,4 @@ class KVCache:
         return k, v
 
 
-__all__ = ["PackedSequences", "KVCache", "KVPages"]
+__all__ = ["PackedSequences", "Rotary", "KVCache", "KVPages"]
