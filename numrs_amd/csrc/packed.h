@@ -27,6 +27,8 @@ struct Seqs : std::enable_shared_from_this<Seqs> {
   SeqTile *by_work = nullptr;   // [blocks] of 128 tokens, those with the most tokens before them first
   SeqTile *by_rest = nullptr;   // [blocks], those with the most tokens after them first
   SeqTile *few_by_work = nullptr, *few_by_rest = nullptr;  // the same of the tiles
+  SeqTile *whole = nullptr;     // [filled]: the sequences that have tokens
+  int64_t filled = 0, longest = 0;
   size_t bytes = 0;
   ~Seqs() { block_free(ctx, in_order, bytes); }
   // Called before a launch that reads the lists: a graph being recorded keeps them for its replays,

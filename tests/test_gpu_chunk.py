@@ -1,7 +1,11 @@
 """Attention of new tokens over a paged cache against float64.  A score is a product of two fp16 pairs (2^-22
 of the terms' magnitudes) summed in fp32, a result a sum of such products over the tokens, so the bounds are
 those of attention over the cache a token at a time: e = 2^-23 (dh + 8) max |q| . |k| / sqrt(dh) for a score,
-(2 e + 2 . 2^-23 (tokens + 8)) p . |v| for a result."""
+(2 e + 2 . 2^-23 (tokens + 8)) p . |v| for a result.  Besides, a weight p f of a token (f its values' factor)
+is split in two fp16 terms relative to the largest of 64: that one is in [2^14, 2^15) and fp16's smallest step
+2^-24, so that a weight is off by up to 2^-25, 2^-39 of the largest.  A value's terms are at most twice the
+largest token's over its factor, so this moves a result by 2^-38 max(p |v|) a token at most: what counts in a
+column where the tokens of any weight have zeros."""
 import ctypes
 import math
 
@@ -86,6 +90,7 @@ def _rows(q, k, v, seen):
         e = U2 * (dh + 8) * np.where(seen, abs(Q) @ abs(K).T, 0).max(1, keepdims=True) / math.sqrt(dh)
         out[:, h] = np.where(some[:, None], p @ V, 0)
         err[:, h] = (2 * e + 2 * U2 * (seen.sum(1, keepdims=True) + 8)) * (p @ abs(V))
+        err[:, h] += 2.0 ** -38 * seen.sum(1, keepdims=True) * (p * abs(V).max(1)).max(1, keepdims=True)
     return out, err
 
 
