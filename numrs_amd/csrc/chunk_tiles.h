@@ -59,9 +59,9 @@ struct Args {
   int exp;
 };
 
-// Rows of a stage whose factors or positions are out of the ordinary: such a stage takes a longer form.
-enum : int { kWild = 1, kOddKey = 2, kOddValue = 4, kMissing = 8 };
-// Factors within these bounds, and queries likewise, cannot make a product leave fp32's range by themselves.
+// Magnitudes within these bounds (or 0) cannot make a product leave fp32's range by themselves.  A stage with a
+// token beyond them, with one that is not finite, or on a page that the cache lacks, goes token by token in plain
+// fp32 (`take_plain`), and so does what a wave's rows see if one of their queries is beyond them.
 constexpr float kSmall = 0x1p-60f, kLarge = 0x1p60f;
 __device__ __forceinline__ bool wild(float x) { return !(x == 0.f || (fabsf(x) >= kSmall && fabsf(x) <= kLarge)); }
 // Values from 2^96 on raise the softmax's reference, so that their sums stay below fp32's largest.
@@ -117,8 +117,7 @@ struct Lds {
   char stages[2 * S::kBytes > 4 * kJoint ? 2 * S::kBytes : 4 * kJoint];
   __device__ __forceinline__ char *stage(int buf) { return stages + buf * S::kBytes; }
   float ks[2][kStage], vs[2][kStage];  // the rows' factors
-  int flags[3];                        // of three stages in turn: one is read, one written, one cleared
-  mask64 odd_key[3], odd_value[3], missing[3];
+  int plain[3];                        // of three stages in turn: one is read, one written, one cleared
 };
 
 // The cached tokens of one sequence and kv head as a block of rows walks over them.
@@ -147,7 +146,7 @@ struct Staging {
   // The token of a place within its stage: a row's, a quad's first, or a factor's.
   static __device__ __forceinline__ int token(int i) {
     const int tid = threadIdx.x;
-    if (i < S::NP) return i * S::kPass + (tid >> S::kLanes);
+    if (i < S::NP) return i * S::kPass + (tid >> S::kLanes);  // (past the stage where it has fewer rows than threads)
     if (i < S::NP + (INT8 ? S::NV : 0)) return min(((i - S::NP) * kThreads + tid) / (DP / 4), kStage / 4 - 1) * 4;
     return tid & (kStage - 1);
   }
@@ -163,15 +162,18 @@ struct Staging {
     for (int i = 0; i < NE; ++i) pages[i] = paging::page_in(entries[i], c.pages);
   }
 
+  // Loads go out whatever the place is, for its nearest neighbour where it is none, and are dropped then: what lies
+  // in slots of no token must not reach the products.
+  static __device__ __forceinline__ int64_t at(const Cache &c, const Walk &w, int pos, int page) {
+    return token_row(c, w.kv, pos, max(page, 0)) * c.dh;
+  }
+  static __device__ __forceinline__ int row_column(const Cache &c) { return 8 * (threadIdx.x & (S::kPieces - 1)); }
   // fp32 rows of keys or values: a thread's eight columns.
   __device__ __forceinline__ void load_rows(const Cache &c, const Walk &w, int stage, const void *from) {
-    const int col = 8 * (threadIdx.x & (S::kPieces - 1));
+    const int col = min(row_column(c), c.dh - 8);
 #pragma unroll
     for (int i = 0; i < S::NP; ++i) {
-      x[i][0] = x[i][1] = f4{};
-      const int tk = token(i);
-      if (pages[i] < 0 || col >= c.dh || tk >= kStage) continue;
-      const float *p = static_cast<const float *>(from) + token_row(c, w.kv, stage * kStage + tk, pages[i]) * c.dh + col;
+      const float *p = static_cast<const float *>(from) + at(c, w, stage * kStage + token(i), pages[i]) + col;
       x[i][0] = *reinterpret_cast<const f4 *>(p), x[i][1] = *reinterpret_cast<const f4 *>(p + 4);
     }
   }
@@ -179,18 +181,13 @@ struct Staging {
     if constexpr (!INT8) {
       load_rows(c, w, stage, c.k);
     } else {
-      const int col = 8 * (threadIdx.x & (S::kPieces - 1));
+      const int col = min(row_column(c), c.dh - 8);
 #pragma unroll
-      for (int i = 0; i < S::NP; ++i) {
-        const int tk = token(i);
-        kc[i] = u2{0x80808080u, 0x80808080u};
-        if (pages[i] < 0 || col >= c.dh || tk >= kStage) continue;
+      for (int i = 0; i < S::NP; ++i)
         kc[i] = *reinterpret_cast<const u2 *>(static_cast<const uint8_t *>(c.k) +
-                                              token_row(c, w.kv, stage * kStage + tk, pages[i]) * c.dh + col);
-      }
-      scale = 0.f;
-      const int page = pages[NE - 1], pos = stage * kStage + token(NE - 1);
-      if (threadIdx.x < 2 * kStage && page >= 0) scale = (threadIdx.x < kStage ? c.ks : c.vs)[token_row(c, w.kv, pos, page)];
+                                              at(c, w, stage * kStage + token(i), pages[i]) + col);
+      const float *from = threadIdx.x & kStage ? c.vs : c.ks;
+      scale = from[token_row(c, w.kv, stage * kStage + token(NE - 1), max(pages[NE - 1], 0))];
     }
   }
   __device__ __forceinline__ void load_values(const Cache &c, const Walk &w, int stage) {
@@ -199,108 +196,73 @@ struct Staging {
     } else {
 #pragma unroll
       for (int i = 0; i < S::NV; ++i) {
-        const int u = i * kThreads + threadIdx.x, col = 4 * (u % (DP / 4));
-        vc[i] = u4{0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};
-        if (pages[S::NP + i] < 0 || col >= c.dh || u >= S::kQuads) continue;
+        const int col = min(4 * ((i * kThreads + (int)threadIdx.x) % (DP / 4)), c.dh - 4);
         vc[i] = *reinterpret_cast<const u4 *>(static_cast<const uint8_t *>(c.v) +
-                                              token_row(c, w.kv, stage * kStage + token(S::NP + i), pages[S::NP + i]) * c.dh +
-                                              4 * col);
+                                              at(c, w, stage * kStage + token(S::NP + i), pages[S::NP + i]) + 4 * col);
       }
     }
   }
 
-  // Rows in fp32 into two terms; returns what is out of the ordinary.
+  // Rows in fp32 into two terms; whether all of them are ordinary.
   template <bool VALUES>
-  __device__ __forceinline__ int split_rows(char *to, float *factors, mask64 *odd) {
+  __device__ __forceinline__ bool split_rows(const Cache &c, char *to, float *factors) {
     const int piece = threadIdx.x & (S::kPieces - 1);
-    int flags = 0;
+    bool good = true;
 #pragma unroll
     for (int i = 0; i < S::NP; ++i) {
       const int tk = token(i);
-      if (tk >= kStage) continue;
+      const bool in = pages[i] >= 0 && row_column(c) < c.dh;
       float v[8];
       unsigned top = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        v[j] = x[i][j >> 2][j & 3];
+        v[j] = in ? x[i][j >> 2][j & 3] : 0.f;
         top = max(top, __builtin_bit_cast(unsigned, v[j]) & 0x7fffffffu);
       }
-      top = row_top<S::kLanes>(top);
-      const bool finite = top < 0x7f800000u;
-      const float big = __builtin_bit_cast(float, top);
-      int e = 0;
-      if (finite) {
-        e = tiles::exponent_for(big);
-      } else {
-        flags |= VALUES ? kOddValue : kOddKey;
-        if (piece == 0) atomicOr(odd, mask64{1} << tk);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 0.f;
-      }
-      if (finite && wild(big)) flags |= kWild;
+      const float big = __builtin_bit_cast(float, row_top<S::kLanes>(top));
+      good &= !wild(big);
+      const int e = tiles::exponent_for(big);
       const Terms t = tiles::split8(v, __builtin_amdgcn_ldexpf(1.f, e));
-      char *p = to + (VALUES ? S::value_place(tk, piece) : S::key_place(tk, piece));
-      *reinterpret_cast<h8 *>(p) = t.h;
-      *reinterpret_cast<h8 *>(p + kStage * S::kRow) = t.m;
-      if (piece == 0) factors[tk] = __builtin_amdgcn_ldexpf(1.f, -e);
+      if (tk < kStage) {
+        char *p = to + (VALUES ? S::value_place(tk, piece) : S::key_place(tk, piece));
+        *reinterpret_cast<h8 *>(p) = t.h;
+        *reinterpret_cast<h8 *>(p + kStage * S::kRow) = t.m;
+        if (piece == 0) factors[tk] = __builtin_amdgcn_ldexpf(1.f, -e);
+      }
     }
-    return flags;
-  }
-  static __device__ __forceinline__ void put_flags(int *to, int flags) {
-    if (flags != 0) atomicOr(to, flags);
+    return good;
   }
 
   // stage: the one that is written, of the block's walk, and its buffers.
   __device__ __forceinline__ void put_keys(Lds<INT8, DP> &s, const Cache &c, const Walk &w, int stage, int buf, int third) {
     char *to = s.stage(buf);
-    int flags = 0;
+    bool good = true;
     if constexpr (!INT8) {
-      flags = split_rows<false>(to, s.ks[buf], &s.odd_key[third]);
+      good = split_rows<false>(c, to, s.ks[buf]);
 #pragma unroll
-      for (int i = 0; i < S::NP; ++i) {
-        const int tk = token(i);
-        if (tk < kStage && pages[i] < 0 && stage * kStage + tk < w.held) {
-          flags |= kMissing;
-          atomicOr(&s.missing[third], mask64{1} << tk);
-        }
-      }
+      for (int i = 0; i < S::NP; ++i) good &= pages[i] >= 0 || stage * kStage + token(i) >= w.held;
     } else {
       const int piece = threadIdx.x & (S::kPieces - 1);
 #pragma unroll
       for (int i = 0; i < S::NP; ++i) {
         const int tk = token(i);
-        if (tk >= kStage) continue;
         u4 h;
         unsigned lo, hi;
         paged::halves(kc[i][0], lo, hi), h[0] = lo, h[1] = hi;
         paged::halves(kc[i][1], lo, hi), h[2] = lo, h[3] = hi;
-        *reinterpret_cast<u4 *>(to + S::key_place(tk, piece)) = h;
+        if (tk < kStage) *reinterpret_cast<u4 *>(to + S::key_place(tk, piece)) = h;
       }
       const int tk = threadIdx.x & (kStage - 1);
-      if (threadIdx.x < kStage) {
-        s.ks[buf][tk] = scale;
-        if (wild(scale)) flags |= kWild;
-        if (pages[NE - 1] < 0 && stage * kStage + tk < w.held) {
-          flags |= kMissing;
-          atomicOr(&s.missing[third], mask64{1} << tk);
-        }
-      } else if (threadIdx.x < 2 * kStage) {
-        const bool finite = fabsf(scale) < INFINITY;
-        if (!finite) {
-          flags |= kOddValue;
-          atomicOr(&s.odd_value[third], mask64{1} << tk);
-        } else if (wild(scale)) {
-          flags |= kWild;
-        }
-        s.vs[buf][tk] = finite ? scale : 0.f;
-      }
+      const float y = pages[NE - 1] >= 0 ? scale : 0.f;
+      if (threadIdx.x < 2 * kStage) (threadIdx.x < kStage ? s.ks : s.vs)[buf][tk] = y;
+      good = !wild(y) && (pages[NE - 1] >= 0 || stage * kStage + tk >= w.held);
     }
-    put_flags(&s.flags[third], flags);
+    if (!good) s.plain[third] = 1;
   }
-  __device__ __forceinline__ void put_values(Lds<INT8, DP> &s, int buf, int third) {
+  __device__ __forceinline__ void put_values(Lds<INT8, DP> &s, const Cache &c, int buf, int third) {
     char *to = s.stage(buf) + S::kKeys;
     if constexpr (!INT8) {
-      put_flags(&s.flags[third], split_rows<true>(to, s.vs[buf], &s.odd_value[third]));
+      if (!split_rows<true>(c, to, s.vs[buf])) s.plain[third] = 1;
     } else {
       // four tokens' values of a column lie together: eight bytes of a product's operand
 #pragma unroll
@@ -355,7 +317,12 @@ __device__ __forceinline__ Terms values_of(const char *p, int token, int b, int 
   return t;
 }
 
-// A cached value, for what the products do not take.
+// A cached key or value.
+template <bool INT8>
+__device__ __forceinline__ float key_at(const Cache &c, int64_t row, int d) {
+  if constexpr (!INT8) return static_cast<const float *>(c.k)[row * c.dh + d];
+  return (float)((int)static_cast<const uint8_t *>(c.k)[row * c.dh + d] - 128) * c.ks[row];
+}
 template <bool INT8>
 __device__ __forceinline__ float value_at(const Cache &c, int64_t row, int d) {
   if constexpr (!INT8) return static_cast<const float *>(c.v)[row * c.dh + d];
@@ -368,200 +335,155 @@ template <bool INT8, int DP>
 struct Rows {
   using S = Shape<INT8, DP>;
   Terms q[S::NS];
-  f16 o[S::NB];
-  float m, l;
-  int fe;    // the scores' exponent
-  int seen;  // tokens that the lane's row sees; 0: none
-  bool some, odd;
-  const float *from;  // the row's query
+  float o[S::NB][16];
+  float m, l;   // l: of the lane's own half of the tokens
+  float f;      // log2(e) / sqrt(dh) over the query's factor, a power of two
+  int seen;     // tokens that the lane's row sees; 0: none
+  bool some;    // of them in the cache so far
+  bool plain;   // a query of the wave is beyond the bounds
 
   __device__ __forceinline__ void start(const Args &a, const float *row, bool live, int sees) {
     const int hi = (threadIdx.x & 63) >> 5;
-    from = row, seen = sees, some = false;
+    seen = sees, some = false;
     tiles::RowValues<DP> x;
     x.load(row, live, a.c.dh, hi);
     bool not_finite = false;
     const float top = x.top(INFINITY, not_finite);
     const int e = tiles::exponent_for(top);
-    fe = a.exp - e;
-    odd = __any(wild(top));
+    f = __builtin_amdgcn_ldexpf(1.f, a.exp - e);
+    plain = __any(not_finite || wild(top));
     x.split_into(q, __builtin_amdgcn_ldexpf(a.mant, e));
     m = kNever, l = 0.f;
 #pragma unroll
-    for (int b = 0; b < S::NB; ++b) o[b] = f16{};
+    for (int b = 0; b < S::NB; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[b][e] = 0.f;
   }
 
-  // KB blocks of 32 tokens from `first` of the stage, whose tokens begin at pos0.
-  template <bool WILD, int KB>
-  __device__ __forceinline__ void take(const Args &a, const Walk &w, Lds<INT8, DP> &lds, int buf, int third, int first,
-                                       int pos0, bool masked) {
+  __device__ __forceinline__ void raise(float now) {
+    const float r = __builtin_amdgcn_exp2f(m - now);
+    m = now;
+    l *= r;
+#pragma unroll
+    for (int b = 0; b < S::NB; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[b][e] *= r;
+  }
+
+  // 32 tokens from `first` of a stage: the products of their keys ...
+  __device__ __forceinline__ void products(Lds<INT8, DP> &lds, int buf, int first, f16 &s) const {
     const int lane = threadIdx.x & 63, c = lane & 31, hi = lane >> 5;
-    const char *keys = lds.stage(buf), *values = keys + S::kKeys;
-    f16 s[KB] = {};
+    const char *keys = lds.stage(buf);
+    auto ask = [&](int st) {
+      const char *p = keys + S::key_place(first + c, 2 * st + hi);
+      Terms k;
+      k.h = *reinterpret_cast<const h8 *>(p);
+      if constexpr (!INT8) k.m = *reinterpret_cast<const h8 *>(p + kStage * S::kRow);
+      return k;
+    };
+    Terms k = ask(0);
+    s = f16{};
 #pragma unroll
-    for (int st = 0; st < S::NS; ++st)
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        const char *p = keys + S::key_place(first + 32 * kb + c, 2 * st + hi);
-        Terms k;
-        k.h = *reinterpret_cast<const h8 *>(p);
-        if constexpr (!INT8) k.m = *reinterpret_cast<const h8 *>(p + kStage * S::kRow);
-        mma_keys<INT8>(s[kb], k, q[st]);
-      }
+    for (int st = 0; st < S::NS; ++st) {
+      Terms next;
+      if (st + 1 < S::NS) next = ask(st + 1);
+      __builtin_amdgcn_sched_barrier(0);  // the next step's operands are asked for before this one's products
+      mma_keys<INT8>(s, k, q[st]);
+      k = next;
+    }
+  }
+
+  // ... and what follows from them; the stage's tokens begin at pos0.
+  __device__ __forceinline__ void take(Lds<INT8, DP> &lds, int buf, int first, int pos0, bool masked, f16 &s) {
+    const int lane = threadIdx.x & 63, hi = lane >> 5;
+    const char *values = lds.stage(buf) + S::kKeys;
     // factors of the rows that a lane's results are, four at a time
-    auto factors = [&](const float *f, int kb, int i) { return *reinterpret_cast<const f4 *>(f + first + 32 * kb + 8 * i + 4 * hi); };
-    float f = 1.f;
-    if constexpr (!WILD) f = __builtin_amdgcn_ldexpf(1.f, fe);
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
+    auto by_factors = [&](const float *factors) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const f4 k = factors(lds.ks[buf], kb, i);
+        const f4 x = *reinterpret_cast<const f4 *>(factors + first + 8 * i + 4 * hi);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float x = s[kb][4 * i + j], by = k[j];
-          if constexpr (WILD)
-            s[kb][4 * i + j] = __builtin_amdgcn_ldexpf(x * __builtin_amdgcn_frexp_mantf(by), __builtin_amdgcn_frexp_expf(by) + fe);
-          else
-            s[kb][4 * i + j] = x * by;
-        }
+        for (int j = 0; j < 4; ++j) s[4 * i + j] *= x[j];
       }
-    int raise = 0;
-    mask64 missing = 0, odd_value = 0;
-    if constexpr (WILD) {
-      missing = uniform((int64_t)lds.missing[third]), odd_value = uniform((int64_t)lds.odd_value[third]);
-      if constexpr (!INT8) {
-        // keys that are not finite: their scores in plain fp32
-        mask64 left = uniform((int64_t)lds.odd_key[third]) >> first;
-        if constexpr (KB == 1) left &= 0xffffffffu;
-        for (; left != 0; left &= left - 1) {
-          const int t = __builtin_ctzll(left), pos = pos0 + first + t;
-          const int page = paging::page_of(w.pages, a.c.max_pages, a.c.shift, a.c.pages, pos);
-          if (page < 0) continue;
-          const float *k = static_cast<const float *>(a.c.k) + token_row(a.c, w.kv, pos, page) * a.c.dh;
-          float x = 0.f;
-          if (seen > 0)
-            for (int d = 0; d < a.c.dh; ++d) x = fmaf(from[d], k[d], x);
-          x *= __builtin_amdgcn_ldexpf(a.mant, a.exp);
-#pragma unroll
-          for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (32 * kb + tiles::out_row(e, hi) == t) s[kb][e] = x;
-        }
-      }
-      float big = 0.f;
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f4 v = factors(lds.vs[buf], kb, i);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) big = fmaxf(big, fabsf(v[j]));
-        }
-      big = half_pair(big, [](float x, float y) { return fmaxf(x, y); });
-      raise = big > 0.f ? __builtin_amdgcn_frexp_expf(big) : 0;  // of the factors for now
-    }
+    };
+    by_factors(lds.ks[buf]);
     const int left = seen - pos0 - first;  // tokens from the first that the row sees
-    if (WILD || masked) {
+    if (masked) {
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int t = 32 * kb + tiles::out_row(e, hi);
-          bool gone = t >= left;
-          if constexpr (WILD) gone |= (missing >> (first + t) & 1) != 0;
-          if (gone) s[kb][e] = -INFINITY;
-        }
+      for (int e = 0; e < 16; ++e)
+        if (tiles::out_row(e, hi) >= left) s[e] = -INFINITY;
     }
-    if constexpr (WILD) {
-      const int n = min(max(left, 0), 32 * KB);
-      const mask64 sees = n == 64 ? ~mask64{0} : (mask64{1} << n) - 1;
-      some |= (~missing >> first & sees) != 0;
-    } else {
-      some |= left > 0;
-    }
-    float most = tiles::over16(s[0], [](float x, float y) { return fmaxf(x, y); });
-    if constexpr (KB == 2) most = fmaxf(most, tiles::over16(s[1], [](float x, float y) { return fmaxf(x, y); }));
-    most = half_pair(most, [](float x, float y) { return fmaxf(x, y); });
-    if constexpr (!WILD) most *= f;
-    const int ev = WILD ? raise : 0;
-    if constexpr (WILD) most += (float)max(0, ev + (INT8 ? 7 : 15) - kRaise);
-    if (__any(most > m + 8.f)) {
-      const float now = fmaxf(m, most), r = __builtin_amdgcn_exp2f(m - now);
-      m = now;
-      l *= r;
+    some |= left > 0;
+    const float most = half_pair(tiles::over16(s, [](float x, float y) { return fmaxf(x, y); }),
+                                 [](float x, float y) { return fmaxf(x, y); }) * f;
+    if (__any(most > m + 8.f)) raise(fmaxf(m, most));
 #pragma unroll
-      for (int b = 0; b < S::NB; ++b)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[b][e] *= r;
-    }
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[kb][e] = __builtin_amdgcn_exp2f(fmaf(s[kb][e], f, -m));
-      l += tiles::over16(s[kb], [](float x, float y) { return x + y; });
-    }
-    if constexpr (WILD) {
-      // values that are not finite: in plain fp32, for the rows that see them
-      mask64 odd = odd_value >> first;
-      if constexpr (KB == 1) odd &= 0xffffffffu;
-      for (; odd != 0; odd &= odd - 1) {
-        const int t = __builtin_ctzll(odd), pos = pos0 + first + t;
-        const int page = paging::page_of(w.pages, a.c.max_pages, a.c.shift, a.c.pages, pos);
-        if (page < 0) continue;
-        const int64_t row = token_row(a.c, w.kv, pos, page);
-        float p = 0.f;
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (32 * kb + tiles::out_row(e, hi) == t) p = s[kb][e];
-        p = half_pair(p, [](float x, float y) { return x + y; });
-        if (t >= left) continue;
-#pragma unroll
-        for (int b = 0; b < S::NB; ++b)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int d = 32 * b + tiles::out_row(e, hi);
-            if (d < a.c.dh) o[b][e] = fmaf(p, value_at<INT8>(a.c, row, d), o[b][e]);
-          }
-      }
-    }
+    for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], f, -m));
+    l += tiles::over16(s, [](float x, float y) { return x + y; });
     // the probabilities times the values' factors, the largest of a row brought to [2^14, 2^15)
-    float top = 0.f;
-    const float down = WILD ? __builtin_amdgcn_ldexpf(1.f, -ev) : 1.f;
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f4 v = factors(lds.vs[buf], kb, i);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[kb][4 * i + j] *= WILD ? v[j] * down : v[j];
-      }
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb) top = tiles::top_of(s[kb], top);
-    top = half_pair(top, [](float x, float y) { return fmaxf(x, y); });
+    by_factors(lds.vs[buf]);
+    const float top = half_pair(tiles::top_of(s, 0.f), [](float x, float y) { return fmaxf(x, y); });
     const int et = max(__builtin_amdgcn_frexp_expf(top), -100);
-    const float lift = __builtin_amdgcn_ldexpf(1.f, 15 - et), back = __builtin_amdgcn_ldexpf(1.f, et - 15 + ev);
-    Terms p[KB][2];
+    const float lift = __builtin_amdgcn_ldexpf(1.f, 15 - et), back = __builtin_amdgcn_ldexpf(1.f, et - 15);
+    float x[16];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      float x[16];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = s[kb][e];
-      p[kb][0] = tiles::split8(x, lift), p[kb][1] = tiles::split8(x + 8, lift);
-    }
+    for (int e = 0; e < 16; ++e) x[e] = s[e];
+    const Terms p[2] = {tiles::split8(x, lift), tiles::split8(x + 8, lift)};
+    constexpr int kSteps = 2;  // of 16 tokens
+    Terms v = values_of<INT8, DP>(values, first, 0, lane);
 #pragma unroll
     for (int b = 0; b < S::NB; ++b) {
       f16 z = {};
 #pragma unroll
-      for (int st = 0; st < 2 * KB; ++st) {
-        const Terms v = values_of<INT8, DP>(values, first + 16 * st, b, lane);
-        mma_keys<INT8>(z, v, p[st >> 1][st & 1]);
+      for (int st = 0; st < kSteps; ++st) {
+        const int nb = st + 1 < kSteps ? b : b + 1, ns = (st + 1) % kSteps;
+        Terms next;
+        if (nb < S::NB) next = values_of<INT8, DP>(values, first + 16 * ns, nb, lane);
+        __builtin_amdgcn_sched_barrier(0);
+        mma_keys<INT8>(z, v, p[st]);
+        v = next;
       }
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[b][e] = fmaf(z[e], back, o[b][e]);
+    }
+  }
+
+  // The same in plain fp32, a token after the other: a lane forms half of its row's score, and adds to its columns
+  // of the result.  What is not finite does what it does in fp32, and only to the rows that see it.
+  __device__ __forceinline__ void take_plain(const Args &a, const Walk &w, const float *row, int from, int to) {
+    const int hi = (threadIdx.x & 63) >> 5, half = (a.c.dh / 8 + 1) / 2 * 8;
+    const float scale = __builtin_amdgcn_ldexpf(a.mant, a.exp);
+#pragma unroll 1
+    for (int pos = from; pos < to; ++pos) {
+      int dh = a.c.dh;
+      asm volatile("" : "+s"(dh));  // what follows from it is formed here, not kept in registers throughout
+      const int page = pos < w.held ? paging::page_of(w.pages, a.c.max_pages, a.c.shift, a.c.pages, pos) : -1;
+      if (page < 0) continue;
+      const int64_t at = token_row(a.c, w.kv, pos, page);
+      float x = 0.f, big = 0.f;
+#pragma unroll 1
+      for (int d = hi * half; d < min(dh, (hi + 1) * half); ++d) {
+        x = fmaf(row[d], key_at<INT8>(a.c, at, d), x);
+        const float v = fabsf(value_at<INT8>(a.c, at, d));
+        if (v < INFINITY) big = fmaxf(big, v);
+      }
+      x = half_pair(x, [](float x, float y) { return x + y; }) * scale;
+      big = half_pair(big, [](float x, float y) { return fmaxf(x, y); });
+      if (pos < seen) {
+        some = true;
+        // values from 2^96 on raise the reference, so that their sums stay below fp32's largest
+        const float now = x + fmaxf(0.f, (float)(__builtin_amdgcn_frexp_expf(big) - 96));
+        if (now > m) raise(now);
+        const float p = __builtin_amdgcn_exp2f(x - m);
+        if (hi == 0 || p != p) l += p;
+#pragma unroll
+        for (int b = 0; b < S::NB; ++b) {
+          asm volatile("" : "+s"(dh));
+#pragma unroll
+          for (int e = 0; e < 16; ++e)  // (a column past the head reads the last one again: it is not written)
+            o[b][e] = fmaf(p, value_at<INT8>(a.c, at, min(32 * b + tiles::out_row(e, hi), dh - 1)), o[b][e]);
+        }
+      }
     }
   }
 };
@@ -580,7 +502,7 @@ __device__ __forceinline__ int stages_of(const Cache &c, int group, int len, int
 template <bool INT8, int DP, int Z>
 __global__ void __launch_bounds__(kThreads, 2) walk_blocks(Args a) {
   using S = Shape<INT8, DP>;
-  constexpr int R = 8 / Z, ROWS = 32 * R, KB = 2 / Z;
+  constexpr int R = 8 / Z, ROWS = 32 * R;
   __shared__ __attribute__((aligned(16))) Lds<INT8, DP> lds;
   __shared__ int64_t pre[kThreads + 1], sums[8];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -656,43 +578,46 @@ __global__ void __launch_bounds__(kThreads, 2) walk_blocks(Args a) {
       const int most = live_rows > 0 ? __builtin_amdgcn_readlane(n_seen, live_rows - 1) : 0;
       Staging<INT8, DP> g;
       g.look(a.c, walk, s0);
-      if (tid < 3) lds.flags[tid] = 0, lds.odd_key[tid] = lds.odd_value[tid] = lds.missing[tid] = 0;
+      if (tid < 3) lds.plain[tid] = 0;
       Rows<INT8, DP> r;
-      r.start(a, a.q + (int64_t)(t.row0 + token) * a.ld_q + (int64_t)head * a.c.dh, live, n_seen);
+      const float *query = a.q + (int64_t)(t.row0 + token) * a.ld_q + (int64_t)head * a.c.dh;
+      r.start(a, query, live, n_seen);
       g.resolve(a.c);
-      __syncthreads();  // the flags are cleared, the last block's buffers free
+      __syncthreads();  // the marks are cleared, the last block's buffers free
       g.load_keys(a.c, walk, s0);
       g.put_keys(lds, a.c, walk, s0, 0, 0);
       g.load_values(a.c, walk, s0);
-      g.put_values(lds, 0, 0);
+      g.put_values(lds, a.c, 0, 0);
       g.look(a.c, walk, s0 + 1);
       for (int i = s0; i < s1; ++i) {
         const int buf = (i - s0) & 1, third = (i - s0) % 3, after = (i - s0 + 1) % 3;
         const bool more = i + 1 < s1;
         __syncthreads();
-        const int flags = __builtin_amdgcn_readfirstlane(lds.flags[third]);
-        if (tid == 0) {
-          const int clear = (i - s0 + 2) % 3;
-          lds.flags[clear] = 0, lds.odd_key[clear] = lds.odd_value[clear] = lds.missing[clear] = 0;
-        }
-        const int pos0 = i * kStage, first = 32 * z;
+        const bool plain = __builtin_amdgcn_readfirstlane(lds.plain[third]) != 0 || r.plain;
+        if (tid == 0) lds.plain[(i - s0 + 2) % 3] = 0;
+        const int pos0 = i * kStage;
         if (more) {
           g.resolve(a.c);
           g.load_keys(a.c, walk, i + 1);
         }
-        if (pos0 + first < most) {
-          const bool masked = pos0 + first + 32 * KB > least;
-          if (flags != 0 || r.odd)
-            r.template take<true, KB>(a, walk, lds, buf, third, first, pos0, masked);
-          else
-            r.template take<false, KB>(a, walk, lds, buf, third, first, pos0, masked);
-        }
+        if (plain) r.take_plain(a, walk, query, pos0 + 32 * z, min(pos0 + 32 * z + kStage / Z, most));
+        f16 s;
+        auto products = [&](int first) {
+          if (pos0 + first < most && !plain) r.products(lds, buf, first, s);
+        };
+        auto take = [&](int first) {
+          if (pos0 + first < most && !plain) r.take(lds, buf, first, pos0, pos0 + first + 32 > least, s);
+        };
+        products(32 * z);
+        if constexpr (Z == 1) take(0);
         if (more) {
           g.put_keys(lds, a.c, walk, i + 1, buf ^ 1, after);
           g.load_values(a.c, walk, i + 1);
-          g.put_values(lds, buf ^ 1, after);
           g.look(a.c, walk, i + 2);
         }
+        if constexpr (Z == 1) products(32);
+        take(Z == 1 ? 32 : 32 * z);
+        if (more) g.put_values(lds, a.c, buf ^ 1, after);
       }
       float l = half_pair(r.l, [](float x, float y) { return x + y; });
       __syncthreads();
@@ -767,42 +692,62 @@ __global__ void __launch_bounds__(kThreads, 2) walk_blocks(Args a) {
   }
 }
 
-// The parts of blocks that were cut, added in order: a wave a row, its halves every other part.
+// The parts of blocks that were cut, added in order: a workgroup a row, 32 threads with four columns each in eight
+// sets of every eighth part, whose loads go out eight at a time.
 template <int DP, int ROWS>
 __global__ void __launch_bounds__(256) join_parts(Args a) {
+  constexpr int kAhead = 8;
   const Cut cut = a.cuts[blockIdx.x];
-  const int lane = threadIdx.x & 63, half = lane >> 5, d = 4 * (lane & 31);
-  for (int r = blockIdx.y * 4 + (int)(threadIdx.x >> 6); cut.parts > 0 && r < cut.rows; r += gridDim.y * 4) {
+  const int tid = threadIdx.x, lane = tid & 63, set = tid >> 5, d = 4 * (tid & 31);
+  __shared__ float tops[4], sums[8];
+  __shared__ f4 outs[8][32];
+  for (int r = blockIdx.y; cut.parts > 0 && r < cut.rows; r += gridDim.y) {
     // the first part is the owner's place 1, the others the next ones' places 0
     auto part = [&](int k) { return a.parts + (int64_t)(k == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + k)) * kPart<DP, ROWS>; };
     float m = kNever;
-    for (int k = lane; k < cut.parts; k += 64) m = fmaxf(m, part(k)[r]);
+    for (int k = tid; k < cut.parts; k += 256) m = fmaxf(m, part(k)[r]);
     m = wave_max(m);
-    float l = 0.f;
-    bool some = false;
+    if (lane == 0) tops[tid >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    float l = -1.f;  // below 0: no token
     f4 o{};
-    for (int k = half; k < cut.parts; k += 2) {
-      const float *x = part(k);
-      const float lk = x[ROWS + r];
-      if (lk < 0.f) continue;
-      const float f = __builtin_amdgcn_exp2f(x[r] - m);
-      some = true, l = fmaf(lk, f, l);
-      if (d < a.c.dh) {
-        const f4 y = *reinterpret_cast<const f4 *>(x + 2 * ROWS + r * DP + d);
+    for (int k0 = set; k0 < cut.parts; k0 += 8 * kAhead) {
+      float ms[kAhead], ls[kAhead];
+      f4 y[kAhead];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = fmaf(y[j], f, o[j]);
+      for (int i = 0; i < kAhead; ++i) {
+        const float *x = part(min(k0 + 8 * i, cut.parts - 1));  // past the last: read again, not added
+        ms[i] = x[r], ls[i] = x[ROWS + r];
+        y[i] = *reinterpret_cast<const f4 *>(x + 2 * ROWS + r * DP + min(d, DP - 4));
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (k0 + 8 * i >= cut.parts || ls[i] < 0.f) continue;
+        const float f = __builtin_amdgcn_exp2f(ms[i] - m);
+        l = fmaf(ls[i], f, fmaxf(l, 0.f));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = fmaf(y[i][j], f, o[j]);
       }
     }
-    auto add = [](float x, float y) { return x + y; };
-    l = half_pair(l, add);
-    some = __any(some);
+    if ((tid & 31) == 0) sums[set] = l;
+    outs[set][tid & 31] = o;
+    __syncthreads();
+    if (set == 0 && d < a.c.dh) {
+      bool some = false;
+      l = 0.f, o = f4{};
+      for (int i = 0; i < 8; ++i) {
+        if (sums[i] < 0.f) continue;
+        some = true, l += sums[i];
+        const f4 y = outs[i][tid];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = half_pair(o[j], add);
-    if (half == 0 && d < a.c.dh) {
+        for (int j = 0; j < 4; ++j) o[j] += y[j];
+      }
       const int row = cut.row + r;
-      const f4 y = some ? o / l : f4{};
-      *reinterpret_cast<f4u *>(a.out + (int64_t)(cut.row0 + row / a.group) * a.ld_out + (int64_t)(cut.head + row % a.group) * a.c.dh + d) = y;
+      *reinterpret_cast<f4u *>(a.out + (int64_t)(cut.row0 + row / a.group) * a.ld_out + (int64_t)(cut.head + row % a.group) * a.c.dh + d) =
+          some ? o / l : f4{};
     }
+    __syncthreads();
   }
 }
 

@@ -180,11 +180,11 @@ def test_bad_tables(hip_ctx, format, n):
 @pytest.mark.parametrize("format", ["f32", "int8"])
 @pytest.mark.parametrize("n", [3, 150])
 def test_values_that_are_not_finite(hip_ctx, format, n):
-    """What is not finite reaches its own head and sequence, and there the rows that see it; infinite keys
-    and values do what fp32 arithmetic does with them."""
+    """What is not finite reaches its own head and sequence, and there the rows that see it (the others have
+    what they had, up to their bounds); infinite keys and values do what fp32 arithmetic does with them."""
     c, rng, H, Hk, dh = hip_ctx, np.random.default_rng(23), 4, 2, 64
     t = _Chunk(c, [n, n, n, n], [200, 70, 0, 333], 16, H, Hk, dh, format, rng).write()
-    clean = t.run().reshape(4, n, Hk, 2, dh)
+    clean, bound = t.run().reshape(4, n, Hk, 2, dh), t.reference()[1].reshape(4, n, Hk, 2, dh)
     at = np.concatenate([[0], np.cumsum(t.total)])
     k, v, q = t.k.copy(), t.v.copy(), t.q.copy()
     t.k[50, 3] = np.nan                            # sequence 0, head 0: every row
@@ -197,7 +197,8 @@ def test_values_that_are_not_finite(hip_ctx, format, n):
     assert np.isnan(got[0, :, 0]).all()
     assert_bits(got[0, :, 1], clean[0, :, 1])
     assert_bits(got[1, :, 0], clean[1, :, 0])
-    assert_bits(got[1, :seen, 1], clean[1, :seen, 1])
+    same = lambda i, rows, h: (abs(got[i, rows, h] - clean[i, rows, h]) <= 2 * bound[i, rows, h]).all()  # noqa: E731
+    assert same(1, slice(seen), 1)
     rest = np.arange(dh) != 5
     if format == "f32":
         assert np.isposinf(got[1, seen:, 1, :, 5]).all()
@@ -205,7 +206,7 @@ def test_values_that_are_not_finite(hip_ctx, format, n):
     else:
         assert np.isnan(got[1, seen:, 1]).all()  # such a row reads back as NaN
     assert_bits(got[2, :, 1], clean[2, :, 1])
-    assert_bits(got[2, :n - 1, 0], clean[2, :n - 1, 0])
+    assert same(2, slice(n - 1), 0)
     assert np.isnan(got[2, n - 1, 0, :, 7]).all()
     if format == "f32":
         others = np.arange(dh) != 7
@@ -227,7 +228,7 @@ def test_values_that_are_not_finite(hip_ctx, format, n):
     bad = np.zeros((4 * n, H), bool)
     bad[0, 0] = bad[2 * n + 1, 1] = True
     assert np.isnan(got[bad]).all()
-    assert_bits(got[~bad], clean[~bad])
+    assert (abs(got - clean) <= 2 * bound.reshape(4 * n, H, dh))[~bad].all()
 
 
 @pytest.mark.parametrize("format", ["f32", "int8"])
