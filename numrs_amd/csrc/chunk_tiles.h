@@ -64,6 +64,8 @@ struct Args {
 // fp32 (`take_plain`), and so does what a wave's rows see if one of their queries is beyond them.
 constexpr float kSmall = 0x1p-60f, kLarge = 0x1p60f;
 __device__ __forceinline__ bool wild(float x) { return !(x == 0.f || (fabsf(x) >= kSmall && fabsf(x) <= kLarge)); }
+// The larger; NaN if one is.
+__device__ __forceinline__ float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 // Values from 2^96 on raise the softmax's reference, so that their sums stay below fp32's largest.
 constexpr int kRaise = 96;
 
@@ -87,6 +89,7 @@ struct Shape {
   static constexpr int kBytes = kKeys + kValues;  // of a stage
   static constexpr int kQuads = kStage / 4 * (DP / 4), NV = (kQuads + kThreads - 1) / kThreads;
 
+  // (A piece 2 st + hi of keys is at the piece hi's place ^ 32 st, a piece 4 b + x of values at x's ^ 64 b.)
   static __device__ __forceinline__ int key_place(int token, int piece) {
     const int turn = kPieces == 16 ? token : kPieces == 8 ? token >> 1 : token >> 2;
     return token * kRow + ((piece ^ turn) & (kPieces - 1)) * 16;
@@ -114,11 +117,18 @@ template <bool INT8, int DP>
 struct Lds {
   using S = Shape<INT8, DP>;
   static constexpr int kJoint = 64 * (16 * S::NB + 4) * 4;  // a wave's results, while sets are joined
+  // (the stages last: an LDS access has 16 bits for a constant offset)
+  float ks[2][kStage], vs[2][kStage];  // the rows' factors
+  int plain[4];                        // of three stages in turn: one is read, one written, one cleared
   char stages[2 * S::kBytes > 4 * kJoint ? 2 * S::kBytes : 4 * kJoint];
   __device__ __forceinline__ char *stage(int buf) { return stages + buf * S::kBytes; }
-  float ks[2][kStage], vs[2][kStage];  // the rows' factors
-  int plain[3];                        // of three stages in turn: one is read, one written, one cleared
 };
+
+// The same value, formed again: what follows from it is not kept in registers around a loop.
+__device__ __forceinline__ int again(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
 
 // The cached tokens of one sequence and kv head as a block of rows walks over them.
 struct Walk {
@@ -137,7 +147,8 @@ struct Staging {
   using S = Shape<INT8, DP>;
   static constexpr int NE = INT8 ? S::NP + S::NV + 1 : S::NP;  // places whose pages it needs
   int32_t entries[NE];
-  int pages[NE];
+  int64_t at[NE];  // the element of the cache that the thread loads first, of a factor its place
+  unsigned have;   // places that the cache has, a bit each
   f4 x[INT8 ? 1 : S::NP][2];
   u2 kc[INT8 ? S::NP : 1];
   u4 vc[INT8 ? S::NV : 1];
@@ -157,49 +168,46 @@ struct Staging {
       entries[i] = pos < w.held ? paging::entry_of(w.pages, c.max_pages, c.shift, pos) : -1;
     }
   }
-  __device__ __forceinline__ void resolve(const Cache &c) {
-#pragma unroll
-    for (int i = 0; i < NE; ++i) pages[i] = paging::page_in(entries[i], c.pages);
-  }
-
-  // Loads go out whatever the place is, for its nearest neighbour where it is none, and are dropped then: what lies
-  // in slots of no token must not reach the products.
-  static __device__ __forceinline__ int64_t at(const Cache &c, const Walk &w, int pos, int page) {
-    return token_row(c, w.kv, pos, max(page, 0)) * c.dh;
-  }
   static __device__ __forceinline__ int row_column(const Cache &c) { return 8 * (threadIdx.x & (S::kPieces - 1)); }
+  // Loads go out whatever the place is, from the cache's first page where it is none, and are dropped then: what
+  // lies in slots of no token must not reach the products.
+  __device__ __forceinline__ void resolve(const Cache &c, const Walk &w, int stage) {
+    have = 0;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      const int page = paging::page_in(entries[i], c.pages);
+      have |= page >= 0 ? 1u << i : 0u;
+      at[i] = token_row(c, w.kv, stage * kStage + token(i), max(page, 0));
+      if (i < S::NP)
+        at[i] = at[i] * c.dh + min(row_column(c), c.dh - 8);
+      else if (i < NE - 1)
+        at[i] = at[i] * c.dh + 4 * min(4 * (((i - S::NP) * kThreads + (int)threadIdx.x) % (DP / 4)), c.dh - 4);
+    }
+  }
   // fp32 rows of keys or values: a thread's eight columns.
-  __device__ __forceinline__ void load_rows(const Cache &c, const Walk &w, int stage, const void *from) {
-    const int col = min(row_column(c), c.dh - 8);
+  __device__ __forceinline__ void load_rows(const void *from) {
 #pragma unroll
     for (int i = 0; i < S::NP; ++i) {
-      const float *p = static_cast<const float *>(from) + at(c, w, stage * kStage + token(i), pages[i]) + col;
+      const float *p = static_cast<const float *>(from) + at[i];
       x[i][0] = *reinterpret_cast<const f4 *>(p), x[i][1] = *reinterpret_cast<const f4 *>(p + 4);
     }
   }
-  __device__ __forceinline__ void load_keys(const Cache &c, const Walk &w, int stage) {
+  __device__ __forceinline__ void load_keys(const Cache &c) {
     if constexpr (!INT8) {
-      load_rows(c, w, stage, c.k);
+      load_rows(c.k);
     } else {
-      const int col = min(row_column(c), c.dh - 8);
 #pragma unroll
-      for (int i = 0; i < S::NP; ++i)
-        kc[i] = *reinterpret_cast<const u2 *>(static_cast<const uint8_t *>(c.k) +
-                                              at(c, w, stage * kStage + token(i), pages[i]) + col);
-      const float *from = threadIdx.x & kStage ? c.vs : c.ks;
-      scale = from[token_row(c, w.kv, stage * kStage + token(NE - 1), max(pages[NE - 1], 0))];
+      for (int i = 0; i < S::NP; ++i) kc[i] = *reinterpret_cast<const u2 *>(static_cast<const uint8_t *>(c.k) + at[i]);
+      scale = (threadIdx.x & kStage ? c.vs : c.ks)[at[NE - 1]];
     }
   }
-  __device__ __forceinline__ void load_values(const Cache &c, const Walk &w, int stage) {
+  __device__ __forceinline__ void load_values(const Cache &c) {
     if constexpr (!INT8) {
-      load_rows(c, w, stage, c.v);
+      load_rows(c.v);
     } else {
 #pragma unroll
-      for (int i = 0; i < S::NV; ++i) {
-        const int col = min(4 * ((i * kThreads + (int)threadIdx.x) % (DP / 4)), c.dh - 4);
-        vc[i] = *reinterpret_cast<const u4 *>(static_cast<const uint8_t *>(c.v) +
-                                              at(c, w, stage * kStage + token(S::NP + i), pages[S::NP + i]) + 4 * col);
-      }
+      for (int i = 0; i < S::NV; ++i)
+        vc[i] = *reinterpret_cast<const u4 *>(static_cast<const uint8_t *>(c.v) + at[S::NP + i]);
     }
   }
 
@@ -211,23 +219,28 @@ struct Staging {
 #pragma unroll
     for (int i = 0; i < S::NP; ++i) {
       const int tk = token(i);
-      const bool in = pages[i] >= 0 && row_column(c) < c.dh;
-      float v[8];
-      unsigned top = 0;
+      const bool in = (have >> i & 1) != 0 && row_column(c) < c.dh;
+      if (__any(!in)) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[j] = in ? x[i][j >> 2][j & 3] : 0.f;
-        top = max(top, __builtin_bit_cast(unsigned, v[j]) & 0x7fffffffu);
+        for (int j = 0; j < 8; ++j) x[i][j >> 2][j & 3] = in ? x[i][j >> 2][j & 3] : 0.f;
       }
-      const float big = __builtin_bit_cast(float, row_top<S::kLanes>(top));
-      good &= !wild(big);
-      const int e = tiles::exponent_for(big);
-      const Terms t = tiles::split8(v, __builtin_amdgcn_ldexpf(1.f, e));
+      float v[8], big = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = x[i][j >> 2][j & 3];
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) big = maximum(maximum(big, fabsf(v[j])), fabsf(v[j + 1]));
+      const unsigned top = row_top<S::kLanes>(__builtin_bit_cast(unsigned, big));
+      // The power of two that puts the largest into [2^14, 2^15), from its exponent's bits; within the bounds
+      // neither it nor its inverse leaves the normal numbers (and beyond them the split is not used).
+      constexpr unsigned kLow = 127 - 60, kHigh = 127 + 60;
+      const unsigned e = max(top >> 23, kLow);
+      good &= e < kHigh && (top >> 23 >= kLow || top == 0);
+      const Terms t = tiles::split8(v, __builtin_bit_cast(float, (268 - e) << 23));
       if (tk < kStage) {
         char *p = to + (VALUES ? S::value_place(tk, piece) : S::key_place(tk, piece));
         *reinterpret_cast<h8 *>(p) = t.h;
         *reinterpret_cast<h8 *>(p + kStage * S::kRow) = t.m;
-        if (piece == 0) factors[tk] = __builtin_amdgcn_ldexpf(1.f, -e);
+        if (piece == 0) factors[tk] = __builtin_bit_cast(float, (e - 14) << 23);
       }
     }
     return good;
@@ -240,7 +253,7 @@ struct Staging {
     if constexpr (!INT8) {
       good = split_rows<false>(c, to, s.ks[buf]);
 #pragma unroll
-      for (int i = 0; i < S::NP; ++i) good &= pages[i] >= 0 || stage * kStage + token(i) >= w.held;
+      for (int i = 0; i < S::NP; ++i) good &= (have >> i & 1) != 0 || stage * kStage + token(i) >= w.held;
     } else {
       const int piece = threadIdx.x & (S::kPieces - 1);
 #pragma unroll
@@ -253,9 +266,10 @@ struct Staging {
         if (tk < kStage) *reinterpret_cast<u4 *>(to + S::key_place(tk, piece)) = h;
       }
       const int tk = threadIdx.x & (kStage - 1);
-      const float y = pages[NE - 1] >= 0 ? scale : 0.f;
+      const bool in = (have >> (NE - 1) & 1) != 0;
+      const float y = in ? scale : 0.f;
       if (threadIdx.x < 2 * kStage) (threadIdx.x < kStage ? s.ks : s.vs)[buf][tk] = y;
-      good = !wild(y) && (pages[NE - 1] >= 0 || stage * kStage + tk >= w.held);
+      good = !wild(y) && (in || stage * kStage + tk >= w.held);
     }
     if (!good) s.plain[third] = 1;
   }
@@ -294,19 +308,23 @@ __device__ __forceinline__ void mma_keys(f16 &acc, const Terms &k, const Terms &
 }
 
 // Columns 32 b + c of 16 tokens, those of lane group g being 4 g .. + 3 and 8 + 4 g .. + 3: the order in which a
-// product leaves its results' rows.
+// product leaves its results' rows.  off: of the first tokens' first columns.
 template <bool INT8, int DP>
-__device__ __forceinline__ Terms values_of(const char *p, int token, int b, int lane) {
+__device__ __forceinline__ int values_place(int token, int lane) {
+  const int g = lane >> 5;
+  if constexpr (INT8) return ((token / 4 + g) * DP + (lane & 31)) * 8;
+  return Shape<INT8, DP>::value_place(token + 4 * g + (lane >> 2 & 3), 2 * (lane >> 4 & 1) + (lane >> 1 & 1)) + (lane & 1) * 8;
+}
+template <bool INT8, int DP>
+__device__ __forceinline__ Terms values_of(const char *p, int off, int st, int b) {
   using S = Shape<INT8, DP>;
   Terms t;
-  const int g = lane >> 5;
   if constexpr (INT8) {
-    const char *at = p + ((token / 4 + g) * DP + 32 * b + (lane & 31)) * 8;
+    const char *at = p + off + (4 * st * DP + 32 * b) * 8;
     const u2 lo = *reinterpret_cast<const u2 *>(at), hi = *reinterpret_cast<const u2 *>(at + 2 * DP * 8);
     t.h = t.m = __builtin_bit_cast(h8, u4{lo[0], lo[1], hi[0], hi[1]});
   } else {
-    const int tk = token + 4 * g + (lane >> 2 & 3), piece = 4 * b + 2 * (lane >> 4 & 1) + (lane >> 1 & 1);
-    const char *at = p + S::value_place(tk, piece) + (lane & 1) * 8;
+    const char *at = p + (off ^ 64 * b) + 16 * st * S::kRow;
     auto term = [](const char *at) {
       const auto a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tiles::lds_s4 *)at);
       const auto b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tiles::lds_s4 *)(at + 8 * S::kRow));
@@ -374,8 +392,9 @@ struct Rows {
   __device__ __forceinline__ void products(Lds<INT8, DP> &lds, int buf, int first, f16 &s) const {
     const int lane = threadIdx.x & 63, c = lane & 31, hi = lane >> 5;
     const char *keys = lds.stage(buf);
+    const int off = again(S::key_place(first + c, hi));
     auto ask = [&](int st) {
-      const char *p = keys + S::key_place(first + c, 2 * st + hi);
+      const char *p = keys + (off ^ 32 * st);
       Terms k;
       k.h = *reinterpret_cast<const h8 *>(p);
       if constexpr (!INT8) k.m = *reinterpret_cast<const h8 *>(p + kStage * S::kRow);
@@ -430,7 +449,8 @@ struct Rows {
     for (int e = 0; e < 16; ++e) x[e] = s[e];
     const Terms p[2] = {tiles::split8(x, lift), tiles::split8(x + 8, lift)};
     constexpr int kSteps = 2;  // of 16 tokens
-    Terms v = values_of<INT8, DP>(values, first, 0, lane);
+    const int off = again(values_place<INT8, DP>(first, lane));
+    Terms v = values_of<INT8, DP>(values, off, 0, 0);
 #pragma unroll
     for (int b = 0; b < S::NB; ++b) {
       f16 z = {};
@@ -438,7 +458,7 @@ struct Rows {
       for (int st = 0; st < kSteps; ++st) {
         const int nb = st + 1 < kSteps ? b : b + 1, ns = (st + 1) % kSteps;
         Terms next;
-        if (nb < S::NB) next = values_of<INT8, DP>(values, first + 16 * ns, nb, lane);
+        if (nb < S::NB) next = values_of<INT8, DP>(values, off, ns, nb);
         __builtin_amdgcn_sched_barrier(0);
         mma_keys<INT8>(z, v, p[st]);
         v = next;
@@ -571,8 +591,18 @@ __global__ void __launch_bounds__(kThreads, 2) walk_blocks(Args a) {
       // the lane's row, and what the wave's first and last see
       const int row = block * ROWS + 32 * rw + c;
       const bool live = row < rows;
-      const int token = live ? row / a.group : 0, head = kv * a.group + (live ? row % a.group : 0);
-      const int n_seen = live ? sees(t.len, end, walk.held, token) : 0;
+      // The token and head of the lane's row; formed again where they are needed.
+      auto token_of = [&](int &head) {
+        const int of = again(live ? row : 0), token = of / a.group;
+        head = kv * a.group + of - token * a.group;
+        return t.row0 + token;
+      };
+      auto query = [&] {
+        int head;
+        const int64_t at = token_of(head);
+        return a.q + at * a.ld_q + (int64_t)head * a.c.dh;
+      };
+      const int n_seen = live ? sees(t.len, end, walk.held, row / a.group) : 0;
       const int live_rows = min(32, rows - block * ROWS - 32 * rw);
       const int least = live_rows < 32 ? 0 : __builtin_amdgcn_readlane(n_seen, 0);
       const int most = live_rows > 0 ? __builtin_amdgcn_readlane(n_seen, live_rows - 1) : 0;
@@ -580,13 +610,12 @@ __global__ void __launch_bounds__(kThreads, 2) walk_blocks(Args a) {
       g.look(a.c, walk, s0);
       if (tid < 3) lds.plain[tid] = 0;
       Rows<INT8, DP> r;
-      const float *query = a.q + (int64_t)(t.row0 + token) * a.ld_q + (int64_t)head * a.c.dh;
-      r.start(a, query, live, n_seen);
-      g.resolve(a.c);
+      r.start(a, query(), live, n_seen);
+      g.resolve(a.c, walk, s0);
       __syncthreads();  // the marks are cleared, the last block's buffers free
-      g.load_keys(a.c, walk, s0);
+      g.load_keys(a.c);
       g.put_keys(lds, a.c, walk, s0, 0, 0);
-      g.load_values(a.c, walk, s0);
+      g.load_values(a.c);
       g.put_values(lds, a.c, 0, 0);
       g.look(a.c, walk, s0 + 1);
       for (int i = s0; i < s1; ++i) {
@@ -597,10 +626,10 @@ __global__ void __launch_bounds__(kThreads, 2) walk_blocks(Args a) {
         if (tid == 0) lds.plain[(i - s0 + 2) % 3] = 0;
         const int pos0 = i * kStage;
         if (more) {
-          g.resolve(a.c);
-          g.load_keys(a.c, walk, i + 1);
+          g.resolve(a.c, walk, i + 1);
+          g.load_keys(a.c);
         }
-        if (plain) r.take_plain(a, walk, query, pos0 + 32 * z, min(pos0 + 32 * z + kStage / Z, most));
+        if (plain) r.take_plain(a, walk, query(), pos0 + 32 * z, min(pos0 + 32 * z + kStage / Z, most));
         f16 s;
         auto products = [&](int first) {
           if (pos0 + first < most && !plain) r.products(lds, buf, first, s);
@@ -612,7 +641,7 @@ __global__ void __launch_bounds__(kThreads, 2) walk_blocks(Args a) {
         if constexpr (Z == 1) take(0);
         if (more) {
           g.put_keys(lds, a.c, walk, i + 1, buf ^ 1, after);
-          g.load_values(a.c, walk, i + 1);
+          g.load_values(a.c);
           g.look(a.c, walk, i + 2);
         }
         if constexpr (Z == 1) products(32);
@@ -663,7 +692,9 @@ __global__ void __launch_bounds__(kThreads, 2) walk_blocks(Args a) {
         float *to;
         float by = 1.f;
         if (whole) {
-          to = a.out + (int64_t)(t.row0 + token) * a.ld_out + (int64_t)head * a.c.dh;
+          int head;
+          const int64_t at = token_of(head);
+          to = a.out + at * a.ld_out + (int64_t)head * a.c.dh;
           by = 1.f / l;
         } else {
           // a workgroup has at most one part that begins its block (place 1) and one that does not
