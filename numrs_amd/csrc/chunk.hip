@@ -23,8 +23,7 @@ int run(numrs_hip_ctx *ctx, const Seqs &s, chunk::Args a) {
   a.cuts = reinterpret_cast<chunk::Cut *>(static_cast<char *>(parts.p) + image);
   chunk::walk_blocks<INT8, DP, Z><<<wgs, chunk::kThreads, 0, ctx->stream>>>(a);
   if (int rc = check_launch(ctx, "walk_blocks")) return rc;
-  const int rows = (int)std::min<int64_t>(ROWS, s.longest * a.group);
-  chunk::join_parts<DP, ROWS><<<dim3(wgs, std::min(rows, 64)), 256, 0, ctx->stream>>>(a);
+  chunk::join_parts<DP, ROWS><<<4 * wgs, 256, 0, ctx->stream>>>(a, (int)wgs);
   return check_launch(ctx, "join_parts");
 }
 

@@ -59,15 +59,23 @@ struct Args {
   int exp;
 };
 
-// Magnitudes within these bounds (or 0) cannot make a product leave fp32's range by themselves.  A stage with a
-// token beyond them, with one that is not finite, or on a page that the cache lacks, goes token by token in plain
-// fp32 (`take_plain`), and so does what a wave's rows see if one of their queries is beyond them.
+// Magnitudes within these bounds (or 0) cannot make a product leave fp32's range by themselves.  A workgroup's walk
+// that meets a token or a query beyond them, one that is not finite, or a page that the cache lacks, is given up and
+// made again in plain fp32, token by token (`take_plain`): some hundred times slower, and it does to each row
+// what fp32 arithmetic does.  (Such a stage alone in that form, within the walk, cost the ordinary ones their
+// registers.)
 constexpr float kSmall = 0x1p-60f, kLarge = 0x1p60f;
 __device__ __forceinline__ bool wild(float x) { return !(x == 0.f || (fabsf(x) >= kSmall && fabsf(x) <= kLarge)); }
 // The larger; NaN if one is.
 __device__ __forceinline__ float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }
-// Values from 2^96 on raise the softmax's reference, so that their sums stay below fp32's largest.
-constexpr int kRaise = 96;
+
+// A magnitude's exponent as its bits have it, 127 for [1, 2).  Tokens whose largest magnitude has one of base - kBelow
+// to base + 1 are split at the walk's base, which brings that to [2^13, 2^14) (so theirs to [2^5, 2^15), and the
+// split's smallest step to 2^-29 of it at most); others at their own, and have a factor.  Past kApart it is odd.
+constexpr unsigned kLow = 127 - 60, kHigh = 127 + 60, kBelow = 8, kApart = 64, kScaled = 13;
+__device__ __forceinline__ float power(unsigned bits) { return __builtin_bit_cast(float, bits << 23); }
+// What a stage's rows may be besides.
+enum : int { kOdd = 1, kMixedKeys = 2, kMixedValues = 4 };
 
 // Floats of a part: references and sums of a block's rows, then their outputs.
 template <int DP, int ROWS>
@@ -87,6 +95,8 @@ struct Shape {
   static constexpr int kKeys = kTerms * kStage * kRow;
   static constexpr int kValues = INT8 ? kStage * DP * 2 : kKeys;
   static constexpr int kBytes = kKeys + kValues;  // of a stage
+  // steps whose queries' second terms lie in LDS: what registers lack for heads above 96
+  static constexpr int kKept = DP > 96 ? 3 : 0;
   static constexpr int kQuads = kStage / 4 * (DP / 4), NV = (kQuads + kThreads - 1) / kThreads;
 
   // (A piece 2 st + hi of keys is at the piece hi's place ^ 32 st, a piece 4 b + x of values at x's ^ 64 b.)
@@ -119,14 +129,21 @@ struct Lds {
   static constexpr int kJoint = 64 * (16 * S::NB + 4) * 4;  // a wave's results, while sets are joined
   // (the stages last: an LDS access has 16 bits for a constant offset)
   float ks[2][kStage], vs[2][kStage];  // the rows' factors
-  int plain[4];                        // of three stages in turn: one is read, one written, one cleared
-  char stages[2 * S::kBytes > 4 * kJoint ? 2 * S::kBytes : 4 * kJoint];
+  int marks[3];                        // of three stages in turn: one is read, one written, one cleared
+  unsigned base[2];                    // the walk's, of keys and of values
+  char kept[8][S::kKept > 0 ? S::kKept : 1][1024] __attribute__((aligned(256)));  // of each wave's queries
+  char stages[2 * S::kBytes > 4 * kJoint ? 2 * S::kBytes : 4 * kJoint] __attribute__((aligned(256)));
   __device__ __forceinline__ char *stage(int buf) { return stages + buf * S::kBytes; }
 };
 
 // The same value, formed again: what follows from it is not kept in registers around a loop.
 __device__ __forceinline__ int again(int v) {
   asm volatile("" : "+v"(v));
+  return v;
+}
+
+__device__ __forceinline__ int again_scalar(int v) {
+  asm volatile("" : "+s"(v));
   return v;
 }
 
@@ -141,142 +158,187 @@ __device__ __forceinline__ int64_t token_row(const Cache &c, int kv, int pos, in
   return paging::page_base(page, c.kv_heads, kv, c.shift, 1) + (pos & ((1 << c.shift) - 1));
 }
 
-// A thread's share of a stage on its way from the cache to LDS.
-template <bool INT8, int DP>
+// A thread's share of a stage on its way from the cache to LDS.  BOTH: keys and values are asked for at once, else
+// one after the other.
+template <bool INT8, int DP, bool BOTH>
 struct Staging {
   using S = Shape<INT8, DP>;
-  static constexpr int NE = INT8 ? S::NP + S::NV + 1 : S::NP;  // places whose pages it needs
-  int32_t entries[NE];
-  int64_t at[NE];  // the element of the cache that the thread loads first, of a factor its place
-  unsigned have;   // places that the cache has, a bit each
-  f4 x[INT8 ? 1 : S::NP][2];
+  // places whose pages it needs: rows; in 8 bits also quads of values, a factor
+  static constexpr int NE = INT8 ? S::NP + S::NV + 1 : S::NP;
+  int32_t entries[NE];  // the places' pages, -1: the cache has none
+  bool whole;      // of the wave's places all are, and all of its columns the head's
+  f4 x[INT8 ? 1 : BOTH ? 2 : 1][INT8 ? 1 : S::NP][2];
   u2 kc[INT8 ? S::NP : 1];
   u4 vc[INT8 ? S::NV : 1];
   float scale;
 
-  // The token of a place within its stage: a row's, a quad's first, or a factor's.
-  static __device__ __forceinline__ int token(int i) {
-    const int tid = threadIdx.x;
+  // The token of a place within its stage.
+  static __device__ __forceinline__ int token(int tid, int i) {
     if (i < S::NP) return i * S::kPass + (tid >> S::kLanes);  // (past the stage where it has fewer rows than threads)
-    if (i < S::NP + (INT8 ? S::NV : 0)) return min(((i - S::NP) * kThreads + tid) / (DP / 4), kStage / 4 - 1) * 4;
+    if (i < NE - 1) return min(((i - S::NP) * kThreads + tid) / (DP / 4), kStage / 4 - 1) * 4;
     return tid & (kStage - 1);
   }
+  static __device__ __forceinline__ int row_column(int tid) { return 8 * (tid & (S::kPieces - 1)); }
+  static __device__ __forceinline__ int quad_column(int tid, int i) { return 4 * ((i * kThreads + tid) % (DP / 4)); }
   __device__ __forceinline__ void look(const Cache &c, const Walk &w, int stage) {
+    const int tid = again(threadIdx.x);
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
-      const int pos = stage * kStage + token(i);
+      const int pos = stage * kStage + token(tid, i);
       entries[i] = pos < w.held ? paging::entry_of(w.pages, c.max_pages, c.shift, pos) : -1;
     }
   }
-  static __device__ __forceinline__ int row_column(const Cache &c) { return 8 * (threadIdx.x & (S::kPieces - 1)); }
   // Loads go out whatever the place is, from the cache's first page where it is none, and are dropped then: what
   // lies in slots of no token must not reach the products.
-  __device__ __forceinline__ void resolve(const Cache &c, const Walk &w, int stage) {
-    have = 0;
+  __device__ __forceinline__ void resolve(const Cache &c) {
+    const int tid = again(threadIdx.x);
+    bool all = row_column(tid) < c.dh;
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
-      const int page = paging::page_in(entries[i], c.pages);
-      have |= page >= 0 ? 1u << i : 0u;
-      at[i] = token_row(c, w.kv, stage * kStage + token(i), max(page, 0));
-      if (i < S::NP)
-        at[i] = at[i] * c.dh + min(row_column(c), c.dh - 8);
-      else if (i < NE - 1)
-        at[i] = at[i] * c.dh + 4 * min(4 * (((i - S::NP) * kThreads + (int)threadIdx.x) % (DP / 4)), c.dh - 4);
+      entries[i] = paging::page_in(entries[i], c.pages);
+      all &= entries[i] >= 0;
     }
+    whole = __all(all);
+  }
+  // The element that a place's load begins at, of a factor its place.
+  __device__ __forceinline__ int64_t at(const Cache &c, const Walk &w, int stage, int i) const {
+    const int tid = again(threadIdx.x);
+    // (page * kv_heads + kv) * page size + slot: a factor of 32 bits, so one multiplication
+    const uint32_t slot = (uint32_t)(stage * kStage + token(tid, i)) & ((1u << c.shift) - 1);
+    const uint64_t row = (uint64_t)(uint32_t)max(entries[i], 0) * ((uint32_t)c.kv_heads << c.shift) +
+                         (((uint32_t)w.kv << c.shift) + slot);
+    if (INT8 && i == NE - 1) return (int64_t)row;
+    return (int64_t)(row * (uint32_t)c.dh + (uint32_t)(i < S::NP ? min(row_column(tid), c.dh - 8) : 4 * min(quad_column(tid, i - S::NP), c.dh - 4)));
   }
   // fp32 rows of keys or values: a thread's eight columns.
-  __device__ __forceinline__ void load_rows(const void *from) {
+  __device__ __forceinline__ void load_rows(const Cache &c, const Walk &w, int stage, const void *from, int which) {
 #pragma unroll
     for (int i = 0; i < S::NP; ++i) {
-      const float *p = static_cast<const float *>(from) + at[i];
-      x[i][0] = *reinterpret_cast<const f4 *>(p), x[i][1] = *reinterpret_cast<const f4 *>(p + 4);
+      const float *p = static_cast<const float *>(from) + at(c, w, stage, i);
+      x[which][i][0] = *reinterpret_cast<const f4 *>(p), x[which][i][1] = *reinterpret_cast<const f4 *>(p + 4);
     }
   }
-  __device__ __forceinline__ void load_keys(const Cache &c) {
+  __device__ __forceinline__ void load_keys(const Cache &c, const Walk &w, int stage) {
     if constexpr (!INT8) {
-      load_rows(c.k);
+      load_rows(c, w, stage, c.k, 0);
     } else {
 #pragma unroll
-      for (int i = 0; i < S::NP; ++i) kc[i] = *reinterpret_cast<const u2 *>(static_cast<const uint8_t *>(c.k) + at[i]);
-      scale = (threadIdx.x & kStage ? c.vs : c.ks)[at[NE - 1]];
+      for (int i = 0; i < S::NP; ++i)
+        kc[i] = *reinterpret_cast<const u2 *>(static_cast<const uint8_t *>(c.k) + at(c, w, stage, i));
+      scale = (threadIdx.x & kStage ? c.vs : c.ks)[at(c, w, stage, NE - 1)];
     }
   }
-  __device__ __forceinline__ void load_values(const Cache &c) {
+  __device__ __forceinline__ void load_values(const Cache &c, const Walk &w, int stage) {
     if constexpr (!INT8) {
-      load_rows(c.v);
+      load_rows(c, w, stage, c.v, BOTH);
     } else {
 #pragma unroll
       for (int i = 0; i < S::NV; ++i)
-        vc[i] = *reinterpret_cast<const u4 *>(static_cast<const uint8_t *>(c.v) + at[S::NP + i]);
+        vc[i] = *reinterpret_cast<const u4 *>(static_cast<const uint8_t *>(c.v) + at(c, w, stage, S::NP + i));
+    }
+  }
+  // What lies in no token's slot, and past the head, becomes zeros.
+  template <bool VALUES>
+  __device__ __forceinline__ void drop(const Cache &c, const Walk &w, int stage) {
+    if (whole) return;
+    const int tid = again(threadIdx.x);
+#pragma unroll
+    for (int i = 0; i < S::NP; ++i) {
+      const bool in = stage * kStage + token(tid, i) < w.held && row_column(tid) < c.dh;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[BOTH && VALUES][i][j >> 2][j & 3] = in ? x[BOTH && VALUES][i][j >> 2][j & 3] : 0.f;
+    }
+  }
+  // The bits of a row's largest magnitude, in all of its lanes.
+  template <bool VALUES>
+  __device__ __forceinline__ unsigned top_of_row(int i) const {
+    const f4(&v)[2] = x[BOTH && VALUES][i];
+    float big = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) big = maximum(maximum(big, fabsf(v[j >> 2][j & 3])), fabsf(v[j >> 2][(j & 3) + 1]));
+    return row_top<S::kLanes>(__builtin_bit_cast(unsigned, big));
+  }
+  // Raises the walk's base to the largest exponent of these rows.
+  template <bool VALUES>
+  __device__ __forceinline__ void raise_base(Lds<INT8, DP> &s, const Cache &c, const Walk &w, int stage) {
+    if constexpr (!INT8) {
+      drop<VALUES>(c, w, stage);
+      unsigned e = kLow;
+#pragma unroll
+      for (int i = 0; i < S::NP; ++i) e = max(e, min(top_of_row<VALUES>(i) >> 23, kHigh));
+      atomicMax(&s.base[VALUES], e);
     }
   }
 
-  // Rows in fp32 into two terms; whether all of them are ordinary.
+  // Rows in fp32 into two terms; returns their marks.
   template <bool VALUES>
-  __device__ __forceinline__ bool split_rows(const Cache &c, char *to, float *factors) {
-    const int piece = threadIdx.x & (S::kPieces - 1);
-    bool good = true;
+  __device__ __forceinline__ int split_rows(const Cache &c, const Walk &w, int stage, char *to, float *factors, unsigned base) {
+    const int tid = again(threadIdx.x);
+    const int piece = tid & (S::kPieces - 1);
+    bool odd = false, mixed = false;
+    drop<VALUES>(c, w, stage);
 #pragma unroll
     for (int i = 0; i < S::NP; ++i) {
-      const int tk = token(i);
-      const bool in = (have >> i & 1) != 0 && row_column(c) < c.dh;
-      if (__any(!in)) {
+      const int tk = token(tid, i);
+      const unsigned top = top_of_row<VALUES>(i), e = top >> 23;
+      const bool near = e - (base - kBelow) <= kBelow + 1 || top == 0;
+      odd |= !near && (e < kLow || e >= kHigh || e - (base - kApart) > 2 * kApart);
+      mixed |= !near;
+      const unsigned own = near ? base : e;
+      float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[i][j >> 2][j & 3] = in ? x[i][j >> 2][j & 3] : 0.f;
-      }
-      float v[8], big = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = x[i][j >> 2][j & 3];
-#pragma unroll
-      for (int j = 0; j < 8; j += 2) big = maximum(maximum(big, fabsf(v[j])), fabsf(v[j + 1]));
-      const unsigned top = row_top<S::kLanes>(__builtin_bit_cast(unsigned, big));
-      // The power of two that puts the largest into [2^14, 2^15), from its exponent's bits; within the bounds
-      // neither it nor its inverse leaves the normal numbers (and beyond them the split is not used).
-      constexpr unsigned kLow = 127 - 60, kHigh = 127 + 60;
-      const unsigned e = max(top >> 23, kLow);
-      good &= e < kHigh && (top >> 23 >= kLow || top == 0);
-      const Terms t = tiles::split8(v, __builtin_bit_cast(float, (268 - e) << 23));
-      if (tk < kStage) {
+      for (int j = 0; j < 8; ++j) v[j] = x[BOTH && VALUES][i][j >> 2][j & 3];
+      const Terms t = tiles::split8(v, power(kScaled + 2 * 127 - own));
+      if (S::kPass <= kStage || tk < kStage) {
         char *p = to + (VALUES ? S::value_place(tk, piece) : S::key_place(tk, piece));
         *reinterpret_cast<h8 *>(p) = t.h;
         *reinterpret_cast<h8 *>(p + kStage * S::kRow) = t.m;
-        if (piece == 0) factors[tk] = __builtin_bit_cast(float, (e - 14) << 23);
+        if (piece == 0) factors[tk] = power(127 + own - base);
       }
     }
-    return good;
+    return (odd ? kOdd : 0) | (mixed ? VALUES ? kMixedValues : kMixedKeys : 0);
+  }
+  static __device__ __forceinline__ void mark(int *to, int marks) {
+    if (marks != 0) atomicOr(to, marks);
   }
 
   // stage: the one that is written, of the block's walk, and its buffers.
-  __device__ __forceinline__ void put_keys(Lds<INT8, DP> &s, const Cache &c, const Walk &w, int stage, int buf, int third) {
+  __device__ __forceinline__ void put_keys(Lds<INT8, DP> &s, const Cache &c, const Walk &w, int stage, int buf, int third,
+                                           unsigned base) {
+    const int tid = again(threadIdx.x);
     char *to = s.stage(buf);
-    bool good = true;
+    int marks = 0;
     if constexpr (!INT8) {
-      good = split_rows<false>(c, to, s.ks[buf]);
-#pragma unroll
-      for (int i = 0; i < S::NP; ++i) good &= (have >> i & 1) != 0 || stage * kStage + token(i) >= w.held;
+      marks = split_rows<false>(c, w, stage, to, s.ks[buf], base);
     } else {
-      const int piece = threadIdx.x & (S::kPieces - 1);
+      const int piece = tid & (S::kPieces - 1);
 #pragma unroll
       for (int i = 0; i < S::NP; ++i) {
-        const int tk = token(i);
+        const int tk = token(tid, i);
         u4 h;
         unsigned lo, hi;
         paged::halves(kc[i][0], lo, hi), h[0] = lo, h[1] = hi;
         paged::halves(kc[i][1], lo, hi), h[2] = lo, h[3] = hi;
-        if (tk < kStage) *reinterpret_cast<u4 *>(to + S::key_place(tk, piece)) = h;
+        if (S::kPass <= kStage || tk < kStage) *reinterpret_cast<u4 *>(to + S::key_place(tk, piece)) = h;
       }
-      const int tk = threadIdx.x & (kStage - 1);
-      const bool in = (have >> (NE - 1) & 1) != 0;
-      const float y = in ? scale : 0.f;
-      if (threadIdx.x < 2 * kStage) (threadIdx.x < kStage ? s.ks : s.vs)[buf][tk] = y;
-      good = !wild(y) && (in || stage * kStage + tk >= w.held);
+      const float y = entries[NE - 1] >= 0 ? scale : 0.f;
+      if (threadIdx.x < 2 * kStage) {
+        (threadIdx.x < kStage ? s.ks : s.vs)[buf][threadIdx.x & (kStage - 1)] = y;
+        if (wild(y)) marks = kOdd;
+      }
     }
-    if (!good) s.plain[third] = 1;
+    if (!whole) {  // a token of the sequence on a page that the cache lacks
+#pragma unroll
+      for (int i = 0; i < S::NP; ++i)
+        if (entries[i] < 0 && stage * kStage + token(tid, i) < w.held) marks |= kOdd;
+    }
+    mark(&s.marks[third], marks);
   }
-  __device__ __forceinline__ void put_values(Lds<INT8, DP> &s, const Cache &c, int buf, int third) {
+  __device__ __forceinline__ void put_values(Lds<INT8, DP> &s, const Cache &c, const Walk &w, int stage, int buf, int third,
+                                             unsigned base) {
     char *to = s.stage(buf) + S::kKeys;
     if constexpr (!INT8) {
-      if (!split_rows<true>(c, to, s.vs[buf])) s.plain[third] = 1;
+      mark(&s.marks[third], split_rows<true>(c, w, stage, to, s.vs[buf], base));
     } else {
       // four tokens' values of a column lie together: eight bytes of a product's operand
 #pragma unroll
@@ -316,23 +378,18 @@ __device__ __forceinline__ int values_place(int token, int lane) {
   return Shape<INT8, DP>::value_place(token + 4 * g + (lane >> 2 & 3), 2 * (lane >> 4 & 1) + (lane >> 1 & 1)) + (lane & 1) * 8;
 }
 template <bool INT8, int DP>
-__device__ __forceinline__ Terms values_of(const char *p, int off, int st, int b) {
+__device__ __forceinline__ h8 values_term(const char *p, int off, int st, int b, int term) {
   using S = Shape<INT8, DP>;
-  Terms t;
   if constexpr (INT8) {
     const char *at = p + off + (4 * st * DP + 32 * b) * 8;
     const u2 lo = *reinterpret_cast<const u2 *>(at), hi = *reinterpret_cast<const u2 *>(at + 2 * DP * 8);
-    t.h = t.m = __builtin_bit_cast(h8, u4{lo[0], lo[1], hi[0], hi[1]});
+    return __builtin_bit_cast(h8, u4{lo[0], lo[1], hi[0], hi[1]});
   } else {
-    const char *at = p + (off ^ 64 * b) + 16 * st * S::kRow;
-    auto term = [](const char *at) {
-      const auto a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tiles::lds_s4 *)at);
-      const auto b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tiles::lds_s4 *)(at + 8 * S::kRow));
-      return __builtin_bit_cast(h8, tiles::s8(__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7)));
-    };
-    t.h = term(at), t.m = term(at + kStage * S::kRow);
+    const char *at = p + (off ^ 64 * b) + 16 * st * S::kRow + term * kStage * S::kRow;
+    const auto a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tiles::lds_s4 *)at);
+    const auto b4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tiles::lds_s4 *)(at + 8 * S::kRow));
+    return __builtin_bit_cast(h8, tiles::s8(__builtin_shufflevector(a, b4, 0, 1, 2, 3, 4, 5, 6, 7)));
   }
-  return t;
 }
 
 // A cached key or value.
@@ -355,27 +412,34 @@ struct Rows {
   Terms q[S::NS];
   float o[S::NB][16];
   float m, l;   // l: of the lane's own half of the tokens
-  float f;      // log2(e) / sqrt(dh) over the query's factor, a power of two
-  int seen;     // tokens that the lane's row sees; 0: none
-  bool some;    // of them in the cache so far
-  bool plain;   // a query of the wave is beyond the bounds
+  int fe;       // log2(e) / sqrt(dh) over the query's factor is a power of two, this one
+  float f;      // and with the keys' base
 
-  __device__ __forceinline__ void start(const Args &a, const float *row, bool live, int sees) {
-    const int hi = (threadIdx.x & 63) >> 5;
-    seen = sees, some = false;
-    tiles::RowValues<DP> x;
-    x.load(row, live, a.c.dh, hi);
-    bool not_finite = false;
-    const float top = x.top(INFINITY, not_finite);
-    const int e = tiles::exponent_for(top);
-    f = __builtin_amdgcn_ldexpf(1.f, a.exp - e);
-    plain = __any(not_finite || wild(top));
-    x.split_into(q, __builtin_amdgcn_ldexpf(a.mant, e));
+  __device__ __forceinline__ void clear() {
     m = kNever, l = 0.f;
 #pragma unroll
     for (int b = 0; b < S::NB; ++b)
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[b][e] = 0.f;
+  }
+  static __device__ __forceinline__ char *kept(Lds<INT8, DP> &lds, int st) {
+    const int tid = again(threadIdx.x);
+    return lds.kept[tid >> 6][st - (S::NS - S::kKept)] + (tid & 63) * 16;
+  }
+  // Returns whether the row's query is ordinary.
+  __device__ __forceinline__ bool start(const Args &a, Lds<INT8, DP> &lds, const float *row, bool live) {
+    const int hi = (threadIdx.x & 63) >> 5;
+    tiles::RowValues<DP> x;
+    x.load(row, live, again_scalar(a.c.dh), hi);
+    bool not_finite = false;
+    const float top = x.top(INFINITY, not_finite);
+    const int e = tiles::exponent_for(top);
+    fe = a.exp - e;
+    x.split_into(q, __builtin_amdgcn_ldexpf(a.mant, e));
+#pragma unroll
+    for (int st = S::NS - S::kKept; st < S::NS; ++st) *reinterpret_cast<h8 *>(kept(lds, st)) = q[st].m;
+    clear();
+    return !(not_finite || wild(top));
   }
 
   __device__ __forceinline__ void raise(float now) {
@@ -388,80 +452,119 @@ struct Rows {
       for (int e = 0; e < 16; ++e) o[b][e] *= r;
   }
 
-  // 32 tokens from `first` of a stage: the products of their keys ...
-  __device__ __forceinline__ void products(Lds<INT8, DP> &lds, int buf, int first, f16 &s) const {
-    const int lane = threadIdx.x & 63, c = lane & 31, hi = lane >> 5;
+  // KB blocks of 32 tokens from `first` of a stage: the products of their keys ...
+  template <int KB>
+  __device__ __forceinline__ void products(Lds<INT8, DP> &lds, int buf, int first, f16 (&s)[KB]) const {
+    const int lane = again(threadIdx.x & 63), off = again(S::key_place(first + (lane & 31), lane >> 5));
     const char *keys = lds.stage(buf);
-    const int off = again(S::key_place(first + c, hi));
-    auto ask = [&](int st) {
-      const char *p = keys + (off ^ 32 * st);
+    auto ask = [&](int n) {  // of step n / KB, block n % KB
+      const char *p = keys + (off ^ 32 * (n / KB)) + n % KB * 32 * S::kRow;
       Terms k;
       k.h = *reinterpret_cast<const h8 *>(p);
       if constexpr (!INT8) k.m = *reinterpret_cast<const h8 *>(p + kStage * S::kRow);
       return k;
     };
-    Terms k = ask(0);
-    s = f16{};
+    auto query = [&](int st) {
+      Terms t = q[st];
+      if (st >= S::NS - S::kKept) t.m = *reinterpret_cast<const h8 *>(kept(lds, st));
+      return t;
+    };
+    constexpr int kAll = S::NS * KB;
+    Terms k = ask(0), now = query(0);
 #pragma unroll
-    for (int st = 0; st < S::NS; ++st) {
+    for (int kb = 0; kb < KB; ++kb) s[kb] = f16{};
+#pragma unroll
+    for (int n = 0; n < kAll; ++n) {
       Terms next;
-      if (st + 1 < S::NS) next = ask(st + 1);
+      if (n + 1 < kAll) next = ask(n + 1);
       __builtin_amdgcn_sched_barrier(0);  // the next step's operands are asked for before this one's products
-      mma_keys<INT8>(s, k, q[st]);
+      mma_keys<INT8>(s[n % KB], k, now);
       k = next;
+      if (n % KB == KB - 1 && n + 1 < kAll) now = query(n / KB + 1);
     }
   }
 
   // ... and what follows from them; the stage's tokens begin at pos0.
-  __device__ __forceinline__ void take(Lds<INT8, DP> &lds, int buf, int first, int pos0, bool masked, f16 &s) {
-    const int lane = threadIdx.x & 63, hi = lane >> 5;
+  // seen(): the tokens that the lane's row sees.
+  template <int KB, class Seen>
+  __device__ __forceinline__ void take(Lds<INT8, DP> &lds, int buf, int first, int pos0, bool masked, int marks,
+                                       int values_base, f16 (&s)[KB], Seen &&seen) {
+    const int hi = again(threadIdx.x & 63) >> 5;
     const char *values = lds.stage(buf) + S::kKeys;
     // factors of the rows that a lane's results are, four at a time
     auto by_factors = [&](const float *factors) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f4 x = *reinterpret_cast<const f4 *>(factors + first + 8 * i + 4 * hi);
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[4 * i + j] *= x[j];
-      }
+        for (int i = 0; i < 4; ++i) {
+          const f4 x = *reinterpret_cast<const f4 *>(factors + first + 32 * kb + 8 * i + 4 * hi);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[kb][4 * i + j] *= x[j];
+        }
     };
-    by_factors(lds.ks[buf]);
-    const int left = seen - pos0 - first;  // tokens from the first that the row sees
+    if (INT8 || (marks & kMixedKeys)) by_factors(lds.ks[buf]);
     if (masked) {
+      const int left = seen() - pos0 - first;  // tokens from the first that the row sees
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (tiles::out_row(e, hi) >= left) s[e] = -INFINITY;
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (32 * kb + tiles::out_row(e, hi) >= left) s[kb][e] = -INFINITY;
     }
-    some |= left > 0;
-    const float most = half_pair(tiles::over16(s, [](float x, float y) { return fmaxf(x, y); }),
-                                 [](float x, float y) { return fmaxf(x, y); }) * f;
+    float most = s[0][0];
+#pragma unroll
+    for (int n = 1; n + 1 < 16 * KB; n += 2) most = maximum(maximum(most, s[n / 16][n % 16]), s[(n + 1) / 16][(n + 1) % 16]);
+    most = maximum(most, s[KB - 1][15]);
+    most = half_pair(most, [](float x, float y) { return maximum(x, y); }) * f;
     if (__any(most > m + 8.f)) raise(fmaxf(m, most));
+    float sums[2] = {0.f, 0.f};
 #pragma unroll
-    for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], f, -m));
-    l += tiles::over16(s, [](float x, float y) { return x + y; });
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[kb][e] = __builtin_amdgcn_exp2f(fmaf(s[kb][e], f, -m));
+        sums[e & 1] += s[kb][e];
+      }
+    l += sums[0] + sums[1];
     // the probabilities times the values' factors, the largest of a row brought to [2^14, 2^15)
-    by_factors(lds.vs[buf]);
-    const float top = half_pair(tiles::top_of(s, 0.f), [](float x, float y) { return fmaxf(x, y); });
-    const int et = max(__builtin_amdgcn_frexp_expf(top), -100);
-    const float lift = __builtin_amdgcn_ldexpf(1.f, 15 - et), back = __builtin_amdgcn_ldexpf(1.f, et - 15);
-    float x[16];
+    float top;
+    if (INT8 || (marks & kMixedValues)) {
+      by_factors(lds.vs[buf]);
+      top = 0.f;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] = s[e];
-    const Terms p[2] = {tiles::split8(x, lift), tiles::split8(x + 8, lift)};
-    constexpr int kSteps = 2;  // of 16 tokens
-    const int off = again(values_place<INT8, DP>(first, lane));
-    Terms v = values_of<INT8, DP>(values, off, 0, 0);
+      for (int kb = 0; kb < KB; ++kb) top = tiles::top_of(s[kb], top);
+      top = half_pair(top, [](float x, float y) { return fmaxf(x, y); });
+    } else {
+      top = __builtin_amdgcn_exp2f(most - m);
+    }
+    const int et = max(__builtin_amdgcn_frexp_expf(top), -100);
+    const float lift = __builtin_amdgcn_ldexpf(1.f, 15 - et), back = __builtin_amdgcn_ldexpf(1.f, et - 15 + values_base);
+    Terms p[KB][2];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      float x[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] = s[kb][e];
+      p[kb][0] = tiles::split8(x, lift), p[kb][1] = tiles::split8(x + 8, lift);
+    }
+    const int off = again(values_place<INT8, DP>(first, again(threadIdx.x & 63)));
+    constexpr int kSteps = 2 * KB;  // of 16 tokens
+    h8 h = values_term<INT8, DP>(values, off, 0, 0, 0);
 #pragma unroll
     for (int b = 0; b < S::NB; ++b) {
       f16 z = {};
 #pragma unroll
       for (int st = 0; st < kSteps; ++st) {
         const int nb = st + 1 < kSteps ? b : b + 1, ns = (st + 1) % kSteps;
-        Terms next;
-        if (nb < S::NB) next = values_of<INT8, DP>(values, off, ns, nb);
+        const Terms &w = p[st >> 1][st & 1];
+        h8 low, next;
+        if constexpr (!INT8) low = values_term<INT8, DP>(values, off, st, b, 1);
+        if (nb < S::NB) next = values_term<INT8, DP>(values, off, ns, nb, 0);
         __builtin_amdgcn_sched_barrier(0);
-        mma_keys<INT8>(z, v, p[st]);
-        v = next;
+        z = __builtin_amdgcn_mfma_f32_32x32x16_f16(h, w.m, z, 0, 0, 0);
+        if constexpr (!INT8) z = __builtin_amdgcn_mfma_f32_32x32x16_f16(low, w.h, z, 0, 0, 0);
+        z = __builtin_amdgcn_mfma_f32_32x32x16_f16(h, w.h, z, 0, 0, 0);
+        h = next;
       }
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[b][e] = fmaf(z[e], back, o[b][e]);
@@ -470,7 +573,9 @@ struct Rows {
 
   // The same in plain fp32, a token after the other: a lane forms half of its row's score, and adds to its columns
   // of the result.  What is not finite does what it does in fp32, and only to the rows that see it.
-  __device__ __forceinline__ void take_plain(const Args &a, const Walk &w, const float *row, int from, int to) {
+  // Returns whether the row sees any of them.
+  __device__ __forceinline__ bool take_plain(const Args &a, const Walk &w, const float *row, int seen, int from, int to) {
+    bool some = false;
     const int hi = (threadIdx.x & 63) >> 5, half = (a.c.dh / 8 + 1) / 2 * 8;
     const float scale = __builtin_amdgcn_ldexpf(a.mant, a.exp);
 #pragma unroll 1
@@ -505,6 +610,7 @@ struct Rows {
         }
       }
     }
+    return some;
   }
 };
 
@@ -522,7 +628,7 @@ __device__ __forceinline__ int stages_of(const Cache &c, int group, int len, int
 template <bool INT8, int DP, int Z>
 __global__ void __launch_bounds__(kThreads, 2) walk_blocks(Args a) {
   using S = Shape<INT8, DP>;
-  constexpr int R = 8 / Z, ROWS = 32 * R;
+  constexpr int R = 8 / Z, ROWS = 32 * R, KB = 2 / Z;
   __shared__ __attribute__((aligned(16))) Lds<INT8, DP> lds;
   __shared__ int64_t pre[kThreads + 1], sums[8];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -602,51 +708,68 @@ __global__ void __launch_bounds__(kThreads, 2) walk_blocks(Args a) {
         const int64_t at = token_of(head);
         return a.q + at * a.ld_q + (int64_t)head * a.c.dh;
       };
-      const int n_seen = live ? sees(t.len, end, walk.held, row / a.group) : 0;
+      auto row_sees = [&] { return live ? sees(t.len, end, walk.held, again(row) / a.group) : 0; };
+      const int n_seen = row_sees();
       const int live_rows = min(32, rows - block * ROWS - 32 * rw);
       const int least = live_rows < 32 ? 0 : __builtin_amdgcn_readlane(n_seen, 0);
       const int most = live_rows > 0 ? __builtin_amdgcn_readlane(n_seen, live_rows - 1) : 0;
-      Staging<INT8, DP> g;
-      g.look(a.c, walk, s0);
-      if (tid < 3) lds.plain[tid] = 0;
+      constexpr bool kBoth = INT8 || Z > 1;
+      Staging<INT8, DP, kBoth> g;
       Rows<INT8, DP> r;
-      r.start(a, query(), live, n_seen);
-      g.resolve(a.c, walk, s0);
-      __syncthreads();  // the marks are cleared, the last block's buffers free
-      g.load_keys(a.c);
-      g.put_keys(lds, a.c, walk, s0, 0, 0);
-      g.load_values(a.c);
-      g.put_values(lds, a.c, 0, 0);
+      g.look(a.c, walk, s0);
+      if (tid < 3) lds.marks[tid] = 0;
+      if (tid < 2) lds.base[tid] = kLow;
+      const bool good = r.start(a, lds, query(), live);
+      g.resolve(a.c);
+      __syncthreads();  // what is marked is cleared, the last block's buffers free
+      if (!good) Staging<INT8, DP, kBoth>::mark(&lds.marks[0], kOdd);
+      g.load_keys(a.c, walk, s0);
+      g.template raise_base<false>(lds, a.c, walk, s0);
+      __syncthreads();
+      const unsigned kbase = __builtin_amdgcn_readfirstlane(lds.base[0]);
+      g.put_keys(lds, a.c, walk, s0, 0, 0, kbase);
+      g.load_values(a.c, walk, s0);
+      g.template raise_base<true>(lds, a.c, walk, s0);
+      __syncthreads();
+      const unsigned vbase = __builtin_amdgcn_readfirstlane(lds.base[1]);
+      g.put_values(lds, a.c, walk, s0, 0, 0, vbase);
       g.look(a.c, walk, s0 + 1);
+      constexpr int kUnscale = INT8 ? 0 : 127 + (int)kScaled;
+      r.f = __builtin_amdgcn_ldexpf(1.f, r.fe + (INT8 ? 0 : (int)kbase - kUnscale));
+      const int values_base = INT8 ? 0 : (int)vbase - kUnscale;
+      bool odd = false;
       for (int i = s0; i < s1; ++i) {
         const int buf = (i - s0) & 1, third = (i - s0) % 3, after = (i - s0 + 1) % 3;
+        const int pos0 = i * kStage, first = 32 * z;
         const bool more = i + 1 < s1;
         __syncthreads();
-        const bool plain = __builtin_amdgcn_readfirstlane(lds.plain[third]) != 0 || r.plain;
-        if (tid == 0) lds.plain[(i - s0 + 2) % 3] = 0;
-        const int pos0 = i * kStage;
+        const int marks = __builtin_amdgcn_readfirstlane(lds.marks[third]);
+        odd = (marks & kOdd) != 0;
+        if (odd) break;
+        if (tid == 0) lds.marks[(i - s0 + 2) % 3] = 0;
         if (more) {
-          g.resolve(a.c, walk, i + 1);
-          g.load_keys(a.c);
+          g.resolve(a.c);
+          g.load_keys(a.c, walk, i + 1);
+          if constexpr (kBoth) g.load_values(a.c, walk, i + 1);
         }
-        if (plain) r.take_plain(a, walk, query(), pos0 + 32 * z, min(pos0 + 32 * z + kStage / Z, most));
-        f16 s;
-        auto products = [&](int first) {
-          if (pos0 + first < most && !plain) r.products(lds, buf, first, s);
-        };
-        auto take = [&](int first) {
-          if (pos0 + first < most && !plain) r.take(lds, buf, first, pos0, pos0 + first + 32 > least, s);
-        };
-        products(32 * z);
-        if constexpr (Z == 1) take(0);
+        const bool mine = pos0 + first < most;
+        f16 s[KB];
+        if (mine) r.template products<KB>(lds, buf, first, s);
         if (more) {
-          g.put_keys(lds, a.c, walk, i + 1, buf ^ 1, after);
-          g.load_values(a.c);
+          g.put_keys(lds, a.c, walk, i + 1, buf ^ 1, after, kbase);
+          if constexpr (!kBoth) g.load_values(a.c, walk, i + 1);
           g.look(a.c, walk, i + 2);
         }
-        if constexpr (Z == 1) products(32);
-        take(Z == 1 ? 32 : 32 * z);
-        if (more) g.put_values(lds, a.c, buf ^ 1, after);
+        if (mine) r.template take<KB>(lds, buf, first, pos0, pos0 + first + 32 * KB > least, marks, values_base, s, row_sees);
+        if (more) g.put_values(lds, a.c, walk, i + 1, buf ^ 1, after, vbase);
+      }
+      bool some = row_sees() > s0 * kStage + 32 * z;  // whether the row sees a token of the wave's
+      if (odd) {
+        r.clear();
+        some = false;
+        const float *row = query();
+        for (int pos = s0 * kStage + 32 * z; pos < min(s1 * kStage, most); pos += 32 * Z)
+          some |= r.take_plain(a, walk, row, row_sees(), pos, min(pos + 32, most));
       }
       float l = half_pair(r.l, [](float x, float y) { return x + y; });
       __syncthreads();
@@ -666,7 +789,7 @@ __global__ void __launch_bounds__(kThreads, 2) walk_blocks(Args a) {
               for (int j = 0; j < 4; ++j) y[j] = r.o[b][4 * i + j];
               to[(4 * b + i) * 64 + lane] = y;
             }
-          to[4 * S::NB * 64 + lane] = f4{r.m, l, r.some ? 1.f : 0.f, 0.f};
+          to[4 * S::NB * 64 + lane] = f4{r.m, l, some ? 1.f : 0.f, 0.f};
         }
         __syncthreads();
         if (z == 0) {
@@ -675,7 +798,7 @@ __global__ void __launch_bounds__(kThreads, 2) walk_blocks(Args a) {
             const f4 *of = reinterpret_cast<const f4 *>(joint + ((k - 1) * R + rw) * kEach);
             const f4 st = of[4 * S::NB * 64 + lane];
             const float now = fmaxf(r.m, st[0]), f0 = __builtin_amdgcn_exp2f(r.m - now), f1 = __builtin_amdgcn_exp2f(st[0] - now);
-            r.m = now, l = fmaf(st[1], f1, l * f0), r.some |= st[2] != 0.f;
+            r.m = now, l = fmaf(st[1], f1, l * f0), some |= st[2] != 0.f;
 #pragma unroll
             for (int b = 0; b < S::NB; ++b)
 #pragma unroll
@@ -688,6 +811,7 @@ __global__ void __launch_bounds__(kThreads, 2) walk_blocks(Args a) {
         }
       }
       const bool whole = s0 == 0 && s1 == stages;
+      const int dh = again_scalar(a.c.dh), lane_half = again(lane) >> 5;
       if (z == 0 && live) {
         float *to;
         float by = 1.f;
@@ -700,18 +824,18 @@ __global__ void __launch_bounds__(kThreads, 2) walk_blocks(Args a) {
           // a workgroup has at most one part that begins its block (place 1) and one that does not
           float *part = a.parts + (int64_t)(2 * p + (s0 == 0)) * kPart<DP, ROWS>;
           const int in = 32 * rw + c;
-          if (hi == 0) part[in] = r.m, part[ROWS + in] = r.some ? l : -1.f;
+          if (hi == 0) part[in] = r.m, part[ROWS + in] = some ? l : -1.f;
           to = part + 2 * ROWS + in * DP;
         }
 #pragma unroll
         for (int b = 0; b < S::NB; ++b)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int d = 32 * b + 8 * i + 4 * hi;
-            if (d >= a.c.dh) continue;
+            const int d = 32 * b + 8 * i + 4 * lane_half;
+            if (d >= dh) continue;
             f4 y;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = whole && !r.some ? 0.f : r.o[b][4 * i + j] * by;
+            for (int j = 0; j < 4; ++j) y[j] = whole && !some ? 0.f : r.o[b][4 * i + j] * by;
             *reinterpret_cast<f4u *>(to + d) = y;
           }
       }
@@ -723,60 +847,129 @@ __global__ void __launch_bounds__(kThreads, 2) walk_blocks(Args a) {
   }
 }
 
-// The parts of blocks that were cut, added in order: a workgroup a row, 32 threads with four columns each in eight
-// sets of every eighth part, whose loads go out eight at a time.
+// The parts of blocks that were cut, added in order.  Every workgroup lists the cut blocks' rows; a row of up to
+// kFew parts goes to a wave, its halves every other part, a row of more to a workgroup, 32 threads with four columns
+// each in eight sets of every eighth part.  Loads go out eight parts at a time.
+constexpr int kFew = 32;
+
 template <int DP, int ROWS>
-__global__ void __launch_bounds__(256) join_parts(Args a) {
+__global__ void __launch_bounds__(256) join_parts(Args a, int wgs) {
   constexpr int kAhead = 8;
-  const Cut cut = a.cuts[blockIdx.x];
-  const int tid = threadIdx.x, lane = tid & 63, set = tid >> 5, d = 4 * (tid & 31);
-  __shared__ float tops[4], sums[8];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  __shared__ int rows[2][257], sums[2][4];
+  __shared__ float tops[4], ls[8];
   __shared__ f4 outs[8][32];
-  for (int r = blockIdx.y; cut.parts > 0 && r < cut.rows; r += gridDim.y) {
-    // the first part is the owner's place 1, the others the next ones' places 0
-    auto part = [&](int k) { return a.parts + (int64_t)(k == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + k)) * kPart<DP, ROWS>; };
-    float m = kNever;
-    for (int k = tid; k < cut.parts; k += 256) m = fmaxf(m, part(k)[r]);
-    m = wave_max(m);
-    if (lane == 0) tops[tid >> 6] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    float l = -1.f;  // below 0: no token
-    f4 o{};
-    for (int k0 = set; k0 < cut.parts; k0 += 8 * kAhead) {
-      float ms[kAhead], ls[kAhead];
-      f4 y[kAhead];
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const float *x = part(min(k0 + 8 * i, cut.parts - 1));  // past the last: read again, not added
-        ms[i] = x[r], ls[i] = x[ROWS + r];
-        y[i] = *reinterpret_cast<const f4 *>(x + 2 * ROWS + r * DP + min(d, DP - 4));
-      }
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        if (k0 + 8 * i >= cut.parts || ls[i] < 0.f) continue;
-        const float f = __builtin_amdgcn_exp2f(ms[i] - m);
-        l = fmaf(ls[i], f, fmaxf(l, 0.f));
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = fmaf(y[i][j], f, o[j]);
-      }
-    }
-    if ((tid & 31) == 0) sums[set] = l;
-    outs[set][tid & 31] = o;
-    __syncthreads();
-    if (set == 0 && d < a.c.dh) {
-      bool some = false;
-      l = 0.f, o = f4{};
-      for (int i = 0; i < 8; ++i) {
-        if (sums[i] < 0.f) continue;
-        some = true, l += sums[i];
-        const f4 y = outs[i][tid];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] += y[j];
-      }
-      const int row = cut.row + r;
+  auto part = [&](int p, int k) {  // the first part is its workgroup's place 1, the others the next ones' places 0
+    return a.parts + (int64_t)(k == 0 ? 2 * p + 1 : 2 * (p + k)) * kPart<DP, ROWS>;
+  };
+  auto put = [&](const Cut &cut, int r, int d, bool some, f4 o, float l) {
+    const int row = cut.row + r;
+    if (d < a.c.dh)
       *reinterpret_cast<f4u *>(a.out + (int64_t)(cut.row0 + row / a.group) * a.ld_out + (int64_t)(cut.head + row % a.group) * a.c.dh + d) =
           some ? o / l : f4{};
+  };
+  for (int p0 = 0; p0 < wgs; p0 += 256) {
+    // rows before each cut block, of few parts and of many
+    const Cut mine = p0 + tid < wgs ? a.cuts[p0 + tid] : Cut{};
+    int v[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      v[k] = mine.parts > 0 && (mine.parts > kFew) == (k == 1) ? mine.rows : 0;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int below = __shfl_up(v[k], d);
+        if (lane >= d) v[k] += below;
+      }
+      if (lane == 63) sums[k][w] = v[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      for (int i = 0; i < w; ++i) v[k] += sums[k][i];
+      rows[k][tid + 1] = v[k];
+      if (tid == 0) rows[k][0] = 0;
+    }
+    __syncthreads();
+    auto find = [&](int k, int row) {  // the cut block that has it
+      int lo = 0, hi = 256;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        (rows[k][mid] <= row ? lo : hi) = mid;
+      }
+      return lo;
+    };
+    for (int i = blockIdx.x * 4 + w; i < rows[0][256]; i += gridDim.x * 4) {
+      const int at = find(0, i), p = p0 + at, r = i - rows[0][at], half = lane >> 5, d = 4 * (lane & 31);
+      const Cut cut = a.cuts[p];
+      float m = kNever, l = -1.f;
+      if (lane < cut.parts) m = part(p, lane)[r], l = part(p, lane)[ROWS + r];
+      const float top = wave_max(l < 0.f ? kNever : m), f = l < 0.f ? 0.f : __builtin_amdgcn_exp2f(m - top);
+      const bool some = __any(l >= 0.f);
+      f4 o{};
+      for (int k0 = 0; k0 < cut.parts; k0 += kAhead) {
+        f4 y[kAhead / 2];
+#pragma unroll
+        for (int k = 0; k < kAhead / 2; ++k)  // past the last: read again, not added
+          y[k] = *reinterpret_cast<const f4 *>(part(p, min(k0 + 2 * k + half, cut.parts - 1)) + 2 * ROWS + r * DP + min(d, DP - 4));
+#pragma unroll
+        for (int k = 0; k < kAhead / 2; ++k) {
+          const float by = __shfl(f, k0 + 2 * k + half);
+          if (k0 + 2 * k + half >= cut.parts || by == 0.f) continue;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[j] = fmaf(y[k][j], by, o[j]);
+        }
+      }
+      auto add = [](float x, float y) { return x + y; };
+      l = wave_sum(l < 0.f ? 0.f : l * f);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = half_pair(o[j], add);
+      if (half == 0) put(cut, r, d, some, o, l);
+    }
+    for (int i = blockIdx.x; i < rows[1][256]; i += gridDim.x) {
+      const int at = find(1, i), p = p0 + at, r = i - rows[1][at], set = tid >> 5, d = 4 * (tid & 31);
+      const Cut cut = a.cuts[p];
+      float m = kNever;
+      for (int k = tid; k < cut.parts; k += 256) m = fmaxf(m, part(p, k)[r]);
+      m = wave_max(m);
+      if (lane == 0) tops[w] = m;
+      __syncthreads();
+      m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+      float l = -1.f;  // below 0: no token
+      f4 o{};
+      for (int k0 = set; k0 < cut.parts; k0 += 8 * kAhead) {
+        float mk[kAhead], lk[kAhead];
+        f4 y[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          const float *x = part(p, min(k0 + 8 * k, cut.parts - 1));
+          mk[k] = x[r], lk[k] = x[ROWS + r];
+          y[k] = *reinterpret_cast<const f4 *>(x + 2 * ROWS + r * DP + min(d, DP - 4));
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          if (k0 + 8 * k >= cut.parts || lk[k] < 0.f) continue;
+          const float f = __builtin_amdgcn_exp2f(mk[k] - m);
+          l = fmaf(lk[k], f, fmaxf(l, 0.f));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[j] = fmaf(y[k][j], f, o[j]);
+        }
+      }
+      if ((tid & 31) == 0) ls[set] = l;
+      outs[set][tid & 31] = o;
+      __syncthreads();
+      if (set == 0) {
+        bool some = false;
+        l = 0.f, o = f4{};
+        for (int k = 0; k < 8; ++k) {
+          if (ls[k] < 0.f) continue;
+          some = true, l += ls[k];
+          const f4 y = outs[k][tid];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[j] += y[j];
+        }
+        put(cut, r, d, some, o, l);
+      }
+      __syncthreads();
     }
     __syncthreads();
   }
