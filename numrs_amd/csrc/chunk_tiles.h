@@ -904,7 +904,7 @@ __global__ void __launch_bounds__(256) join_parts(Args a, int wgs) {
       float m = kNever, l = -1.f;
       if (lane < cut.parts) m = part(p, lane)[r], l = part(p, lane)[ROWS + r];
       const float top = wave_max(l < 0.f ? kNever : m), f = l < 0.f ? 0.f : __builtin_amdgcn_exp2f(m - top);
-      const bool some = __any(l >= 0.f);
+      const bool some = __any(!(l < 0.f));  // (NaN too)
       f4 o{};
       for (int k0 = 0; k0 < cut.parts; k0 += kAhead) {
         f4 y[kAhead / 2];
