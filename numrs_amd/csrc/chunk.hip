@@ -61,9 +61,15 @@ extern "C" int numrs_hip_attention_paged_chunk(numrs_hip_ctx *ctx, const numrs_h
   if (q == nullptr || out == nullptr) return fail(ctx, NUMRS_HIP_E_INVALID, "%s: null pointer", what);
   if (int rc = s.keep()) return rc;
   DeviceScope dev(ctx);
+  // Sequences of one row, whose group's heads fill a sixteenth of a block of rows at most, go the way of the
+  // decoding steps.
+  if (s.singles > 0)
+    if (int rc = paged_steps(ctx, *cache, q, ld_q, heads, table, max_pages, ends, s.singles, s.single, out, ld_out))
+      return rc;
+  if (s.severals == 0) return NUMRS_HIP_OK;
   chunk::Args a{{cache->k, cache->v, cache->k_scale, cache->v_scale, cache->pages, max_pages, table,
                  paging::log2_of(cache->page_size), (int)hk, (int)dh},
-                s.whole, ends, q, out, nullptr, nullptr, ld_q, ld_out, (int)s.filled, (int)heads, (int)(heads / hk), 0.f, 0};
+                s.several, ends, q, out, nullptr, nullptr, ld_q, ld_out, (int)s.severals, (int)heads, (int)(heads / hk), 0.f, 0};
   a.mant = std::frexp(kLog2e / std::sqrt((float)dh), &a.exp);
   const bool few = s.longest * a.group <= 128;
   if (cache->format == NUMRS_HIP_KV_INT8) return few ? run_dp<true, 2>(ctx, s, a) : run_dp<true, 1>(ctx, s, a);

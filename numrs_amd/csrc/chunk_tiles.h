@@ -724,13 +724,17 @@ __global__ void __launch_bounds__(kThreads, 2) walk_blocks(Args a) {
       __syncthreads();  // what is marked is cleared, the last block's buffers free
       if (!good) Staging<INT8, DP, kBoth>::mark(&lds.marks[0], kOdd);
       g.load_keys(a.c, walk, s0);
+      if constexpr (kBoth) g.load_values(a.c, walk, s0);
       g.template raise_base<false>(lds, a.c, walk, s0);
-      __syncthreads();
+      if constexpr (kBoth) g.template raise_base<true>(lds, a.c, walk, s0);
+      if constexpr (!INT8) __syncthreads();
       const unsigned kbase = __builtin_amdgcn_readfirstlane(lds.base[0]);
       g.put_keys(lds, a.c, walk, s0, 0, 0, kbase);
-      g.load_values(a.c, walk, s0);
-      g.template raise_base<true>(lds, a.c, walk, s0);
-      __syncthreads();
+      if constexpr (!kBoth) {
+        g.load_values(a.c, walk, s0);
+        g.template raise_base<true>(lds, a.c, walk, s0);
+        __syncthreads();
+      }
       const unsigned vbase = __builtin_amdgcn_readfirstlane(lds.base[1]);
       g.put_values(lds, a.c, walk, s0, 0, 0, vbase);
       g.look(a.c, walk, s0 + 1);

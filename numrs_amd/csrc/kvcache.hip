@@ -397,6 +397,49 @@ int check_rows(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cache, const numrs_
 
 }  // namespace
 
+namespace numrs_hip {
+
+int paged_steps(numrs_hip_ctx *ctx, const numrs_hip_kv_cache &cache, const float *q, int64_t ld_q, int64_t heads,
+                const int32_t *table, int64_t max_pages, const int32_t *lengths, int64_t n, const SeqTile *list,
+                float *out, int64_t ld_out) {
+  const int hk = (int)cache.kv_heads, dh = (int)cache.head_dim, group = (int)heads / hk;
+  const int blocks = (group + 15) / 16;
+  // A workgroup of eight waves a CU, which the registers allow, each with an even share of the tokens;
+  // a kv head has as many at most as two levels of joins add.  Against two of four waves, with all loads
+  // through the caches, us: 333 tokens of 8 heads of 64 in fp32 11.6, 11; 34 thousand tokens of 40 sequences
+  // in 8 bits 39, 52; 131072 tokens of one head of 128 41, 50; 640 thousand tokens of 96 sequences, 5.2 GB, 868,
+  // 882 (784 past the caches as now).  Shares of 2 to 16 units
+  // at least, which leave fewer parts to join, were slower throughout.
+  const int shares = std::min(std::max(1, (ctx->num_cus + hk * blocks - 1) / (hk * blocks)),
+                              paged::kJoin * paged::kJoin);
+  const int64_t wgs = (int64_t)shares * hk * blocks;
+  TempBlock parts(ctx);
+  const int dp = (dh + 31) / 32 * 32;
+  if (int rc = parts.alloc((size_t)(2 * wgs * (32 + 16 * dp)) * sizeof(float))) return rc;
+  unsigned *arrivals = nullptr;
+  if (int rc = arrival_counters(ctx, (size_t)(3 * wgs), &arrivals)) return rc;
+  const paged::SplitArgs a{device_cache(cache, table, max_pages), q, lengths, out, parts.f(), arrivals, ld_q,
+                           ld_out, (int)n, (int)heads, blocks, shares,
+                           kLog2e / std::sqrt((float)dh), list};
+  auto launch = [&](auto padded) {
+    constexpr int DP = decltype(padded)::value;
+    auto kind = [&](auto int8, auto listed) {
+      paged::split_rows<decltype(int8)::value, DP, decltype(listed)::value>
+          <<<(unsigned)wgs, 64 * paged::kWaves, 0, ctx->stream>>>(a);
+    };
+    with_kind(cache.format == NUMRS_HIP_KV_INT8, list != nullptr, kind);
+  };
+  switch (dp) {
+    case 32: launch(std::integral_constant<int, 32>{}); break;
+    case 64: launch(std::integral_constant<int, 64>{}); break;
+    case 96: launch(std::integral_constant<int, 96>{}); break;
+    default: launch(std::integral_constant<int, 128>{});
+  }
+  return check_launch(ctx, "split_rows");
+}
+
+}  // namespace numrs_hip
+
 extern "C" {
 
 int numrs_hip_kv_cache_write(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cache,
@@ -493,39 +536,7 @@ int numrs_hip_attention_paged(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cach
   if (q == nullptr || out == nullptr)
     return fail(ctx, NUMRS_HIP_E_INVALID, "attention_paged: null pointer");
   DeviceScope dev(ctx);
-  const int hk = (int)cache->kv_heads, dh = (int)cache->head_dim, group = (int)heads / hk;
-  const int blocks = (group + 15) / 16;
-  // A workgroup of eight waves a CU, which the registers allow, each with an even share of the tokens;
-  // a kv head has as many at most as two levels of joins add.  Against two of four waves, with all loads
-  // through the caches, us: 333 tokens of 8 heads of 64 in fp32 11.6, 11; 34 thousand tokens of 40 sequences
-  // in 8 bits 39, 52; 131072 tokens of one head of 128 41, 50; 640 thousand tokens of 96 sequences, 5.2 GB, 868,
-  // 882 (784 past the caches as now).  Shares of 2 to 16 units
-  // at least, which leave fewer parts to join, were slower throughout.
-  const int shares = std::min(std::max(1, (ctx->num_cus + hk * blocks - 1) / (hk * blocks)),
-                              paged::kJoin * paged::kJoin);
-  const int64_t wgs = (int64_t)shares * hk * blocks;
-  TempBlock parts(ctx);
-  const int dp = (dh + 31) / 32 * 32;
-  if (int rc = parts.alloc((size_t)(2 * wgs * (32 + 16 * dp)) * sizeof(float))) return rc;
-  unsigned *arrivals = nullptr;
-  if (int rc = arrival_counters(ctx, (size_t)(3 * wgs), &arrivals)) return rc;
-  const paged::SplitArgs a{device_cache(*cache, table, max_pages), q, lengths, out, parts.f(), arrivals, ld_q,
-                           ld_out, (int)n, (int)heads, blocks, shares,
-                           kLog2e / std::sqrt((float)dh)};
-  auto launch = [&](auto padded) {
-    constexpr int DP = decltype(padded)::value;
-    if (cache->format == NUMRS_HIP_KV_F32)
-      paged::split_rows<false, DP><<<(unsigned)wgs, 64 * paged::kWaves, 0, ctx->stream>>>(a);
-    else
-      paged::split_rows<true, DP><<<(unsigned)wgs, 64 * paged::kWaves, 0, ctx->stream>>>(a);
-  };
-  switch (dp) {
-    case 32: launch(std::integral_constant<int, 32>{}); break;
-    case 64: launch(std::integral_constant<int, 64>{}); break;
-    case 96: launch(std::integral_constant<int, 96>{}); break;
-    default: launch(std::integral_constant<int, 128>{});
-  }
-  return check_launch(ctx, "split_rows");
+  return paged_steps(ctx, *cache, q, ld_q, heads, table, max_pages, lengths, n, nullptr, out, ld_out);
 }
 
 }  // extern "C"

@@ -27,8 +27,8 @@ struct Seqs : std::enable_shared_from_this<Seqs> {
   SeqTile *by_work = nullptr;   // [blocks] of 128 tokens, those with the most tokens before them first
   SeqTile *by_rest = nullptr;   // [blocks], those with the most tokens after them first
   SeqTile *few_by_work = nullptr, *few_by_rest = nullptr;  // the same of the tiles
-  SeqTile *whole = nullptr;     // [filled]: the sequences that have tokens
-  int64_t filled = 0, longest = 0;
+  SeqTile *several = nullptr, *single = nullptr;  // the sequences of several tokens, and of one
+  int64_t severals = 0, singles = 0, longest = 0;
   size_t bytes = 0;
   ~Seqs() { block_free(ctx, in_order, bytes); }
   // Called before a launch that reads the lists: a graph being recorded keeps them for its replays,
@@ -55,6 +55,11 @@ int packed_backward(numrs_hip_ctx *ctx, const Seqs &s, const float *q, int64_t l
                     const float *v, int64_t ld_kv, const float *out, const float *dout,
                     int64_t ld_out, const float *stats, float *dq, float *dk, float *dv,
                     PackedHeads h, int accumulate);
+
+// numrs_hip_attention_paged without its checks; with a list, of those n sequences of one row each of a packed batch.
+int paged_steps(numrs_hip_ctx *ctx, const numrs_hip_kv_cache &cache, const float *q, int64_t ld_q, int64_t heads,
+                const int32_t *table, int64_t max_pages, const int32_t *lengths, int64_t n, const SeqTile *list,
+                float *out, int64_t ld_out);
 
 // Makes the context's device current for a call, and the caller's again after it.
 struct DeviceScope {

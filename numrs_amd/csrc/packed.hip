@@ -467,11 +467,10 @@ int numrs_hip_seqs_create(numrs_hip_ctx *ctx, const int64_t *lengths, int64_t n,
       lists.insert(lists.end(), list.begin(), list.end());
     };
     add(blocks, false), add(blocks, true), add(tiles, false), add(tiles, true);
-    for (const SeqTile &t : tiles) {
-      if (t.t0 != 0) continue;
-      lists.push_back(t), ++s->filled;
-      s->longest = std::max<int64_t>(s->longest, t.len);
-    }
+    for (const SeqTile &t : tiles)
+      if (t.t0 == 0 && t.len > 1) lists.push_back(t), ++s->severals, s->longest = std::max<int64_t>(s->longest, t.len);
+    for (const SeqTile &t : tiles)
+      if (t.len == 1) lists.push_back(t), ++s->singles;
     auto h = std::make_unique<numrs_hip_seqs>();
     if (!lists.empty()) {
       void *p = nullptr;
@@ -480,7 +479,7 @@ int numrs_hip_seqs_create(numrs_hip_ctx *ctx, const int64_t *lengths, int64_t n,
       s->in_order = static_cast<SeqTile *>(p), s->bytes = bytes;
       s->by_work = s->in_order + s->tiles, s->by_rest = s->by_work + s->blocks;
       s->few_by_work = s->by_rest + s->blocks, s->few_by_rest = s->few_by_work + s->tiles;
-      s->whole = s->few_by_rest + s->tiles;
+      s->several = s->few_by_rest + s->tiles, s->single = s->several + s->severals;
       if (int rc = numrs_hip_upload(ctx, p, lists.data(), bytes)) return rc;
     }
     h->s = std::move(s);

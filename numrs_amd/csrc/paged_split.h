@@ -79,7 +79,19 @@ struct SplitArgs {
   int64_t ld_q, ld_out;
   int n, heads, blocks, shares;  // blocks: of 16 query heads in a group; shares: workgroups of a kv head's block
   float alpha;                   // log2(e) / sqrt(dh)
+  const numrs_hip::SeqTile *list;  // of the n sequences of one row each, where not all of the table's are
 };
+// The table's row, and the query row, of the i-th sequence.
+template <bool LISTED>
+__device__ __forceinline__ int table_row(const SplitArgs &a, int i) {
+  if constexpr (LISTED) return a.list[i].seq;
+  return i;
+}
+template <bool LISTED>
+__device__ __forceinline__ int query_row(const SplitArgs &a, int i) {
+  if constexpr (LISTED) return a.list[i].row0;
+  return i;
+}
 
 constexpr int kUnit = 64;       // tokens
 constexpr int kJoin = 16;       // parts that one workgroup adds: two levels for up to kJoin^2 shares
@@ -465,7 +477,7 @@ __device__ __forceinline__ bool arrive(unsigned *counter, int count, int *flag) 
   return __builtin_amdgcn_readfirstlane(*flag) != 0;
 }
 
-template <bool INT8, int DP>
+template <bool INT8, int DP, bool LISTED>
 __global__ void __launch_bounds__(64 * kWaves, 2) split_rows(SplitArgs a) {
   using S = State<INT8, DP>;
   constexpr int kStep = 16 * S::NB, kThreads = 64 * kWaves, kCols = S::NU * 64 + 4;
@@ -485,7 +497,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) split_rows(SplitArgs a) {
   // Of kThreads sequences from i0 on: their tokens, and the units before each in pre, with `base`
   // before the first; returns their end.
   auto scan = [&](int i0, int64_t base) {
-    const int len = i0 + tid < a.n ? (int)paging::held(a.lengths[i0 + tid], a.c.max_pages, a.c.shift) : 0;
+    const int len = i0 + tid < a.n ? (int)paging::held(a.lengths[table_row<LISTED>(a, i0 + tid)], a.c.max_pages, a.c.shift) : 0;
     // a sequence without tokens has a row to write too
     int64_t v = i0 + tid < a.n ? max(1, (int)(((unsigned)len + kUnit - 1) / kUnit)) : 0;
 #pragma unroll
@@ -554,7 +566,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) split_rows(SplitArgs a) {
       st.clear();
       if (mine >= 0) {
         const int i = i0 + mine;
-        const int32_t *row = a.c.table + (int64_t)i * a.c.max_pages;
+        const int32_t *row = a.c.table + (int64_t)table_row<LISTED>(a, i) * a.c.max_pages;
         char *queries = reinterpret_cast<char *>(so[w]);
         int32_t entries[S::NB];
         int pages[S::NB], next[S::NB];
@@ -575,7 +587,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) split_rows(SplitArgs a) {
         int64_t pos = my.from + (w - first) * kStep;
         look(pos);
         const int head = cb * 16 + (lane & 15);
-        const auto q = S::ask(a, i, kv * group + min(head, group - 1), head < group);
+        const auto q = S::ask(a, query_row<LISTED>(a, i), kv * group + min(head, group - 1), head < group);
         resolve();
         if (pos < my.end) S::load_keys(a.c, kv, pos, next, past, x), S::load_values(a.c, kv, pos, next, past, x);
         look(pos + ahead);
@@ -615,7 +627,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) split_rows(SplitArgs a) {
       used = 0;
       for (; j < last; ++j) {
         const Stretch s = stretch(j);
-        const int i = i0 + j, c = tid >> 5, col = tid & 31, w1 = used + s.waves;
+        const int i = query_row<LISTED>(a, i0 + j), c = tid >> 5, col = tid & 31, w1 = used + s.waves;
         Row r{kNever, -1.f, {}};
         for (int k = used; k < w1; ++k) r.m = fmaxf(r.m, sm[k][c]);
         for (int k = used; k < w1; ++k) {
