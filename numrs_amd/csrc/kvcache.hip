@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(256) append_rows(AppendArgs b) {
   if (blockIdx.x >= b.keys) {
     const unsigned n = b.row.slots > 0 ? (b.row.slots + b.row.per - 1) / b.row.per : 1, i = blockIdx.x - b.keys;
     const int h0 = i % n * b.row.per;
-    rotary::rotate_part(b.row, b.row.tiles[i / n / b.parts], i / n % b.parts, h0, min(h0 + b.row.per, b.row.slots));
+    rotary::rotate_part<PAST>(b.row, b.row.tiles[i / n / b.parts], i / n % b.parts, h0, min(h0 + b.row.per, b.row.slots));
     return;
   }
   const RowArgs &a = b.c;

@@ -211,7 +211,22 @@ __device__ __forceinline__ int token_of(const SeqTile &t, int part, int lanes) {
   return r < min(t.len, t.t0 + kTile) ? r : -1;
 }
 
+// Rows past the caches, or through them.
+template <bool PAST>
+__device__ __forceinline__ f4 get4(const float *p) {
+  if constexpr (PAST) return __builtin_nontemporal_load(reinterpret_cast<const f4u *>(p));
+  return *reinterpret_cast<const f4u *>(p);
+}
+template <bool PAST>
+__device__ __forceinline__ void put4(float *p, f4 v) {
+  if constexpr (PAST)
+    __builtin_nontemporal_store(f4u(v), reinterpret_cast<f4u *>(p));
+  else
+    *reinterpret_cast<f4u *>(p) = v;
+}
+
 // A part of a tile's tokens, some of its heads: the angles are formed once for all of them.
+template <bool PAST>
 __device__ __forceinline__ void rotate_part(const RowArgs &a, const SeqTile &t, int part, int h0, int h1) {
   const int i = threadIdx.x & ((1 << a.lanes) - 1), r = token_of(t, part, a.lanes);
   const Item it = item_of(i, a.dh, a.turn);
@@ -224,7 +239,7 @@ __device__ __forceinline__ void rotate_part(const RowArgs &a, const SeqTile &t, 
     lo = f4{}, hi = f4{};
     if (it.in && h < h1) {
       const float *p = px + (int64_t)h * a.dh;
-      lo = *reinterpret_cast<const f4u *>(p + it.d0), hi = *reinterpret_cast<const f4u *>(p + it.d1);
+      lo = get4<PAST>(p + it.d0), hi = get4<PAST>(p + it.d1);
     }
   };
   f4 lo, hi;
@@ -252,7 +267,7 @@ __device__ __forceinline__ void rotate_part(const RowArgs &a, const SeqTile &t, 
     }
     if (it.in) {
       float *p = py + (int64_t)h * a.dh;
-      *reinterpret_cast<f4u *>(p + it.d0) = y0, *reinterpret_cast<f4u *>(p + it.d1) = y1;
+      put4<PAST>(p + it.d0, y0), put4<PAST>(p + it.d1, y1);
     }
   }
 }

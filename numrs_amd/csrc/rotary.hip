@@ -13,9 +13,10 @@ namespace {
 using namespace numrs_hip;
 using namespace rotary;
 
+template <bool PAST>
 __global__ void __launch_bounds__(256) rotate_rows(RowArgs a, int parts) {
   const int h0 = blockIdx.y * a.per;
-  rotate_part(a, a.tiles[blockIdx.x / parts], blockIdx.x % parts, h0, min(h0 + a.per, a.slots));
+  rotate_part<PAST>(a, a.tiles[blockIdx.x / parts], blockIdx.x % parts, h0, min(h0 + a.per, a.slots));
 }
 
 struct BackArgs {
@@ -28,6 +29,7 @@ struct BackArgs {
 
 // With g = R^T dy and xh = x / sqrt(mean(x^2) + eps):
 //   dw = sum g xh,   dx = (g w - xh mean(g w xh)) / sqrt(mean(x^2) + eps).
+template <bool PAST>
 __global__ void __launch_bounds__(256) rotate_rows_back(BackArgs b, int parts) {
   __shared__ double sum[256][8];
   const RowArgs &a = b.r;
@@ -81,10 +83,10 @@ __global__ void __launch_bounds__(256) rotate_rows_back(BackArgs b, int parts) {
     f4 g0{}, g1{}, x0{}, x1{};
     if (it.in) {
       const float *p = pg + (int64_t)h * a.dh;
-      g0 = *reinterpret_cast<const f4u *>(p + it.d0), g1 = *reinterpret_cast<const f4u *>(p + it.d1);
+      g0 = get4<PAST>(p + it.d0), g1 = get4<PAST>(p + it.d1);
       if (pw != nullptr) {
         p = px + (int64_t)h * a.dh;
-        x0 = *reinterpret_cast<const f4u *>(p + it.d0), x1 = *reinterpret_cast<const f4u *>(p + it.d1);
+        x0 = get4<PAST>(p + it.d0), x1 = get4<PAST>(p + it.d1);
       }
     }
     if (now < 2) {
@@ -111,25 +113,60 @@ __global__ void __launch_bounds__(256) rotate_rows_back(BackArgs b, int parts) {
     if (it.in && a.y != nullptr) {
       float *p = py + (int64_t)h * a.dh;
       if (b.accumulate) g0 += f4(*reinterpret_cast<f4u *>(p + it.d0)), g1 += f4(*reinterpret_cast<f4u *>(p + it.d1));
-      *reinterpret_cast<f4u *>(p + it.d0) = g0, *reinterpret_cast<f4u *>(p + it.d1) = g1;
+      put4<PAST>(p + it.d0, g0), put4<PAST>(p + it.d1, g1);
     }
   }
   flush(kind);
 }
 
-// The workgroups' sums added in order: eight columns a workgroup, 32 threads with every 32nd workgroup's.
-// A column's query and key parts belong to one thread, so that one array may be both gradients.
-__global__ void __launch_bounds__(256) add_sums(const double *sums, int64_t n, int dh, float *dq, float *dk, int acc_q, int acc_k) {
-  __shared__ double part[2][32][8];
-  const int col = threadIdx.x & 7, from = threadIdx.x >> 3, d = blockIdx.x * 8 + col;
-  double q = 0.0, k = 0.0;
-  for (int64_t i = from; i < n; i += 32) q += sums[i * 2 * dh + d], k += sums[(i * 2 + 1) * dh + d];
-  part[0][from][col] = q, part[1][from][col] = k;
+// The workgroups' sums [n][2][dh] added in order: a thread a column, a workgroup every gridDim.x-th of them, whose
+// results the last workgroup to finish adds.  A column's query and key parts belong to one thread then, so that one
+// array may be both gradients.  (16 workgroups with every column of eight: 29 us for 2048 sums of 256 columns.)
+__global__ void __launch_bounds__(256)
+    add_sums(const double *sums, int n, int dh, double *partial, unsigned *arrivals, float *dq, float *dk, int acc_q, int acc_k) {
+  __shared__ int last;
+  const int d = threadIdx.x, cols = 2 * dh;
+  constexpr int kAhead = 8;
+  if (d < cols) {
+    double s = 0.0;
+    for (int i = blockIdx.x; i < n; i += kAhead * gridDim.x) {
+      double x[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) x[k] = i + k * (int)gridDim.x < n ? sums[(int64_t)(i + k * (int)gridDim.x) * cols + d] : 0.0;
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) s += x[k];
+    }
+    __hip_atomic_store(partial + blockIdx.x * cols + d, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  if (from != 0) return;
-  for (int i = 1; i < 32; ++i) q += part[0][i][col], k += part[1][i][col];
+  if (d == 0) {
+    last = __hip_atomic_fetch_add(arrivals, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == gridDim.x;
+    if (last) __hip_atomic_store(arrivals, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!last || d >= dh) return;
+  double q = 0.0, k = 0.0;
+  for (int i = 0; i < (int)gridDim.x; i += kAhead) {
+    double x[kAhead], y[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const double *p = partial + min(i + j, (int)gridDim.x - 1) * cols + d;
+      x[j] = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      y[j] = __hip_atomic_load(p + dh, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (i + j < (int)gridDim.x) q += x[j], k += y[j];
+  }
   if (dq != nullptr) dq[d] = (float)(acc_q ? dq[d] + q : q);
   if (dk != nullptr) dk[d] = (float)(acc_k ? dk[d] + k : k);
+}
+
+// Whether rows go past the caches: where a call reads and writes more than half of the last cache's 256 MB, so that
+// they would take the place of what the next kernel reads.
+bool rows_past(const Seqs &s, const RowArgs &a, int arrays) {
+  return s.total * (a.heads + 2 * a.kv_heads) * a.dh * (int64_t)sizeof(float) * arrays > int64_t{128} << 20;
 }
 
 int check_rows(numrs_hip_ctx *ctx, const numrs_hip_seqs *seqs, int64_t ld_a, int64_t ld_b, int64_t ld_c,
@@ -180,7 +217,11 @@ int numrs_hip_qk_rotary_forward(numrs_hip_ctx *ctx, const numrs_hip_seqs *seqs, 
   const RowArgs a = row_args(s, ends, x, ld_x, q_weight, k_weight, eps, rotary, y, ld_y, heads, kv_heads, dh,
                              heads + (x == y ? 1 : 2) * kv_heads);
   const int parts = parts_of(a.lanes);
-  rotate_rows<<<dim3((unsigned)(s.tiles * parts), (a.slots + a.per - 1) / a.per), 256, 0, ctx->stream>>>(a, parts);
+  const dim3 grid((unsigned)(s.tiles * parts), (a.slots + a.per - 1) / a.per);
+  if (rows_past(s, a, 2))
+    rotate_rows<true><<<grid, 256, 0, ctx->stream>>>(a, parts);
+  else
+    rotate_rows<false><<<grid, 256, 0, ctx->stream>>>(a, parts);
   return check_launch(ctx, "rotate_rows");
 }
 
@@ -225,10 +266,19 @@ int numrs_hip_qk_rotary_backward(numrs_hip_ctx *ctx, const numrs_hip_seqs *seqs,
     if (int rc = sums.alloc((size_t)(groups * 2 * dh) * sizeof(double))) return rc;
     b.sums = static_cast<double *>(sums.p);
   }
-  rotate_rows_back<<<grid, 256, 0, ctx->stream>>>(b, parts);
+  if (rows_past(s, b.r, 3))
+    rotate_rows_back<true><<<grid, 256, 0, ctx->stream>>>(b, parts);
+  else
+    rotate_rows_back<false><<<grid, 256, 0, ctx->stream>>>(b, parts);
   if (int rc = check_launch(ctx, "rotate_rows_back")) return rc;
   if (!weights) return NUMRS_HIP_OK;
-  add_sums<<<(unsigned)(dh / 8), 256, 0, ctx->stream>>>(b.sums, groups, (int)dh, dq_weight, dk_weight, acc_q, acc_k);
+  const unsigned adders = (unsigned)std::min<int64_t>(64, (groups + 7) / 8);
+  TempBlock partial(ctx);
+  if (int rc = partial.alloc((size_t)(adders * 2 * dh) * sizeof(double))) return rc;
+  unsigned *arrivals = nullptr;
+  if (int rc = arrival_counters(ctx, 1, &arrivals)) return rc;
+  add_sums<<<adders, 256, 0, ctx->stream>>>(b.sums, (int)groups, (int)dh, static_cast<double *>(partial.p), arrivals,
+                                            dq_weight, dk_weight, acc_q, acc_k);
   return check_launch(ctx, "add_sums");
 }
 
