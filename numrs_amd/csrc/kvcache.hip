@@ -279,9 +279,13 @@ __global__ void __launch_bounds__(256) append_rows(AppendArgs b) {
   const SeqTile t = a.tiles[blockIdx.x / a.c.kv_heads];
   const int g = blockIdx.x % a.c.kv_heads, dh = a.c.dh;
   const bool nb = ra.turn.pairs;
-  for_groups(a.c, t, g, a.ends, ra.lanes, [&](const Group &x, int four_i) {
-    const int i = four_i / 4;
-    const rotary::Item it = rotary::item_of(i, dh, ra.turn);
+  // What no row decides is asked for before the rows' pages are looked up.
+  const int i = threadIdx.x & ((1 << ra.lanes) - 1);
+  const rotary::Item it = rotary::item_of(i, dh, ra.turn);
+  const rotary::Steps steps = rotary::steps_of(ra.turn, i, it);
+  rotary::Weight w;
+  w.load(ra.wk, it, nb);
+  for_groups(a.c, t, g, a.ends, ra.lanes, [&](const Group &x, int) {
     f4 k0[4], k1[4], v0[4], v1[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -292,10 +296,9 @@ __global__ void __launch_bounds__(256) append_rows(AppendArgs b) {
       k0[r] = paged::load<f4u, PAST>(k + 4 * it.d0), k1[r] = paged::load<f4u, PAST>(k + 4 * it.d1);
       v0[r] = paged::load<f4u, PAST>(v + 32 * i), v1[r] = paged::load<f4u, PAST>(v + 32 * i + 16);
     }
-    rotary::Weight w;
-    w.load(ra.wk, it, nb);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
+      if (x.row[r] < 0) continue;  // (a step has one row of four: the others' code is not even fetched)
       double y[8];
       rotary::pairs_of(k0[r], k1[r], nb, y);
       if (ra.wk != nullptr) {
@@ -303,7 +306,7 @@ __global__ void __launch_bounds__(256) append_rows(AppendArgs b) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[j] = y[j] * s * w.w[j];
       }
-      if (x.row[r] >= 0) rotary::turn<false>(y, rotary::units_of(ra.turn, i, it, x.pos + r), it.turned);
+      rotary::turn<false>(y, rotary::units_of(steps, it, x.pos + r), it.turned);
       rotary::columns_of(y, nb, k0[r], k1[r]);
     }
     if constexpr (!INT8) {
@@ -315,8 +318,8 @@ __global__ void __launch_bounds__(256) append_rows(AppendArgs b) {
         *reinterpret_cast<f4 *>(v + 8 * i) = v0[r], *reinterpret_cast<f4 *>(v + 8 * i + 4) = v1[r];
       }
     } else {
-      u4 kc0, kc1, vc0, vc1;
-      f4 ks, vs;
+      u4 kc0{}, kc1{}, vc0{}, vc1{};
+      f4 ks{}, vs{};
       unsigned top[8];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -326,6 +329,7 @@ __global__ void __launch_bounds__(256) append_rows(AppendArgs b) {
       max_of(top, ra.lanes);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
+        if (x.row[r] < 0) continue;
         ks[r] = scale_of(top[r]), vs[r] = scale_of(top[4 + r]);
         kc0[r] = codes_of(k0[r], ks[r]), kc1[r] = codes_of(k1[r], ks[r]);
         vc0[r] = codes_of(v0[r], vs[r]), vc1[r] = codes_of(v1[r], vs[r]);

@@ -124,14 +124,26 @@ __device__ __forceinline__ void unit_of(double turns, int64_t pos, double &c, do
   s = q & 2 ? -n : n;
 }
 
+// Circles a position, of a lane's four pairs.
+struct Steps {
+  double turns[4];
+};
+__device__ __forceinline__ Steps steps_of(const Turn &t, int i, const Item &x) {
+  Steps s{};
+  if (x.turned) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s.turns[j] = t.turns[4 * i + j];
+  }
+  return s;
+}
 struct Units {
   double c[4], s[4];
 };
-__device__ __forceinline__ Units units_of(const Turn &t, int i, const Item &x, int64_t pos) {
+__device__ __forceinline__ Units units_of(const Steps &t, const Item &x, int64_t pos) {
   Units u{};
   if (x.turned) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) unit_of(t.turns[4 * i + j], pos, u.c[j], u.s[j]);
+    for (int j = 0; j < 4; ++j) unit_of(t.turns[j], pos, u.c[j], u.s[j]);
   }
   return u;
 }
@@ -244,7 +256,7 @@ __device__ __forceinline__ void rotate_part(const RowArgs &a, const SeqTile &t, 
   };
   f4 lo, hi;
   ask(h0, lo, hi);
-  const Units u = units_of(a.turn, i, it, start + r);
+  const Units u = units_of(steps_of(a.turn, i, it), it, start + r);
   Weight w;
   int kind = -1;
   for (int h = h0; h < h1; ++h) {

@@ -41,7 +41,7 @@ __global__ void __launch_bounds__(256) rotate_rows_back(BackArgs b, int parts) {
   const float *px = a.x + row * a.ld_x, *pg = b.dy + row * b.ld_dy;
   float *py = a.y + row * a.ld_y;
   const bool nb = a.turn.pairs, live = r >= 0;
-  const Units u = units_of(a.turn, i, it, start + r);
+  const Units u = units_of(steps_of(a.turn, i, it), it, start + r);
   double acc[8] = {};
   Weight w;
   int kind = -1;
