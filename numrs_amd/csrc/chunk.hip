@@ -12,8 +12,21 @@ using namespace numrs_hip;
 
 constexpr float kLog2e = 1.44269504088896341f;
 
-template <bool INT8, int DP, int Z>
-int run(numrs_hip_ctx *ctx, const Seqs &s, chunk::Args a) {
+// From kManyRows query rows of a kv head on a sequence, over caches in fp32, stages are made images first, which costs
+// a pass over the cached tokens and saves every block of 256 rows its own splitting.  On MI355X, without against with,
+// us, 32 heads of 128 in groups of 4 over 8192 tokens: 256 rows 68, 81; 512 rows 91, 101; 1024 rows 158, 156; 2048
+// rows 268, 251; of four sequences in groups of 8: 1024 rows over 8192 158, 156; 2048 over 2048 109, 104; 16384 rows
+// over 2000 to 16384 2000, 1643; heads of 64 over 2048: 1024 rows 74, 75; 2048 rows 120, 116.  The images have room
+// for all that the pages can hold, since only the device knows what they do; past kMostImages they are not made.
+constexpr int64_t kManyRows = 1024, kMostImages = int64_t{1} << 30;
+// Up to so many rows blocks have 128 in two sets of waves, beyond 256 in one, which reads the tokens half as often.
+// 256 against 128, us: 128 rows over 131072 tokens 68, 69; 32 heads of 128 over 8192, fp32 and 8 bits: 32 rows 44, 44
+// and 35, 33; 128 rows 51, 51 and 40, 42; 256 rows 65, 65 and 52, 52; 512 rows 93, 113 and 74, 87; eight sequences
+// over 500, heads of 64: 64 rows 25, 24; 256 rows 38, 34; 512 rows 47, 53.
+constexpr int64_t kFewRows = 256;
+
+template <bool INT8, int DP, int Z, bool PACKED>
+int walk(numrs_hip_ctx *ctx, chunk::Args a) {
   constexpr int ROWS = 256 / Z;
   const unsigned wgs = (unsigned)ctx->num_cus;
   TempBlock parts(ctx);
@@ -21,10 +34,29 @@ int run(numrs_hip_ctx *ctx, const Seqs &s, chunk::Args a) {
   if (int rc = parts.alloc(image + wgs * sizeof(chunk::Cut))) return rc;
   a.parts = parts.f();
   a.cuts = reinterpret_cast<chunk::Cut *>(static_cast<char *>(parts.p) + image);
-  chunk::walk_blocks<INT8, DP, Z><<<wgs, chunk::kThreads, 0, ctx->stream>>>(a);
+  chunk::walk_blocks<INT8, DP, Z, PACKED><<<wgs, chunk::kThreads, 0, ctx->stream>>>(a);
   if (int rc = check_launch(ctx, "walk_blocks")) return rc;
   chunk::join_parts<DP, ROWS><<<4 * wgs, 256, 0, ctx->stream>>>(a, (int)wgs);
   return check_launch(ctx, "join_parts");
+}
+
+template <bool INT8, int DP, int Z>
+int run(numrs_hip_ctx *ctx, const Seqs &s, chunk::Args a) {
+  if constexpr (!INT8 && Z == 1) {
+    const int64_t rows = (s.total - s.singles) * a.group;
+    const int64_t stages = ((a.c.max_pages << a.c.shift) + chunk::kStage - 1) / chunk::kStage;
+    const int64_t images = s.severals * a.c.kv_heads * stages, bytes = images * chunk::kImage<DP>;
+    if (rows >= s.severals * kManyRows && bytes <= kMostImages) {
+      TempBlock block(ctx);
+      if (int rc = block.alloc((size_t)bytes)) return rc;
+      a.images = static_cast<char *>(block.p);
+      a.most_stages = (int)stages;
+      chunk::pack_stages<DP><<<(unsigned)images, chunk::kThreads, 0, ctx->stream>>>(a);
+      if (int rc = check_launch(ctx, "pack_stages")) return rc;
+      return walk<INT8, DP, Z, true>(ctx, a);
+    }
+  }
+  return walk<INT8, DP, Z, false>(ctx, a);
 }
 
 template <bool INT8, int Z>
@@ -57,6 +89,8 @@ extern "C" int numrs_hip_attention_paged_chunk(numrs_hip_ctx *ctx, const numrs_h
   if (paging::bad_stride(ld_q, heads * dh) || paging::bad_stride(ld_out, heads * dh))
     return fail(ctx, NUMRS_HIP_E_SHAPE, "%s: a row stride is below its row's width or above 2^31 - 1", what);
   if (paging::bad_grid(s.tiles * heads)) return fail(ctx, NUMRS_HIP_E_SHAPE, "%s: too many tokens times heads", what);
+  if (s.longest * (heads / hk) > INT32_MAX - 1024)  // (rows are counted in 32 bits, in blocks)
+    return fail(ctx, NUMRS_HIP_E_SHAPE, "%s: too many new tokens times heads of a group in one sequence", what);
   if (s.total == 0) return NUMRS_HIP_OK;
   if (q == nullptr || out == nullptr) return fail(ctx, NUMRS_HIP_E_INVALID, "%s: null pointer", what);
   if (int rc = s.keep()) return rc;
@@ -69,9 +103,9 @@ extern "C" int numrs_hip_attention_paged_chunk(numrs_hip_ctx *ctx, const numrs_h
   if (s.severals == 0) return NUMRS_HIP_OK;
   chunk::Args a{{cache->k, cache->v, cache->k_scale, cache->v_scale, cache->pages, max_pages, table,
                  paging::log2_of(cache->page_size), (int)hk, (int)dh},
-                s.several, ends, q, out, nullptr, nullptr, ld_q, ld_out, (int)s.severals, (int)heads, (int)(heads / hk), 0.f, 0};
+                s.several, ends, q, out, nullptr, nullptr, 0, nullptr, ld_q, ld_out, (int)s.severals, (int)heads, (int)(heads / hk), 0.f, 0};
   a.mant = std::frexp(kLog2e / std::sqrt((float)dh), &a.exp);
-  const bool few = s.longest * a.group <= 128;
+  const bool few = s.longest * a.group <= kFewRows;
   if (cache->format == NUMRS_HIP_KV_INT8) return few ? run_dp<true, 2>(ctx, s, a) : run_dp<true, 1>(ctx, s, a);
   return few ? run_dp<false, 2>(ctx, s, a) : run_dp<false, 1>(ctx, s, a);
 }

@@ -52,6 +52,8 @@ struct Args {
   const int32_t *ends;
   const float *q;
   float *out, *parts;
+  char *images;  // of stages, [n][kv_heads][most_stages]
+  int most_stages;
   Cut *cuts;  // [workgroups]
   int64_t ld_q, ld_out;
   int n, heads, group;
@@ -122,15 +124,26 @@ __device__ __forceinline__ unsigned row_top(unsigned v) {
   return v;
 }
 
+// A stage's bases, marks and factors, the last kilobyte of its image where it has one.
+struct Head {
+  unsigned base[2];  // of keys and of values
+  int marks, none[61];
+  float ks[kStage], vs[kStage];
+  char rest[256];
+};
+static_assert(sizeof(Head) == 1024);
+template <int DP>
+constexpr int kImage = Shape<false, DP>::kBytes + (int)sizeof(Head);
+
 // What a workgroup shares.
 template <bool INT8, int DP>
 struct Lds {
   using S = Shape<INT8, DP>;
   static constexpr int kJoint = 64 * (16 * S::NB + 4) * 4;  // a wave's results, while sets are joined
   // (the stages last: an LDS access has 16 bits for a constant offset)
-  float ks[2][kStage], vs[2][kStage];  // the rows' factors
-  int marks[3];                        // of three stages in turn: one is read, one written, one cleared
-  unsigned base[2];                    // the walk's, of keys and of values
+  Head heads[2] __attribute__((aligned(256)));
+  int marks[3];      // of three stages in turn: one is read, one written, one cleared
+  unsigned base[2];  // the walk's, of keys and of values
   char kept[8][S::kKept > 0 ? S::kKept : 1][1024] __attribute__((aligned(256)));  // of each wave's queries
   char stages[2 * S::kBytes > 4 * kJoint ? 2 * S::kBytes : 4 * kJoint] __attribute__((aligned(256)));
   __device__ __forceinline__ char *stage(int buf) { return stages + buf * S::kBytes; }
@@ -184,8 +197,8 @@ struct Staging {
     const int tid = again(threadIdx.x);
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
-      const int pos = stage * kStage + token(tid, i);
-      entries[i] = pos < w.held ? paging::entry_of(w.pages, c.max_pages, c.shift, pos) : -1;
+      const unsigned pos = (unsigned)(stage * kStage + token(tid, i));  // (past 2^31: not held)
+      entries[i] = pos < (unsigned)w.held ? paging::entry_of(w.pages, c.max_pages, c.shift, pos) : -1;
     }
   }
   // Loads go out whatever the place is, from the cache's first page where it is none, and are dropped then: what
@@ -244,7 +257,7 @@ struct Staging {
     const int tid = again(threadIdx.x);
 #pragma unroll
     for (int i = 0; i < S::NP; ++i) {
-      const bool in = stage * kStage + token(tid, i) < w.held && row_column(tid) < c.dh;
+      const bool in = (unsigned)(stage * kStage + token(tid, i)) < (unsigned)w.held && row_column(tid) < c.dh;
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[BOTH && VALUES][i][j >> 2][j & 3] = in ? x[BOTH && VALUES][i][j >> 2][j & 3] : 0.f;
     }
@@ -260,13 +273,13 @@ struct Staging {
   }
   // Raises the walk's base to the largest exponent of these rows.
   template <bool VALUES>
-  __device__ __forceinline__ void raise_base(Lds<INT8, DP> &s, const Cache &c, const Walk &w, int stage) {
+  __device__ __forceinline__ void raise_base(unsigned (&base)[2], const Cache &c, const Walk &w, int stage) {
     if constexpr (!INT8) {
       drop<VALUES>(c, w, stage);
       unsigned e = kLow;
 #pragma unroll
       for (int i = 0; i < S::NP; ++i) e = max(e, min(top_of_row<VALUES>(i) >> 23, kHigh));
-      atomicMax(&s.base[VALUES], e);
+      atomicMax(&base[VALUES], e);
     }
   }
 
@@ -302,6 +315,17 @@ struct Staging {
     if (marks != 0) atomicOr(to, marks);
   }
 
+  // Marks of tokens of the sequence on pages that the cache lacks.
+  __device__ __forceinline__ int lacking(const Walk &w, int stage) const {
+    const int tid = again(threadIdx.x);
+    int marks = 0;
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < S::NP; ++i)
+        if (entries[i] < 0 && (unsigned)(stage * kStage + token(tid, i)) < (unsigned)w.held) marks |= kOdd;
+    }
+    return marks;
+  }
   // stage: the one that is written, of the block's walk, and its buffers.
   __device__ __forceinline__ void put_keys(Lds<INT8, DP> &s, const Cache &c, const Walk &w, int stage, int buf, int third,
                                            unsigned base) {
@@ -309,7 +333,7 @@ struct Staging {
     char *to = s.stage(buf);
     int marks = 0;
     if constexpr (!INT8) {
-      marks = split_rows<false>(c, w, stage, to, s.ks[buf], base);
+      marks = split_rows<false>(c, w, stage, to, s.heads[buf].ks, base);
     } else {
       const int piece = tid & (S::kPieces - 1);
 #pragma unroll
@@ -323,22 +347,17 @@ struct Staging {
       }
       const float y = entries[NE - 1] >= 0 ? scale : 0.f;
       if (threadIdx.x < 2 * kStage) {
-        (threadIdx.x < kStage ? s.ks : s.vs)[buf][threadIdx.x & (kStage - 1)] = y;
+        (threadIdx.x < kStage ? s.heads[buf].ks : s.heads[buf].vs)[threadIdx.x & (kStage - 1)] = y;
         if (wild(y)) marks = kOdd;
       }
     }
-    if (!whole) {  // a token of the sequence on a page that the cache lacks
-#pragma unroll
-      for (int i = 0; i < S::NP; ++i)
-        if (entries[i] < 0 && stage * kStage + token(tid, i) < w.held) marks |= kOdd;
-    }
-    mark(&s.marks[third], marks);
+    mark(&s.marks[third], marks | lacking(w, stage));
   }
   __device__ __forceinline__ void put_values(Lds<INT8, DP> &s, const Cache &c, const Walk &w, int stage, int buf, int third,
                                              unsigned base) {
     char *to = s.stage(buf) + S::kKeys;
     if constexpr (!INT8) {
-      mark(&s.marks[third], split_rows<true>(c, w, stage, to, s.vs[buf], base));
+      mark(&s.marks[third], split_rows<true>(c, w, stage, to, s.heads[buf].vs, base));
     } else {
       // four tokens' values of a column lie together: eight bytes of a product's operand
 #pragma unroll
@@ -502,7 +521,7 @@ struct Rows {
           for (int j = 0; j < 4; ++j) s[kb][4 * i + j] *= x[j];
         }
     };
-    if (INT8 || (marks & kMixedKeys)) by_factors(lds.ks[buf]);
+    if (INT8 || (marks & kMixedKeys)) by_factors(lds.heads[buf].ks);
     if (masked) {
       const int left = seen() - pos0 - first;  // tokens from the first that the row sees
 #pragma unroll
@@ -529,7 +548,7 @@ struct Rows {
     // the probabilities times the values' factors, the largest of a row brought to [2^14, 2^15)
     float top;
     if (INT8 || (marks & kMixedValues)) {
-      by_factors(lds.vs[buf]);
+      by_factors(lds.heads[buf].vs);
       top = 0.f;
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) top = tiles::top_of(s[kb], top);
@@ -625,7 +644,40 @@ __device__ __forceinline__ int stages_of(const Cache &c, int group, int len, int
   return max(1, (n + kStage - 1) / kStage);
 }
 
-template <bool INT8, int DP, int Z>
+// The images of the stages that the walks will take: split once for all blocks of rows.  A workgroup a stage.
+template <int DP>
+__global__ void __launch_bounds__(kThreads) pack_stages(Args a) {
+  using S = Shape<false, DP>;
+  __shared__ unsigned base[2];
+  __shared__ int marks;
+  const int tid = threadIdx.x, i = (int)(blockIdx.x / a.most_stages), stage = (int)(blockIdx.x % a.most_stages), kv = i % a.c.kv_heads;
+  const SeqTile t = a.seqs[i / a.c.kv_heads];
+  const int end = __builtin_amdgcn_readfirstlane(a.ends[t.seq]);
+  const Walk walk{a.c.table + (int64_t)t.seq * a.c.max_pages, (int)paging::held(end, a.c.max_pages, a.c.shift), kv};
+  if (stage > 0 && stage * kStage >= walk.held) return;
+  Staging<false, DP, true> g;
+  g.look(a.c, walk, stage);
+  if (tid < 2) base[tid] = kLow;
+  if (tid == 2) marks = 0;
+  g.resolve(a.c);
+  g.load_keys(a.c, walk, stage);
+  g.load_values(a.c, walk, stage);
+  __syncthreads();
+  g.template raise_base<false>(base, a.c, walk, stage);
+  g.template raise_base<true>(base, a.c, walk, stage);
+  __syncthreads();
+  char *image = a.images + (int64_t)blockIdx.x * kImage<DP>;
+  Head *head = reinterpret_cast<Head *>(image + S::kBytes);
+  const unsigned kbase = base[0], vbase = base[1];
+  int found = g.template split_rows<false>(a.c, walk, stage, image, head->ks, kbase);
+  found |= g.template split_rows<true>(a.c, walk, stage, image + S::kKeys, head->vs, vbase);
+  g.mark(&marks, found | g.lacking(walk, stage));
+  __syncthreads();
+  if (tid == 0) head->base[0] = kbase, head->base[1] = vbase, head->marks = marks;
+}
+
+// PACKED: the stages are images already.
+template <bool INT8, int DP, int Z, bool PACKED>
 __global__ void __launch_bounds__(kThreads, 2) walk_blocks(Args a) {
   using S = Shape<INT8, DP>;
   constexpr int R = 8 / Z, ROWS = 32 * R, KB = 2 / Z;
@@ -716,42 +768,70 @@ __global__ void __launch_bounds__(kThreads, 2) walk_blocks(Args a) {
       constexpr bool kBoth = INT8 || Z > 1;
       Staging<INT8, DP, kBoth> g;
       Rows<INT8, DP> r;
-      g.look(a.c, walk, s0);
-      if (tid < 3) lds.marks[tid] = 0;
-      if (tid < 2) lds.base[tid] = kLow;
-      const bool good = r.start(a, lds, query(), live);
-      g.resolve(a.c);
-      __syncthreads();  // what is marked is cleared, the last block's buffers free
-      if (!good) Staging<INT8, DP, kBoth>::mark(&lds.marks[0], kOdd);
-      g.load_keys(a.c, walk, s0);
-      if constexpr (kBoth) g.load_values(a.c, walk, s0);
-      g.template raise_base<false>(lds, a.c, walk, s0);
-      if constexpr (kBoth) g.template raise_base<true>(lds, a.c, walk, s0);
-      if constexpr (!INT8) __syncthreads();
-      const unsigned kbase = __builtin_amdgcn_readfirstlane(lds.base[0]);
-      g.put_keys(lds, a.c, walk, s0, 0, 0, kbase);
-      if constexpr (!kBoth) {
-        g.load_values(a.c, walk, s0);
-        g.template raise_base<true>(lds, a.c, walk, s0);
+      // A stage's image on its way to LDS.
+      auto fetch = [&](int stage, int buf) {
+        const char *from = a.images + ((int64_t)((i0 + j) * a.c.kv_heads + kv) * a.most_stages + stage) * kImage<DP> + lane * 16;
+#pragma unroll
+        for (int k = 0; k < S::kBytes / 8192; ++k) tiles::copy16(from + (k * 8 + w) * 1024, lds.stage(buf) + (k * 8 + w) * 1024);
+        if (w == 0) tiles::copy16(from + S::kBytes, &lds.heads[buf]);
+      };
+      unsigned kbase = 0, vbase = 0;
+      if constexpr (PACKED) {
+        __syncthreads();  // the last block's buffers are free
+        if (tid == 0) lds.marks[0] = 0;
+        fetch(s0, 0);
+        const bool good = r.start(a, lds, query(), live);
         __syncthreads();
+        if (!good) g.mark(&lds.marks[0], kOdd);
+      } else {
+        g.look(a.c, walk, s0);
+        if (tid < 3) lds.marks[tid] = 0;
+        if (tid < 2) lds.base[tid] = kLow;
+        const bool good = r.start(a, lds, query(), live);
+        g.resolve(a.c);
+        __syncthreads();  // what is marked is cleared, the last block's buffers free
+        if (!good) Staging<INT8, DP, kBoth>::mark(&lds.marks[0], kOdd);
+        g.load_keys(a.c, walk, s0);
+        if constexpr (kBoth) g.load_values(a.c, walk, s0);
+        g.template raise_base<false>(lds.base, a.c, walk, s0);
+        if constexpr (kBoth) g.template raise_base<true>(lds.base, a.c, walk, s0);
+        if constexpr (!INT8) __syncthreads();
+        kbase = __builtin_amdgcn_readfirstlane(lds.base[0]);
+        g.put_keys(lds, a.c, walk, s0, 0, 0, kbase);
+        if constexpr (!kBoth) {
+          g.load_values(a.c, walk, s0);
+          g.template raise_base<true>(lds.base, a.c, walk, s0);
+          __syncthreads();
+        }
+        vbase = __builtin_amdgcn_readfirstlane(lds.base[1]);
+        g.put_values(lds, a.c, walk, s0, 0, 0, vbase);
+        g.look(a.c, walk, s0 + 1);
       }
-      const unsigned vbase = __builtin_amdgcn_readfirstlane(lds.base[1]);
-      g.put_values(lds, a.c, walk, s0, 0, 0, vbase);
-      g.look(a.c, walk, s0 + 1);
       constexpr int kUnscale = INT8 ? 0 : 127 + (int)kScaled;
-      r.f = __builtin_amdgcn_ldexpf(1.f, r.fe + (INT8 ? 0 : (int)kbase - kUnscale));
-      const int values_base = INT8 ? 0 : (int)vbase - kUnscale;
+      auto based = [&] { r.f = __builtin_amdgcn_ldexpf(1.f, r.fe + (INT8 ? 0 : (int)kbase - kUnscale)); };
+      based();
       bool odd = false;
       for (int i = s0; i < s1; ++i) {
         const int buf = (i - s0) & 1, third = (i - s0) % 3, after = (i - s0 + 1) % 3;
         const int pos0 = i * kStage, first = 32 * z;
         const bool more = i + 1 < s1;
-        __syncthreads();
-        const int marks = __builtin_amdgcn_readfirstlane(lds.marks[third]);
+        if constexpr (PACKED)
+          tiles::fetched();
+        else
+          __syncthreads();
+        const int marks = __builtin_amdgcn_readfirstlane(PACKED ? lds.marks[0] | lds.heads[buf].marks : lds.marks[third]);
         odd = (marks & kOdd) != 0;
         if (odd) break;
-        if (tid == 0) lds.marks[(i - s0 + 2) % 3] = 0;
-        if (more) {
+        if constexpr (PACKED) {
+          if (more) fetch(i + 1, buf ^ 1);
+          kbase = __builtin_amdgcn_readfirstlane(lds.heads[buf].base[0]);
+          vbase = __builtin_amdgcn_readfirstlane(lds.heads[buf].base[1]);
+          based();
+        } else if (tid == 0) {
+          lds.marks[(i - s0 + 2) % 3] = 0;
+        }
+        const int values_base = INT8 ? 0 : (int)vbase - kUnscale;
+        if (!PACKED && more) {
           g.resolve(a.c);
           g.load_keys(a.c, walk, i + 1);
           if constexpr (kBoth) g.load_values(a.c, walk, i + 1);
@@ -759,13 +839,13 @@ __global__ void __launch_bounds__(kThreads, 2) walk_blocks(Args a) {
         const bool mine = pos0 + first < most;
         f16 s[KB];
         if (mine) r.template products<KB>(lds, buf, first, s);
-        if (more) {
+        if (!PACKED && more) {
           g.put_keys(lds, a.c, walk, i + 1, buf ^ 1, after, kbase);
           if constexpr (!kBoth) g.load_values(a.c, walk, i + 1);
           g.look(a.c, walk, i + 2);
         }
         if (mine) r.template take<KB>(lds, buf, first, pos0, pos0 + first + 32 * KB > least, marks, values_base, s, row_sees);
-        if (more) g.put_values(lds, a.c, walk, i + 1, buf ^ 1, after, vbase);
+        if (!PACKED && more) g.put_values(lds, a.c, walk, i + 1, buf ^ 1, after, vbase);
       }
       bool some = row_sees() > s0 * kStage + 32 * z;  // whether the row sees a token of the wave's
       if (odd) {

@@ -411,3 +411,95 @@ def test_refusals(hip_ctx):
         x.attention_paged_chunk(t.s.cache, t.seqs, 4, t.ends, t.table)
     with nr.Context(0) as other, pytest.raises(ValueError, match="one context"):
         nr.Tensor.new(t.q, ctx=other).attention_paged_chunk(t.s.cache, t.seqs, 4, t.table, t.ends)
+
+
+# From 1024 rows of a kv head on a sequence the cached tokens are laid out for the matrix cores first (fp32): every
+# head size's layout, sequences of one and of none between, tables too wide for that.
+MANY = [
+    ([1100], [500], 16, 1, 1, 8, 0),
+    ([200, 300], [0, 700], 64, 14, 2, 40, 3),
+    ([260], [3000], 16, 8, 2, 64, 0),
+    ([400], [64], 32, 12, 4, 96, 1),
+    ([1030], [63], 1024, 1, 1, 32, 0),
+    ([512, 1, 0, 700], [2, 900, 7, 0], 16, 12, 3, 128, 0),
+    ([300], [400], 1024, 4, 1, 128, 1100),
+]
+
+
+@pytest.mark.parametrize("i", range(len(MANY)))
+def test_many_rows(hip_ctx, i):
+    new, context, page, H, Hk, dh, wider = MANY[i]
+    t = _Chunk(hip_ctx, new, context, page, H, Hk, dh, "f32", np.random.default_rng(40 + i), wider=wider).write()
+    got = t.run()
+    t.check(got)
+    assert_bits(t.run(), got, "the same call again")
+
+
+@pytest.mark.parametrize("gap", [20, 60, 100])
+@pytest.mark.parametrize("which", ["k", "v", "q"])
+def test_many_rows_of_very_different_size(hip_ctx, which, gap):
+    rng = np.random.default_rng(50 + gap)
+    t = _Chunk(hip_ctx, [300], [200], 16, 8, 2, 64, "f32", rng)
+    x = getattr(t, which)
+    x *= np.ldexp(np.float32(1), -(rng.integers(0, 2, len(x)) * gap)).astype(np.float32)[:, None]
+    t.check(t.write().run())
+
+
+def test_many_rows_with_what_is_not_finite(hip_ctx):
+    """A key, a query and a value that are not finite, a page that is missing, ends below the new tokens."""
+    c, rng, n, H, Hk, dh, page = hip_ctx, np.random.default_rng(60), 150, 16, 2, 32, 16
+    t = _Chunk(c, [n] * 5, [106] * 5, page, H, Hk, dh, "f32", rng).write()
+    clean, bound = t.reference()
+    clean, bound = clean.reshape(5, n, Hk, H // Hk, dh), bound.reshape(5, n, Hk, H // Hk, dh)
+    t.k[40, 3] = np.nan                   # sequence 0, head 0: every row
+    t.v[256 + 106 + 70, dh + 5] = np.inf  # sequence 1, head 1: the rows from 70 on, column 5
+    t.write()
+    t.q[2 * n + 9, 4] = np.nan            # sequence 2, row 9, the first query head
+    table, ends = t.s.table.copy(), np.array([256, 256, 256, 256, n - 1], np.int32)
+    table[3, 2] = -1
+    t.table, t.ends = c.to_device(table), c.to_device(ends)
+    got = t.run().reshape(5, n, Hk, H // Hk, dh)
+    assert np.isnan(got[0, :, 0]).all()
+    _check(got[0, :, 1], clean[0, :, 1], bound[0, :, 1], "beside a key that is NaN")
+    assert np.isposinf(got[1, 70:, 1, :, 5]).all()
+    rest = np.arange(dh) != 5
+    _check(got[1, 70:, 1][..., rest], clean[1, 70:, 1][..., rest], bound[1, 70:, 1][..., rest], "beside an infinite value")
+    _check(got[1, :70, 1], clean[1, :70, 1], bound[1, :70, 1], "before an infinite value")
+    _check(got[1, :, 0], clean[1, :, 0], bound[1, :, 0], "another head")
+    assert np.isnan(got[2, 9, 0, 0]).all()
+    others = np.ones((n, Hk, H // Hk), bool)
+    others[9, 0, 0] = False
+    _check(got[2][others], clean[2][others], bound[2][others], "beside a query that is NaN")
+    (k, v), q = t.stands()[3], t.q.reshape(5, n, H, dh)
+    at = np.arange(256)
+    seen = (at <= 106 + np.arange(n)[:, None]) & (at // page != 2)
+    ref, err = _rows(q[3], k, v, seen)
+    _check(got[3].reshape(n, H, dh), ref, err, "a page that is missing")
+    k, v = t.stands()[4]
+    ref, err = _rows(q[4], k, v, at <= np.arange(-1, n - 1)[:, None])
+    assert (got[4, 0] == 0).all()
+    _check(got[4].reshape(n, H, dh), ref, err, "an end below the new tokens")
+
+
+def test_many_rows_recorded_and_replayed(hip_ctx):
+    """What was laid out for one replay is not what the next reads: keys, values and ends change between them."""
+    c, rng = hip_ctx, np.random.default_rng(61)
+    t = _Chunk(c, [300, 2], [200, 50], 16, 16, 2, 64, "f32", rng).write()
+    w = 16 * 64
+    qd, out = c.to_device(t.q), c.empty((t.T, w))
+    step = lambda: c._check(L.load().numrs_hip_attention_paged_chunk(  # noqa: E731
+        c.handle, ctypes.byref(t.s.cache.pages), t.seqs.handle, qd.ptr, w, 16, t.table.ptr, t.most, t.ends.ptr, out.ptr, w))
+    step()
+    graph = nr.StepGraph(c, step)
+    for e in ([500, 52], [300, 52], [470, 10], [500, 2]):
+        t.k, t.v = rand(rng, t.k.shape), rand(rng, t.v.shape)
+        t.write()
+        t.ends.upload(np.array(e, np.int32))
+        graph.replay()
+        first = out.numpy()
+        out.fill(0)
+        step()
+        assert_bits(out.numpy(), first)
+        if e == [500, 52]:
+            t.check(first.reshape(t.T, 16, 64))
+    graph.close()
