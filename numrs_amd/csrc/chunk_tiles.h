@@ -4,19 +4,29 @@
 // r % group of token r / group, so that a block of rows is full whatever the group, and all of it reads the cached
 // tokens once.  As in packed_tiles.h a score is S^T = K Q^T and a result O^T += V^T P^T, with 32x32x16 products of
 // two-term fp16 splits, h + m, three products each (m h, h m, h h); 8-bit codes are exact in fp16, one term, two
-// products.  What the cache holds is split where it is staged:
-//   fp32    each token's row of a head, times the power of two that puts its largest magnitude into [2^14, 2^15);
-//   8 bits  the codes less 128.
-// The row's factor (that power of two's inverse, or its scale) is applied to its scores, and to its probabilities
-// before they are split: no token's size costs another its bits, and both formats are one walk.
+// products.  What the cache holds is split a stage of 64 tokens at a time:
+//   fp32    tokens times a power of two that they share, the base, or one of their own where their size is far from it
+//           (kBelow), which is then a factor of theirs;
+//   8 bits  the codes less 128; the scale is the token's factor.
+// A factor is applied to the token's scores, and to its probabilities before they are split: no token's size costs
+// another its bits, and both formats are one walk.
 //
-// A workgroup has eight waves: R = 8 / Z of 32 rows, in Z sets with every Z-th 32 tokens of a stage each.  The next
-// stage's keys are asked for before this one's scores are formed and split after them, its values before the
-// softmax and after the results: sixteen registers hold either on the way.
+// A workgroup has eight waves: R = 8 / Z of 32 rows, in Z sets with every Z-th 32 tokens of a stage each.  Z is 1 for
+// many rows, where a stage that is read feeds twice as many products, and 2 for few.  Stages lie in LDS twice.  The next
+// one's keys are asked for before this one's scores are formed and split after them, its values before the softmax
+// and after the results.  Where many blocks of rows read the same tokens, pack_stages splits them once, into images of
+// what a stage is in LDS, and a walk copies those: neither registers nor instructions are spent on them.
 //
 // The work is (kv head, block of rows, stage of tokens), in that order.  It is dealt evenly to one workgroup a CU,
 // whatever the lengths, which only the device knows; a block that is cut leaves parts (m, l, O) that
 // join_parts adds in order in a second launch: no workgroup waits for another.
+//
+// What bounds it, on MI355X: 8192 tokens over 6144 cached on the mean, 16 heads of 128 in groups of 8, fp32, take 1643
+// us, 293 TFLOP/s of the formula's and so 878 of the matrix cores' fp16, where a large library product in fp16 reaches
+// 1085; the cores are busy for about half of the time at the 1.5 GHz that the power leaves, the rest is softmax and
+// splits of probabilities, which two waves a SIMD overlap in part.  Waves half a stage apart, scores formed beside the
+// stage before's softmax, wave priorities and deeper prefetch gave nothing.  512 tokens over 8192, 32 heads in groups
+// of 4: 259 us, 27 of it images, 16 joins.  16 tokens over 131072, one kv head: 69 us, 134 MB, 61 of it the walk.
 #pragma once
 
 #include "packed_tiles.h"
@@ -197,8 +207,8 @@ struct Staging {
     const int tid = again(threadIdx.x);
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
-      const unsigned pos = (unsigned)(stage * kStage + token(tid, i));  // (past 2^31: not held)
-      entries[i] = pos < (unsigned)w.held ? paging::entry_of(w.pages, c.max_pages, c.shift, pos) : -1;
+      const int pos = stage * kStage + token(tid, i);
+      entries[i] = pos < w.held ? paging::entry_of(w.pages, c.max_pages, c.shift, pos) : -1;
     }
   }
   // Loads go out whatever the place is, from the cache's first page where it is none, and are dropped then: what
@@ -257,7 +267,7 @@ struct Staging {
     const int tid = again(threadIdx.x);
 #pragma unroll
     for (int i = 0; i < S::NP; ++i) {
-      const bool in = (unsigned)(stage * kStage + token(tid, i)) < (unsigned)w.held && row_column(tid) < c.dh;
+      const bool in = stage * kStage + token(tid, i) < w.held && row_column(tid) < c.dh;
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[BOTH && VALUES][i][j >> 2][j & 3] = in ? x[BOTH && VALUES][i][j >> 2][j & 3] : 0.f;
     }
@@ -322,7 +332,7 @@ struct Staging {
     if (!whole) {
 #pragma unroll
       for (int i = 0; i < S::NP; ++i)
-        if (entries[i] < 0 && (unsigned)(stage * kStage + token(tid, i)) < (unsigned)w.held) marks |= kOdd;
+        if (entries[i] < 0 && stage * kStage + token(tid, i) < w.held) marks |= kOdd;
     }
     return marks;
   }

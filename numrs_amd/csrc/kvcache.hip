@@ -505,6 +505,8 @@ int numrs_hip_kv_cache_append(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cach
   if (paging::bad_grid(s.tiles * (hk + 2 * parts)))
     return fail(ctx, NUMRS_HIP_E_SHAPE, "%s: too many tokens times heads", what);
   if (s.total == 0) return NUMRS_HIP_OK;
+  if (q != nullptr && paging::rows_meet(qkv, (heads + 2 * hk) * dh, q, heads * dh))
+    return fail(ctx, NUMRS_HIP_E_INVALID, "%s: the queries' result overlaps the projection", what);
   if (int rc = s.keep()) return rc;
   DeviceScope dev(ctx);
   AppendArgs b{{device_cache(*cache, table, max_pages), s.in_order, ends, nullptr, nullptr, nullptr, nullptr, ld},

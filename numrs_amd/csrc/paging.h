@@ -99,6 +99,12 @@ inline bool bad_stride(int64_t ld, int64_t width) { return ld < width || ld >= i
 // More workgroups of 256 threads than a launch, of at most 2^32 - 1 threads, can have.
 inline bool bad_grid(int64_t groups) { return groups >= int64_t{1} << 24; }
 
+// Whether the first rows of two arrays meet, na and nb floats from a and b on.
+inline bool rows_meet(const float *a, int64_t na, const float *b, int64_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + (uintptr_t)nb * sizeof(float) && y < x + (uintptr_t)na * sizeof(float);
+}
+
 // Lengths of a packed batch: their sum, or -1 if one is negative or they pass 2^30 tokens.
 inline int64_t packed_total(const int64_t *lengths, int64_t n) {
   int64_t total = 0;

@@ -503,3 +503,34 @@ def test_many_rows_recorded_and_replayed(hip_ctx):
         if e == [500, 52]:
             t.check(first.reshape(t.T, 16, 64))
     graph.close()
+
+
+def test_many_rows_of_many_sequences(hip_ctx):
+    """600 sequences of 16 tokens and 64 heads on one key head: more of them than a workgroup has threads."""
+    rng = np.random.default_rng(62)
+    t = _Chunk(hip_ctx, [16] * 600, rng.integers(0, 50, 600).tolist(), 16, 64, 1, 8, "f32", rng).write()
+    got = t.run()
+    t.check(got, only=[0, 1, 255, 511, 512, 513, 598, 599])
+    assert np.isfinite(got).all()
+
+
+def test_refusals_of_sizes_and_places(hip_ctx):
+    """Results over their inputs, tables and groups past what is counted in 32 bits."""
+    c, lib, rng = hip_ctx, L.load(), np.random.default_rng(63)
+    t = _Chunk(c, [5, 3], [2, 0], 16, 4, 2, 16, "f32", rng).write()
+    h, cp, fn = c.handle, ctypes.byref(t.s.cache.pages), lib.numrs_hip_attention_paged_chunk
+    q, out = c.to_device(t.q), c.empty((8, 64))
+    args = lambda dst, most=t.most: [h, cp, t.seqs.handle, q.ptr, 64, 4, t.table.ptr, most, t.ends.ptr, dst, 64]  # noqa: E731
+    assert fn(*args(out.ptr)) == 0
+    assert fn(*args(q.ptr)) == L.E_INVALID and fn(*args(q.ptr + 63 * 4)) == L.E_INVALID
+    assert fn(*args(q.ptr - 63 * 4)) == L.E_INVALID
+    assert fn(*args(out.ptr, 2 ** 27)) == L.E_SHAPE
+    one = nr.KVCache(4, 16, 1, 8, "f32", ctx=c)
+    long = nr.PackedSequences([40000], ctx=c)
+    assert fn(h, ctypes.byref(one.pages), long.handle, q.ptr, 65535 * 8, 65535, t.table.ptr, 1, t.ends.ptr, out.ptr,
+              65535 * 8) == L.E_SHAPE
+    x, app = c.to_device(rand(rng, (8, 192))), lib.numrs_hip_kv_cache_append
+    args = lambda dst: [h, cp, t.seqs.handle, x.ptr, 192, None, None, 1e-6, None, dst, 192, 4, t.table.ptr, t.most,  # noqa: E731
+                        t.ends.ptr]
+    assert app(*args(x.ptr)) == L.E_INVALID and app(*args(x.ptr + 127 * 4)) == L.E_INVALID
+    assert app(*args(x.ptr + 128 * 4)) == 0  # beside the projection, in the same rows
