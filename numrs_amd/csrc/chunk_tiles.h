@@ -992,19 +992,28 @@ __global__ void __launch_bounds__(256) join_parts(Args a, int wgs) {
       }
       return lo;
     };
-    for (int i = blockIdx.x * 4 + w; i < rows[0][256]; i += gridDim.x * 4) {
-      const int at = find(0, i), p = p0 + at, r = i - rows[0][at], half = lane >> 5, d = 4 * (lane & 31);
+    // a wave's rows follow each other: the block is looked up once
+    const int waves = gridDim.x * 4, share = (rows[0][256] + waves - 1) / waves;
+    const int i0 = min((int)(blockIdx.x * 4 + w) * share, rows[0][256]), i1 = min(i0 + share, rows[0][256]);
+    int at = i0 < i1 ? __builtin_amdgcn_readfirstlane(find(0, i0)) : 0;
+    for (int i = i0; i < i1; ++i) {
+      while (rows[0][at + 1] <= i) ++at;
+      const int p = p0 + at, r = i - rows[0][at], half = lane >> 5, d = 4 * (lane & 31);
       const Cut cut = a.cuts[p];
+      f4 y[kAhead / 2];
+      auto ask = [&](int k0) {
+#pragma unroll
+        for (int k = 0; k < kAhead / 2; ++k)  // past the last: read again, not added
+          y[k] = *reinterpret_cast<const f4 *>(part(p, min(k0 + 2 * k + half, cut.parts - 1)) + 2 * ROWS + r * DP + min(d, DP - 4));
+      };
       float m = kNever, l = -1.f;
       if (lane < cut.parts) m = part(p, lane)[r], l = part(p, lane)[ROWS + r];
+      ask(0);
       const float top = wave_max(l < 0.f ? kNever : m), f = l < 0.f ? 0.f : __builtin_amdgcn_exp2f(m - top);
       const bool some = __any(!(l < 0.f));  // (NaN too)
       f4 o{};
       for (int k0 = 0; k0 < cut.parts; k0 += kAhead) {
-        f4 y[kAhead / 2];
-#pragma unroll
-        for (int k = 0; k < kAhead / 2; ++k)  // past the last: read again, not added
-          y[k] = *reinterpret_cast<const f4 *>(part(p, min(k0 + 2 * k + half, cut.parts - 1)) + 2 * ROWS + r * DP + min(d, DP - 4));
+        if (k0 > 0) ask(k0);
 #pragma unroll
         for (int k = 0; k < kAhead / 2; ++k) {
           const float by = __shfl(f, k0 + 2 * k + half);
