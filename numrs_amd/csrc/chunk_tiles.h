@@ -48,6 +48,12 @@ typedef unsigned u2 __attribute__((ext_vector_type(2)));
 typedef unsigned long long mask64;
 
 constexpr int kThreads = 512, kStage = 64;  // threads of a workgroup, tokens of a stage
+// Units that a block counts beside its stages, for its queries, its first stage's wait and its results: without them the
+// workgroups with many short blocks were the last.  None, 1, 2, 3 and 4 of them, us: five pieces of prompts beside 24
+// single tokens over 8 bits 164, 139, 126, 129, 129; 2048 tokens each over 6144, 0, 16384 and 2000 1629, 1502, 1400,
+// 1376, 1386; 512 over 8192 257, 254, 248, 247, 250; 100 each over 500, six times, 46, 37, 40, 39, 39; 16 over
+// 131056, one block, 71, 72, 74, 73, 74 (2048 stages are 8 for each workgroup, 2051 are 9 for some).
+constexpr int kTurn = 3;
 
 // What a cut block's parts are joined into: written by the workgroup that has its first stage.
 struct Cut {
@@ -703,7 +709,7 @@ __global__ void __launch_bounds__(kThreads, 2) walk_blocks(Args a) {
     if (i0 + tid < a.n) {
       const SeqTile t = a.seqs[i0 + tid];
       const int end = a.ends[t.seq], blocks = (t.len * a.group + ROWS - 1) / ROWS;
-      for (int b = 0; b < blocks; ++b) v += stages_of<ROWS>(a.c, a.group, t.len, end, b);
+      for (int b = 0; b < blocks; ++b) v += kTurn + stages_of<ROWS>(a.c, a.group, t.len, end, b);
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -748,13 +754,16 @@ __global__ void __launch_bounds__(kThreads, 2) walk_blocks(Args a) {
     int block = 0, stages;
     for (;; ++block) {
       stages = stages_of<ROWS>(a.c, a.group, t.len, end, block);
-      if (x < at + stages) break;
-      at += stages;
+      if (x < at + kTurn + stages) break;
+      at += kTurn + stages;
     }
     for (; u < end_unit && block * ROWS < rows; ++block) {
       stages = stages_of<ROWS>(a.c, a.group, t.len, end, block);
-      const int s0 = (int)(x - at), s1 = (int)min((int64_t)stages, s0 + (end_unit - u));
-      const int64_t first_unit = u - s0;  // of the block
+      const int u0 = (int)(x - at), u1 = (int)min((int64_t)(kTurn + stages), u0 + (end_unit - u));
+      const int64_t first_unit = u - u0;  // of the block
+      u += u1 - u0, x += u1 - u0, at += kTurn + stages;
+      const int s0 = max(0, u0 - kTurn), s1 = u1 - kTurn;
+      if (s0 >= s1) continue;
 
       // the lane's row, and what the wave's first and last see
       const int row = block * ROWS + 32 * rw + c;
@@ -934,9 +943,7 @@ __global__ void __launch_bounds__(kThreads, 2) walk_blocks(Args a) {
           }
       }
       if (tid == 0 && s0 == 0 && !whole)
-        a.cuts[p] = {owner(first_unit + stages - 1) - p + 1, block * ROWS, min(ROWS, rows - block * ROWS), t.row0, kv * a.group};
-      u += s1 - s0;
-      x += s1 - s0, at += stages;
+        a.cuts[p] = {owner(first_unit + kTurn + stages - 1) - p + 1, block * ROWS, min(ROWS, rows - block * ROWS), t.row0, kv * a.group};
     }
   }
 }
