@@ -507,7 +507,7 @@ int numrs_hip_attention_paged(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cach
  * largest of its 64 tokens.  What is not finite, has its largest magnitude outside
  * 2^-60 .. 2^60, lies 2^64 from its neighbours or on a page that is missing is
  * taken in plain fp32 together with the tokens beside it, some hundred times
- * slower.  Of an fp32 cache that a sequence reads with 1024 rows or more (tokens
+ * slower.  Of an fp32 cache that a sequence reads with 2048 rows or more (tokens
  * times heads / kv_heads) a workspace of up to 1 GB has the tokens laid out.
  * No backward, no atomics on values: the same call gives the same bits. */
 int numrs_hip_attention_paged_chunk(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cache,

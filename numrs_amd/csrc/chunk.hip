@@ -14,15 +14,16 @@ constexpr float kLog2e = 1.44269504088896341f;
 
 // From kManyRows query rows of a kv head on a sequence, over caches in fp32, stages are made images first, which costs
 // a pass over the cached tokens and saves every block of 256 rows its own splitting.  On MI355X, without against with,
-// us, 32 heads of 128 in groups of 4 over 8192 tokens: 256 rows 68, 81; 512 rows 91, 101; 1024 rows 158, 156; 2048
-// rows 268, 251; of four sequences in groups of 8: 1024 rows over 8192 158, 156; 2048 over 2048 109, 104; 16384 rows
-// over 2000 to 16384 2000, 1643; heads of 64 over 2048: 1024 rows 74, 75; 2048 rows 120, 116.  The images have room
-// for all that the pages can hold, since only the device knows what they do; past kMostImages they are not made.
-constexpr int64_t kManyRows = 1024, kMostImages = int64_t{1} << 30;
+// us, 32 heads of 128 in groups of 4 over 8192 tokens: 256 rows 70, 84; 512 rows 95, 105; 1024 rows 145, 149; 2048
+// rows 260, 242; of four sequences in groups of 8: 1024 rows over 8192 147, 146; 2048 over 2048 101, 97; 4096 over none
+// 65, 63; 16384 over 0 to 16384 1546, 1352; heads of 64 over 2048: 1024 rows 67, 71; 2048 rows 110, 110.  The images
+// have room for all that the pages can hold, since only the device knows what they do; past kMostImages they are not
+// made.
+constexpr int64_t kManyRows = 2048, kMostImages = int64_t{1} << 30;
 // Up to so many rows blocks have 128 in two sets of waves, beyond 256 in one, which reads the tokens half as often.
-// 256 against 128, us: 128 rows over 131072 tokens 68, 69; 32 heads of 128 over 8192, fp32 and 8 bits: 32 rows 44, 44
-// and 35, 33; 128 rows 51, 51 and 40, 42; 256 rows 65, 65 and 52, 52; 512 rows 93, 113 and 74, 87; eight sequences
-// over 500, heads of 64: 64 rows 25, 24; 256 rows 38, 34; 512 rows 47, 53.
+// 256 against 128, us: 128 rows over 131072 tokens 70, 71; 32 heads of 128 over 8192, fp32 and 8 bits: 32 rows 44, 44
+// and 34, 33; 128 rows 50, 51 and 39, 41; 256 rows 68, 66 and 51, 52; 512 rows 95, 97 and 68, 75; eight sequences
+// over 500, heads of 64: 64 rows 24, 24; 128 rows 27, 28; 256 rows 35, 32; 512 rows 46, 47.
 constexpr int64_t kFewRows = 256;
 
 template <bool INT8, int DP, int Z, bool PACKED>
@@ -101,7 +102,7 @@ extern "C" int numrs_hip_attention_paged_chunk(numrs_hip_ctx *ctx, const numrs_h
   if (int rc = s.keep()) return rc;
   DeviceScope dev(ctx);
   // Sequences of one row go the way of the decoding steps, made for few rows and many tokens: 24 of them, of 1 to 5000
-  // tokens, beside five pieces of prompts, 8 heads of 128 in 8 bits: 194 us as blocks of rows, 174 so.
+  // tokens, beside five pieces of prompts, 8 heads of 128 in 8 bits: 20 us less than as blocks of rows.
   if (s.singles > 0)
     if (int rc = paged_steps(ctx, *cache, q, ld_q, heads, table, max_pages, ends, s.singles, s.single, out, ld_out))
       return rc;

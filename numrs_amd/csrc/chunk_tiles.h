@@ -21,12 +21,11 @@
 // whatever the lengths, which only the device knows; a block that is cut leaves parts (m, l, O) that
 // join_parts adds in order in a second launch: no workgroup waits for another.
 //
-// What bounds it, on MI355X: 8192 tokens over 6144 cached on the mean, 16 heads of 128 in groups of 8, fp32, take 1643
-// us, 293 TFLOP/s of the formula's and so 878 of the matrix cores' fp16, where a large library product in fp16 reaches
-// 1085; the cores are busy for about half of the time at the 1.5 GHz that the power leaves, the rest is softmax and
-// splits of probabilities, which two waves a SIMD overlap in part.  Waves half a stage apart, scores formed beside the
-// stage before's softmax, wave priorities and deeper prefetch gave nothing.  512 tokens over 8192, 32 heads in groups
-// of 4: 259 us, 27 of it images, 16 joins.  16 tokens over 131072, one kv head: 69 us, 134 MB, 61 of it the walk.
+// What bounds it, on MI355X: 8192 tokens over 6144 cached on the mean, 16 heads of 128 in groups of 8, fp32, take 1352
+// us, 355 TFLOP/s of the formula's and so 1066 of the matrix cores' fp16, where a large library product in fp16 reaches
+// 1085 to 1295: the power, at which the clock is 1.4 GHz.  Waves half a stage apart, scores formed beside the stage
+// before's softmax, wave priorities and deeper prefetch gave nothing.  512 tokens over 8192, 32 heads in groups of 4:
+// 251 us, 27 of it images, 14 joins.  16 tokens over 131072, one kv head: 70 to 77 us, 134 MB, 61 of it the walk.
 #pragma once
 
 #include "packed_tiles.h"

@@ -413,8 +413,8 @@ def test_refusals(hip_ctx):
         nr.Tensor.new(t.q, ctx=other).attention_paged_chunk(t.s.cache, t.seqs, 4, t.table, t.ends)
 
 
-# From 1024 rows of a kv head on a sequence the cached tokens are laid out for the matrix cores first (fp32): every
-# head size's layout, sequences of one and of none between, tables too wide for that.
+# From 2048 rows of a kv head on a sequence the cached tokens are laid out for the matrix cores first (fp32): fewer and
+# more of them, every head size's layout, sequences of one and of none between, tables too wide for that.
 MANY = [
     ([1100], [500], 16, 1, 1, 8, 0),
     ([200, 300], [0, 700], 64, 14, 2, 40, 3),
@@ -423,6 +423,11 @@ MANY = [
     ([1030], [63], 1024, 1, 1, 32, 0),
     ([512, 1, 0, 700], [2, 900, 7, 0], 16, 12, 3, 128, 0),
     ([300], [400], 1024, 4, 1, 128, 1100),
+    ([2100], [500], 16, 1, 1, 8, 0),
+    ([300, 340], [0, 700], 64, 14, 2, 40, 3),
+    ([700], [64], 32, 12, 4, 96, 1),
+    ([2050], [63], 1024, 1, 1, 32, 0),
+    ([520], [400], 1024, 4, 1, 128, 1100),
 ]
 
 
@@ -435,19 +440,21 @@ def test_many_rows(hip_ctx, i):
     assert_bits(t.run(), got, "the same call again")
 
 
+@pytest.mark.parametrize("n", [300, 600])
 @pytest.mark.parametrize("gap", [20, 60, 100])
 @pytest.mark.parametrize("which", ["k", "v", "q"])
-def test_many_rows_of_very_different_size(hip_ctx, which, gap):
+def test_many_rows_of_very_different_size(hip_ctx, which, gap, n):
     rng = np.random.default_rng(50 + gap)
-    t = _Chunk(hip_ctx, [300], [200], 16, 8, 2, 64, "f32", rng)
+    t = _Chunk(hip_ctx, [n], [200], 16, 8, 2, 64, "f32", rng)
     x = getattr(t, which)
     x *= np.ldexp(np.float32(1), -(rng.integers(0, 2, len(x)) * gap)).astype(np.float32)[:, None]
     t.check(t.write().run())
 
 
-def test_many_rows_with_what_is_not_finite(hip_ctx):
+@pytest.mark.parametrize("H", [16, 32])
+def test_many_rows_with_what_is_not_finite(hip_ctx, H):
     """A key, a query and a value that are not finite, a page that is missing, ends below the new tokens."""
-    c, rng, n, H, Hk, dh, page = hip_ctx, np.random.default_rng(60), 150, 16, 2, 32, 16
+    c, rng, n, Hk, dh, page = hip_ctx, np.random.default_rng(60), 150, 2, 32, 16
     t = _Chunk(c, [n] * 5, [106] * 5, page, H, Hk, dh, "f32", rng).write()
     clean, bound = t.reference()
     clean, bound = clean.reshape(5, n, Hk, H // Hk, dh), bound.reshape(5, n, Hk, H // Hk, dh)
@@ -481,14 +488,15 @@ def test_many_rows_with_what_is_not_finite(hip_ctx):
     _check(got[4].reshape(n, H, dh), ref, err, "an end below the new tokens")
 
 
-def test_many_rows_recorded_and_replayed(hip_ctx):
+@pytest.mark.parametrize("H", [16, 32])
+def test_many_rows_recorded_and_replayed(hip_ctx, H):
     """What was laid out for one replay is not what the next reads: keys, values and ends change between them."""
     c, rng = hip_ctx, np.random.default_rng(61)
-    t = _Chunk(c, [300, 2], [200, 50], 16, 16, 2, 64, "f32", rng).write()
-    w = 16 * 64
+    t = _Chunk(c, [300, 2], [200, 50], 16, H, 2, 64, "f32", rng).write()
+    w = H * 64
     qd, out = c.to_device(t.q), c.empty((t.T, w))
     step = lambda: c._check(L.load().numrs_hip_attention_paged_chunk(  # noqa: E731
-        c.handle, ctypes.byref(t.s.cache.pages), t.seqs.handle, qd.ptr, w, 16, t.table.ptr, t.most, t.ends.ptr, out.ptr, w))
+        c.handle, ctypes.byref(t.s.cache.pages), t.seqs.handle, qd.ptr, w, H, t.table.ptr, t.most, t.ends.ptr, out.ptr, w))
     step()
     graph = nr.StepGraph(c, step)
     for e in ([500, 52], [300, 52], [470, 10], [500, 2]):
@@ -501,14 +509,15 @@ def test_many_rows_recorded_and_replayed(hip_ctx):
         step()
         assert_bits(out.numpy(), first)
         if e == [500, 52]:
-            t.check(first.reshape(t.T, 16, 64))
+            t.check(first.reshape(t.T, H, 64))
     graph.close()
 
 
-def test_many_rows_of_many_sequences(hip_ctx):
-    """600 sequences of 16 tokens and 64 heads on one key head: more of them than a workgroup has threads."""
+@pytest.mark.parametrize("n", [16, 33])
+def test_many_rows_of_many_sequences(hip_ctx, n):
+    """600 sequences of a few tokens and 64 heads on one key head: more of them than a workgroup has threads."""
     rng = np.random.default_rng(62)
-    t = _Chunk(hip_ctx, [16] * 600, rng.integers(0, 50, 600).tolist(), 16, 64, 1, 8, "f32", rng).write()
+    t = _Chunk(hip_ctx, [n] * 600, rng.integers(0, 50, 600).tolist(), 16, 64, 1, 8, "f32", rng).write()
     got = t.run()
     t.check(got, only=[0, 1, 255, 511, 512, 513, 598, 599])
     assert np.isfinite(got).all()
