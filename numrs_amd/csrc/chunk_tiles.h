@@ -87,7 +87,7 @@ __device__ __forceinline__ bool wild(float x) { return !(x == 0.f || (fabsf(x) >
 __device__ __forceinline__ float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 // A magnitude's exponent as its bits have it, 127 for [1, 2).  Tokens whose largest magnitude has one of base - kBelow
-// to base + 1 are split at the walk's base, which brings that to [2^13, 2^14) (so theirs to [2^5, 2^15), and the
+// to base + 1 are split at the base, the first stage's largest or an image's own, which brings that to [2^13, 2^14) (so theirs to [2^5, 2^15), and the
 // split's smallest step to 2^-29 of it at most); others at their own, and have a factor.  Past kApart it is odd.
 constexpr unsigned kLow = 127 - 60, kHigh = 127 + 60, kBelow = 8, kApart = 64, kScaled = 13;
 __device__ __forceinline__ float power(unsigned bits) { return __builtin_bit_cast(float, bits << 23); }

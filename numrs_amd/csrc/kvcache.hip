@@ -265,7 +265,10 @@ struct AppendArgs {
 };
 
 // Keys, normed and rotated, and values on their way into the cache: a workgroup a tile and kv head, a thread four
-// positions and eight columns.  After them a workgroup a tile's part and some of the query heads.
+// positions and eight columns.  After them a workgroup a tile's part and some of the query heads.  A projection of 460 MB
+// into fp32 pages 195 us (4.7 TB/s, the memory's); a token for each of 40 sequences into 8 bits 8.3 us, a chain of loads and
+// arithmetic.  Rows of a group that are not there are skipped whole: their instructions, fetched for nothing, took 1 us
+// of a step and 14 of the large call.
 template <bool INT8, bool PAST>
 __global__ void __launch_bounds__(256) append_rows(AppendArgs b) {
   if (blockIdx.x >= b.keys) {

@@ -284,7 +284,9 @@ __device__ __forceinline__ void rotate_part(const RowArgs &a, const SeqTile &t, 
   }
 }
 
-// Parts of a tile, and how many heads a workgroup takes so that there are several workgroups a CU.
+// Parts of a tile, and how many heads a workgroup takes so that there are eight workgroups a CU.  2, 4, 8 and 16 of them, us:
+// 62 MB of ragged prompts 13.9, 13.1, 12.6, 15.5 (angles are formed again for each part of the heads); 4096 tokens of 24 heads
+// of 64 10.9, 10.2, 10.0, 12.8; 16384 tokens of 32 heads of 128 103, 103, 103, 106.
 inline int parts_of(int lanes) { return kTile / (256 >> lanes) > 0 ? kTile / (256 >> lanes) : 1; }
 inline int heads_each(const numrs_hip_ctx *ctx, int64_t parts, int slots) {
   const int64_t want = 8 * (int64_t)ctx->num_cus, split = (want + parts - 1) / parts;
