@@ -610,3 +610,79 @@ def test_a_recorded_training_step(engine):
     assert abs(a.q_norm.values() - 1).max() > 0
     graph.close()
     del filler
+
+
+def test_calls_past_the_caches(hip_ctx):
+    """Calls of more than 128 MB, whose rows go past the caches, against calls of their sequences one by one: the same
+    bits; the weights' gradients, sums of four rounded ones, within half a step of each."""
+    c, lib, H, Hk, dh, n = hip_ctx, L.load(), 20, 4, 128, 1750
+    W = (H + 2 * Hk) * dh
+    rng = np.random.default_rng(80)
+    x, dy = rand(rng, (4 * n, W)), rand(rng, (4 * n, W))
+    rot = nr.Rotary(dh, layout="pairs")
+    xd, gd, y, dx = c.to_device(x), c.to_device(dy), c.empty(x.shape), c.empty(x.shape)
+    wq, wk, r = c.to_device(rand(rng, dh)), c.to_device(rand(rng, dh)), ctypes.byref(rot.spec)
+
+    def both(seqs, ends, at, to, back, dq, dk):
+        at *= W * 4
+        c._check(lib.numrs_hip_qk_rotary_forward(c.handle, seqs.handle, ends, xd.ptr + at, W, wq.ptr, wk.ptr, EPS, r,
+                                                 to.ptr, W, H, Hk, dh))
+        c._check(lib.numrs_hip_qk_rotary_backward(c.handle, seqs.handle, ends, xd.ptr + at, W, wq.ptr, wk.ptr, EPS, r,
+                                                  gd.ptr + at, W, back.ptr, W, dq.ptr, dk.ptr, H, Hk, dh, 0))
+
+    dq, dk, one_y, one_dx = c.empty((dh,)), c.empty((dh,)), c.empty((n, W)), c.empty((n, W))
+    both(nr.PackedSequences([n] * 4, ctx=c), None, 0, y, dx, dq, dk)
+    whole, got_y, got_dx = [dq.numpy(), dk.numpy()], y.numpy(), dx.numpy()
+    parts, one = [], nr.PackedSequences([n], ctx=c)
+    for i in range(4):
+        both(one, None, i * n, one_y, one_dx, dq, dk)
+        parts.append([dq.numpy().astype(np.float64), dk.numpy().astype(np.float64)])
+        assert_bits(one_y.numpy(), got_y[i * n:(i + 1) * n], "y")
+        assert_bits(one_dx.numpy(), got_dx[i * n:(i + 1) * n], "dx")
+    for k in range(2):
+        p = np.array([q[k] for q in parts])
+        # what 64-bit sums leave of terms that cancel: a head's normed values are below sqrt(dh), gradients below 8
+        size = 4 * n * (H if k == 0 else Hk) * dh ** 0.5 * 8
+        bound = HALF * (abs(p).sum(0) + abs(p.sum(0))) + 64 * U64 * size * 4 * n
+        assert (abs(whole[k] - p.sum(0)) <= bound).all()
+    # the same call again, and both in place
+    both(nr.PackedSequences([n] * 4, ctx=c), None, 0, y, dx, dq, dk)
+    assert_bits(dq.numpy(), whole[0])
+    assert_bits(dk.numpy(), whole[1])
+    all4 = nr.PackedSequences([n] * 4, ctx=c)
+    c._check(lib.numrs_hip_qk_rotary_backward(c.handle, all4.handle, None, xd.ptr, W, wq.ptr, wk.ptr, EPS, r, gd.ptr, W,
+                                              gd.ptr, W, None, None, H, Hk, dh, 0))
+    assert_bits(gd.numpy(), got_dx, "gradient in place")
+    c._check(lib.numrs_hip_qk_rotary_forward(c.handle, all4.handle, None, xd.ptr, W, wq.ptr, wk.ptr, EPS, r, xd.ptr, W,
+                                             H, Hk, dh))
+    assert_bits(xd.numpy(), got_y, "in place")
+
+
+@pytest.mark.parametrize("format", ["f32", "int8"])
+def test_append_past_the_caches(hip_ctx, format):
+    """An append of more than 128 MB of keys and values, against appends of its sequences one by one."""
+    c, lib, H, Hk, dh, n, page = hip_ctx, L.load(), 20, 20, 128, 1700, 64
+    rng = np.random.default_rng(81)
+    t = _Case([n] * 4, H, Hk, dh, rng, starts=[0, 5, 64, 130])
+    total = [n + s for s in t.starts]
+    s = _Paged(c, total, page, Hk, dh, format, rng)
+    xd, wq, wk, q = c.to_device(t.x), _d(c, t.wq), _d(c, t.wk), c.empty((4 * n, H * dh))
+    before = s.raw()
+
+    def call(seqs, row, i):
+        c._check(lib.numrs_hip_kv_cache_append(
+            c.handle, ctypes.byref(s.cache.pages), seqs.handle, xd.ptr + row * t.W * 4, t.W, wq.ptr, wk.ptr, EPS,
+            ctypes.byref(t.rot.spec), q.ptr + row * H * dh * 4, H * dh, H, s.td.ptr + i * s.table.shape[1] * 4,
+            s.table.shape[1], s.ends.ptr + i * 4))
+
+    call(nr.PackedSequences([n] * 4, ctx=c), 0, 0)
+    want, queries = s.raw(), q.numpy()
+    for a, b in zip((s.cache.k, s.cache.v, s.cache.k_scale, s.cache.v_scale), before):
+        a.upload(b)
+    q.fill(0)
+    one = nr.PackedSequences([n], ctx=c)
+    for i in range(4):
+        call(one, i * n, i)
+    for got, ref in zip(s.raw(), want):
+        assert np.array_equal(got, ref, equal_nan=got.dtype == np.float32)
+    assert_bits(q.numpy(), queries, "q")
