@@ -166,10 +166,11 @@ __global__ void __launch_bounds__(256)
   if (dk != nullptr) dk[d] = (float)(acc_k ? dk[d] + k : k);
 }
 
-// Whether rows go past the caches: where a call reads and writes more than half of the last cache's 256 MB, so that
-// they would take the place of what the next kernel reads.
+// Whether rows go past the caches: where a call reads and writes more than the last cache's 256 MB.  On MI355X, through
+// against past, us: forward of 64 MB 25.1, 24.6; 128 MB 42, 54; 256 MB 108, 107; 512 MB 207, 195; forward and backward of
+// 32 MB 45, 43; 48 MB 57, 57; 96 MB 97, 98; 256 MB 271, 260.
 bool rows_past(const Seqs &s, const RowArgs &a, int arrays) {
-  return s.total * (a.heads + 2 * a.kv_heads) * a.dh * (int64_t)sizeof(float) * arrays > int64_t{128} << 20;
+  return s.total * (a.heads + 2 * a.kv_heads) * a.dh * (int64_t)sizeof(float) * arrays > int64_t{256} << 20;
 }
 
 int check_rows(numrs_hip_ctx *ctx, const numrs_hip_seqs *seqs, int64_t ld_a, int64_t ld_b, int64_t ld_c,

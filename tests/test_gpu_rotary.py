@@ -613,9 +613,9 @@ def test_a_recorded_training_step(engine):
 
 
 def test_calls_past_the_caches(hip_ctx):
-    """Calls of more than 128 MB, whose rows go past the caches, against calls of their sequences one by one: the same
+    """Calls of more than 256 MB, whose rows go past the caches, against calls of their sequences one by one: the same
     bits; the weights' gradients, sums of four rounded ones, within half a step of each."""
-    c, lib, H, Hk, dh, n = hip_ctx, L.load(), 20, 4, 128, 1750
+    c, lib, H, Hk, dh, n = hip_ctx, L.load(), 20, 4, 128, 2500
     W = (H + 2 * Hk) * dh
     rng = np.random.default_rng(80)
     x, dy = rand(rng, (4 * n, W)), rand(rng, (4 * n, W))
