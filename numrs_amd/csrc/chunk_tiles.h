@@ -1015,7 +1015,8 @@ __global__ void __launch_bounds__(256) join_parts(Args a, int wgs) {
       float m = kNever, l = -1.f;
       if (lane < cut.parts) m = part(p, lane)[r], l = part(p, lane)[ROWS + r];
       ask(0);
-      const float top = wave_max(l < 0.f ? kNever : m), f = l < 0.f ? 0.f : __builtin_amdgcn_exp2f(m - top);
+      // (a part without a token has the factor -1: only such a part is left out, since 0 times what is not finite is NaN)
+      const float top = wave_max(l < 0.f ? kNever : m), f = l < 0.f ? -1.f : __builtin_amdgcn_exp2f(m - top);
       const bool some = __any(!(l < 0.f));  // (NaN too)
       f4 o{};
       for (int k0 = 0; k0 < cut.parts; k0 += kAhead) {
@@ -1023,7 +1024,7 @@ __global__ void __launch_bounds__(256) join_parts(Args a, int wgs) {
 #pragma unroll
         for (int k = 0; k < kAhead / 2; ++k) {
           const float by = __shfl(f, k0 + 2 * k + half);
-          if (k0 + 2 * k + half >= cut.parts || by == 0.f) continue;
+          if (k0 + 2 * k + half >= cut.parts || by < 0.f) continue;
 #pragma unroll
           for (int j = 0; j < 4; ++j) o[j] = fmaf(y[k][j], by, o[j]);
         }

@@ -543,3 +543,42 @@ def test_refusals_of_sizes_and_places(hip_ctx):
                         t.ends.ptr]
     assert app(*args(x.ptr)) == L.E_INVALID and app(*args(x.ptr + 127 * 4)) == L.E_INVALID
     assert app(*args(x.ptr + 128 * 4)) == 0  # beside the projection, in the same rows
+
+
+# Where a bad token and the one that takes all of the softmax lie: in one stage, in stages of a block that nobody
+# cuts, in up to 32 parts, in more, among images, and in the decoding steps.
+FAR = [
+    ([2], [50], 4, 2),
+    ([2] * 64, [638] * 64, 8, 8),
+    ([2], [1280], 2, 1),
+    ([3, 2], [700, 1300], 8, 2),
+    ([2], [3840], 2, 1),
+    ([2100], [1000], 1, 1),
+    ([1], [50], 4, 2),
+    ([1], [1280], 2, 1),
+]
+
+
+@pytest.mark.parametrize("format", ["f32", "int8"])
+@pytest.mark.parametrize("bad_first", [True, False])
+@pytest.mark.parametrize("i", range(len(FAR)))
+def test_what_is_not_finite_far_below_the_softmax(hip_ctx, i, bad_first, format):
+    """A NaN and an infinite value on tokens whose scores lie 200 below another's: their probabilities are 0 in
+    fp32, and 0 times either is NaN, whichever way the tokens are dealt and joined."""
+    new, context, H, Hk = FAR[i]
+    dh, rng = 64, np.random.default_rng(70 + i)
+    t = _Chunk(hip_ctx, new, context, 64, H, Hk, dh, format, rng)
+    t.q[:] = 0
+    t.q[:, ::dh] = 8  # over sqrt(64): a score is a key's first column
+    t.k[:, ::dh] = 0
+    first, last = 5, context[0] - 3
+    low, high = (first, last) if bad_first else (last, first)
+    t.k[high, ::dh] = 200
+    t.v[low, 3], t.v[low + 1, 4] = np.nan, np.inf  # of the first sequence and head
+    got, n = t.write().run(), new[0]
+    t.v[low, 3] = t.v[low + 1, 4] = 0
+    ref, err = t.reference()
+    bad = np.zeros(got.shape, bool)
+    bad[:n, :H // Hk, slice(3, 5) if format == "f32" else slice(None)] = True
+    assert np.isnan(got[bad]).all(), f"{np.isfinite(got[bad]).sum()} of {bad.sum()} are finite"
+    assert (abs(got - ref) <= err)[~bad].all()
