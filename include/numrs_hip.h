@@ -477,7 +477,7 @@ int numrs_hip_kv_cache_read(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cache,
  * and written to q [total, heads * head_dim] (rows ld_q apart) for the attention
  * that follows.  Positions are ends[i] - length_i + place.  The same bits as
  * numrs_hip_qk_rotary_forward and numrs_hip_kv_cache_write in turn.  q may be
- * NULL (keys and values only) but must not overlap the rows of qkv. */
+ * NULL (keys and values only); one whose rows meet qkv's is refused. */
 int numrs_hip_kv_cache_append(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cache,
                               const numrs_hip_seqs *seqs, const float *qkv, int64_t ld,
                               const float *q_weight, const float *k_weight, float eps,
@@ -499,9 +499,9 @@ int numrs_hip_attention_paged(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cach
  * q and out are [total, heads * head_dim], rows ld_q and ld_out apart, heads
  * grouped as above.  Tokens past what the table's pages can hold, and on pages
  * that the cache does not have, are left out; a row without any token is zeros.
- * Sequences of one new token go the way of numrs_hip_attention_paged.  out must
- * not overlap q; a table's row has pages for fewer than 2^31 tokens, and a
- * sequence's new tokens times heads / kv_heads stay below that too.
+ * Sequences of one new token go the way of numrs_hip_attention_paged.  out whose
+ * rows meet q's is refused; a table's row has pages for fewer than 2^31 tokens, and
+ * a sequence's new tokens times heads / kv_heads stay below that too.
  * Products are of two fp16 terms each, relative to a query's or a token's largest
  * magnitude: 2^-22 of the terms, sums in fp32; a weight is held to 2^-39 of the
  * largest of its 64 tokens.  What is not finite, has its largest magnitude outside

@@ -97,7 +97,7 @@ extern "C" int numrs_hip_attention_paged_chunk(numrs_hip_ctx *ctx, const numrs_h
     return fail(ctx, NUMRS_HIP_E_SHAPE, "%s: a table's row has pages for 2^31 tokens or more", what);
   if (s.total == 0) return NUMRS_HIP_OK;
   if (q == nullptr || out == nullptr) return fail(ctx, NUMRS_HIP_E_INVALID, "%s: null pointer", what);
-  if (paging::rows_meet(q, heads * dh, out, heads * dh))
+  if (paging::rows_meet({q, heads * dh, ld_q}, {out, heads * dh, ld_out}, s.total))
     return fail(ctx, NUMRS_HIP_E_INVALID, "%s: the result overlaps the queries", what);
   if (int rc = s.keep()) return rc;
   DeviceScope dev(ctx);

@@ -508,7 +508,7 @@ int numrs_hip_kv_cache_append(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cach
   if (paging::bad_grid(s.tiles * (hk + 2 * parts)))
     return fail(ctx, NUMRS_HIP_E_SHAPE, "%s: too many tokens times heads", what);
   if (s.total == 0) return NUMRS_HIP_OK;
-  if (q != nullptr && paging::rows_meet(qkv, (heads + 2 * hk) * dh, q, heads * dh))
+  if (q != nullptr && paging::rows_meet({qkv, (heads + 2 * hk) * dh, ld}, {q, heads * dh, ld_q}, s.total))
     return fail(ctx, NUMRS_HIP_E_INVALID, "%s: the queries' result overlaps the projection", what);
   if (int rc = s.keep()) return rc;
   DeviceScope dev(ctx);

@@ -99,10 +99,34 @@ inline bool bad_stride(int64_t ld, int64_t width) { return ld < width || ld >= i
 // More workgroups of 256 threads than a launch, of at most 2^32 - 1 threads, can have.
 inline bool bad_grid(int64_t groups) { return groups >= int64_t{1} << 24; }
 
-// Whether the first rows of two arrays meet, na and nb floats from a and b on.
-inline bool rows_meet(const float *a, int64_t na, const float *b, int64_t nb) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-  return x < y + (uintptr_t)nb * sizeof(float) && y < x + (uintptr_t)na * sizeof(float);
+// Rows of an array that a call reads or writes: `width` floats each from `at` on, ld floats apart, ld >= width.
+struct Rows {
+  const float *at;
+  int64_t width, ld;
+};
+// Whether any of the first `rows` rows of a meets any of b.  Column blocks side by side in the same rows do not.
+inline bool rows_meet(const Rows &a, const Rows &b, int64_t rows) {
+  typedef __int128 wide;  // (bytes of 2^30 rows, 2^31 floats apart, and an address)
+  if (rows <= 0 || a.width <= 0 || b.width <= 0) return false;
+  const wide f = sizeof(float), na = a.width * f, nb = b.width * f, la = a.ld * f, lb = b.ld * f;
+  const wide from = (wide) reinterpret_cast<uintptr_t>(b.at) - (wide) reinterpret_cast<uintptr_t>(a.at);  // a to b
+  if (from >= (rows - 1) * la + na || from + (rows - 1) * lb + nb <= 0) return false;
+  if (la == lb) {
+    // b's row j lies from + (j - i) la beyond a's row i: the least such distance above -nb that two rows have
+    const wide x = -nb - from, below = x >= 0 ? x / la : -((la - 1 - x) / la);  // x / la rounded down
+    const wide d = below + 1 < -(wide)(rows - 1) ? -(wide)(rows - 1) : below + 1;
+    return d < rows && from + d * la < na;
+  }
+  wide x = 0, y = from;  // the rows of both in their order
+  for (int64_t i = 0, j = 0; i < rows && j < rows;) {
+    if (x + na <= y)
+      ++i, x += la;
+    else if (y + nb <= x)
+      ++j, y += lb;
+    else
+      return true;
+  }
+  return false;
 }
 
 // Lengths of a packed batch: their sum, or -1 if one is negative or they pass 2^30 tokens.

@@ -582,3 +582,31 @@ def test_what_is_not_finite_far_below_the_softmax(hip_ctx, i, bad_first, format)
     bad[:n, :H // Hk, slice(3, 5) if format == "f32" else slice(None)] = True
     assert np.isnan(got[bad]).all(), f"{np.isfinite(got[bad]).sum()} of {bad.sum()} are finite"
     assert (abs(got - ref) <= err)[~bad].all()
+
+
+def test_results_in_their_inputs_rows(hip_ctx):
+    """A result one or several rows into its input, at the same stride or another, is refused; column blocks side by
+    side in the same rows are not."""
+    c, lib, rng = hip_ctx, L.load(), np.random.default_rng(80)
+    t = _Chunk(c, [5, 3], [2, 0], 16, 4, 2, 16, "f32", rng).write()
+    h, cp = c.handle, ctypes.byref(t.s.cache.pages)
+    big = c.to_device(rand(rng, (40, 200)))
+    q = big.ptr + 4 * 16 * 200
+    chunk = lambda at, ld: lib.numrs_hip_attention_paged_chunk(  # noqa: E731
+        h, cp, t.seqs.handle, q, 200, 4, t.table.ptr, t.most, t.ends.ptr, q + 4 * at, ld)
+    for at in (0, 200, 7 * 200, -200, -7 * 200, 3 * 200 + 63, -3 * 200 - 63, 200 - 63):
+        assert chunk(at, 200) == L.E_INVALID, at
+    for at, ld in ((-64, 70), (0, 400), (-7 * 100, 100)):
+        assert chunk(at, ld) == L.E_INVALID, (at, ld)
+    assert b"overlaps" in lib.numrs_hip_last_error(h)
+    before = big.numpy()
+    for at in (64, 200 - 64, -64, 8 * 200 - 10):
+        assert chunk(at, 200) == 0, at
+    assert chunk(100, 400) == 0
+    assert_bits(big.numpy()[16:24, :64], before[16:24, :64])
+    app = lambda at, ld: lib.numrs_hip_kv_cache_append(  # noqa: E731
+        h, cp, t.seqs.handle, q, 200, None, None, 1e-6, None, q + 4 * at, ld, 4, t.table.ptr, t.most, t.ends.ptr)
+    for at, ld in ((200, 200), (-200, 200), (5 * 200 + 127, 200), (-6 * 200 - 63, 200), (0, 64), (-64, 300)):
+        assert app(at, ld) == L.E_INVALID, (at, ld)
+    for at in (128, -64, -72):
+        assert app(at, 200) == 0, at
