@@ -413,12 +413,14 @@ typedef struct numrs_hip_rotary {
 
 /* x and y are projections [total, (heads + 2 kv_heads) * dh] of a packed batch,
  * the column blocks q, k and v, rows ld_x and ld_y apart; v is copied.  y may be
- * x, with one stride: v is then left alone.  A token's position is its place in
- * its sequence or, with `ends` (int32 [n], device), ends[i] - length_i + place.
- * q_weight and k_weight are NULL where those heads are not normed.
+ * x, with one stride: v is then left alone; other overlaps are refused.  A
+ * token's position is its place in its sequence or, with `ends` (int32 [n],
+ * device), ends[i] - length_i + place.  q_weight and k_weight are NULL where
+ * those heads are not normed.
  * Backward: from dy the gradient of x and of the weights; x is only read for
- * heads that are normed.  dx may be dy (one stride, nothing added), dx and the
- * weights' gradients may be NULL, and one array may be both weights' gradient.
+ * heads that are normed.  dx may be dy (one stride, nothing added) or x (one
+ * stride), dx and the weights' gradients may be NULL, and one array may be both
+ * weights' gradient; other overlaps of these are refused.
  * `accumulate` has a bit for each that is added to instead of written; where the
  * weights share one array, the second's is to be set.  No atomics: the same call
  * gives the same bits. */

@@ -215,6 +215,9 @@ int numrs_hip_qk_rotary_forward(numrs_hip_ctx *ctx, const numrs_hip_seqs *seqs, 
   if (x == nullptr || y == nullptr) return fail(ctx, NUMRS_HIP_E_INVALID, "qk_rotary: null pointer");
   if (x == y && ld_x != ld_y)
     return fail(ctx, NUMRS_HIP_E_SHAPE, "qk_rotary: in place, both row strides must be the same");
+  const int64_t width = (heads + 2 * kv_heads) * dh;
+  if (x != y && paging::rows_meet({x, width, ld_x}, {y, width, ld_y}, s.total))
+    return fail(ctx, NUMRS_HIP_E_INVALID, "qk_rotary: the result overlaps the projection");
   if (int rc = s.keep()) return rc;
   DeviceScope dev(ctx);
   // in place the values are there already
@@ -258,6 +261,17 @@ int numrs_hip_qk_rotary_backward(numrs_hip_ctx *ctx, const numrs_hip_seqs *seqs,
   if (dx == dy && (acc || ld_dx != ld_dy))
     return fail(ctx, NUMRS_HIP_E_INVALID,
                 "qk_rotary_backward: in place, the row strides must be the same and nothing is added");
+  if (dx != nullptr) {
+    // (each value of x is read by the thread that writes its gradient, before it does: dx may be x too)
+    const int64_t width = (heads + 2 * kv_heads) * dh, from = q_weight != nullptr ? 0 : heads * dh,
+                  to = k_weight != nullptr ? (heads + kv_heads) * dh : q_weight != nullptr ? heads * dh : from;
+    if ((dx != dy && paging::rows_meet({dy, width, ld_dy}, {dx, width, ld_dx}, s.total)) ||
+        ((dx != x || ld_dx != ld_x) && paging::rows_meet({x + from, to - from, ld_x}, {dx, width, ld_dx}, s.total)))
+      return fail(ctx, NUMRS_HIP_E_INVALID, "qk_rotary_backward: dx overlaps what it is formed from");
+  }
+  if (dq_weight != dk_weight && dq_weight != nullptr && dk_weight != nullptr &&
+      paging::rows_meet({dq_weight, dh, dh}, {dk_weight, dh, dh}, 1))
+    return fail(ctx, NUMRS_HIP_E_INVALID, "qk_rotary_backward: the weights' gradients overlap");
   if (int rc = s.keep()) return rc;
   BackArgs b{row_args(s, ends, x, ld_x, q_weight, k_weight, eps, rotary, dx, ld_dx, heads, kv_heads, dh,
                       heads + (dx == dy || dx == nullptr ? 1 : 2) * kv_heads),

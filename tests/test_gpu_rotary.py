@@ -686,3 +686,36 @@ def test_append_past_the_caches(hip_ctx, format):
     for got, ref in zip(s.raw(), want):
         assert np.array_equal(got, ref, equal_nan=got.dtype == np.float32)
     assert_bits(q.numpy(), queries, "q")
+
+
+def test_results_in_their_inputs_rows(hip_ctx):
+    """Results over their inputs are refused but where the header allows them, those with the bits of a call of
+    separate arrays."""
+    c, lib, rng = hip_ctx, L.load(), np.random.default_rng(90)
+    t = _Case([150, 7, 64], 4, 2, 16, rng)
+    seqs, w, W = nr.PackedSequences(t.lengths, ctx=c), c.to_device(t.wq), t.W
+    T, h, r, ld = t.T, c.handle, ctypes.byref(t.rot.spec), 2 * t.W + 16
+    big = c.to_device(rand(rng, (3 * T, ld)))
+    x = big.ptr + 4 * T * ld
+    fwd = lambda to, ld_y: lib.numrs_hip_qk_rotary_forward(  # noqa: E731
+        h, seqs.handle, None, x, ld, w.ptr, w.ptr, EPS, r, to, ld_y, 4, 2, 16)
+    for at, ld_y in ((1, ld), (ld, ld), (-ld, ld), (5 * ld + W - 1, ld), (-5 * ld - W + 1, ld), (1, W), (-W, ld - 1)):
+        assert fwd(x + 4 * at, ld_y) == L.E_INVALID, (at, ld_y)
+    assert fwd(x + 4 * W, ld) == 0 and fwd(x - 4 * W, ld) == 0
+    bwd = lambda gy, ld_g, to, ld_dx, wq=w.ptr, wk=w.ptr, dq=None, dk=None: lib.numrs_hip_qk_rotary_backward(  # noqa: E731
+        h, seqs.handle, None, x, ld, wq, wk, EPS, r, gy, ld_g, to, ld_dx, dq, dk, 4, 2, 16, 0)
+    g, dx = c.to_device(rand(rng, (3 * T, ld), 0.1)), c.empty((T, W))
+    gy = g.ptr + 4 * T * ld
+    for at in (1, ld, -ld, 5 * ld + 95, -5 * ld - W + 1):
+        assert bwd(gy, ld, gy + 4 * at, ld) == L.E_INVALID, at  # over dy
+        assert bwd(gy, ld, x + 4 * at, ld) == L.E_INVALID, at   # over x
+    assert bwd(gy, ld, x, ld - 1) == L.E_INVALID and bwd(gy, ld, gy + 4, ld - 1) == L.E_INVALID
+    # only what is read of x counts: the normed heads, its columns 0 to 63 or 64 to 95
+    assert bwd(gy, ld, x + 4 * 64, ld, wk=None) == 0 and bwd(gy, ld, x + 4 * 63, ld, wk=None) == L.E_INVALID
+    assert bwd(gy, ld, x + 4 * 96, ld, wq=None) == 0 and bwd(gy, ld, x + 4 * 95, ld, wq=None) == L.E_INVALID
+    assert bwd(gy, ld, x + 4 * 5 * ld, ld, wq=None, wk=None) == 0
+    two = c.empty((24,))
+    assert bwd(gy, ld, dx.ptr, W, dq=two.ptr, dk=two.ptr + 4 * 8) == L.E_INVALID
+    assert bwd(gy, ld, dx.ptr, W) == 0
+    assert bwd(gy, ld, x, ld) == 0  # the gradient in x's place
+    assert_bits(big.numpy()[T:2 * T, :W], dx.numpy())
