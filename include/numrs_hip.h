@@ -507,9 +507,10 @@ int numrs_hip_attention_paged(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cach
  * Products are of two fp16 terms each, relative to a query's or a token's largest
  * magnitude: 2^-22 of the terms, sums in fp32; a weight is held to 2^-39 of the
  * largest of its 64 tokens.  What is not finite, has its largest magnitude outside
- * 2^-60 .. 2^60, lies 2^64 from its neighbours or on a page that is missing is
- * taken in plain fp32 together with the tokens beside it, some hundred times
- * slower.  Of an fp32 cache that a sequence reads with 2048 rows or more (tokens
+ * 2^-60 .. 2^60 (in 8 bits, its scale), is more than 2^64 times the largest of
+ * the first 64 tokens that a workgroup takes, or less than 2^-64 of it, or lies on
+ * a page that is missing is taken in plain fp32 together with the tokens beside
+ * it, some hundred times slower.  Of an fp32 cache that a sequence reads with 2048 rows or more (tokens
  * times heads / kv_heads) a workspace of up to 1 GB has the tokens laid out.
  * No backward, no atomics on values: the same call gives the same bits. */
 int numrs_hip_attention_paged_chunk(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cache,

@@ -91,6 +91,9 @@ __device__ __forceinline__ float maximum(float a, float b) { return __builtin_el
 // split's smallest step to 2^-29 of it at most); others at their own, and have a factor.  Past kApart it is odd.
 constexpr unsigned kLow = 127 - 60, kHigh = 127 + 60, kBelow = 8, kApart = 64, kScaled = 13;
 __device__ __forceinline__ float power(unsigned bits) { return __builtin_bit_cast(float, bits << 23); }
+// The base of what a first stage was raised to.  One of zeros only says nothing of those after it: from [1, 2) no
+// size that is ordinary is past kApart.
+__device__ __forceinline__ unsigned base_of(unsigned raised) { return raised == 0 ? 127 : raised; }
 // What a stage's rows may be besides.
 enum : int { kOdd = 1, kMixedKeys = 2, kMixedValues = 4 };
 
@@ -286,14 +289,17 @@ struct Staging {
     for (int j = 0; j < 8; j += 2) big = maximum(maximum(big, fabsf(v[j >> 2][j & 3])), fabsf(v[j >> 2][(j & 3) + 1]));
     return row_top<S::kLanes>(__builtin_bit_cast(unsigned, big));
   }
-  // Raises the walk's base to the largest exponent of these rows.
+  // Raises the walk's base to the largest exponent of these rows; rows of zeros leave it at 0 (see base_of).
   template <bool VALUES>
   __device__ __forceinline__ void raise_base(unsigned (&base)[2], const Cache &c, const Walk &w, int stage) {
     if constexpr (!INT8) {
       drop<VALUES>(c, w, stage);
-      unsigned e = kLow;
+      unsigned e = 0;
 #pragma unroll
-      for (int i = 0; i < S::NP; ++i) e = max(e, min(top_of_row<VALUES>(i) >> 23, kHigh));
+      for (int i = 0; i < S::NP; ++i) {
+        const unsigned top = top_of_row<VALUES>(i);
+        if (top != 0) e = max(e, min(max(top >> 23, kLow), kHigh));
+      }
       atomicMax(&base[VALUES], e);
     }
   }
@@ -672,7 +678,7 @@ __global__ void __launch_bounds__(kThreads) pack_stages(Args a) {
   if (stage > 0 && stage * kStage >= walk.held) return;
   Staging<false, DP, true> g;
   g.look(a.c, walk, stage);
-  if (tid < 2) base[tid] = kLow;
+  if (tid < 2) base[tid] = 0;
   if (tid == 2) marks = 0;
   g.resolve(a.c);
   g.load_keys(a.c, walk, stage);
@@ -683,7 +689,7 @@ __global__ void __launch_bounds__(kThreads) pack_stages(Args a) {
   __syncthreads();
   char *image = a.images + (int64_t)blockIdx.x * kImage<DP>;
   Head *head = reinterpret_cast<Head *>(image + S::kBytes);
-  const unsigned kbase = base[0], vbase = base[1];
+  const unsigned kbase = base_of(base[0]), vbase = base_of(base[1]);
   int found = g.template split_rows<false>(a.c, walk, stage, image, head->ks, kbase);
   found |= g.template split_rows<true>(a.c, walk, stage, image + S::kKeys, head->vs, vbase);
   g.mark(&marks, found | g.lacking(walk, stage));
@@ -804,7 +810,7 @@ __global__ void __launch_bounds__(kThreads, 2) walk_blocks(Args a) {
       } else {
         g.look(a.c, walk, s0);
         if (tid < 3) lds.marks[tid] = 0;
-        if (tid < 2) lds.base[tid] = kLow;
+        if (tid < 2) lds.base[tid] = 0;
         const bool good = r.start(a, lds, query(), live);
         g.resolve(a.c);
         __syncthreads();  // what is marked is cleared, the last block's buffers free
@@ -814,14 +820,14 @@ __global__ void __launch_bounds__(kThreads, 2) walk_blocks(Args a) {
         g.template raise_base<false>(lds.base, a.c, walk, s0);
         if constexpr (kBoth) g.template raise_base<true>(lds.base, a.c, walk, s0);
         if constexpr (!INT8) __syncthreads();
-        kbase = __builtin_amdgcn_readfirstlane(lds.base[0]);
+        kbase = base_of(__builtin_amdgcn_readfirstlane(lds.base[0]));
         g.put_keys(lds, a.c, walk, s0, 0, 0, kbase);
         if constexpr (!kBoth) {
           g.load_values(a.c, walk, s0);
           g.template raise_base<true>(lds.base, a.c, walk, s0);
           __syncthreads();
         }
-        vbase = __builtin_amdgcn_readfirstlane(lds.base[1]);
+        vbase = base_of(__builtin_amdgcn_readfirstlane(lds.base[1]));
         g.put_values(lds, a.c, walk, s0, 0, 0, vbase);
         g.look(a.c, walk, s0 + 1);
       }

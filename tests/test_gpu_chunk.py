@@ -610,3 +610,27 @@ def test_results_in_their_inputs_rows(hip_ctx):
         assert app(at, ld) == L.E_INVALID, (at, ld)
     for at in (128, -64, -72):
         assert app(at, 200) == 0, at
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("dh", [32, 64, 128])
+@pytest.mark.parametrize("new,H,Hk", [([2] * 64, 8, 8), ([66] * 64, 32, 8), ([520], 4, 1)])
+def test_a_beginning_of_zeros(hip_ctx, new, H, Hk, dh, which):
+    """128 tokens of zeros, then keys (or values) from 8 to 16 and 2^7 times those over queries of 2^-7: each is a
+    product of two terms at a power of two of its own, so that all sums are the same ones and results have the same
+    bits (of the values, 2^7 times).  In plain fp32, token by token, the larger ones' would differ."""
+    rng = np.random.default_rng(81)
+    t = _Chunk(hip_ctx, new, [640 - new[0]] * len(new), 64, H, Hk, dh, "f32", rng)
+    x = getattr(t, which)
+    x *= 8
+    x[:, ::dh] = rng.uniform(8, 15, (len(x), Hk))  # a token's largest
+    x.reshape(len(new), 640, -1)[:, :128] = 0
+    t.q /= 8
+    first = t.write().run()
+    t.check(first, only=[0, len(new) - 1])
+    x *= np.float32(128)
+    if which == "k":
+        t.q /= 128
+        assert_bits(t.write().run(), first)
+    else:
+        assert_bits(t.write().run(), first * np.float32(128))
