@@ -50,12 +50,17 @@ class Rotary:
             if not base > 0:
                 raise ValueError("the base must be positive")
             freqs = float(base) ** (-2.0 * np.arange(dims // 2) / dims)
-        self.freqs = np.array(freqs, np.float64).ravel()
-        if self.freqs.size != dims // 2:
-            raise ValueError(f"{dims // 2} frequencies are needed, not {self.freqs.size}")
+        freqs = np.array(freqs, np.float64).ravel()
+        if freqs.size != dims // 2:
+            raise ValueError(f"{dims // 2} frequencies are needed, not {freqs.size}")
         self.head_dim, self.dims, self.layout = int(head_dim), dims, layout
-        at = self.freqs.ctypes.data_as(ctypes.POINTER(ctypes.c_double))
+        at = freqs.ctypes.data_as(ctypes.POINTER(ctypes.c_double))
         self.spec = L.RotarySpec(at, dims, LAYOUTS[layout])
+        self.spec.kept = freqs  # (the structure has their address only)
+
+    @property
+    def freqs(self) -> np.ndarray:
+        return self.spec.kept
 
 
 class PackedSequences:

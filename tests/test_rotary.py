@@ -93,3 +93,18 @@ def test_python_rotary():
                      ((64,), {"freqs": [1.0]}), ((4,), {})):
         with pytest.raises(ValueError):
             nr.Rotary(*args, **kw)
+
+
+def test_a_description_keeps_its_frequencies():
+    """`spec` holds an address: what it leads to lives as long as it does, and is what `freqs` shows."""
+    r = nr.Rotary(64, freqs=np.arange(32.0))
+    spec = r.spec
+    del r
+    others = [np.full(32, 7.0) for _ in range(4)]  # takes the place of what was given back
+    assert spec.freqs[:32] == list(range(32))
+    r = nr.Rotary(64)
+    with pytest.raises(AttributeError):
+        r.freqs = np.zeros(32)
+    r.freqs[3] = 0.25
+    assert r.spec.freqs[:32] == r.freqs.tolist()
+    del others
