@@ -12,13 +12,14 @@ using namespace numrs_hip;
 
 constexpr float kLog2e = 1.44269504088896341f;
 
-// From kManyRows query rows of a kv head on a sequence, over caches in fp32, stages are made images first, which costs
-// a pass over the cached tokens and saves every block of 256 rows its own splitting.  On MI355X, without against with,
+// From kManyRows query rows of a kv head on a sequence (the batch's mean), over caches in fp32, stages are made images
+// first, which costs a pass over the cached tokens and saves every block of 256 rows its own splitting.  On MI355X, without against with,
 // us, 32 heads of 128 in groups of 4 over 8192 tokens: 256 rows 70, 84; 512 rows 95, 105; 1024 rows 145, 149; 2048
 // rows 260, 242; of four sequences in groups of 8: 1024 rows over 8192 147, 146; 2048 over 2048 101, 97; 4096 over none
 // 65, 63; 16384 over 0 to 16384 1546, 1352; heads of 64 over 2048: 1024 rows 67, 71; 2048 rows 110, 110.  The images
-// have room for all that the pages can hold, since only the device knows what they do; past kMostImages they are not
-// made.
+// have room for all that the table's width can hold, since only the device knows what it does; past kMostImages they
+// are not made, and a table that is wider than its sequences need can lose them so (two sequences of 2048 rows and 8 kv
+// heads of 128: from 65536 tokens on).
 constexpr int64_t kManyRows = 2048, kMostImages = int64_t{1} << 30;
 // Up to so many rows blocks have 128 in two sets of waves, beyond 256 in one, which reads the tokens half as often.
 // 256 against 128, us: 128 rows over 131072 tokens 70, 71; 32 heads of 128 over 8192, fp32 and 8 bits: 32 rows 44, 44
@@ -109,7 +110,8 @@ extern "C" int numrs_hip_attention_paged_chunk(numrs_hip_ctx *ctx, const numrs_h
   if (s.severals == 0) return NUMRS_HIP_OK;
   chunk::Args a{{cache->k, cache->v, cache->k_scale, cache->v_scale, cache->pages, max_pages, table,
                  paging::log2_of(cache->page_size), (int)hk, (int)dh},
-                s.several, ends, q, out, nullptr, nullptr, 0, nullptr, ld_q, ld_out, (int)s.severals, (int)heads, (int)(heads / hk), 0.f, 0};
+                s.several, ends, q, out, nullptr, nullptr, 0, nullptr, ld_q, ld_out, (int)s.severals,
+                (int)(heads / hk), 0.f, 0};
   a.mant = std::frexp(kLog2e / std::sqrt((float)dh), &a.exp);
   const bool few = s.longest * a.group <= kFewRows;
   if (cache->format == NUMRS_HIP_KV_INT8) return few ? run_dp<true, 2>(ctx, s, a) : run_dp<true, 1>(ctx, s, a);

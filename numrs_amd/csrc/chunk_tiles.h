@@ -71,7 +71,7 @@ struct Args {
   int most_stages;
   Cut *cuts;  // [workgroups]
   int64_t ld_q, ld_out;
-  int n, heads, group;
+  int n, group;
   float mant;  // log2(e) / sqrt(dh) is mant 2^exp, mant in [0.5, 1)
   int exp;
 };
@@ -87,8 +87,9 @@ __device__ __forceinline__ bool wild(float x) { return !(x == 0.f || (fabsf(x) >
 __device__ __forceinline__ float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 // A magnitude's exponent as its bits have it, 127 for [1, 2).  Tokens whose largest magnitude has one of base - kBelow
-// to base + 1 are split at the base, the first stage's largest or an image's own, which brings that to [2^13, 2^14) (so theirs to [2^5, 2^15), and the
-// split's smallest step to 2^-29 of it at most); others at their own, and have a factor.  Past kApart it is odd.
+// to base + 1 are split at the base, the largest of the walk's first stage or an image's own, which brings that to
+// [2^13, 2^14) (so theirs to [2^5, 2^15), and the split's smallest step to 2^-29 of it at most); others at their own,
+// and have a factor.  Past kApart it is odd.
 constexpr unsigned kLow = 127 - 60, kHigh = 127 + 60, kBelow = 8, kApart = 64, kScaled = 13;
 __device__ __forceinline__ float power(unsigned bits) { return __builtin_bit_cast(float, bits << 23); }
 // The base of what a first stage was raised to.  One of zeros only says nothing of those after it: from [1, 2) no
@@ -100,8 +101,6 @@ enum : int { kOdd = 1, kMixedKeys = 2, kMixedValues = 4 };
 // Floats of a part: references and sums of a block's rows, then their outputs.
 template <int DP, int ROWS>
 constexpr int kPart = ROWS * (2 + DP);
-
-__device__ __forceinline__ int log_lanes(int dp) { return dp > 64 ? 4 : dp > 32 ? 3 : 2; }
 
 // A head size rounded up to DP in LDS: a row of keys (or fp32 values) of a term is kRow bytes, its pieces of 16
 // bytes out of place by the token, so that neither the reads of a product (one piece of 32 tokens; or of the

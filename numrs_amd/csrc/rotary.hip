@@ -3,9 +3,9 @@
 //
 // Both directions are bound by memory: each value is read once and written once, and the angles, the same for
 // all heads of a token, are formed once for a token and a workgroup's heads.  On MI355X: 62 MB of ragged prompts in
-// 12.4 us (5.0 TB/s); 16384 tokens of 16 + 8 + 8 heads of 128 with norms forward 103 to 108 us (5.2 TB/s, past the
-// caches), backward 140 (3.8 TB/s), the weights' sums 9; 4096 tokens of 24 heads of 64 forward 10, backward 14, sums 7;
-// 64 tokens 3.5, latency.
+// 12.4 us (5.0 TB/s); 16384 tokens of 16 + 8 + 8 heads of 128 with norms forward 105 to 108 us (5.0 to 5.1 TB/s, past
+// the caches), backward 137 to 143 (which reads the normed heads again: 738 MB, 5.2 to 5.4 TB/s), the weights' sums 9
+// to 10; 4096 tokens of 24 heads of 64 forward 10, backward 14, sums 8; 64 tokens 3.5, latency.
 #include <algorithm>
 
 #include "rotary.h"
