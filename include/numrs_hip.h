@@ -499,7 +499,7 @@ int numrs_hip_attention_paged(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cach
 
 /* Attention of a packed batch's new tokens over the cache, where they are already
  * (numrs_hip_kv_cache_append): token r of sequence i, at position p = ends[i] -
- * length_i + r, attends to the cached tokens 0 .. p of its sequence.  q and out
+ * length_i + r, attends to the cached tokens 0 .. p of its sequence. q and out
  * are [total, heads * head_dim], rows ld_q and ld_out apart, heads grouped as
  * above.  Tokens past what the table's pages can hold, and on pages that the
  * cache does not have, are left out; a row without any token is zeros.  out whose
@@ -507,17 +507,18 @@ int numrs_hip_attention_paged(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cach
  * and a sequence's new tokens times heads / kv_heads stay below that too.
  * Sequences of one new token go the way of numrs_hip_attention_paged, with its
  * limit of values; what follows is of the others.  Products are of two fp16 terms
- * each, relative to a query's or a token's largest magnitude: 2^-22 of the terms,
- * sums in fp32; a weight is held to 2^-39 of the largest of its 64 tokens.  What
- * is not finite, has its largest magnitude outside 2^-60 .. 2^60 (in 8 bits, its
- * scale), is more than 2^64 times the largest of the first 64 tokens that a
- * workgroup takes, or less than 2^-64 of it, or lies on a page that is missing is
- * taken in plain fp32 together with the tokens beside it, some hundred times
- * slower.  Where the sequences of several new tokens have 2048 rows (tokens times
- * heads / kv_heads) and more of a kv head on the mean, their tokens in an fp32
- * cache are laid out in a workspace first: it has room for all that the table's
- * width can hold of them, and where that is above 1 GB, they are not.  No
- * backward, no atomics on values: the same call gives the same bits. */
+ * each, sums in fp32: a query, key or value is held to 2^-22 of itself or 2^-30
+ * of the largest magnitude of its head and token, whichever is more, a weight to
+ * 2^-39 of the largest of its 64 tokens.  What is not finite, has its largest
+ * magnitude outside 2^-60 .. 2^60 (in 8 bits, its scale), is more than 2^64 times
+ * the largest of the first 64 tokens that a workgroup takes, or less than 2^-64
+ * of it, or lies on a page that is missing is taken in plain fp32 together with
+ * the tokens beside it, some hundred times slower.  Where the sequences of
+ * several new tokens have 2048 rows (tokens times heads / kv_heads) and more of a
+ * kv head on the mean, their tokens in an fp32 cache are laid out in a workspace
+ * first: it has room for all that the table's width can hold of them, and where
+ * that is above 1 GB, they are not.  No backward, no atomics on values: the same
+ * call gives the same bits. */
 int numrs_hip_attention_paged_chunk(numrs_hip_ctx *ctx, const numrs_hip_kv_cache *cache,
                                     const numrs_hip_seqs *seqs, const float *q, int64_t ld_q,
                                     int64_t heads, const int32_t *table, int64_t max_pages,

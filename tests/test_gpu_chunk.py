@@ -634,3 +634,25 @@ def test_a_beginning_of_zeros(hip_ctx, new, H, Hk, dh, which):
         assert_bits(t.write().run(), first)
     else:
         assert_bits(t.write().run(), first * np.float32(128))
+
+
+@pytest.mark.parametrize("n", [2, 300, 600])
+@pytest.mark.parametrize("gap", [0, 8, 9])
+def test_values_far_below_their_tokens_largest(hip_ctx, gap, n):
+    """A row whose softmax is its own token's gives that token's value, the token 2^-gap of those before it: to 2^-22 of
+    itself or 2^-30 of the token's largest, to 2^-39 of that for the weight, and to the 2^-23 of each of four roundings
+    (the weight, the product's sum, the sum over stages, 1 / l and what it multiplies)."""
+    H, Hk, dh, rng = 8, 2, 64, np.random.default_rng(82)
+    t = _Chunk(hip_ctx, [n], [200], 16, H, Hk, dh, "f32", rng)
+    m = n + 200
+    t.k[:], t.q[:] = 0, 0
+    t.k[:, ::dh] = 256 * np.arange(m)[:, None] / 8  # each 200 and more above the one before
+    t.q[:, ::dh] = 64
+    t.v *= np.ldexp(np.float32(1), -rng.integers(0, 30, t.v.shape)).astype(np.float32)
+    t.v[:, 1::dh] = 1.5
+    t.v[200:] *= np.float32(2.0 ** -gap)
+    got = t.write().run()
+    v = np.repeat(t.v[200:].reshape(n, Hk, dh), H // Hk, axis=1).astype(np.float64)
+    top = abs(v).max(-1, keepdims=True)
+    err = np.maximum(2.0 ** -22 * abs(v), 2.0 ** -30 * top) + 2.0 ** -39 * top + 5 * U2 * abs(v)
+    assert (abs(got - v) <= err).all(), (abs(got - v) / err).max()
